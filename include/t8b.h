@@ -551,6 +551,77 @@ int t8b_collect_rollout(t8b_sim* sim, t8b_policy* policy, t8b_rollout* rollout, 
                         uint64_t update, size_t horizon, float reward_scale, void* stream);
 int t8b_rollout_synchronize(t8b_rollout* rollout, void* stream);
 
+/* ------------------------------------------------------------------ torso operators
+ * Operators of a residual policy torso (no reference counterpart: the reference's network is two
+ * tanh layers). A matrix is row-major: `rows` rows of consecutive elements, `stride` elements
+ * from one row's start to the next's, which may be anything from the row's length up; vectors
+ * (weights of a norm, biases, mean, rstd) are packed. All pointers are device pointers. Nothing
+ * is allocated: what a call needs beside its outputs is a workspace (256-byte aligned) of the
+ * size that the query beside it gives for the same sizes, free again once the call's work on
+ * `stream` is done. Work is queued on `stream` of the current device and ordered on it alone;
+ * the calls can be captured into a graph after a first call of the same form. Zero rows are
+ * allowed (outputs with rows stay empty, parameters' gradients become zero). Outputs must not
+ * overlap inputs unless it is said. Every sum and statistic is held in fp32; results repeat
+ * bit for bit for the same arguments. */
+enum { T8B_F32 = 0, T8B_BF16 = 1, T8B_F16 = 2 };
+enum { T8B_LINEAR = 0, T8B_RELU = 1, T8B_GELU = 2, T8B_SILU = 3, T8B_TANH = 4 }; /* GELU: z Phi(z) */
+
+/* Layer norm: y = (x - mean) rstd weight + bias over each row's n elements, rstd = 1 /
+ * sqrt(variance + epsilon). x and y are of any type each; weight and bias (of parameter_type) may
+ * be NULL (1 and 0); mean and rstd [rows] are written unless NULL. y may be x itself where n is at
+ * most 8192. */
+int t8b_layer_norm_forward(const void* x, int x_type, int64_t x_stride, const void* weight, const void* bias,
+                           int parameter_type, float epsilon, int64_t rows, int64_t n, void* y, int y_type,
+                           int64_t y_stride, float* mean, float* rstd, void* stream);
+/* Its gradients from dy (of y's type) and the forward pass's mean and rstd: dx (of x's type), to
+ * which residual_gradient (of x's type) is added unless NULL, and dweight and dbias (of
+ * parameter_type), each skipped where NULL; without both no workspace is needed. */
+size_t t8b_layer_norm_workspace(int64_t rows, int64_t n);
+int t8b_layer_norm_backward(const void* dy, int y_type, int64_t dy_stride, const void* x, int x_type, int64_t x_stride,
+                            const void* weight, int parameter_type, const float* mean, const float* rstd,
+                            const void* residual_gradient, int64_t residual_stride, int64_t rows, int64_t n, void* dx,
+                            int64_t dx_stride, void* dweight, void* dbias, void* workspace, size_t workspace_bytes,
+                            void* stream);
+
+/* Linear map with its epilogue: y = activation(x weight^T + bias) + residual, x [rows][in] and
+ * weight [out][in] of `type` (T8B_BF16 or T8B_F16; products are summed in fp32), bias [out] of
+ * bias_type (T8B_F32 or `type`; NULL: none), residual [rows][out] of y_type (NULL: none), y of
+ * y_type (T8B_F32 or `type`). `pre` [rows][out] of `type`, unless NULL, receives x weight^T + bias
+ * for the gradient. y may be the residual's own storage. The workspace is used, and may be NULL
+ * otherwise, where the rows of x or of weight do not start on 16-byte boundaries. */
+size_t t8b_linear_workspace(int64_t rows, int64_t in, int64_t out, int backward);
+int t8b_linear_forward(int type, const void* x, int64_t x_stride, const void* weight, int64_t weight_stride,
+                       const void* bias, int bias_type, int activation, const void* residual, int64_t residual_stride,
+                       int64_t rows, int64_t in, int64_t out, void* y, int y_type, int64_t y_stride, void* pre,
+                       int64_t pre_stride, void* workspace, size_t workspace_bytes, void* stream);
+/* Its gradients from dy [rows][out] of `type`: with dz = dy activation'(pre), dx = dz weight,
+ * dweight [out][in] = dz^T x (both of `type`) and dbias = the columns' sums of dz (of bias_type),
+ * each skipped where NULL. `pre` is not read where the activation is T8B_LINEAR. dz is rounded to
+ * `type` for the matrix products (not for dbias). The residual's gradient is dy itself. */
+int t8b_linear_backward(int type, const void* dy, int64_t dy_stride, const void* x, int64_t x_stride,
+                        const void* weight, int64_t weight_stride, const void* pre, int64_t pre_stride, int bias_type,
+                        int activation, int64_t rows, int64_t in, int64_t out, void* dx, int64_t dx_stride,
+                        void* dweight, int64_t dweight_stride, void* dbias, void* workspace, size_t workspace_bytes,
+                        void* stream);
+
+/* Gated projection: h = activation(gate) up, where [gate | up] = x weight^T + bias: weight
+ * [2 out][in] and bias [2 out] hold the gate's rows first, then the up projection's. `pre`
+ * [rows][2 out], unless NULL, receives [gate | up]. Types as for the linear map; h is of `type`. */
+size_t t8b_gated_workspace(int64_t rows, int64_t in, int64_t out, int backward);
+int t8b_gated_forward(int type, const void* x, int64_t x_stride, const void* weight, int64_t weight_stride,
+                      const void* bias, int bias_type, int activation, int64_t rows, int64_t in, int64_t out, void* h,
+                      int64_t h_stride, void* pre, int64_t pre_stride, void* workspace, size_t workspace_bytes,
+                      void* stream);
+/* Its gradients from dh [rows][out]: with dz = [dh up activation'(gate) | dh activation(gate)],
+ * dx = dz weight, dweight [2 out][in] = dz^T x, dbias [2 out] = the columns' sums of dz. */
+int t8b_gated_backward(int type, const void* dh, int64_t dh_stride, const void* x, int64_t x_stride, const void* weight,
+                       int64_t weight_stride, const void* pre, int64_t pre_stride, int bias_type, int activation,
+                       int64_t rows, int64_t in, int64_t out, void* dx, int64_t dx_stride, void* dweight,
+                       int64_t dweight_stride, void* dbias, void* workspace, size_t workspace_bytes, void* stream);
+/* Synchronises `stream` and reports whether a wait inside an operator's kernel ran out of its
+ * limit on this device since the last call (T8B_ECUDA; the outputs of that call are not valid). */
+int t8b_operators_status(void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -9,6 +9,7 @@ from __future__ import annotations
 import os
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
@@ -33,7 +34,7 @@ def build(verbose: bool = False) -> Path:
     BUILD.mkdir(exist_ok=True)
     LIB.parent.mkdir(exist_ok=True)
     newest_header = _newest_header()
-    objects = []
+    objects, commands = [], []
     for source in sorted(CSRC.glob("*.cu")):
         obj = BUILD / (source.stem + ".o")
         objects.append(obj)
@@ -42,7 +43,10 @@ def build(verbose: bool = False) -> Path:
         cmd = [NVCC, *ARCH, *COMMON, *EXTRA.get(source.name, []), "-c", str(source), "-o", str(obj)]
         if verbose:
             print(" ".join(cmd), flush=True)
-        subprocess.run(cmd, check=True)
+        commands.append(cmd)
+    with ThreadPoolExecutor(max_workers=os.cpu_count() or 1) as pool:
+        for done in [pool.submit(subprocess.run, cmd, check=True) for cmd in commands]:
+            done.result()
     if not LIB.exists() or LIB.stat().st_mtime < max(o.stat().st_mtime for o in objects):
         cmd = [NVCC, *ARCH, "-shared", "-o", str(LIB), *map(str, objects), "-lcudart", "-lcuda", "-ldl"]
         if verbose:

@@ -1,0 +1,165 @@
+// What the operator kernels (layer norm, linear, gated) share: element types and their
+// conversions, activations and their slopes, and the host-side argument checks.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cstdint>
+#include <limits>
+#include <string>
+
+#include "common.cuh"
+
+namespace t8b {
+namespace op {
+
+using bf16 = __nv_bfloat16;
+using f16 = __half;
+
+// ------------------------------------------------------------------ element types
+template <typename T>
+struct Element;
+template <>
+struct Element<float> {
+    static constexpr int kType = T8B_F32;
+    __device__ static float load(float v) { return v; }
+    __device__ static float store(float v) { return v; }
+};
+template <>
+struct Element<bf16> {
+    static constexpr int kType = T8B_BF16;
+    __device__ static float load(bf16 v) { return __bfloat162float(v); }
+    __device__ static bf16 store(float v) { return __float2bfloat16_rn(v); }
+    __device__ static float2 unpack(uint32_t w) { return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&w)); }
+    __device__ static uint32_t pack(float a, float b) {
+        __nv_bfloat162 p = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<uint32_t*>(&p);
+    }
+};
+template <>
+struct Element<f16> {
+    static constexpr int kType = T8B_F16;
+    __device__ static float load(f16 v) { return __half2float(v); }
+    __device__ static f16 store(float v) { return __float2half_rn(v); }
+    __device__ static float2 unpack(uint32_t w) { return __half22float2(*reinterpret_cast<__half2*>(&w)); }
+    __device__ static uint32_t pack(float a, float b) {
+        __half2 p = __floats2half2_rn(a, b);
+        return *reinterpret_cast<uint32_t*>(&p);
+    }
+};
+
+// One element of an array whose type is known at run time (parameters: read once per block).
+__device__ __forceinline__ float load_any(const void* p, int type, size_t i) {
+    if (type == T8B_F32) return static_cast<const float*>(p)[i];
+    if (type == T8B_BF16) return __bfloat162float(static_cast<const bf16*>(p)[i]);
+    return __half2float(static_cast<const f16*>(p)[i]);
+}
+__device__ __forceinline__ void store_any(void* p, int type, size_t i, float v) {
+    if (type == T8B_F32) {
+        static_cast<float*>(p)[i] = v;
+    } else if (type == T8B_BF16) {
+        static_cast<bf16*>(p)[i] = __float2bfloat16_rn(v);
+    } else {
+        static_cast<f16*>(p)[i] = __float2half_rn(v);
+    }
+}
+
+// V consecutive elements as they lie in memory, moved by the widest access that V allows
+// (p aligned to the pack's size, or V = 1).
+template <typename T, int V>
+struct alignas(sizeof(T) * V) Pack {
+    T v[V];
+};
+
+// ------------------------------------------------------------------ activations
+// In fp32. Where z is infinite or NaN they give what the formula does: silu(-inf) and gelu(-inf)
+// are NaN (0 * inf), as z / (1 + exp(-z)) is.
+__device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.0f, 1.0f + __expf(-z)); }
+__device__ __forceinline__ float normal_cdf(float z) { return 0.5f * (1.0f + erff(z * 0.70710678118654752f)); }
+template <int ACT>
+__device__ __forceinline__ float activate(float z) {
+    if (ACT == T8B_RELU) return z > 0.0f ? z : (z != z ? z : 0.0f);
+    if (ACT == T8B_GELU) return z * normal_cdf(z);
+    if (ACT == T8B_SILU) return z * sigmoid(z);
+    if (ACT == T8B_TANH) return tanhf(z);
+    return z;
+}
+// activate(z) and its derivative
+template <int ACT>
+__device__ __forceinline__ void activate_slope(float z, float& value, float& slope) {
+    if (ACT == T8B_RELU) {
+        value = activate<T8B_RELU>(z);
+        slope = z > 0.0f ? 1.0f : 0.0f;
+    } else if (ACT == T8B_GELU) {
+        const float cdf = normal_cdf(z);
+        value = z * cdf;
+        slope = cdf + z * 0.39894228040143268f * __expf(-0.5f * z * z);
+    } else if (ACT == T8B_SILU) {
+        const float s = sigmoid(z);
+        value = z * s;
+        slope = s * (1.0f + z * (1.0f - s));
+    } else if (ACT == T8B_TANH) {
+        value = tanhf(z);
+        slope = 1.0f - value * value;
+    } else {
+        value = z;
+        slope = 1.0f;
+    }
+}
+
+// Calls body with the activation as a compile-time constant.
+template <int N>
+struct Constant {
+    static constexpr int value = N;
+};
+template <typename Body>
+__host__ __device__ __forceinline__ void with_activation(int act, Body&& body) {
+    switch (act) {
+        case T8B_RELU: body(Constant<T8B_RELU>{}); break;
+        case T8B_GELU: body(Constant<T8B_GELU>{}); break;
+        case T8B_SILU: body(Constant<T8B_SILU>{}); break;
+        case T8B_TANH: body(Constant<T8B_TANH>{}); break;
+        default: body(Constant<T8B_LINEAR>{}); break;
+    }
+}
+
+// ------------------------------------------------------------------ host checks
+inline size_t type_size(int type) { return type == T8B_F32 ? 4 : 2; }
+inline bool is_type(int type) { return type == T8B_F32 || type == T8B_BF16 || type == T8B_F16; }
+inline bool aligned(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) % bytes) == 0; }
+inline size_t round_up(size_t v, size_t to) { return (v + to - 1) / to * to; }
+
+// A row-major matrix argument: its rows must not overlap, its last element must be addressable.
+inline void check_matrix(const char* what, const void* data, int64_t rows, int64_t columns, int64_t stride) {
+    if (rows == 0) return;
+    if (data == nullptr) raise(T8B_EINVAL, std::string(what) + " is null");
+    if (rows > 1 && stride < columns) raise(T8B_EINVAL, std::string(what) + ": a row stride below the row's length");
+    if (stride < 0 || (rows > 1 && stride > std::numeric_limits<int64_t>::max() / 8 / rows)) {
+        raise(T8B_EINVAL, std::string(what) + ": the row stride is out of range");
+    }
+}
+
+// [first, last) of the bytes a matrix spans.
+struct Span {
+    uintptr_t first, last;
+    Span(const void* data, int64_t rows, int64_t columns, int64_t stride, size_t size)
+        : first(reinterpret_cast<uintptr_t>(data)), last(first) {
+        if (data != nullptr && rows > 0 && columns > 0) last = first + ((rows - 1) * stride + columns) * size;
+    }
+    bool overlaps(const Span& o) const { return first < o.last && o.first < last; }
+};
+
+// A kernel's dynamic shared memory and cluster shape, configured once per device.
+template <typename Kernel>
+inline void allow_smem(Kernel kernel, size_t bytes, uint64_t& configured) {
+    int device = 0;
+    check(cudaGetDevice(&device), "cudaGetDevice");
+    const uint64_t bit = 1ull << (device & 63);
+    if ((__atomic_load_n(&configured, __ATOMIC_ACQUIRE) & bit) != 0) return;
+    check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)), "shared memory");
+    __atomic_fetch_or(&configured, bit, __ATOMIC_RELEASE);
+}
+
+}  // namespace op
+}  // namespace t8b

@@ -1,0 +1,203 @@
+// C entries of the linear map and the gated projection: argument checks, and the flag of waits
+// that ran out.
+#include "ops_linear.cuh"
+
+namespace t8b {
+namespace op {
+
+extern template void linear_forward<bf16>(const LinearCall&);
+extern template void linear_forward<f16>(const LinearCall&);
+extern template void linear_backward<bf16>(const LinearGradCall&);
+extern template void linear_backward<f16>(const LinearGradCall&);
+
+__device__ int g_stalled;
+
+int* stall_flag() {
+    static std::atomic<int*> flags[64];
+    int device = 0;
+    check(cudaGetDevice(&device), "cudaGetDevice");
+    std::atomic<int*>& flag = flags[device & 63];
+    int* p = flag.load(std::memory_order_acquire);
+    if (p == nullptr) {
+        check(cudaGetSymbolAddress(reinterpret_cast<void**>(&p), g_stalled), "stall flag");
+        flag.store(p, std::memory_order_release);
+    }
+    return p;
+}
+
+namespace {
+
+constexpr int64_t kMostRows = (1ll << 31) - 1024, kMostColumns = 1 << 22;
+
+void check_sizes(const char* what, int64_t rows, int64_t in, int64_t out) {
+    if (rows < 0 || rows > kMostRows) raise(T8B_EINVAL, std::string(what) + ": rows out of range");
+    if (in < 1 || in > kMostColumns || out < 1 || out > kMostColumns) {
+        raise(T8B_EINVAL, std::string(what) + ": features must be from 1 to 4194304");
+    }
+}
+
+void check_types(const char* what, int type, bool bias, int bias_type, int y_type, int activation) {
+    if (type != T8B_BF16 && type != T8B_F16) raise(T8B_EINVAL, std::string(what) + ": operands are bf16 or f16");
+    if (bias && bias_type != T8B_F32 && bias_type != type) raise(T8B_EINVAL, std::string(what) + ": the bias is fp32 or of the operands' type");
+    if (y_type != T8B_F32 && y_type != type) raise(T8B_EINVAL, std::string(what) + ": the output is fp32 or of the operands' type");
+    if (activation < T8B_LINEAR || activation > T8B_TANH) raise(T8B_EINVAL, std::string(what) + ": unknown activation");
+}
+
+void check_workspace(const char* what, const void* workspace, size_t have, size_t need) {
+    if (need > 0 && (workspace == nullptr || have < need || !aligned(workspace, 256))) {
+        raise(T8B_EINVAL, std::string(what) + ": the workspace is missing, not 256-byte aligned or below " + std::to_string(need) + " bytes");
+    }
+}
+
+void forward(const char* what, int type, LinearCall& c, void* workspace, size_t workspace_bytes) {
+    check_sizes(what, c.rows, c.in, c.out);
+    check_types(what, type, c.bias != nullptr, c.bias_type, c.y_type, c.activation);
+    const int64_t columns = c.gated ? 2 * c.out : c.out;
+    check_matrix(what, c.x, c.rows, c.in, c.x_stride);
+    check_matrix(what, c.weight, columns, c.in, c.weight_stride);
+    check_matrix(what, c.y, c.rows, c.out, c.y_stride);
+    if (c.residual) check_matrix(what, c.residual, c.rows, c.out, c.residual_stride);
+    if (c.pre) check_matrix(what, c.pre, c.rows, columns, c.pre_stride);
+    if (c.rows == 0) return;
+    const size_t ys = type_size(c.y_type);
+    const Span x(c.x, c.rows, c.in, c.x_stride, 2), w(c.weight, columns, c.in, c.weight_stride, 2);
+    const Span y(c.y, c.rows, c.out, c.y_stride, ys), pre(c.pre, c.rows, columns, c.pre_stride, 2);
+    const Span residual(c.residual, c.rows, c.out, c.residual_stride, ys);
+    const Span bias(c.bias, 1, columns, columns, type_size(c.bias_type));
+    const bool in_place = c.residual == c.y && c.residual_stride == c.y_stride;
+    if (y.overlaps(x) || y.overlaps(w) || y.overlaps(pre) || y.overlaps(bias) || (y.overlaps(residual) && !in_place) ||
+        pre.overlaps(x) || pre.overlaps(w) || pre.overlaps(residual) || pre.overlaps(bias)) {
+        raise(T8B_EINVAL, std::string(what) + ": an output overlaps another argument");
+    }
+    const bool packs = !tma_rows(c.x, c.rows, c.x_stride, 2) || !tma_rows(c.weight, columns, c.weight_stride, 2);
+    check_workspace(what, workspace, workspace_bytes, packs ? Workspace(c.rows, c.in, columns).forward_bytes : 0);
+    c.workspace = static_cast<unsigned char*>(workspace);
+    if (type == T8B_BF16) {
+        linear_forward<bf16>(c);
+    } else {
+        linear_forward<f16>(c);
+    }
+}
+
+void backward(const char* what, int type, LinearGradCall& c, void* workspace, size_t workspace_bytes) {
+    check_sizes(what, c.rows, c.in, c.out);
+    check_types(what, type, c.dbias != nullptr, c.bias_type, type, c.activation);
+    const int64_t columns = c.gated ? 2 * c.out : c.out;
+    check_matrix(what, c.dy, c.rows, c.out, c.dy_stride);
+    const bool reads_pre = c.gated || c.activation != T8B_LINEAR;
+    if (reads_pre) {
+        check_matrix(what, c.pre, c.rows, columns, c.pre_stride);
+    } else {
+        c.pre = nullptr;
+    }
+    if (c.dx) check_matrix(what, c.weight, columns, c.in, c.weight_stride);
+    if (c.dx) check_matrix(what, c.dx, c.rows, c.in, c.dx_stride);
+    if (c.dweight) check_matrix(what, c.x, c.rows, c.in, c.x_stride);
+    if (c.dweight) check_matrix(what, c.dweight, columns, c.in, c.dweight_stride);
+    if (c.rows == 0) {
+        if (c.dweight) {
+            check(cudaMemset2DAsync(c.dweight, c.dweight_stride * 2, 0, c.in * 2, columns, c.stream), "clear dweight");
+        }
+        if (c.dbias) check(cudaMemsetAsync(c.dbias, 0, columns * type_size(c.bias_type), c.stream), "clear dbias");
+        return;
+    }
+    const Span dy(c.dy, c.rows, c.out, c.dy_stride, 2), pre(c.pre, c.rows, columns, c.pre_stride, 2);
+    const Span x(c.dweight ? c.x : nullptr, c.rows, c.in, c.x_stride, 2);
+    const Span w(c.dx ? c.weight : nullptr, columns, c.in, c.weight_stride, 2);
+    const Span out[3] = {Span(c.dx, c.rows, c.in, c.dx_stride, 2), Span(c.dweight, columns, c.in, c.dweight_stride, 2),
+                         Span(c.dbias, 1, columns, columns, type_size(c.bias_type))};
+    for (int i = 0; i < 3; ++i) {
+        if (out[i].overlaps(dy) || out[i].overlaps(pre) || out[i].overlaps(x) || out[i].overlaps(w) || out[i].overlaps(out[(i + 1) % 3])) {
+            raise(T8B_EINVAL, std::string(what) + ": an output overlaps another argument");
+        }
+    }
+    check_workspace(what, workspace, workspace_bytes, Workspace(c.rows, c.in, columns).bytes);
+    c.workspace = static_cast<unsigned char*>(workspace);
+    if (type == T8B_BF16) {
+        linear_backward<bf16>(c);
+    } else {
+        linear_backward<f16>(c);
+    }
+}
+
+size_t workspace_size(int64_t rows, int64_t in, int64_t columns, int backward) {
+    if (rows < 1 || rows > kMostRows || in < 1 || columns < 1 || in > kMostColumns || columns > 2 * kMostColumns) return 0;
+    const Workspace w(rows, in, columns);
+    return backward ? w.bytes : w.forward_bytes;
+}
+
+}  // namespace
+}  // namespace op
+}  // namespace t8b
+
+using namespace t8b;
+using namespace t8b::op;
+
+extern "C" size_t t8b_linear_workspace(int64_t rows, int64_t in, int64_t out, int backward) {
+    return workspace_size(rows, in, out, backward);
+}
+extern "C" size_t t8b_gated_workspace(int64_t rows, int64_t in, int64_t out, int backward) {
+    return workspace_size(rows, in, 2 * out, backward);
+}
+
+extern "C" int t8b_linear_forward(int type, const void* x, int64_t x_stride, const void* weight, int64_t weight_stride,
+                                  const void* bias, int bias_type, int activation, const void* residual,
+                                  int64_t residual_stride, int64_t rows, int64_t in, int64_t out, void* y, int y_type,
+                                  int64_t y_stride, void* pre, int64_t pre_stride, void* workspace, size_t workspace_bytes,
+                                  void* stream) {
+    return guarded([&] {
+        LinearCall c{x, weight, bias, residual, y, pre, x_stride, weight_stride, residual_stride, y_stride, pre_stride, rows, in,
+                     out, bias_type, activation, y_type, false, nullptr, static_cast<cudaStream_t>(stream)};
+        forward("linear", type, c, workspace, workspace_bytes);
+    });
+}
+
+extern "C" int t8b_gated_forward(int type, const void* x, int64_t x_stride, const void* weight, int64_t weight_stride,
+                                 const void* bias, int bias_type, int activation, int64_t rows, int64_t in, int64_t out,
+                                 void* h, int64_t h_stride, void* pre, int64_t pre_stride, void* workspace,
+                                 size_t workspace_bytes, void* stream) {
+    return guarded([&] {
+        LinearCall c{x, weight, bias, nullptr, h, pre, x_stride, weight_stride, 0, h_stride, pre_stride, rows, in, out,
+                     bias_type, activation, type, true, nullptr, static_cast<cudaStream_t>(stream)};
+        forward("gated", type, c, workspace, workspace_bytes);
+    });
+}
+
+extern "C" int t8b_linear_backward(int type, const void* dy, int64_t dy_stride, const void* x, int64_t x_stride,
+                                   const void* weight, int64_t weight_stride, const void* pre, int64_t pre_stride,
+                                   int bias_type, int activation, int64_t rows, int64_t in, int64_t out, void* dx,
+                                   int64_t dx_stride, void* dweight, int64_t dweight_stride, void* dbias, void* workspace,
+                                   size_t workspace_bytes, void* stream) {
+    return guarded([&] {
+        LinearGradCall c{dy, x, weight, pre, dx, dweight, dbias, dy_stride, x_stride, weight_stride, pre_stride, dx_stride,
+                         dweight_stride, rows, in, out, bias_type, activation, false, nullptr, static_cast<cudaStream_t>(stream)};
+        backward("linear", type, c, workspace, workspace_bytes);
+    });
+}
+
+extern "C" int t8b_gated_backward(int type, const void* dh, int64_t dh_stride, const void* x, int64_t x_stride,
+                                  const void* weight, int64_t weight_stride, const void* pre, int64_t pre_stride,
+                                  int bias_type, int activation, int64_t rows, int64_t in, int64_t out, void* dx,
+                                  int64_t dx_stride, void* dweight, int64_t dweight_stride, void* dbias, void* workspace,
+                                  size_t workspace_bytes, void* stream) {
+    return guarded([&] {
+        LinearGradCall c{dh, x, weight, pre, dx, dweight, dbias, dh_stride, x_stride, weight_stride, pre_stride, dx_stride,
+                         dweight_stride, rows, in, out, bias_type, activation, true, nullptr, static_cast<cudaStream_t>(stream)};
+        backward("gated", type, c, workspace, workspace_bytes);
+    });
+}
+
+extern "C" int t8b_operators_status(void* stream) {
+    return guarded([&] {
+        cudaStream_t st = static_cast<cudaStream_t>(stream);
+        int stalled = 0;
+        int* flag = stall_flag();
+        check(cudaMemcpyAsync(&stalled, flag, sizeof(int), cudaMemcpyDeviceToHost, st), "read stall flag");
+        check(cudaStreamSynchronize(st), "read stall flag");
+        if (stalled) {
+            check(cudaMemsetAsync(flag, 0, sizeof(int), st), "clear stall flag");
+            check(cudaStreamSynchronize(st), "clear stall flag");
+            raise(T8B_ECUDA, "a wait inside an operator's kernel ran out");
+        }
+    });
+}

@@ -1,0 +1,683 @@
+// The linear map and the gated projection for one element type (bf16 or f16): epilogues over the
+// GEMM of ops_gemm.cuh, the elementwise half of the backward passes, and the host side that plans
+// and queues a call. ops_bf16.cu and ops_f16.cu instantiate it; ops_linear.cu holds the C entries.
+#pragma once
+
+#include <algorithm>
+#include <atomic>
+
+#include "gemm_host.cuh"
+#include "ops_gemm.cuh"
+
+namespace t8b {
+namespace op {
+
+// The device's flag for waits that ran out (ops_linear.cu).
+int* stall_flag();
+
+struct LinearCall {
+    const void *x, *weight, *bias, *residual;
+    void *y, *pre;
+    int64_t x_stride, weight_stride, residual_stride, y_stride, pre_stride;
+    int64_t rows, in, out;
+    int bias_type, activation, y_type;
+    bool gated;
+    unsigned char* workspace;
+    cudaStream_t stream;
+};
+struct LinearGradCall {
+    const void *dy, *x, *weight, *pre;
+    void *dx, *dweight, *dbias;
+    int64_t dy_stride, x_stride, weight_stride, pre_stride, dx_stride, dweight_stride;
+    int64_t rows, in, out;
+    int bias_type, activation;
+    bool gated;
+    unsigned char* workspace;
+    cudaStream_t stream;
+};
+template <typename E>
+void linear_forward(const LinearCall& c);
+template <typename E>
+void linear_backward(const LinearGradCall& c);
+
+// ------------------------------------------------------------------ planning
+// A GEMM's tile (pairs of CTAs on 256 x 256 or 256 x 128, or one CTA on 128 x 64) and the number of
+// parts its k blocks are split into.
+struct GemmPlan {
+    int pair, bn, splits;
+};
+constexpr int kClusters = 74, kSms = 148;
+constexpr int kMaxSplits = 64;
+
+inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Cycles of the busiest CTA as the plan's cost: waves x (k blocks x their MMA cycles + the tile's
+// latency), plus the pass that joins the parts (its traffic over the chip's, and its launch).
+inline GemmPlan plan_gemm(int64_t m, int64_t n, int64_t k, bool may_split) {
+    struct Form {
+        int pair, bn;
+        double block_cycles, tile_cycles;
+    };
+    static constexpr Form forms[] = {{1, 256, 540, 3500}, {1, 128, 330, 2600}, {0, 64, 220, 2200}};
+    const int64_t k_blocks = ceil_div(k, tc::BK);
+    GemmPlan best{1, 256, 1};
+    double least = 1e300;
+    for (const Form& f : forms) {
+        const int64_t tiles = ceil_div(m, f.pair ? 256 : 128) * ceil_div(n, f.bn);
+        const int64_t workers = f.pair ? kClusters : kSms;
+        const int64_t most = may_split ? std::min<int64_t>(kMaxSplits, std::max<int64_t>(1, k_blocks / 4)) : 1;
+        for (int64_t splits = 1; splits <= most; ++splits) {
+            const double waves = static_cast<double>(ceil_div(tiles * splits, workers));
+            double cost = waves * (static_cast<double>(ceil_div(k_blocks, splits)) * f.block_cycles + f.tile_cycles);
+            if (splits > 1) cost += 6000.0 + static_cast<double>(splits) * m * n * 8.0 / 2500.0;
+            if (cost < least) {
+                least = cost;
+                best = GemmPlan{f.pair, f.bn, static_cast<int>(splits)};
+            }
+        }
+    }
+    return best;
+}
+
+// The parts of a split GEMM: fp32 [splits][rows to whole tiles][columns to whole pieces].
+inline size_t split_rows(int64_t m) { return round_up(m, 256); }
+inline size_t split_pitch(int64_t n) { return round_up(n, 4); }
+
+// Row parts of the elementwise backward pass (each gives one row of partial column sums).
+constexpr int kGradRows = 8;
+inline int grad_parts(int64_t rows, int64_t columns) {
+    const int64_t across = ceil_div(columns, 256);
+    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(ceil_div(rows, kGradRows), ceil_div(kSms * 6, across))));
+}
+
+// The workspace, in this order; each part starts on a 256-byte boundary. A forward pass uses the
+// first two, and them only for operands whose rows do not suit TMA.
+struct Workspace {
+    size_t x, weight, forward_bytes, dz, sums, parts, bytes;
+    size_t dz_pitch, x_pitch;
+    Workspace(int64_t rows, int64_t in, int64_t columns) {
+        x_pitch = round_up(in, 8);
+        dz_pitch = round_up(columns, 8);
+        size_t at = 0;
+        const auto take = [&](size_t size) {
+            const size_t here = at;
+            at += round_up(size, 256);
+            return here;
+        };
+        x = take(rows * x_pitch * 2);
+        weight = take(columns * x_pitch * 2);
+        forward_bytes = at;
+        dz = take(rows * dz_pitch * 2);
+        sums = take(static_cast<size_t>(grad_parts(rows, columns)) * columns * 4);
+        const GemmPlan p = plan_gemm(columns, in, rows, true);
+        parts = take(p.splits > 1 ? p.splits * split_rows(columns) * split_pitch(in) * 4 : 0);
+        bytes = at;
+    }
+};
+
+// ------------------------------------------------------------------ epilogues
+// 32 fp32 values as the packed 16-bit or fp32 pieces of a staging tile's row.
+template <typename T, int BYTES>
+__device__ __forceinline__ void stage32(unsigned char* tile, int row, int at, const float (&v)[32]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            *reinterpret_cast<float4*>(piece<BYTES>(tile, row, at / 4 + q)) = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+        }
+    } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            *reinterpret_cast<uint4*>(piece<BYTES>(tile, row, at / 8 + q)) =
+                make_uint4(Element<T>::pack(v[8 * q], v[8 * q + 1]), Element<T>::pack(v[8 * q + 2], v[8 * q + 3]),
+                           Element<T>::pack(v[8 * q + 4], v[8 * q + 5]), Element<T>::pack(v[8 * q + 6], v[8 * q + 7]));
+        }
+    }
+}
+template <typename T, int BYTES>
+__device__ __forceinline__ void add32(unsigned char* tile, int row, int at, float (&v)[32]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            const float4 r = *reinterpret_cast<const float4*>(piece<BYTES>(tile, row, at / 4 + q));
+            v[4 * q] += r.x;
+            v[4 * q + 1] += r.y;
+            v[4 * q + 2] += r.z;
+            v[4 * q + 3] += r.w;
+        }
+    } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const uint4 r = *reinterpret_cast<const uint4*>(piece<BYTES>(tile, row, at / 8 + q));
+            const uint32_t words[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float2 f = Element<T>::unpack(words[k]);
+                v[8 * q + 2 * k] += f.x;
+                v[8 * q + 2 * k + 1] += f.y;
+            }
+        }
+    }
+}
+// 32 bias values through the warp's vector, one read a lane, then added to every row.
+__device__ __forceinline__ float bias_at(const void* bias, int type, int c, int columns) {
+    return bias != nullptr && c < columns ? load_any(bias, type, c) : 0.0f;
+}
+__device__ __forceinline__ void add_bias32(float* vector, float mine, int lane, float (&v)[32]) {
+    __syncwarp();
+    vector[lane] = mine;
+    __syncwarp();
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+        const float4 b = reinterpret_cast<const float4*>(vector)[q];
+        v[4 * q] += b.x;
+        v[4 * q + 1] += b.y;
+        v[4 * q + 2] += b.z;
+        v[4 * q + 3] += b.w;
+    }
+}
+
+// y = activation(acc + bias) + residual in the type O, and acc + bias as `pre`; without FULL, acc
+// alone (gradients, and the fp32 parts of a split GEMM). A half of the epilogue warps takes half
+// of the tile's columns, in chunks of a 128-byte row (64 bytes where half a tile is narrower).
+template <typename E, typename O, int BN, bool FULL>
+struct EpiLinear {
+    static constexpr int kWide = sizeof(O) == 4 || BN < 128 ? 32 : 64;  // columns of a chunk
+    static constexpr int kBytes = kWide * sizeof(O);
+    static constexpr int kPreBytes = kWide * 2;
+    static constexpr int kChunks = BN / 2 / kWide;
+    Tiled y, residual, pre;
+    const void* bias;
+    int bias_type, activation, has_residual, has_pre, split_rows;
+
+    __device__ __forceinline__ int column(const Warp& w, int chunk) const { return w.tn * BN + w.half * (BN / 2) + chunk * kWide; }
+    // y's staging tile, `ahead` chunks from the next one sent: the two in turn, or the second where
+    // the first holds `pre`
+    __device__ __forceinline__ int tile_of(const Warp& w, int ahead) const { return FULL && has_pre ? 1 : (w.turn + ahead) & 1; }
+    __device__ __forceinline__ void fetch_chunk(Warp& w, int chunk, int ahead) const {
+        const int col = column(w, chunk), i = tile_of(w, ahead);
+        if (chunk >= kChunks || col >= y.columns) return;
+        fetch<O, kBytes>(residual, w.tiles + i * kStageTile, w.bars + i, w.row0, col, w.lane);
+        if (residual.tma) w.in_flight |= 1u << i;
+    }
+    __device__ __forceinline__ void begin(Warp& w) const {
+        if (!FULL || !has_residual || w.row0 >= y.rows) return;
+        free_tiles<0>(w.lane);
+        fetch_chunk(w, 0, 0);
+        if (!has_pre) fetch_chunk(w, 1, 1);
+    }
+    __device__ __forceinline__ bool finish(Warp& w) const {
+        if (w.row0 >= y.rows) return true;
+        const int row0 = w.row0 + w.split * split_rows;
+#pragma unroll 1
+        for (int chunk = 0; chunk < kChunks; ++chunk) {
+            const int col = column(w, chunk), i = tile_of(w, 0);
+            if (col >= y.columns) break;
+            unsigned char* tile = w.tiles + i * kStageTile;
+            if (FULL && has_residual) {
+                if (residual.tma && !w.wait(i)) return false;
+            } else if (FULL && has_pre) {
+                free_tiles<0>(w.lane);
+            } else {
+                free_tiles<1>(w.lane);
+            }
+#pragma unroll 1
+            for (int at = 0; at < kWide; at += 32) {
+                float v[32];
+                float b = 0.0f;
+                if (FULL) b = bias_at(bias, bias_type, col + at + w.lane, y.columns);
+                tc::tmem_load32(w.taddr + w.half * (BN / 2) + chunk * kWide + at, v);
+                if (FULL) {
+                    if (bias != nullptr) add_bias32(w.vector, b, w.lane, v);
+                    if (has_pre) stage32<E, kPreBytes>(w.tiles, w.lane, at, v);
+                    with_activation(activation, [&](auto act) {
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) v[k] = activate<decltype(act)::value>(v[k]);
+                    });
+                    if (has_residual) add32<O, kBytes>(tile, w.lane, at, v);
+                }
+                stage32<O, kBytes>(tile, w.lane, at, v);
+            }
+            if (FULL && has_pre) send<E, kPreBytes>(pre, w.tiles, row0, col, w.lane);
+            send<O, kBytes>(y, tile, row0, col, w.lane);
+            ++w.turn;
+            if (FULL && has_residual) {  // into the tile just sent
+                const int next = chunk + (has_pre ? 1 : 2);
+                if (next < kChunks) {
+                    free_tiles<0>(w.lane);
+                    fetch_chunk(w, next, 1);
+                }
+            }
+        }
+        return true;
+    }
+};
+
+// h = activation(gate) up; the accumulator's first BN / 2 columns are the gate's, the others the
+// up projection's of the same columns of h.
+template <typename E, int BN>
+struct EpiGated {
+    static constexpr int kHalf = BN / 2;
+    static constexpr int kWide = BN == 256 ? 64 : 32;
+    static constexpr int kBytes = kWide * 2;
+    Tiled h, gate, up;
+    const void* bias;
+    int bias_type, activation, has_pre;
+
+    __device__ __forceinline__ void begin(Warp&) const {}
+    __device__ __forceinline__ bool finish(Warp& w) const {
+        const int first = w.half * kWide, col = w.tn * kHalf + first;
+        if (w.row0 >= h.rows || first >= kHalf || col >= h.columns) return true;
+        uint32_t packed[kWide / 2];
+        if (has_pre) free_tiles<0>(w.lane);
+#pragma unroll
+        for (int at = 0; at < kWide; at += 32) {
+            float g[32], u[32];
+            const int c = col + at + w.lane;
+            float bg = 0.0f, bu = 0.0f;
+            if (bias != nullptr && c < h.columns) {
+                bg = load_any(bias, bias_type, c);
+                bu = load_any(bias, bias_type, h.columns + c);
+            }
+            tc::tmem_load32(w.taddr + first + at, g);
+            tc::tmem_load32(w.taddr + kHalf + first + at, u);
+            if (bias != nullptr) {
+                add_bias32(w.vector, bg, w.lane, g);
+                add_bias32(w.vector + 32, bu, w.lane, u);
+            }
+            if (has_pre) {
+                stage32<E, kBytes>(w.tiles, w.lane, at, g);
+                stage32<E, kBytes>(w.tiles + kStageTile, w.lane, at, u);
+            }
+            with_activation(activation, [&](auto act) {
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                    packed[at / 2 + k] = Element<E>::pack(activate<decltype(act)::value>(g[2 * k]) * u[2 * k],
+                                                          activate<decltype(act)::value>(g[2 * k + 1]) * u[2 * k + 1]);
+                }
+            });
+        }
+        unsigned char* tile = w.tiles;
+        if (has_pre) {
+            send<E, kBytes>(gate, w.tiles, w.row0, col, w.lane);
+            send<E, kBytes>(up, w.tiles + kStageTile, w.row0, col, w.lane);
+            if (up.tma) free_tiles<1>(w.lane); else free_tiles<0>(w.lane);  // the gate's tile
+        } else {
+            tile += (w.turn++ & 1) * kStageTile;
+            free_tiles<1>(w.lane);
+        }
+#pragma unroll
+        for (int q = 0; q < kWide / 8; ++q) {
+            *reinterpret_cast<uint4*>(piece<kBytes>(tile, w.lane, q)) =
+                make_uint4(packed[4 * q], packed[4 * q + 1], packed[4 * q + 2], packed[4 * q + 3]);
+        }
+        send<E, kBytes>(h, tile, w.row0, col, w.lane);
+        return true;
+    }
+};
+
+// ------------------------------------------------------------------ elementwise kernels
+// Rows of `in` with any stride, copied to rows of `pitch` (a multiple of 8) elements: operands whose
+// rows do not start on 16-byte boundaries, which TMA asks for. One 16-byte piece a thread.
+template <typename E>
+__global__ void k_pack(const E* in, int64_t stride, int64_t rows, int columns, E* out, int pitch) {
+    const int pieces = pitch / 8;
+    const int64_t total = rows * pieces;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
+         i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+        const int64_t row = i / pieces;
+        const int c = static_cast<int>(i - row * pieces) * 8;
+        Pack<E, 8> p;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) p.v[j] = c + j < columns ? in[row * stride + c + j] : Element<E>::store(0.0f);
+        *reinterpret_cast<Pack<E, 8>*>(out + row * pitch + c) = p;
+    }
+}
+
+// The elementwise half of a backward pass: dz (rows of `pitch` elements) from dy and pre, and this
+// block row's column sums of dz in fp32, before dz is rounded. A thread holds V columns over its
+// rows; block (32, kGradRows).
+//   linear: dz = dy activation'(pre);  gated: dz = [dy up activation'(gate) | dy activation(gate)]
+template <typename E, bool GATED, int V>
+__global__ void __launch_bounds__(32 * kGradRows)
+    k_activation_grad(const E* dy, int64_t dy_stride, const E* pre, int64_t pre_stride, int64_t rows, int columns,
+                      int activation, E* dz, int64_t pitch, float* sums) {
+    constexpr int PARTS = GATED ? 2 : 1;
+    __shared__ float joined[kGradRows][32 * V + 1];
+    const int c = (blockIdx.x * 32 + threadIdx.x) * V;
+    const bool in = c < columns;
+    float sum[PARTS][V];
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) sum[p][j] = 0.0f;
+    }
+    with_activation(activation, [&](auto act) {
+        constexpr int ACT = decltype(act)::value;
+        for (int64_t row = static_cast<int64_t>(blockIdx.y) * kGradRows + threadIdx.y; in && row < rows;
+             row += static_cast<int64_t>(gridDim.y) * kGradRows) {
+            const Pack<E, V> d = *reinterpret_cast<const Pack<E, V>*>(dy + row * dy_stride + c);
+            Pack<E, V> z{}, u{}, out{};
+            if (GATED || ACT != T8B_LINEAR) z = *reinterpret_cast<const Pack<E, V>*>(pre + row * pre_stride + c);
+            if (GATED) u = *reinterpret_cast<const Pack<E, V>*>(pre + row * pre_stride + columns + c);
+            float value[V], slope[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) activate_slope<ACT>(Element<E>::load(z.v[j]), value[j], slope[j]);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float of_z = Element<E>::load(d.v[j]) * slope[j] * (GATED ? Element<E>::load(u.v[j]) : 1.0f);
+                sum[0][j] += of_z;
+                out.v[j] = Element<E>::store(of_z);
+            }
+            if (dz) *reinterpret_cast<Pack<E, V>*>(dz + row * pitch + c) = out;
+            if (GATED) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    const float of_u = Element<E>::load(d.v[j]) * value[j];
+                    sum[PARTS - 1][j] += of_u;
+                    out.v[j] = Element<E>::store(of_u);
+                }
+                if (dz) *reinterpret_cast<Pack<E, V>*>(dz + row * pitch + columns + c) = out;
+            }
+        }
+    });
+    if (sums == nullptr) return;
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p) {
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < V; ++j) joined[threadIdx.y][threadIdx.x * V + j] = sum[p][j];
+        __syncthreads();
+        for (int k = threadIdx.y * 32 + threadIdx.x; k < 32 * V; k += 32 * kGradRows) {
+            const int column = blockIdx.x * 32 * V + k;
+            if (column >= columns) continue;
+            float v = 0.0f;
+#pragma unroll
+            for (int r = 0; r < kGradRows; ++r) v += joined[r][k];
+            sums[static_cast<size_t>(blockIdx.y) * columns * PARTS + p * columns + column] = v;
+        }
+    }
+}
+
+// dbias from the block rows' column sums, in a fixed order. Block (32, 16).
+static __global__ void k_bias_grad(const float* sums, int count, int columns, void* out, int type) {
+    __shared__ float joined[16][33];
+    const int c = blockIdx.x * 32 + threadIdx.x;
+    float v = 0.0f;
+    if (c < columns) {
+#pragma unroll 4
+        for (int r = threadIdx.y; r < count; r += 16) v += sums[static_cast<size_t>(r) * columns + c];
+    }
+    joined[threadIdx.y][threadIdx.x] = v;
+    __syncthreads();
+    if (threadIdx.y != 0 || c >= columns) return;
+#pragma unroll
+    for (int r = 1; r < 16; ++r) v += joined[r][threadIdx.x];
+    store_any(out, type, c, v);
+}
+
+// The parts of a split GEMM, added in order and rounded once.
+template <typename E>
+__global__ void k_join_parts(const float* parts, int splits, size_t part_elements, int pitch, int rows, int columns, E* out,
+                             int64_t stride) {
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+    const int pieces = pitch / 4;
+    if (i >= static_cast<int64_t>(rows) * pieces) return;
+    const int row = static_cast<int>(i / pieces), c = static_cast<int>(i % pieces) * 4;
+    const float* p = parts + static_cast<size_t>(row) * pitch + c;
+    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+    for (int s = 0; s < splits; ++s, p += part_elements) {
+        const float4 v = *reinterpret_cast<const float4*>(p);
+        sum.x += v.x;
+        sum.y += v.y;
+        sum.z += v.z;
+        sum.w += v.w;
+    }
+    const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+    E* to = out + static_cast<int64_t>(row) * stride + c;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if (c + j < columns) to[j] = Element<E>::store(v[j]);
+    }
+}
+
+// ------------------------------------------------------------------ host side
+template <typename T>
+CUtensorMap tensor_map(const void* base, uint64_t inner, uint64_t outer, uint64_t pitch, uint32_t box_inner, uint32_t box_outer,
+                       CUtensorMapSwizzle swizzle) {
+    constexpr CUtensorMapDataType type = Element<T>::kType == T8B_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+        : Element<T>::kType == T8B_BF16                               ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                                      : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    CUtensorMap map;
+    const cuuint64_t dims[2] = {inner, outer};
+    const cuuint64_t strides[1] = {pitch * sizeof(T)};
+    const cuuint32_t box[2] = {box_inner, box_outer};
+    const cuuint32_t element[2] = {1, 1};
+    const CUresult r = tensor_map_encoder()(&map, type, 2, const_cast<void*>(base), dims, strides, box, element,
+                                            CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) raise(T8B_ECUDA, "cuTensorMapEncodeTiled failed: " + std::to_string(static_cast<int>(r)));
+    return map;
+}
+
+// Rows that TMA can address: 16-byte starts, and a row stride below its 2^40 bytes.
+inline bool tma_rows(const void* p, int64_t rows, int64_t stride, size_t size) {
+    return aligned(p, 16) && (rows <= 1 || ((stride * size) % 16 == 0 && stride * size < (1ull << 40)));
+}
+inline int64_t tma_pitch(int64_t rows, int64_t columns, int64_t stride, size_t size) {
+    return rows <= 1 ? round_up(columns, 16 / size) : stride;
+}
+
+template <typename T, int BYTES>
+Tiled tiled(const void* data, int64_t rows, int64_t columns, int64_t stride) {
+    Tiled t{};
+    t.data = const_cast<void*>(data);
+    t.stride = stride;
+    t.rows = static_cast<int>(rows);
+    t.columns = static_cast<int>(columns);
+    t.tma = data != nullptr && tma_rows(data, rows, stride, sizeof(T));
+    if (t.tma) {
+        t.map = tensor_map<T>(data, columns, rows, tma_pitch(rows, columns, stride, sizeof(T)), BYTES / sizeof(T), 32,
+                              BYTES == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+    }
+    return t;
+}
+
+// A GEMM operand: row-major [rows][k] (K-major) or [k][rows] (MN-major), rows on 16-byte boundaries.
+struct Matrix {
+    const void* data;
+    int64_t rows, k, pitch;
+};
+
+template <typename E, int CG, int BN, bool A_MN, bool B_MN, class Epi>
+void launch_gemm(const char* label, const Matrix& a, const Matrix& b, int64_t columns, int second, int splits, const Epi& epi,
+                 cudaStream_t stream) {
+    using P = Plan<CG, BN>;
+    auto kernel = k_gemm<E, CG, BN, A_MN, B_MN, Epi>;
+    static uint64_t configured = 0;
+    allow_smem(kernel, P::kSmemBytes, configured);
+    Shape s{};
+    s.tiles_m = static_cast<int>(ceil_div(a.rows, tc::BM * CG));
+    s.tiles_n = static_cast<int>(ceil_div(columns, second ? BN / 2 : BN));
+    s.k_blocks = static_cast<int>(ceil_div(a.k, tc::BK));
+    s.splits = splits;
+    s.second = second;
+    s.error = stall_flag();
+    const auto k_major = [](const Matrix& m, uint32_t box) {
+        return tensor_map<E>(m.data, m.k, m.rows, tma_pitch(m.rows, m.k, m.pitch, 2), tc::BK, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    };
+    const auto mn_major = [](const Matrix& m) {
+        return tensor_map<E>(m.data, m.rows, m.k, tma_pitch(m.k, m.rows, m.pitch, 2), 64, tc::BK, CU_TENSOR_MAP_SWIZZLE_128B);
+    };
+    const CUtensorMap map_a = A_MN ? mn_major(a) : k_major(a, tc::BM);
+    const CUtensorMap map_b = B_MN ? mn_major(b) : k_major(b, second ? BN / 2 : BN / CG);
+    const int64_t work = static_cast<int64_t>(s.tiles_m) * s.tiles_n * s.splits;
+    const int grid = static_cast<int>(std::min<int64_t>(work, CG == 2 ? kClusters : kSms)) * CG;
+    launch(label, kernel, grid, kGemmThreads, P::kSmemBytes, stream, map_a, map_b, s, epi);
+    check(cudaGetLastError(), label);
+}
+
+// A matrix as a GEMM operand: where its rows do not suit TMA, a packed copy in the workspace.
+template <typename E>
+Matrix operand(const void* data, int64_t rows, int64_t columns, int64_t stride, unsigned char* copy, cudaStream_t stream) {
+    if (tma_rows(data, rows, stride, sizeof(E))) return Matrix{data, rows, columns, tma_pitch(rows, columns, stride, sizeof(E))};
+    const int64_t pitch = round_up(columns, 8);
+    const int64_t pieces = rows * (pitch / 8);
+    launch("k_pack", k_pack<E>, static_cast<unsigned>(std::min<int64_t>(ceil_div(pieces, 256), kSms * 16)), 256, 0, stream,
+           static_cast<const E*>(data), stride, rows, static_cast<int>(columns), reinterpret_cast<E*>(copy), static_cast<int>(pitch));
+    return Matrix{copy, rows, columns, pitch};
+}
+// [rows][k] read along its rows' other axis: the same storage as an MN-major operand.
+inline Matrix transposed(const Matrix& m) { return Matrix{m.data, m.k, m.rows, m.pitch}; }
+
+template <typename E, typename O, int CG, int BN>
+void forward_tile(const LinearCall& c, const Matrix& x, const Matrix& w) {
+    using Epi = EpiLinear<E, O, BN, true>;
+    Epi epi{};
+    epi.y = tiled<O, Epi::kBytes>(c.y, c.rows, c.out, c.y_stride);
+    if (c.residual) epi.residual = tiled<O, Epi::kBytes>(c.residual, c.rows, c.out, c.residual_stride);
+    if (c.pre) epi.pre = tiled<E, Epi::kPreBytes>(c.pre, c.rows, c.out, c.pre_stride);
+    epi.residual.rows = static_cast<int>(c.rows);
+    epi.residual.columns = static_cast<int>(c.out);
+    epi.bias = c.bias;
+    epi.bias_type = c.bias_type;
+    epi.activation = c.activation;
+    epi.has_residual = c.residual != nullptr;
+    epi.has_pre = c.pre != nullptr;
+    launch_gemm<E, CG, BN, false, false>("k_linear", x, w, c.out, 0, 1, epi, c.stream);
+}
+template <typename E, int CG, int BN>
+void gated_tile(const LinearCall& c, const Matrix& x, const Matrix& w) {
+    using Epi = EpiGated<E, BN>;
+    Epi epi{};
+    epi.h = tiled<E, Epi::kBytes>(c.y, c.rows, c.out, c.y_stride);
+    if (c.pre) {
+        epi.gate = tiled<E, Epi::kBytes>(c.pre, c.rows, c.out, c.pre_stride);
+        epi.up = tiled<E, Epi::kBytes>(static_cast<E*>(c.pre) + c.out, c.rows, c.out, c.pre_stride);
+    }
+    epi.bias = c.bias;
+    epi.bias_type = c.bias_type;
+    epi.activation = c.activation;
+    epi.has_pre = c.pre != nullptr;
+    launch_gemm<E, CG, BN, false, false>("k_gated", x, w, c.out, static_cast<int>(c.out), 1, epi, c.stream);
+}
+
+template <typename E>
+void linear_forward(const LinearCall& c) {
+    const int64_t columns = c.gated ? 2 * c.out : c.out;
+    const Workspace at(c.rows, c.in, columns);
+    const Matrix x = operand<E>(c.x, c.rows, c.in, c.x_stride, c.workspace + at.x, c.stream);
+    const Matrix w = operand<E>(c.weight, columns, c.in, c.weight_stride, c.workspace + at.weight, c.stream);
+    const GemmPlan p = plan_gemm(c.rows, columns, c.in, false);
+    if (c.gated) {
+        if (p.bn == 256) {
+            gated_tile<E, 2, 256>(c, x, w);
+        } else if (p.bn == 128) {
+            gated_tile<E, 2, 128>(c, x, w);
+        } else {
+            gated_tile<E, 1, 64>(c, x, w);
+        }
+    } else if (c.y_type == T8B_F32) {
+        if (p.bn == 256) {
+            forward_tile<E, float, 2, 256>(c, x, w);
+        } else if (p.bn == 128) {
+            forward_tile<E, float, 2, 128>(c, x, w);
+        } else {
+            forward_tile<E, float, 1, 64>(c, x, w);
+        }
+    } else {
+        if (p.bn == 256) {
+            forward_tile<E, E, 2, 256>(c, x, w);
+        } else if (p.bn == 128) {
+            forward_tile<E, E, 2, 128>(c, x, w);
+        } else {
+            forward_tile<E, E, 1, 64>(c, x, w);
+        }
+    }
+}
+
+// out [a.rows][b.rows] = A . B^T without bias or activation, in E; split k parts go through `parts`.
+template <typename E, int CG, int BN, bool A_MN>
+void product_tile(const char* label, const Matrix& a, const Matrix& b, int splits, void* out, int64_t stride, float* parts,
+                  cudaStream_t stream) {
+    if (splits == 1) {
+        using Epi = EpiLinear<E, E, BN, false>;
+        Epi epi{};
+        epi.y = tiled<E, Epi::kBytes>(out, a.rows, b.rows, stride);
+        launch_gemm<E, CG, BN, A_MN, true>(label, a, b, b.rows, 0, 1, epi, stream);
+        return;
+    }
+    if constexpr (A_MN) {
+        using Epi = EpiLinear<E, float, BN, false>;
+        Epi epi{};
+        const int64_t rows = split_rows(a.rows), pitch = split_pitch(b.rows);
+        epi.y = tiled<float, Epi::kBytes>(parts, rows * splits, b.rows, pitch);
+        epi.split_rows = static_cast<int>(rows);
+        launch_gemm<E, CG, BN, A_MN, true>(label, a, b, b.rows, 0, splits, epi, stream);
+        launch("k_join_parts", k_join_parts<E>, blocks(a.rows * (pitch / 4), 256), 256, 0, stream, static_cast<const float*>(parts),
+               splits, static_cast<size_t>(rows) * pitch, static_cast<int>(pitch), static_cast<int>(a.rows),
+               static_cast<int>(b.rows), static_cast<E*>(out), stride);
+    }
+}
+template <typename E, bool A_MN>
+void product(const char* label, const Matrix& a, const Matrix& b, const GemmPlan& p, void* out, int64_t stride, float* parts,
+             cudaStream_t stream) {
+    if (p.bn == 256) {
+        product_tile<E, 2, 256, A_MN>(label, a, b, p.splits, out, stride, parts, stream);
+    } else if (p.bn == 128) {
+        product_tile<E, 2, 128, A_MN>(label, a, b, p.splits, out, stride, parts, stream);
+    } else {
+        product_tile<E, 1, 64, A_MN>(label, a, b, p.splits, out, stride, parts, stream);
+    }
+}
+
+template <typename E, bool GATED, int V>
+void activation_grad(const LinearGradCall& c, E* dz, int64_t pitch, float* sums) {
+    const int columns = static_cast<int>(c.out);
+    const dim3 grid(blocks(columns, 32 * V), grad_parts(c.rows, GATED ? 2 * c.out : c.out));
+    launch("k_activation_grad", k_activation_grad<E, GATED, V>, grid, dim3(32, kGradRows), 0, c.stream,
+           static_cast<const E*>(c.dy), c.dy_stride, static_cast<const E*>(c.pre), c.pre_stride, c.rows, columns, c.activation, dz,
+           pitch, sums);
+    check(cudaGetLastError(), "activation gradient");
+}
+
+template <typename E>
+void linear_backward(const LinearGradCall& c) {
+    const int64_t columns = c.gated ? 2 * c.out : c.out;
+    const Workspace at(c.rows, c.in, columns);
+    // dz is dy itself where there is neither a gate nor an activation and its rows suit TMA
+    const bool own = c.gated || c.activation != T8B_LINEAR || !tma_rows(c.dy, c.rows, c.dy_stride, sizeof(E));
+    E* dz_out = own && (c.dx || c.dweight) ? reinterpret_cast<E*>(c.workspace + at.dz) : nullptr;
+    float* sums = c.dbias ? reinterpret_cast<float*>(c.workspace + at.sums) : nullptr;
+    Matrix dz{c.dy, c.rows, columns, tma_pitch(c.rows, columns, c.dy_stride, sizeof(E))};
+    if (dz_out) dz = Matrix{dz_out, c.rows, columns, static_cast<int64_t>(at.dz_pitch)};
+    if (dz_out || sums) {
+        // eight columns a thread where every row of dy, pre and dz starts on a 16-byte boundary
+        const bool wide = c.out % 8 == 0 && aligned(c.dy, 16) && c.dy_stride % 8 == 0 &&
+            (c.pre == nullptr || (aligned(c.pre, 16) && c.pre_stride % 8 == 0));
+        const int64_t pitch = static_cast<int64_t>(at.dz_pitch);
+        if (c.gated) {
+            wide ? activation_grad<E, true, 8>(c, dz_out, pitch, sums) : activation_grad<E, true, 1>(c, dz_out, pitch, sums);
+        } else {
+            wide ? activation_grad<E, false, 8>(c, dz_out, pitch, sums) : activation_grad<E, false, 1>(c, dz_out, pitch, sums);
+        }
+    }
+    if (sums) {
+        launch("k_bias_grad", k_bias_grad, blocks(columns, 32), dim3(32, 16), 0, c.stream, static_cast<const float*>(sums),
+               grad_parts(c.rows, columns), static_cast<int>(columns), c.dbias, c.bias_type);
+    }
+    if (c.dx) {
+        const Matrix w = operand<E>(c.weight, columns, c.in, c.weight_stride, c.workspace + at.weight, c.stream);
+        product<E, false>("k_input_grad", dz, transposed(w), plan_gemm(c.rows, c.in, columns, false), c.dx, c.dx_stride, nullptr,
+                          c.stream);
+    }
+    if (c.dweight) {
+        const Matrix x = operand<E>(c.x, c.rows, c.in, c.x_stride, c.workspace + at.x, c.stream);
+        product<E, true>("k_weight_grad", transposed(dz), transposed(x), plan_gemm(columns, c.in, c.rows, true), c.dweight,
+                         c.dweight_stride, reinterpret_cast<float*>(c.workspace + at.parts), c.stream);
+    }
+    check(cudaGetLastError(), "linear backward");
+}
+
+}  // namespace op
+}  // namespace t8b

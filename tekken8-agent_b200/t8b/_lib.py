@@ -360,3 +360,24 @@ PROTOTYPES.update({
     "t8b_collect_rollout": (C.c_int, [vp, vp, vp, vp, u64, u64, C.c_size_t, C.c_float, vp]),
     "t8b_rollout_synchronize": (C.c_int, [vp, vp]),
 })
+
+# ------------------------------------------------------------------ torso operators
+i64 = C.c_int64
+PROTOTYPES.update({
+    "t8b_layer_norm_forward": (C.c_int, [vp, C.c_int, i64, vp, vp, C.c_int, C.c_float, i64, i64, vp, C.c_int, i64, vp,
+                                         vp, vp]),
+    "t8b_layer_norm_workspace": (C.c_size_t, [i64, i64]),
+    "t8b_layer_norm_backward": (C.c_int, [vp, C.c_int, i64, vp, C.c_int, i64, vp, C.c_int, vp, vp, vp, i64, i64, i64,
+                                          vp, i64, vp, vp, vp, C.c_size_t, vp]),
+    "t8b_linear_workspace": (C.c_size_t, [i64, i64, i64, C.c_int]),
+    "t8b_linear_forward": (C.c_int, [C.c_int, vp, i64, vp, i64, vp, C.c_int, C.c_int, vp, i64, i64, i64, i64, vp,
+                                     C.c_int, i64, vp, i64, vp, C.c_size_t, vp]),
+    "t8b_linear_backward": (C.c_int, [C.c_int, vp, i64, vp, i64, vp, i64, vp, i64, C.c_int, C.c_int, i64, i64, i64, vp,
+                                      i64, vp, i64, vp, vp, C.c_size_t, vp]),
+    "t8b_gated_workspace": (C.c_size_t, [i64, i64, i64, C.c_int]),
+    "t8b_gated_forward": (C.c_int, [C.c_int, vp, i64, vp, i64, vp, C.c_int, C.c_int, i64, i64, i64, vp, i64, vp, i64,
+                                    vp, C.c_size_t, vp]),
+    "t8b_gated_backward": (C.c_int, [C.c_int, vp, i64, vp, i64, vp, i64, vp, i64, C.c_int, C.c_int, i64, i64, i64, vp,
+                                     i64, vp, i64, vp, vp, C.c_size_t, vp]),
+    "t8b_operators_status": (C.c_int, [vp]),
+})
