@@ -73,16 +73,50 @@ struct alignas(sizeof(T) * V) Pack {
 };
 
 // ------------------------------------------------------------------ activations
-// In fp32. Where z is infinite or NaN they give what the formula does: silu(-inf) and gelu(-inf)
-// are NaN (0 * inf), as z / (1 + exp(-z)) is.
-__device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.0f, 1.0f + __expf(-z)); }
-__device__ __forceinline__ float normal_cdf(float z) { return 0.5f * (1.0f + erff(z * 0.70710678118654752f)); }
+// In fp32, from the machine's 2^x and 1/x (each good to about 2^-22): exp(v) = 2^(v log2 e),
+//   sigmoid(z) = 1 / (1 + exp(-z)),
+//   tanh(z) = 1 - 2 / (1 + exp(2z)), and below |z| = 0.2, where that difference cancels, the
+//     series z - z^3/3 + 2 z^5/15 - 17 z^7/315 (its next term is below 2^-27 of z there),
+//   Phi(z) = (1 + erf(z / sqrt 2)) / 2 with erfc(x) = t (a1 + t (a2 + ... t a5)) exp(-x^2),
+//     t = 1 / (1 + p x), x >= 0: Abramowitz and Stegun, Handbook of Mathematical Functions,
+//     7.1.26 (good to 1.5e-7); the lower tail is that product itself, so it does not cancel.
+// Where z is infinite they give what the formulas do: silu(-inf) and gelu(-inf) are NaN (0 * inf).
+__device__ __forceinline__ float power_of_two(float v) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ float reciprocal(float v) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+constexpr float kLog2E = 1.4426950408889634f;
+__device__ __forceinline__ float sigmoid(float z) { return reciprocal(1.0f + power_of_two(-kLog2E * z)); }
+__device__ __forceinline__ float hyperbolic_tangent(float z) {
+    const float square = z * z;
+    const float near = z * fmaf(square, fmaf(square, fmaf(square, -17.0f / 315.0f, 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
+    const float far = fmaf(-2.0f, reciprocal(1.0f + power_of_two(2.0f * kLog2E * z)), 1.0f);
+    return fabsf(z) < 0.2f ? near : far;
+}
+// Phi(z), and exp(-z^2 / 2) on the way
+__device__ __forceinline__ float normal_cdf(float z, float& gauss) {
+    gauss = power_of_two(-0.5f * kLog2E * z * z);
+    const float t = reciprocal(fmaf(0.3275911f * 0.70710678118654752f, fabsf(z), 1.0f));
+    const float series =
+        t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+    const float tail = 0.5f * series * gauss;
+    return z > 0.0f ? 1.0f - tail : tail;
+}
 template <int ACT>
 __device__ __forceinline__ float activate(float z) {
     if (ACT == T8B_RELU) return z > 0.0f ? z : (z != z ? z : 0.0f);
-    if (ACT == T8B_GELU) return z * normal_cdf(z);
+    if (ACT == T8B_GELU) {
+        float gauss;
+        return z * normal_cdf(z, gauss);
+    }
     if (ACT == T8B_SILU) return z * sigmoid(z);
-    if (ACT == T8B_TANH) return tanhf(z);
+    if (ACT == T8B_TANH) return hyperbolic_tangent(z);
     return z;
 }
 // activate(z) and its derivative
@@ -92,16 +126,17 @@ __device__ __forceinline__ void activate_slope(float z, float& value, float& slo
         value = activate<T8B_RELU>(z);
         slope = z > 0.0f ? 1.0f : 0.0f;
     } else if (ACT == T8B_GELU) {
-        const float cdf = normal_cdf(z);
+        float gauss;
+        const float cdf = normal_cdf(z, gauss);
         value = z * cdf;
-        slope = cdf + z * 0.39894228040143268f * __expf(-0.5f * z * z);
+        slope = fmaf(0.39894228040143268f * z, gauss, cdf);
     } else if (ACT == T8B_SILU) {
         const float s = sigmoid(z);
         value = z * s;
-        slope = s * (1.0f + z * (1.0f - s));
+        slope = s * fmaf(z, 1.0f - s, 1.0f);
     } else if (ACT == T8B_TANH) {
-        value = tanhf(z);
-        slope = 1.0f - value * value;
+        value = hyperbolic_tangent(z);
+        slope = fmaf(-value, value, 1.0f);
     } else {
         value = z;
         slope = 1.0f;

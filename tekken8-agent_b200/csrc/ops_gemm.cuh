@@ -7,13 +7,15 @@
 // k-block where a single CTA's 128 x BN tile needs BN * 128 B of B: at BN = 256, 32 KB for 512
 // cycles of MMA against 48 KB.
 //
-// Warps of a CTA (320 threads, persistent over work items = tile x k split):
+// Warps of a CTA (576 threads, persistent over work items = tile x k split):
 //   warp 0     TMA producer: waits for its own empty[stage], loads its CTA's A and B parts; the
 //              bytes of both CTAs are counted by the first CTA's full[stage];
 //   warp 1     (first CTA) MMA issuer: commits each stage to empty[stage] of both CTAs, a finished
 //              accumulator to acc_full[buffer] of both;
-//   warps 2-9  epilogue: quarter = warp % 4 gives the 32 tensor-memory lanes (rows), half the
-//              columns; each arrives once at the first CTA's acc_empty[buffer].
+//   warps 2-17 epilogue: quarter = warp % 4 gives the 32 tensor-memory lanes (rows), group a
+//              quarter of the columns; each arrives once at the first CTA's acc_empty[buffer].
+//              An epilogue is a chain of latencies (tensor memory, special functions, staging,
+//              its store's reads), so 16 warps, and not 8, share a tile (see EpiGated).
 // Two accumulator buffers of BN columns let the epilogue of one tile overlap the MMAs of the next.
 // Operands are K-major (rows of K elements) or MN-major (K rows), see gemm.cuh.
 //
@@ -29,9 +31,9 @@
 namespace t8b {
 namespace op {
 
-constexpr int kGemmThreads = 320;
-constexpr int kEpiWarps = 8;
-constexpr int kStageTile = 4096;  // one staging tile of an epilogue warp: 32 rows of up to 128 bytes
+constexpr int kEpiWarps = 16;
+constexpr int kGemmThreads = 64 + 32 * kEpiWarps;
+constexpr int kStaging = 4096;  // an epilogue warp's staging: 32 rows of 128 bytes
 
 // ------------------------------------------------------------------ PTX of the pair form
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -132,39 +134,52 @@ struct Tiled {
     int tma;
 };
 
-// Sends a staging tile (rows row0.., columns col0.. of m) out. All lanes; the tile may be
-// restaged after free_tiles().
+// Sends a staging tile (rows row0.., columns col0.. of m) out, by TMA from one lane of the warp
+// that `issues`, else rows from r0 on in steps of `step`. The tile was written by this warp, or,
+// after a barrier, by the two of a pair; it may be written again after free_tiles() (TMA), or
+// after the callers have met (element by element).
+__device__ __forceinline__ void publish() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 template <typename T, int BYTES>
-__device__ __forceinline__ void send(const Tiled& m, unsigned char* tile, int row0, int col0, int lane) {
+__device__ __forceinline__ void send(const Tiled& m, unsigned char* tile, int row0, int col0, int lane, bool issues = true,
+                                     int r0 = 0, int step = 1) {
     if (m.tma) {
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) {
+        if (issues && lane == 0) {
             if (row0 < m.rows && col0 < m.columns) tc::tma_store(&m.map, tile, col0, row0);
             tc::bulk_commit();
         }
         return;
     }
-    __syncwarp();
     constexpr int W = BYTES / sizeof(T);
+    constexpr int kPer = 16 / sizeof(T);
     const int rows = min(32, m.rows - row0);
-    T* out = static_cast<T*>(m.data) + static_cast<int64_t>(row0) * m.stride + col0;
-    for (int r = 0; r < rows; ++r, out += m.stride) {
+    T* out = static_cast<T*>(m.data) + static_cast<int64_t>(row0 + r0) * m.stride + col0;
+    for (int r = r0; r < rows; r += step, out += step * m.stride) {
 #pragma unroll
         for (int c = lane; c < W; c += 32) {
-            constexpr int kPer = 16 / sizeof(T);
             if (col0 + c < m.columns) out[c] = reinterpret_cast<const T*>(piece<BYTES>(tile, r, c / kPer))[c % kPer];
         }
     }
     __syncwarp();
 }
-// This warp's staging tiles, all but the `pending` sent last, may be written again.
+// This lane's stores, all but the `pending` issued last, have read their staging tiles.
 template <int PENDING>
-__device__ __forceinline__ void free_tiles(int lane) {
+__device__ __forceinline__ void wait_sent(int lane) {
     if (lane == 0) {
         if (PENDING == 0) tc::bulk_wait_read(); else tc::bulk_wait_read_all_but_one();
     }
+}
+// The same for a warp that sends its own tiles: all its lanes may write them again.
+template <int PENDING>
+__device__ __forceinline__ void free_tiles(int lane) {
+    wait_sent<PENDING>(lane);
     __syncwarp();
+}
+// A warp's own tile, written by all lanes, goes out.
+template <typename T, int BYTES>
+__device__ __forceinline__ void send_own(const Tiled& m, unsigned char* tile, int row0, int col0, int lane) {
+    if (m.tma) publish();
+    __syncwarp();
+    send<T, BYTES>(m, tile, row0, col0, lane);
 }
 
 // Fetches a tile of m into a free staging tile; by TMA it arrives on `bar` (lane 0 waits).
@@ -178,38 +193,51 @@ __device__ __forceinline__ void fetch(const Tiled& m, unsigned char* tile, uint6
         return;
     }
     constexpr int W = BYTES / sizeof(T);
+    constexpr int kPer = 16 / sizeof(T);
     const int rows = min(32, m.rows - row0);
     const T* in = static_cast<const T*>(m.data) + static_cast<int64_t>(row0) * m.stride + col0;
     for (int r = 0; r < rows; ++r, in += m.stride) {
 #pragma unroll
         for (int c = lane; c < W; c += 32) {
-            constexpr int kPer = 16 / sizeof(T);
             if (col0 + c < m.columns) reinterpret_cast<T*>(piece<BYTES>(tile, r, c / kPer))[c % kPer] = in[c];
         }
     }
     __syncwarp();
 }
 
-// What an epilogue sees: one warp of a tile.
+// What an epilogue sees: one warp of a tile. The warps of groups 2j and 2j + 1 with the same
+// quarter are a pair; their stagings lie side by side.
 struct Warp {
     int row0;              // first of the warp's 32 rows
     int tn;                // the tile's index along the columns
-    int split, half, lane;
+    int split, group, lane, pair;
     uint32_t taddr;        // the warp's lanes of the tile's accumulator
-    unsigned char* tiles;  // two staging tiles of kStageTile bytes
-    float* vector;         // 64 floats for a bias
-    uint64_t* bars;        // two barriers, one for each staging tile
-    uint32_t phases;       // their parities, bits 0 and 1
-    uint32_t in_flight;    // fetches not waited for yet, bits 0 and 1
-    int turn;              // staging tiles sent so far
+    unsigned char* tiles;  // its staging, kStaging bytes
+    float* vector;         // 32 floats for a bias
+    uint64_t* bar;         // a fetch's arrival
+    uint32_t phase;        // its parity
+    bool in_flight;        // a fetch not waited for yet
+    int turn;              // tiles sent so far, where an epilogue alternates between two
     volatile int* abort;
 
-    // the fetch into staging tile i has arrived
-    __device__ __forceinline__ bool wait(int i, uint32_t limit = tc::kSpinLimit) {
-        const bool ok = tc::bar_wait(bars + i, (phases >> i) & 1u, abort, limit);
-        phases ^= 1u << i;
-        in_flight &= ~(1u << i);
+    // the fetch has arrived
+    __device__ __forceinline__ bool wait() {
+        const bool ok = tc::bar_wait(bar, phase, abort);
+        phase ^= 1u;
+        in_flight = false;
         return ok;
+    }
+    // the two warps of the pair meet (both always do: see the vote in k_gemm)
+    __device__ __forceinline__ void meet() const { asm volatile("bar.sync %0, 64;" ::"r"(1 + pair) : "memory"); }
+    // whether both say yes
+    __device__ __forceinline__ bool vote(bool yes) const {
+        uint32_t both;
+        asm volatile(
+            "{\n .reg .pred p, q;\n setp.ne.u32 q, %2, 0;\n bar.red.and.pred p, %1, 64, q;\n selp.u32 %0, 1, 0, p;\n}\n"
+            : "=r"(both)
+            : "r"(1 + pair), "r"(yes ? 1u : 0u)
+            : "memory");
+        return both != 0;
     }
 };
 
@@ -222,20 +250,59 @@ struct Shape {
     int* error;
 };
 
+// A CTA's (or pair's) work items, one in `step`, columns fastest, then rows, then parts of k. Each
+// item is the last one plus a fixed step in the mixed radix, so the one thread that issues the MMAs
+// does not divide between tiles.
+struct Walk {
+    int tiles_m, tiles_n, splits, k_blocks;
+    int dn, dm, ds;
+    int tn, tm, split, kb0, kb1;
+    __device__ __forceinline__ Walk(const Shape& s, int first, int step)
+        : tiles_m(s.tiles_m), tiles_n(s.tiles_n), splits(s.splits), k_blocks(s.k_blocks) {
+        dn = step % tiles_n;
+        dm = step / tiles_n % tiles_m;
+        ds = step / tiles_n / tiles_m;
+        tn = first % tiles_n;
+        tm = first / tiles_n % tiles_m;
+        split = first / tiles_n / tiles_m;
+        range();
+    }
+    __device__ __forceinline__ bool more() const { return split < splits; }
+    __device__ __forceinline__ void next() {
+        const int before = split;
+        tn += dn;
+        if (tn >= tiles_n) {
+            tn -= tiles_n;
+            ++tm;
+        }
+        tm += dm;
+        if (tm >= tiles_m) {
+            tm -= tiles_m;
+            ++split;
+        }
+        split += ds;
+        if (split != before) range();
+    }
+    __device__ __forceinline__ void range() {  // k_blocks * (splits + 1) fits 32 bits
+        kb0 = splits == 1 ? 0 : static_cast<int>(static_cast<uint32_t>(k_blocks) * split / splits);
+        kb1 = splits == 1 ? k_blocks : static_cast<int>(static_cast<uint32_t>(k_blocks) * (split + 1) / splits);
+    }
+};
+
 template <int CG, int BN>
 struct Plan {
     static constexpr int kABytes = tc::BM * tc::BK * 2;
     static constexpr int kBRows = BN / CG;
     static constexpr int kBBytes = kBRows * tc::BK * 2;
     static constexpr int kStageBytes = kABytes + kBBytes;
-    static constexpr int kEpiBytes = kEpiWarps * (2 * kStageTile + 256);
+    static constexpr int kEpiBytes = kEpiWarps * (kStaging + 128);
     static constexpr int kBarBytes = 384;
     static constexpr int kBudget = 232448 - kEpiBytes - kBarBytes;
     static constexpr int kStages = kBudget / kStageBytes > 8 ? 8 : kBudget / kStageBytes;
     static constexpr int kTmemCols = 2 * BN < 32 ? 32 : 2 * BN;
     static constexpr int kSmemBytes = kStages * kStageBytes + kEpiBytes + kBarBytes;
     static_assert(kStages >= 3, "at least three stages");
-    static_assert(kBarBytes >= (2 * kStages + 4 + 2 * kEpiWarps) * 8 + 8, "barriers");
+    static_assert(kBarBytes >= (2 * kStages + 4 + kEpiWarps) * 8 + 8, "barriers");
 };
 
 template <typename E, int CG, int BN, bool A_MN, bool B_MN, class Epi>
@@ -245,13 +312,13 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kGemmThreads, 1)
     using P = Plan<CG, BN>;
     extern __shared__ __align__(1024) unsigned char base[];
     unsigned char* epi_tiles = base + P::kStages * P::kStageBytes;
-    float* vectors = reinterpret_cast<float*>(epi_tiles + kEpiWarps * 2 * kStageTile);
+    float* vectors = reinterpret_cast<float*>(epi_tiles + kEpiWarps * kStaging);
     uint64_t* full = reinterpret_cast<uint64_t*>(epi_tiles + P::kEpiBytes);
     uint64_t* empty = full + P::kStages;
     uint64_t* acc_full = empty + P::kStages;
     uint64_t* acc_empty = acc_full + 2;
     uint64_t* fetched = acc_empty + 2;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(fetched + 2 * kEpiWarps);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(fetched + kEpiWarps);
     volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     if ((tc::smem_addr(base) & 1023u) != 0) {  // the swizzles count on it; every thread sees the same
@@ -269,7 +336,7 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kGemmThreads, 1)
             tc::bar_init(acc_full + i, 1);
             tc::bar_init(acc_empty + i, CG * kEpiWarps);
         }
-        for (int i = 0; i < 2 * kEpiWarps; ++i) tc::bar_init(fetched + i, 1);
+        for (int i = 0; i < kEpiWarps; ++i) tc::bar_init(fetched + i, 1);
         *abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -279,17 +346,7 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kGemmThreads, 1)
     if (CG == 2) cluster_arrive_wait();  // the peer's barriers are initialised
     tc::fence_after();
     const uint32_t tmem = *tmem_slot;
-    const int total = s.tiles_m * s.tiles_n * s.splits;
     const int first = blockIdx.x / CG, step = gridDim.x / CG;
-
-    auto decode = [&](int work, int& tm, int& tn, int& kb0, int& kb1, int& split) {
-        tn = work % s.tiles_n;
-        const int rest = work / s.tiles_n;
-        tm = rest % s.tiles_m;
-        split = rest / s.tiles_m;
-        kb0 = static_cast<int>(static_cast<long long>(s.k_blocks) * split / s.splits);
-        kb1 = static_cast<int>(static_cast<long long>(s.k_blocks) * (split + 1) / s.splits);
-    };
     auto stop = [&]() {
         *abort = 1;
         atomicExch(s.error, 1);
@@ -299,11 +356,9 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kGemmThreads, 1)
         if (lane == 0) {
             int stage = 0, started = 0;
             uint32_t phase = 0;
-            for (int work = first; work < total && !*abort; work += step) {
-                int tm, tn, kb0, kb1, split;
-                decode(work, tm, tn, kb0, kb1, split);
-                const int row = (tm * CG + rank) * tc::BM;
-                for (int kb = kb0; kb < kb1; ++kb) {
+            for (Walk t(s, first, step); t.more() && !*abort; t.next()) {
+                const int row = (t.tm * CG + rank) * tc::BM;
+                for (int kb = t.kb0; kb < t.kb1; ++kb) {
                     if (!tc::bar_wait(empty + stage, phase ^ 1u, abort)) {
                         stop();
                         break;
@@ -321,15 +376,15 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kGemmThreads, 1)
                     if (B_MN) {
 #pragma unroll
                         for (int j = 0; j < P::kBRows / 64; ++j) {
-                            load_tile<CG>(b + j * 8192, &map_b, bar, tn * BN + rank * P::kBRows + j * 64, kb * tc::BK);
+                            load_tile<CG>(b + j * 8192, &map_b, bar, t.tn * BN + rank * P::kBRows + j * 64, kb * tc::BK);
                         }
                     } else if (s.second == 0) {
-                        load_tile<CG>(b, &map_b, bar, kb * tc::BK, tn * BN + rank * P::kBRows);
+                        load_tile<CG>(b, &map_b, bar, kb * tc::BK, t.tn * BN + rank * P::kBRows);
                     } else if (CG == 2) {
-                        load_tile<CG>(b, &map_b, bar, kb * tc::BK, rank * s.second + tn * (BN / 2));
+                        load_tile<CG>(b, &map_b, bar, kb * tc::BK, rank * s.second + t.tn * (BN / 2));
                     } else {
-                        load_tile<CG>(b, &map_b, bar, kb * tc::BK, tn * (BN / 2));
-                        load_tile<CG>(b + P::kBBytes / 2, &map_b, bar, kb * tc::BK, s.second + tn * (BN / 2));
+                        load_tile<CG>(b, &map_b, bar, kb * tc::BK, t.tn * (BN / 2));
+                        load_tile<CG>(b + P::kBBytes / 2, &map_b, bar, kb * tc::BK, s.second + t.tn * (BN / 2));
                     }
                     if (started < P::kStages) ++started;
                     if (++stage == P::kStages) {
@@ -354,9 +409,7 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kGemmThreads, 1)
             constexpr uint32_t idesc = instruction<E>(tc::BM * CG, BN, A_MN, B_MN);
             int stage = 0, acc = 0;
             uint32_t phase = 0, acc_phase = 0;
-            for (int work = first; work < total && !*abort; work += step) {
-                int tm, tn, kb0, kb1, split;
-                decode(work, tm, tn, kb0, kb1, split);
+            for (Walk t(s, first, step); t.more() && !*abort; t.next()) {
                 if (!tc::bar_wait(acc_empty + acc, acc_phase ^ 1u, abort)) {
                     stop();
                     break;
@@ -364,7 +417,7 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kGemmThreads, 1)
                 tc::fence_after();
                 const uint32_t d = tmem + static_cast<uint32_t>(acc * BN);
                 bool ok = true;
-                for (int kb = kb0; kb < kb1; ++kb) {
+                for (int kb = t.kb0; kb < t.kb1; ++kb) {
                     if (!tc::bar_wait(full + stage, phase, abort)) {
                         stop();
                         ok = false;
@@ -377,7 +430,7 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kGemmThreads, 1)
                     for (int k = 0; k < tc::BK / 16; ++k) {
                         const uint64_t da = A_MN ? tc::sw128_desc(a + k * 2048, 8192, 1024) : tc::sw128_desc(a + k * 32, 16, 1024);
                         const uint64_t db = B_MN ? tc::sw128_desc(b + k * 2048, 8192, 1024) : tc::sw128_desc(b + k * 32, 16, 1024);
-                        mma<CG>(d, da, db, idesc, (kb > kb0 || k > 0) ? 1u : 0u);
+                        mma<CG>(d, da, db, idesc, (kb > t.kb0 || k > 0) ? 1u : 0u);
                     }
                     commit<CG>(empty + stage);
                     if (++stage == P::kStages) {
@@ -396,34 +449,35 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kGemmThreads, 1)
     } else {
         const int e = warp - 2, quarter = warp & 3;
         Warp w;
-        w.half = e >> 2;
+        w.group = e >> 2;
         w.lane = lane;
-        w.tiles = epi_tiles + e * 2 * kStageTile;
-        w.vector = vectors + e * 64;
-        w.bars = fetched + 2 * e;
-        w.phases = 0;
-        w.in_flight = 0;
+        w.pair = quarter * 2 + (w.group >> 1);
+        w.tiles = epi_tiles + (w.pair * 2 + (w.group & 1)) * kStaging;
+        w.vector = vectors + e * 32;
+        w.bar = fetched + e;
+        w.phase = 0;
+        w.in_flight = false;
         w.turn = 0;
         w.abort = abort;
         int acc = 0;
         uint32_t acc_phase = 0;
-        for (int work = first; work < total && !*abort; work += step) {
-            int tm, tn, kb0, kb1, split;
-            decode(work, tm, tn, kb0, kb1, split);
-            w.row0 = (tm * CG + rank) * tc::BM + quarter * 32;
-            w.tn = tn;
-            w.split = split;
+        bool good = true;
+        for (Walk t(s, first, step); t.more(); t.next()) {
+            w.row0 = (t.tm * CG + rank) * tc::BM + quarter * 32;
+            w.tn = t.tn;
+            w.split = t.split;
             w.taddr = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * BN);
-            epi.begin(w);
-            if (!tc::bar_wait(acc_full + acc, acc_phase, abort)) {
+            bool ok = good && !*abort;
+            if (ok) {
+                epi.begin(w);
+                ok = tc::bar_wait(acc_full + acc, acc_phase, abort);
+            }
+            if (!w.vote(ok)) {  // the warps of a pair go on, or stop, together
                 stop();
                 break;
             }
             tc::fence_after();
-            if (!epi.finish(w)) {
-                stop();
-                break;
-            }
+            good = epi.finish(w);
             tc::fence_before();
             __syncwarp();
             if (lane == 0) {
@@ -439,9 +493,8 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kGemmThreads, 1)
                 acc_phase ^= 1u;
             }
         }
-        for (int i = 0; i < 2; ++i) {  // after a stall a fetch may still be in flight
-            for (uint32_t n = 0; ((w.in_flight >> i) & 1u) && n < kDrainLimit && !tc::bar_try(w.bars + i, (w.phases >> i) & 1u); ++n) {
-            }
+        if (!good) stop();
+        for (uint32_t n = 0; w.in_flight && n < kDrainLimit && !tc::bar_try(w.bar, w.phase); ++n) {  // after a stall
         }
         if (lane == 0) tc::bulk_wait();  // this warp's stores have landed
         __syncwarp();

@@ -177,140 +177,147 @@ __device__ __forceinline__ void add_bias32(float* vector, float mine, int lane, 
 }
 
 // y = activation(acc + bias) + residual in the type O, and acc + bias as `pre`; without FULL, acc
-// alone (gradients, and the fp32 parts of a split GEMM). A half of the epilogue warps takes half
-// of the tile's columns, in chunks of a 128-byte row (64 bytes where half a tile is narrower).
+// alone (gradients, and the fp32 parts of a split GEMM). A group of epilogue warps takes a quarter
+// of the tile's columns (at least one chunk) in chunks of a 128-byte row (64 where a tile of 64
+// columns has no more): stores of 64-byte rows took 158 us where 128-byte rows take 130 (75,776 x 128
+// times 2,816 x 128, where stores are most of the work). A chunk's residual is fetched into
+// the staging tile while the MMAs run; y replaces it, then `pre`, read again from tensor memory.
 template <typename E, typename O, int BN, bool FULL>
 struct EpiLinear {
-    static constexpr int kWide = sizeof(O) == 4 || BN < 128 ? 32 : 64;  // columns of a chunk
+    static constexpr int kWide = sizeof(O) == 2 && BN >= 128 ? 64 : 32;  // columns of a chunk
     static constexpr int kBytes = kWide * sizeof(O);
     static constexpr int kPreBytes = kWide * 2;
-    static constexpr int kChunks = BN / 2 / kWide;
+    static constexpr int kColumns = BN / 4 < kWide ? kWide : BN / 4;  // of a group
+    static constexpr int kChunks = kColumns / kWide;
     Tiled y, residual, pre;
     const void* bias;
     int bias_type, activation, has_residual, has_pre, split_rows;
 
-    __device__ __forceinline__ int column(const Warp& w, int chunk) const { return w.tn * BN + w.half * (BN / 2) + chunk * kWide; }
-    // y's staging tile, `ahead` chunks from the next one sent: the two in turn, or the second where
-    // the first holds `pre`
-    __device__ __forceinline__ int tile_of(const Warp& w, int ahead) const { return FULL && has_pre ? 1 : (w.turn + ahead) & 1; }
-    __device__ __forceinline__ void fetch_chunk(Warp& w, int chunk, int ahead) const {
-        const int col = column(w, chunk), i = tile_of(w, ahead);
+    __device__ __forceinline__ int column(const Warp& w, int chunk) const { return w.tn * BN + w.group * kColumns + chunk * kWide; }
+    __device__ __forceinline__ bool idle(const Warp& w) const { return w.row0 >= y.rows || w.group * kColumns >= BN; }
+    __device__ __forceinline__ void fetch_chunk(Warp& w, int chunk) const {
+        const int col = column(w, chunk);
         if (chunk >= kChunks || col >= y.columns) return;
-        fetch<O, kBytes>(residual, w.tiles + i * kStageTile, w.bars + i, w.row0, col, w.lane);
-        if (residual.tma) w.in_flight |= 1u << i;
+        free_tiles<0>(w.lane);
+        fetch<O, kBytes>(residual, w.tiles, w.bar, w.row0, col, w.lane);
+        w.in_flight = residual.tma;
     }
     __device__ __forceinline__ void begin(Warp& w) const {
-        if (!FULL || !has_residual || w.row0 >= y.rows) return;
-        free_tiles<0>(w.lane);
-        fetch_chunk(w, 0, 0);
-        if (!has_pre) fetch_chunk(w, 1, 1);
+        if (FULL && has_residual && !idle(w)) fetch_chunk(w, 0);
+    }
+    // 32 columns of acc + bias
+    __device__ __forceinline__ void load(const Warp& w, int chunk, int at, float (&v)[32]) const {
+        float b = 0.0f;
+        if (FULL) b = bias_at(bias, bias_type, column(w, chunk) + at + w.lane, y.columns);
+        tc::tmem_load32(w.taddr + w.group * kColumns + chunk * kWide + at, v);
+        if (FULL && bias != nullptr) add_bias32(w.vector, b, w.lane, v);
     }
     __device__ __forceinline__ bool finish(Warp& w) const {
-        if (w.row0 >= y.rows) return true;
+        if (idle(w)) return true;
         const int row0 = w.row0 + w.split * split_rows;
 #pragma unroll 1
         for (int chunk = 0; chunk < kChunks; ++chunk) {
-            const int col = column(w, chunk), i = tile_of(w, 0);
+            const int col = column(w, chunk);
             if (col >= y.columns) break;
-            unsigned char* tile = w.tiles + i * kStageTile;
             if (FULL && has_residual) {
-                if (residual.tma && !w.wait(i)) return false;
-            } else if (FULL && has_pre) {
-                free_tiles<0>(w.lane);
+                if (residual.tma && !w.wait()) return false;
             } else {
-                free_tiles<1>(w.lane);
+                free_tiles<0>(w.lane);
             }
-#pragma unroll 1
+#pragma unroll
             for (int at = 0; at < kWide; at += 32) {
                 float v[32];
-                float b = 0.0f;
-                if (FULL) b = bias_at(bias, bias_type, col + at + w.lane, y.columns);
-                tc::tmem_load32(w.taddr + w.half * (BN / 2) + chunk * kWide + at, v);
+                load(w, chunk, at, v);
                 if (FULL) {
-                    if (bias != nullptr) add_bias32(w.vector, b, w.lane, v);
-                    if (has_pre) stage32<E, kPreBytes>(w.tiles, w.lane, at, v);
                     with_activation(activation, [&](auto act) {
 #pragma unroll
                         for (int k = 0; k < 32; ++k) v[k] = activate<decltype(act)::value>(v[k]);
                     });
-                    if (has_residual) add32<O, kBytes>(tile, w.lane, at, v);
+                    if (has_residual) add32<O, kBytes>(w.tiles, w.lane, at, v);
                 }
-                stage32<O, kBytes>(tile, w.lane, at, v);
+                stage32<O, kBytes>(w.tiles, w.lane, at, v);
             }
-            if (FULL && has_pre) send<E, kPreBytes>(pre, w.tiles, row0, col, w.lane);
-            send<O, kBytes>(y, tile, row0, col, w.lane);
-            ++w.turn;
-            if (FULL && has_residual) {  // into the tile just sent
-                const int next = chunk + (has_pre ? 1 : 2);
-                if (next < kChunks) {
-                    free_tiles<0>(w.lane);
-                    fetch_chunk(w, next, 1);
+            send_own<O, kBytes>(y, w.tiles, row0, col, w.lane);
+            if (FULL && has_pre) {
+                free_tiles<0>(w.lane);
+#pragma unroll 1
+                for (int at = 0; at < kWide; at += 32) {
+                    float v[32];
+                    load(w, chunk, at, v);
+                    stage32<E, kPreBytes>(w.tiles, w.lane, at, v);
                 }
+                send_own<E, kPreBytes>(pre, w.tiles, row0, col, w.lane);
             }
+            if (FULL && has_residual) fetch_chunk(w, chunk + 1);
         }
         return true;
     }
 };
 
 // h = activation(gate) up; the accumulator's first BN / 2 columns are the gate's, the others the
-// up projection's of the same columns of h.
+// up projection's of the same columns of h. A warp takes 32 columns of h; the two of a pair stage
+// theirs side by side in tiles of 64 columns (128-byte rows, see EpiLinear), of which the pair has
+// two: gate and up go out through one each, h through the gate's once its store has read it.
 template <typename E, int BN>
 struct EpiGated {
     static constexpr int kHalf = BN / 2;
-    static constexpr int kWide = BN == 256 ? 64 : 32;
-    static constexpr int kBytes = kWide * 2;
+    static constexpr bool kPaired = kHalf >= 64;
+    static constexpr int kBytes = kPaired ? 128 : 64;
     Tiled h, gate, up;
     const void* bias;
     int bias_type, activation, has_pre;
 
+    __device__ __forceinline__ void meet(const Warp& w) const {
+        if (kPaired) w.meet(); else __syncwarp();
+    }
+    __device__ __forceinline__ void put(const Tiled& m, const Warp& w, unsigned char* tile, int col, bool issues, const float (&v)[32]) const {
+        stage32<E, kBytes>(tile, w.lane, kPaired ? (w.group & 1) * 32 : 0, v);
+        if (m.tma) publish();
+        meet(w);
+        send<E, kBytes>(m, tile, w.row0, col, w.lane, issues, kPaired ? w.group & 1 : 0, kPaired ? 2 : 1);
+        if (!m.tma) meet(w);
+    }
     __device__ __forceinline__ void begin(Warp&) const {}
     __device__ __forceinline__ bool finish(Warp& w) const {
-        const int first = w.half * kWide, col = w.tn * kHalf + first;
-        if (w.row0 >= h.rows || first >= kHalf || col >= h.columns) return true;
-        uint32_t packed[kWide / 2];
-        if (has_pre) free_tiles<0>(w.lane);
-#pragma unroll
-        for (int at = 0; at < kWide; at += 32) {
-            float g[32], u[32];
-            const int c = col + at + w.lane;
-            float bg = 0.0f, bu = 0.0f;
-            if (bias != nullptr && c < h.columns) {
-                bg = load_any(bias, bias_type, c);
-                bu = load_any(bias, bias_type, h.columns + c);
-            }
-            tc::tmem_load32(w.taddr + first + at, g);
-            tc::tmem_load32(w.taddr + kHalf + first + at, u);
-            if (bias != nullptr) {
-                add_bias32(w.vector, bg, w.lane, g);
-                add_bias32(w.vector + 32, bu, w.lane, u);
-            }
-            if (has_pre) {
-                stage32<E, kBytes>(w.tiles, w.lane, at, g);
-                stage32<E, kBytes>(w.tiles + kStageTile, w.lane, at, u);
-            }
-            with_activation(activation, [&](auto act) {
-#pragma unroll
-                for (int k = 0; k < 16; ++k) {
-                    packed[at / 2 + k] = Element<E>::pack(activate<decltype(act)::value>(g[2 * k]) * u[2 * k],
-                                                          activate<decltype(act)::value>(g[2 * k + 1]) * u[2 * k + 1]);
-                }
-            });
+        const int first = w.group * 32;                                                // this warp's columns of the tile
+        const int together = kPaired ? (w.group >> 1) * 64 : first;                    // and the pair's
+        const int col = w.tn * kHalf + together, mine = w.tn * kHalf + first + w.lane;
+        if (w.row0 >= h.rows || together >= kHalf || col >= h.columns) return true;    // the same for both of a pair
+        const bool issues = !kPaired || (w.group & 1) == 0;
+        unsigned char* tile = w.tiles - (kPaired && !issues ? kStaging : 0);
+        unsigned char* other = tile + (kPaired ? kStaging : kStaging / 2);
+        float g[32], u[32];
+        float bg = 0.0f, bu = 0.0f;
+        if (bias != nullptr && mine < h.columns) {
+            bg = load_any(bias, bias_type, mine);
+            bu = load_any(bias, bias_type, h.columns + mine);
         }
-        unsigned char* tile = w.tiles;
+        tc::tmem_load32(w.taddr + first, g);
+        if (bias != nullptr) add_bias32(w.vector, bg, w.lane, g);
         if (has_pre) {
-            send<E, kBytes>(gate, w.tiles, w.row0, col, w.lane);
-            send<E, kBytes>(up, w.tiles + kStageTile, w.row0, col, w.lane);
-            if (up.tma) free_tiles<1>(w.lane); else free_tiles<0>(w.lane);  // the gate's tile
+            if (issues) wait_sent<0>(w.lane);
+            meet(w);
+            put(gate, w, tile, col, issues, g);
+        }
+        with_activation(activation, [&](auto act) {
+#pragma unroll
+            for (int k = 0; k < 32; ++k) g[k] = activate<decltype(act)::value>(g[k]);
+        });
+        tc::tmem_load32(w.taddr + kHalf + first, u);
+        if (bias != nullptr) add_bias32(w.vector, bu, w.lane, u);
+        if (has_pre) {
+            put(up, w, other, col, issues, u);
+            if (issues) {
+                if (up.tma) wait_sent<1>(w.lane); else wait_sent<0>(w.lane);  // the gate's tile
+            }
         } else {
-            tile += (w.turn++ & 1) * kStageTile;
-            free_tiles<1>(w.lane);
+            if ((w.turn++ & 1) != 0) tile = other;
+            if (issues) wait_sent<1>(w.lane);  // the tile sent before last
         }
 #pragma unroll
-        for (int q = 0; q < kWide / 8; ++q) {
-            *reinterpret_cast<uint4*>(piece<kBytes>(tile, w.lane, q)) =
-                make_uint4(packed[4 * q], packed[4 * q + 1], packed[4 * q + 2], packed[4 * q + 3]);
-        }
-        send<E, kBytes>(h, tile, w.row0, col, w.lane);
+        for (int k = 0; k < 32; ++k) g[k] *= u[k];
+        meet(w);
+        put(h, w, tile, col, issues, g);
         return true;
     }
 };
