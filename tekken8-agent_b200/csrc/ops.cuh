@@ -72,6 +72,38 @@ struct alignas(sizeof(T) * V) Pack {
     T v[V];
 };
 
+// Two fp32 values in a register pair, and the machine's packed operations on them: one instruction
+// for both, each rounded as its scalar form.
+struct Two {
+    unsigned long long bits;
+    __device__ __forceinline__ Two() : bits(0) {}
+    __device__ __forceinline__ Two(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(bits) : "f"(a), "f"(b)); }
+    __device__ __forceinline__ float2 get() const {
+        float2 v;
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(bits));
+        return v;
+    }
+    __device__ __forceinline__ float sum() const {
+        const float2 v = get();
+        return v.x + v.y;
+    }
+};
+__device__ __forceinline__ Two operator+(const Two& a, const Two& b) {
+    Two r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits));
+    return r;
+}
+__device__ __forceinline__ Two operator*(const Two& a, const Two& b) {
+    Two r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits));
+    return r;
+}
+__device__ __forceinline__ Two multiply_add(const Two& a, const Two& b, const Two& c) {
+    Two r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits), "l"(c.bits));
+    return r;
+}
+
 // ------------------------------------------------------------------ activations
 // In fp32, from the machine's 2^x and 1/x (each good to about 2^-22): exp(v) = 2^(v log2 e),
 //   sigmoid(z) = 1 / (1 + exp(-z)),

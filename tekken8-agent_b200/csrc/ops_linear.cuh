@@ -342,8 +342,13 @@ __global__ void k_pack(const E* in, int64_t stride, int64_t rows, int columns, E
 
 // The elementwise half of a backward pass: dz (rows of `pitch` elements) from dy and pre, and this
 // block row's column sums of dz in fp32, before dz is rounded. A thread holds V columns over its
-// rows; block (32, kGradRows).
+// rows, and reads the next rows while it works on these; block (32, kGradRows).
 //   linear: dz = dy activation'(pre);  gated: dz = [dy up activation'(gate) | dy activation(gate)]
+// Bound by memory: it reads dy and pre and writes dz once.
+template <typename E, int V>
+struct GradRow {
+    Pack<E, V> d, z, u;
+};
 template <typename E, bool GATED, int V>
 __global__ void __launch_bounds__(32 * kGradRows)
     k_activation_grad(const E* dy, int64_t dy_stride, const E* pre, int64_t pre_stride, int64_t rows, int columns,
@@ -358,35 +363,55 @@ __global__ void __launch_bounds__(32 * kGradRows)
 #pragma unroll
         for (int j = 0; j < V; ++j) sum[p][j] = 0.0f;
     }
-    with_activation(activation, [&](auto act) {
-        constexpr int ACT = decltype(act)::value;
-        for (int64_t row = static_cast<int64_t>(blockIdx.y) * kGradRows + threadIdx.y; in && row < rows;
-             row += static_cast<int64_t>(gridDim.y) * kGradRows) {
-            const Pack<E, V> d = *reinterpret_cast<const Pack<E, V>*>(dy + row * dy_stride + c);
-            Pack<E, V> z{}, u{}, out{};
-            if (GATED || ACT != T8B_LINEAR) z = *reinterpret_cast<const Pack<E, V>*>(pre + row * pre_stride + c);
-            if (GATED) u = *reinterpret_cast<const Pack<E, V>*>(pre + row * pre_stride + columns + c);
-            float value[V], slope[V];
-#pragma unroll
-            for (int j = 0; j < V; ++j) activate_slope<ACT>(Element<E>::load(z.v[j]), value[j], slope[j]);
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const float of_z = Element<E>::load(d.v[j]) * slope[j] * (GATED ? Element<E>::load(u.v[j]) : 1.0f);
-                sum[0][j] += of_z;
-                out.v[j] = Element<E>::store(of_z);
-            }
-            if (dz) *reinterpret_cast<Pack<E, V>*>(dz + row * pitch + c) = out;
-            if (GATED) {
+    if (in) {
+        with_activation(activation, [&](auto act) {
+            constexpr int ACT = decltype(act)::value;
+            const int64_t first = static_cast<int64_t>(blockIdx.y) * kGradRows + threadIdx.y;
+            const int64_t step = static_cast<int64_t>(gridDim.y) * kGradRows;
+            const E* from_dy = dy + first * dy_stride + c;
+            const E* from_pre = GATED || ACT != T8B_LINEAR ? pre + first * pre_stride + c : nullptr;
+            E* to = dz ? dz + first * pitch + c : nullptr;
+            auto read = [&](GradRow<E, V>& r) {
+                r.d = *reinterpret_cast<const Pack<E, V>*>(from_dy);
+                if (GATED || ACT != T8B_LINEAR) r.z = *reinterpret_cast<const Pack<E, V>*>(from_pre);
+                if (GATED) r.u = *reinterpret_cast<const Pack<E, V>*>(from_pre + columns);
+                from_dy += step * dy_stride;
+                if (GATED || ACT != T8B_LINEAR) from_pre += step * pre_stride;
+            };
+            auto use = [&](const GradRow<E, V>& r) {
+                Pack<E, V> out, out_up;
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
-                    const float of_u = Element<E>::load(d.v[j]) * value[j];
-                    sum[PARTS - 1][j] += of_u;
-                    out.v[j] = Element<E>::store(of_u);
+                    float value, slope;
+                    const float d = Element<E>::load(r.d.v[j]);
+                    activate_slope<ACT>(GATED || ACT != T8B_LINEAR ? Element<E>::load(r.z.v[j]) : 0.0f, value, slope);
+                    const float of_z = d * slope * (GATED ? Element<E>::load(r.u.v[j]) : 1.0f);
+                    sum[0][j] += of_z;
+                    out.v[j] = Element<E>::store(of_z);
+                    if (GATED) {
+                        const float of_u = d * value;
+                        sum[PARTS - 1][j] += of_u;
+                        out_up.v[j] = Element<E>::store(of_u);
+                    }
                 }
-                if (dz) *reinterpret_cast<Pack<E, V>*>(dz + row * pitch + columns + c) = out;
+                if (to) {
+                    *reinterpret_cast<Pack<E, V>*>(to) = out;
+                    if (GATED) *reinterpret_cast<Pack<E, V>*>(to + columns) = out_up;
+                    to += step * pitch;
+                }
+            };
+            GradRow<E, V> a, b;
+            int64_t row = first;
+            if (row < rows) read(a);
+            for (; row < rows; row += 2 * step) {
+                const bool second = row + step < rows;
+                if (second) read(b);
+                use(a);
+                if (row + 2 * step < rows) read(a);
+                if (second) use(b);
             }
-        }
-    });
+        });
+    }
     if (sums == nullptr) return;
 #pragma unroll
     for (int p = 0; p < PARTS; ++p) {

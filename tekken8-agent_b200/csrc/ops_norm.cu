@@ -4,9 +4,9 @@
 //   dx = rstd (g - sum(g)/n - xhat sum(g xhat)/n) + residual gradient,   g = dy w,  xhat = (x - mean) rstd
 //   dw = sum over rows of dy xhat,   db = sum over rows of dy
 //
-// Bound by memory: a pass reads x (and dy) once and writes y (or dx) once. A row of up to 512
-// elements belongs to one warp and lies in its registers, 16 elements a lane; a longer one (to
-// 8,192) to one block, 16 elements a thread. The statistics are two passes over those registers
+// Bound by memory: a pass reads x (and dy) once and writes y (or dx) once. A row of up to 128, 256
+// or 512 elements belongs to 8, 16 or 32 lanes of a warp and lies in their registers, 16 elements a
+// lane; a longer one (to 8,192) to one block, 16 elements a thread. The statistics are two passes over those registers
 // (the mean, then the squares of the differences), so no row is read twice and no variance is a
 // difference of large sums. The grid is persistent: a lane keeps its columns' parameters, and in
 // the backward pass its columns' sums of dw and db, in registers over all the rows its warp takes;
@@ -24,6 +24,11 @@ constexpr int kHeld = 16;        // elements of a row that one thread holds
 constexpr int kWarps = 8;        // warps (rows in flight) of a block in the warp form
 constexpr int kBlockMax = 512;   // threads of a block in the block form
 constexpr int kPartialRows = 16; // rows of threads in k_norm_parameters
+// Resident blocks of the warp form: as many as its registers allow (a lane holds w, b and the next
+// row forward; w, dw, db and a row of each input backward).
+constexpr int kForwardBlocks = 2, kBackwardBlocks = 2;
+// Threads that share a row of n elements, 16 a thread: 8, 16 or 32 lanes, or a block of them.
+constexpr int group_of(int64_t n) { return n <= 8 * kHeld ? 8 : n <= 16 * kHeld ? 16 : n <= 32 * kHeld ? 32 : 0; }
 
 struct Norm {
     const void* x;
@@ -40,16 +45,16 @@ struct Norm {
     float epsilon;
 };
 
-// Sums a (and b) over the row's threads: a warp, or the block with one barrier (shared values
-// alternate between two buffers, so the barrier of the next sum protects those of this one).
-template <bool WARP, int COUNT>
+// Sums over the row's threads: G lanes of a warp, or (G = 0) the block with one barrier (shared
+// values alternate between two buffers, so the barrier of the next sum protects those of this one).
+template <int G, int COUNT>
 __device__ __forceinline__ void row_sum(float (&v)[COUNT], float (*shared)[kBlockMax / 32][2], int& turn) {
 #pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) {
+    for (int o = (G ? G : 32) / 2; o >= 1; o >>= 1) {
 #pragma unroll
         for (int k = 0; k < COUNT; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
     }
-    if (WARP) return;
+    if (G) return;
     const int warps = blockDim.x >> 5;
     auto& buffer = shared[turn];
     turn ^= 1;
@@ -59,146 +64,354 @@ __device__ __forceinline__ void row_sum(float (&v)[COUNT], float (*shared)[kBloc
     }
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < COUNT; ++k) {
-        float sum = 0.0f;
-        for (int w = 0; w < warps; ++w) sum += buffer[w][k];
-        v[k] = sum;
+    for (int k = 0; k < COUNT; ++k) v[k] = 0.0f;
+    for (int w = 0; w < warps; ++w) {
+        const float2 one = *reinterpret_cast<const float2*>(buffer[w]);
+        v[0] += one.x;
+        if (COUNT == 2) v[COUNT - 1] += one.y;
     }
 }
 
-// Thread t of a row's G threads holds elements (i G + t) V + j, i < NV, j < V.
+// Thread t of a row's G threads holds elements (i G + t) V + j, i < NV, j < V; those beyond the row
+// are 0. Rows come through a ring of stages in shared memory that a thread fills (cp.async, the
+// same 16 or 8 bytes that it will read) and reads alone, so the ring needs no barrier and a warp has
+// its next rows in flight while it works on one (262,144 x 512 in bf16: backward 205 us against 297
+// without it, forward 88 against 123). Single elements are read when they are used: 4-byte copies
+// take as many instructions as the elements (65,536 x 151 in fp32, backward: 55 us against 37).
 template <typename T, int V, int NV>
-__device__ __forceinline__ void load_row(const T* row, int t, int group, int n, float (&v)[NV * V]) {
+struct Rows {
+    static constexpr int kPack = V * sizeof(T);
+    static constexpr bool kRing = V > 1;
+    static constexpr int kBytes = kRing ? NV * kPack : 0;  // of a thread and a stage
+    const T* from;  // this thread's first element of the next row to fetch (or, without a ring, to get)
+    int64_t step;   // elements to the row after it
+    int first, apart, n;  // its first column, and columns to its next pack
+
+    __device__ __forceinline__ Rows(const void* base, int64_t stride, int64_t row, int64_t rows_apart, int t, int group, int columns)
+        : from(static_cast<const T*>(base) + row * stride + t * V), step(rows_apart * stride), first(t * V), apart(group * V), n(columns) {}
+    // slot: this thread's first pack in a stage, consecutive packs `pitch` bytes apart
+    __device__ __forceinline__ void fetch(uint32_t slot, int pitch) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int c = (i * group + t) * V;
-        Pack<T, V> p;
-        const bool in = c < n;
-        if (in) p = *reinterpret_cast<const Pack<T, V>*>(row + c);
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[i * V + j] = in ? Element<T>::load(p.v[j]) : 0.0f;
+        for (int i = 0; i < NV; ++i) {
+            if (first + i * apart < n) {
+                if constexpr (kPack == 16) {
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slot + i * pitch), "l"(from + i * apart) : "memory");
+                } else if constexpr (kRing) {
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(slot + i * pitch), "l"(from + i * apart) : "memory");
+                }
+            }
+        }
+        from += step;
     }
+    __device__ __forceinline__ void get(const unsigned char* slot, int pitch, Two (&v)[NV * V / 2]) {
+        if constexpr (kRing) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const bool in = first + i * apart < n;
+                if constexpr (sizeof(T) == 2) {
+                    Pack<uint32_t, V / 2> p;
+                    if (in) p = *reinterpret_cast<const Pack<uint32_t, V / 2>*>(slot + i * pitch);
+#pragma unroll
+                    for (int j = 0; j < V / 2; ++j) {
+                        const float2 f = Element<T>::unpack(in ? p.v[j] : 0u);
+                        v[i * (V / 2) + j] = Two(f.x, f.y);
+                    }
+                } else {
+                    Pack<float, V> p;
+                    if (in) p = *reinterpret_cast<const Pack<float, V>*>(slot + i * pitch);
+#pragma unroll
+                    for (int j = 0; j < V / 2; ++j) v[i * (V / 2) + j] = Two(in ? p.v[2 * j] : 0.0f, in ? p.v[2 * j + 1] : 0.0f);
+                }
+            }
+        } else {
+            float f[NV];
+#pragma unroll
+            for (int i = 0; i < NV; ++i) f[i] = first + i * apart < n ? Element<T>::load(from[i * apart]) : 0.0f;
+#pragma unroll
+            for (int i = 0; i < NV / 2; ++i) v[i] = Two(f[2 * i], f[2 * i + 1]);
+            from += step;
+        }
+    }
+};
+__device__ __forceinline__ void ring_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int PENDING>
+__device__ __forceinline__ void ring_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory");
 }
+// Stages of a ring of `bytes` a thread and a stage: two blocks of 256 threads fit an SM, and more
+// than two rows ahead gained nothing (262,144 x 512 forward in bf16: 88 us, with three 99).
+constexpr int ring_stages(int bytes) { return bytes == 0 || 384 / bytes < 3 ? 2 : 3; }
+
+// to: this thread's first element of the row
 template <typename T, int V, int NV>
-__device__ __forceinline__ void store_row(T* row, int t, int group, int n, const float (&v)[NV * V]) {
+__device__ __forceinline__ void store_row(T* to, int first, int apart, int n, const Two (&v)[NV * V / 2]) {
+    if constexpr (V == 1) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int c = (i * group + t) * V;
-        if (c < n) {
-            Pack<T, V> p;
+        for (int i = 0; i < NV; ++i) {
+            const float2 f = v[i / 2].get();
+            if (first + i * apart < n) to[i * apart] = Element<T>::store(i % 2 ? f.y : f.x);
+        }
+    } else {
 #pragma unroll
-            for (int j = 0; j < V; ++j) p.v[j] = Element<T>::store(v[i * V + j]);
-            *reinterpret_cast<Pack<T, V>*>(row + c) = p;
+        for (int i = 0; i < NV; ++i) {
+            if (first + i * apart >= n) continue;
+            if constexpr (sizeof(T) == 2) {
+                Pack<uint32_t, V / 2> p;
+#pragma unroll
+                for (int j = 0; j < V / 2; ++j) {
+                    const float2 f = v[i * (V / 2) + j].get();
+                    p.v[j] = Element<T>::pack(f.x, f.y);
+                }
+                *reinterpret_cast<Pack<uint32_t, V / 2>*>(to + i * apart) = p;
+            } else {
+                Pack<float, V> p;
+#pragma unroll
+                for (int j = 0; j < V / 2; ++j) {
+                    const float2 f = v[i * (V / 2) + j].get();
+                    p.v[2 * j] = f.x;
+                    p.v[2 * j + 1] = f.y;
+                }
+                *reinterpret_cast<Pack<float, V>*>(to + i * apart) = p;
+            }
         }
     }
 }
 template <int V, int NV>
 __device__ __forceinline__ void load_parameter(const void* p, int type, float missing, int t, int group, int n,
-                                               float (&v)[NV * V]) {
+                                               Two (&v)[NV * V / 2]) {
+    float f[NV * V];
 #pragma unroll
     for (int i = 0; i < NV * V; ++i) {
         const int c = ((i / V) * group + t) * V + i % V;
-        v[i] = p != nullptr && c < n ? load_any(p, type, c) : missing;
+        f[i] = p != nullptr && c < n ? load_any(p, type, c) : missing;
     }
+#pragma unroll
+    for (int i = 0; i < NV * V / 2; ++i) v[i] = Two(f[2 * i], f[2 * i + 1]);
 }
 
-template <typename TX, typename TY, int V, int NV, bool WARP>
-__global__ void __launch_bounds__(WARP ? 32 * kWarps : kBlockMax) k_norm_forward(Norm a) {
-    __shared__ float shared[2][kBlockMax / 32][2];
+template <typename TX, int V, int NV>
+struct ForwardRing {
+    static constexpr int kBytes = Rows<TX, V, NV>::kBytes;
+    static constexpr int kStages = ring_stages(kBytes);
+};
+template <typename TX, typename TY, int V, int NV>
+struct BackwardRing {
+    static constexpr int kX = Rows<TX, V, NV>::kBytes, kDy = Rows<TY, V, NV>::kBytes;
+    static constexpr int kBytes = 2 * kX + kDy;
+    static constexpr int kStages = ring_stages(kBytes);
+};
+
+// Where this thread stands: thread t of the `group` that shares a row, which is the `row`-th of
+// those that the block has in flight.
+template <int G>
+struct Seat {
+    static constexpr bool kWarp = G != 0;
+    int group, t, row, rows;
+    __device__ __forceinline__ Seat()
+        : group(kWarp ? G : blockDim.x), t(kWarp ? threadIdx.x % (kWarp ? G : 1) : threadIdx.x),
+          row(kWarp ? threadIdx.x / (kWarp ? G : 1) : 0), rows(kWarp ? blockDim.x / (kWarp ? G : 1) : 1) {}
+};
+
+template <typename TX, typename TY, int V, int G>
+__global__ void __launch_bounds__(G ? 32 * kWarps : kBlockMax, G ? kForwardBlocks : 1) k_norm_forward(Norm a) {
+    constexpr int NV = kHeld / V;
+    using Ring = ForwardRing<TX, V, NV>;
+    constexpr int S = Ring::kStages;
+    extern __shared__ __align__(16) unsigned char ring[];
+    __shared__ __align__(8) float shared[2][kBlockMax / 32][2];
     int turn = 0;
-    const int group = WARP ? 32 : blockDim.x, t = WARP ? threadIdx.x & 31 : threadIdx.x;
-    const int64_t first = WARP ? static_cast<int64_t>(blockIdx.x) * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
-    const int64_t step = WARP ? static_cast<int64_t>(gridDim.x) * (blockDim.x >> 5) : gridDim.x;
-    float w[NV * V], b[NV * V];
-    load_parameter<V, NV>(a.weight, a.parameter_type, 1.0f, t, group, a.n, w);
-    load_parameter<V, NV>(a.bias, a.parameter_type, 0.0f, t, group, a.n, b);
-    const float scale = 1.0f / static_cast<float>(a.n);
-    for (int64_t row = first; row < a.rows; row += step) {
-        float v[NV * V];
-        load_row<TX, V, NV>(static_cast<const TX*>(a.x) + row * a.x_stride, t, group, a.n, v);
-        float sum[1] = {0.0f};
+    const Seat<G> seat;
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * seat.rows + seat.row;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * seat.rows;
+    Rows<TX, V, NV> x(a.x, a.x_stride, first, step, seat.t, seat.group, a.n);
+    const int pitch = blockDim.x * V * static_cast<int>(sizeof(TX)), stage_bytes = blockDim.x * Ring::kBytes;
+    const unsigned char* mine = ring + threadIdx.x * V * sizeof(TX);
+    const uint32_t slot = static_cast<uint32_t>(__cvta_generic_to_shared(mine));
+    if (Ring::kBytes) {
 #pragma unroll
-        for (int i = 0; i < NV * V; ++i) sum[0] += v[i];
-        row_sum<WARP>(sum, shared, turn);
-        const float mean = sum[0] * scale;
-        float squares[1] = {0.0f};
-#pragma unroll
-        for (int i = 0; i < NV * V; ++i) {
-            const int c = ((i / V) * group + t) * V;
-            v[i] = v[i] - mean;
-            if (c < a.n) squares[0] += v[i] * v[i];
+        for (int k = 0; k < S - 1; ++k) {
+            if (first + k * step < a.rows) x.fetch(slot + k * stage_bytes, pitch);
+            ring_commit();
         }
-        row_sum<WARP>(squares, shared, turn);
-        const float rstd = rsqrtf(squares[0] * scale + a.epsilon);
+    }
+    Two w[kHeld / 2], b[kHeld / 2];
+    load_parameter<V, NV>(a.weight, a.parameter_type, 1.0f, seat.t, seat.group, a.n, w);
+    load_parameter<V, NV>(a.bias, a.parameter_type, 0.0f, seat.t, seat.group, a.n, b);
+    const float scale = 1.0f / static_cast<float>(a.n);
+    const bool whole = a.n == seat.group * kHeld;  // every thread holds as many elements as it can
+    const int at = seat.t * V, apart = seat.group * V;
+    TY* y = static_cast<TY*>(a.y) + first * a.y_stride + at;
+    const int64_t y_step = step * a.y_stride;
+    int stage = 0;
+    // lanes whose row is past the end go on with their warp (its sums take every lane) and store nothing
+    for (int64_t row = first; row - seat.row % (G && G < 32 ? 32 / (G ? G : 1) : 1) < a.rows; row += step, y += y_step) {
+        const bool live = row < a.rows;
+        Two v[kHeld / 2];
+        if (Ring::kBytes) {
+            if (row + (S - 1) * step < a.rows) x.fetch(slot + (stage == 0 ? S - 1 : stage - 1) * stage_bytes, pitch);
+            ring_commit();
+            ring_wait<S - 1>();
+        }
+        if (Ring::kBytes || live) x.get(mine + stage * stage_bytes, pitch, v);
+        stage = stage == S - 1 ? 0 : stage + 1;
+        Two total;
 #pragma unroll
-        for (int i = 0; i < NV * V; ++i) v[i] = v[i] * rstd * w[i] + b[i];
-        store_row<TY, V, NV>(static_cast<TY*>(a.y) + row * a.y_stride, t, group, a.n, v);
-        if (t == 0) {
+        for (int i = 0; i < kHeld / 2; ++i) total = total + v[i];
+        float sum[1] = {total.sum()};
+        row_sum<G>(sum, shared, turn);
+        const float mean = sum[0] * scale;
+        const Two off(-mean, -mean);
+        Two squared;
+        if (whole) {
+#pragma unroll
+            for (int i = 0; i < kHeld / 2; ++i) {
+                v[i] = v[i] + off;
+                squared = multiply_add(v[i], v[i], squared);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kHeld / 2; ++i) {
+                float2 d = (v[i] + off).get();
+                if (at + (2 * i / V) * apart >= a.n) d.x = 0.0f;
+                if (at + ((2 * i + 1) / V) * apart >= a.n) d.y = 0.0f;
+                v[i] = Two(d.x, d.y);
+                squared = multiply_add(v[i], v[i], squared);
+            }
+        }
+        float squares[1] = {squared.sum()};
+        row_sum<G>(squares, shared, turn);
+        const float rstd = rsqrtf(squares[0] * scale + a.epsilon);
+        const Two scaled(rstd, rstd);
+#pragma unroll
+        for (int i = 0; i < kHeld / 2; ++i) v[i] = multiply_add(v[i] * scaled, w[i], b[i]);
+        if (!live) continue;
+        store_row<TY, V, NV>(y, at, apart, a.n, v);
+        if (seat.t == 0) {
             if (a.mean) a.mean[row] = mean;
             if (a.rstd) a.rstd[row] = rstd;
         }
     }
+    ring_wait<0>();
 }
 
-template <typename TX, typename TY, int V, int NV, bool WARP>
-__global__ void __launch_bounds__(WARP ? 32 * kWarps : kBlockMax) k_norm_backward(Norm a) {
-    __shared__ float shared[2][kBlockMax / 32][2];
-    __shared__ float joined[WARP ? kWarps : 1][WARP ? 32 * NV * V : 1];
+template <typename TX, typename TY, int V, int G>
+__global__ void __launch_bounds__(G ? 32 * kWarps : kBlockMax, G ? kBackwardBlocks : 1) k_norm_backward(Norm a) {
+    constexpr int NV = kHeld / V;
+    using Ring = BackwardRing<TX, TY, V, NV>;
+    constexpr int S = Ring::kStages;
+    extern __shared__ __align__(16) unsigned char ring[];
+    __shared__ __align__(8) float shared[2][kBlockMax / 32][2];
     int turn = 0;
-    const int group = WARP ? 32 : blockDim.x, t = WARP ? threadIdx.x & 31 : threadIdx.x;
-    const int64_t first = WARP ? static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5) : blockIdx.x;
-    const int64_t step = WARP ? static_cast<int64_t>(gridDim.x) * kWarps : gridDim.x;
-    float w[NV * V], dw[NV * V], db[NV * V];
-    load_parameter<V, NV>(a.weight, a.parameter_type, 1.0f, t, group, a.n, w);
-#pragma unroll
-    for (int i = 0; i < NV * V; ++i) dw[i] = db[i] = 0.0f;
-    const float scale = 1.0f / static_cast<float>(a.n);
-    for (int64_t row = first; row < a.rows; row += step) {
-        float x[NV * V], g[NV * V];
-        load_row<TX, V, NV>(static_cast<const TX*>(a.x) + row * a.x_stride, t, group, a.n, x);
-        load_row<TY, V, NV>(static_cast<const TY*>(a.dy) + row * a.dy_stride, t, group, a.n, g);
-        const float mean = a.mean[row], rstd = a.rstd[row];
-        float sum[2] = {0.0f, 0.0f};
-#pragma unroll
-        for (int i = 0; i < NV * V; ++i) {
-            x[i] = (x[i] - mean) * rstd;  // beyond the row g is 0, and so is every use of x
-            dw[i] += g[i] * x[i];
-            db[i] += g[i];
-            g[i] *= w[i];
-            sum[0] += g[i];
-            sum[1] += g[i] * x[i];
+    const Seat<G> seat;
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * seat.rows + seat.row;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * seat.rows;
+    Rows<TX, V, NV> x(a.x, a.x_stride, first, step, seat.t, seat.group, a.n);
+    Rows<TX, V, NV> residual(a.residual, a.residual_stride, first, step, seat.t, seat.group, a.n);
+    Rows<TY, V, NV> dy(a.dy, a.dy_stride, first, step, seat.t, seat.group, a.n);
+    const int x_pitch = blockDim.x * V * static_cast<int>(sizeof(TX)), dy_pitch = blockDim.x * V * static_cast<int>(sizeof(TY));
+    const int stage_bytes = blockDim.x * Ring::kBytes;
+    // a stage: x, residual, dy
+    const unsigned char* mine_x = ring + threadIdx.x * V * sizeof(TX);
+    const unsigned char* mine_dy = ring + 2 * blockDim.x * Ring::kX + threadIdx.x * V * sizeof(TY);
+    const int residual_at = blockDim.x * Ring::kX;
+    const uint32_t slot_x = static_cast<uint32_t>(__cvta_generic_to_shared(mine_x));
+    const uint32_t slot_dy = static_cast<uint32_t>(__cvta_generic_to_shared(mine_dy));
+    auto fetch = [&](int stage, int64_t row) {
+        if (!Ring::kBytes) return;
+        if (row < a.rows) {
+            x.fetch(slot_x + stage * stage_bytes, x_pitch);
+            dy.fetch(slot_dy + stage * stage_bytes, dy_pitch);
+            if (a.residual) residual.fetch(slot_x + residual_at + stage * stage_bytes, x_pitch);
         }
-        row_sum<WARP>(sum, shared, turn);
-        const float of_g = sum[0] * scale, of_gx = sum[1] * scale;
+        ring_commit();
+    };
 #pragma unroll
-        for (int i = 0; i < NV * V; ++i) x[i] = rstd * (g[i] - of_g - x[i] * of_gx);
-        if (a.residual) {
-            load_row<TX, V, NV>(static_cast<const TX*>(a.residual) + row * a.residual_stride, t, group, a.n, g);
-#pragma unroll
-            for (int i = 0; i < NV * V; ++i) x[i] += g[i];
-        }
-        store_row<TX, V, NV>(static_cast<TX*>(a.y) + row * a.y_stride, t, group, a.n, x);
+    for (int k = 0; k < S - 1; ++k) fetch(k, first + k * step);
+    float next_mean = 0.0f, next_rstd = 0.0f;
+    if (first < a.rows) {
+        next_mean = a.mean[first];
+        next_rstd = a.rstd[first];
     }
+    Two w[kHeld / 2], dw[kHeld / 2], db[kHeld / 2];
+    load_parameter<V, NV>(a.weight, a.parameter_type, 1.0f, seat.t, seat.group, a.n, w);
+    const float scale = 1.0f / static_cast<float>(a.n);
+    const int at = seat.t * V, apart = seat.group * V;
+    TX* dx = static_cast<TX*>(a.y) + first * a.y_stride + at;
+    const int64_t dx_step = step * a.y_stride;
+    int stage = 0;
+    for (int64_t row = first; row - seat.row % (G && G < 32 ? 32 / (G ? G : 1) : 1) < a.rows; row += step, dx += dx_step) {
+        const bool live = row < a.rows;
+        fetch(stage == 0 ? S - 1 : stage - 1, row + (S - 1) * step);
+        const float mean = next_mean, rstd = next_rstd;
+        if (row + step < a.rows) {
+            next_mean = a.mean[row + step];
+            next_rstd = a.rstd[row + step];
+        }
+        if (Ring::kBytes) ring_wait<S - 1>();
+        Two v[kHeld / 2], g[kHeld / 2];
+        if (live) {
+            x.get(mine_x + stage * stage_bytes, x_pitch, v);
+            dy.get(mine_dy + stage * stage_bytes, dy_pitch, g);
+        }
+        Two of_g, of_gx;
+        {
+            const Two off(-mean, -mean), scaled(rstd, rstd);
+#pragma unroll
+            for (int i = 0; i < kHeld / 2; ++i) {
+                v[i] = (v[i] + off) * scaled;  // beyond the row dy is 0, and so is all that v adds
+                if (live) dw[i] = multiply_add(g[i], v[i], dw[i]);
+                db[i] = db[i] + g[i];
+                g[i] = g[i] * w[i];
+                of_g = of_g + g[i];
+                of_gx = multiply_add(g[i], v[i], of_gx);
+            }
+        }
+        float sum[2] = {of_g.sum(), of_gx.sum()};
+        row_sum<G>(sum, shared, turn);
+        if (live) {
+            const float c0 = -rstd * (sum[0] * scale), c1 = -rstd * (sum[1] * scale);
+            const Two of_one(c0, c0), of_x(c1, c1), of_dy(rstd, rstd);
+#pragma unroll
+            for (int i = 0; i < kHeld / 2; ++i) v[i] = multiply_add(g[i], of_dy, multiply_add(v[i], of_x, of_one));
+            if (a.residual) {
+                residual.get(mine_x + residual_at + stage * stage_bytes, x_pitch, g);
+#pragma unroll
+                for (int i = 0; i < kHeld / 2; ++i) v[i] = v[i] + g[i];
+            }
+            store_row<TX, V, NV>(dx, at, apart, a.n, v);
+        }
+        stage = stage == S - 1 ? 0 : stage + 1;
+    }
+    ring_wait<0>();
     if (a.partial == nullptr) return;
     float* out = a.partial + static_cast<size_t>(blockIdx.x) * a.n;
+    if (G) {
+        // the rows' sums meet in shared memory, over the ring: [rows of the block][group kHeld]
+        float* joined = reinterpret_cast<float*>(ring);
+        const int width = G * kHeld;
 #pragma unroll
-    for (int which = 0; which < 2; ++which, out += static_cast<size_t>(gridDim.x) * a.n) {
-        if (WARP) {
+        for (int which = 0; which < 2; ++which, out += static_cast<size_t>(gridDim.x) * a.n) {
             __syncthreads();
 #pragma unroll
-            for (int i = 0; i < NV * V; ++i) joined[threadIdx.x >> 5][((i / V) * 32 + t) * V + i % V] = which ? db[i] : dw[i];
+            for (int i = 0; i < kHeld; ++i) {
+                const float2 pair = (which ? db[i / 2] : dw[i / 2]).get();
+                joined[seat.row * width + at + (i / V) * apart + i % V] = i % 2 ? pair.y : pair.x;
+            }
             __syncthreads();
-            for (int c = threadIdx.x; c < a.n; c += 32 * kWarps) {
+            for (int c = threadIdx.x; c < a.n; c += blockDim.x) {
                 float v = 0.0f;
-#pragma unroll
-                for (int k = 0; k < kWarps; ++k) v += joined[k][c];
+                for (int k = 0; k < seat.rows; ++k) v += joined[k * width + c];
                 out[c] = v;
             }
-        } else {
+        }
+    } else {
 #pragma unroll
-            for (int i = 0; i < NV * V; ++i) {
-                const int c = ((i / V) * group + t) * V + i % V;
-                if (c < a.n) out[c] = which ? db[i] : dw[i];
+        for (int i = 0; i < kHeld; ++i) {
+            const int c = at + (i / V) * apart + i % V;
+            const float2 w2 = dw[i / 2].get(), b2 = db[i / 2].get();
+            if (c < a.n) {
+                out[c] = i % 2 ? w2.y : w2.x;
+                out[static_cast<size_t>(gridDim.x) * a.n + c] = i % 2 ? b2.y : b2.x;
             }
         }
     }
@@ -227,13 +440,13 @@ __global__ void k_norm_parameters(const float* partial, int count, int n, void* 
 // ------------------------------------------------------------------ rows beyond 8,192 elements
 __device__ __forceinline__ float block_sum(float v, float (*shared)[kBlockMax / 32][2], int& turn) {
     float s[1] = {v};
-    row_sum<false>(s, shared, turn);
+    row_sum<0>(s, shared, turn);
     return s[0];
 }
 
 template <typename TX, typename TY>
 __global__ void __launch_bounds__(kBlockMax) k_wide_forward(Norm a) {
-    __shared__ float shared[2][kBlockMax / 32][2];
+    __shared__ __align__(8) float shared[2][kBlockMax / 32][2];
     int turn = 0;
     const float scale = 1.0f / static_cast<float>(a.n);
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
@@ -263,7 +476,7 @@ __global__ void __launch_bounds__(kBlockMax) k_wide_forward(Norm a) {
 // dx alone; k_wide_columns sums the parameters' gradients.
 template <typename TX, typename TY>
 __global__ void __launch_bounds__(kBlockMax) k_wide_backward(Norm a) {
-    __shared__ float shared[2][kBlockMax / 32][2];
+    __shared__ __align__(8) float shared[2][kBlockMax / 32][2];
     int turn = 0;
     const float scale = 1.0f / static_cast<float>(a.n);
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
@@ -279,7 +492,7 @@ __global__ void __launch_bounds__(kBlockMax) k_wide_backward(Norm a) {
             sum[0] += g;
             sum[1] += g * ((Element<TX>::load(x[c]) - mean) * rstd);
         }
-        row_sum<false>(sum, shared, turn);
+        row_sum<0>(sum, shared, turn);
         const float of_g = sum[0] * scale, of_gx = sum[1] * scale;
         for (int c = threadIdx.x; c < a.n; c += kBlockMax) {
             const float w = a.weight ? load_any(a.weight, a.parameter_type, c) : 1.0f;
@@ -315,41 +528,46 @@ int multiprocessors() {
     return count;
 }
 
-// Blocks of the backward pass: what is resident at once (two blocks of 8 warps an SM), and no more
-// than there are rows to take. The workspace is sized by the same rule.
-constexpr int kBackwardBlocksPerSm = 2;
+// Threads and rows in flight of a block, and the grid: what is resident at once, and no more than
+// there are rows to take. The backward pass's workspace is sized by the same rule.
+int threads_of(int64_t n) { return group_of(n) ? 32 * kWarps : static_cast<int>(round_up((n + kHeld - 1) / kHeld, 32)); }
+int blocks_of(int64_t rows, int64_t n, int per_sm, int sms) {
+    const int64_t in_flight = group_of(n) ? 32 * kWarps / group_of(n) : 1;
+    const int64_t resident = group_of(n) ? per_sm : per_sm * 32 * kWarps / threads_of(n);
+    return static_cast<int>(std::max<int64_t>(1, std::min((rows + in_flight - 1) / in_flight, sms * resident)));
+}
 int backward_blocks(int64_t rows, int64_t n, int sms) {
     if (n > kHeld * kBlockMax) return static_cast<int>(std::min<int64_t>(rows, 64));
-    const int64_t want = n <= kHeld * 32 ? (rows + kWarps - 1) / kWarps : rows;
-    const int64_t threads = n <= kHeld * 32 ? 32 * kWarps : round_up((n + kHeld - 1) / kHeld, 32);
-    const int64_t resident = static_cast<int64_t>(sms) * std::max<int64_t>(1, kBackwardBlocksPerSm * 32 * kWarps / threads);
-    return static_cast<int>(std::max<int64_t>(1, std::min(want, resident)));
+    return blocks_of(rows, n, kBackwardBlocks, sms);
+}
+
+template <typename TX, typename TY, int V, int G>
+void launch_norm(const Norm& a, bool backward, int sms, cudaStream_t stream) {
+    constexpr int kMost = G ? 32 * kWarps : kBlockMax;
+    const int threads = threads_of(a.n);
+    static uint64_t configured = 0;
+    if (backward) {
+        using Ring = BackwardRing<TX, TY, V, kHeld / V>;
+        constexpr int kJoined = G ? 32 * kWarps * kHeld * 4 : 0;
+        allow_smem(k_norm_backward<TX, TY, V, G>, std::max(Ring::kStages * Ring::kBytes * kMost, kJoined), configured);
+        launch("k_norm_backward", k_norm_backward<TX, TY, V, G>, backward_blocks(a.rows, a.n, sms), threads,
+               std::max(Ring::kStages * Ring::kBytes * threads, kJoined), stream, a);
+    } else {
+        using Ring = ForwardRing<TX, V, kHeld / V>;
+        static uint64_t forward_configured = 0;
+        allow_smem(k_norm_forward<TX, TY, V, G>, Ring::kStages * Ring::kBytes * kMost, forward_configured);
+        launch("k_norm_forward", k_norm_forward<TX, TY, V, G>, blocks_of(a.rows, a.n, kForwardBlocks, sms), threads,
+               Ring::kStages * Ring::kBytes * threads, stream, a);
+    }
 }
 
 template <typename TX, typename TY, int V>
 void run(const Norm& a, bool backward, int sms, cudaStream_t stream) {
-    constexpr int NV = kHeld / V;
-    const bool warp = a.n <= kHeld * 32;
-    const int threads = warp ? 32 * kWarps : static_cast<int>(round_up((a.n + kHeld - 1) / kHeld, 32));
-    if (backward) {
-        const int grid = backward_blocks(a.rows, a.n, sms);
-        if (!warp) {
-            launch("k_norm_backward", k_norm_backward<TX, TY, V, NV, false>, grid, threads, 0, stream, a);
-        } else if (a.n <= kHeld * 16) {
-            launch("k_norm_backward", k_norm_backward<TX, TY, V, NV / 2 ? NV / 2 : 1, true>, grid, threads, 0, stream, a);
-        } else {
-            launch("k_norm_backward", k_norm_backward<TX, TY, V, NV, true>, grid, threads, 0, stream, a);
-        }
-        return;
-    }
-    const int64_t want = warp ? (a.rows + kWarps - 1) / kWarps : a.rows;
-    const int grid = static_cast<int>(std::min<int64_t>(want, static_cast<int64_t>(sms) * std::max(1, 1024 / threads)));
-    if (!warp) {
-        launch("k_norm_forward", k_norm_forward<TX, TY, V, NV, false>, grid, threads, 0, stream, a);
-    } else if (a.n <= kHeld * 16) {
-        launch("k_norm_forward", k_norm_forward<TX, TY, V, NV / 2 ? NV / 2 : 1, true>, grid, threads, 0, stream, a);
-    } else {
-        launch("k_norm_forward", k_norm_forward<TX, TY, V, NV, true>, grid, threads, 0, stream, a);
+    switch (group_of(a.n)) {
+        case 8: launch_norm<TX, TY, V, 8>(a, backward, sms, stream); break;
+        case 16: launch_norm<TX, TY, V, 16>(a, backward, sms, stream); break;
+        case 32: launch_norm<TX, TY, V, 32>(a, backward, sms, stream); break;
+        default: launch_norm<TX, TY, V, 0>(a, backward, sms, stream); break;
     }
 }
 
