@@ -217,9 +217,10 @@ struct Span {
     bool overlaps(const Span& o) const { return first < o.last && o.first < last; }
 };
 
-// A kernel's dynamic shared memory and cluster shape, configured once per device.
+// A kernel's dynamic shared memory, allowed once per device.
 template <typename Kernel>
 inline void allow_smem(Kernel kernel, size_t bytes, uint64_t& configured) {
+    if (bytes <= 32 * 1024) return;  // with the static part, below what needs no leave
     int device = 0;
     check(cudaGetDevice(&device), "cudaGetDevice");
     const uint64_t bit = 1ull << (device & 63);

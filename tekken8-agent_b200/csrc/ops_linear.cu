@@ -69,7 +69,7 @@ void forward(const char* what, int type, LinearCall& c, void* workspace, size_t 
         pre.overlaps(x) || pre.overlaps(w) || pre.overlaps(residual) || pre.overlaps(bias)) {
         raise(T8B_EINVAL, std::string(what) + ": an output overlaps another argument");
     }
-    const bool packs = !tma_rows(c.x, c.rows, c.x_stride, 2) || !tma_rows(c.weight, columns, c.weight_stride, 2);
+    const bool packs = !is_few(c.rows, c.in) && (!tma_rows(c.x, c.rows, c.x_stride, 2) || !tma_rows(c.weight, columns, c.weight_stride, 2));
     check_workspace(what, workspace, workspace_bytes, packs ? Workspace(c.rows, c.in, columns).forward_bytes : 0);
     c.workspace = static_cast<unsigned char*>(workspace);
     if (type == T8B_BF16) {

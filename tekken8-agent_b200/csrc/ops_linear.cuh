@@ -66,7 +66,9 @@ inline GemmPlan plan_gemm(int64_t m, int64_t n, int64_t k, bool may_split) {
         const int64_t tiles = ceil_div(m, f.pair ? 256 : 128) * ceil_div(n, f.bn);
         const int64_t workers = f.pair ? kClusters : kSms;
         const int64_t most = may_split ? std::min<int64_t>(kMaxSplits, std::max<int64_t>(1, k_blocks / 4)) : 1;
-        for (int64_t splits = 1; splits <= most; ++splits) {
+        // the parts that fill one to four waves; more or fewer leave workers idle
+        for (int64_t wave = 0; wave <= (most > 1 ? 4 : 0); ++wave) {
+            const int64_t splits = wave == 0 ? 1 : std::min<int64_t>(most, std::max<int64_t>(1, wave * workers / tiles));
             const double waves = static_cast<double>(ceil_div(tiles * splits, workers));
             double cost = waves * (static_cast<double>(ceil_div(k_blocks, splits)) * f.block_cycles + f.tile_cycles);
             if (splits > 1) cost += 6000.0 + static_cast<double>(splits) * m * n * 8.0 / 2500.0;
@@ -79,6 +81,12 @@ inline GemmPlan plan_gemm(int64_t m, int64_t n, int64_t k, bool may_split) {
     return best;
 }
 
+// Whether a forward pass goes row by row (k_few_rows) and not by tiles: measured (bf16, us by rows /
+// by tiles), 512 -> 512: 1 row 4.2 / 8.3, 16 rows 6.2 / 8.3, 64 rows 10.3 / 8.3; gated 512 -> 1,408:
+// 16 rows 8.3 / 8.3, 24 rows 12.4 / 8.3; 2,048 -> 2,048: 1 row 6.2 / 16.5, 4 rows 9.2 / 16.5, 16
+// rows 26 / 16.5.
+inline bool is_few(int64_t rows, int64_t in) { return rows <= 4 || (rows <= 16 && in <= 512); }
+
 // The parts of a split GEMM: fp32 [splits][rows to whole tiles][columns to whole pieces].
 inline size_t split_rows(int64_t m) { return round_up(m, 256); }
 inline size_t split_pitch(int64_t n) { return round_up(n, 4); }
@@ -87,7 +95,7 @@ inline size_t split_pitch(int64_t n) { return round_up(n, 4); }
 constexpr int kGradRows = 8;
 inline int grad_parts(int64_t rows, int64_t columns) {
     const int64_t across = ceil_div(columns, 256);
-    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(ceil_div(rows, kGradRows), ceil_div(kSms * 6, across))));
+    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(ceil_div(rows, kGradRows), ceil_div(kSms * 3, across))));
 }
 
 // The workspace, in this order; each part starts on a 256-byte boundary. A forward pass uses the
@@ -340,56 +348,192 @@ __global__ void k_pack(const E* in, int64_t stride, int64_t rows, int columns, E
     }
 }
 
+// A forward pass of few rows: a warp per output column (or per gate and up column), its lanes over
+// the row of the weight in 16-byte pieces (WIDE; single elements where rows are not aligned), R rows
+// of x at a time. Bound by the latency of one pass over the weight, spread over every SM, where a
+// tile of the tensor-core kernel would wait for its k blocks one after the other.
+template <typename E>
+struct FewRows {
+    const E *x, *weight;
+    const void *bias, *residual;
+    void* y;
+    E* pre;
+    int64_t x_stride, weight_stride, residual_stride, y_stride, pre_stride;
+    int rows, in, out, bias_type, activation, y_type;
+};
+constexpr int kFewWarps = 8;
+template <typename E, bool GATED, int R, bool WIDE>
+__global__ void __launch_bounds__(32 * kFewWarps) k_few_rows(FewRows<E> a) {
+    constexpr int PARTS = GATED ? 2 : 1;
+    const int lane = threadIdx.x & 31;
+    const int row0 = blockIdx.y * R, live = min(R, a.rows - row0);
+    for (int c = blockIdx.x * kFewWarps + (threadIdx.x >> 5); c < a.out; c += gridDim.x * kFewWarps) {
+        const E* w[PARTS];
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) w[p] = a.weight + (static_cast<int64_t>(p) * a.out + c) * a.weight_stride;
+        const E* x = a.x + row0 * a.x_stride;
+        float sum[PARTS][R];
+        int done = 0;
+        if (WIDE) {
+            Two pair[PARTS][R];
+            const int pieces = a.in / 8;
+#pragma unroll 2
+            for (int i = lane; i < pieces; i += 32) {
+                Pack<uint32_t, 4> words[PARTS];
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p) words[p] = *reinterpret_cast<const Pack<uint32_t, 4>*>(w[p] + i * 8);
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    if (r >= live) break;
+                    const Pack<uint32_t, 4> row = *reinterpret_cast<const Pack<uint32_t, 4>*>(x + r * a.x_stride + i * 8);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float2 xv = Element<E>::unpack(row.v[j]);
+#pragma unroll
+                        for (int p = 0; p < PARTS; ++p) {
+                            const float2 wv = Element<E>::unpack(words[p].v[j]);
+                            pair[p][r] = multiply_add(Two(xv.x, xv.y), Two(wv.x, wv.y), pair[p][r]);
+                        }
+                    }
+                }
+            }
+            done = pieces * 8;
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p) {
+#pragma unroll
+                for (int r = 0; r < R; ++r) sum[p][r] = pair[p][r].sum();
+            }
+        } else {
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p) {
+#pragma unroll
+                for (int r = 0; r < R; ++r) sum[p][r] = 0.0f;
+            }
+        }
+#pragma unroll 4
+        for (int i = done + lane; i < a.in; i += 32) {
+            float wv[PARTS];
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p) wv[p] = Element<E>::load(w[p][i]);
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                if (r >= live) break;
+                const float xv = Element<E>::load(x[r * a.x_stride + i]);
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p) sum[p][r] = fmaf(xv, wv[p], sum[p][r]);
+            }
+        }
+        float mine[PARTS];  // lane r: row r's sums
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) {
+            mine[p] = 0.0f;
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                float v = sum[p][r];
+#pragma unroll
+                for (int o = 16; o >= 1; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+                if (lane == r) mine[p] = v;
+            }
+            if (a.bias) mine[p] += load_any(a.bias, a.bias_type, static_cast<size_t>(p) * a.out + c);
+        }
+        if (lane >= live) continue;
+        const int64_t row = row0 + lane;
+        if (a.pre) {
+#pragma unroll
+            for (int p = 0; p < PARTS; ++p) a.pre[row * a.pre_stride + static_cast<int64_t>(p) * a.out + c] = Element<E>::store(mine[p]);
+        }
+        float v = 0.0f;
+        with_activation(a.activation, [&](auto act) { v = activate<decltype(act)::value>(mine[0]); });
+        if (GATED) v *= mine[PARTS - 1];
+        if (a.residual) v += load_any(a.residual, a.y_type, row * a.residual_stride + c);
+        store_any(a.y, a.y_type, row * a.y_stride + c, v);
+    }
+}
+
 // The elementwise half of a backward pass: dz (rows of `pitch` elements) from dy and pre, and this
 // block row's column sums of dz in fp32, before dz is rounded. A thread holds V columns over its
-// rows, and reads the next rows while it works on these; block (32, kGradRows).
+// rows; block (32, kGradRows).
 //   linear: dz = dy activation'(pre);  gated: dz = [dy up activation'(gate) | dy activation(gate)]
-// Bound by memory: it reads dy and pre and writes dz once.
-template <typename E, int V>
-struct GradRow {
-    Pack<E, V> d, z, u;
-};
+// Bound by memory: it reads dy and pre and writes dz once. With V = 8 a thread's next rows come
+// through its own part of a ring in shared memory (cp.async, as in the layer norm's kernels).
+constexpr int kGradStages = 4;
 template <typename E, bool GATED, int V>
-__global__ void __launch_bounds__(32 * kGradRows)
+constexpr int grad_ring_bytes() { return V == 8 ? kGradStages * (GATED ? 3 : 2) * 16 * 32 * kGradRows : 0; }
+
+template <typename E, bool GATED, int V>
+__global__ void __launch_bounds__(32 * kGradRows, 3)
     k_activation_grad(const E* dy, int64_t dy_stride, const E* pre, int64_t pre_stride, int64_t rows, int columns,
                       int activation, E* dz, int64_t pitch, float* sums) {
     constexpr int PARTS = GATED ? 2 : 1;
+    constexpr bool RING = V == 8;
+    constexpr int kThreads = 32 * kGradRows;
+    constexpr int kStage = (GATED ? 3 : 2) * 16 * kThreads;
+    extern __shared__ __align__(16) unsigned char ring[];
     __shared__ float joined[kGradRows][32 * V + 1];
     const int c = (blockIdx.x * 32 + threadIdx.x) * V;
-    const bool in = c < columns;
     float sum[PARTS][V];
 #pragma unroll
     for (int p = 0; p < PARTS; ++p) {
 #pragma unroll
         for (int j = 0; j < V; ++j) sum[p][j] = 0.0f;
     }
-    if (in) {
+    if (c < columns) {
         with_activation(activation, [&](auto act) {
             constexpr int ACT = decltype(act)::value;
+            constexpr bool READS = GATED || ACT != T8B_LINEAR;  // pre
             const int64_t first = static_cast<int64_t>(blockIdx.y) * kGradRows + threadIdx.y;
             const int64_t step = static_cast<int64_t>(gridDim.y) * kGradRows;
             const E* from_dy = dy + first * dy_stride + c;
-            const E* from_pre = GATED || ACT != T8B_LINEAR ? pre + first * pre_stride + c : nullptr;
+            const E* from_pre = READS ? pre + first * pre_stride + c : nullptr;
             E* to = dz ? dz + first * pitch + c : nullptr;
-            auto read = [&](GradRow<E, V>& r) {
-                r.d = *reinterpret_cast<const Pack<E, V>*>(from_dy);
-                if (GATED || ACT != T8B_LINEAR) r.z = *reinterpret_cast<const Pack<E, V>*>(from_pre);
-                if (GATED) r.u = *reinterpret_cast<const Pack<E, V>*>(from_pre + columns);
-                from_dy += step * dy_stride;
-                if (GATED || ACT != T8B_LINEAR) from_pre += step * pre_stride;
+            unsigned char* mine = ring + (threadIdx.y * 32 + threadIdx.x) * 16;
+            const uint32_t slot = static_cast<uint32_t>(__cvta_generic_to_shared(mine));
+            auto copy = [&](uint32_t at, const E* from) {
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at), "l"(from) : "memory");
             };
-            auto use = [&](const GradRow<E, V>& r) {
-                Pack<E, V> out, out_up;
+            auto fetch = [&](int stage, bool any) {
+                if (any) {
+                    const uint32_t at = slot + stage * kStage;
+                    copy(at, from_dy);
+                    if (READS) copy(at + 16 * kThreads, from_pre);
+                    if (GATED) copy(at + 32 * kThreads, from_pre + columns);
+                    from_dy += step * dy_stride;
+                    if (READS) from_pre += step * pre_stride;
+                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            };
+            if (RING) {
+#pragma unroll
+                for (int k = 0; k < kGradStages - 1; ++k) fetch(k, first + k * step < rows);
+            }
+            int stage = 0;
+            for (int64_t row = first; row < rows; row += step) {
+                Pack<E, V> d, z{}, u{}, out, out_up;
+                if (RING) {
+                    fetch((stage + kGradStages - 1) % kGradStages, row + (kGradStages - 1) * step < rows);
+                    asm volatile("cp.async.wait_group %0;" ::"n"(kGradStages - 1) : "memory");
+                    const unsigned char* at = mine + stage * kStage;
+                    d = *reinterpret_cast<const Pack<E, V>*>(at);
+                    if (READS) z = *reinterpret_cast<const Pack<E, V>*>(at + 16 * kThreads);
+                    if (GATED) u = *reinterpret_cast<const Pack<E, V>*>(at + 32 * kThreads);
+                    stage = (stage + 1) % kGradStages;
+                } else {
+                    d = *reinterpret_cast<const Pack<E, V>*>(from_dy);
+                    if (READS) z = *reinterpret_cast<const Pack<E, V>*>(from_pre);
+                    if (GATED) u = *reinterpret_cast<const Pack<E, V>*>(from_pre + columns);
+                    from_dy += step * dy_stride;
+                    if (READS) from_pre += step * pre_stride;
+                }
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
                     float value, slope;
-                    const float d = Element<E>::load(r.d.v[j]);
-                    activate_slope<ACT>(GATED || ACT != T8B_LINEAR ? Element<E>::load(r.z.v[j]) : 0.0f, value, slope);
-                    const float of_z = d * slope * (GATED ? Element<E>::load(r.u.v[j]) : 1.0f);
+                    const float g = Element<E>::load(d.v[j]);
+                    activate_slope<ACT>(Element<E>::load(z.v[j]), value, slope);
+                    const float of_z = g * slope * (GATED ? Element<E>::load(u.v[j]) : 1.0f);
                     sum[0][j] += of_z;
                     out.v[j] = Element<E>::store(of_z);
                     if (GATED) {
-                        const float of_u = d * value;
+                        const float of_u = g * value;
                         sum[PARTS - 1][j] += of_u;
                         out_up.v[j] = Element<E>::store(of_u);
                     }
@@ -399,17 +543,8 @@ __global__ void __launch_bounds__(32 * kGradRows)
                     if (GATED) *reinterpret_cast<Pack<E, V>*>(to + columns) = out_up;
                     to += step * pitch;
                 }
-            };
-            GradRow<E, V> a, b;
-            int64_t row = first;
-            if (row < rows) read(a);
-            for (; row < rows; row += 2 * step) {
-                const bool second = row + step < rows;
-                if (second) read(b);
-                use(a);
-                if (row + 2 * step < rows) read(a);
-                if (second) use(b);
             }
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
         });
     }
     if (sums == nullptr) return;
@@ -419,7 +554,7 @@ __global__ void __launch_bounds__(32 * kGradRows)
 #pragma unroll
         for (int j = 0; j < V; ++j) joined[threadIdx.y][threadIdx.x * V + j] = sum[p][j];
         __syncthreads();
-        for (int k = threadIdx.y * 32 + threadIdx.x; k < 32 * V; k += 32 * kGradRows) {
+        for (int k = threadIdx.y * 32 + threadIdx.x; k < 32 * V; k += kThreads) {
             const int column = blockIdx.x * 32 * V + k;
             if (column >= columns) continue;
             float v = 0.0f;
@@ -594,9 +729,54 @@ void gated_tile(const LinearCall& c, const Matrix& x, const Matrix& w) {
     launch_gemm<E, CG, BN, false, false>("k_gated", x, w, c.out, static_cast<int>(c.out), 1, epi, c.stream);
 }
 
+template <typename E, bool GATED, int R>
+void few_rows(const LinearCall& c) {
+    FewRows<E> a{};
+    a.x = static_cast<const E*>(c.x);
+    a.weight = static_cast<const E*>(c.weight);
+    a.bias = c.bias;
+    a.residual = c.residual;
+    a.y = c.y;
+    a.pre = static_cast<E*>(c.pre);
+    a.x_stride = c.x_stride;
+    a.weight_stride = c.weight_stride;
+    a.residual_stride = c.residual_stride;
+    a.y_stride = c.y_stride;
+    a.pre_stride = c.pre_stride;
+    a.rows = static_cast<int>(c.rows);
+    a.in = static_cast<int>(c.in);
+    a.out = static_cast<int>(c.out);
+    a.bias_type = c.bias_type;
+    a.activation = c.activation;
+    a.y_type = c.y_type;
+    const dim3 grid(static_cast<unsigned>(std::min<int64_t>(ceil_div(c.out, kFewWarps), kSms * 8)), static_cast<unsigned>(ceil_div(c.rows, R)));
+    const bool wide = aligned(c.x, 16) && aligned(c.weight, 16) && (c.rows == 1 || c.x_stride % 8 == 0) &&
+        (c.weight_stride % 8 == 0 || (c.out == 1 && !GATED));
+    if (wide) {
+        launch("k_few_rows", k_few_rows<E, GATED, R, true>, grid, 32 * kFewWarps, 0, c.stream, a);
+    } else {
+        launch("k_few_rows", k_few_rows<E, GATED, R, false>, grid, 32 * kFewWarps, 0, c.stream, a);
+    }
+    check(cudaGetLastError(), "few rows");
+}
+template <typename E, bool GATED>
+void few_rows(const LinearCall& c) {
+    if (c.rows == 1) {
+        few_rows<E, GATED, 1>(c);
+    } else if (c.rows <= 4) {
+        few_rows<E, GATED, 4>(c);
+    } else {
+        few_rows<E, GATED, 8>(c);
+    }
+}
+
 template <typename E>
 void linear_forward(const LinearCall& c) {
     const int64_t columns = c.gated ? 2 * c.out : c.out;
+    if (is_few(c.rows, c.in)) {
+        c.gated ? few_rows<E, true>(c) : few_rows<E, false>(c);
+        return;
+    }
     const Workspace at(c.rows, c.in, columns);
     const Matrix x = operand<E>(c.x, c.rows, c.in, c.x_stride, c.workspace + at.x, c.stream);
     const Matrix w = operand<E>(c.weight, columns, c.in, c.weight_stride, c.workspace + at.weight, c.stream);
@@ -667,7 +847,10 @@ template <typename E, bool GATED, int V>
 void activation_grad(const LinearGradCall& c, E* dz, int64_t pitch, float* sums) {
     const int columns = static_cast<int>(c.out);
     const dim3 grid(blocks(columns, 32 * V), grad_parts(c.rows, GATED ? 2 * c.out : c.out));
-    launch("k_activation_grad", k_activation_grad<E, GATED, V>, grid, dim3(32, kGradRows), 0, c.stream,
+    constexpr int kRing = grad_ring_bytes<E, GATED, V>();
+    static uint64_t configured = 0;
+    allow_smem(k_activation_grad<E, GATED, V>, kRing, configured);
+    launch("k_activation_grad", k_activation_grad<E, GATED, V>, grid, dim3(32, kGradRows), kRing, c.stream,
            static_cast<const E*>(c.dy), c.dy_stride, static_cast<const E*>(c.pre), c.pre_stride, c.rows, columns, c.activation, dz,
            pitch, sums);
     check(cudaGetLastError(), "activation gradient");

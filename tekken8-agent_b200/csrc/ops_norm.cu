@@ -13,6 +13,7 @@
 // the blocks' sums are joined in a fixed order by k_norm_parameters, so results repeat bit for bit.
 // Rows of more than 8,192 elements go through the k_wide_* kernels, which read a row again from L2.
 #include <algorithm>
+#include <atomic>
 
 #include "ops.cuh"
 
@@ -522,9 +523,14 @@ __global__ void __launch_bounds__(256) k_wide_columns(Norm a) {
 
 // ------------------------------------------------------------------ dispatch
 int multiprocessors() {
-    int device = 0, count = 0;
+    static std::atomic<int> counts[64];
+    int device = 0;
     check(cudaGetDevice(&device), "cudaGetDevice");
-    check(cudaDeviceGetAttribute(&count, cudaDevAttrMultiProcessorCount, device), "SM count");
+    int count = counts[device & 63].load(std::memory_order_relaxed);
+    if (count == 0) {
+        check(cudaDeviceGetAttribute(&count, cudaDevAttrMultiProcessorCount, device), "SM count");
+        counts[device & 63].store(count, std::memory_order_relaxed);
+    }
     return count;
 }
 

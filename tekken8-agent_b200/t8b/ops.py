@@ -20,6 +20,7 @@ _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3, "tanh": 4}
 
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch.cuda.current_device
 _entries: dict = {}
 
 
@@ -41,6 +42,8 @@ def _check(status):
 class _On:
     """The tensors' device and the stream of a call, current while it allocates and queues."""
 
+    __slots__ = ("index", "stream", "entered")
+
     def __init__(self, tensor, stream):
         self.index = tensor.get_device()
         if self.index < 0:
@@ -48,20 +51,18 @@ class _On:
         self.stream = stream
 
     def __enter__(self):
-        self._device = self._stream = None
-        if torch.cuda.current_device() != self.index:
-            self._device = torch.cuda.device(self.index)
-            self._device.__enter__()
+        self.entered = ()
+        if _current_device() != self.index:
+            self.entered += (torch.cuda.device(self.index),)
         if self.stream is not None:
-            self._stream = torch.cuda.stream(self.stream)
-            self._stream.__enter__()
+            self.entered += (torch.cuda.stream(self.stream),)
+        for each in self.entered:
+            each.__enter__()
         return _raw_stream(self.index)
 
     def __exit__(self, *exc):
-        if self._stream is not None:
-            self._stream.__exit__(*exc)
-        if self._device is not None:
-            self._device.__exit__(*exc)
+        for each in reversed(self.entered):
+            each.__exit__(*exc)
 
 
 def _rows(t, name, columns, device, dtype=None):
@@ -127,11 +128,11 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, out_dtype=None, sav
         raise ValueError("layer norm parameters are fp32, bf16 or f16")
     pw, pb = _vector(weight, "weight", n, on.index, kind), _vector(bias, "bias", n, on.index, kind)
     with on as raw:
-        y = torch.empty(x.shape, dtype=out_dtype, device=x.device)
+        y = x.new_empty(x.shape, dtype=out_dtype)
         mean = rstd = None
         if save:
-            mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-            rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+            mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
+            rstd = x.new_empty(x.shape[:-1], dtype=torch.float32)
         _check(_entry("t8b_layer_norm_forward")(
             px, _TYPES[x.dtype], stride, pw, pb, _TYPES[kind[0]], eps, rows, n, y.data_ptr(), _TYPES[out_dtype], n,
             mean.data_ptr() if save else 0, rstd.data_ptr() if save else 0, raw))
@@ -165,11 +166,11 @@ def layer_norm_backward(dy, x, weight, bias, mean, rstd, residual_gradient=None,
     statistics = [_vector(v.reshape(-1) if v.dim() != 1 else v, name, rows, device, (torch.float32,))
                   for v, name in ((mean, "mean"), (rstd, "rstd"))]
     with on as raw:
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        dx = x.new_empty(x.shape, dtype=x.dtype)
         dweight = torch.empty_like(weight) if weight is not None else None
         dbias = torch.empty_like(bias) if bias is not None else None
         size = _entry("t8b_layer_norm_workspace")(rows, n) if first is not None else 0
-        workspace = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+        workspace = x.new_empty(size, dtype=torch.uint8) if size else None
         _check(_entry("t8b_layer_norm_backward")(
             pdy, _TYPES[dy.dtype], dy_stride, px, _TYPES[x.dtype], x_stride, pw, _TYPES[kind[0]], *statistics, pr,
             r_stride, rows, n, dx.data_ptr(), n, dweight.data_ptr() if dweight is not None else 0,
@@ -196,7 +197,7 @@ def _forward_workspace(name, px, x_stride, pw, w_stride, rows, n, out, x):
     if not ((px | pw) & 15 or (x_stride | w_stride) & 7) or rows == 0:
         return None, 0, 0
     size = _entry(name)(rows, n, out, 0)
-    workspace = torch.empty(size, dtype=torch.uint8, device=x.device)
+    workspace = x.new_empty(size, dtype=torch.uint8)
     return workspace, workspace.data_ptr(), size
 
 
@@ -218,8 +219,8 @@ def linear(x, weight, bias=None, activation: str = "none", residual=None, out_dt
             raise ValueError(f"residual has shape {tuple(residual.shape)}, expected {shape}")
         pr, _, r_stride = _rows(residual, "residual", out, on.index, out_dtype)
     with on as raw:
-        y = torch.empty(shape, dtype=out_dtype, device=x.device)
-        pre = torch.empty(shape, dtype=kind, device=x.device) if save else None
+        y = x.new_empty(shape, dtype=out_dtype)
+        pre = x.new_empty(shape, dtype=kind) if save else None
         workspace, pws, size = _forward_workspace("t8b_linear_workspace", px, x_stride, pw, w_stride, rows, n, out, x)
         _check(_entry("t8b_linear_forward")(
             _TYPES[kind], px, x_stride, pw, w_stride, pb, _TYPES[bias.dtype] if bias is not None else 0, act, pr,
@@ -235,8 +236,8 @@ def gated(x, weight, bias=None, activation: str = "silu", save: bool = False, st
     act, out = _activation(activation), columns // 2
     pb = _vector(bias, "bias", columns, on.index, (torch.float32, kind))
     with on as raw:
-        h = torch.empty((*x.shape[:-1], out), dtype=kind, device=x.device)
-        pre = torch.empty((*x.shape[:-1], columns), dtype=kind, device=x.device) if save else None
+        h = x.new_empty((*x.shape[:-1], out), dtype=kind)
+        pre = x.new_empty((*x.shape[:-1], columns), dtype=kind) if save else None
         workspace, pws, size = _forward_workspace("t8b_gated_workspace", px, x_stride, pw, w_stride, rows, n, out, x)
         _check(_entry("t8b_gated_forward")(
             _TYPES[kind], px, x_stride, pw, w_stride, pb, _TYPES[bias.dtype] if bias is not None else 0, act, rows, n,
@@ -259,11 +260,11 @@ def _backward(entry, query, parts, dy, x, weight, bias, pre, activation, input_g
         pp, _, p_stride = _rows(pre, "pre", columns, on.index, kind)
     _vector(bias, "bias", columns, on.index, (torch.float32, kind))
     with on as raw:
-        dx = torch.empty(x.shape, dtype=kind, device=x.device) if input_gradient else None
-        dweight = torch.empty((columns, n), dtype=kind, device=x.device)
+        dx = x.new_empty(x.shape, dtype=kind) if input_gradient else None
+        dweight = x.new_empty((columns, n), dtype=kind)
         dbias = torch.empty_like(bias) if bias is not None else None
         size = _entry(query)(rows, n, out, 1)
-        workspace = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+        workspace = x.new_empty(size, dtype=torch.uint8) if size else None
         _check(_entry(entry)(
             _TYPES[kind], pdy, dy_stride, px, x_stride, pw, w_stride, pp, p_stride,
             _TYPES[bias.dtype] if bias is not None else 0, act, rows, n, out, dx.data_ptr() if input_gradient else 0,
