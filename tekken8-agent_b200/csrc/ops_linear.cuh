@@ -51,14 +51,18 @@ constexpr int kMaxSplits = 64;
 
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Cycles of the busiest CTA as the plan's cost: waves x (k blocks x their MMA cycles + the tile's
-// latency), plus the pass that joins the parts (its traffic over the chip's, and its launch).
+// Cycles of the busiest CTA as the plan's cost: waves x (k blocks x cycles + the tile's latency), plus
+// the pass that joins the parts (its traffic over the chip's, and its launch). The cycles are fits to
+// measured products: a narrower tile costs nearly as many a k-block, because what the MMAs read from
+// shared memory bounds them, and less latency. 65,536 x 512 x 512 took 42.7 / 54.0 / 88.2 us by
+// 256 / 128 / 64 columns, 4,096 rows of it 12.4 / 10.5 / 12.2, 512 rows 10.8 / 10.5 / 8.4; its weight's
+// gradient 41 us in 18 parts, 318 in one.
 inline GemmPlan plan_gemm(int64_t m, int64_t n, int64_t k, bool may_split) {
     struct Form {
         int pair, bn;
         double block_cycles, tile_cycles;
     };
-    static constexpr Form forms[] = {{1, 256, 540, 3500}, {1, 128, 330, 2600}, {0, 64, 220, 2200}};
+    static constexpr Form forms[] = {{1, 256, 600, 4400}, {1, 128, 570, 2400}, {0, 64, 540, 720}};
     const int64_t k_blocks = ceil_div(k, tc::BK);
     GemmPlan best{1, 256, 1};
     double least = 1e300;
@@ -71,7 +75,7 @@ inline GemmPlan plan_gemm(int64_t m, int64_t n, int64_t k, bool may_split) {
             const int64_t splits = wave == 0 ? 1 : std::min<int64_t>(most, std::max<int64_t>(1, wave * workers / tiles));
             const double waves = static_cast<double>(ceil_div(tiles * splits, workers));
             double cost = waves * (static_cast<double>(ceil_div(k_blocks, splits)) * f.block_cycles + f.tile_cycles);
-            if (splits > 1) cost += 6000.0 + static_cast<double>(splits) * m * n * 8.0 / 2500.0;
+            if (splits > 1) cost += 4000.0 + static_cast<double>(splits) * m * n * 8.0 / 2500.0;
             if (cost < least) {
                 least = cost;
                 best = GemmPlan{f.pair, f.bn, static_cast<int>(splits)};
@@ -461,7 +465,7 @@ template <typename E, bool GATED, int V>
 constexpr int grad_ring_bytes() { return V == 8 ? kGradStages * (GATED ? 3 : 2) * 16 * 32 * kGradRows : 0; }
 
 template <typename E, bool GATED, int V>
-__global__ void __launch_bounds__(32 * kGradRows, 3)
+__global__ void __launch_bounds__(32 * kGradRows, V == 8 ? 3 : 5)
     k_activation_grad(const E* dy, int64_t dy_stride, const E* pre, int64_t pre_stride, int64_t rows, int columns,
                       int activation, E* dz, int64_t pitch, float* sums) {
     constexpr int PARTS = GATED ? 2 : 1;
@@ -506,24 +510,8 @@ __global__ void __launch_bounds__(32 * kGradRows, 3)
 #pragma unroll
                 for (int k = 0; k < kGradStages - 1; ++k) fetch(k, first + k * step < rows);
             }
-            int stage = 0;
-            for (int64_t row = first; row < rows; row += step) {
-                Pack<E, V> d, z{}, u{}, out, out_up;
-                if (RING) {
-                    fetch((stage + kGradStages - 1) % kGradStages, row + (kGradStages - 1) * step < rows);
-                    asm volatile("cp.async.wait_group %0;" ::"n"(kGradStages - 1) : "memory");
-                    const unsigned char* at = mine + stage * kStage;
-                    d = *reinterpret_cast<const Pack<E, V>*>(at);
-                    if (READS) z = *reinterpret_cast<const Pack<E, V>*>(at + 16 * kThreads);
-                    if (GATED) u = *reinterpret_cast<const Pack<E, V>*>(at + 32 * kThreads);
-                    stage = (stage + 1) % kGradStages;
-                } else {
-                    d = *reinterpret_cast<const Pack<E, V>*>(from_dy);
-                    if (READS) z = *reinterpret_cast<const Pack<E, V>*>(from_pre);
-                    if (GATED) u = *reinterpret_cast<const Pack<E, V>*>(from_pre + columns);
-                    from_dy += step * dy_stride;
-                    if (READS) from_pre += step * pre_stride;
-                }
+            auto use = [&](const Pack<E, V>& d, const Pack<E, V>& z, const Pack<E, V>& u) {
+                Pack<E, V> out, out_up;
 #pragma unroll
                 for (int j = 0; j < V; ++j) {
                     float value, slope;
@@ -543,6 +531,43 @@ __global__ void __launch_bounds__(32 * kGradRows, 3)
                     if (GATED) *reinterpret_cast<Pack<E, V>*>(to + columns) = out_up;
                     to += step * pitch;
                 }
+            };
+            int stage = 0;
+            int64_t row = first;
+            if (!RING) {  // four rows' elements in flight
+                constexpr int kBatch = 4;
+                for (; row + (kBatch - 1) * step < rows; row += kBatch * step) {
+                    Pack<E, V> d[kBatch], z[kBatch], u[kBatch];
+#pragma unroll
+                    for (int k = 0; k < kBatch; ++k) {
+                        d[k] = *reinterpret_cast<const Pack<E, V>*>(from_dy);
+                        z[k] = READS ? *reinterpret_cast<const Pack<E, V>*>(from_pre) : Pack<E, V>{};
+                        u[k] = GATED ? *reinterpret_cast<const Pack<E, V>*>(from_pre + columns) : Pack<E, V>{};
+                        from_dy += step * dy_stride;
+                        if (READS) from_pre += step * pre_stride;
+                    }
+#pragma unroll
+                    for (int k = 0; k < kBatch; ++k) use(d[k], z[k], u[k]);
+                }
+            }
+            for (; row < rows; row += step) {
+                Pack<E, V> d, z{}, u{};
+                if (RING) {
+                    fetch((stage + kGradStages - 1) % kGradStages, row + (kGradStages - 1) * step < rows);
+                    asm volatile("cp.async.wait_group %0;" ::"n"(kGradStages - 1) : "memory");
+                    const unsigned char* at = mine + stage * kStage;
+                    d = *reinterpret_cast<const Pack<E, V>*>(at);
+                    if (READS) z = *reinterpret_cast<const Pack<E, V>*>(at + 16 * kThreads);
+                    if (GATED) u = *reinterpret_cast<const Pack<E, V>*>(at + 32 * kThreads);
+                    stage = (stage + 1) % kGradStages;
+                } else {
+                    d = *reinterpret_cast<const Pack<E, V>*>(from_dy);
+                    if (READS) z = *reinterpret_cast<const Pack<E, V>*>(from_pre);
+                    if (GATED) u = *reinterpret_cast<const Pack<E, V>*>(from_pre + columns);
+                    from_dy += step * dy_stride;
+                    if (READS) from_pre += step * pre_stride;
+                }
+                use(d, z, u);
             }
             asm volatile("cp.async.wait_group 0;" ::: "memory");
         });
@@ -565,47 +590,59 @@ __global__ void __launch_bounds__(32 * kGradRows, 3)
     }
 }
 
-// dbias from the block rows' column sums, in a fixed order. Block (32, 16).
-static __global__ void k_bias_grad(const float* sums, int count, int columns, void* out, int type) {
-    __shared__ float joined[16][33];
-    const int c = blockIdx.x * 32 + threadIdx.x;
+// What the last pass of a backward adds up, in a fixed order: the parts of a split weight gradient
+// (rounded once), four columns a thread, and the block rows' column sums of dz (dbias), 32 columns a
+// block. The first `join_blocks` blocks do the one, the others the other. Block (32, 8).
+struct Totals {
+    const float* parts;
+    size_t part_elements;
+    int splits, pitch, rows, columns;
+    void* out;
+    int64_t stride;
+    unsigned join_blocks;
+    const float* sums;
+    int sums_rows, bias_columns;
+    void* dbias;
+    int bias_type;
+};
+template <typename E>
+__global__ void __launch_bounds__(256) k_totals(Totals a) {
+    if (blockIdx.x < a.join_blocks) {
+        const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.y * 32 + threadIdx.x;
+        const int pieces = a.pitch / 4;
+        if (i >= static_cast<int64_t>(a.rows) * pieces) return;
+        const int row = static_cast<int>(i / pieces), c = static_cast<int>(i % pieces) * 4;
+        const float* p = a.parts + static_cast<size_t>(row) * a.pitch + c;
+        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+        for (int s = 0; s < a.splits; ++s, p += a.part_elements) {
+            const float4 v = *reinterpret_cast<const float4*>(p);
+            sum.x += v.x;
+            sum.y += v.y;
+            sum.z += v.z;
+            sum.w += v.w;
+        }
+        const float v[4] = {sum.x, sum.y, sum.z, sum.w};
+        E* to = static_cast<E*>(a.out) + static_cast<int64_t>(row) * a.stride + c;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (c + j < a.columns) to[j] = Element<E>::store(v[j]);
+        }
+        return;
+    }
+    __shared__ float joined[8][33];
+    const int c = (blockIdx.x - a.join_blocks) * 32 + threadIdx.x;
     float v = 0.0f;
-    if (c < columns) {
-#pragma unroll 4
-        for (int r = threadIdx.y; r < count; r += 16) v += sums[static_cast<size_t>(r) * columns + c];
+    if (c < a.bias_columns) {
+#pragma unroll 8
+        for (int r = threadIdx.y; r < a.sums_rows; r += 8) v += a.sums[static_cast<size_t>(r) * a.bias_columns + c];
     }
     joined[threadIdx.y][threadIdx.x] = v;
     __syncthreads();
-    if (threadIdx.y != 0 || c >= columns) return;
+    if (threadIdx.y != 0 || c >= a.bias_columns) return;
 #pragma unroll
-    for (int r = 1; r < 16; ++r) v += joined[r][threadIdx.x];
-    store_any(out, type, c, v);
-}
-
-// The parts of a split GEMM, added in order and rounded once.
-template <typename E>
-__global__ void k_join_parts(const float* parts, int splits, size_t part_elements, int pitch, int rows, int columns, E* out,
-                             int64_t stride) {
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-    const int pieces = pitch / 4;
-    if (i >= static_cast<int64_t>(rows) * pieces) return;
-    const int row = static_cast<int>(i / pieces), c = static_cast<int>(i % pieces) * 4;
-    const float* p = parts + static_cast<size_t>(row) * pitch + c;
-    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-    for (int s = 0; s < splits; ++s, p += part_elements) {
-        const float4 v = *reinterpret_cast<const float4*>(p);
-        sum.x += v.x;
-        sum.y += v.y;
-        sum.z += v.z;
-        sum.w += v.w;
-    }
-    const float v[4] = {sum.x, sum.y, sum.z, sum.w};
-    E* to = out + static_cast<int64_t>(row) * stride + c;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        if (c + j < columns) to[j] = Element<E>::store(v[j]);
-    }
+    for (int r = 1; r < 8; ++r) v += joined[r][threadIdx.x];
+    store_any(a.dbias, a.bias_type, c, v);
 }
 
 // ------------------------------------------------------------------ host side
@@ -808,10 +845,11 @@ void linear_forward(const LinearCall& c) {
     }
 }
 
-// out [a.rows][b.rows] = A . B^T without bias or activation, in E; split k parts go through `parts`.
+// out [a.rows][b.rows] = A . B^T without bias or activation, in E; the parts of a split k go to
+// `parts`, and what is left to do to `totals`.
 template <typename E, int CG, int BN, bool A_MN>
 void product_tile(const char* label, const Matrix& a, const Matrix& b, int splits, void* out, int64_t stride, float* parts,
-                  cudaStream_t stream) {
+                  Totals* totals, cudaStream_t stream) {
     if (splits == 1) {
         using Epi = EpiLinear<E, E, BN, false>;
         Epi epi{};
@@ -826,20 +864,26 @@ void product_tile(const char* label, const Matrix& a, const Matrix& b, int split
         epi.y = tiled<float, Epi::kBytes>(parts, rows * splits, b.rows, pitch);
         epi.split_rows = static_cast<int>(rows);
         launch_gemm<E, CG, BN, A_MN, true>(label, a, b, b.rows, 0, splits, epi, stream);
-        launch("k_join_parts", k_join_parts<E>, blocks(a.rows * (pitch / 4), 256), 256, 0, stream, static_cast<const float*>(parts),
-               splits, static_cast<size_t>(rows) * pitch, static_cast<int>(pitch), static_cast<int>(a.rows),
-               static_cast<int>(b.rows), static_cast<E*>(out), stride);
+        totals->parts = parts;
+        totals->part_elements = static_cast<size_t>(rows) * pitch;
+        totals->splits = splits;
+        totals->pitch = static_cast<int>(pitch);
+        totals->rows = static_cast<int>(a.rows);
+        totals->columns = static_cast<int>(b.rows);
+        totals->out = out;
+        totals->stride = stride;
+        totals->join_blocks = blocks(a.rows * (pitch / 4), 256);
     }
 }
 template <typename E, bool A_MN>
 void product(const char* label, const Matrix& a, const Matrix& b, const GemmPlan& p, void* out, int64_t stride, float* parts,
-             cudaStream_t stream) {
+             Totals* totals, cudaStream_t stream) {
     if (p.bn == 256) {
-        product_tile<E, 2, 256, A_MN>(label, a, b, p.splits, out, stride, parts, stream);
+        product_tile<E, 2, 256, A_MN>(label, a, b, p.splits, out, stride, parts, totals, stream);
     } else if (p.bn == 128) {
-        product_tile<E, 2, 128, A_MN>(label, a, b, p.splits, out, stride, parts, stream);
+        product_tile<E, 2, 128, A_MN>(label, a, b, p.splits, out, stride, parts, totals, stream);
     } else {
-        product_tile<E, 1, 64, A_MN>(label, a, b, p.splits, out, stride, parts, stream);
+        product_tile<E, 1, 64, A_MN>(label, a, b, p.splits, out, stride, parts, totals, stream);
     }
 }
 
@@ -877,20 +921,27 @@ void linear_backward(const LinearGradCall& c) {
             wide ? activation_grad<E, false, 8>(c, dz_out, pitch, sums) : activation_grad<E, false, 1>(c, dz_out, pitch, sums);
         }
     }
-    if (sums) {
-        launch("k_bias_grad", k_bias_grad, blocks(columns, 32), dim3(32, 16), 0, c.stream, static_cast<const float*>(sums),
-               grad_parts(c.rows, columns), static_cast<int>(columns), c.dbias, c.bias_type);
-    }
+    Totals totals{};
     if (c.dx) {
         const Matrix w = operand<E>(c.weight, columns, c.in, c.weight_stride, c.workspace + at.weight, c.stream);
         product<E, false>("k_input_grad", dz, transposed(w), plan_gemm(c.rows, c.in, columns, false), c.dx, c.dx_stride, nullptr,
-                          c.stream);
+                          nullptr, c.stream);
     }
     if (c.dweight) {
         const Matrix x = operand<E>(c.x, c.rows, c.in, c.x_stride, c.workspace + at.x, c.stream);
         product<E, true>("k_weight_grad", transposed(dz), transposed(x), plan_gemm(columns, c.in, c.rows, true), c.dweight,
-                         c.dweight_stride, reinterpret_cast<float*>(c.workspace + at.parts), c.stream);
+                         c.dweight_stride, reinterpret_cast<float*>(c.workspace + at.parts), &totals, c.stream);
     }
+    unsigned grid = totals.join_blocks;
+    if (sums) {
+        totals.sums = sums;
+        totals.sums_rows = grad_parts(c.rows, columns);
+        totals.bias_columns = static_cast<int>(columns);
+        totals.dbias = c.dbias;
+        totals.bias_type = c.bias_type;
+        grid += blocks(columns, 32);
+    }
+    if (grid > 0) launch("k_totals", k_totals<E>, grid, dim3(32, 8), 0, c.stream, totals);
     check(cudaGetLastError(), "linear backward");
 }
 
