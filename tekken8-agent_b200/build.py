@@ -1,5 +1,7 @@
 """Builds the sm_100a shared library of the hot path (lib/libt8b.so) with nvcc.
 
+bindings/operators.cpp becomes the Python module t8b/_operators.so.
+
 Every .cu under csrc/ becomes one object; the engine translation unit is compiled with
 --fmad=false (a fused multiply-add would round once where the reference CPU engine rounds
 twice). Objects go to _build/ and are rebuilt when a source or header is newer.
@@ -17,6 +19,8 @@ ROOT = HERE.parent
 CSRC = HERE / "csrc"
 BUILD = HERE / "_build"
 LIB = HERE / "lib" / "libt8b.so"
+MODULE_SOURCE = HERE / "bindings" / "operators.cpp"
+MODULE = HERE / "t8b" / "_operators.so"
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 COMMON = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
@@ -28,6 +32,19 @@ EXTRA = {"sim.cu": ["--fmad=false"]}
 def _newest_header() -> float:
     headers = list(CSRC.glob("*.cuh")) + list((ROOT / "include").glob("*.h"))
     return max((h.stat().st_mtime for h in headers), default=0.0)
+
+
+def _module_command() -> list[str]:
+    """The Python module of the torso operators, against the installed torch's headers and libraries."""
+    import sysconfig
+    import torch
+    from torch.utils.cpp_extension import include_paths, library_paths
+    cuda = Path(NVCC).resolve().parent.parent
+    includes = [*include_paths(), str(cuda / "include"), sysconfig.get_paths()["include"], str(ROOT / "include")]
+    libraries = [flag for path in library_paths() for flag in (f"-L{path}", f"-Wl,-rpath,{path}")]
+    return ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+            *(f"-I{path}" for path in includes), str(MODULE_SOURCE), "-o", str(MODULE), *libraries,
+            "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
 
 
 def build(verbose: bool = False) -> Path:
@@ -44,6 +61,11 @@ def build(verbose: bool = False) -> Path:
         if verbose:
             print(" ".join(cmd), flush=True)
         commands.append(cmd)
+    header = ROOT / "include" / "t8b.h"
+    if not MODULE.exists() or MODULE.stat().st_mtime < max(MODULE_SOURCE.stat().st_mtime, header.stat().st_mtime):
+        commands.append(_module_command())
+        if verbose:
+            print(" ".join(commands[-1]), flush=True)
     with ThreadPoolExecutor(max_workers=os.cpu_count() or 1) as pool:
         for done in [pool.submit(subprocess.run, cmd, check=True) for cmd in commands]:
             done.result()
