@@ -86,20 +86,26 @@ struct Rows {
     static constexpr int kBytes = kRing ? NV * kPack : 0;  // of a thread and a stage
     const T* from;  // this thread's first element of the next row to fetch (or, without a ring, to get)
     int64_t step;   // elements to the row after it
-    int first, apart, n;  // its first column, and columns to its next pack
+    int first, apart, n;         // its first column, and columns to its next pack
+    uint32_t at[NV], bytes[NV];  // its packs: elements from `from`, and what of them the row has (the copy fills the rest with 0)
 
     __device__ __forceinline__ Rows(const void* base, int64_t stride, int64_t row, int64_t rows_apart, int t, int group, int columns)
-        : from(static_cast<const T*>(base) + row * stride + t * V), step(rows_apart * stride), first(t * V), apart(group * V), n(columns) {}
+        : from(static_cast<const T*>(base) + row * stride), step(rows_apart * stride), first(t * V), apart(group * V), n(columns) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const bool in = first + i * apart < n;
+            at[i] = in ? first + i * apart : 0;
+            bytes[i] = in ? kPack : 0;
+        }
+    }
     // slot: this thread's first pack in a stage, consecutive packs `pitch` bytes apart
     __device__ __forceinline__ void fetch(uint32_t slot, int pitch) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            if (first + i * apart < n) {
-                if constexpr (kPack == 16) {
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slot + i * pitch), "l"(from + i * apart) : "memory");
-                } else if constexpr (kRing) {
-                    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(slot + i * pitch), "l"(from + i * apart) : "memory");
-                }
+            if constexpr (kPack == 16) {
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(slot + i * pitch), "l"(from + at[i]), "r"(bytes[i]) : "memory");
+            } else if constexpr (kRing) {
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(slot + i * pitch), "l"(from + at[i]), "r"(bytes[i]) : "memory");
             }
         }
         from += step;
@@ -108,26 +114,29 @@ struct Rows {
         if constexpr (kRing) {
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                const bool in = first + i * apart < n;
                 if constexpr (sizeof(T) == 2) {
-                    Pack<uint32_t, V / 2> p;
-                    if (in) p = *reinterpret_cast<const Pack<uint32_t, V / 2>*>(slot + i * pitch);
+                    const Pack<uint32_t, V / 2> p = *reinterpret_cast<const Pack<uint32_t, V / 2>*>(slot + i * pitch);
 #pragma unroll
                     for (int j = 0; j < V / 2; ++j) {
-                        const float2 f = Element<T>::unpack(in ? p.v[j] : 0u);
+                        const float2 f = Element<T>::unpack(p.v[j]);
                         v[i * (V / 2) + j] = Two(f.x, f.y);
                     }
                 } else {
-                    Pack<float, V> p;
-                    if (in) p = *reinterpret_cast<const Pack<float, V>*>(slot + i * pitch);
+                    const Pack<float, V> p = *reinterpret_cast<const Pack<float, V>*>(slot + i * pitch);
 #pragma unroll
-                    for (int j = 0; j < V / 2; ++j) v[i * (V / 2) + j] = Two(in ? p.v[2 * j] : 0.0f, in ? p.v[2 * j + 1] : 0.0f);
+                    for (int j = 0; j < V / 2; ++j) v[i * (V / 2) + j] = Two(p.v[2 * j], p.v[2 * j + 1]);
                 }
             }
         } else {
+            T raw[NV];
             float f[NV];
 #pragma unroll
-            for (int i = 0; i < NV; ++i) f[i] = first + i * apart < n ? Element<T>::load(from[i * apart]) : 0.0f;
+            for (int i = 0; i < NV; ++i) {  // the loads first, all in flight
+                raw[i] = Element<T>::store(0.0f);
+                if (first + i * apart < n) raw[i] = from[first + i * apart];
+            }
+#pragma unroll
+            for (int i = 0; i < NV; ++i) f[i] = Element<T>::load(raw[i]);
 #pragma unroll
             for (int i = 0; i < NV / 2; ++i) v[i] = Two(f[2 * i], f[2 * i + 1]);
             from += step;
@@ -202,15 +211,26 @@ struct BackwardRing {
     static constexpr int kStages = ring_stages(kBytes);
 };
 
-// Where this thread stands: thread t of the `group` that shares a row, which is the `row`-th of
-// those that the block has in flight.
+// Where this thread stands: thread t of the `group` that shares a row, on the block's rows first,
+// first + step and so on, `mine` of them; the warp goes on for `turns` rows (a row of fewer than 32
+// lanes may end before its warp does: the sums take every lane).
 template <int G>
 struct Seat {
     static constexpr bool kWarp = G != 0;
-    int group, t, row, rows;
-    __device__ __forceinline__ Seat()
+    static constexpr int kPerWarp = kWarp ? 32 / (kWarp ? G : 1) : 1;
+    int group, t, row, rows, mine, turns;
+    int64_t first, step;
+    __device__ __forceinline__ explicit Seat(int64_t total)
         : group(kWarp ? G : blockDim.x), t(kWarp ? threadIdx.x % (kWarp ? G : 1) : threadIdx.x),
-          row(kWarp ? threadIdx.x / (kWarp ? G : 1) : 0), rows(kWarp ? blockDim.x / (kWarp ? G : 1) : 1) {}
+          row(kWarp ? threadIdx.x / (kWarp ? G : 1) : 0), rows(kWarp ? blockDim.x / (kWarp ? G : 1) : 1) {
+        first = static_cast<int64_t>(blockIdx.x) * rows + row;
+        step = static_cast<int64_t>(gridDim.x) * rows;
+        mine = count(first, total);
+        turns = count(first - row % kPerWarp, total);
+    }
+    __device__ __forceinline__ int count(int64_t from, int64_t total) const {
+        return from < total ? static_cast<int>((total - from + step - 1) / step) : 0;
+    }
 };
 
 template <typename TX, typename TY, int V, int G>
@@ -221,17 +241,15 @@ __global__ void __launch_bounds__(G ? 32 * kWarps : kBlockMax, G ? kForwardBlock
     extern __shared__ __align__(16) unsigned char ring[];
     __shared__ __align__(8) float shared[2][kBlockMax / 32][2];
     int turn = 0;
-    const Seat<G> seat;
-    const int64_t first = static_cast<int64_t>(blockIdx.x) * seat.rows + seat.row;
-    const int64_t step = static_cast<int64_t>(gridDim.x) * seat.rows;
-    Rows<TX, V, NV> x(a.x, a.x_stride, first, step, seat.t, seat.group, a.n);
+    const Seat<G> seat(a.rows);
+    Rows<TX, V, NV> x(a.x, a.x_stride, seat.first, seat.step, seat.t, seat.group, a.n);
     const int pitch = blockDim.x * V * static_cast<int>(sizeof(TX)), stage_bytes = blockDim.x * Ring::kBytes;
     const unsigned char* mine = ring + threadIdx.x * V * sizeof(TX);
     const uint32_t slot = static_cast<uint32_t>(__cvta_generic_to_shared(mine));
     if (Ring::kBytes) {
 #pragma unroll
         for (int k = 0; k < S - 1; ++k) {
-            if (first + k * step < a.rows) x.fetch(slot + k * stage_bytes, pitch);
+            if (k < seat.mine) x.fetch(slot + k * stage_bytes, pitch);
             ring_commit();
         }
     }
@@ -241,15 +259,16 @@ __global__ void __launch_bounds__(G ? 32 * kWarps : kBlockMax, G ? kForwardBlock
     const float scale = 1.0f / static_cast<float>(a.n);
     const bool whole = a.n == seat.group * kHeld;  // every thread holds as many elements as it can
     const int at = seat.t * V, apart = seat.group * V;
-    TY* y = static_cast<TY*>(a.y) + first * a.y_stride + at;
-    const int64_t y_step = step * a.y_stride;
+    TY* y = static_cast<TY*>(a.y) + seat.first * a.y_stride + at;
+    const int64_t y_step = seat.step * a.y_stride;
+    float* to_mean = a.mean ? a.mean + seat.first : nullptr;
+    float* to_rstd = a.rstd ? a.rstd + seat.first : nullptr;
     int stage = 0;
-    // lanes whose row is past the end go on with their warp (its sums take every lane) and store nothing
-    for (int64_t row = first; row - seat.row % (G && G < 32 ? 32 / (G ? G : 1) : 1) < a.rows; row += step, y += y_step) {
-        const bool live = row < a.rows;
+    for (int k = 0; k < seat.turns; ++k, y += y_step) {
+        const bool live = k < seat.mine;
         Two v[kHeld / 2];
         if (Ring::kBytes) {
-            if (row + (S - 1) * step < a.rows) x.fetch(slot + (stage == 0 ? S - 1 : stage - 1) * stage_bytes, pitch);
+            if (k + S - 1 < seat.mine) x.fetch(slot + (stage == 0 ? S - 1 : stage - 1) * stage_bytes, pitch);
             ring_commit();
             ring_wait<S - 1>();
         }
@@ -288,8 +307,8 @@ __global__ void __launch_bounds__(G ? 32 * kWarps : kBlockMax, G ? kForwardBlock
         if (!live) continue;
         store_row<TY, V, NV>(y, at, apart, a.n, v);
         if (seat.t == 0) {
-            if (a.mean) a.mean[row] = mean;
-            if (a.rstd) a.rstd[row] = rstd;
+            if (to_mean) to_mean[k * seat.step] = mean;
+            if (to_rstd) to_rstd[k * seat.step] = rstd;
         }
     }
     ring_wait<0>();
@@ -303,12 +322,10 @@ __global__ void __launch_bounds__(G ? 32 * kWarps : kBlockMax, G ? kBackwardBloc
     extern __shared__ __align__(16) unsigned char ring[];
     __shared__ __align__(8) float shared[2][kBlockMax / 32][2];
     int turn = 0;
-    const Seat<G> seat;
-    const int64_t first = static_cast<int64_t>(blockIdx.x) * seat.rows + seat.row;
-    const int64_t step = static_cast<int64_t>(gridDim.x) * seat.rows;
-    Rows<TX, V, NV> x(a.x, a.x_stride, first, step, seat.t, seat.group, a.n);
-    Rows<TX, V, NV> residual(a.residual, a.residual_stride, first, step, seat.t, seat.group, a.n);
-    Rows<TY, V, NV> dy(a.dy, a.dy_stride, first, step, seat.t, seat.group, a.n);
+    const Seat<G> seat(a.rows);
+    Rows<TX, V, NV> x(a.x, a.x_stride, seat.first, seat.step, seat.t, seat.group, a.n);
+    Rows<TX, V, NV> residual(a.residual, a.residual_stride, seat.first, seat.step, seat.t, seat.group, a.n);
+    Rows<TY, V, NV> dy(a.dy, a.dy_stride, seat.first, seat.step, seat.t, seat.group, a.n);
     const int x_pitch = blockDim.x * V * static_cast<int>(sizeof(TX)), dy_pitch = blockDim.x * V * static_cast<int>(sizeof(TY));
     const int stage_bytes = blockDim.x * Ring::kBytes;
     // a stage: x, residual, dy
@@ -317,9 +334,9 @@ __global__ void __launch_bounds__(G ? 32 * kWarps : kBlockMax, G ? kBackwardBloc
     const int residual_at = blockDim.x * Ring::kX;
     const uint32_t slot_x = static_cast<uint32_t>(__cvta_generic_to_shared(mine_x));
     const uint32_t slot_dy = static_cast<uint32_t>(__cvta_generic_to_shared(mine_dy));
-    auto fetch = [&](int stage, int64_t row) {
+    auto fetch = [&](int stage, bool any) {
         if (!Ring::kBytes) return;
-        if (row < a.rows) {
+        if (any) {
             x.fetch(slot_x + stage * stage_bytes, x_pitch);
             dy.fetch(slot_dy + stage * stage_bytes, dy_pitch);
             if (a.residual) residual.fetch(slot_x + residual_at + stage * stage_bytes, x_pitch);
@@ -327,26 +344,38 @@ __global__ void __launch_bounds__(G ? 32 * kWarps : kBlockMax, G ? kBackwardBloc
         ring_commit();
     };
 #pragma unroll
-    for (int k = 0; k < S - 1; ++k) fetch(k, first + k * step);
-    float next_mean = 0.0f, next_rstd = 0.0f;
-    if (first < a.rows) {
-        next_mean = a.mean[first];
-        next_rstd = a.rstd[first];
+    for (int k = 0; k < S - 1; ++k) fetch(k, k < seat.mine);
+    // the statistics of this row and the next two
+    const float* from_mean = a.mean + seat.first;
+    const float* from_rstd = a.rstd + seat.first;
+    float means[2] = {0.0f, 0.0f}, rstds[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        if (k < seat.mine) {
+            means[k] = from_mean[k * seat.step];
+            rstds[k] = from_rstd[k * seat.step];
+        }
     }
+    from_mean += 2 * seat.step;
+    from_rstd += 2 * seat.step;
     Two w[kHeld / 2], dw[kHeld / 2], db[kHeld / 2];
     load_parameter<V, NV>(a.weight, a.parameter_type, 1.0f, seat.t, seat.group, a.n, w);
     const float scale = 1.0f / static_cast<float>(a.n);
     const int at = seat.t * V, apart = seat.group * V;
-    TX* dx = static_cast<TX*>(a.y) + first * a.y_stride + at;
-    const int64_t dx_step = step * a.y_stride;
+    TX* dx = static_cast<TX*>(a.y) + seat.first * a.y_stride + at;
+    const int64_t dx_step = seat.step * a.y_stride;
     int stage = 0;
-    for (int64_t row = first; row - seat.row % (G && G < 32 ? 32 / (G ? G : 1) : 1) < a.rows; row += step, dx += dx_step) {
-        const bool live = row < a.rows;
-        fetch(stage == 0 ? S - 1 : stage - 1, row + (S - 1) * step);
-        const float mean = next_mean, rstd = next_rstd;
-        if (row + step < a.rows) {
-            next_mean = a.mean[row + step];
-            next_rstd = a.rstd[row + step];
+    for (int k = 0; k < seat.turns; ++k, dx += dx_step) {
+        const bool live = k < seat.mine;
+        fetch(stage == 0 ? S - 1 : stage - 1, k + S - 1 < seat.mine);
+        const float mean = means[0], rstd = rstds[0];
+        means[0] = means[1];
+        rstds[0] = rstds[1];
+        if (k + 2 < seat.mine) {
+            means[1] = *from_mean;
+            rstds[1] = *from_rstd;
+            from_mean += seat.step;
+            from_rstd += seat.step;
         }
         if (Ring::kBytes) ring_wait<S - 1>();
         Two v[kHeld / 2], g[kHeld / 2];
@@ -630,7 +659,7 @@ void dispatch(const Norm& a, int x_type, int y_type, bool backward, cudaStream_t
 }
 
 void check_sizes(int64_t rows, int64_t n) {
-    if (rows < 0) raise(T8B_EINVAL, "layer norm: a negative number of rows");
+    if (rows < 0 || rows > (1ll << 32)) raise(T8B_EINVAL, "layer norm: rows from 0 to 4294967296");
     if (n < 1 || n > (1 << 24)) raise(T8B_EINVAL, "layer norm: rows have 1 to 16777216 elements");
 }
 
