@@ -229,5 +229,27 @@ inline void allow_smem(Kernel kernel, size_t bytes, uint64_t& configured) {
     __atomic_fetch_or(&configured, bit, __ATOMIC_RELEASE);
 }
 
+// A launch in a chain of kernels of one call: with `chained` its blocks may start before the kernel
+// before it has ended, as soon as every block of that one has passed release_next(); they must call
+// wait_previous() before they touch what it writes, and before they end.
+template <typename Kernel, typename... Args>
+inline void launch_chain(const char* label, Kernel kernel, dim3 grid, dim3 block, size_t smem, cudaStream_t stream, bool chained,
+                         const Args&... args) {
+    LaunchScope scope(label, stream);
+    cudaLaunchConfig_t config{};
+    config.gridDim = grid;
+    config.blockDim = block;
+    config.dynamicSmemBytes = smem;
+    config.stream = stream;
+    cudaLaunchAttribute attribute[1];
+    attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute[0].val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = attribute;
+    config.numAttrs = chained ? 1 : 0;
+    check(cudaLaunchKernelEx(&config, kernel, args...), label);
+}
+__device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void release_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 }  // namespace op
 }  // namespace t8b

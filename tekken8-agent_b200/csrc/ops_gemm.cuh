@@ -244,9 +244,14 @@ struct Warp {
 // Polls a CTA that gives up makes for the loads it has in flight.
 constexpr uint32_t kDrainLimit = 1u << 18;
 
+// kInput: it writes what this kernel reads. kBeside: it does not, and this kernel's CTAs fill the SMs
+// that it leaves idle, but what came before it is this kernel's input too (all of that had ended
+// before any of its CTAs let this one start).
+enum { kNothing = 0, kInput = 1, kBeside = 2 };
 struct Shape {
     int tiles_m, tiles_n, splits, k_blocks;
     int second;  // B's second half starts at this row (gated projections); 0: B is one matrix
+    int after;   // what the kernel before this one in the chain is to it: kNothing, kInput or kBeside
     int* error;
 };
 
@@ -345,6 +350,8 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kGemmThreads, 1)
     __syncthreads();
     if (CG == 2) cluster_arrive_wait();  // the peer's barriers are initialised
     tc::fence_after();
+    if (s.after == kInput) wait_previous();
+    release_next();
     const uint32_t tmem = *tmem_slot;
     const int first = blockIdx.x / CG, step = gridDim.x / CG;
     auto stop = [&]() {
@@ -503,6 +510,7 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kGemmThreads, 1)
     tc::fence_before();
     __syncthreads();
     if (CG == 2) cluster_arrive_wait();  // no CTA of a pair ends while the other may still signal it
+    if (s.after == kBeside) wait_previous();  // the next kernel's wait for this one covers both
     if (warp == 2) {
         tc::fence_after();
         tmem_free<CG>(tmem, P::kTmemCols);

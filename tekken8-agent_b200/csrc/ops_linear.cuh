@@ -607,6 +607,7 @@ struct Totals {
 };
 template <typename E>
 __global__ void __launch_bounds__(256) k_totals(Totals a) {
+    wait_previous();
     if (blockIdx.x < a.join_blocks) {
         const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.y * 32 + threadIdx.x;
         const int pieces = a.pitch / 4;
@@ -694,8 +695,8 @@ struct Matrix {
 };
 
 template <typename E, int CG, int BN, bool A_MN, bool B_MN, class Epi>
-void launch_gemm(const char* label, const Matrix& a, const Matrix& b, int64_t columns, int second, int splits, const Epi& epi,
-                 cudaStream_t stream) {
+void launch_gemm(const char* label, const Matrix& a, const Matrix& b, int64_t columns, int second, int splits, int after,
+                 const Epi& epi, cudaStream_t stream) {
     using P = Plan<CG, BN>;
     auto kernel = k_gemm<E, CG, BN, A_MN, B_MN, Epi>;
     static uint64_t configured = 0;
@@ -706,6 +707,7 @@ void launch_gemm(const char* label, const Matrix& a, const Matrix& b, int64_t co
     s.k_blocks = static_cast<int>(ceil_div(a.k, tc::BK));
     s.splits = splits;
     s.second = second;
+    s.after = after;
     s.error = stall_flag();
     const auto k_major = [](const Matrix& m, uint32_t box) {
         return tensor_map<E>(m.data, m.k, m.rows, tma_pitch(m.rows, m.k, m.pitch, 2), tc::BK, box, CU_TENSOR_MAP_SWIZZLE_128B);
@@ -717,8 +719,7 @@ void launch_gemm(const char* label, const Matrix& a, const Matrix& b, int64_t co
     const CUtensorMap map_b = B_MN ? mn_major(b) : k_major(b, second ? BN / 2 : BN / CG);
     const int64_t work = static_cast<int64_t>(s.tiles_m) * s.tiles_n * s.splits;
     const int grid = static_cast<int>(std::min<int64_t>(work, CG == 2 ? kClusters : kSms)) * CG;
-    launch(label, kernel, grid, kGemmThreads, P::kSmemBytes, stream, map_a, map_b, s, epi);
-    check(cudaGetLastError(), label);
+    launch_chain(label, kernel, grid, kGemmThreads, P::kSmemBytes, stream, after != kNothing, map_a, map_b, s, epi);
 }
 
 // A matrix as a GEMM operand: where its rows do not suit TMA, a packed copy in the workspace.
@@ -748,7 +749,7 @@ void forward_tile(const LinearCall& c, const Matrix& x, const Matrix& w) {
     epi.activation = c.activation;
     epi.has_residual = c.residual != nullptr;
     epi.has_pre = c.pre != nullptr;
-    launch_gemm<E, CG, BN, false, false>("k_linear", x, w, c.out, 0, 1, epi, c.stream);
+    launch_gemm<E, CG, BN, false, false>("k_linear", x, w, c.out, 0, 1, kNothing, epi, c.stream);
 }
 template <typename E, int CG, int BN>
 void gated_tile(const LinearCall& c, const Matrix& x, const Matrix& w) {
@@ -763,7 +764,7 @@ void gated_tile(const LinearCall& c, const Matrix& x, const Matrix& w) {
     epi.bias_type = c.bias_type;
     epi.activation = c.activation;
     epi.has_pre = c.pre != nullptr;
-    launch_gemm<E, CG, BN, false, false>("k_gated", x, w, c.out, static_cast<int>(c.out), 1, epi, c.stream);
+    launch_gemm<E, CG, BN, false, false>("k_gated", x, w, c.out, static_cast<int>(c.out), 1, kNothing, epi, c.stream);
 }
 
 template <typename E, bool GATED, int R>
@@ -848,13 +849,13 @@ void linear_forward(const LinearCall& c) {
 // out [a.rows][b.rows] = A . B^T without bias or activation, in E; the parts of a split k go to
 // `parts`, and what is left to do to `totals`.
 template <typename E, int CG, int BN, bool A_MN>
-void product_tile(const char* label, const Matrix& a, const Matrix& b, int splits, void* out, int64_t stride, float* parts,
-                  Totals* totals, cudaStream_t stream) {
+void product_tile(const char* label, const Matrix& a, const Matrix& b, int splits, int after, void* out, int64_t stride,
+                  float* parts, Totals* totals, cudaStream_t stream) {
     if (splits == 1) {
         using Epi = EpiLinear<E, E, BN, false>;
         Epi epi{};
         epi.y = tiled<E, Epi::kBytes>(out, a.rows, b.rows, stride);
-        launch_gemm<E, CG, BN, A_MN, true>(label, a, b, b.rows, 0, 1, epi, stream);
+        launch_gemm<E, CG, BN, A_MN, true>(label, a, b, b.rows, 0, 1, after, epi, stream);
         return;
     }
     if constexpr (A_MN) {
@@ -863,7 +864,7 @@ void product_tile(const char* label, const Matrix& a, const Matrix& b, int split
         const int64_t rows = split_rows(a.rows), pitch = split_pitch(b.rows);
         epi.y = tiled<float, Epi::kBytes>(parts, rows * splits, b.rows, pitch);
         epi.split_rows = static_cast<int>(rows);
-        launch_gemm<E, CG, BN, A_MN, true>(label, a, b, b.rows, 0, splits, epi, stream);
+        launch_gemm<E, CG, BN, A_MN, true>(label, a, b, b.rows, 0, splits, after, epi, stream);
         totals->parts = parts;
         totals->part_elements = static_cast<size_t>(rows) * pitch;
         totals->splits = splits;
@@ -876,14 +877,14 @@ void product_tile(const char* label, const Matrix& a, const Matrix& b, int split
     }
 }
 template <typename E, bool A_MN>
-void product(const char* label, const Matrix& a, const Matrix& b, const GemmPlan& p, void* out, int64_t stride, float* parts,
-             Totals* totals, cudaStream_t stream) {
+void product(const char* label, const Matrix& a, const Matrix& b, const GemmPlan& p, int after, void* out, int64_t stride,
+             float* parts, Totals* totals, cudaStream_t stream) {
     if (p.bn == 256) {
-        product_tile<E, 2, 256, A_MN>(label, a, b, p.splits, out, stride, parts, totals, stream);
+        product_tile<E, 2, 256, A_MN>(label, a, b, p.splits, after, out, stride, parts, totals, stream);
     } else if (p.bn == 128) {
-        product_tile<E, 2, 128, A_MN>(label, a, b, p.splits, out, stride, parts, totals, stream);
+        product_tile<E, 2, 128, A_MN>(label, a, b, p.splits, after, out, stride, parts, totals, stream);
     } else {
-        product_tile<E, 1, 64, A_MN>(label, a, b, p.splits, out, stride, parts, totals, stream);
+        product_tile<E, 1, 64, A_MN>(label, a, b, p.splits, after, out, stride, parts, totals, stream);
     }
 }
 
@@ -921,15 +922,20 @@ void linear_backward(const LinearGradCall& c) {
             wide ? activation_grad<E, false, 8>(c, dz_out, pitch, sums) : activation_grad<E, false, 1>(c, dz_out, pitch, sums);
         }
     }
+    // operands that have to be packed first, so that the two products are neighbours in the chain
+    Matrix w{}, x{};
+    if (c.dx) w = operand<E>(c.weight, columns, c.in, c.weight_stride, c.workspace + at.weight, c.stream);
+    if (c.dweight) x = operand<E>(c.x, c.rows, c.in, c.x_stride, c.workspace + at.x, c.stream);
+    const bool packed = (c.dx && w.data != c.weight) || (c.dweight && x.data != c.x);
+    int after = dz_out || sums || packed ? kInput : kNothing;
     Totals totals{};
     if (c.dx) {
-        const Matrix w = operand<E>(c.weight, columns, c.in, c.weight_stride, c.workspace + at.weight, c.stream);
-        product<E, false>("k_input_grad", dz, transposed(w), plan_gemm(c.rows, c.in, columns, false), c.dx, c.dx_stride, nullptr,
-                          nullptr, c.stream);
+        product<E, false>("k_input_grad", dz, transposed(w), plan_gemm(c.rows, c.in, columns, false), after, c.dx, c.dx_stride,
+                          nullptr, nullptr, c.stream);
+        after = kBeside;
     }
     if (c.dweight) {
-        const Matrix x = operand<E>(c.x, c.rows, c.in, c.x_stride, c.workspace + at.x, c.stream);
-        product<E, true>("k_weight_grad", transposed(dz), transposed(x), plan_gemm(columns, c.in, c.rows, true), c.dweight,
+        product<E, true>("k_weight_grad", transposed(dz), transposed(x), plan_gemm(columns, c.in, c.rows, true), after, c.dweight,
                          c.dweight_stride, reinterpret_cast<float*>(c.workspace + at.parts), &totals, c.stream);
     }
     unsigned grid = totals.join_blocks;
@@ -941,7 +947,7 @@ void linear_backward(const LinearGradCall& c) {
         totals.bias_type = c.bias_type;
         grid += blocks(columns, 32);
     }
-    if (grid > 0) launch("k_totals", k_totals<E>, grid, dim3(32, 8), 0, c.stream, totals);
+    if (grid > 0) launch_chain("k_totals", k_totals<E>, grid, dim3(32, 8), 0, c.stream, true, totals);
     check(cudaGetLastError(), "linear backward");
 }
 
