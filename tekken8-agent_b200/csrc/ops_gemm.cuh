@@ -12,11 +12,15 @@
 //              bytes of both CTAs are counted by the first CTA's full[stage];
 //   warp 1     (first CTA) MMA issuer: commits each stage to empty[stage] of both CTAs, a finished
 //              accumulator to acc_full[buffer] of both;
-//   warps 2-17 epilogue: quarter = warp % 4 gives the 32 tensor-memory lanes (rows), group a
-//              quarter of the columns; each arrives once at the first CTA's acc_empty[buffer].
-//              An epilogue is a chain of latencies (tensor memory, special functions, staging,
-//              its store's reads), so 16 warps, and not 8, share a tile (see EpiGated).
-// Two accumulator buffers of BN columns let the epilogue of one tile overlap the MMAs of the next.
+//   warps 2-17 epilogue, in two sets of eight: a set takes every second tile, the one whose
+//              accumulator is its buffer. quarter = warp % 4 gives the 32 tensor-memory lanes (rows),
+//              group half of the columns; each warp arrives once at the first CTA's acc_empty.
+// Two accumulator buffers of BN columns let the epilogue of one tile overlap the MMAs of the next. An
+// epilogue is a chain of latencies (tensor memory, special functions, staging, its stores), so two
+// tiles' chains run side by side, and not sixteen warps on one: 75,776 x 512 to 2,816 columns took
+// 199 us with all warps on a tile and takes 188 (1,164 TFLOP/s; the library's product 187); without
+// any epilogue 147. At 2,048 in k it is 594 us (1,471 TFLOP/s, library 592), with the SMs' clock held
+// near 1.4 GHz by the power limit.
 // Operands are K-major (rows of K elements) or MN-major (K rows), see gemm.cuh.
 //
 // Every wait is bounded: a stall sets the error flag; the first CTA then waits (bounded) for the
@@ -31,7 +35,7 @@
 namespace t8b {
 namespace op {
 
-constexpr int kEpiWarps = 16;
+constexpr int kEpiWarps = 16, kSetWarps = 8;
 constexpr int kGemmThreads = 64 + 32 * kEpiWarps;
 constexpr int kStaging = 4096;  // an epilogue warp's staging: 32 rows of 128 bytes
 
@@ -134,26 +138,25 @@ struct Tiled {
     int tma;
 };
 
-// Sends a staging tile (rows row0.., columns col0.. of m) out, by TMA from one lane of the warp
-// that `issues`, else rows from r0 on in steps of `step`. The tile was written by this warp, or,
-// after a barrier, by the two of a pair; it may be written again after free_tiles() (TMA), or
-// after the callers have met (element by element).
-__device__ __forceinline__ void publish() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// Sends a staging tile (rows row0.., columns col0.. of m), written by all lanes, out: by TMA, or
+// element by element. The tile may be written again after free_tile().
 template <typename T, int BYTES>
-__device__ __forceinline__ void send(const Tiled& m, unsigned char* tile, int row0, int col0, int lane, bool issues = true,
-                                     int r0 = 0, int step = 1) {
+__device__ __forceinline__ void send(const Tiled& m, unsigned char* tile, int row0, int col0, int lane) {
     if (m.tma) {
-        if (issues && lane == 0) {
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) {
             if (row0 < m.rows && col0 < m.columns) tc::tma_store(&m.map, tile, col0, row0);
             tc::bulk_commit();
         }
         return;
     }
+    __syncwarp();
     constexpr int W = BYTES / sizeof(T);
     constexpr int kPer = 16 / sizeof(T);
     const int rows = min(32, m.rows - row0);
-    T* out = static_cast<T*>(m.data) + static_cast<int64_t>(row0 + r0) * m.stride + col0;
-    for (int r = r0; r < rows; r += step, out += step * m.stride) {
+    T* out = static_cast<T*>(m.data) + static_cast<int64_t>(row0) * m.stride + col0;
+    for (int r = 0; r < rows; ++r, out += m.stride) {
 #pragma unroll
         for (int c = lane; c < W; c += 32) {
             if (col0 + c < m.columns) out[c] = reinterpret_cast<const T*>(piece<BYTES>(tile, r, c / kPer))[c % kPer];
@@ -161,25 +164,10 @@ __device__ __forceinline__ void send(const Tiled& m, unsigned char* tile, int ro
     }
     __syncwarp();
 }
-// This lane's stores, all but the `pending` issued last, have read their staging tiles.
-template <int PENDING>
-__device__ __forceinline__ void wait_sent(int lane) {
-    if (lane == 0) {
-        if (PENDING == 0) tc::bulk_wait_read(); else tc::bulk_wait_read_all_but_one();
-    }
-}
-// The same for a warp that sends its own tiles: all its lanes may write them again.
-template <int PENDING>
-__device__ __forceinline__ void free_tiles(int lane) {
-    wait_sent<PENDING>(lane);
+// This warp's stores have read its staging tile.
+__device__ __forceinline__ void free_tile(int lane) {
+    if (lane == 0) tc::bulk_wait_read();
     __syncwarp();
-}
-// A warp's own tile, written by all lanes, goes out.
-template <typename T, int BYTES>
-__device__ __forceinline__ void send_own(const Tiled& m, unsigned char* tile, int row0, int col0, int lane) {
-    if (m.tma) publish();
-    __syncwarp();
-    send<T, BYTES>(m, tile, row0, col0, lane);
 }
 
 // Fetches a tile of m into a free staging tile; by TMA it arrives on `bar` (lane 0 waits).
@@ -205,19 +193,17 @@ __device__ __forceinline__ void fetch(const Tiled& m, unsigned char* tile, uint6
     __syncwarp();
 }
 
-// What an epilogue sees: one warp of a tile. The warps of groups 2j and 2j + 1 with the same
-// quarter are a pair; their stagings lie side by side.
+// What an epilogue sees: one warp of a tile.
 struct Warp {
-    int row0;              // first of the warp's 32 rows
-    int tn;                // the tile's index along the columns
-    int split, group, lane, pair;
-    uint32_t taddr;        // the warp's lanes of the tile's accumulator
-    unsigned char* tiles;  // its staging, kStaging bytes
-    float* vector;         // 32 floats for a bias
-    uint64_t* bar;         // a fetch's arrival
-    uint32_t phase;        // its parity
-    bool in_flight;        // a fetch not waited for yet
-    int turn;              // tiles sent so far, where an epilogue alternates between two
+    int row0;             // first of the warp's 32 rows
+    int tn;               // the tile's index along the columns
+    int split, group, lane;
+    uint32_t taddr;       // the warp's lanes of the tile's accumulator
+    unsigned char* tile;  // its staging, kStaging bytes
+    float* vector;        // 32 floats for a bias
+    uint64_t* bar;        // a fetch's arrival
+    uint32_t phase;       // its parity
+    bool in_flight;       // a fetch not waited for yet
     volatile int* abort;
 
     // the fetch has arrived
@@ -226,18 +212,6 @@ struct Warp {
         phase ^= 1u;
         in_flight = false;
         return ok;
-    }
-    // the two warps of the pair meet (both always do: see the vote in k_gemm)
-    __device__ __forceinline__ void meet() const { asm volatile("bar.sync %0, 64;" ::"r"(1 + pair) : "memory"); }
-    // whether both say yes
-    __device__ __forceinline__ bool vote(bool yes) const {
-        uint32_t both;
-        asm volatile(
-            "{\n .reg .pred p, q;\n setp.ne.u32 q, %2, 0;\n bar.red.and.pred p, %1, 64, q;\n selp.u32 %0, 1, 0, p;\n}\n"
-            : "=r"(both)
-            : "r"(1 + pair), "r"(yes ? 1u : 0u)
-            : "memory");
-        return both != 0;
     }
 };
 
@@ -339,7 +313,7 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kGemmThreads, 1)
         }
         for (int i = 0; i < 2; ++i) {
             tc::bar_init(acc_full + i, 1);
-            tc::bar_init(acc_empty + i, CG * kEpiWarps);
+            tc::bar_init(acc_empty + i, CG * kSetWarps);
         }
         for (int i = 0; i < kEpiWarps; ++i) tc::bar_init(fetched + i, 1);
         *abort = 0;
@@ -454,37 +428,34 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kGemmThreads, 1)
             }
         }
     } else {
-        const int e = warp - 2, quarter = warp & 3;
+        const int e = warp - 2, quarter = warp & 3, acc = e / kSetWarps;
         Warp w;
-        w.group = e >> 2;
+        w.group = (e >> 2) & 1;
         w.lane = lane;
-        w.pair = quarter * 2 + (w.group >> 1);
-        w.tiles = epi_tiles + (w.pair * 2 + (w.group & 1)) * kStaging;
+        w.tile = epi_tiles + e * kStaging;
         w.vector = vectors + e * 32;
         w.bar = fetched + e;
         w.phase = 0;
         w.in_flight = false;
-        w.turn = 0;
         w.abort = abort;
-        int acc = 0;
+        w.taddr = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * BN);
         uint32_t acc_phase = 0;
-        bool good = true;
-        for (Walk t(s, first, step); t.more(); t.next()) {
+        Walk t(s, first, step);
+        if (acc == 1) t.next();
+        for (; t.more() && !*abort; t.next(), t.next(), acc_phase ^= 1u) {
             w.row0 = (t.tm * CG + rank) * tc::BM + quarter * 32;
             w.tn = t.tn;
             w.split = t.split;
-            w.taddr = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * BN);
-            bool ok = good && !*abort;
-            if (ok) {
-                epi.begin(w);
-                ok = tc::bar_wait(acc_full + acc, acc_phase, abort);
-            }
-            if (!w.vote(ok)) {  // the warps of a pair go on, or stop, together
+            epi.begin(w);
+            if (!tc::bar_wait(acc_full + acc, acc_phase, abort)) {
                 stop();
                 break;
             }
             tc::fence_after();
-            good = epi.finish(w);
+            if (!epi.finish(w)) {
+                stop();
+                break;
+            }
             tc::fence_before();
             __syncwarp();
             if (lane == 0) {
@@ -495,12 +466,7 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kGemmThreads, 1)
                                  : "memory");
                 }
             }
-            if (++acc == 2) {
-                acc = 0;
-                acc_phase ^= 1u;
-            }
         }
-        if (!good) stop();
         for (uint32_t n = 0; w.in_flight && n < kDrainLimit && !tc::bar_try(w.bar, w.phase); ++n) {  // after a stall
         }
         if (lane == 0) tc::bulk_wait();  // this warp's stores have landed

@@ -189,33 +189,33 @@ __device__ __forceinline__ void add_bias32(float* vector, float mine, int lane, 
 }
 
 // y = activation(acc + bias) + residual in the type O, and acc + bias as `pre`; without FULL, acc
-// alone (gradients, and the fp32 parts of a split GEMM). A group of epilogue warps takes a quarter
-// of the tile's columns (at least one chunk) in chunks of a 128-byte row (64 where a tile of 64
-// columns has no more): stores of 64-byte rows took 158 us where 128-byte rows take 130 (75,776 x 128
-// times 2,816 x 128, where stores are most of the work). A chunk's residual is fetched into
-// the staging tile while the MMAs run; y replaces it, then `pre`, read again from tensor memory.
+// alone (gradients, and the fp32 parts of a split GEMM). A group of epilogue warps takes half of the
+// tile's columns in chunks of a 128-byte row (64 where a tile of 64 columns has no more): stores of
+// 64-byte rows took 158 us where 128-byte rows take 130 (75,776 x 128 times 2,816 x 128, where stores
+// are most of the work), one store for four warps' rows 147. A chunk's residual is fetched into the
+// staging tile, the first one's while the MMAs run; y replaces it, then `pre`, read again from
+// tensor memory.
 template <typename E, typename O, int BN, bool FULL>
 struct EpiLinear {
     static constexpr int kWide = sizeof(O) == 2 && BN >= 128 ? 64 : 32;  // columns of a chunk
     static constexpr int kBytes = kWide * sizeof(O);
     static constexpr int kPreBytes = kWide * 2;
-    static constexpr int kColumns = BN / 4 < kWide ? kWide : BN / 4;  // of a group
+    static constexpr int kColumns = BN / 2;  // of a group
     static constexpr int kChunks = kColumns / kWide;
     Tiled y, residual, pre;
     const void* bias;
     int bias_type, activation, has_residual, has_pre, split_rows;
 
     __device__ __forceinline__ int column(const Warp& w, int chunk) const { return w.tn * BN + w.group * kColumns + chunk * kWide; }
-    __device__ __forceinline__ bool idle(const Warp& w) const { return w.row0 >= y.rows || w.group * kColumns >= BN; }
     __device__ __forceinline__ void fetch_chunk(Warp& w, int chunk) const {
         const int col = column(w, chunk);
         if (chunk >= kChunks || col >= y.columns) return;
-        free_tiles<0>(w.lane);
-        fetch<O, kBytes>(residual, w.tiles, w.bar, w.row0, col, w.lane);
+        free_tile(w.lane);
+        fetch<O, kBytes>(residual, w.tile, w.bar, w.row0, col, w.lane);
         w.in_flight = residual.tma;
     }
     __device__ __forceinline__ void begin(Warp& w) const {
-        if (FULL && has_residual && !idle(w)) fetch_chunk(w, 0);
+        if (FULL && has_residual && w.row0 < y.rows) fetch_chunk(w, 0);
     }
     // 32 columns of acc + bias
     __device__ __forceinline__ void load(const Warp& w, int chunk, int at, float (&v)[32]) const {
@@ -225,7 +225,7 @@ struct EpiLinear {
         if (FULL && bias != nullptr) add_bias32(w.vector, b, w.lane, v);
     }
     __device__ __forceinline__ bool finish(Warp& w) const {
-        if (idle(w)) return true;
+        if (w.row0 >= y.rows) return true;
         const int row0 = w.row0 + w.split * split_rows;
 #pragma unroll 1
         for (int chunk = 0; chunk < kChunks; ++chunk) {
@@ -234,7 +234,7 @@ struct EpiLinear {
             if (FULL && has_residual) {
                 if (residual.tma && !w.wait()) return false;
             } else {
-                free_tiles<0>(w.lane);
+                free_tile(w.lane);
             }
 #pragma unroll
             for (int at = 0; at < kWide; at += 32) {
@@ -245,20 +245,20 @@ struct EpiLinear {
 #pragma unroll
                         for (int k = 0; k < 32; ++k) v[k] = activate<decltype(act)::value>(v[k]);
                     });
-                    if (has_residual) add32<O, kBytes>(w.tiles, w.lane, at, v);
+                    if (has_residual) add32<O, kBytes>(w.tile, w.lane, at, v);
                 }
-                stage32<O, kBytes>(w.tiles, w.lane, at, v);
+                stage32<O, kBytes>(w.tile, w.lane, at, v);
             }
-            send_own<O, kBytes>(y, w.tiles, row0, col, w.lane);
+            send<O, kBytes>(y, w.tile, row0, col, w.lane);
             if (FULL && has_pre) {
-                free_tiles<0>(w.lane);
+                free_tile(w.lane);
 #pragma unroll 1
                 for (int at = 0; at < kWide; at += 32) {
                     float v[32];
                     load(w, chunk, at, v);
-                    stage32<E, kPreBytes>(w.tiles, w.lane, at, v);
+                    stage32<E, kPreBytes>(w.tile, w.lane, at, v);
                 }
-                send_own<E, kPreBytes>(pre, w.tiles, row0, col, w.lane);
+                send<E, kPreBytes>(pre, w.tile, row0, col, w.lane);
             }
             if (FULL && has_residual) fetch_chunk(w, chunk + 1);
         }
@@ -267,69 +267,60 @@ struct EpiLinear {
 };
 
 // h = activation(gate) up; the accumulator's first BN / 2 columns are the gate's, the others the
-// up projection's of the same columns of h. A warp takes 32 columns of h; the two of a pair stage
-// theirs side by side in tiles of 64 columns (128-byte rows, see EpiLinear), of which the pair has
-// two: gate and up go out through one each, h through the gate's once its store has read it.
+// up projection's of the same columns of h. A warp takes 64 columns of h (32 where a tile has no
+// more) as one staging tile: h goes out through it, then gate and up, each read again from tensor
+// memory, once the store before has read it.
 template <typename E, int BN>
 struct EpiGated {
     static constexpr int kHalf = BN / 2;
-    static constexpr bool kPaired = kHalf >= 64;
-    static constexpr int kBytes = kPaired ? 128 : 64;
+    static constexpr int kWide = kHalf >= 128 ? 64 : 32;  // columns of a warp
+    static constexpr int kBytes = kWide * 2;
     Tiled h, gate, up;
     const void* bias;
     int bias_type, activation, has_pre;
 
-    __device__ __forceinline__ void meet(const Warp& w) const {
-        if (kPaired) w.meet(); else __syncwarp();
-    }
-    __device__ __forceinline__ void put(const Tiled& m, const Warp& w, unsigned char* tile, int col, bool issues, const float (&v)[32]) const {
-        stage32<E, kBytes>(tile, w.lane, kPaired ? (w.group & 1) * 32 : 0, v);
-        if (m.tma) publish();
-        meet(w);
-        send<E, kBytes>(m, tile, w.row0, col, w.lane, issues, kPaired ? w.group & 1 : 0, kPaired ? 2 : 1);
-        if (!m.tma) meet(w);
-    }
     __device__ __forceinline__ void begin(Warp&) const {}
+    // 32 columns of acc + bias of the gate (part 0) or the up projection (1), from column `at` of the warp's
+    __device__ __forceinline__ void load(const Warp& w, int part, int at, float (&v)[32]) const {
+        const int column = w.group * kWide + at;
+        float b = 0.0f;
+        if (bias != nullptr) {
+            const int c = w.tn * kHalf + column + w.lane;
+            if (c < h.columns) b = load_any(bias, bias_type, part * h.columns + c);
+        }
+        tc::tmem_load32(w.taddr + part * kHalf + column, v);
+        if (bias != nullptr) add_bias32(w.vector, b, w.lane, v);
+    }
     __device__ __forceinline__ bool finish(Warp& w) const {
-        const int first = w.group * 32;                                                // this warp's columns of the tile
-        const int together = kPaired ? (w.group >> 1) * 64 : first;                    // and the pair's
-        const int col = w.tn * kHalf + together, mine = w.tn * kHalf + first + w.lane;
-        if (w.row0 >= h.rows || together >= kHalf || col >= h.columns) return true;    // the same for both of a pair
-        const bool issues = !kPaired || (w.group & 1) == 0;
-        unsigned char* tile = w.tiles - (kPaired && !issues ? kStaging : 0);
-        unsigned char* other = tile + (kPaired ? kStaging : kStaging / 2);
-        float g[32], u[32];
-        float bg = 0.0f, bu = 0.0f;
-        if (bias != nullptr && mine < h.columns) {
-            bg = load_any(bias, bias_type, mine);
-            bu = load_any(bias, bias_type, h.columns + mine);
-        }
-        tc::tmem_load32(w.taddr + first, g);
-        if (bias != nullptr) add_bias32(w.vector, bg, w.lane, g);
-        if (has_pre) {
-            if (issues) wait_sent<0>(w.lane);
-            meet(w);
-            put(gate, w, tile, col, issues, g);
-        }
-        with_activation(activation, [&](auto act) {
+        const int col = w.tn * kHalf + w.group * kWide;
+        if (w.row0 >= h.rows || w.group * kWide >= kHalf || col >= h.columns) return true;
+        free_tile(w.lane);
+#pragma unroll 1
+        for (int at = 0; at < kWide; at += 32) {
+            float g[32], u[32];
+            load(w, 0, at, g);
+            with_activation(activation, [&](auto act) {
 #pragma unroll
-            for (int k = 0; k < 32; ++k) g[k] = activate<decltype(act)::value>(g[k]);
-        });
-        tc::tmem_load32(w.taddr + kHalf + first, u);
-        if (bias != nullptr) add_bias32(w.vector, bu, w.lane, u);
-        if (has_pre) {
-            put(up, w, other, col, issues, u);
-            if (issues) {
-                if (up.tma) wait_sent<1>(w.lane); else wait_sent<0>(w.lane);  // the gate's tile
+                for (int k = 0; k < 32; ++k) g[k] = activate<decltype(act)::value>(g[k]);
+            });
+            load(w, 1, at, u);
+#pragma unroll
+            for (int k = 0; k < 32; ++k) g[k] *= u[k];
+            stage32<E, kBytes>(w.tile, w.lane, at, g);
+        }
+        send<E, kBytes>(h, w.tile, w.row0, col, w.lane);
+        if (!has_pre) return true;
+#pragma unroll 1
+        for (int part = 0; part < 2; ++part) {
+            free_tile(w.lane);
+#pragma unroll
+            for (int at = 0; at < kWide; at += 32) {
+                float v[32];
+                load(w, part, at, v);
+                stage32<E, kBytes>(w.tile, w.lane, at, v);
             }
-        } else {
-            if ((w.turn++ & 1) != 0) tile = other;
-            if (issues) wait_sent<1>(w.lane);  // the tile sent before last
+            send<E, kBytes>(part ? up : gate, w.tile, w.row0, col, w.lane);
         }
-#pragma unroll
-        for (int k = 0; k < 32; ++k) g[k] *= u[k];
-        meet(w);
-        put(h, w, tile, col, issues, g);
         return true;
     }
 };
