@@ -327,19 +327,31 @@ struct EpiGated {
 
 // ------------------------------------------------------------------ elementwise kernels
 // Rows of `in` with any stride, copied to rows of `pitch` (a multiple of 8) elements: operands whose
-// rows do not start on 16-byte boundaries, which TMA asks for. One 16-byte piece a thread.
+// rows do not start on 16-byte boundaries, which TMA asks for. One 16-byte piece a thread; both
+// operands of a product in one launch.
+struct PackJob {
+    const void* in;
+    void* out;
+    int64_t stride, rows, pitch;
+    int columns;
+};
 template <typename E>
-__global__ void k_pack(const E* in, int64_t stride, int64_t rows, int columns, E* out, int pitch) {
-    const int pieces = pitch / 8;
-    const int64_t total = rows * pieces;
+__global__ void k_pack(PackJob first, PackJob second) {
+    const int64_t pieces = first.rows * (first.pitch / 8), total = pieces + second.rows * (second.pitch / 8);
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
          i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-        const int64_t row = i / pieces;
-        const int c = static_cast<int>(i - row * pieces) * 8;
+        const PackJob& job = i < pieces ? first : second;
+        const int64_t at = i < pieces ? i : i - pieces;
+        const int64_t row = at / (job.pitch / 8);
+        const int c = static_cast<int>(at - row * (job.pitch / 8)) * 8;
+        const E* in = static_cast<const E*>(job.in) + row * job.stride + c;
         Pack<E, 8> p;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) p.v[j] = c + j < columns ? in[row * stride + c + j] : Element<E>::store(0.0f);
-        *reinterpret_cast<Pack<E, 8>*>(out + row * pitch + c) = p;
+        for (int j = 0; j < 8; ++j) {
+            p.v[j] = Element<E>::store(0.0f);
+            if (c + j < job.columns) p.v[j] = in[j];
+        }
+        *reinterpret_cast<Pack<E, 8>*>(static_cast<E*>(job.out) + row * job.pitch + c) = p;
     }
 }
 
@@ -713,15 +725,23 @@ void launch_gemm(const char* label, const Matrix& a, const Matrix& b, int64_t co
     launch_chain(label, kernel, grid, kGemmThreads, P::kSmemBytes, stream, after != kNothing, map_a, map_b, s, epi);
 }
 
-// A matrix as a GEMM operand: where its rows do not suit TMA, a packed copy in the workspace.
+// A matrix as a GEMM operand: where its rows do not suit TMA, a copy in the workspace, which pack()
+// makes.
 template <typename E>
-Matrix operand(const void* data, int64_t rows, int64_t columns, int64_t stride, unsigned char* copy, cudaStream_t stream) {
+Matrix operand(const void* data, int64_t rows, int64_t columns, int64_t stride, unsigned char* copy, PackJob& job) {
     if (tma_rows(data, rows, stride, sizeof(E))) return Matrix{data, rows, columns, tma_pitch(rows, columns, stride, sizeof(E))};
-    const int64_t pitch = round_up(columns, 8);
-    const int64_t pieces = rows * (pitch / 8);
-    launch("k_pack", k_pack<E>, static_cast<unsigned>(std::min<int64_t>(ceil_div(pieces, 256), kSms * 16)), 256, 0, stream,
-           static_cast<const E*>(data), stride, rows, static_cast<int>(columns), reinterpret_cast<E*>(copy), static_cast<int>(pitch));
-    return Matrix{copy, rows, columns, pitch};
+    job = PackJob{data, copy, stride, rows, static_cast<int64_t>(round_up(columns, 8)), static_cast<int>(columns)};
+    return Matrix{copy, rows, columns, job.pitch};
+}
+// Whether there was anything to pack.
+template <typename E>
+bool pack(const PackJob (&jobs)[2], cudaStream_t stream) {
+    const int64_t pieces = (jobs[0].rows * jobs[0].pitch + jobs[1].rows * jobs[1].pitch) / 8;
+    if (pieces == 0) return false;
+    launch("k_pack", k_pack<E>, static_cast<unsigned>(std::min<int64_t>(ceil_div(pieces, 256), kSms * 16)), 256, 0, stream, jobs[0],
+           jobs[1]);
+    check(cudaGetLastError(), "pack operands");
+    return true;
 }
 // [rows][k] read along its rows' other axis: the same storage as an MN-major operand.
 inline Matrix transposed(const Matrix& m) { return Matrix{m.data, m.k, m.rows, m.pitch}; }
@@ -807,8 +827,10 @@ void linear_forward(const LinearCall& c) {
         return;
     }
     const Workspace at(c.rows, c.in, columns);
-    const Matrix x = operand<E>(c.x, c.rows, c.in, c.x_stride, c.workspace + at.x, c.stream);
-    const Matrix w = operand<E>(c.weight, columns, c.in, c.weight_stride, c.workspace + at.weight, c.stream);
+    PackJob jobs[2]{};
+    const Matrix x = operand<E>(c.x, c.rows, c.in, c.x_stride, c.workspace + at.x, jobs[0]);
+    const Matrix w = operand<E>(c.weight, columns, c.in, c.weight_stride, c.workspace + at.weight, jobs[1]);
+    pack<E>(jobs, c.stream);
     const GemmPlan p = plan_gemm(c.rows, columns, c.in, false);
     if (c.gated) {
         if (p.bn == 256) {
@@ -913,11 +935,12 @@ void linear_backward(const LinearGradCall& c) {
             wide ? activation_grad<E, false, 8>(c, dz_out, pitch, sums) : activation_grad<E, false, 1>(c, dz_out, pitch, sums);
         }
     }
-    // operands that have to be packed first, so that the two products are neighbours in the chain
+    // operands are packed first, so that the two products are neighbours in the chain
+    PackJob jobs[2]{};
     Matrix w{}, x{};
-    if (c.dx) w = operand<E>(c.weight, columns, c.in, c.weight_stride, c.workspace + at.weight, c.stream);
-    if (c.dweight) x = operand<E>(c.x, c.rows, c.in, c.x_stride, c.workspace + at.x, c.stream);
-    const bool packed = (c.dx && w.data != c.weight) || (c.dweight && x.data != c.x);
+    if (c.dx) w = operand<E>(c.weight, columns, c.in, c.weight_stride, c.workspace + at.weight, jobs[0]);
+    if (c.dweight) x = operand<E>(c.x, c.rows, c.in, c.x_stride, c.workspace + at.x, jobs[1]);
+    const bool packed = pack<E>(jobs, c.stream);
     int after = dz_out || sums || packed ? kInput : kNothing;
     Totals totals{};
     if (c.dx) {
