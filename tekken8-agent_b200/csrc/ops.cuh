@@ -248,6 +248,10 @@ inline void launch_chain(const char* label, Kernel kernel, dim3 grid, dim3 block
     config.numAttrs = chained ? 1 : 0;
     check(cudaLaunchKernelEx(&config, kernel, args...), label);
 }
+// What the kernel before it in a chain is to a kernel. kInput: it writes what this one reads. kBeside:
+// it does not, and this one's blocks fill the SMs that it leaves idle, but what came before it is this
+// one's input too (all of that had ended before any of its blocks let this one start).
+enum { kNothing = 0, kInput = 1, kBeside = 2 };
 __device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void release_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

@@ -229,10 +229,6 @@ __device__ __forceinline__ bool wait_idle(uint64_t* bar, uint32_t parity, volati
 // Polls a CTA that gives up makes for the loads it has in flight.
 constexpr uint32_t kDrainLimit = 1u << 18;
 
-// kInput: it writes what this kernel reads. kBeside: it does not, and this kernel's CTAs fill the SMs
-// that it leaves idle, but what came before it is this kernel's input too (all of that had ended
-// before any of its CTAs let this one start).
-enum { kNothing = 0, kInput = 1, kBeside = 2 };
 struct Shape {
     int tiles_m, tiles_n, splits, k_blocks;
     int second;  // B's second half starts at this row (gated projections); 0: B is one matrix

@@ -336,7 +336,7 @@ struct PackJob {
     int columns;
 };
 template <typename E>
-__global__ void k_pack(PackJob first, PackJob second) {
+__global__ void k_pack(PackJob first, PackJob second, int after) {
     const int64_t pieces = first.rows * (first.pitch / 8), total = pieces + second.rows * (second.pitch / 8);
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
          i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
@@ -353,6 +353,7 @@ __global__ void k_pack(PackJob first, PackJob second) {
         }
         *reinterpret_cast<Pack<E, 8>*>(static_cast<E*>(job.out) + row * job.pitch + c) = p;
     }
+    if (after == kBeside) wait_previous();  // the next kernel's wait for this one covers both
 }
 
 // A forward pass of few rows: a warp per output column (or per gate and up column), its lanes over
@@ -471,6 +472,7 @@ template <typename E, bool GATED, int V>
 __global__ void __launch_bounds__(32 * kGradRows, V == 8 ? 3 : 5)
     k_activation_grad(const E* dy, int64_t dy_stride, const E* pre, int64_t pre_stride, int64_t rows, int columns,
                       int activation, E* dz, int64_t pitch, float* sums) {
+    release_next();  // operands may be packed beside it
     constexpr int PARTS = GATED ? 2 : 1;
     constexpr bool RING = V == 8;
     constexpr int kThreads = 32 * kGradRows;
@@ -735,19 +737,18 @@ Matrix operand(const void* data, int64_t rows, int64_t columns, int64_t stride, 
 }
 // Whether there was anything to pack.
 template <typename E>
-bool pack(const PackJob (&jobs)[2], cudaStream_t stream) {
+bool pack(const PackJob (&jobs)[2], int after, cudaStream_t stream) {
     const int64_t pieces = (jobs[0].rows * jobs[0].pitch + jobs[1].rows * jobs[1].pitch) / 8;
     if (pieces == 0) return false;
-    launch("k_pack", k_pack<E>, static_cast<unsigned>(std::min<int64_t>(ceil_div(pieces, 256), kSms * 16)), 256, 0, stream, jobs[0],
-           jobs[1]);
-    check(cudaGetLastError(), "pack operands");
+    launch_chain("k_pack", k_pack<E>, static_cast<unsigned>(std::min<int64_t>(ceil_div(pieces, 256), kSms * 16)), 256, 0, stream,
+                 after != kNothing, jobs[0], jobs[1], after);
     return true;
 }
 // [rows][k] read along its rows' other axis: the same storage as an MN-major operand.
 inline Matrix transposed(const Matrix& m) { return Matrix{m.data, m.k, m.rows, m.pitch}; }
 
 template <typename E, typename O, int CG, int BN>
-void forward_tile(const LinearCall& c, const Matrix& x, const Matrix& w) {
+void forward_tile(const LinearCall& c, const Matrix& x, const Matrix& w, int after) {
     using Epi = EpiLinear<E, O, BN, true>;
     Epi epi{};
     epi.y = tiled<O, Epi::kBytes>(c.y, c.rows, c.out, c.y_stride);
@@ -760,10 +761,10 @@ void forward_tile(const LinearCall& c, const Matrix& x, const Matrix& w) {
     epi.activation = c.activation;
     epi.has_residual = c.residual != nullptr;
     epi.has_pre = c.pre != nullptr;
-    launch_gemm<E, CG, BN, false, false>("k_linear", x, w, c.out, 0, 1, kNothing, epi, c.stream);
+    launch_gemm<E, CG, BN, false, false>("k_linear", x, w, c.out, 0, 1, after, epi, c.stream);
 }
 template <typename E, int CG, int BN>
-void gated_tile(const LinearCall& c, const Matrix& x, const Matrix& w) {
+void gated_tile(const LinearCall& c, const Matrix& x, const Matrix& w, int after) {
     using Epi = EpiGated<E, BN>;
     Epi epi{};
     epi.h = tiled<E, Epi::kBytes>(c.y, c.rows, c.out, c.y_stride);
@@ -775,7 +776,7 @@ void gated_tile(const LinearCall& c, const Matrix& x, const Matrix& w) {
     epi.bias_type = c.bias_type;
     epi.activation = c.activation;
     epi.has_pre = c.pre != nullptr;
-    launch_gemm<E, CG, BN, false, false>("k_gated", x, w, c.out, static_cast<int>(c.out), 1, kNothing, epi, c.stream);
+    launch_gemm<E, CG, BN, false, false>("k_gated", x, w, c.out, static_cast<int>(c.out), 1, after, epi, c.stream);
 }
 
 template <typename E, bool GATED, int R>
@@ -830,31 +831,31 @@ void linear_forward(const LinearCall& c) {
     PackJob jobs[2]{};
     const Matrix x = operand<E>(c.x, c.rows, c.in, c.x_stride, c.workspace + at.x, jobs[0]);
     const Matrix w = operand<E>(c.weight, columns, c.in, c.weight_stride, c.workspace + at.weight, jobs[1]);
-    pack<E>(jobs, c.stream);
+    const int after = pack<E>(jobs, kNothing, c.stream) ? kInput : kNothing;
     const GemmPlan p = plan_gemm(c.rows, columns, c.in, false);
     if (c.gated) {
         if (p.bn == 256) {
-            gated_tile<E, 2, 256>(c, x, w);
+            gated_tile<E, 2, 256>(c, x, w, after);
         } else if (p.bn == 128) {
-            gated_tile<E, 2, 128>(c, x, w);
+            gated_tile<E, 2, 128>(c, x, w, after);
         } else {
-            gated_tile<E, 1, 64>(c, x, w);
+            gated_tile<E, 1, 64>(c, x, w, after);
         }
     } else if (c.y_type == T8B_F32) {
         if (p.bn == 256) {
-            forward_tile<E, float, 2, 256>(c, x, w);
+            forward_tile<E, float, 2, 256>(c, x, w, after);
         } else if (p.bn == 128) {
-            forward_tile<E, float, 2, 128>(c, x, w);
+            forward_tile<E, float, 2, 128>(c, x, w, after);
         } else {
-            forward_tile<E, float, 1, 64>(c, x, w);
+            forward_tile<E, float, 1, 64>(c, x, w, after);
         }
     } else {
         if (p.bn == 256) {
-            forward_tile<E, E, 2, 256>(c, x, w);
+            forward_tile<E, E, 2, 256>(c, x, w, after);
         } else if (p.bn == 128) {
-            forward_tile<E, E, 2, 128>(c, x, w);
+            forward_tile<E, E, 2, 128>(c, x, w, after);
         } else {
-            forward_tile<E, E, 1, 64>(c, x, w);
+            forward_tile<E, E, 1, 64>(c, x, w, after);
         }
     }
 }
@@ -940,7 +941,7 @@ void linear_backward(const LinearGradCall& c) {
     Matrix w{}, x{};
     if (c.dx) w = operand<E>(c.weight, columns, c.in, c.weight_stride, c.workspace + at.weight, jobs[0]);
     if (c.dweight) x = operand<E>(c.x, c.rows, c.in, c.x_stride, c.workspace + at.x, jobs[1]);
-    const bool packed = pack<E>(jobs, c.stream);
+    const bool packed = pack<E>(jobs, dz_out || sums ? kBeside : kNothing, c.stream);
     int after = dz_out || sums || packed ? kInput : kNothing;
     Totals totals{};
     if (c.dx) {

@@ -449,6 +449,7 @@ __global__ void __launch_bounds__(G ? 32 * kWarps : kBlockMax, G ? kBackwardBloc
 
 // dw and db from the blocks' sums, in a fixed order. Block (32, kPartialRows): 32 columns.
 __global__ void k_norm_parameters(const float* partial, int count, int n, void* dw, void* db, int type) {
+    wait_previous();
     __shared__ float sums[kPartialRows][33];
     void* out = blockIdx.y ? db : dw;
     if (out == nullptr) return;
@@ -757,9 +758,9 @@ extern "C" int t8b_layer_norm_backward(const void* dy, int y_type, int64_t dy_st
         a.parameter_type = parameter_type;
         dispatch(a, x_type, y_type, true, st);
         if (parameters) {
-            launch("k_norm_parameters", k_norm_parameters, dim3(blocks(n, 32), 2), dim3(32, kPartialRows), 0, st,
-                   static_cast<const float*>(workspace), backward_blocks(rows, n, multiprocessors()), a.n, dweight, dbias,
-                   parameter_type);
+            launch_chain("k_norm_parameters", k_norm_parameters, dim3(blocks(n, 32), 2), dim3(32, kPartialRows), 0, st, true,
+                         static_cast<const float*>(workspace), backward_blocks(rows, n, multiprocessors()), a.n, dweight, dbias,
+                         parameter_type);
         }
         check(cudaGetLastError(), "layer norm launch");
     });
