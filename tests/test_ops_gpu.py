@@ -364,6 +364,17 @@ def test_gradients_against_differences(cuda, name):
         assert abs(float((got.double() * way).sum()) - want) <= 4 * 2 ** -8 * float((got.double() * way).abs().sum())
 
 
+@pytest.mark.parametrize("n", [130, 512, 515, 1001])
+def test_layer_norm_in_place(cuda, n):
+    """y may be x itself, rows that share packs included."""
+    import torch
+    from t8b import _lib, ops
+    x = torch.randn(3000, n, device="cuda").bfloat16()
+    want = ops.layer_norm(x)
+    status = _lib.lib().t8b_layer_norm_forward(x.data_ptr(), 1, n, 0, 0, 0, 1e-5, 3000, n, x.data_ptr(), 1, n, 0, 0, None)
+    assert status == 0 and torch.equal(x, want)
+
+
 def test_infinities_and_nan_stay_in_their_rows(cuda):
     import torch
     from t8b import ops
