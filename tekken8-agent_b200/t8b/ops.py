@@ -7,7 +7,8 @@ stride between them (a column range of a wider buffer is fine). Matrix operands 
 both of one type; a bias is fp32 or of that type; norms take fp32 too. Outputs are new tensors. Work
 is queued on `stream` (a torch.cuda.Stream; torch's current stream by default), where inputs must be
 ready, and outputs and workspaces belong to that stream as torch's own do. A call of the wrong types
-or shapes raises ValueError before anything is queued.
+or shapes raises ValueError before anything is queued. Nothing is recorded for automatic
+differentiation: the gradients are the *_backward functions.
 
 The checks and allocations are the module _operators (bindings/operators.cpp, built by build.py).
 """
