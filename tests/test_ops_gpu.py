@@ -364,6 +364,59 @@ def test_gradients_against_differences(cuda, name):
         assert abs(float((got.double() * way).sum()) - want) <= 4 * 2 ** -8 * float((got.double() * way).abs().sum())
 
 
+def tail64(t, rows):
+    return t[-rows:].double()
+
+
+def test_offsets_past_32_bits(cuda):
+    """Matrices of more than 2^31 elements: their last rows against the formulas."""
+    import torch
+    from t8b import ops
+    E, k = torch.bfloat16, 5
+    g = torch.Generator(device="cuda").manual_seed(3)
+
+    def normal(rows, n, scale=1.0):
+        t = torch.empty(rows, n, device="cuda", dtype=E)
+        t.normal_(0.0, scale, generator=g)
+        return t
+
+    x = normal(4_300_001, 512)
+    y, mean, rstd = ops.layer_norm(x, save=True)
+    want, m, r, xhat, slip, _ = norm64(x[-k:], None, None)
+    close(y[-k:], want, 2 ** -17 * slip)
+    dy = normal(4_300_001, 512)
+    dx, _, _ = ops.layer_norm_backward(dy, x, None, None, mean, rstd)
+    d = tail64(dy, k)
+    ref = r * (d - d.mean(-1, keepdim=True) - xhat * (d * xhat).mean(-1, keepdim=True))
+    close(dx[-k:], ref, 2 ** -16 * r * (d.abs() + d.abs().mean(-1, keepdim=True) + slip * (d * slip).abs().mean(-1, keepdim=True)))
+    del y, dx, dy
+    w = normal(40, 512, 512 ** -0.5)
+    close(ops.linear(x, w)[-k:], *linear64(x[-k:], w, None))
+    del x
+    x, w = normal(1_200_003, 64), normal(2048, 64, 0.125)
+    y, pre = ops.gated(x, w, activation="relu", save=True)
+    z, slip = linear64(x[-k:], w, None)
+    close(pre[-k:], z, slip, "pre")
+    dh = normal(1_200_003, 1024, 0.125)
+    dx, dw, _ = ops.gated_backward(dh, x, w, None, pre, activation="relu")
+    dz, _ = backward64(dh[-k:], x[-k:], w, pre[-k:], "relu", True)
+    mags = dz.abs() @ w.double().abs()
+    close(dx[-k:], dz @ w.double(), (unit(E) * (1 + 2 ** -8) + (2048 + 16) * 2.0 ** -23) * mags, "dx")
+    total = torch.zeros(2048, 64, dtype=torch.float64, device="cuda")
+    size = torch.zeros_like(total)
+    for at in range(0, x.shape[0], 100_000):
+        rows = slice(at, at + 100_000)
+        part, _ = backward64(dh[rows], x[rows], w, pre[rows], "relu", True)
+        total += part.T @ x[rows].double()
+        size += part.abs().T @ x[rows].double().abs()
+    close(dw, total, (unit(E) * (1 + 2 ** -8) + (x.shape[0] + 16) * 2.0 ** -23) * size, "dweight")
+    del y, pre, dh, dx, x
+    x, w = normal(1, 32768), normal(70_001, 32768, 32768 ** -0.5)
+    z, slip = linear64(x, w[-k:], None)
+    close(ops.linear(x, w)[:, -k:], z, slip)
+    ops.status()
+
+
 @pytest.mark.parametrize("n", [130, 512, 515, 1001])
 def test_layer_norm_in_place(cuda, n):
     """y may be x itself, rows that share packs included."""
