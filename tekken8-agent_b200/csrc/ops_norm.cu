@@ -4,11 +4,11 @@
 //   dx = rstd (g - sum(g)/n - xhat sum(g xhat)/n) + residual gradient,   g = dy w,  xhat = (x - mean) rstd
 //   dw = sum over rows of dy xhat,   db = sum over rows of dy
 //
-// Bound by memory: a pass reads x (and dy) once and writes y (or dx) once. A row of up to 128, 256
-// or 512 elements belongs to 8, 16 or 32 lanes of a warp and lies in their registers, 16 elements a
-// lane; a longer one (to 8,192) to one block, 16 elements a thread. The statistics are two passes over those registers
-// (the mean, then the squares of the differences), so no row is read twice and no variance is a
-// difference of large sums. The grid is persistent: a lane keeps its columns' parameters, and in
+// Bound by memory: a pass reads x (and dy) once and writes y (or dx) once. A row of up to 128, 256,
+// 512 or 1,024 elements belongs to 8, 16 or 32 lanes of a warp and lies in their registers, 16 or 32
+// elements a lane; a longer one (to 8,192) to one block, 32 elements a thread. The statistics are two
+// passes over those registers (the mean, then the squares of the differences), so no row is read
+// twice and no variance is a difference of large sums. The grid is persistent: a lane keeps its columns' parameters, and in
 // the backward pass its columns' sums of dw and db, in registers over all the rows its warp takes;
 // the blocks' sums are joined in a fixed order by k_norm_parameters, so results repeat bit for bit.
 // Rows of more than 8,192 elements go through the k_wide_* kernels, which read a row again from L2.
@@ -21,15 +21,23 @@ namespace t8b {
 namespace op {
 namespace {
 
-constexpr int kHeld = 16;        // elements of a row that one thread holds
-constexpr int kWarps = 8;        // warps (rows in flight) of a block in the warp form
-constexpr int kBlockMax = 512;   // threads of a block in the block form
-constexpr int kPartialRows = 16; // rows of threads in k_norm_parameters
-// Resident blocks of the warp form: as many as its registers allow (a lane holds w, b and the next
-// row forward; w, dw, db and a row of each input backward).
-constexpr int kForwardBlocks = 2, kBackwardBlocks = 2;
-// Threads that share a row of n elements, 16 a thread: 8, 16 or 32 lanes, or a block of them.
-constexpr int group_of(int64_t n) { return n <= 8 * kHeld ? 8 : n <= 16 * kHeld ? 16 : n <= 32 * kHeld ? 32 : 0; }
+constexpr int kWarps = 8;          // warps of a block of the forms that give a row to lanes of one warp
+constexpr int kThreads = 32 * kWarps;  // and the most threads of a block that shares a row
+constexpr int kMostColumns = 32 * kThreads;
+constexpr int kWideThreads = 512;  // threads of a block in the forms for rows beyond that
+constexpr int kPartialRows = 16;   // rows of threads in k_norm_parameters
+// How a row of n elements is shared: by 8, 16 or 32 lanes that hold 16 elements each, by 32 lanes that
+// hold 32 (kLong), or by a block whose threads hold 32 (0). The more a thread holds, the fewer
+// instructions and barriers an element costs; at 16 elements two blocks of the backward pass are
+// resident, at 32 one. 65,536 x 768 in bf16, 32 lanes by 32 against a block by 16: forward 37 / 57 us,
+// backward 64 / 79; 8,192 x 8,192, a block by 32 against by 16: 51 / 73, 90 / 96.
+constexpr int kLong = 64;
+constexpr int group_of(int64_t n) { return n <= 128 ? 8 : n <= 256 ? 16 : n <= 512 ? 32 : n <= 1024 ? kLong : 0; }
+__host__ __device__ constexpr int lanes_of(int group) { return group == kLong ? 32 : group; }
+__host__ __device__ constexpr int held_of(int group) { return group == kLong || group == 0 ? 32 : 16; }
+// Resident blocks: as many as the registers allow (a thread holds w, b and a row forward; w, dw, db and
+// two rows backward).
+__host__ __device__ constexpr int resident_blocks(int group, bool backward) { return backward && held_of(group) == 32 ? 1 : 2; }
 
 struct Norm {
     const void* x;
@@ -50,7 +58,7 @@ struct Norm {
 // Sums over the row's threads: G lanes of a warp, or (G = 0) the block with one barrier (shared
 // values alternate between two buffers, so the barrier of the next sum protects those of this one).
 template <int G, int COUNT>
-__device__ __forceinline__ void row_sum(float (&v)[COUNT], float (*shared)[kBlockMax / 32][2], int& turn) {
+__device__ __forceinline__ void row_sum(float (&v)[COUNT], float (*shared)[kWideThreads / 32][2], int& turn) {
 #pragma unroll
     for (int o = (G ? G : 32) / 2; o >= 1; o >>= 1) {
 #pragma unroll
@@ -255,14 +263,15 @@ struct Seat {
 };
 
 template <typename TX, typename TY, int V, bool SHIFT, int G>
-__global__ void __launch_bounds__(G ? 32 * kWarps : kBlockMax, G ? kForwardBlocks : 1) k_norm_forward(Norm a) {
-    constexpr int NV = kHeld / V;
+__global__ void __launch_bounds__(kThreads, resident_blocks(G, false)) k_norm_forward(Norm a) {
+    constexpr int HELD = held_of(G), LANES = lanes_of(G);
+    constexpr int NV = HELD / V;
     using Ring = ForwardRing<TX, V, NV>;
     constexpr int S = Ring::kStages;
     extern __shared__ __align__(16) unsigned char ring[];
-    __shared__ __align__(8) float shared[2][kBlockMax / 32][2];
+    __shared__ __align__(8) float shared[2][kWideThreads / 32][2];
     int turn = 0;
-    const Seat<G> seat(a.rows);
+    const Seat<LANES> seat(a.rows);
     const int at = seat.t * V - (SHIFT ? static_cast<int>(seat.first % V * a.shift % V) : 0), apart = seat.group * V;
     Rows<TX, V, NV, SHIFT> x(a.x, a.x_stride, seat.first, seat.step, at, apart, a.n);
     const int pitch = blockDim.x * V * static_cast<int>(sizeof(TX)), stage_bytes = blockDim.x * Ring::kBytes;
@@ -275,11 +284,11 @@ __global__ void __launch_bounds__(G ? 32 * kWarps : kBlockMax, G ? kForwardBlock
             ring_commit();
         }
     }
-    Two w[kHeld / 2], b[kHeld / 2];
+    Two w[HELD / 2], b[HELD / 2];
     load_parameter<V, NV>(a.weight, a.parameter_type, 1.0f, at, apart, a.n, w);
     load_parameter<V, NV>(a.bias, a.parameter_type, 0.0f, at, apart, a.n, b);
     const float scale = 1.0f / static_cast<float>(a.n);
-    const bool whole = !SHIFT && a.n == seat.group * kHeld;  // every thread holds as many elements as it can
+    const bool whole = !SHIFT && a.n == seat.group * HELD;  // every thread holds as many elements as it can
     TY* y = static_cast<TY*>(a.y) + seat.first * a.y_stride;
     const int64_t y_step = seat.step * a.y_stride;
     const auto outside = [&](int e) {  // whether held element e is not the row's
@@ -291,7 +300,7 @@ __global__ void __launch_bounds__(G ? 32 * kWarps : kBlockMax, G ? kForwardBlock
     int stage = 0;
     for (int k = 0; k < seat.turns; ++k, y += y_step) {
         const bool live = k < seat.mine;
-        Two v[kHeld / 2];
+        Two v[HELD / 2];
         if (Ring::kBytes) {
             if (k + S - 1 < seat.mine) x.fetch(slot + (stage == 0 ? S - 1 : stage - 1) * stage_bytes, pitch);
             ring_commit();
@@ -301,21 +310,21 @@ __global__ void __launch_bounds__(G ? 32 * kWarps : kBlockMax, G ? kForwardBlock
         stage = stage == S - 1 ? 0 : stage + 1;
         Two total;
 #pragma unroll
-        for (int i = 0; i < kHeld / 2; ++i) total = total + v[i];
+        for (int i = 0; i < HELD / 2; ++i) total = total + v[i];
         float sum[1] = {total.sum()};
-        row_sum<G>(sum, shared, turn);
+        row_sum<LANES>(sum, shared, turn);
         const float mean = sum[0] * scale;
         const Two off(-mean, -mean);
         Two squared;
         if (whole) {
 #pragma unroll
-            for (int i = 0; i < kHeld / 2; ++i) {
+            for (int i = 0; i < HELD / 2; ++i) {
                 v[i] = v[i] + off;
                 squared = multiply_add(v[i], v[i], squared);
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < kHeld / 2; ++i) {
+            for (int i = 0; i < HELD / 2; ++i) {
                 float2 d = (v[i] + off).get();
                 if (outside(2 * i)) d.x = 0.0f;
                 if (outside(2 * i + 1)) d.y = 0.0f;
@@ -324,11 +333,11 @@ __global__ void __launch_bounds__(G ? 32 * kWarps : kBlockMax, G ? kForwardBlock
             }
         }
         float squares[1] = {squared.sum()};
-        row_sum<G>(squares, shared, turn);
+        row_sum<LANES>(squares, shared, turn);
         const float rstd = rsqrtf(squares[0] * scale + a.epsilon);
         const Two scaled(rstd, rstd);
 #pragma unroll
-        for (int i = 0; i < kHeld / 2; ++i) v[i] = multiply_add(v[i] * scaled, w[i], b[i]);
+        for (int i = 0; i < HELD / 2; ++i) v[i] = multiply_add(v[i] * scaled, w[i], b[i]);
         if (!live) continue;
         store_row<TY, V, NV, SHIFT>(y, at, apart, a.n, v);
         if (seat.t == 0) {
@@ -340,14 +349,15 @@ __global__ void __launch_bounds__(G ? 32 * kWarps : kBlockMax, G ? kForwardBlock
 }
 
 template <typename TX, typename TY, int V, bool SHIFT, int G>
-__global__ void __launch_bounds__(G ? 32 * kWarps : kBlockMax, G ? kBackwardBlocks : 1) k_norm_backward(Norm a) {
-    constexpr int NV = kHeld / V;
+__global__ void __launch_bounds__(kThreads, resident_blocks(G, true)) k_norm_backward(Norm a) {
+    constexpr int HELD = held_of(G), LANES = lanes_of(G);
+    constexpr int NV = HELD / V;
     using Ring = BackwardRing<TX, TY, V, NV>;
     constexpr int S = Ring::kStages;
     extern __shared__ __align__(16) unsigned char ring[];
-    __shared__ __align__(8) float shared[2][kBlockMax / 32][2];
+    __shared__ __align__(8) float shared[2][kWideThreads / 32][2];
     int turn = 0;
-    const Seat<G> seat(a.rows);
+    const Seat<LANES> seat(a.rows);
     const int at = seat.t * V - (SHIFT ? static_cast<int>(seat.first % V * a.shift % V) : 0), apart = seat.group * V;
     Rows<TX, V, NV, SHIFT> x(a.x, a.x_stride, seat.first, seat.step, at, apart, a.n);
     Rows<TX, V, NV, SHIFT> residual(a.residual, a.residual_stride, seat.first, seat.step, at, apart, a.n);
@@ -384,7 +394,7 @@ __global__ void __launch_bounds__(G ? 32 * kWarps : kBlockMax, G ? kBackwardBloc
     }
     from_mean += 2 * seat.step;
     from_rstd += 2 * seat.step;
-    Two w[kHeld / 2], dw[kHeld / 2], db[kHeld / 2];
+    Two w[HELD / 2], dw[HELD / 2], db[HELD / 2];
     load_parameter<V, NV>(a.weight, a.parameter_type, 1.0f, at, apart, a.n, w);
     const float scale = 1.0f / static_cast<float>(a.n);
     TX* dx = static_cast<TX*>(a.y) + seat.first * a.y_stride;
@@ -403,7 +413,7 @@ __global__ void __launch_bounds__(G ? 32 * kWarps : kBlockMax, G ? kBackwardBloc
             from_rstd += seat.step;
         }
         if (Ring::kBytes) ring_wait<S - 1>();
-        Two v[kHeld / 2], g[kHeld / 2];
+        Two v[HELD / 2], g[HELD / 2];
         if (live) {
             x.get(mine_x + stage * stage_bytes, x_pitch, v);
             dy.get(mine_dy + stage * stage_bytes, dy_pitch, g);
@@ -412,7 +422,7 @@ __global__ void __launch_bounds__(G ? 32 * kWarps : kBlockMax, G ? kBackwardBloc
         {
             const Two off(-mean, -mean), scaled(rstd, rstd);
 #pragma unroll
-            for (int i = 0; i < kHeld / 2; ++i) {
+            for (int i = 0; i < HELD / 2; ++i) {
                 v[i] = (v[i] + off) * scaled;  // beyond the row dy is 0, and so is all that v adds
                 if (live) dw[i] = multiply_add(g[i], v[i], dw[i]);
                 db[i] = db[i] + g[i];
@@ -422,16 +432,16 @@ __global__ void __launch_bounds__(G ? 32 * kWarps : kBlockMax, G ? kBackwardBloc
             }
         }
         float sum[2] = {of_g.sum(), of_gx.sum()};
-        row_sum<G>(sum, shared, turn);
+        row_sum<LANES>(sum, shared, turn);
         if (live) {
             const float c0 = -rstd * (sum[0] * scale), c1 = -rstd * (sum[1] * scale);
             const Two of_one(c0, c0), of_x(c1, c1), of_dy(rstd, rstd);
 #pragma unroll
-            for (int i = 0; i < kHeld / 2; ++i) v[i] = multiply_add(g[i], of_dy, multiply_add(v[i], of_x, of_one));
+            for (int i = 0; i < HELD / 2; ++i) v[i] = multiply_add(g[i], of_dy, multiply_add(v[i], of_x, of_one));
             if (a.residual) {
                 residual.get(mine_x + residual_at + stage * stage_bytes, x_pitch, g);
 #pragma unroll
-                for (int i = 0; i < kHeld / 2; ++i) v[i] = v[i] + g[i];
+                for (int i = 0; i < HELD / 2; ++i) v[i] = v[i] + g[i];
             }
             store_row<TX, V, NV, SHIFT>(dx, at, apart, a.n, v);
         }
@@ -441,14 +451,14 @@ __global__ void __launch_bounds__(G ? 32 * kWarps : kBlockMax, G ? kBackwardBloc
     if (a.partial == nullptr) return;
     float* out = a.partial + static_cast<size_t>(blockIdx.x) * a.n;
     if (G) {
-        // the rows' sums meet in shared memory, over the ring: [rows of the block][group kHeld]
+        // the rows' sums meet in shared memory, over the ring: [rows of the block][group HELD]
         float* joined = reinterpret_cast<float*>(ring);
-        const int width = G * kHeld;
+        const int width = LANES * HELD;
 #pragma unroll
         for (int which = 0; which < 2; ++which, out += static_cast<size_t>(gridDim.x) * a.n) {
             __syncthreads();
 #pragma unroll
-            for (int i = 0; i < kHeld; ++i) {
+            for (int i = 0; i < HELD; ++i) {
                 const float2 pair = (which ? db[i / 2] : dw[i / 2]).get();
                 const int c = at + (i / V) * apart + i % V;
                 if (c >= 0 && c < a.n) joined[seat.row * width + c] = i % 2 ? pair.y : pair.x;
@@ -462,7 +472,7 @@ __global__ void __launch_bounds__(G ? 32 * kWarps : kBlockMax, G ? kBackwardBloc
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < kHeld; ++i) {
+        for (int i = 0; i < HELD; ++i) {
             const int c = at + (i / V) * apart + i % V;
             const float2 w2 = dw[i / 2].get(), b2 = db[i / 2].get();
             if (c >= 0 && c < a.n) {
@@ -495,30 +505,30 @@ __global__ void k_norm_parameters(const float* partial, int count, int n, void* 
 }
 
 // ------------------------------------------------------------------ rows beyond 8,192 elements
-__device__ __forceinline__ float block_sum(float v, float (*shared)[kBlockMax / 32][2], int& turn) {
+__device__ __forceinline__ float block_sum(float v, float (*shared)[kWideThreads / 32][2], int& turn) {
     float s[1] = {v};
     row_sum<0>(s, shared, turn);
     return s[0];
 }
 
 template <typename TX, typename TY>
-__global__ void __launch_bounds__(kBlockMax) k_wide_forward(Norm a) {
-    __shared__ __align__(8) float shared[2][kBlockMax / 32][2];
+__global__ void __launch_bounds__(kWideThreads) k_wide_forward(Norm a) {
+    __shared__ __align__(8) float shared[2][kWideThreads / 32][2];
     int turn = 0;
     const float scale = 1.0f / static_cast<float>(a.n);
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const TX* x = static_cast<const TX*>(a.x) + row * a.x_stride;
         TY* y = static_cast<TY*>(a.y) + row * a.y_stride;
         float v = 0.0f;
-        for (int c = threadIdx.x; c < a.n; c += kBlockMax) v += Element<TX>::load(x[c]);
+        for (int c = threadIdx.x; c < a.n; c += kWideThreads) v += Element<TX>::load(x[c]);
         const float mean = block_sum(v, shared, turn) * scale;
         v = 0.0f;
-        for (int c = threadIdx.x; c < a.n; c += kBlockMax) {
+        for (int c = threadIdx.x; c < a.n; c += kWideThreads) {
             const float d = Element<TX>::load(x[c]) - mean;
             v += d * d;
         }
         const float rstd = rsqrtf(block_sum(v, shared, turn) * scale + a.epsilon);
-        for (int c = threadIdx.x; c < a.n; c += kBlockMax) {
+        for (int c = threadIdx.x; c < a.n; c += kWideThreads) {
             const float w = a.weight ? load_any(a.weight, a.parameter_type, c) : 1.0f;
             const float b = a.bias ? load_any(a.bias, a.parameter_type, c) : 0.0f;
             y[c] = Element<TY>::store((Element<TX>::load(x[c]) - mean) * rstd * w + b);
@@ -532,8 +542,8 @@ __global__ void __launch_bounds__(kBlockMax) k_wide_forward(Norm a) {
 
 // dx alone; k_wide_columns sums the parameters' gradients.
 template <typename TX, typename TY>
-__global__ void __launch_bounds__(kBlockMax) k_wide_backward(Norm a) {
-    __shared__ __align__(8) float shared[2][kBlockMax / 32][2];
+__global__ void __launch_bounds__(kWideThreads) k_wide_backward(Norm a) {
+    __shared__ __align__(8) float shared[2][kWideThreads / 32][2];
     int turn = 0;
     const float scale = 1.0f / static_cast<float>(a.n);
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
@@ -543,7 +553,7 @@ __global__ void __launch_bounds__(kBlockMax) k_wide_backward(Norm a) {
         TX* dx = static_cast<TX*>(a.y) + row * a.y_stride;
         const float mean = a.mean[row], rstd = a.rstd[row];
         float sum[2] = {0.0f, 0.0f};
-        for (int c = threadIdx.x; c < a.n; c += kBlockMax) {
+        for (int c = threadIdx.x; c < a.n; c += kWideThreads) {
             const float w = a.weight ? load_any(a.weight, a.parameter_type, c) : 1.0f;
             const float g = Element<TY>::load(dy[c]) * w;
             sum[0] += g;
@@ -551,7 +561,7 @@ __global__ void __launch_bounds__(kBlockMax) k_wide_backward(Norm a) {
         }
         row_sum<0>(sum, shared, turn);
         const float of_g = sum[0] * scale, of_gx = sum[1] * scale;
-        for (int c = threadIdx.x; c < a.n; c += kBlockMax) {
+        for (int c = threadIdx.x; c < a.n; c += kWideThreads) {
             const float w = a.weight ? load_any(a.weight, a.parameter_type, c) : 1.0f;
             const float g = Element<TY>::load(dy[c]) * w;
             const float h = (Element<TX>::load(x[c]) - mean) * rstd;
@@ -592,10 +602,11 @@ int multiprocessors() {
 
 // Threads and rows in flight of a block, and the grid: what is resident at once, and no more than
 // there are rows to take; `n` counts what a row's threads have to hold, shift included.
-int threads_of(int64_t n) { return group_of(n) ? 32 * kWarps : static_cast<int>(round_up((n + kHeld - 1) / kHeld, 32)); }
-int blocks_of(int64_t rows, int64_t n, int per_sm, int sms) {
-    const int64_t in_flight = group_of(n) ? 32 * kWarps / group_of(n) : 1;
-    const int64_t resident = sms * (group_of(n) ? per_sm : per_sm * 32 * kWarps / threads_of(n));
+int threads_of(int64_t n) { return group_of(n) ? kThreads : static_cast<int>(round_up((n + 31) / 32, 32)); }
+int blocks_of(int64_t rows, int64_t n, bool backward, int sms) {
+    const int group = group_of(n);
+    const int64_t in_flight = group ? kThreads / lanes_of(group) : 1;
+    const int64_t resident = sms * resident_blocks(group, backward) * (kThreads / threads_of(n));
     const int64_t want = (rows + in_flight - 1) / in_flight;
     // a block's next row is a multiple of 8 rows on, whatever V is
     return static_cast<int>(std::max<int64_t>(1, want <= resident ? want : in_flight == 1 ? resident / 8 * 8 : resident));
@@ -605,20 +616,19 @@ constexpr int kWideBlocks = 64;
 // The blocks whose sums of dw and db a backward pass leaves.
 template <typename TX, typename TY, int V, bool SHIFT, int G>
 int launch_norm(const Norm& a, bool backward, int sms, cudaStream_t stream) {
-    constexpr int kMost = G ? 32 * kWarps : kBlockMax;
     const int64_t held = a.n + (SHIFT ? V - 1 : 0);
-    const int threads = threads_of(held), grid = blocks_of(a.rows, held, backward ? kBackwardBlocks : kForwardBlocks, sms);
+    const int threads = threads_of(held), grid = blocks_of(a.rows, held, backward, sms);
     if (backward) {
-        using Ring = BackwardRing<TX, TY, V, kHeld / V>;
-        constexpr int kJoined = G ? 32 * kWarps * kHeld * 4 : 0;
+        using Ring = BackwardRing<TX, TY, V, held_of(G) / V>;
+        constexpr int kJoined = G ? kThreads * held_of(G) * 4 : 0;
         static uint64_t configured = 0;
-        allow_smem(k_norm_backward<TX, TY, V, SHIFT, G>, std::max(Ring::kStages * Ring::kBytes * kMost, kJoined), configured);
+        allow_smem(k_norm_backward<TX, TY, V, SHIFT, G>, std::max(Ring::kStages * Ring::kBytes * kThreads, kJoined), configured);
         launch("k_norm_backward", k_norm_backward<TX, TY, V, SHIFT, G>, grid, threads,
                std::max(Ring::kStages * Ring::kBytes * threads, kJoined), stream, a);
     } else {
-        using Ring = ForwardRing<TX, V, kHeld / V>;
+        using Ring = ForwardRing<TX, V, held_of(G) / V>;
         static uint64_t configured = 0;
-        allow_smem(k_norm_forward<TX, TY, V, SHIFT, G>, Ring::kStages * Ring::kBytes * kMost, configured);
+        allow_smem(k_norm_forward<TX, TY, V, SHIFT, G>, Ring::kStages * Ring::kBytes * kThreads, configured);
         launch("k_norm_forward", k_norm_forward<TX, TY, V, SHIFT, G>, grid, threads, Ring::kStages * Ring::kBytes * threads, stream, a);
     }
     return grid;
@@ -633,6 +643,7 @@ int run(const Norm& a, bool backward, int sms, cudaStream_t stream) {
     }
     switch (group) {
         case 32: return launch_norm<TX, TY, V, SHIFT, 32>(a, backward, sms, stream);
+        case kLong: return launch_norm<TX, TY, V, SHIFT, kLong>(a, backward, sms, stream);
         default: return launch_norm<TX, TY, V, SHIFT, 0>(a, backward, sms, stream);
     }
 }
@@ -641,14 +652,14 @@ template <typename TX, typename TY>
 int norm(const Norm& given, bool backward, cudaStream_t stream) {
     Norm a = given;
     const int sms = multiprocessors();
-    if (a.n > kHeld * kBlockMax) {
+    if (a.n > kMostColumns) {
         const int grid = static_cast<int>(std::min<int64_t>(a.rows, sms * 4)), parts = static_cast<int>(std::min<int64_t>(a.rows, kWideBlocks));
         if (!backward) {
-            launch("k_norm_forward", k_wide_forward<TX, TY>, grid, kBlockMax, 0, stream, a);
+            launch("k_norm_forward", k_wide_forward<TX, TY>, grid, kWideThreads, 0, stream, a);
             return grid;
         }
         if (a.partial) launch("k_norm_columns", k_wide_columns<TX, TY>, dim3(blocks(a.n, 256), parts), 256, 0, stream, a);
-        launch("k_norm_backward", k_wide_backward<TX, TY>, grid, kBlockMax, 0, stream, a);
+        launch("k_norm_backward", k_wide_backward<TX, TY>, grid, kWideThreads, 0, stream, a);
         return parts;
     }
     // 16 bytes a lane of the wider type where every matrix starts on its vector's boundary: as they
@@ -664,7 +675,7 @@ int norm(const Norm& given, bool backward, cudaStream_t stream) {
     const bool alike = a.y_stride % V == a.shift && (a.dy == nullptr || a.dy_stride % V == a.shift) &&
         (a.residual == nullptr || a.residual_stride % V == a.shift);
     if (bases && alike && a.shift == 0 && a.n % V == 0) return run<TX, TY, V, false>(a, backward, sms, stream);
-    if (bases && alike && a.n > kHeld * 16 && a.n + V - 1 <= kHeld * kBlockMax) return run<TX, TY, V, true>(a, backward, sms, stream);
+    if (bases && alike && a.n > 256 && a.n + V - 1 <= kMostColumns) return run<TX, TY, V, true>(a, backward, sms, stream);
     return run<TX, TY, 1, false>(a, backward, sms, stream);
 }
 
@@ -706,7 +717,7 @@ extern "C" int t8b_layer_norm_forward(const void* x, int x_type, int64_t x_strid
         check_matrix("layer norm y", y, rows, n, y_stride);
         if (rows == 0) return;
         const Span to(y, rows, n, y_stride, type_size(y_type)), from(x, rows, n, x_stride, type_size(x_type));
-        if (to.overlaps(from) && !(x == y && x_stride == y_stride && x_type == y_type && n <= kHeld * kBlockMax)) {
+        if (to.overlaps(from) && !(x == y && x_stride == y_stride && x_type == y_type && n <= kMostColumns)) {
             raise(T8B_EINVAL, "layer norm: y may be x itself in rows of up to 8192 elements, and overlap it in no other way");
         }
         Norm a{};
@@ -731,7 +742,7 @@ extern "C" size_t t8b_layer_norm_workspace(int64_t rows, int64_t n) {
     if (rows < 1 || n < 1) return 0;
     // the most blocks of any form, on any device of up to 256 multiprocessors, so that it needs none to answer
     int most = kWideBlocks;
-    if (n <= kHeld * kBlockMax) most = std::max(blocks_of(rows, n, kBackwardBlocks, 256), blocks_of(rows, n + 7, kBackwardBlocks, 256));
+    if (n <= kMostColumns) most = std::max(blocks_of(rows, n, true, 256), blocks_of(rows, n + 7, true, 256));
     return static_cast<size_t>(2) * most * static_cast<size_t>(n) * sizeof(float);
 }
 
