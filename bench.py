@@ -149,8 +149,19 @@ def max_over_ranks(values, device):
     return t.tolist()
 
 
+def reference_missing():
+    """Why the reference's CPU library cannot be had (None where it can)."""
+    from oracle import ref
+    if ref.LIB.exists() or (ref.REFERENCE / "src").exists():
+        return None
+    return "the reference's CPU library is not built and its sources are not here"
+
+
 def cpu_baseline(args, features, env, sample_envs=2048, sample_horizon=16):
     """The CPU leg on the host cores, on a bounded sample of the same workload."""
+    missing = reference_missing()
+    if missing:
+        return {"unavailable": missing}
     from oracle.cpu_iteration import CpuIteration
     threads = os.cpu_count() or 1
     it = CpuIteration(roster_raw(), features, env, sample_envs, sample_horizon, args.epochs, args.minibatches,
@@ -247,6 +258,10 @@ def kernel_table(args, profile, steps, peaks):
 def run_reference(args):
     world, rank, local = distributed()
     if rank != 0:
+        return
+    missing = reference_missing()
+    if missing:
+        print(json.dumps({"impl": "reference", "unavailable": missing}), flush=True)
         return
     # the reference arm loads only the oracle's libraries (the reference's own CPU code), no product code
     from oracle import ref
@@ -697,7 +712,7 @@ def run_engine(args):
     e2e_s = (time.perf_counter() - wall0) / args.steps
     got = hashes.cpu().numpy().view(np.uint64)
     cpu = None
-    if not args.no_cpu_baseline:
+    if not args.no_cpu_baseline and not reference_missing():
         from oracle import ref
         threads = os.cpu_count() or 1
         t0 = time.perf_counter()
