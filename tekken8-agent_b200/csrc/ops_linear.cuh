@@ -44,7 +44,7 @@ void linear_backward(const LinearGradCall& c);
 // A GEMM's tile (pairs of CTAs on 256 x 256 or 256 x 128, or one CTA on 128 x 64) and the number of
 // parts its k blocks are split into.
 struct GemmPlan {
-    int pair, bn, splits;
+    int bn, splits;
 };
 constexpr int kClusters = 74, kSms = 148;
 constexpr int kMaxSplits = 64;
@@ -62,9 +62,9 @@ inline GemmPlan plan_gemm(int64_t m, int64_t n, int64_t k, bool may_split) {
         int pair, bn;
         double block_cycles, tile_cycles;
     };
-    static constexpr Form forms[] = {{1, 256, 600, 4400}, {1, 128, 570, 2400}, {0, 64, 540, 720}};
+    static constexpr Form forms[] = {{1, 256, 600, 4400}, {1, 128, 570, 2400}, {0, 64, 540, 1400}};
     const int64_t k_blocks = ceil_div(k, tc::BK);
-    GemmPlan best{1, 256, 1};
+    GemmPlan best{256, 1};
     double least = 1e300;
     for (const Form& f : forms) {
         const int64_t tiles = ceil_div(m, f.pair ? 256 : 128) * ceil_div(n, f.bn);
@@ -78,7 +78,7 @@ inline GemmPlan plan_gemm(int64_t m, int64_t n, int64_t k, bool may_split) {
             if (splits > 1) cost += 4000.0 + static_cast<double>(splits) * m * n * 8.0 / 2500.0;
             if (cost < least) {
                 least = cost;
-                best = GemmPlan{f.pair, f.bn, static_cast<int>(splits)};
+                best = GemmPlan{f.bn, static_cast<int>(splits)};
             }
         }
     }
