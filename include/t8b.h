@@ -587,9 +587,16 @@ int t8b_layer_norm_backward(const void* dy, int y_type, int64_t dy_stride, const
  * weight [out][in] of `type` (T8B_BF16 or T8B_F16; products are summed in fp32), bias [out] of
  * bias_type (T8B_F32 or `type`; NULL: none), residual [rows][out] of y_type (NULL: none), y of
  * y_type (T8B_F32 or `type`). `pre` [rows][out] of `type`, unless NULL, receives x weight^T + bias
- * for the gradient. y may be the residual's own storage. The workspace is used, and may be NULL
- * otherwise, where the rows of x or of weight do not start on 16-byte boundaries. */
-size_t t8b_linear_workspace(int64_t rows, int64_t in, int64_t out, int backward);
+ * for the gradient. y may be the residual's own storage. The workspace (`what` says which parts a
+ * call needs: bits of T8B_WORKSPACE_*) may be NULL where none is needed. */
+enum {
+    T8B_WORKSPACE_BACKWARD = 1, /* a backward call */
+    T8B_WORKSPACE_X = 2,        /* the rows of x do not start on 16-byte boundaries */
+    T8B_WORKSPACE_WEIGHT = 4,   /* nor those of weight */
+    T8B_WORKSPACE_DZ = 8,       /* backward, with an activation or a gate, or dy's rows do not either */
+    T8B_WORKSPACE_ALL = 15,     /* enough for any call of these sizes */
+};
+size_t t8b_linear_workspace(int64_t rows, int64_t in, int64_t out, int what);
 int t8b_linear_forward(int type, const void* x, int64_t x_stride, const void* weight, int64_t weight_stride,
                        const void* bias, int bias_type, int activation, const void* residual, int64_t residual_stride,
                        int64_t rows, int64_t in, int64_t out, void* y, int y_type, int64_t y_stride, void* pre,
@@ -607,7 +614,7 @@ int t8b_linear_backward(int type, const void* dy, int64_t dy_stride, const void*
 /* Gated projection: h = activation(gate) up, where [gate | up] = x weight^T + bias: weight
  * [2 out][in] and bias [2 out] hold the gate's rows first, then the up projection's. `pre`
  * [rows][2 out], unless NULL, receives [gate | up]. Types as for the linear map; h is of `type`. */
-size_t t8b_gated_workspace(int64_t rows, int64_t in, int64_t out, int backward);
+size_t t8b_gated_workspace(int64_t rows, int64_t in, int64_t out, int what);
 int t8b_gated_forward(int type, const void* x, int64_t x_stride, const void* weight, int64_t weight_stride,
                       const void* bias, int bias_type, int activation, int64_t rows, int64_t in, int64_t out, void* h,
                       int64_t h_stride, void* pre, int64_t pre_stride, void* workspace, size_t workspace_bytes,

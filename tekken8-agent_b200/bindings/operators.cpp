@@ -311,11 +311,14 @@ struct Operands {
         vector_of(bias, "bias", columns, on.device, t);
         return t;
     }
-    // room for packed copies, where a forward pass may want them
-    size_t forward_room(decltype(&t8b_linear_workspace) query) const {
-        const uintptr_t at = reinterpret_cast<uintptr_t>(x.data) | reinterpret_cast<uintptr_t>(weight.data);
-        return (at & 15) != 0 || ((x.stride | weight.stride) & 7) != 0 ? query(x.rows, in, out, 0) : 0;
+    // the operands whose rows do not suit TMA, as the library's own rule has it
+    static bool off(const Rows& r) {
+        return (reinterpret_cast<uintptr_t>(r.data) & 15) != 0 || (r.rows > 1 && ((r.stride & 7) != 0 || r.stride >= (1ll << 39)));
     }
+    int packed(bool of_x, bool of_weight) const {
+        return (of_x && off(x) ? T8B_WORKSPACE_X : 0) | (of_weight && off(weight) ? T8B_WORKSPACE_WEIGHT : 0);
+    }
+    size_t room(decltype(&t8b_linear_workspace) query, int what) const { return what ? query(x.rows, in, out, what) : 0; }
 };
 
 // x, weight, bias, activation, residual, out_dtype, save
@@ -339,7 +342,7 @@ PyObject* linear(PyObject*, PyObject* const* args, Py_ssize_t given) {
         const Tensor y = make(x, shape, y_type);
         Tensor pre, workspace;
         if (save) pre = make(x, shape, o.type);
-        const size_t size = o.forward_room(entry.linear_workspace);
+        const size_t size = o.room(entry.linear_workspace, o.packed(true, true));
         if (size) workspace = make_bytes(x, size);
         done(entry.linear_forward(o.type, o.x.data, o.x.stride, o.weight.data, o.weight.stride, pointer(bias), b_type, act, r.data,
                                   r.stride, o.x.rows, o.in, o.out, y.data_ptr(), y_type, o.out, pointer(pre), o.out,
@@ -360,7 +363,7 @@ PyObject* gated(PyObject*, PyObject* const* args, Py_ssize_t given) {
         const Tensor h = make(x, Shape(x, o.out), o.type);
         Tensor pre, workspace;
         if (save) pre = make(x, Shape(x, o.columns), o.type);
-        const size_t size = o.forward_room(entry.gated_workspace);
+        const size_t size = o.room(entry.gated_workspace, o.packed(true, true));
         if (size) workspace = make_bytes(x, size);
         done(entry.gated_forward(o.type, o.x.data, o.x.stride, o.weight.data, o.weight.stride, pointer(bias), b_type, act, o.x.rows,
                                  o.in, o.out, h.data_ptr(), o.out, pointer(pre), o.columns, pointer(workspace), size, o.on.stream()));
@@ -396,7 +399,9 @@ PyObject* backward(PyObject*, PyObject* const* args, Py_ssize_t given) {
         if (a.flag(6)) dx = make(x, x.sizes(), o.type);
         const Tensor dweight = make(x, {o.columns, o.in}, o.type);
         if (bias.defined()) dbias = make(x, {o.columns}, b_type);
-        const size_t size = (PARTS == 2 ? entry.gated_workspace : entry.linear_workspace)(o.x.rows, o.in, o.out, 1);
+        int what = T8B_WORKSPACE_BACKWARD | o.packed(true, dx.defined());
+        if (PARTS == 2 || act != T8B_LINEAR || Operands::off(d)) what |= T8B_WORKSPACE_DZ;
+        const size_t size = o.room(PARTS == 2 ? entry.gated_workspace : entry.linear_workspace, what);
         if (size) workspace = make_bytes(x, size);
         done((PARTS == 2 ? entry.gated_backward : entry.linear_backward)(
             o.type, d.data, d.stride, o.x.data, o.x.stride, o.weight.data, o.weight.stride, z.data, z.stride, b_type, act, o.x.rows,

@@ -69,8 +69,11 @@ void forward(const char* what, int type, LinearCall& c, void* workspace, size_t 
         pre.overlaps(x) || pre.overlaps(w) || pre.overlaps(residual) || pre.overlaps(bias)) {
         raise(T8B_EINVAL, std::string(what) + ": an output overlaps another argument");
     }
-    const bool packs = !is_few(c.rows, c.in) && (!tma_rows(c.x, c.rows, c.x_stride, 2) || !tma_rows(c.weight, columns, c.weight_stride, 2));
-    check_workspace(what, workspace, workspace_bytes, packs ? Workspace(c.rows, c.in, columns).forward_bytes : 0);
+    if (!is_few(c.rows, c.in)) {
+        if (!tma_rows(c.x, c.rows, c.x_stride, 2)) c.what |= T8B_WORKSPACE_X;
+        if (!tma_rows(c.weight, columns, c.weight_stride, 2)) c.what |= T8B_WORKSPACE_WEIGHT;
+    }
+    check_workspace(what, workspace, workspace_bytes, Workspace(c.rows, c.in, columns, c.what).bytes);
     c.workspace = static_cast<unsigned char*>(workspace);
     if (type == T8B_BF16) {
         linear_forward<bf16>(c);
@@ -111,7 +114,11 @@ void backward(const char* what, int type, LinearGradCall& c, void* workspace, si
             raise(T8B_EINVAL, std::string(what) + ": an output overlaps another argument");
         }
     }
-    check_workspace(what, workspace, workspace_bytes, Workspace(c.rows, c.in, columns).bytes);
+    c.what = T8B_WORKSPACE_BACKWARD;
+    if (c.dweight && !tma_rows(c.x, c.rows, c.x_stride, 2)) c.what |= T8B_WORKSPACE_X;
+    if (c.dx && !tma_rows(c.weight, columns, c.weight_stride, 2)) c.what |= T8B_WORKSPACE_WEIGHT;
+    if ((c.dx || c.dweight) && (reads_pre || !tma_rows(c.dy, c.rows, c.dy_stride, 2))) c.what |= T8B_WORKSPACE_DZ;
+    check_workspace(what, workspace, workspace_bytes, Workspace(c.rows, c.in, columns, c.what).bytes);
     c.workspace = static_cast<unsigned char*>(workspace);
     if (type == T8B_BF16) {
         linear_backward<bf16>(c);
@@ -120,10 +127,9 @@ void backward(const char* what, int type, LinearGradCall& c, void* workspace, si
     }
 }
 
-size_t workspace_size(int64_t rows, int64_t in, int64_t columns, int backward) {
+size_t workspace_size(int64_t rows, int64_t in, int64_t columns, int what) {
     if (rows < 1 || rows > kMostRows || in < 1 || columns < 1 || in > kMostColumns || columns > 2 * kMostColumns) return 0;
-    const Workspace w(rows, in, columns);
-    return backward ? w.bytes : w.forward_bytes;
+    return Workspace(rows, in, columns, what).bytes;
 }
 
 }  // namespace
@@ -133,11 +139,11 @@ size_t workspace_size(int64_t rows, int64_t in, int64_t columns, int backward) {
 using namespace t8b;
 using namespace t8b::op;
 
-extern "C" size_t t8b_linear_workspace(int64_t rows, int64_t in, int64_t out, int backward) {
-    return workspace_size(rows, in, out, backward);
+extern "C" size_t t8b_linear_workspace(int64_t rows, int64_t in, int64_t out, int what) {
+    return workspace_size(rows, in, out, what);
 }
-extern "C" size_t t8b_gated_workspace(int64_t rows, int64_t in, int64_t out, int backward) {
-    return workspace_size(rows, in, 2 * out, backward);
+extern "C" size_t t8b_gated_workspace(int64_t rows, int64_t in, int64_t out, int what) {
+    return workspace_size(rows, in, 2 * out, what);
 }
 
 extern "C" int t8b_linear_forward(int type, const void* x, int64_t x_stride, const void* weight, int64_t weight_stride,
@@ -147,7 +153,7 @@ extern "C" int t8b_linear_forward(int type, const void* x, int64_t x_stride, con
                                   void* stream) {
     return guarded([&] {
         LinearCall c{x, weight, bias, residual, y, pre, x_stride, weight_stride, residual_stride, y_stride, pre_stride, rows, in,
-                     out, bias_type, activation, y_type, false, nullptr, static_cast<cudaStream_t>(stream)};
+                     out, bias_type, activation, y_type, false, 0, nullptr, static_cast<cudaStream_t>(stream)};
         forward("linear", type, c, workspace, workspace_bytes);
     });
 }
@@ -158,7 +164,7 @@ extern "C" int t8b_gated_forward(int type, const void* x, int64_t x_stride, cons
                                  size_t workspace_bytes, void* stream) {
     return guarded([&] {
         LinearCall c{x, weight, bias, nullptr, h, pre, x_stride, weight_stride, 0, h_stride, pre_stride, rows, in, out,
-                     bias_type, activation, type, true, nullptr, static_cast<cudaStream_t>(stream)};
+                     bias_type, activation, type, true, 0, nullptr, static_cast<cudaStream_t>(stream)};
         forward("gated", type, c, workspace, workspace_bytes);
     });
 }
@@ -170,7 +176,7 @@ extern "C" int t8b_linear_backward(int type, const void* dy, int64_t dy_stride, 
                                    size_t workspace_bytes, void* stream) {
     return guarded([&] {
         LinearGradCall c{dy, x, weight, pre, dx, dweight, dbias, dy_stride, x_stride, weight_stride, pre_stride, dx_stride,
-                         dweight_stride, rows, in, out, bias_type, activation, false, nullptr, static_cast<cudaStream_t>(stream)};
+                         dweight_stride, rows, in, out, bias_type, activation, false, 0, nullptr, static_cast<cudaStream_t>(stream)};
         backward("linear", type, c, workspace, workspace_bytes);
     });
 }
@@ -182,7 +188,7 @@ extern "C" int t8b_gated_backward(int type, const void* dh, int64_t dh_stride, c
                                   size_t workspace_bytes, void* stream) {
     return guarded([&] {
         LinearGradCall c{dh, x, weight, pre, dx, dweight, dbias, dh_stride, x_stride, weight_stride, pre_stride, dx_stride,
-                         dweight_stride, rows, in, out, bias_type, activation, true, nullptr, static_cast<cudaStream_t>(stream)};
+                         dweight_stride, rows, in, out, bias_type, activation, true, 0, nullptr, static_cast<cudaStream_t>(stream)};
         backward("gated", type, c, workspace, workspace_bytes);
     });
 }

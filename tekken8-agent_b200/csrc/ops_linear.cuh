@@ -22,6 +22,7 @@ struct LinearCall {
     int64_t rows, in, out;
     int bias_type, activation, y_type;
     bool gated;
+    int what;  // the parts of the workspace it uses (T8B_WORKSPACE_*)
     unsigned char* workspace;
     cudaStream_t stream;
 };
@@ -32,6 +33,7 @@ struct LinearGradCall {
     int64_t rows, in, out;
     int bias_type, activation;
     bool gated;
+    int what;  // the parts of the workspace it uses (T8B_WORKSPACE_*)
     unsigned char* workspace;
     cudaStream_t stream;
 };
@@ -102,27 +104,27 @@ inline int grad_parts(int64_t rows, int64_t columns) {
     return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(ceil_div(rows, kGradRows), ceil_div(kSms * 3, across))));
 }
 
-// The workspace, in this order; each part starts on a 256-byte boundary. A forward pass uses the
-// first two, and them only for operands whose rows do not suit TMA.
+// The workspace of a call, in this order and as far as `what` (T8B_WORKSPACE_* bits) says; each part
+// starts on a 256-byte boundary.
 struct Workspace {
-    size_t x, weight, forward_bytes, dz, sums, parts, bytes;
-    size_t dz_pitch, x_pitch;
-    Workspace(int64_t rows, int64_t in, int64_t columns) {
-        x_pitch = round_up(in, 8);
+    size_t x, weight, dz, sums, parts, bytes;
+    size_t dz_pitch;
+    Workspace(int64_t rows, int64_t in, int64_t columns, int what) {
+        const size_t x_pitch = round_up(in, 8);
         dz_pitch = round_up(columns, 8);
         size_t at = 0;
-        const auto take = [&](size_t size) {
+        const auto take = [&](bool wanted, size_t size) {
             const size_t here = at;
-            at += round_up(size, 256);
+            if (wanted) at += round_up(size, 256);
             return here;
         };
-        x = take(rows * x_pitch * 2);
-        weight = take(columns * x_pitch * 2);
-        forward_bytes = at;
-        dz = take(rows * dz_pitch * 2);
-        sums = take(static_cast<size_t>(grad_parts(rows, columns)) * columns * 4);
-        const GemmPlan p = plan_gemm(columns, in, rows, true);
-        parts = take(p.splits > 1 ? p.splits * split_rows(columns) * split_pitch(in) * 4 : 0);
+        const bool backward = (what & T8B_WORKSPACE_BACKWARD) != 0;
+        x = take((what & T8B_WORKSPACE_X) != 0, rows * x_pitch * 2);
+        weight = take((what & T8B_WORKSPACE_WEIGHT) != 0, columns * x_pitch * 2);
+        dz = take(backward && (what & T8B_WORKSPACE_DZ) != 0, rows * dz_pitch * 2);
+        sums = take(backward, static_cast<size_t>(grad_parts(rows, columns)) * columns * 4);
+        const int splits = backward ? plan_gemm(columns, in, rows, true).splits : 1;
+        parts = take(splits > 1, splits * split_rows(columns) * split_pitch(in) * 4);
         bytes = at;
     }
 };
@@ -827,7 +829,7 @@ void linear_forward(const LinearCall& c) {
         c.gated ? few_rows<E, true>(c) : few_rows<E, false>(c);
         return;
     }
-    const Workspace at(c.rows, c.in, columns);
+    const Workspace at(c.rows, c.in, columns, c.what);
     PackJob jobs[2]{};
     const Matrix x = operand<E>(c.x, c.rows, c.in, c.x_stride, c.workspace + at.x, jobs[0]);
     const Matrix w = operand<E>(c.weight, columns, c.in, c.weight_stride, c.workspace + at.weight, jobs[1]);
@@ -918,10 +920,9 @@ void activation_grad(const LinearGradCall& c, E* dz, int64_t pitch, float* sums)
 template <typename E>
 void linear_backward(const LinearGradCall& c) {
     const int64_t columns = c.gated ? 2 * c.out : c.out;
-    const Workspace at(c.rows, c.in, columns);
+    const Workspace at(c.rows, c.in, columns, c.what);
     // dz is dy itself where there is neither a gate nor an activation and its rows suit TMA
-    const bool own = c.gated || c.activation != T8B_LINEAR || !tma_rows(c.dy, c.rows, c.dy_stride, sizeof(E));
-    E* dz_out = own && (c.dx || c.dweight) ? reinterpret_cast<E*>(c.workspace + at.dz) : nullptr;
+    E* dz_out = (c.what & T8B_WORKSPACE_DZ) != 0 ? reinterpret_cast<E*>(c.workspace + at.dz) : nullptr;
     float* sums = c.dbias ? reinterpret_cast<float*>(c.workspace + at.sums) : nullptr;
     Matrix dz{c.dy, c.rows, columns, tma_pitch(c.rows, columns, c.dy_stride, sizeof(E))};
     if (dz_out) dz = Matrix{dz_out, c.rows, columns, static_cast<int64_t>(at.dz_pitch)};

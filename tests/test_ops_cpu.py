@@ -32,9 +32,12 @@ def test_workspace_queries():
     from t8b import _lib
     lib = _lib.lib()
     for rows, n, m in ((1, 1, 1), (7, 151, 33), (65536, 512, 1408), (2051, 1001, 1333)):
-        forward, backward = lib.t8b_linear_workspace(rows, n, m, 0), lib.t8b_linear_workspace(rows, n, m, 1)
+        forward, backward = lib.t8b_linear_workspace(rows, n, m, 6), lib.t8b_linear_workspace(rows, n, m, 15)
         assert forward >= 2 * (rows * n + m * n) and backward >= forward + 2 * rows * m
-        assert lib.t8b_gated_workspace(rows, n, m, 1) >= backward
+        assert lib.t8b_gated_workspace(rows, n, m, 15) >= backward
+        assert lib.t8b_linear_workspace(rows, n, m, 0) == 0
+        parts = [lib.t8b_linear_workspace(rows, n, m, what) for what in (1, 9, 11, 15)]
+        assert parts == sorted(parts) and parts[1] - parts[0] >= 2 * rows * m
         assert lib.t8b_layer_norm_workspace(rows, n) >= 8 * n
     for bad in ((0, 8, 8), (-1, 8, 8), (8, 0, 8), (8, 8, 1 << 30)):
-        assert lib.t8b_linear_workspace(*bad, 1) == 0
+        assert lib.t8b_linear_workspace(*bad, 15) == 0

@@ -570,7 +570,7 @@ def test_c_entries_refuse_what_they_cannot_take(cuda):
         assert lib.t8b_last_error()
     assert linear(rows=0, x=0, y=0) == 0
     assert linear(r=py) == 0  # in place on the residual
-    need = lib.t8b_linear_workspace(32, 32, 32, 1)
+    need = lib.t8b_linear_workspace(32, 32, 32, 1)  # packed rows, no activation: no copies, no dz
     work = torch.empty(need, dtype=torch.uint8, device="cuda")
     out = torch.zeros(64, 64, device="cuda", dtype=E)
 
@@ -581,7 +581,8 @@ def test_c_entries_refuse_what_they_cannot_take(cuda):
         return lib.t8b_linear_backward(*a.values(), None)
 
     assert backward() == 0
-    for bad in (dict(size=need - 1), dict(work=0), dict(work=work.data_ptr() + 16), dict(dx=px, dw=out.data_ptr()),
+    assert lib.t8b_linear_workspace(32, 32, 32, 15) > need
+    for bad in (dict(size=need - 1), dict(work=0), dict(x=px + 2, dw=out.data_ptr(), dx=0), dict(act=4, p=pw), dict(work=work.data_ptr() + 16), dict(dx=px, dw=out.data_ptr()),
                 dict(dx=py), dict(act=4), dict(dw=out.data_ptr()), dict(dxs=3), dict(type=0)):
         assert backward(**bad) == _lib.T8B_EINVAL, bad
     mean = torch.zeros(64, device="cuda")
