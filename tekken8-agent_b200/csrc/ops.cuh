@@ -229,9 +229,11 @@ inline void allow_smem(Kernel kernel, size_t bytes, uint64_t& configured) {
     __atomic_fetch_or(&configured, bit, __ATOMIC_RELEASE);
 }
 
-// A launch in a chain of kernels of one call: with `chained` its blocks may start before the kernel
-// before it has ended, as soon as every block of that one has passed release_next(); they must call
-// wait_previous() before they touch what it writes, and before they end.
+// A launch behind whatever the stream holds: with `chained` its blocks may start before the kernel
+// before it has ended, as soon as every block of that one has passed release_next() (or ended, for
+// a kernel that does not call it), so launch latency and prologues overlap its tail. They call
+// wait_previous() before they touch memory that it may read or write, and only then release the next,
+// so that by induction everything earlier has ended too.
 template <typename Kernel, typename... Args>
 inline void launch_chain(const char* label, Kernel kernel, dim3 grid, dim3 block, size_t smem, cudaStream_t stream, bool chained,
                          const Args&... args) {
@@ -248,10 +250,11 @@ inline void launch_chain(const char* label, Kernel kernel, dim3 grid, dim3 block
     config.numAttrs = chained ? 1 : 0;
     check(cudaLaunchKernelEx(&config, kernel, args...), label);
 }
-// What the kernel before it in a chain is to a kernel. kInput: it writes what this one reads. kBeside:
-// it does not, and this one's blocks fill the SMs that it leaves idle, but what came before it is this
-// one's input too (all of that had ended before any of its blocks let this one start).
-enum { kNothing = 0, kInput = 1, kBeside = 2 };
+// What the kernel before it is to a kernel. kInput: anything, so this one waits for it first. kBeside:
+// another of the same call that shares nothing with this one, whose blocks fill the SMs that it leaves
+// idle and wait for it before they end; what came before it had ended before any of its blocks let
+// this one start.
+enum { kInput = 1, kBeside = 2 };
 __device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void release_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

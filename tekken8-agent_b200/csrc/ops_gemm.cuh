@@ -232,7 +232,7 @@ constexpr uint32_t kDrainLimit = 1u << 18;
 struct Shape {
     int tiles_m, tiles_n, splits, k_blocks;
     int second;  // B's second half starts at this row (gated projections); 0: B is one matrix
-    int after;   // what the kernel before this one in the chain is to it: kNothing, kInput or kBeside
+    int after;   // what the kernel before this one is to it: kInput or kBeside
     int* error;
 };
 

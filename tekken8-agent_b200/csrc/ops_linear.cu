@@ -73,7 +73,7 @@ void forward(const char* what, int type, LinearCall& c, void* workspace, size_t 
         if (!tma_rows(c.x, c.rows, c.x_stride, 2)) c.what |= T8B_WORKSPACE_X;
         if (!tma_rows(c.weight, columns, c.weight_stride, 2)) c.what |= T8B_WORKSPACE_WEIGHT;
     }
-    check_workspace(what, workspace, workspace_bytes, Workspace(c.rows, c.in, columns, c.what).bytes);
+    check_workspace(what, workspace, workspace_bytes, Workspace(c.rows, c.in, c.out, c.gated, c.what).bytes);
     c.workspace = static_cast<unsigned char*>(workspace);
     if (type == T8B_BF16) {
         linear_forward<bf16>(c);
@@ -118,7 +118,7 @@ void backward(const char* what, int type, LinearGradCall& c, void* workspace, si
     if (c.dweight && !tma_rows(c.x, c.rows, c.x_stride, 2)) c.what |= T8B_WORKSPACE_X;
     if (c.dx && !tma_rows(c.weight, columns, c.weight_stride, 2)) c.what |= T8B_WORKSPACE_WEIGHT;
     if ((c.dx || c.dweight) && (reads_pre || !tma_rows(c.dy, c.rows, c.dy_stride, 2))) c.what |= T8B_WORKSPACE_DZ;
-    check_workspace(what, workspace, workspace_bytes, Workspace(c.rows, c.in, columns, c.what).bytes);
+    check_workspace(what, workspace, workspace_bytes, Workspace(c.rows, c.in, c.out, c.gated, c.what).bytes);
     c.workspace = static_cast<unsigned char*>(workspace);
     if (type == T8B_BF16) {
         linear_backward<bf16>(c);
@@ -127,9 +127,9 @@ void backward(const char* what, int type, LinearGradCall& c, void* workspace, si
     }
 }
 
-size_t workspace_size(int64_t rows, int64_t in, int64_t columns, int what) {
-    if (rows < 1 || rows > kMostRows || in < 1 || columns < 1 || in > kMostColumns || columns > 2 * kMostColumns) return 0;
-    return Workspace(rows, in, columns, what).bytes;
+size_t workspace_size(int64_t rows, int64_t in, int64_t out, bool gated, int what) {
+    if (rows < 1 || rows > kMostRows || in < 1 || out < 1 || in > kMostColumns || out > kMostColumns) return 0;
+    return Workspace(rows, in, out, gated, what).bytes;
 }
 
 }  // namespace
@@ -140,10 +140,10 @@ using namespace t8b;
 using namespace t8b::op;
 
 extern "C" size_t t8b_linear_workspace(int64_t rows, int64_t in, int64_t out, int what) {
-    return workspace_size(rows, in, out, what);
+    return workspace_size(rows, in, out, false, what);
 }
 extern "C" size_t t8b_gated_workspace(int64_t rows, int64_t in, int64_t out, int what) {
-    return workspace_size(rows, in, 2 * out, what);
+    return workspace_size(rows, in, out, true, what);
 }
 
 extern "C" int t8b_linear_forward(int type, const void* x, int64_t x_stride, const void* weight, int64_t weight_stride,

@@ -97,11 +97,15 @@ inline bool is_few(int64_t rows, int64_t in) { return rows <= 4 || (rows <= 16 &
 inline size_t split_rows(int64_t m) { return round_up(m, 256); }
 inline size_t split_pitch(int64_t n) { return round_up(n, 4); }
 
-// Row parts of the elementwise backward pass (each gives one row of partial column sums).
-constexpr int kGradRows = 8;
-inline int grad_parts(int64_t rows, int64_t columns) {
-    const int64_t across = ceil_div(columns, 256);
-    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(ceil_div(rows, kGradRows), ceil_div(kSms * 3, across))));
+// Row parts of the elementwise backward pass over dy's columns (each gives one row of partial column
+// sums): with 256 columns a block, two blocks an SM, and no more resident, so that they spread evenly
+// even where they start behind a kernel that leaves some SMs first (three where they find room: 460 us
+// for the gated backward of 65,536 x 1,408 against 426).
+constexpr int kGradRows = 8, kGradBlocks = 2;
+constexpr size_t kGradSmem = 100 * 1024;
+inline int grad_parts(int64_t rows, int64_t out) {
+    const int64_t across = ceil_div(out, 256);
+    return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(ceil_div(rows, kGradRows), kSms * kGradBlocks / across)));
 }
 
 // The workspace of a call, in this order and as far as `what` (T8B_WORKSPACE_* bits) says; each part
@@ -109,7 +113,8 @@ inline int grad_parts(int64_t rows, int64_t columns) {
 struct Workspace {
     size_t x, weight, dz, sums, parts, bytes;
     size_t dz_pitch;
-    Workspace(int64_t rows, int64_t in, int64_t columns, int what) {
+    Workspace(int64_t rows, int64_t in, int64_t out, bool gated, int what) {
+        const int64_t columns = gated ? 2 * out : out;
         const size_t x_pitch = round_up(in, 8);
         dz_pitch = round_up(columns, 8);
         size_t at = 0;
@@ -122,7 +127,7 @@ struct Workspace {
         x = take((what & T8B_WORKSPACE_X) != 0, rows * x_pitch * 2);
         weight = take((what & T8B_WORKSPACE_WEIGHT) != 0, columns * x_pitch * 2);
         dz = take(backward && (what & T8B_WORKSPACE_DZ) != 0, rows * dz_pitch * 2);
-        sums = take(backward, static_cast<size_t>(grad_parts(rows, columns)) * columns * 4);
+        sums = take(backward, static_cast<size_t>(grad_parts(rows, out)) * columns * 4);
         const int splits = backward ? plan_gemm(columns, in, rows, true).splits : 1;
         parts = take(splits > 1, splits * split_rows(columns) * split_pitch(in) * 4);
         bytes = at;
@@ -339,6 +344,8 @@ struct PackJob {
 };
 template <typename E>
 __global__ void k_pack(PackJob first, PackJob second, int after) {
+    if (after == kInput) wait_previous();
+    release_next();
     const int64_t pieces = first.rows * (first.pitch / 8), total = pieces + second.rows * (second.pitch / 8);
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < total;
          i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
@@ -374,6 +381,8 @@ struct FewRows {
 constexpr int kFewWarps = 8;
 template <typename E, bool GATED, int R, bool WIDE>
 __global__ void __launch_bounds__(32 * kFewWarps) k_few_rows(FewRows<E> a) {
+    wait_previous();
+    release_next();
     constexpr int PARTS = GATED ? 2 : 1;
     const int lane = threadIdx.x & 31;
     const int row0 = blockIdx.y * R, live = min(R, a.rows - row0);
@@ -471,9 +480,10 @@ template <typename E, bool GATED, int V>
 constexpr int grad_ring_bytes() { return V == 8 ? kGradStages * (GATED ? 3 : 2) * 16 * 32 * kGradRows : 0; }
 
 template <typename E, bool GATED, int V>
-__global__ void __launch_bounds__(32 * kGradRows, V == 8 ? 3 : 5)
+__global__ void __launch_bounds__(32 * kGradRows, V == 8 ? kGradBlocks : 5)
     k_activation_grad(const E* dy, int64_t dy_stride, const E* pre, int64_t pre_stride, int64_t rows, int columns,
                       int activation, E* dz, int64_t pitch, float* sums) {
+    wait_previous();
     release_next();  // operands may be packed beside it
     constexpr int PARTS = GATED ? 2 : 1;
     constexpr bool RING = V == 8;
@@ -615,6 +625,7 @@ struct Totals {
 template <typename E>
 __global__ void __launch_bounds__(256) k_totals(Totals a) {
     wait_previous();
+    release_next();
     if (blockIdx.x < a.join_blocks) {
         const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.y * 32 + threadIdx.x;
         const int pieces = a.pitch / 4;
@@ -726,7 +737,7 @@ void launch_gemm(const char* label, const Matrix& a, const Matrix& b, int64_t co
     const CUtensorMap map_b = B_MN ? mn_major(b) : k_major(b, second ? BN / 2 : BN / CG);
     const int64_t work = static_cast<int64_t>(s.tiles_m) * s.tiles_n * s.splits;
     const int grid = static_cast<int>(std::min<int64_t>(work, CG == 2 ? kClusters : kSms)) * CG;
-    launch_chain(label, kernel, grid, kGemmThreads, P::kSmemBytes, stream, after != kNothing, map_a, map_b, s, epi);
+    launch_chain(label, kernel, grid, kGemmThreads, P::kSmemBytes, stream, true, map_a, map_b, s, epi);
 }
 
 // A matrix as a GEMM operand: where its rows do not suit TMA, a copy in the workspace, which pack()
@@ -737,20 +748,18 @@ Matrix operand(const void* data, int64_t rows, int64_t columns, int64_t stride, 
     job = PackJob{data, copy, stride, rows, static_cast<int64_t>(round_up(columns, 8)), static_cast<int>(columns)};
     return Matrix{copy, rows, columns, job.pitch};
 }
-// Whether there was anything to pack.
 template <typename E>
-bool pack(const PackJob (&jobs)[2], int after, cudaStream_t stream) {
+void pack(const PackJob (&jobs)[2], int after, cudaStream_t stream) {
     const int64_t pieces = (jobs[0].rows * jobs[0].pitch + jobs[1].rows * jobs[1].pitch) / 8;
-    if (pieces == 0) return false;
+    if (pieces == 0) return;
     launch_chain("k_pack", k_pack<E>, static_cast<unsigned>(std::min<int64_t>(ceil_div(pieces, 256), kSms * 16)), 256, 0, stream,
-                 after != kNothing, jobs[0], jobs[1], after);
-    return true;
+                 true, jobs[0], jobs[1], after);
 }
 // [rows][k] read along its rows' other axis: the same storage as an MN-major operand.
 inline Matrix transposed(const Matrix& m) { return Matrix{m.data, m.k, m.rows, m.pitch}; }
 
 template <typename E, typename O, int CG, int BN>
-void forward_tile(const LinearCall& c, const Matrix& x, const Matrix& w, int after) {
+void forward_tile(const LinearCall& c, const Matrix& x, const Matrix& w) {
     using Epi = EpiLinear<E, O, BN, true>;
     Epi epi{};
     epi.y = tiled<O, Epi::kBytes>(c.y, c.rows, c.out, c.y_stride);
@@ -763,10 +772,10 @@ void forward_tile(const LinearCall& c, const Matrix& x, const Matrix& w, int aft
     epi.activation = c.activation;
     epi.has_residual = c.residual != nullptr;
     epi.has_pre = c.pre != nullptr;
-    launch_gemm<E, CG, BN, false, false>("k_linear", x, w, c.out, 0, 1, after, epi, c.stream);
+    launch_gemm<E, CG, BN, false, false>("k_linear", x, w, c.out, 0, 1, kInput, epi, c.stream);
 }
 template <typename E, int CG, int BN>
-void gated_tile(const LinearCall& c, const Matrix& x, const Matrix& w, int after) {
+void gated_tile(const LinearCall& c, const Matrix& x, const Matrix& w) {
     using Epi = EpiGated<E, BN>;
     Epi epi{};
     epi.h = tiled<E, Epi::kBytes>(c.y, c.rows, c.out, c.y_stride);
@@ -778,7 +787,7 @@ void gated_tile(const LinearCall& c, const Matrix& x, const Matrix& w, int after
     epi.bias_type = c.bias_type;
     epi.activation = c.activation;
     epi.has_pre = c.pre != nullptr;
-    launch_gemm<E, CG, BN, false, false>("k_gated", x, w, c.out, static_cast<int>(c.out), 1, after, epi, c.stream);
+    launch_gemm<E, CG, BN, false, false>("k_gated", x, w, c.out, static_cast<int>(c.out), 1, kInput, epi, c.stream);
 }
 
 template <typename E, bool GATED, int R>
@@ -805,9 +814,9 @@ void few_rows(const LinearCall& c) {
     const bool wide = aligned(c.x, 16) && aligned(c.weight, 16) && (c.rows == 1 || c.x_stride % 8 == 0) &&
         (c.weight_stride % 8 == 0 || (c.out == 1 && !GATED));
     if (wide) {
-        launch("k_few_rows", k_few_rows<E, GATED, R, true>, grid, 32 * kFewWarps, 0, c.stream, a);
+        launch_chain("k_few_rows", k_few_rows<E, GATED, R, true>, grid, 32 * kFewWarps, 0, c.stream, true, a);
     } else {
-        launch("k_few_rows", k_few_rows<E, GATED, R, false>, grid, 32 * kFewWarps, 0, c.stream, a);
+        launch_chain("k_few_rows", k_few_rows<E, GATED, R, false>, grid, 32 * kFewWarps, 0, c.stream, true, a);
     }
     check(cudaGetLastError(), "few rows");
 }
@@ -829,35 +838,35 @@ void linear_forward(const LinearCall& c) {
         c.gated ? few_rows<E, true>(c) : few_rows<E, false>(c);
         return;
     }
-    const Workspace at(c.rows, c.in, columns, c.what);
+    const Workspace at(c.rows, c.in, c.out, c.gated, c.what);
     PackJob jobs[2]{};
     const Matrix x = operand<E>(c.x, c.rows, c.in, c.x_stride, c.workspace + at.x, jobs[0]);
     const Matrix w = operand<E>(c.weight, columns, c.in, c.weight_stride, c.workspace + at.weight, jobs[1]);
-    const int after = pack<E>(jobs, kNothing, c.stream) ? kInput : kNothing;
+    pack<E>(jobs, kInput, c.stream);
     const GemmPlan p = plan_gemm(c.rows, columns, c.in, false);
     if (c.gated) {
         if (p.bn == 256) {
-            gated_tile<E, 2, 256>(c, x, w, after);
+            gated_tile<E, 2, 256>(c, x, w);
         } else if (p.bn == 128) {
-            gated_tile<E, 2, 128>(c, x, w, after);
+            gated_tile<E, 2, 128>(c, x, w);
         } else {
-            gated_tile<E, 1, 64>(c, x, w, after);
+            gated_tile<E, 1, 64>(c, x, w);
         }
     } else if (c.y_type == T8B_F32) {
         if (p.bn == 256) {
-            forward_tile<E, float, 2, 256>(c, x, w, after);
+            forward_tile<E, float, 2, 256>(c, x, w);
         } else if (p.bn == 128) {
-            forward_tile<E, float, 2, 128>(c, x, w, after);
+            forward_tile<E, float, 2, 128>(c, x, w);
         } else {
-            forward_tile<E, float, 1, 64>(c, x, w, after);
+            forward_tile<E, float, 1, 64>(c, x, w);
         }
     } else {
         if (p.bn == 256) {
-            forward_tile<E, E, 2, 256>(c, x, w, after);
+            forward_tile<E, E, 2, 256>(c, x, w);
         } else if (p.bn == 128) {
-            forward_tile<E, E, 2, 128>(c, x, w, after);
+            forward_tile<E, E, 2, 128>(c, x, w);
         } else {
-            forward_tile<E, E, 1, 64>(c, x, w, after);
+            forward_tile<E, E, 1, 64>(c, x, w);
         }
     }
 }
@@ -907,11 +916,12 @@ void product(const char* label, const Matrix& a, const Matrix& b, const GemmPlan
 template <typename E, bool GATED, int V>
 void activation_grad(const LinearGradCall& c, E* dz, int64_t pitch, float* sums) {
     const int columns = static_cast<int>(c.out);
-    const dim3 grid(blocks(columns, 32 * V), grad_parts(c.rows, GATED ? 2 * c.out : c.out));
-    constexpr int kRing = grad_ring_bytes<E, GATED, V>();
+    const dim3 grid(blocks(columns, 32 * V), grad_parts(c.rows, c.out));
+    constexpr size_t kRing = V == 8 ? kGradSmem : 0;
+    static_assert(grad_ring_bytes<E, GATED, V>() <= kRing, "ring");
     static uint64_t configured = 0;
     allow_smem(k_activation_grad<E, GATED, V>, kRing, configured);
-    launch("k_activation_grad", k_activation_grad<E, GATED, V>, grid, dim3(32, kGradRows), kRing, c.stream,
+    launch_chain("k_activation_grad", k_activation_grad<E, GATED, V>, grid, dim3(32, kGradRows), kRing, c.stream, true,
            static_cast<const E*>(c.dy), c.dy_stride, static_cast<const E*>(c.pre), c.pre_stride, c.rows, columns, c.activation, dz,
            pitch, sums);
     check(cudaGetLastError(), "activation gradient");
@@ -920,7 +930,7 @@ void activation_grad(const LinearGradCall& c, E* dz, int64_t pitch, float* sums)
 template <typename E>
 void linear_backward(const LinearGradCall& c) {
     const int64_t columns = c.gated ? 2 * c.out : c.out;
-    const Workspace at(c.rows, c.in, columns, c.what);
+    const Workspace at(c.rows, c.in, c.out, c.gated, c.what);
     // dz is dy itself where there is neither a gate nor an activation and its rows suit TMA
     E* dz_out = (c.what & T8B_WORKSPACE_DZ) != 0 ? reinterpret_cast<E*>(c.workspace + at.dz) : nullptr;
     float* sums = c.dbias ? reinterpret_cast<float*>(c.workspace + at.sums) : nullptr;
@@ -942,8 +952,8 @@ void linear_backward(const LinearGradCall& c) {
     Matrix w{}, x{};
     if (c.dx) w = operand<E>(c.weight, columns, c.in, c.weight_stride, c.workspace + at.weight, jobs[0]);
     if (c.dweight) x = operand<E>(c.x, c.rows, c.in, c.x_stride, c.workspace + at.x, jobs[1]);
-    const bool packed = pack<E>(jobs, dz_out || sums ? kBeside : kNothing, c.stream);
-    int after = dz_out || sums || packed ? kInput : kNothing;
+    pack<E>(jobs, dz_out || sums ? kBeside : kInput, c.stream);
+    int after = kInput;
     Totals totals{};
     if (c.dx) {
         product<E, false>("k_input_grad", dz, transposed(w), plan_gemm(c.rows, c.in, columns, false), after, c.dx, c.dx_stride,
@@ -957,7 +967,7 @@ void linear_backward(const LinearGradCall& c) {
     unsigned grid = totals.join_blocks;
     if (sums) {
         totals.sums = sums;
-        totals.sums_rows = grad_parts(c.rows, columns);
+        totals.sums_rows = grad_parts(c.rows, c.out);
         totals.bias_columns = static_cast<int>(columns);
         totals.dbias = c.dbias;
         totals.bias_type = c.bias_type;

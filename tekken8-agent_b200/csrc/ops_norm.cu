@@ -268,6 +268,8 @@ __global__ void __launch_bounds__(kThreads, resident_blocks(G, false)) k_norm_fo
     constexpr int NV = HELD / V;
     using Ring = ForwardRing<TX, V, NV>;
     constexpr int S = Ring::kStages;
+    wait_previous();
+    release_next();
     extern __shared__ __align__(16) unsigned char ring[];
     __shared__ __align__(8) float shared[2][kWideThreads / 32][2];
     int turn = 0;
@@ -354,6 +356,8 @@ __global__ void __launch_bounds__(kThreads, resident_blocks(G, true)) k_norm_bac
     constexpr int NV = HELD / V;
     using Ring = BackwardRing<TX, TY, V, NV>;
     constexpr int S = Ring::kStages;
+    wait_previous();
+    release_next();
     extern __shared__ __align__(16) unsigned char ring[];
     __shared__ __align__(8) float shared[2][kWideThreads / 32][2];
     int turn = 0;
@@ -486,6 +490,7 @@ __global__ void __launch_bounds__(kThreads, resident_blocks(G, true)) k_norm_bac
 // dw and db from the blocks' sums, in a fixed order. Block (32, kPartialRows): 32 columns.
 __global__ void k_norm_parameters(const float* partial, int count, int n, void* dw, void* db, int type) {
     wait_previous();
+    release_next();
     __shared__ float sums[kPartialRows][33];
     void* out = blockIdx.y ? db : dw;
     if (out == nullptr) return;
@@ -623,13 +628,14 @@ int launch_norm(const Norm& a, bool backward, int sms, cudaStream_t stream) {
         constexpr int kJoined = G ? kThreads * held_of(G) * 4 : 0;
         static uint64_t configured = 0;
         allow_smem(k_norm_backward<TX, TY, V, SHIFT, G>, std::max(Ring::kStages * Ring::kBytes * kThreads, kJoined), configured);
-        launch("k_norm_backward", k_norm_backward<TX, TY, V, SHIFT, G>, grid, threads,
-               std::max(Ring::kStages * Ring::kBytes * threads, kJoined), stream, a);
+        launch_chain("k_norm_backward", k_norm_backward<TX, TY, V, SHIFT, G>, grid, threads,
+                     std::max(Ring::kStages * Ring::kBytes * threads, kJoined), stream, true, a);
     } else {
         using Ring = ForwardRing<TX, V, held_of(G) / V>;
         static uint64_t configured = 0;
         allow_smem(k_norm_forward<TX, TY, V, SHIFT, G>, Ring::kStages * Ring::kBytes * kThreads, configured);
-        launch("k_norm_forward", k_norm_forward<TX, TY, V, SHIFT, G>, grid, threads, Ring::kStages * Ring::kBytes * threads, stream, a);
+        launch_chain("k_norm_forward", k_norm_forward<TX, TY, V, SHIFT, G>, grid, threads, Ring::kStages * Ring::kBytes * threads,
+                     stream, true, a);
     }
     return grid;
 }

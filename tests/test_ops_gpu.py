@@ -506,6 +506,70 @@ def test_leading_axes_and_other_streams(cuda):
     assert torch.equal(y, y2) and torch.equal(grads[1], ops.gated_backward(y2, n2, w, None, pre2)[1])
 
 
+def test_calls_between_other_work(cuda):
+    """An operator's kernels may start before the work ahead of them has ended; they see it all the
+    same: behind copies, other kernels, events of other streams, themselves, and so in a captured
+    graph. Integer-valued data make every sum exact, so equality is of bits."""
+    import torch
+    from t8b import ops
+    E = torch.bfloat16
+    g = torch.Generator(device="cuda").manual_seed(9)
+    rows, n = 4096, 256
+    w = torch.randint(-1, 2, (n, n), device="cuda", generator=g).to(E)
+    w2 = torch.randint(-1, 2, (2 * n, n), device="cuda", generator=g).to(E)
+    side = torch.cuda.Stream()
+    inputs = [torch.randint(-2, 3, (rows, n), device="cuda", generator=g).to(E) for _ in range(6)]
+
+    def chain(x):
+        """Every way in: a copy, a kernel of torch's, a wait for another stream, memory cleared."""
+        at = torch.empty_like(x)
+        at.copy_(x)
+        y = ops.linear(at, w, activation="relu")                       # behind a copy
+        y = (y * 0.0625).round()                                        # behind an operator
+        fork = torch.cuda.current_stream()
+        side.wait_stream(fork)
+        with torch.cuda.stream(side):
+            z = ops.gated(y.clamp(-4, 4), w2, activation="relu")
+            z = (z * 2.0 ** -12).round()
+        fork.wait_stream(side)
+        zero = torch.zeros_like(z)                                      # a memset
+        few = ops.linear((z + zero)[:3].clamp(-4, 4), w)
+        dx, dw, _ = ops.linear_backward(y.clamp(-4, 4), at, w)          # behind a wait
+        h = ops.layer_norm(dx, out_dtype=torch.float32)
+        return y, z, few, dx, dw, h, ops.layer_norm(h)                  # behind itself
+
+    torch.cuda.synchronize()
+    want = []
+    for x in inputs:
+        out = chain(x)
+        torch.cuda.synchronize()
+        want.append([t.clone() for t in out])
+    x64 = inputs[0].double()
+    assert torch.equal(want[0][0].double(), ((x64 @ w.double().T).clamp(min=0) .to(E).double() * 0.0625).to(E).double().round())
+    for _ in range(3):  # nothing waited for between the calls
+        got = [chain(x) for x in inputs]
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert all(torch.equal(p, q) for p, q in zip(a, b))
+    graph = torch.cuda.CUDAGraph()
+    static = inputs[0].clone()
+    with torch.cuda.graph(graph):
+        out = chain(static)
+    for x, b in zip(inputs, want):
+        static.copy_(x)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(out, b))
+    first = torch.cuda.CUDAGraph()  # an operator as a graph's first node
+    with torch.cuda.graph(first):
+        y = ops.layer_norm(static)
+    static.copy_(inputs[3])
+    first.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, ops.layer_norm(inputs[3]))
+    ops.status()
+
+
 def test_operators_refuse_what_they_cannot_take(cuda):
     import torch
     from t8b import ops
