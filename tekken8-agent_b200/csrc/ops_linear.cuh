@@ -54,12 +54,12 @@ constexpr int kMaxSplits = 64;
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Cycles of the busiest CTA as the plan's cost: waves x (k blocks x cycles + the tile's latency), plus
-// the pass that joins the parts (its traffic over the chip's, and its launch). The cycles are fits to
+// the pass that joins the parts (its traffic over the chip's, and `join_cycles`). The cycles are fits to
 // measured products: a narrower tile costs nearly as many a k-block, because what the MMAs read from
 // shared memory bounds them, and less latency. 65,536 x 512 x 512 took 42.7 / 54.0 / 88.2 us by
 // 256 / 128 / 64 columns, 4,096 rows of it 12.4 / 10.5 / 12.2, 512 rows 10.8 / 10.5 / 8.4; its weight's
 // gradient 41 us in 18 parts, 318 in one.
-inline GemmPlan plan_gemm(int64_t m, int64_t n, int64_t k, bool may_split) {
+inline GemmPlan plan_gemm(int64_t m, int64_t n, int64_t k, bool may_split, double join_cycles = 4000) {
     struct Form {
         int pair, bn;
         double block_cycles, tile_cycles;
@@ -77,7 +77,7 @@ inline GemmPlan plan_gemm(int64_t m, int64_t n, int64_t k, bool may_split) {
             const int64_t splits = wave == 0 ? 1 : std::min<int64_t>(most, std::max<int64_t>(1, wave * workers / tiles));
             const double waves = static_cast<double>(ceil_div(tiles * splits, workers));
             double cost = waves * (static_cast<double>(ceil_div(k_blocks, splits)) * f.block_cycles + f.tile_cycles);
-            if (splits > 1) cost += 4000.0 + static_cast<double>(splits) * m * n * 8.0 / 2500.0;
+            if (splits > 1) cost += join_cycles + static_cast<double>(splits) * m * n * 8.0 / 2500.0;
             if (cost < least) {
                 least = cost;
                 best = GemmPlan{f.bn, static_cast<int>(splits)};
@@ -93,9 +93,21 @@ inline GemmPlan plan_gemm(int64_t m, int64_t n, int64_t k, bool may_split) {
 // rows 26 / 16.5.
 inline bool is_few(int64_t rows, int64_t in) { return rows <= 4 || (rows <= 16 && in <= 512); }
 
+// The gradients' products. The weight's sums over the rows and is split wherever that pays; the input's
+// where few rows leave SMs idle behind a long sum over the columns: whole backward passes in us, one part
+// / split, linear 64 x 512 x 1,408 10.9 / 9.0, 64 x 512 x 8,192 43 / 17.7, 2,048 x 512 x 8,192 63 / 41,
+// gated 64 x 512 x 4,096 45 / 19.6. Never above 16,384 rows, where tiles of any width fill the chip.
+// The other product runs beside it on the SMs it leaves, so its split has to save more: at the cost
+// of a lone join 512 x 512 x 1,408 took 14.5 for 11.4.
+inline GemmPlan weight_grad_plan(int64_t rows, int64_t in, int64_t columns) { return plan_gemm(columns, in, rows, true); }
+inline GemmPlan input_grad_plan(int64_t rows, int64_t in, int64_t columns) {
+    return plan_gemm(rows, in, columns, rows <= 16384, 8000);
+}
+
 // The parts of a split GEMM: fp32 [splits][rows to whole tiles][columns to whole pieces].
 inline size_t split_rows(int64_t m) { return round_up(m, 256); }
 inline size_t split_pitch(int64_t n) { return round_up(n, 4); }
+inline size_t split_bytes(const GemmPlan& p, int64_t m, int64_t n) { return p.splits * split_rows(m) * split_pitch(n) * 4; }
 
 // Row parts of the elementwise backward pass over dy's columns (each gives one row of partial column
 // sums): with 256 columns a block, two blocks an SM, and no more resident, so that they spread evenly
@@ -111,7 +123,7 @@ inline int grad_parts(int64_t rows, int64_t out) {
 // The workspace of a call, in this order and as far as `what` (T8B_WORKSPACE_* bits) says; each part
 // starts on a 256-byte boundary.
 struct Workspace {
-    size_t x, weight, dz, sums, parts, bytes;
+    size_t x, weight, dz, sums, weight_parts, input_parts, bytes;
     size_t dz_pitch;
     Workspace(int64_t rows, int64_t in, int64_t out, bool gated, int what) {
         const int64_t columns = gated ? 2 * out : out;
@@ -128,8 +140,10 @@ struct Workspace {
         weight = take((what & T8B_WORKSPACE_WEIGHT) != 0, columns * x_pitch * 2);
         dz = take(backward && (what & T8B_WORKSPACE_DZ) != 0, rows * dz_pitch * 2);
         sums = take(backward, static_cast<size_t>(grad_parts(rows, out)) * columns * 4);
-        const int splits = backward ? plan_gemm(columns, in, rows, true).splits : 1;
-        parts = take(splits > 1, splits * split_rows(columns) * split_pitch(in) * 4);
+        const GemmPlan one{0, 1}, of_weight = backward ? weight_grad_plan(rows, in, columns) : one;
+        const GemmPlan of_input = backward ? input_grad_plan(rows, in, columns) : one;
+        weight_parts = take(of_weight.splits > 1, split_bytes(of_weight, columns, in));
+        input_parts = take(of_input.splits > 1, split_bytes(of_input, rows, in));
         bytes = at;
     }
 };
@@ -607,16 +621,19 @@ __global__ void __launch_bounds__(32 * kGradRows, V == 8 ? kGradBlocks : 5)
     }
 }
 
-// What the last pass of a backward adds up, in a fixed order: the parts of a split weight gradient
-// (rounded once), four columns a thread, and the block rows' column sums of dz (dbias), 32 columns a
-// block. The first `join_blocks` blocks do the one, the others the other. Block (32, 8).
-struct Totals {
+// What the last pass of a backward adds up, in a fixed order: the parts of split gradients (rounded
+// once), four columns a thread, and the block rows' column sums of dz (dbias), 32 columns a block. The
+// first blocks join the weight's gradient, the next the input's, the others the bias's. Block (32, 8).
+struct Join {
     const float* parts;
     size_t part_elements;
     int splits, pitch, rows, columns;
     void* out;
     int64_t stride;
-    unsigned join_blocks;
+    unsigned blocks;
+};
+struct Totals {
+    Join weight, input;
     const float* sums;
     int sums_rows, bias_columns;
     void* dbias;
@@ -626,15 +643,19 @@ template <typename E>
 __global__ void __launch_bounds__(256) k_totals(Totals a) {
     wait_previous();
     release_next();
-    if (blockIdx.x < a.join_blocks) {
-        const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.y * 32 + threadIdx.x;
-        const int pieces = a.pitch / 4;
-        if (i >= static_cast<int64_t>(a.rows) * pieces) return;
+    const unsigned joins = a.weight.blocks + a.input.blocks;
+    if (blockIdx.x < joins) {
+        const bool first = blockIdx.x < a.weight.blocks;
+        const Join& join = first ? a.weight : a.input;
+        const unsigned block = first ? blockIdx.x : blockIdx.x - a.weight.blocks;
+        const int64_t i = static_cast<int64_t>(block) * 256 + threadIdx.y * 32 + threadIdx.x;
+        const int pieces = join.pitch / 4;
+        if (i >= static_cast<int64_t>(join.rows) * pieces) return;
         const int row = static_cast<int>(i / pieces), c = static_cast<int>(i % pieces) * 4;
-        const float* p = a.parts + static_cast<size_t>(row) * a.pitch + c;
+        const float* p = join.parts + static_cast<size_t>(row) * join.pitch + c;
         float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 8
-        for (int s = 0; s < a.splits; ++s, p += a.part_elements) {
+        for (int s = 0; s < join.splits; ++s, p += join.part_elements) {
             const float4 v = *reinterpret_cast<const float4*>(p);
             sum.x += v.x;
             sum.y += v.y;
@@ -642,15 +663,15 @@ __global__ void __launch_bounds__(256) k_totals(Totals a) {
             sum.w += v.w;
         }
         const float v[4] = {sum.x, sum.y, sum.z, sum.w};
-        E* to = static_cast<E*>(a.out) + static_cast<int64_t>(row) * a.stride + c;
+        E* to = static_cast<E*>(join.out) + static_cast<int64_t>(row) * join.stride + c;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            if (c + j < a.columns) to[j] = Element<E>::store(v[j]);
+            if (c + j < join.columns) to[j] = Element<E>::store(v[j]);
         }
         return;
     }
     __shared__ float joined[8][33];
-    const int c = (blockIdx.x - a.join_blocks) * 32 + threadIdx.x;
+    const int c = (blockIdx.x - joins) * 32 + threadIdx.x;
     float v = 0.0f;
     if (c < a.bias_columns) {
 #pragma unroll 8
@@ -872,10 +893,10 @@ void linear_forward(const LinearCall& c) {
 }
 
 // out [a.rows][b.rows] = A . B^T without bias or activation, in E; the parts of a split k go to
-// `parts`, and what is left to do to `totals`.
+// `parts`, and what is left to do to `join`.
 template <typename E, int CG, int BN, bool A_MN>
 void product_tile(const char* label, const Matrix& a, const Matrix& b, int splits, int after, void* out, int64_t stride,
-                  float* parts, Totals* totals, cudaStream_t stream) {
+                  float* parts, Join& join, cudaStream_t stream) {
     if (splits == 1) {
         using Epi = EpiLinear<E, E, BN, false>;
         Epi epi{};
@@ -883,33 +904,31 @@ void product_tile(const char* label, const Matrix& a, const Matrix& b, int split
         launch_gemm<E, CG, BN, A_MN, true>(label, a, b, b.rows, 0, 1, after, epi, stream);
         return;
     }
-    if constexpr (A_MN) {
-        using Epi = EpiLinear<E, float, BN, false>;
-        Epi epi{};
-        const int64_t rows = split_rows(a.rows), pitch = split_pitch(b.rows);
-        epi.y = tiled<float, Epi::kBytes>(parts, rows * splits, b.rows, pitch);
-        epi.split_rows = static_cast<int>(rows);
-        launch_gemm<E, CG, BN, A_MN, true>(label, a, b, b.rows, 0, splits, after, epi, stream);
-        totals->parts = parts;
-        totals->part_elements = static_cast<size_t>(rows) * pitch;
-        totals->splits = splits;
-        totals->pitch = static_cast<int>(pitch);
-        totals->rows = static_cast<int>(a.rows);
-        totals->columns = static_cast<int>(b.rows);
-        totals->out = out;
-        totals->stride = stride;
-        totals->join_blocks = blocks(a.rows * (pitch / 4), 256);
-    }
+    using Epi = EpiLinear<E, float, BN, false>;
+    Epi epi{};
+    const int64_t rows = split_rows(a.rows), pitch = split_pitch(b.rows);
+    epi.y = tiled<float, Epi::kBytes>(parts, rows * splits, b.rows, pitch);
+    epi.split_rows = static_cast<int>(rows);
+    launch_gemm<E, CG, BN, A_MN, true>(label, a, b, b.rows, 0, splits, after, epi, stream);
+    join.parts = parts;
+    join.part_elements = static_cast<size_t>(rows) * pitch;
+    join.splits = splits;
+    join.pitch = static_cast<int>(pitch);
+    join.rows = static_cast<int>(a.rows);
+    join.columns = static_cast<int>(b.rows);
+    join.out = out;
+    join.stride = stride;
+    join.blocks = blocks(a.rows * (pitch / 4), 256);
 }
 template <typename E, bool A_MN>
 void product(const char* label, const Matrix& a, const Matrix& b, const GemmPlan& p, int after, void* out, int64_t stride,
-             float* parts, Totals* totals, cudaStream_t stream) {
+             float* parts, Join& join, cudaStream_t stream) {
     if (p.bn == 256) {
-        product_tile<E, 2, 256, A_MN>(label, a, b, p.splits, after, out, stride, parts, totals, stream);
+        product_tile<E, 2, 256, A_MN>(label, a, b, p.splits, after, out, stride, parts, join, stream);
     } else if (p.bn == 128) {
-        product_tile<E, 2, 128, A_MN>(label, a, b, p.splits, after, out, stride, parts, totals, stream);
+        product_tile<E, 2, 128, A_MN>(label, a, b, p.splits, after, out, stride, parts, join, stream);
     } else {
-        product_tile<E, 1, 64, A_MN>(label, a, b, p.splits, after, out, stride, parts, totals, stream);
+        product_tile<E, 1, 64, A_MN>(label, a, b, p.splits, after, out, stride, parts, join, stream);
     }
 }
 
@@ -956,15 +975,15 @@ void linear_backward(const LinearGradCall& c) {
     int after = kInput;
     Totals totals{};
     if (c.dx) {
-        product<E, false>("k_input_grad", dz, transposed(w), plan_gemm(c.rows, c.in, columns, false), after, c.dx, c.dx_stride,
-                          nullptr, nullptr, c.stream);
+        product<E, false>("k_input_grad", dz, transposed(w), input_grad_plan(c.rows, c.in, columns), after, c.dx, c.dx_stride,
+                          reinterpret_cast<float*>(c.workspace + at.input_parts), totals.input, c.stream);
         after = kBeside;
     }
     if (c.dweight) {
-        product<E, true>("k_weight_grad", transposed(dz), transposed(x), plan_gemm(columns, c.in, c.rows, true), after, c.dweight,
-                         c.dweight_stride, reinterpret_cast<float*>(c.workspace + at.parts), &totals, c.stream);
+        product<E, true>("k_weight_grad", transposed(dz), transposed(x), weight_grad_plan(c.rows, c.in, columns), after, c.dweight,
+                         c.dweight_stride, reinterpret_cast<float*>(c.workspace + at.weight_parts), totals.weight, c.stream);
     }
-    unsigned grid = totals.join_blocks;
+    unsigned grid = totals.weight.blocks + totals.input.blocks;
     if (sums) {
         totals.sums = sums;
         totals.sums_rows = grad_parts(c.rows, c.out);

@@ -320,6 +320,34 @@ def test_linear_and_gated_backward(cuda, rows, n, m, et, gated):
     ops.status()
 
 
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("rows,n,m", [(1, 65, 2816), (17, 512, 1408), (40, 96, 4096), (300, 151, 5001), (1025, 33, 3001)])
+@pytest.mark.parametrize("et", ["bf16", "f16"])
+def test_gradients_of_few_rows_and_many_columns(cuda, rows, n, m, et, gated):
+    """Long sums over the columns for few tiles of the input's gradient: its parts are joined in fp32."""
+    import torch
+    from t8b import ops
+    E = types()[et]
+    u = unit(E) * (1 + 2 ** -8)
+    g = torch.Generator(device="cuda").manual_seed(rows + 3 * n + 11 * m)
+    columns = 2 * m if gated else m
+    fn = ops.gated_backward if gated else ops.linear_backward
+    for slack in (0, 3):
+        x, dy = matrix(g, rows, n, E, slack, 0), matrix(g, rows, m, E, slack, 0, 0.125)
+        w, pre = matrix(g, columns, n, E, slack, 0, n ** -0.5), matrix(g, rows, columns, E, slack, 0, 1.5)
+        b = bias_of(g, "f32", columns, E)
+        dz, slip = backward64(dy, x, w, pre, "silu", gated)
+        rounded = slip + u * dz.abs() + tiny(E)
+        w64, x64 = w.double(), x.double()
+        first = fn(dy, x, w, b, pre, activation="silu")
+        close(first[0], dz @ w64, rounded @ w64.abs() + (columns + 16) * 2.0 ** -23 * (dz.abs() @ w64.abs()), f"dx {slack}")
+        close(first[1], dz.T @ x64, rounded.T @ x64.abs() + (rows + 16) * 2.0 ** -23 * (dz.abs().T @ x64.abs()), f"dw {slack}")
+        close(first[2], dz.sum(0), slip.sum(0) + (rows + 16) * 2.0 ** -24 * dz.abs().sum(0), f"db {slack}")
+        dx, dw, db = fn(dy, x, w, None, pre, activation="silu")  # no bias: the joins alone in the last pass
+        assert db is None and torch.equal(dx, first[0]) and torch.equal(dw, first[1])
+    ops.status()
+
+
 @pytest.mark.parametrize("name", ["norm", "linear", "gated"])
 def test_gradients_against_differences(cuda, name):
     """The gradient along a random direction equals the loss's central difference along it, taken
