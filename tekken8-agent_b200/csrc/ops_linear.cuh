@@ -87,10 +87,10 @@ inline GemmPlan plan_gemm(int64_t m, int64_t n, int64_t k, bool may_split, doubl
     return best;
 }
 
-// Whether a forward pass goes row by row (k_few_rows) and not by tiles: measured (bf16, us by rows /
-// by tiles), 512 -> 512: 1 row 4.2 / 8.3, 16 rows 6.2 / 8.3, 64 rows 10.3 / 8.3; gated 512 -> 1,408:
-// 16 rows 8.3 / 8.3, 24 rows 12.4 / 8.3; 2,048 -> 2,048: 1 row 6.2 / 16.5, 4 rows 9.2 / 16.5, 16
-// rows 26 / 16.5.
+// Whether a forward pass goes row by row (k_few_rows) and not by tiles: measured (bf16, us a call among
+// others, by rows / by tiles), 512 -> 512: 1 row 2.2 / 5.6, 16 rows 5.0 / 5.6, 64 rows 9.2 / 5.6; gated 512 ->
+// 1,408: 16 rows 7.0 / 6.6, 24 rows 11.6 / 6.6; 2,048 -> 2,048: 1 row 4.1 / 13.1, 4 rows 7.5 / 13.1, 8
+// rows 14.7 / 13.1; 4,096 -> 512: 4 rows 12.1 / 22.5, 8 rows 25.6 / 22.5.
 inline bool is_few(int64_t rows, int64_t in) { return rows <= 4 || (rows <= 16 && in <= 512); }
 
 // The gradients' products. The weight's sums over the rows and is split wherever that pays; the input's
