@@ -427,15 +427,19 @@ __global__ void __launch_bounds__(kThreads, resident_blocks(G, true)) k_norm_bac
             const Two off(-mean, -mean), scaled(rstd, rstd);
 #pragma unroll
             for (int i = 0; i < HELD / 2; ++i) {
-                v[i] = (v[i] + off) * scaled;  // beyond the row dy is 0, and so is all that v adds
-                if (live) dw[i] = multiply_add(g[i], v[i], dw[i]);
+                // Beyond the row x and dy are 0 and add 0 to every sum. sum(g xhat) is rstd times sum(g
+                // (x - mean)): a product with xhat would be 0 * inf there where mean * rstd overflows.
+                v[i] = v[i] + off;
+                const Two xhat = v[i] * scaled;
+                if (live) dw[i] = multiply_add(g[i], xhat, dw[i]);
                 db[i] = db[i] + g[i];
                 g[i] = g[i] * w[i];
                 of_g = of_g + g[i];
                 of_gx = multiply_add(g[i], v[i], of_gx);
+                v[i] = xhat;
             }
         }
-        float sum[2] = {of_g.sum(), of_gx.sum()};
+        float sum[2] = {of_g.sum(), of_gx.sum() * rstd};
         row_sum<LANES>(sum, shared, turn);
         if (live) {
             const float c0 = -rstd * (sum[0] * scale), c1 = -rstd * (sum[1] * scale);

@@ -1,0 +1,33 @@
+"""Edges of the torso operators: values, arguments and streams at which they could go wrong."""
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("n", [1, 100, 151, 320, 515, 700, 1500, 2049, 8185])
+@pytest.mark.parametrize("type_name", ["float32", "bfloat16"])
+def test_layer_norm_backward_of_constant_rows_of_large_values(cuda, n, type_name):
+    """xhat of a constant row is 0, so dx = rstd (g - mean(g)) + residual and dweight's term is 0, however
+    large mean * rstd is: what a thread holds beyond the row must not enter. Small integers in dy make
+    n * mean(g) exact; dx is off by the roundings of mean(g), the difference and two products, each
+    2^-24 of rstd times (|g| + |mean(g)|) at most, and by its own rounding."""
+    import torch
+    from t8b import ops
+    T = getattr(torch, type_name)
+    rows, eps = 37, 1e-5
+    g = torch.Generator(device="cuda").manual_seed(n)
+    x = torch.full((rows, n), 2.0 ** 121, device="cuda", dtype=T)  # 2^121 / sqrt(1e-5) > 2^128
+    x[1::2] = -1.0
+    dy = torch.randint(-3, 4, (rows, n), device="cuda", generator=g).to(T)
+    w, b = torch.ones(n, device="cuda"), torch.zeros(n, device="cuda")
+    mean = x[:, 0].float().contiguous()
+    rstd = torch.full((rows,), eps ** -0.5, device="cuda")
+    dx, dw, db = ops.layer_norm_backward(dy, x, w, b, mean, rstd)
+    d, r = dy.double(), rstd.double()[:, None]
+    average = d.mean(1, keepdim=True)
+    want = r * (d - average)
+    unit = 2.0 ** -24 if T is torch.float32 else 2.0 ** -8
+    limit = 8 * 2.0 ** -24 * r * (d.abs() + average.abs()) + unit * want.abs()
+    assert bool(((dx.double() - want).abs() <= limit).all())
+    assert not dw.any()
+    assert torch.equal(db.double(), d.sum(0))
