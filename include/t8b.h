@@ -555,7 +555,8 @@ int t8b_rollout_synchronize(t8b_rollout* rollout, void* stream);
  * Operators of a residual policy torso (no reference counterpart: the reference's network is two
  * tanh layers). A matrix is row-major: `rows` rows of consecutive elements, `stride` elements
  * from one row's start to the next's, which may be anything from the row's length up; vectors
- * (weights of a norm, biases, mean, rstd) are packed. All pointers are device pointers. Nothing
+ * (weights of a norm, biases, mean, rstd) are packed. All pointers are device pointers, each aligned to
+ * its elements (others are refused). Nothing
  * is allocated: what a call needs beside its outputs is a workspace (256-byte aligned) of the
  * size that the query beside it gives for the same sizes, free again once the call's work on
  * `stream` is done. Work is queued on `stream` of the current device and ordered on it alone;

@@ -197,10 +197,15 @@ inline bool is_type(int type) { return type == T8B_F32 || type == T8B_BF16 || ty
 inline bool aligned(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) % bytes) == 0; }
 inline size_t round_up(size_t v, size_t to) { return (v + to - 1) / to * to; }
 
+// An array argument (or NULL): the kernels read it by whole elements.
+inline void check_elements(const char* what, const void* data, size_t size) {
+    if (!aligned(data, size)) raise(T8B_EINVAL, std::string(what) + ": a pointer that is not aligned to its elements");
+}
 // A row-major matrix argument: its rows must not overlap, its last element must be addressable.
-inline void check_matrix(const char* what, const void* data, int64_t rows, int64_t columns, int64_t stride) {
+inline void check_matrix(const char* what, const void* data, int64_t rows, int64_t columns, int64_t stride, size_t size) {
     if (rows == 0) return;
     if (data == nullptr) raise(T8B_EINVAL, std::string(what) + " is null");
+    check_elements(what, data, size);
     if (rows > 1 && stride < columns) raise(T8B_EINVAL, std::string(what) + ": a row stride below the row's length");
     if (stride < 0 || (rows > 1 && stride > std::numeric_limits<int64_t>::max() / 8 / rows)) {
         raise(T8B_EINVAL, std::string(what) + ": the row stride is out of range");

@@ -53,13 +53,14 @@ void forward(const char* what, int type, LinearCall& c, void* workspace, size_t 
     check_sizes(what, c.rows, c.in, c.out);
     check_types(what, type, c.bias != nullptr, c.bias_type, c.y_type, c.activation);
     const int64_t columns = c.gated ? 2 * c.out : c.out;
-    check_matrix(what, c.x, c.rows, c.in, c.x_stride);
-    check_matrix(what, c.weight, columns, c.in, c.weight_stride);
-    check_matrix(what, c.y, c.rows, c.out, c.y_stride);
-    if (c.residual) check_matrix(what, c.residual, c.rows, c.out, c.residual_stride);
-    if (c.pre) check_matrix(what, c.pre, c.rows, columns, c.pre_stride);
-    if (c.rows == 0) return;
     const size_t ys = type_size(c.y_type);
+    check_matrix(what, c.x, c.rows, c.in, c.x_stride, 2);
+    check_matrix(what, c.weight, columns, c.in, c.weight_stride, 2);
+    check_matrix(what, c.y, c.rows, c.out, c.y_stride, ys);
+    if (c.residual) check_matrix(what, c.residual, c.rows, c.out, c.residual_stride, ys);
+    if (c.pre) check_matrix(what, c.pre, c.rows, columns, c.pre_stride, 2);
+    if (c.bias) check_elements(what, c.bias, type_size(c.bias_type));
+    if (c.rows == 0) return;
     const Span x(c.x, c.rows, c.in, c.x_stride, 2), w(c.weight, columns, c.in, c.weight_stride, 2);
     const Span y(c.y, c.rows, c.out, c.y_stride, ys), pre(c.pre, c.rows, columns, c.pre_stride, 2);
     const Span residual(c.residual, c.rows, c.out, c.residual_stride, ys);
@@ -86,17 +87,18 @@ void backward(const char* what, int type, LinearGradCall& c, void* workspace, si
     check_sizes(what, c.rows, c.in, c.out);
     check_types(what, type, c.dbias != nullptr, c.bias_type, type, c.activation);
     const int64_t columns = c.gated ? 2 * c.out : c.out;
-    check_matrix(what, c.dy, c.rows, c.out, c.dy_stride);
+    check_matrix(what, c.dy, c.rows, c.out, c.dy_stride, 2);
     const bool reads_pre = c.gated || c.activation != T8B_LINEAR;
     if (reads_pre) {
-        check_matrix(what, c.pre, c.rows, columns, c.pre_stride);
+        check_matrix(what, c.pre, c.rows, columns, c.pre_stride, 2);
     } else {
         c.pre = nullptr;
     }
-    if (c.dx) check_matrix(what, c.weight, columns, c.in, c.weight_stride);
-    if (c.dx) check_matrix(what, c.dx, c.rows, c.in, c.dx_stride);
-    if (c.dweight) check_matrix(what, c.x, c.rows, c.in, c.x_stride);
-    if (c.dweight) check_matrix(what, c.dweight, columns, c.in, c.dweight_stride);
+    if (c.dx) check_matrix(what, c.weight, columns, c.in, c.weight_stride, 2);
+    if (c.dx) check_matrix(what, c.dx, c.rows, c.in, c.dx_stride, 2);
+    if (c.dweight) check_matrix(what, c.x, c.rows, c.in, c.x_stride, 2);
+    if (c.dweight) check_matrix(what, c.dweight, columns, c.in, c.dweight_stride, 2);
+    if (c.dbias) check_elements(what, c.dbias, type_size(c.bias_type));
     if (c.rows == 0) {
         if (c.dweight) {
             check(cudaMemset2DAsync(c.dweight, c.dweight_stride * 2, 0, c.in * 2, columns, c.stream), "clear dweight");

@@ -723,8 +723,10 @@ extern "C" int t8b_layer_norm_forward(const void* x, int x_type, int64_t x_strid
         if (!(epsilon >= 0.0f) || epsilon > std::numeric_limits<float>::max()) {
             raise(T8B_EINVAL, "layer norm: epsilon must be finite and not negative");
         }
-        check_matrix("layer norm x", x, rows, n, x_stride);
-        check_matrix("layer norm y", y, rows, n, y_stride);
+        check_matrix("layer norm x", x, rows, n, x_stride, type_size(x_type));
+        check_matrix("layer norm y", y, rows, n, y_stride, type_size(y_type));
+        for (const void* vector : {weight, bias}) check_elements("layer norm parameters", vector, type_size(parameter_type));
+        for (const float* vector : {mean, rstd}) check_elements("layer norm mean and rstd", vector, sizeof(float));
         if (rows == 0) return;
         const Span to(y, rows, n, y_stride, type_size(y_type)), from(x, rows, n, x_stride, type_size(x_type));
         if (to.overlaps(from) && !(x == y && x_stride == y_stride && x_type == y_type && n <= kMostColumns)) {
@@ -764,10 +766,15 @@ extern "C" int t8b_layer_norm_backward(const void* dy, int y_type, int64_t dy_st
     return guarded([&] {
         check_sizes(rows, n);
         if (!is_type(x_type) || !is_type(y_type) || !is_type(parameter_type)) raise(T8B_EINVAL, "layer norm: unknown type");
-        check_matrix("layer norm dy", dy, rows, n, dy_stride);
-        check_matrix("layer norm x", x, rows, n, x_stride);
-        check_matrix("layer norm dx", dx, rows, n, dx_stride);
-        if (residual_gradient) check_matrix("layer norm residual gradient", residual_gradient, rows, n, residual_stride);
+        const size_t xs = type_size(x_type), ys = type_size(y_type);
+        check_matrix("layer norm dy", dy, rows, n, dy_stride, ys);
+        check_matrix("layer norm x", x, rows, n, x_stride, xs);
+        check_matrix("layer norm dx", dx, rows, n, dx_stride, xs);
+        if (residual_gradient) check_matrix("layer norm residual gradient", residual_gradient, rows, n, residual_stride, xs);
+        for (const void* vector : {weight, static_cast<const void*>(dweight), static_cast<const void*>(dbias)}) {
+            check_elements("layer norm parameters", vector, type_size(parameter_type));
+        }
+        for (const float* vector : {mean, rstd}) check_elements("layer norm mean and rstd", vector, sizeof(float));
         if (rows > 0 && (mean == nullptr || rstd == nullptr)) raise(T8B_EINVAL, "layer norm: mean and rstd are null");
         cudaStream_t st = static_cast<cudaStream_t>(stream);
         const bool parameters = dweight != nullptr || dbias != nullptr;
@@ -776,7 +783,6 @@ extern "C" int t8b_layer_norm_backward(const void* dy, int y_type, int64_t dy_st
             if (dbias) check(cudaMemsetAsync(dbias, 0, n * type_size(parameter_type), st), "clear dbias");
             return;
         }
-        const size_t xs = type_size(x_type), ys = type_size(y_type);
         const Span to(dx, rows, n, dx_stride, xs);
         if (to.overlaps(Span(x, rows, n, x_stride, xs)) || to.overlaps(Span(dy, rows, n, dy_stride, ys)) ||
             to.overlaps(Span(residual_gradient, rows, n, residual_stride, xs))) {
