@@ -87,10 +87,12 @@ def gated_backward(dh, x, weight, bias=None, pre=None, activation: str = "silu",
     return _operators.gated_backward(dh, x, weight, bias, pre, activation, input_gradient)
 
 
-def status(stream=None):
-    """Waits for `stream` (torch's current one) and raises T8bError if a wait inside an operator's
-    kernel ran out of its limit since the last call: that call's outputs are not valid."""
-    raw = stream.cuda_stream if stream is not None else torch.cuda.current_stream().cuda_stream
-    result = _lib.lib().t8b_operators_status(raw)
+def status(stream=None, device=None):
+    """Waits for `stream` (by default torch's current one of `device`, or of the current device) and
+    raises T8bError if a wait inside an operator's kernel ran out of its limit on that device since the
+    last call: that call's outputs are not valid. Each device keeps its own record."""
+    with torch.cuda.device(stream.device if stream is not None else device):
+        raw = (stream if stream is not None else torch.cuda.current_stream()).cuda_stream
+        result = _lib.lib().t8b_operators_status(raw)
     if result != T8B_OK:
         raise T8bError(result, _lib.lib().t8b_last_error().decode())

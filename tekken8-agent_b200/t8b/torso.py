@@ -122,7 +122,7 @@ def fit(torso: ResidualTorso, observations: torch.Tensor, targets: torch.Tensor,
             torso.parameters[name].grad = grads[name].to(torch.float32)
         optimizer.step()
         torso.refresh()
-    ops.status()
+    ops.status(device=observations.device)
     return losses
 
 

@@ -41,3 +41,52 @@ def test_pointers_off_their_elements_are_refused(entry, names, elements):
         for off in {1, size // 2}:
             assert call(entry, names, **{name: names[name] + off}) == _lib.T8B_EINVAL, (name, off)
             assert b"aligned to its elements" in _lib.lib().t8b_last_error(), (name, off)
+
+
+class FakeDevice:
+    """torch.cuda.device, as far as it says which device is current."""
+    current = 0
+
+    def __init__(self, device):
+        import torch
+        self.index = FakeDevice.current if device is None else torch.device(device).index
+
+    def __enter__(self):
+        self.before, FakeDevice.current = FakeDevice.current, self.index
+
+    def __exit__(self, *error):
+        FakeDevice.current = self.before
+
+
+class FakeStream:
+    def __init__(self, index):
+        import torch
+        self.device, self.cuda_stream = torch.device("cuda", index), 1000 + index
+
+
+def test_status_reads_the_record_of_the_streams_device(monkeypatch):
+    """The library answers for the current device: each stream's own has to be current."""
+    import torch
+    from t8b import _lib, ops
+    asked = []
+
+    class Library:
+        @staticmethod
+        def t8b_operators_status(raw):
+            asked.append((FakeDevice.current, raw))
+            return _lib.T8B_OK if FakeDevice.current != 2 else _lib.T8B_ECUDA
+
+        @staticmethod
+        def t8b_last_error():
+            return b"a wait ran out"
+
+    monkeypatch.setattr(torch.cuda, "device", FakeDevice)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: FakeStream(FakeDevice.current))
+    monkeypatch.setattr(ops._lib, "lib", lambda: Library)
+    ops.status()
+    ops.status(FakeStream(1))
+    ops.status(device=torch.device("cuda", 3))
+    with pytest.raises(_lib.T8bError):
+        ops.status(FakeStream(2))
+    assert asked == [(0, 1000), (1, 1001), (3, 1003), (2, 1002)]
+    assert FakeDevice.current == 0
