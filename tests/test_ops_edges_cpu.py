@@ -90,3 +90,17 @@ def test_status_reads_the_record_of_the_streams_device(monkeypatch):
         ops.status(FakeStream(2))
     assert asked == [(0, 1000), (1, 1001), (3, 1003), (2, 1002)]
     assert FakeDevice.current == 0
+
+
+def test_a_stream_of_another_device_is_refused():
+    """A call runs where its tensors are; a stream elsewhere could not order it."""
+    import torch
+    from t8b import ops
+    x, w = torch.zeros(2, 8, dtype=torch.bfloat16), torch.zeros(4, 8, dtype=torch.bfloat16)
+    at = FakeStream(1)
+    for refused in (lambda: ops.linear(x, w, stream=at), lambda: ops.linear_backward(x, x, w, stream=at),
+                    lambda: ops.gated(x, w, stream=at), lambda: ops.gated_backward(x, x, w, stream=at),
+                    lambda: ops.layer_norm(x, stream=at),
+                    lambda: ops.layer_norm_backward(x, x, None, None, x, x, stream=at)):
+        with pytest.raises(ValueError, match="the stream is on cuda:1, x on cpu"):
+            refused()
