@@ -627,8 +627,12 @@ int t8b_gated_backward(int type, const void* dh, int64_t dh_stride, const void* 
                        int64_t rows, int64_t in, int64_t out, void* dx, int64_t dx_stride, void* dweight,
                        int64_t dweight_stride, void* dbias, void* workspace, size_t workspace_bytes, void* stream);
 /* Synchronises `stream` and reports whether a wait inside an operator's kernel ran out of its
- * limit on this device since the last call (T8B_ECUDA; the outputs of that call are not valid). */
+ * limit on the current device since the last call that reported one (T8B_ECUDA; the outputs of the
+ * calls queued since then are not valid). Each stall is reported once, by one caller. */
 int t8b_operators_status(void* stream);
+/* Test hook for it: queues a kernel whose one thread waits as the operators' kernels do, on a barrier
+ * that nothing arrives at, and gives up after spin_limit polls (at most 2^20). */
+int t8b_debug_operators_stall(uint32_t spin_limit, void* stream);
 
 #ifdef __cplusplus
 }

@@ -23,7 +23,7 @@
 // near 1.4 GHz by the power limit.
 // Operands are K-major (rows of K elements) or MN-major (K rows), see gemm.cuh.
 //
-// Every wait is bounded: a stall sets the error flag; the first CTA then waits (bounded) for the
+// Every wait is bounded: a stall is counted; the first CTA then waits (bounded) for the
 // loads in flight, the CTAs meet, free their tensor memory and return.
 #pragma once
 
@@ -233,7 +233,7 @@ struct Shape {
     int tiles_m, tiles_n, splits, k_blocks;
     int second;  // B's second half starts at this row (gated projections); 0: B is one matrix
     int after;   // what the kernel before this one is to it: kInput or kBeside
-    int* error;
+    unsigned* stalls;  // the device's count of waits that ran out
 };
 
 // A CTA's (or pair's) work items, one in `step`, columns fastest, then rows, then parts of k. Each
@@ -308,7 +308,7 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kGemmThreads, 1)
     volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     if ((tc::smem_addr(base) & 1023u) != 0) {  // the swizzles count on it; every thread sees the same
-        if (threadIdx.x == 0) atomicExch(s.error, 1);
+        if (threadIdx.x == 0) atomicAdd(s.stalls, 1u);
         return;
     }
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -337,7 +337,7 @@ __global__ void __cluster_dims__(CG, 1, 1) __launch_bounds__(kGemmThreads, 1)
     const int first = blockIdx.x / CG, step = gridDim.x / CG;
     auto stop = [&]() {
         *abort = 1;
-        atomicExch(s.error, 1);
+        atomicAdd(s.stalls, 1u);
     };
 
     if (warp == 0) {

@@ -1,5 +1,7 @@
-// C entries of the linear map and the gated projection: argument checks, and the flag of waits
+// C entries of the linear map and the gated projection: argument checks, and the count of waits
 // that ran out.
+#include <mutex>
+
 #include "ops_linear.cuh"
 
 namespace t8b {
@@ -10,17 +12,18 @@ extern template void linear_forward<f16>(const LinearCall&);
 extern template void linear_backward<bf16>(const LinearGradCall&);
 extern template void linear_backward<f16>(const LinearGradCall&);
 
-__device__ int g_stalled;
+// Only ever counted up: a reader that cleared it could lose a stall counted after its read.
+__device__ unsigned g_stalls;
 
-int* stall_flag() {
-    static std::atomic<int*> flags[64];
+unsigned* stall_count() {
+    static std::atomic<unsigned*> counts[64];
     int device = 0;
     check(cudaGetDevice(&device), "cudaGetDevice");
-    std::atomic<int*>& flag = flags[device & 63];
-    int* p = flag.load(std::memory_order_acquire);
+    std::atomic<unsigned*>& count = counts[device & 63];
+    unsigned* p = count.load(std::memory_order_acquire);
     if (p == nullptr) {
-        check(cudaGetSymbolAddress(reinterpret_cast<void**>(&p), g_stalled), "stall flag");
-        flag.store(p, std::memory_order_release);
+        check(cudaGetSymbolAddress(reinterpret_cast<void**>(&p), g_stalls), "stall count");
+        count.store(p, std::memory_order_release);
     }
     return p;
 }
@@ -198,14 +201,45 @@ extern "C" int t8b_gated_backward(int type, const void* dh, int64_t dh_stride, c
 extern "C" int t8b_operators_status(void* stream) {
     return guarded([&] {
         cudaStream_t st = static_cast<cudaStream_t>(stream);
-        int stalled = 0;
-        int* flag = stall_flag();
-        check(cudaMemcpyAsync(&stalled, flag, sizeof(int), cudaMemcpyDeviceToHost, st), "read stall flag");
-        check(cudaStreamSynchronize(st), "read stall flag");
-        if (stalled) {
-            check(cudaMemsetAsync(flag, 0, sizeof(int), st), "clear stall flag");
-            check(cudaStreamSynchronize(st), "clear stall flag");
-            raise(T8B_ECUDA, "a wait inside an operator's kernel ran out");
-        }
+        static std::mutex mutex;
+        static unsigned reported[64];
+        int device = 0;
+        check(cudaGetDevice(&device), "cudaGetDevice");
+        unsigned count = 0;
+        check(cudaMemcpyAsync(&count, stall_count(), sizeof(count), cudaMemcpyDeviceToHost, st), "read stall count");
+        check(cudaStreamSynchronize(st), "read stall count");
+        const std::lock_guard<std::mutex> lock(mutex);
+        unsigned& last = reported[device & 63];
+        if (static_cast<int>(count - last) <= 0) return;  // nothing new, or another caller has read further
+        last = count;
+        raise(T8B_ECUDA, "a wait inside an operator's kernel ran out");
+    });
+}
+
+namespace t8b {
+namespace op {
+namespace {
+
+// One thread waits as the products' kernels do, on a barrier that nothing arrives at, and counts the
+// stall as they do once `limit` polls are over.
+__global__ void k_stall(uint32_t limit, unsigned* stalls) {
+    __shared__ uint64_t bar;
+    __shared__ int abort;
+    if (threadIdx.x != 0) return;
+    abort = 0;
+    tc::bar_init(&bar, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    if (!tc::bar_wait(&bar, 0, &abort, limit)) atomicAdd(stalls, 1u);
+}
+
+}  // namespace
+}  // namespace op
+}  // namespace t8b
+
+extern "C" int t8b_debug_operators_stall(uint32_t spin_limit, void* stream) {
+    return guarded([&] {
+        if (spin_limit == 0 || spin_limit > (1u << 20)) raise(T8B_EINVAL, "operators stall: 1 to 2^20 polls");
+        launch("k_stall", k_stall, 1, 32, 0, static_cast<cudaStream_t>(stream), spin_limit, stall_count());
+        check(cudaGetLastError(), "operators stall");
     });
 }

@@ -12,8 +12,8 @@
 namespace t8b {
 namespace op {
 
-// The device's flag for waits that ran out (ops_linear.cu).
-int* stall_flag();
+// The device's count of waits that ran out (ops_linear.cu).
+unsigned* stall_count();
 
 struct LinearCall {
     const void *x, *weight, *bias, *residual;
@@ -747,7 +747,7 @@ void launch_gemm(const char* label, const Matrix& a, const Matrix& b, int64_t co
     s.splits = splits;
     s.second = second;
     s.after = after;
-    s.error = stall_flag();
+    s.stalls = stall_count();
     const auto k_major = [](const Matrix& m, uint32_t box) {
         return tensor_map<E>(m.data, m.k, m.rows, tma_pitch(m.rows, m.k, m.pitch, 2), tc::BK, box, CU_TENSOR_MAP_SWIZZLE_128B);
     };

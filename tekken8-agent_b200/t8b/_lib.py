@@ -380,4 +380,5 @@ PROTOTYPES.update({
     "t8b_gated_backward": (C.c_int, [C.c_int, vp, i64, vp, i64, vp, i64, vp, i64, C.c_int, C.c_int, i64, i64, i64, vp,
                                      i64, vp, i64, vp, vp, C.c_size_t, vp]),
     "t8b_operators_status": (C.c_int, [vp]),
+    "t8b_debug_operators_stall": (C.c_int, [C.c_uint32, vp]),
 })

@@ -31,3 +31,54 @@ def test_layer_norm_backward_of_constant_rows_of_large_values(cuda, n, type_name
     assert bool(((dx.double() - want).abs() <= limit).all())
     assert not dw.any()
     assert torch.equal(db.double(), d.sum(0))
+
+
+def test_each_stall_is_reported_once(cuda):
+    """A wait that ran out on one stream is reported whichever stream is asked, once, and not lost where
+    other threads ask meanwhile."""
+    import threading
+    import time
+    import torch
+    from t8b import _lib, ops
+    side, other = torch.cuda.Stream(), torch.cuda.Stream()
+
+    def stall():
+        _lib.call("t8b_debug_operators_stall", 64, side.cuda_stream)
+        side.synchronize()
+
+    ops.status()
+    stall()
+    with pytest.raises(_lib.T8bError, match="ran out"):
+        ops.status(other)
+    ops.status(side)
+    stall()
+    stall()
+    with pytest.raises(_lib.T8bError, match="ran out"):
+        ops.status()
+    ops.status()
+
+    reports, done = [], threading.Event()
+
+    def poll(stream):
+        while not done.is_set():
+            try:
+                ops.status(stream)
+            except _lib.T8bError:
+                reports.append(stream)
+
+    threads = [threading.Thread(target=poll, args=(s,)) for s in (other, torch.cuda.Stream())]
+    for t in threads:
+        t.start()
+    try:
+        for i in range(300):
+            stall()
+            until = time.monotonic() + 10
+            while len(reports) <= i and time.monotonic() < until:
+                time.sleep(0)
+            assert len(reports) == i + 1
+    finally:
+        done.set()
+        for t in threads:
+            t.join()
+    ops.status()
+    assert len(reports) == 300
