@@ -42,6 +42,7 @@ struct Refused : std::invalid_argument {
 struct Failed {
     int status;
 };
+struct Raised {};  // a Python exception that is set already
 [[noreturn]] void refuse(const std::string& why) { throw Refused(why); }
 
 std::string text(at::IntArrayRef shape) {
@@ -146,7 +147,11 @@ struct Arguments {
         return THPVariable_Unpack(at[i]);
     }
     Tensor optional(int i, const char* name) const { return at[i] == Py_None ? Tensor() : tensor(i, name); }
-    bool flag(int i) const { return PyObject_IsTrue(at[i]) == 1; }
+    bool flag(int i) const {
+        const int truth = PyObject_IsTrue(at[i]);
+        if (truth < 0) throw Raised();
+        return truth == 1;
+    }
     // a torch.dtype as a T8B type; None: `missing`
     int type(int i, int missing) const {
         if (at[i] == Py_None) return missing;
@@ -196,6 +201,7 @@ PyObject* answer(Body&& body) {
         return body();
     } catch (const Refused& error) {
         PyErr_SetString(PyExc_ValueError, error.what());
+    } catch (const Raised&) {
     } catch (const Failed& error) {
         PyObject* args = Py_BuildValue("(is)", error.status, entry.last_error());
         if (args != nullptr) {
@@ -226,7 +232,7 @@ PyObject* layer_norm(PyObject*, PyObject* const* args, Py_ssize_t given) {
         const Arguments a(args, given, 6);
         const Tensor x = a.tensor(0, "x"), weight = a.optional(1, "weight"), bias = a.optional(2, "bias");
         const double eps = PyFloat_AsDouble(args[3]);
-        if (eps == -1.0 && PyErr_Occurred()) return nullptr;
+        if (eps == -1.0 && PyErr_Occurred()) throw Raised();
         const On on(x);
         const int x_type = type_of(x, "x"), y_type = a.type(4, x_type);
         const int64_t n = x.dim() ? x.size(-1) : 0;

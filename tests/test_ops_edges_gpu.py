@@ -82,3 +82,20 @@ def test_each_stall_is_reported_once(cuda):
             t.join()
     ops.status()
     assert len(reports) == 300
+
+
+def test_an_option_without_a_truth_value_raises_its_own_error(cuda):
+    import torch
+    from t8b import ops
+
+    class Neither:
+        def __bool__(self):
+            raise KeyError("neither")
+
+    x, w = torch.zeros(4, 16, device="cuda").bfloat16(), torch.zeros(8, 16, device="cuda").bfloat16()
+    y = torch.zeros(4, 8, device="cuda").bfloat16()
+    for call in (lambda: ops.layer_norm(x, save=Neither()), lambda: ops.linear(x, w, save=Neither()),
+                 lambda: ops.gated(x, w, save=Neither()), lambda: ops.linear_backward(y, x, w, input_gradient=Neither()),
+                 lambda: ops.gated_backward(y[:, :4], x, w, pre=y, input_gradient=Neither())):
+        with pytest.raises(KeyError, match="neither"):
+            call()
