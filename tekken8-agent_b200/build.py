@@ -1,6 +1,8 @@
 """Builds the sm_100a shared library of the hot path (lib/libt8b.so) with nvcc.
 
-bindings/operators.cpp becomes the Python module t8b/_operators.so.
+bindings/operators.cpp becomes the Python module t8b/_operators.so, which links the installed torch and is
+rebuilt when that changes. The library needs none of it: without torch it is built alone, and a module that
+does not compile is reported once the library is linked.
 
 Every .cu under csrc/ becomes one object; the engine translation unit is compiled with
 --fmad=false (a fused multiply-add would round once where the reference CPU engine rounds
@@ -12,6 +14,7 @@ import os
 import subprocess
 import sys
 from concurrent.futures import ThreadPoolExecutor
+from importlib import metadata
 from pathlib import Path
 
 HERE = Path(__file__).resolve().parent
@@ -47,6 +50,28 @@ def _module_command() -> list[str]:
             "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
 
 
+def _module_job(verbose: bool):
+    """What builds the Python module (None where it is up to date, or where there is no torch to link)."""
+    stamp = BUILD / "operators.txt"
+    try:
+        against = f"torch {metadata.version('torch')} python {sys.version}"
+        newest = max(MODULE_SOURCE.stat().st_mtime, (ROOT / "include" / "t8b.h").stat().st_mtime)
+        if MODULE.exists() and MODULE.stat().st_mtime >= newest and stamp.exists() and stamp.read_text() == against:
+            return None
+        command = _module_command()
+    except ImportError as missing:
+        print(f"t8b/_operators.so is not built: {missing}", file=sys.stderr)
+        return None
+    if verbose:
+        print(" ".join(command), flush=True)
+
+    def run():
+        subprocess.run(command, check=True)
+        stamp.write_text(against)
+
+    return run
+
+
 def build(verbose: bool = False) -> Path:
     BUILD.mkdir(exist_ok=True)
     LIB.parent.mkdir(exist_ok=True)
@@ -61,19 +86,19 @@ def build(verbose: bool = False) -> Path:
         if verbose:
             print(" ".join(cmd), flush=True)
         commands.append(cmd)
-    header = ROOT / "include" / "t8b.h"
-    if not MODULE.exists() or MODULE.stat().st_mtime < max(MODULE_SOURCE.stat().st_mtime, header.stat().st_mtime):
-        commands.append(_module_command())
-        if verbose:
-            print(" ".join(commands[-1]), flush=True)
     with ThreadPoolExecutor(max_workers=os.cpu_count() or 1) as pool:
-        for done in [pool.submit(subprocess.run, cmd, check=True) for cmd in commands]:
+        compiled = [pool.submit(subprocess.run, cmd, check=True) for cmd in commands]
+        job = _module_job(verbose)
+        module = pool.submit(job) if job else None
+        for done in compiled:
             done.result()
-    if not LIB.exists() or LIB.stat().st_mtime < max(o.stat().st_mtime for o in objects):
-        cmd = [NVCC, *ARCH, "-shared", "-o", str(LIB), *map(str, objects), "-lcudart", "-lcuda", "-ldl"]
-        if verbose:
-            print(" ".join(cmd), flush=True)
-        subprocess.run(cmd, check=True)
+        if not LIB.exists() or LIB.stat().st_mtime < max(o.stat().st_mtime for o in objects):
+            cmd = [NVCC, *ARCH, "-shared", "-o", str(LIB), *map(str, objects), "-lcudart", "-lcuda", "-ldl"]
+            if verbose:
+                print(" ".join(cmd), flush=True)
+            subprocess.run(cmd, check=True)
+        if module:
+            module.result()
     return LIB
 
 
