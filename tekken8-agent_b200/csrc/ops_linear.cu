@@ -73,7 +73,7 @@ void forward(const char* what, int type, LinearCall& c, void* workspace, size_t 
         pre.overlaps(x) || pre.overlaps(w) || pre.overlaps(residual) || pre.overlaps(bias)) {
         raise(T8B_EINVAL, std::string(what) + ": an output overlaps another argument");
     }
-    if (!is_few(c.rows, c.in)) {
+    if (!is_few(c.rows, c.in, c.out, c.gated)) {
         if (!tma_rows(c.x, c.rows, c.x_stride, 2)) c.what |= T8B_WORKSPACE_X;
         if (!tma_rows(c.weight, columns, c.weight_stride, 2)) c.what |= T8B_WORKSPACE_WEIGHT;
     }

@@ -87,11 +87,19 @@ inline GemmPlan plan_gemm(int64_t m, int64_t n, int64_t k, bool may_split, doubl
     return best;
 }
 
-// Whether a forward pass goes row by row (k_few_rows) and not by tiles: measured (bf16, us a call among
-// others, by rows / by tiles), 512 -> 512: 1 row 2.2 / 5.6, 16 rows 5.0 / 5.6, 64 rows 9.2 / 5.6; gated 512 ->
-// 1,408: 16 rows 7.0 / 6.6, 24 rows 11.6 / 6.6; 2,048 -> 2,048: 1 row 4.1 / 13.1, 4 rows 7.5 / 13.1, 8
-// rows 14.7 / 13.1; 4,096 -> 512: 4 rows 12.1 / 22.5, 8 rows 25.6 / 22.5.
-inline bool is_few(int64_t rows, int64_t in) { return rows <= 4 || (rows <= 16 && in <= 512); }
+// Whether a forward pass goes row by row (k_few_rows) and not by tiles. Up to 4 rows always. Up to 16 rows
+// where the sums are short, the warps, one for each column of the output and group of 8 rows, are resident
+// at once (beyond that they take a second turn), and a gate's second sums do not make up for it. Measured
+// (bf16, us a call among others, by rows / by tiles): 512 -> 512: 1 row 2.2 / 5.6, 16 rows 4.9 / 5.7;
+// 512 -> 2,816: 4 rows 3.7 / 5.8, 8 rows 5.6 / 5.8, 9 rows 6.9 / 5.8; 512 -> 1,408: 16 rows 5.5 / 5.8; 512 -> 1,792:
+// 16 rows 8.8 / 5.9; 512 -> 8,192: 4 rows 6.4 / 7.6, 5 rows 10.0 / 7.7; gated 512 -> 1,408: 8 rows 6.3 / 6.5, 9
+// rows 6.9 / 6.7, 16 rows 7.0 / 6.6; gated 256 -> 1,408: 16 rows 4.8 / 5.4; 2,048 -> 2,048: 4 rows 7.4 / 13.1, 8 rows
+// 14.6 / 13.1; 4,096 -> 512: 4 rows 12.1 / 22.5, 8 rows 25.4 / 22.4. Rows off 16-byte boundaries cross earlier,
+// 151 -> 512: 4 rows 5.1 / 6.1, 8 rows 8.4 / 6.2; they keep the rule, with which their call needs no workspace.
+inline bool is_few(int64_t rows, int64_t in, int64_t out, bool gated) {
+    const int64_t warps = out * ceil_div(rows, 8);
+    return rows <= 4 || (rows <= 16 && in <= 512 && warps <= 2816 && (gated ? 2 : 1) * warps * in <= 2816 * 512);
+}
 
 // The gradients' products. The weight's sums over the rows and is split wherever that pays; the input's
 // where few rows leave SMs idle behind a long sum over the columns: whole backward passes in us, one part
@@ -855,7 +863,7 @@ void few_rows(const LinearCall& c) {
 template <typename E>
 void linear_forward(const LinearCall& c) {
     const int64_t columns = c.gated ? 2 * c.out : c.out;
-    if (is_few(c.rows, c.in)) {
+    if (is_few(c.rows, c.in, c.out, c.gated)) {
         c.gated ? few_rows<E, true>(c) : few_rows<E, false>(c);
         return;
     }

@@ -99,3 +99,35 @@ def test_an_option_without_a_truth_value_raises_its_own_error(cuda):
                  lambda: ops.gated_backward(y[:, :4], x, w, pre=y, input_gradient=Neither())):
         with pytest.raises(KeyError, match="neither"):
             call()
+
+
+@pytest.mark.parametrize("gated,rows,n,m,label", [
+    (False, 4, 512, 8192, "k_few_rows"), (False, 5, 512, 8192, "k_linear"), (False, 8, 512, 2816, "k_few_rows"),
+    (False, 9, 512, 2816, "k_linear"), (False, 16, 512, 1408, "k_few_rows"), (False, 16, 512, 1409, "k_linear"),
+    (False, 16, 513, 64, "k_linear"), (False, 17, 64, 64, "k_linear"), (True, 8, 512, 1408, "k_few_rows"),
+    (True, 9, 512, 1408, "k_gated"), (True, 16, 512, 704, "k_few_rows"), (True, 16, 151, 1409, "k_gated"), (True, 16, 256, 1408, "k_few_rows"),
+    (True, 16, 512, 705, "k_gated"),
+])
+def test_forward_passes_of_few_rows_take_the_form_that_measured_faster(cuda, gated, rows, n, m, label):
+    """Small integers: every sum is exact in fp32, so the outputs are equal whichever form computes them."""
+    import torch
+    from t8b import ops, profile
+    E = torch.bfloat16
+    g = torch.Generator(device="cuda").manual_seed(rows + n + m)
+    columns = 2 * m if gated else m
+    x = torch.randint(-2, 3, (rows, n), device="cuda", generator=g).to(E)
+    w = torch.randint(-1, 2, (columns, n), device="cuda", generator=g).to(E)
+    b = torch.randint(-3, 4, (columns,), device="cuda", generator=g).float()
+    profile.enable()
+    try:
+        got = ops.gated(x, w, b, activation="relu") if gated else ops.linear(x, w, b, out_dtype=torch.float32)
+        launched = profile.report()
+    finally:
+        profile.enable(False)
+    assert set(launched) - {"k_pack"} == {label}
+    z = x.double() @ w.double().T + b.double()
+    if gated:
+        z = z[:, :m].clamp(min=0) * z[:, m:]
+        assert torch.equal(got.double(), z.to(E).double())
+    else:
+        assert torch.equal(got.double(), z)
