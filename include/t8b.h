@@ -605,7 +605,8 @@ int t8b_linear_forward(int type, const void* x, int64_t x_stride, const void* we
 /* Its gradients from dy [rows][out] of `type`: with dz = dy activation'(pre), dx = dz weight,
  * dweight [out][in] = dz^T x (both of `type`) and dbias = the columns' sums of dz (of bias_type),
  * each skipped where NULL. `pre` is not read where the activation is T8B_LINEAR. dz is rounded to
- * `type` for the matrix products (not for dbias). The residual's gradient is dy itself. */
+ * `type` for the matrix products (not for dbias), in f16 with that type's range. The residual's gradient is dy
+ * itself. */
 int t8b_linear_backward(int type, const void* dy, int64_t dy_stride, const void* x, int64_t x_stride,
                         const void* weight, int64_t weight_stride, const void* pre, int64_t pre_stride, int bias_type,
                         int activation, int64_t rows, int64_t in, int64_t out, void* dx, int64_t dx_stride,

@@ -108,10 +108,12 @@ __device__ __forceinline__ Two multiply_add(const Two& a, const Two& b, const Tw
 // In fp32, from the machine's 2^x and 1/x (each good to about 2^-22): exp(v) = 2^(v log2 e),
 //   sigmoid(z) = 1 / (1 + exp(-z)),
 //   tanh(z) = 1 - 2 / (1 + exp(2z)), and below |z| = 0.2, where that difference cancels, the
-//     series z - z^3/3 + 2 z^5/15 - 17 z^7/315 (its next term is below 2^-27 of z there),
+//     series z - z^3/3 + 2 z^5/15 - 17 z^7/315 (its next term is at most 2^-24 of z there),
 //   Phi(z) = (1 + erf(z / sqrt 2)) / 2 with erfc(x) = t (a1 + t (a2 + ... t a5)) exp(-x^2),
 //     t = 1 / (1 + p x), x >= 0: Abramowitz and Stegun, Handbook of Mathematical Functions,
-//     7.1.26 (good to 1.5e-7); the lower tail is that product itself, so it does not cancel.
+//     7.1.26. Its error is 1.5e-7 absolute, so Phi is good to 7e-8 and fp32's roundings. The lower tail is
+//     that product itself, not a difference from 1, but its relative error grows all the same: 5e-5 at z =
+//     -3, 5e-4 at -4, 1.6e-3 at -5, 3.6e-3 at -6 (half a bf16 spacing is 3.9e-3; gelu(-6) is 6e-9).
 // Where z is infinite they give what the formulas do: silu(-inf) and gelu(-inf) are NaN (0 * inf).
 __device__ __forceinline__ float power_of_two(float v) {
     float r;

@@ -30,7 +30,7 @@ constexpr int kPartialRows = 16;   // rows of threads in k_norm_parameters
 // hold 32 (kLong), or by a block whose threads hold 32 (0). The more a thread holds, the fewer
 // instructions and barriers an element costs; at 16 elements two blocks of the backward pass are
 // resident, at 32 one. 65,536 x 768 in bf16, 32 lanes by 32 against a block by 16: forward 37 / 57 us,
-// backward 64 / 79; 8,192 x 8,192, a block by 32 against by 16: 51 / 73, 90 / 96.
+// backward 65 / 79; 8,192 x 8,192, a block by 32 against by 16: 49 / 73, 89 / 96.
 constexpr int kLong = 64;
 constexpr int group_of(int64_t n) { return n <= 128 ? 8 : n <= 256 ? 16 : n <= 512 ? 32 : n <= 1024 ? kLong : 0; }
 __host__ __device__ constexpr int lanes_of(int group) { return group == kLong ? 32 : group; }
@@ -90,8 +90,8 @@ __device__ __forceinline__ void row_sum(float (&v)[COUNT], float (*shared)[kWide
 //
 // Rows come through a ring of stages in shared memory that a thread fills (cp.async, the same 16 or 8
 // bytes that it will read) and reads alone, so the ring needs no barrier and a warp has its next rows
-// in flight while it works on one (262,144 x 512 in bf16: backward 205 us against 297 without it,
-// forward 88 against 123). Single elements (V = 1) are read when they are used: 4-byte copies take as
+// in flight while it works on one (262,144 x 512 in bf16, when the ring came in: backward 297 -> 205 us,
+// forward 123 -> 88; the backward pass takes 133 now). Single elements (V = 1) are read when they are used: 4-byte copies take as
 // many instructions as the elements (65,536 x 151 in fp32, backward: 55 us against 37).
 template <typename T, int V, int NV, bool SHIFT>
 struct Rows {
@@ -674,9 +674,9 @@ int norm(const Norm& given, bool backward, cudaStream_t stream) {
     }
     // 16 bytes a lane of the wider type where every matrix starts on its vector's boundary: as they
     // lie where every row does too; shifted where the rows' starts differ from it alike in all of them
-    // and rows are longer than 256; single elements otherwise. Shifted against single, bf16, us:
-    // 20,000 x 3,001 forward 86 / 127, backward 94 / 142; 100,000 x 333 forward 51 / 56, backward
-    // 74 / 70; 65,536 x 151 forward 20.0 / 16.7, backward 29.0 / 25.3.
+    // and rows are longer than 256; single elements otherwise. Shifted against single, us, bf16:
+    // 20,000 x 3,001 forward 71 / 95, backward 111 / 155; 40,000 x 801 44 / 39, 56 / 66; 100,000 x 333 48 / 53,
+    // 71 / 67; 65,536 x 151 17.6 / 15.2, 27.7 / 24.6; fp32: 100,000 x 333 47 / 59, 74 / 76.
     constexpr int V = 16 / (sizeof(TX) > sizeof(TY) ? sizeof(TX) : sizeof(TY));
     const size_t ys = backward ? sizeof(TX) : sizeof(TY);
     const bool bases = aligned(a.x, V * sizeof(TX)) && aligned(a.dy, V * sizeof(TY)) && aligned(a.residual, V * sizeof(TX)) && aligned(a.y, V * ys);
