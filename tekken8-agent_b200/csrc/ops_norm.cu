@@ -429,14 +429,14 @@ __global__ void __launch_bounds__(kThreads, resident_blocks(G, true)) k_norm_bac
             for (int i = 0; i < HELD / 2; ++i) {
                 // Beyond the row x and dy are 0 and add 0 to every sum. sum(g xhat) is rstd times sum(g
                 // (x - mean)): a product with xhat would be 0 * inf there where mean * rstd overflows.
+                const Two given = g[i];
                 v[i] = v[i] + off;
-                const Two xhat = v[i] * scaled;
-                if (live) dw[i] = multiply_add(g[i], xhat, dw[i]);
-                db[i] = db[i] + g[i];
-                g[i] = g[i] * w[i];
+                db[i] = db[i] + given;
+                g[i] = given * w[i];
                 of_g = of_g + g[i];
                 of_gx = multiply_add(g[i], v[i], of_gx);
-                v[i] = xhat;
+                v[i] = v[i] * scaled;
+                if (live) dw[i] = multiply_add(given, v[i], dw[i]);
             }
         }
         float sum[2] = {of_g.sum(), of_gx.sum() * rstd};
@@ -676,7 +676,7 @@ int norm(const Norm& given, bool backward, cudaStream_t stream) {
     // lie where every row does too; shifted where the rows' starts differ from it alike in all of them
     // and rows are longer than 256; single elements otherwise. Shifted against single, us, bf16:
     // 20,000 x 3,001 forward 71 / 95, backward 111 / 155; 40,000 x 801 44 / 39, 56 / 66; 100,000 x 333 48 / 53,
-    // 71 / 67; 65,536 x 151 17.6 / 15.2, 27.7 / 24.6; fp32: 100,000 x 333 47 / 59, 74 / 76.
+    // 71 / 67; 65,536 x 151 17.6 / 15.2, 27.7 / 24.6; fp32: 100,000 x 333 47 / 59, 70 / 76.
     constexpr int V = 16 / (sizeof(TX) > sizeof(TY) ? sizeof(TX) : sizeof(TY));
     const size_t ys = backward ? sizeof(TX) : sizeof(TY);
     const bool bases = aligned(a.x, V * sizeof(TX)) && aligned(a.dy, V * sizeof(TY)) && aligned(a.residual, V * sizeof(TX)) && aligned(a.y, V * ys);
