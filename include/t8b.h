@@ -627,6 +627,118 @@ int t8b_gated_backward(int type, const void* dh, int64_t dh_stride, const void* 
                        int64_t weight_stride, const void* pre, int64_t pre_stride, int bias_type, int activation,
                        int64_t rows, int64_t in, int64_t out, void* dx, int64_t dx_stride, void* dweight,
                        int64_t dweight_stride, void* dbias, void* workspace, size_t workspace_bytes, void* stream);
+/* ------------------------------------------------------------------ memory operators
+ * Operators of a policy with memory (no reference counterpart: the reference's policy sees one
+ * observation, or a fixed history): a short causal convolution and a selective state space scan
+ * over sequences, each with its gradients and its form for single steps, and the clipped policy
+ * loss over raw logits. The rules of the torso operators hold (device pointers aligned to their
+ * elements, caller's workspaces, one stream, fixed orders of all sums, no allocation).
+ *
+ * Data of a sequence lie in tracks: the elements of step t of sequence s are consecutive at
+ * data + s * sequence + t * step (elements; a rollout's [step][fight] order is a track like any
+ * other). Inputs may share rows (a stride of 0), outputs may not overlap anything. */
+typedef struct {
+    void* data; /* read only where it is an input */
+    int64_t sequence, step;
+} t8b_track_t;
+/* `sequences` sequences of `steps` steps. Where reset[s * reset_sequence + t * reset_step] is not
+ * 0 (NULL: nowhere), a new round begins at step t: nothing before it, the initial state included,
+ * reaches it. lengths [sequences] (NULL: all are `steps`; others are taken into 0 ... steps) ends
+ * sequences early: what lies at and past a sequence's length is not read, its outputs and
+ * gradients there are 0 and its final state is the one after its last step. */
+typedef struct {
+    int64_t sequences, steps, channels;
+    const uint8_t* reset;
+    int64_t reset_sequence, reset_step;
+    const int32_t* lengths;
+} t8b_sequences_t;
+
+/* Causal convolution, one filter a channel: y_t = activation(bias + sum over j < width of
+ * weight[width - 1 - j] x_(t-j)). x and y are of `type`; weight [channels][width] (width 2 to 4)
+ * and bias [channels] (NULL: none) of parameter_type (T8B_F32 or `type`). state [sequences][width -
+ * 1][channels] of `type` holds the inputs before the first step, oldest first (NULL: zeros);
+ * final_state, of its shape, receives the last ones unless NULL (0 where a round has had fewer). */
+int t8b_causal_conv_forward(const t8b_sequences_t* sequences, int type, t8b_track_t x, const void* weight,
+                            const void* bias, int parameter_type, int width, int activation, const void* state,
+                            t8b_track_t y, void* final_state, void* stream);
+/* Its gradients from dy and, unless NULL, the final state's: dx, dweight and dbias (of
+ * parameter_type) and dstate (of `type`), each skipped where NULL. */
+size_t t8b_causal_conv_workspace(const t8b_sequences_t* sequences, int width);
+int t8b_causal_conv_backward(const t8b_sequences_t* sequences, int type, t8b_track_t dy, t8b_track_t x,
+                             const void* weight, const void* bias, int parameter_type, int width, int activation,
+                             const void* state, const void* final_gradient, t8b_track_t dx, void* dweight, void* dbias,
+                             void* dstate, void* workspace, size_t workspace_bytes, void* stream);
+/* One step of every sequence (steps and lengths are not read; reset one flag a sequence): `state`
+ * moves on by x. */
+int t8b_causal_conv_step(const t8b_sequences_t* sequences, int type, t8b_track_t x, const void* weight, const void* bias,
+                         int parameter_type, int width, int activation, void* state, t8b_track_t y, void* stream);
+
+/* Selective scan. Per channel, with v = delta + delta_bias, D = softplus(v) (or v itself without
+ * `softplus`), and for every state n
+ *   h_t[n] = exp(D_t a[n]) h_(t-1)[n] + D_t u_t B_t[n],   y_t = (sum over n of C_t[n] h_t[n] + d u_t) silu(z_t).
+ * u, delta, z (data NULL: no gate), b, c and y are of `type`; everything else is fp32: a
+ * [channels][states], d and delta_bias [channels] (NULL: none), states h [sequences][channels]
+ * [states] (NULL: zeros). A step of b and c holds `groups` rows of `states` values, b_group and
+ * c_group elements apart; group g serves channels g channels/groups to (g + 1) channels/groups - 1.
+ * 1 to 64 states. */
+typedef struct {
+    int type, softplus;
+    int64_t groups, states;
+    t8b_track_t u, delta, z, b, c;
+    int64_t b_group, c_group;
+    const float *a, *d, *delta_bias, *state;
+} t8b_scan_t;
+/* `saved`, unless NULL, receives what the backward pass needs (t8b_selective_scan_saved floats);
+ * `backward` of the workspace query: 0 for this call, 1 for the backward call. */
+size_t t8b_selective_scan_saved(const t8b_sequences_t* sequences, int64_t groups, int64_t states);
+size_t t8b_selective_scan_workspace(const t8b_sequences_t* sequences, int64_t groups, int64_t states, int backward);
+int t8b_selective_scan_forward(const t8b_sequences_t* sequences, const t8b_scan_t* scan, t8b_track_t y,
+                               float* final_state, float* saved, void* workspace, size_t workspace_bytes, void* stream);
+/* Gradients from dy (of `type`), `saved` and, unless NULL, the final state's: du, ddelta and dz as
+ * u, db and dc as b and c; da, dd, ddelta_bias and dstate fp32. du, ddelta, db, dc and da are always
+ * written, the others skipped where their data is NULL. */
+typedef struct {
+    t8b_track_t du, ddelta, dz, db, dc;
+    int64_t db_group, dc_group;
+    float *da, *dd, *ddelta_bias, *dstate;
+} t8b_scan_gradients_t;
+int t8b_selective_scan_backward(const t8b_sequences_t* sequences, const t8b_scan_t* scan, t8b_track_t dy,
+                                const float* saved, const float* final_gradient, const t8b_scan_gradients_t* gradients,
+                                void* workspace, size_t workspace_bytes, void* stream);
+/* One step of every sequence (as above); scan->state is not read, `state` moves on. */
+int t8b_selective_scan_step(const t8b_sequences_t* sequences, const t8b_scan_t* scan, float* state, t8b_track_t y,
+                            void* stream);
+
+/* Clipped policy loss of each row's action over its legal logits: with p = softmax(logits), lp =
+ * log p[action], r = exp(lp - old), H = -sum p log p and K the divergence from a frozen reference
+ * policy q,
+ *   loss = -min(r advantage, min(max(r, 1 - clip_low), 1 + clip_high) advantage) + kl K - entropy H.
+ * The reference: T8B_REFERENCE_LOGITS its logits (K = sum p (log p - log q) over the legal ones),
+ * T8B_REFERENCE_SAMPLED its log-probability of the action (K = exp(e) - e - 1, e = log q - lp).
+ * A row whose action is not one of its legal ones (negative, past the end, masked: padding) gives 0
+ * everywhere, whatever else it holds. mask: T8B_MASK_BITS one bit an action in 32-bit words as the
+ * simulator's packed masks, T8B_MASK_BYTES one byte; mask_stride in words or bytes. */
+enum { T8B_MASK_NONE = 0, T8B_MASK_BITS = 1, T8B_MASK_BYTES = 2 };
+enum { T8B_REFERENCE_NONE = 0, T8B_REFERENCE_LOGITS = 1, T8B_REFERENCE_SAMPLED = 2 };
+typedef struct {
+    int type, mask_kind, reference_kind; /* type of logits, a reference's logits and dlogits */
+    float clip_low, clip_high, kl, entropy;
+    int64_t rows, n;
+    const void* logits;
+    int64_t logits_stride;
+    const int64_t* actions;
+    const float *old_log_probabilities, *advantages;
+    const void* mask;
+    int64_t mask_stride;
+    const void* reference;
+    int64_t reference_stride;
+    const float* weights; /* [rows] each row's loss counts so much in dlogits; NULL: 1 / rows */
+} t8b_policy_loss_t;
+/* loss, log_probabilities, entropies and divergences [rows] (any may be NULL), and unless NULL
+ * dlogits: the gradient of sum over rows of weight loss, 0 at masked logits. 1 to 2^24 logits a row. */
+int t8b_policy_loss(const t8b_policy_loss_t* call, float* loss, float* log_probabilities, float* entropies,
+                    float* divergences, void* dlogits, int64_t dlogits_stride, void* stream);
+
 /* Synchronises `stream` and reports whether a wait inside an operator's kernel ran out of its
  * limit on the current device since the last call that reported one (T8B_ECUDA; the outputs of the
  * calls queued since then are not valid). Each stall is reported once, by one caller. */

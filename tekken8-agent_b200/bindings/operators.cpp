@@ -1,4 +1,4 @@
-// The Python side of the torso operators: one call from tensors to the C entries of t8b.h. It checks
+// The Python side of the operators: one call from tensors to the C entries of t8b.h. It checks
 // the tensors, allocates the outputs and the workspace on torch's current stream, and queues the
 // work there; t8b/ops.py documents each function and names its arguments. ctypes takes about as long
 // for the twenty arguments of an entry as everything here.
@@ -11,6 +11,7 @@
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
 #include <cstring>
 #include <stdexcept>
 #include <string>
@@ -32,6 +33,16 @@ struct Entries {
     decltype(&t8b_gated_workspace) gated_workspace;
     decltype(&t8b_gated_forward) gated_forward;
     decltype(&t8b_gated_backward) gated_backward;
+    decltype(&t8b_causal_conv_forward) causal_conv_forward;
+    decltype(&t8b_causal_conv_workspace) causal_conv_workspace;
+    decltype(&t8b_causal_conv_backward) causal_conv_backward;
+    decltype(&t8b_causal_conv_step) causal_conv_step;
+    decltype(&t8b_selective_scan_saved) selective_scan_saved;
+    decltype(&t8b_selective_scan_workspace) selective_scan_workspace;
+    decltype(&t8b_selective_scan_forward) selective_scan_forward;
+    decltype(&t8b_selective_scan_backward) selective_scan_backward;
+    decltype(&t8b_selective_scan_step) selective_scan_step;
+    decltype(&t8b_policy_loss) policy_loss;
 } entry{};
 PyObject* library_error = nullptr;  // T8bError(status, message)
 PyObject* memory_error = nullptr;   // torch.OutOfMemoryError
@@ -135,7 +146,7 @@ struct On {
 };
 
 // ------------------------------------------------------------------ arguments
-constexpr Py_ssize_t kMost = 10;
+constexpr Py_ssize_t kMost = 15;
 struct Arguments {
     PyObject* const* at;
     Arguments(PyObject* const* args, Py_ssize_t given, Py_ssize_t expected) : at(args) {
@@ -147,6 +158,11 @@ struct Arguments {
         return THPVariable_Unpack(at[i]);
     }
     Tensor optional(int i, const char* name) const { return at[i] == Py_None ? Tensor() : tensor(i, name); }
+    double number(int i) const {
+        const double v = PyFloat_AsDouble(at[i]);
+        if (v == -1.0 && PyErr_Occurred()) throw Raised();
+        return v;
+    }
     bool flag(int i) const {
         const int truth = PyObject_IsTrue(at[i]);
         if (truth < 0) throw Raised();
@@ -416,6 +432,357 @@ PyObject* backward(PyObject*, PyObject* const* args, Py_ssize_t given) {
     });
 }
 
+// ------------------------------------------------------------------ sequences
+// What the sequence operators share: [sequences][steps][...] tensors of any strides with a contiguous last axis
+// (single steps: [sequences][...]), resets and lengths.
+struct Tracks {
+    const On on;
+    const bool step;
+    int type;
+    t8b_sequences_t q{};
+    bool by_step = false;  // whether x lies [step][sequence]: outputs do too
+    Tracks(const Tensor& x, const char* name, bool step_) : on(x), step(step_), type(type_of(x, name)) {
+        if (x.dim() != (step ? 2 : 3)) {
+            refuse(std::string(name) + " has shape " + text(x.sizes()) + ", expected " + (step ? "[sequences][channels]" : "[sequences][steps][channels]"));
+        }
+        q.sequences = x.size(0);
+        q.steps = step ? 1 : x.size(1);
+        q.channels = x.size(-1);
+        by_step = !step && q.sequences > 1 && q.steps > 1 && x.stride(0) < x.stride(1);
+    }
+    void place(const Tensor& t, const char* name) const {
+        if (t.layout() != at::kStrided) refuse(std::string(name) + " must be a dense tensor");
+        if (!t.is_cuda() || t.get_device() != on.device) refuse(std::string(name) + " is on another device");
+    }
+    void expect(const Tensor& t, const char* name, at::IntArrayRef shape, at::ScalarType scalar_type) const {
+        place(t, name);
+        if (t.sizes() != shape) refuse(std::string(name) + " has shape " + text(t.sizes()) + ", expected " + text(shape));
+        if (t.scalar_type() != scalar_type) refuse(std::string(name) + " is " + c10::toString(t.scalar_type()) + ", expected " + c10::toString(scalar_type));
+    }
+    void* packed(const Tensor& t, const char* name, at::IntArrayRef shape, int element) const {
+        if (!t.defined()) return nullptr;
+        expect(t, name, shape, scalar(element));
+        if (!t.is_contiguous()) refuse(std::string(name) + " must be contiguous");
+        return t.data_ptr();
+    }
+    // a tensor of x's type and first axes
+    t8b_track_t track(const Tensor& t, const char* name, int64_t width) const {
+        if (!t.defined()) return {};
+        if (step) {
+            expect(t, name, {q.sequences, width}, scalar(type));
+        } else {
+            expect(t, name, {q.sequences, q.steps, width}, scalar(type));
+        }
+        if (width > 1 && t.stride(-1) != 1) refuse(std::string(name) + ": the last axis must be contiguous");
+        return {t.data_ptr(), t.stride(0), step ? 0 : t.stride(1)};
+    }
+    void rounds(const Tensor& reset, const Tensor& lengths) {
+        if (reset.defined()) {
+            place(reset, "reset");
+            const bool fits = step ? reset.dim() == 1 && reset.size(0) == q.sequences
+                                   : reset.dim() == 2 && reset.size(0) == q.sequences && reset.size(1) == q.steps;
+            if (!fits) refuse("reset has shape " + text(reset.sizes()) + ", expected " + (step ? "[sequences]" : "[sequences][steps]"));
+            if (reset.scalar_type() != at::kBool && reset.scalar_type() != at::kByte) refuse("reset must be bool or uint8");
+            q.reset = static_cast<const uint8_t*>(reset.data_ptr());
+            q.reset_sequence = reset.stride(0);
+            q.reset_step = step ? 0 : reset.stride(1);
+        }
+        if (lengths.defined()) {
+            expect(lengths, "lengths", {q.sequences}, at::kInt);
+            if (!lengths.is_contiguous()) refuse("lengths must be contiguous");
+            q.lengths = lengths.data_ptr<int32_t>();
+        }
+    }
+    // an output [sequences][steps][width...], in the order of x
+    Tensor output(const Tensor& like, int64_t groups, int64_t width, bool grouped) const {
+        const auto options = like.options().dtype(scalar(type));
+        const int64_t row = groups * width;
+        if (step) return at::empty({q.sequences, row}, options);
+        const int64_t s = by_step ? row : q.steps * row, t = by_step ? q.sequences * row : row;
+        if (grouped) return at::empty_strided({q.sequences, q.steps, groups, width}, {s, t, width, 1}, options);
+        return at::empty_strided({q.sequences, q.steps, row}, {s, t, 1}, options);
+    }
+    t8b_track_t fresh(const Tensor& t) const { return t.defined() ? t8b_track_t{t.data_ptr(), t.stride(0), step ? 0 : t.stride(1)} : t8b_track_t{}; }
+};
+
+// ------------------------------------------------------------------ causal convolution
+struct Filter {
+    int width = 0, type = T8B_F32;
+    void *weight = nullptr, *bias = nullptr;
+    Filter(const Tracks& k, const Tensor& tw, const Tensor& tb) {
+        type = type_of(tw, "weight");
+        if (type != T8B_F32 && type != k.type) refuse("weight must be fp32 or of x's type");
+        if (tw.dim() != 2) refuse("weight has shape " + text(tw.sizes()) + ", expected [channels][width]");
+        width = static_cast<int>(std::min<int64_t>(tw.size(1), 1 << 20));
+        weight = k.packed(tw, "weight", {k.q.channels, tw.size(1)}, type);
+        bias = k.packed(tb, "bias", {k.q.channels}, type);
+    }
+};
+
+// x, weight, bias, activation, state, reset, lengths, final
+PyObject* causal_conv(PyObject*, PyObject* const* args, Py_ssize_t given) {
+    return answer([&]() -> PyObject* {
+        const Arguments a(args, given, 8);
+        const Tensor x = a.tensor(0, "x"), weight = a.tensor(1, "weight"), bias = a.optional(2, "bias"), state = a.optional(4, "state");
+        const Tensor reset = a.optional(5, "reset"), lengths = a.optional(6, "lengths");
+        const int act = a.activation(3);
+        Tracks k(x, "x", false);
+        const t8b_track_t in = k.track(x, "x", k.q.channels);
+        k.rounds(reset, lengths);
+        const Filter f(k, weight, bias);
+        const void* ps = k.packed(state, "state", {k.q.sequences, f.width - 1, k.q.channels}, k.type);
+        const bool last = a.flag(7);
+        if (f.width < 2 || f.width > 4) refuse("weight has shape " + text(weight.sizes()) + ": a width of 2 to 4");
+        const Tensor y = k.output(x, 1, k.q.channels, false);
+        Tensor end;
+        if (last) end = make(x, {k.q.sequences, f.width - 1, k.q.channels}, k.type);
+        done(entry.causal_conv_forward(&k.q, k.type, in, f.weight, f.bias, f.type, f.width, act, ps, k.fresh(y), pointer(end), k.on.stream()));
+        return last ? wrap_all(y, end) : wrap(y);
+    });
+}
+
+// dy, x, weight, bias, activation, state, reset, lengths, dfinal
+PyObject* causal_conv_backward(PyObject*, PyObject* const* args, Py_ssize_t given) {
+    return answer([&]() -> PyObject* {
+        const Arguments a(args, given, 9);
+        const Tensor dy = a.tensor(0, "dy"), x = a.tensor(1, "x"), weight = a.tensor(2, "weight"), bias = a.optional(3, "bias");
+        const Tensor state = a.optional(5, "state"), reset = a.optional(6, "reset"), lengths = a.optional(7, "lengths"), dfinal = a.optional(8, "dfinal");
+        const int act = a.activation(4);
+        Tracks k(x, "x", false);
+        const t8b_track_t in = k.track(x, "x", k.q.channels), d = k.track(dy, "dy", k.q.channels);
+        k.rounds(reset, lengths);
+        const Filter f(k, weight, bias);
+        if (f.width < 2 || f.width > 4) refuse("weight has shape " + text(weight.sizes()) + ": a width of 2 to 4");
+        const void* ps = k.packed(state, "state", {k.q.sequences, f.width - 1, k.q.channels}, k.type);
+        const void* pf = k.packed(dfinal, "dfinal", {k.q.sequences, f.width - 1, k.q.channels}, k.type);
+        const Tensor dx = k.output(x, 1, k.q.channels, false), dweight = make(x, weight.sizes(), f.type);
+        Tensor dbias, dstate;
+        if (bias.defined()) dbias = make(x, {k.q.channels}, f.type);
+        if (state.defined()) dstate = make(x, state.sizes(), k.type);
+        const size_t size = entry.causal_conv_workspace(&k.q, f.width);
+        const Tensor workspace = make_bytes(x, size);
+        done(entry.causal_conv_backward(&k.q, k.type, d, in, f.weight, f.bias, f.type, f.width, act, ps, pf, k.fresh(dx), dweight.data_ptr(),
+                                        pointer(dbias), pointer(dstate), workspace.data_ptr(), size, k.on.stream()));
+        return wrap_all(dx, dweight, dbias, dstate);
+    });
+}
+
+// x, weight, bias, state, activation, reset
+PyObject* causal_conv_step(PyObject*, PyObject* const* args, Py_ssize_t given) {
+    return answer([&]() -> PyObject* {
+        const Arguments a(args, given, 6);
+        const Tensor x = a.tensor(0, "x"), weight = a.tensor(1, "weight"), bias = a.optional(2, "bias"), state = a.tensor(3, "state");
+        const Tensor reset = a.optional(5, "reset");
+        const int act = a.activation(4);
+        Tracks k(x, "x", true);
+        const t8b_track_t in = k.track(x, "x", k.q.channels);
+        k.rounds(reset, Tensor());
+        const Filter f(k, weight, bias);
+        if (f.width < 2 || f.width > 4) refuse("weight has shape " + text(weight.sizes()) + ": a width of 2 to 4");
+        void* ps = k.packed(state, "state", {k.q.sequences, f.width - 1, k.q.channels}, k.type);
+        const Tensor y = k.output(x, 1, k.q.channels, false);
+        done(entry.causal_conv_step(&k.q, k.type, in, f.weight, f.bias, f.type, f.width, act, ps, k.fresh(y), k.on.stream()));
+        return wrap(y);
+    });
+}
+
+// ------------------------------------------------------------------ selective scan
+struct Scanned {
+    t8b_scan_t scan{};
+    bool grouped = false;  // b and c have an axis of groups
+    Scanned(const Tracks& k, const Tensor& u, const Tensor& delta, const Tensor& a, const Tensor& b, const Tensor& c, const Tensor& d,
+            const Tensor& z, const Tensor& delta_bias, bool softplus) {
+        scan.type = k.type;
+        scan.softplus = softplus;
+        scan.u = k.track(u, "u", k.q.channels);
+        scan.delta = k.track(delta, "delta", k.q.channels);
+        scan.z = k.track(z, "z", k.q.channels);
+        if (a.dim() != 2) refuse("a has shape " + text(a.sizes()) + ", expected [channels][states]");
+        scan.states = a.size(1);
+        if (scan.states < 1 || scan.states > 64) refuse("a has shape " + text(a.sizes()) + ": 1 to 64 states");
+        scan.a = static_cast<const float*>(k.packed(a, "a", {k.q.channels, scan.states}, T8B_F32));
+        scan.d = static_cast<const float*>(k.packed(d, "d", {k.q.channels}, T8B_F32));
+        scan.delta_bias = static_cast<const float*>(k.packed(delta_bias, "delta_bias", {k.q.channels}, T8B_F32));
+        const int plain = k.step ? 2 : 3;
+        grouped = b.dim() == plain + 1;
+        scan.groups = grouped ? b.size(plain - 1) : 1;
+        if (scan.groups < 1 || k.q.channels % scan.groups != 0) refuse("b has shape " + text(b.sizes()) + ": its groups must divide the channels");
+        scan.b = shared(k, b, "b", scan.b_group);
+        scan.c = shared(k, c, "c", scan.c_group);
+    }
+    t8b_track_t shared(const Tracks& k, const Tensor& t, const char* name, int64_t& group) const {
+        group = scan.states;
+        if (!grouped) return k.track(t, name, scan.states);
+        if (k.step) {
+            k.expect(t, name, {k.q.sequences, scan.groups, scan.states}, scalar(k.type));
+        } else {
+            k.expect(t, name, {k.q.sequences, k.q.steps, scan.groups, scan.states}, scalar(k.type));
+        }
+        if (scan.states > 1 && t.stride(-1) != 1) refuse(std::string(name) + ": the last axis must be contiguous");
+        if (scan.groups > 1) group = t.stride(-2);
+        return {t.data_ptr(), t.stride(0), k.step ? 0 : t.stride(1)};
+    }
+};
+
+// u, delta, a, b, c, d, z, delta_bias, softplus, state, reset, lengths, final, save
+PyObject* selective_scan(PyObject*, PyObject* const* args, Py_ssize_t given) {
+    return answer([&]() -> PyObject* {
+        const Arguments a(args, given, 14);
+        const Tensor u = a.tensor(0, "u"), delta = a.tensor(1, "delta"), ta = a.tensor(2, "a"), b = a.tensor(3, "b"), c = a.tensor(4, "c");
+        const Tensor d = a.optional(5, "d"), z = a.optional(6, "z"), delta_bias = a.optional(7, "delta_bias"), state = a.optional(9, "state");
+        const Tensor reset = a.optional(10, "reset"), lengths = a.optional(11, "lengths");
+        Tracks k(u, "u", false);
+        k.rounds(reset, lengths);
+        Scanned s(k, u, delta, ta, b, c, d, z, delta_bias, a.flag(8));
+        s.scan.state = static_cast<const float*>(k.packed(state, "state", {k.q.sequences, k.q.channels, s.scan.states}, T8B_F32));
+        const bool last = a.flag(12), save = a.flag(13);
+        const Tensor y = k.output(u, 1, k.q.channels, false);
+        Tensor end, saved, workspace;
+        if (last) end = make(u, {k.q.sequences, k.q.channels, s.scan.states}, T8B_F32);
+        if (save) saved = make(u, {static_cast<int64_t>(entry.selective_scan_saved(&k.q, s.scan.groups, s.scan.states))}, T8B_F32);
+        const size_t size = entry.selective_scan_workspace(&k.q, s.scan.groups, s.scan.states, 0);
+        if (size) workspace = make_bytes(u, size);
+        done(entry.selective_scan_forward(&k.q, &s.scan, k.fresh(y), static_cast<float*>(pointer(end)), static_cast<float*>(pointer(saved)),
+                                          pointer(workspace), size, k.on.stream()));
+        return last ? (save ? wrap_all(y, end, saved) : wrap_all(y, end)) : save ? wrap_all(y, saved) : wrap(y);
+    });
+}
+
+// dy, u, delta, a, b, c, saved, d, z, delta_bias, softplus, state, reset, lengths, dfinal
+PyObject* selective_scan_backward(PyObject*, PyObject* const* args, Py_ssize_t given) {
+    return answer([&]() -> PyObject* {
+        const Arguments a(args, given, 15);
+        const Tensor dy = a.tensor(0, "dy"), u = a.tensor(1, "u"), delta = a.tensor(2, "delta"), ta = a.tensor(3, "a"), b = a.tensor(4, "b");
+        const Tensor c = a.tensor(5, "c"), saved = a.tensor(6, "saved"), d = a.optional(7, "d"), z = a.optional(8, "z");
+        const Tensor delta_bias = a.optional(9, "delta_bias"), state = a.optional(11, "state"), reset = a.optional(12, "reset");
+        const Tensor lengths = a.optional(13, "lengths"), dfinal = a.optional(14, "dfinal");
+        Tracks k(u, "u", false);
+        k.rounds(reset, lengths);
+        Scanned s(k, u, delta, ta, b, c, d, z, delta_bias, a.flag(10));
+        const int64_t states = s.scan.states;
+        s.scan.state = static_cast<const float*>(k.packed(state, "state", {k.q.sequences, k.q.channels, states}, T8B_F32));
+        const void* pf = k.packed(dfinal, "dfinal", {k.q.sequences, k.q.channels, states}, T8B_F32);
+        const void* ps = k.packed(saved, "saved", {static_cast<int64_t>(entry.selective_scan_saved(&k.q, s.scan.groups, states))}, T8B_F32);
+        const t8b_track_t given_dy = k.track(dy, "dy", k.q.channels);
+        const Tensor du = k.output(u, 1, k.q.channels, false), ddelta = k.output(u, 1, k.q.channels, false);
+        const Tensor db = k.output(u, s.scan.groups, states, s.grouped), dc = k.output(u, s.scan.groups, states, s.grouped);
+        const Tensor da = make(u, {k.q.channels, states}, T8B_F32);
+        Tensor dz, dd, dbias, dstate;
+        if (z.defined()) dz = k.output(u, 1, k.q.channels, false);
+        if (d.defined()) dd = make(u, {k.q.channels}, T8B_F32);
+        if (delta_bias.defined()) dbias = make(u, {k.q.channels}, T8B_F32);
+        if (state.defined()) dstate = make(u, state.sizes(), T8B_F32);
+        t8b_scan_gradients_t g{};
+        g.du = k.fresh(du);
+        g.ddelta = k.fresh(ddelta);
+        g.dz = k.fresh(dz);
+        g.db = k.fresh(db);
+        g.dc = k.fresh(dc);
+        g.db_group = g.dc_group = states;
+        g.da = da.data_ptr<float>();
+        g.dd = static_cast<float*>(pointer(dd));
+        g.ddelta_bias = static_cast<float*>(pointer(dbias));
+        g.dstate = static_cast<float*>(pointer(dstate));
+        const size_t size = entry.selective_scan_workspace(&k.q, s.scan.groups, states, 1);
+        const Tensor workspace = make_bytes(u, size);
+        done(entry.selective_scan_backward(&k.q, &s.scan, given_dy, static_cast<const float*>(ps), static_cast<const float*>(pf), &g,
+                                           workspace.data_ptr(), size, k.on.stream()));
+        return wrap_all(du, ddelta, da, db, dc, dd, dz, dbias, dstate);
+    });
+}
+
+// u, delta, a, b, c, state, d, z, delta_bias, softplus, reset
+PyObject* selective_scan_step(PyObject*, PyObject* const* args, Py_ssize_t given) {
+    return answer([&]() -> PyObject* {
+        const Arguments a(args, given, 11);
+        const Tensor u = a.tensor(0, "u"), delta = a.tensor(1, "delta"), ta = a.tensor(2, "a"), b = a.tensor(3, "b"), c = a.tensor(4, "c");
+        const Tensor state = a.tensor(5, "state"), d = a.optional(6, "d"), z = a.optional(7, "z"), delta_bias = a.optional(8, "delta_bias");
+        const Tensor reset = a.optional(10, "reset");
+        Tracks k(u, "u", true);
+        k.rounds(reset, Tensor());
+        const Scanned s(k, u, delta, ta, b, c, d, z, delta_bias, a.flag(9));
+        void* ps = k.packed(state, "state", {k.q.sequences, k.q.channels, s.scan.states}, T8B_F32);
+        const Tensor y = k.output(u, 1, k.q.channels, false);
+        done(entry.selective_scan_step(&k.q, &s.scan, static_cast<float*>(ps), k.fresh(y), k.on.stream()));
+        return wrap(y);
+    });
+}
+
+// ------------------------------------------------------------------ policy loss
+// logits, actions, old_log_probabilities, advantages, mask, reference, weights, clip, clip_high, kl, entropy, gradient
+PyObject* policy_loss(PyObject*, PyObject* const* args, Py_ssize_t given) {
+    return answer([&]() -> PyObject* {
+        const Arguments a(args, given, 12);
+        const Tensor logits = a.tensor(0, "logits"), actions = a.tensor(1, "actions"), old = a.tensor(2, "old_log_probabilities");
+        const Tensor advantages = a.tensor(3, "advantages"), mask = a.optional(4, "mask"), reference = a.optional(5, "reference");
+        const Tensor weights = a.optional(6, "weights");
+        const On on(logits);
+        if (logits.dim() < 1) refuse("logits has shape (), expected [rows][logits]");
+        t8b_policy_loss_t c{};
+        c.type = type_of(logits, "logits");
+        c.n = logits.size(-1);
+        const Rows z = rows_of(logits, "logits", c.n, on.device);
+        const auto lead = logits.sizes().slice(0, logits.dim() - 1);
+        auto per_row = [&](const Tensor& t, const char* name, at::ScalarType type) -> const void* {
+            if (!t.defined()) return nullptr;
+            if (!t.is_cuda() || t.get_device() != on.device) refuse(std::string(name) + " is on another device");
+            if (t.scalar_type() != type) refuse(std::string(name) + " is " + c10::toString(t.scalar_type()) + ", expected " + c10::toString(type));
+            if (t.sizes() != lead) refuse(std::string(name) + " has shape " + text(t.sizes()) + ", expected one value a row, " + text(lead));
+            if (!t.is_contiguous()) refuse(std::string(name) + " must be contiguous");
+            return t.data_ptr();
+        };
+        c.rows = z.rows;
+        c.logits = z.data;
+        c.logits_stride = z.stride;
+        c.actions = static_cast<const int64_t*>(per_row(actions, "actions", at::kLong));
+        c.old_log_probabilities = static_cast<const float*>(per_row(old, "old_log_probabilities", at::kFloat));
+        c.advantages = static_cast<const float*>(per_row(advantages, "advantages", at::kFloat));
+        c.weights = static_cast<const float*>(per_row(weights, "weights", at::kFloat));
+        if (mask.defined()) {
+            const bool bits = mask.scalar_type() == at::kInt;
+            if (!bits && mask.scalar_type() != at::kBool && mask.scalar_type() != at::kByte) {
+                refuse("mask must be bool or uint8 (one value a logit) or int32 (one bit)");
+            }
+            if (mask.dim() < 1 || mask.sizes().slice(0, mask.dim() - 1) != lead) refuse("mask has shape " + text(mask.sizes()) + ", logits " + text(logits.sizes()));
+            const Rows m = rows_of(mask, "mask", bits ? (c.n + 31) / 32 : c.n, on.device);
+            c.mask_kind = bits ? T8B_MASK_BITS : T8B_MASK_BYTES;
+            c.mask = m.data;
+            c.mask_stride = m.stride;
+        }
+        if (reference.defined()) {
+            if (reference.dim() == logits.dim()) {
+                if (reference.sizes() != logits.sizes()) refuse("reference has shape " + text(reference.sizes()) + ", logits " + text(logits.sizes()));
+                if (reference.scalar_type() != logits.scalar_type()) refuse("a reference's logits must have the logits' type");
+                const Rows r = rows_of(reference, "reference", c.n, on.device);
+                c.reference_kind = T8B_REFERENCE_LOGITS;
+                c.reference = r.data;
+                c.reference_stride = r.stride;
+            } else {
+                c.reference = per_row(reference, "reference", at::kFloat);
+                c.reference_kind = T8B_REFERENCE_SAMPLED;
+            }
+        }
+        c.clip_low = static_cast<float>(a.number(7));
+        c.clip_high = args[8] == Py_None ? c.clip_low : static_cast<float>(a.number(8));
+        c.kl = static_cast<float>(a.number(9));
+        c.entropy = static_cast<float>(a.number(10));
+        const bool gradient = a.flag(11);
+        const Tensor loss = make(logits, lead, T8B_F32), lp = make(logits, lead, T8B_F32), entropies = make(logits, lead, T8B_F32);
+        const Tensor divergences = make(logits, lead, T8B_F32);
+        Tensor dlogits;
+        int64_t stride = c.n;
+        if (gradient) {  // rows start on 16 bytes, as the matrix products that read them like
+            const int64_t pack = c.type == T8B_F32 ? 4 : 8;
+            stride = (c.n + pack - 1) / pack * pack;
+            dlogits = make(logits, Shape(logits, stride), c.type);
+            if (stride != c.n) dlogits = dlogits.narrow(-1, 0, c.n);
+        }
+        done(entry.policy_loss(&c, loss.data_ptr<float>(), lp.data_ptr<float>(), entropies.data_ptr<float>(), divergences.data_ptr<float>(),
+                               pointer(dlogits), stride, on.stream()));
+        return gradient ? wrap_all(loss, lp, entropies, divergences, dlogits) : wrap_all(loss, lp, entropies, divergences);
+    });
+}
+
 // bind(T8bError, torch.OutOfMemoryError, addresses of the entries in the order of Entries)
 PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t given) {
     constexpr Py_ssize_t kEntries = sizeof(Entries) / sizeof(void*);
@@ -450,6 +817,13 @@ PyMethodDef methods[] = {
     T8B_METHOD("linear_backward", backward<1>),
     T8B_METHOD("gated", gated),
     T8B_METHOD("gated_backward", backward<2>),
+    T8B_METHOD("causal_conv", causal_conv),
+    T8B_METHOD("causal_conv_backward", causal_conv_backward),
+    T8B_METHOD("causal_conv_step", causal_conv_step),
+    T8B_METHOD("selective_scan", selective_scan),
+    T8B_METHOD("selective_scan_backward", selective_scan_backward),
+    T8B_METHOD("selective_scan_step", selective_scan_step),
+    T8B_METHOD("policy_loss", policy_loss),
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_operators", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -1,0 +1,471 @@
+// Clipped policy loss over each row's legal logits, with entropy and the divergence from a reference
+// policy, and its gradient in the same pass.
+//
+//   lp = z[a] - lse(z),  r = exp(lp - old),  loss = -min(r A, clip(r) A) + kl K - entropy H
+//   dloss/dz_i = p_i (c + kl (z_i - q_i) + entropy (z_i - m)) + [i = a] slope,
+//   slope = dloss/dlp = -r A where the unclipped term is the smaller (0 where not) + the sampled K's 1 - exp(e)
+//
+// where c gathers what is the same for a whole row. Bound by memory: logits (and a reference's) once in,
+// the gradient once out. A row of up to 1,024 logits lies in the registers of one warp. A longer one belongs to a
+// block that reads it twice, for its sums and for its gradient; the second read comes from L2, where
+// the rows that are worked on at once fit many times over. Sums of exponentials are joined in 64 bits and the logarithm
+// is taken there: the ratio and the divergence are differences of it.
+#include "ops_memory.cuh"
+
+namespace t8b {
+namespace op {
+namespace {
+
+constexpr int kWarps = 4;          // warps of a block that gives a row to each
+constexpr int kMostHeld = 32;      // logits of a lane there
+constexpr int kMostThreads = 512;  // threads of a block that shares a row
+
+struct Loss {
+    const void* logits;
+    const void* reference;
+    const void* mask;
+    const int64_t* actions;
+    const float *old, *advantages, *weights;
+    float *loss, *log_probabilities, *entropies, *divergences;
+    void* gradient;
+    int64_t logits_stride, reference_stride, mask_stride, gradient_stride, rows;
+    int n, mask_kind, reference_kind;
+    float low, high, kl, entropy, even;  // the clipped ratio's range; even: the weight without weights
+};
+
+// Which of `count` consecutive actions from e on are legal, a bit each; they lie in one word.
+template <int COUNT>
+__device__ __forceinline__ uint32_t legal_bits(const Loss& a, int64_t row, int e) {
+    uint32_t bits = COUNT == 32 ? 0xffffffffu : (1u << COUNT) - 1;
+    if (a.mask_kind == T8B_MASK_BITS) {
+        bits &= static_cast<const uint32_t*>(a.mask)[row * a.mask_stride + e / 32] >> (e % 32);
+    } else if (a.mask_kind == T8B_MASK_BYTES) {
+        const uint8_t* m = static_cast<const uint8_t*>(a.mask) + row * a.mask_stride + e;
+        bits = 0;
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) bits |= e + i < a.n && m[i] != 0 ? 1u << i : 0u;
+    }
+    return e + COUNT <= a.n ? bits : bits & ((1u << max(a.n - e, 0)) - 1);
+}
+__device__ __forceinline__ bool legal(const Loss& a, int64_t row, int64_t action) {
+    return action >= 0 && action < a.n && (legal_bits<1>(a, row, static_cast<int>(action)) & 1) != 0;
+}
+
+// A row's sums: m the largest legal logit, total = sum e, spread = sum e (z - m), apart = sum e (z - q)
+// with e = exp(z - m); the same of the reference as far as it is needed.
+struct Sums {
+    float m = -INFINITY, q_m = -INFINITY;
+    float spread = 0.0f, apart = 0.0f;
+    double total = 0.0, q_total = 0.0;
+};
+// What a row's gradient needs beside its logits.
+struct Slopes {
+    float scale, slope, base;  // weight / total; weight slope; c
+};
+
+// The row's outputs from its sums; every thread that calls it gets the slopes, `writes` stores.
+__device__ __forceinline__ Slopes finish(const Loss& a, int64_t row, int64_t action, float chosen, const Sums& s, bool writes) {
+    const double log_total = log(s.total);
+    const double lp = static_cast<double>(chosen) - static_cast<double>(s.m) - log_total;
+    const float share = static_cast<float>(1.0 / s.total);
+    const float entropy = static_cast<float>(log_total - static_cast<double>(s.spread * share));
+    const float advantage = a.advantages[row];
+    const float ratio = expf(static_cast<float>(lp - static_cast<double>(a.old[row])));
+    const float free = ratio * advantage, held = fminf(fmaxf(ratio, a.low), a.high) * advantage;
+    float loss = -(free <= held || free != free ? free : held), slope = free <= held || free != free ? -free : 0.0f;
+    float divergence = 0.0f, shift = 0.0f;
+    if (a.reference_kind == T8B_REFERENCE_LOGITS) {
+        // log p_i - log q_i = (z_i - q_i) - shift
+        const double gap = (static_cast<double>(s.m) + log_total) - (static_cast<double>(s.q_m) + log(s.q_total));
+        shift = static_cast<float>(gap);
+        divergence = static_cast<float>(static_cast<double>(s.apart) * (1.0 / s.total) - gap);
+    } else if (a.reference_kind == T8B_REFERENCE_SAMPLED) {
+        const double gap = static_cast<double>(static_cast<const float*>(a.reference)[row]) - lp;
+        const float e = static_cast<float>(gap);
+        // exp(e) - 1 - e, by its series where the difference would cancel
+        const float grown = expm1f(e);
+        divergence = fabsf(e) < 0.1f
+            ? e * e * fmaf(e, fmaf(e, fmaf(e, fmaf(e, 1.0f / 720.0f, 1.0f / 120.0f), 1.0f / 24.0f), 1.0f / 6.0f), 0.5f)
+            : grown - e;
+        slope -= a.kl * grown;
+    }
+    loss += a.kl * divergence - a.entropy * entropy;
+    if (writes) {
+        if (a.loss) a.loss[row] = loss;
+        if (a.log_probabilities) a.log_probabilities[row] = static_cast<float>(lp);
+        if (a.entropies) a.entropies[row] = entropy;
+        if (a.divergences) a.divergences[row] = divergence;
+    }
+    const float weight = a.weights ? a.weights[row] : a.even;
+    Slopes out;
+    out.scale = weight * share;
+    out.slope = weight * slope;
+    out.base = -slope + a.entropy * (entropy - static_cast<float>(log_total));
+    if (a.reference_kind == T8B_REFERENCE_LOGITS) out.base -= a.kl * (shift + divergence);
+    return out;
+}
+__device__ __forceinline__ void finish_nothing(const Loss& a, int64_t row) {
+    for (float* p : {a.loss, a.log_probabilities, a.entropies, a.divergences}) {
+        if (p) p[row] = 0.0f;
+    }
+}
+
+// One warp a row; lane l holds the packs l, l + 32, ... of V logits, up to HELD logits.
+template <typename T, int V, int HELD, bool REFERENCE>
+__global__ void __launch_bounds__(32 * kWarps) k_policy_loss(Loss a) {
+    constexpr int PACKS = HELD / V;
+    wait_previous();
+    release_next();
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (row >= a.rows) return;
+    const T* z = static_cast<const T*>(a.logits) + row * a.logits_stride;
+    const T* q = REFERENCE ? static_cast<const T*>(a.reference) + row * a.reference_stride : nullptr;
+    T* g = a.gradient ? static_cast<T*>(a.gradient) + row * a.gradient_stride : nullptr;
+    float v[HELD], w[REFERENCE ? HELD : 1];
+    uint32_t bits[PACKS];
+    Pack<T, V> raw[PACKS], raw_q[REFERENCE ? PACKS : 1];
+#pragma unroll
+    for (int i = 0; i < PACKS; ++i) {
+        const int e = (i * 32 + lane) * V;
+        bits[i] = 0;
+        if (e < a.n) {  // n is a multiple of V
+            raw[i] = load_pack<T, V>(z + e);
+            if (REFERENCE) raw_q[REFERENCE ? i : 0] = load_pack<T, V>(q + e);
+            bits[i] = legal_bits<V>(a, row, e);
+        }
+    }
+    const int64_t action = a.actions[row];
+    if (!legal(a, row, action)) {
+        if (lane == 0) finish_nothing(a, row);
+        if (g == nullptr) return;
+        float zero[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) zero[i] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < PACKS; ++i) {
+            const int e = (i * 32 + lane) * V;
+            if (e < a.n) *reinterpret_cast<Pack<T, V>*>(g + e) = pack<T, V>(zero);
+        }
+        return;
+    }
+    const float chosen = Element<T>::load(z[action]);
+    Sums s;
+#pragma unroll
+    for (int i = 0; i < PACKS; ++i) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const bool in = bits[i] >> j & 1;
+            v[i * V + j] = in ? Element<T>::load(raw[i].v[j]) : -INFINITY;
+            s.m = fmaxf(s.m, v[i * V + j]);
+            if (REFERENCE) {
+                w[REFERENCE ? i * V + j : 0] = in ? Element<T>::load(raw_q[REFERENCE ? i : 0].v[j]) : -INFINITY;
+                s.q_m = fmaxf(s.q_m, w[REFERENCE ? i * V + j : 0]);
+            }
+        }
+    }
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) {
+        s.m = fmaxf(s.m, __shfl_xor_sync(0xffffffffu, s.m, o));
+        if (REFERENCE) s.q_m = fmaxf(s.q_m, __shfl_xor_sync(0xffffffffu, s.q_m, o));
+    }
+    // e into v, and what multiplies p beside the row's constant into w
+    float total = 0.0f, q_total = 0.0f, extra[HELD];
+#pragma unroll
+    for (int i = 0; i < HELD; ++i) {
+        const bool in = bits[i / V] >> (i % V) & 1;
+        const float off = v[i] - s.m, e = in ? exponential(off) : 0.0f;
+        const bool counts = e != 0.0f;  // a logit of -inf adds nothing
+        total += e;
+        s.spread += counts ? e * off : 0.0f;
+        extra[i] = a.entropy * off;
+        if (REFERENCE) {
+            const float away = v[i] - w[REFERENCE ? i : 0];
+            s.apart += counts ? e * away : 0.0f;
+            extra[i] = fmaf(a.kl, away, extra[i]);
+            q_total += in ? exponential(w[REFERENCE ? i : 0] - s.q_m) : 0.0f;
+        }
+        v[i] = e;
+    }
+    s.total = total;
+    s.q_total = q_total;
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) {
+        s.total += __shfl_xor_sync(0xffffffffu, s.total, o);
+        s.spread += __shfl_xor_sync(0xffffffffu, s.spread, o);
+        if (REFERENCE) {
+            s.q_total += __shfl_xor_sync(0xffffffffu, s.q_total, o);
+            s.apart += __shfl_xor_sync(0xffffffffu, s.apart, o);
+        }
+    }
+    const Slopes k = finish(a, row, action, chosen, s, lane == 0);
+    if (g == nullptr) return;
+#pragma unroll
+    for (int i = 0; i < PACKS; ++i) {
+        const int e = (i * 32 + lane) * V;
+        if (e >= a.n) continue;
+        float out[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const float p = v[i * V + j] * k.scale;
+            out[j] = (v[i * V + j] != 0.0f ? p * (k.base + extra[i * V + j]) : 0.0f) + (e + j == action ? k.slope : 0.0f);
+        }
+        *reinterpret_cast<Pack<T, V>*>(g + e) = pack<T, V>(out);
+    }
+}
+
+// One block a row, V consecutive logits a thread and a turn.
+template <typename T, int V, bool REFERENCE>
+__global__ void __launch_bounds__(kMostThreads) k_policy_loss_long(Loss a) {
+    wait_previous();
+    release_next();
+    __shared__ float most[2][kMostThreads / 32], sums[2][kMostThreads / 32];
+    __shared__ double totals[2][kMostThreads / 32];
+    const int64_t row = blockIdx.x;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    const T* z = static_cast<const T*>(a.logits) + row * a.logits_stride;
+    const T* q = REFERENCE ? static_cast<const T*>(a.reference) + row * a.reference_stride : nullptr;
+    T* g = a.gradient ? static_cast<T*>(a.gradient) + row * a.gradient_stride : nullptr;
+    const int64_t action = a.actions[row];
+    const int whole = a.n / V * V, step = blockDim.x * V;
+    if (!legal(a, row, action)) {
+        if (threadIdx.x == 0) finish_nothing(a, row);
+        if (g == nullptr) return;
+        float zero[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) zero[i] = 0.0f;
+        for (int e = threadIdx.x * V; e < whole; e += step) *reinterpret_cast<Pack<T, V>*>(g + e) = pack<T, V>(zero);
+        for (int e = whole + threadIdx.x; e < a.n; e += blockDim.x) g[e] = Element<T>::store(0.0f);
+        return;
+    }
+    const float chosen = Element<T>::load(z[action]);
+    Sums s;
+    float total = 0.0f, q_total = 0.0f;
+    // the sums so far, moved to a new largest logit
+    auto take = [&](const float (&v)[V], const float (&w)[V], uint32_t bits) {
+        float m = s.m, q_m = s.q_m;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const bool in = bits >> j & 1;
+            m = fmaxf(m, in ? v[j] : -INFINITY);
+            if (REFERENCE) q_m = fmaxf(q_m, in ? w[j] : -INFINITY);
+        }
+        if (m > s.m) {
+            const float f = exponential(s.m - m);
+            s.spread = total != 0.0f ? f * fmaf(s.m - m, total, s.spread) : 0.0f;
+            total *= f;
+            s.apart *= f;
+            s.m = m;
+        }
+        if (REFERENCE && q_m > s.q_m) {
+            q_total *= exponential(s.q_m - q_m);
+            s.q_m = q_m;
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const bool in = bits >> j & 1;  // -inf adds nothing, also while it is all that the thread has seen
+            const float off = v[j] - s.m, e = in && v[j] != -INFINITY ? exponential(off) : 0.0f;
+            const bool counts = e != 0.0f;
+            total += e;
+            s.spread += counts ? e * off : 0.0f;
+            if (REFERENCE) {
+                s.apart += counts ? e * (v[j] - w[j]) : 0.0f;
+                q_total += in && w[j] != -INFINITY ? exponential(w[j] - s.q_m) : 0.0f;
+            }
+        }
+    };
+#pragma unroll 2
+    for (int e = threadIdx.x * V; e < whole; e += step) {
+        float v[V], w[V];
+        unpack<T, V>(load_pack<T, V>(z + e), v);
+        if (REFERENCE) unpack<T, V>(load_pack<T, V>(q + e), w);
+        take(v, w, legal_bits<V>(a, row, e));
+    }
+    for (int e = whole + threadIdx.x; e < a.n; e += blockDim.x) {
+        float v[V], w[V];
+        v[0] = Element<T>::load(z[e]);
+        w[0] = REFERENCE ? Element<T>::load(q[e]) : 0.0f;
+        take(v, w, legal_bits<1>(a, row, e));
+    }
+    // the threads' sums, each moved to the row's largest logit
+    float m = s.m, q_m = s.q_m;
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) {
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        if (REFERENCE) q_m = fmaxf(q_m, __shfl_xor_sync(0xffffffffu, q_m, o));
+    }
+    if (lane == 0) {
+        most[0][warp] = m;
+        most[1][warp] = q_m;
+    }
+    __syncthreads();
+    for (int i = 0; i < warps; ++i) {
+        m = fmaxf(m, most[0][i]);
+        if (REFERENCE) q_m = fmaxf(q_m, most[1][i]);
+    }
+    if (total != 0.0f) {
+        const float f = exponential(s.m - m);
+        s.spread = f * fmaf(s.m - m, total, s.spread);
+        s.apart *= f;
+        total *= f;
+    }
+    if (q_total != 0.0f) q_total *= exponential(s.q_m - q_m);
+    s.m = m;
+    s.q_m = q_m;
+    s.total = total;
+    s.q_total = q_total;
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) {
+        s.total += __shfl_xor_sync(0xffffffffu, s.total, o);
+        s.spread += __shfl_xor_sync(0xffffffffu, s.spread, o);
+        if (REFERENCE) {
+            s.q_total += __shfl_xor_sync(0xffffffffu, s.q_total, o);
+            s.apart += __shfl_xor_sync(0xffffffffu, s.apart, o);
+        }
+    }
+    if (lane == 0) {
+        totals[0][warp] = s.total;
+        totals[1][warp] = s.q_total;
+        sums[0][warp] = s.spread;
+        sums[1][warp] = s.apart;
+    }
+    __syncthreads();
+    s.total = s.q_total = 0.0;
+    s.spread = s.apart = 0.0f;
+    for (int i = 0; i < warps; ++i) {
+        s.total += totals[0][i];
+        s.q_total += totals[1][i];
+        s.spread += sums[0][i];
+        s.apart += sums[1][i];
+    }
+    const Slopes k = finish(a, row, action, chosen, s, threadIdx.x == 0);
+    if (g == nullptr) return;
+    auto slope_of = [&](float v, float w, bool in, int e) {
+        const float off = v - s.m, p = in ? exponential(off) * k.scale : 0.0f;
+        float extra = a.entropy * off;
+        if (REFERENCE) extra = fmaf(a.kl, v - w, extra);
+        return (p != 0.0f ? p * (k.base + extra) : 0.0f) + (e == action ? k.slope : 0.0f);
+    };
+#pragma unroll 2
+    for (int e = threadIdx.x * V; e < whole; e += step) {
+        float v[V], w[V];
+        unpack<T, V>(load_pack<T, V>(z + e), v);
+        if (REFERENCE) unpack<T, V>(load_pack<T, V>(q + e), w);
+        const uint32_t bits = legal_bits<V>(a, row, e);
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = slope_of(v[j], REFERENCE ? w[j] : 0.0f, bits >> j & 1, e + j);
+        *reinterpret_cast<Pack<T, V>*>(g + e) = pack<T, V>(v);
+    }
+    for (int e = whole + threadIdx.x; e < a.n; e += blockDim.x) {
+        g[e] = Element<T>::store(slope_of(Element<T>::load(z[e]), REFERENCE ? Element<T>::load(q[e]) : 0.0f, legal_bits<1>(a, row, e) & 1, e));
+    }
+}
+
+// ------------------------------------------------------------------ dispatch
+template <typename T, int V, bool REFERENCE>
+void launch_loss(const Loss& a, cudaStream_t stream) {
+    if (a.n <= 32 * kMostHeld && a.n % V == 0) {
+        const int held = static_cast<int>((a.n + 32 * V - 1) / (32 * V)) * V;
+        auto kernel = held <= 8 ? k_policy_loss<T, V, 8, REFERENCE> : held <= 16 ? k_policy_loss<T, V, 16, REFERENCE> : k_policy_loss<T, V, 32, REFERENCE>;
+        launch_chain("k_policy_loss", kernel, blocks(a.rows, kWarps), 32 * kWarps, 0, stream, true, a);
+        return;
+    }
+    const int threads = a.n <= 4096 ? 128 : a.n <= 16384 ? 256 : kMostThreads;
+    launch_chain("k_policy_loss_long", k_policy_loss_long<T, V, REFERENCE>, static_cast<unsigned>(a.rows), threads, 0, stream, true, a);
+}
+
+}  // namespace
+}  // namespace op
+}  // namespace t8b
+
+using namespace t8b;
+using namespace t8b::op;
+
+extern "C" int t8b_policy_loss(const t8b_policy_loss_t* call, float* loss, float* log_probabilities, float* entropies, float* divergences,
+                               void* dlogits, int64_t dlogits_stride, void* stream) {
+    return guarded([&] {
+        if (call == nullptr) raise(T8B_EINVAL, "policy loss: the call is null");
+        const t8b_policy_loss_t& c = *call;
+        if (!is_type(c.type)) raise(T8B_EINVAL, "policy loss: unknown type");
+        if (c.mask_kind < T8B_MASK_NONE || c.mask_kind > T8B_MASK_BYTES) raise(T8B_EINVAL, "policy loss: unknown kind of mask");
+        if (c.reference_kind < T8B_REFERENCE_NONE || c.reference_kind > T8B_REFERENCE_SAMPLED) {
+            raise(T8B_EINVAL, "policy loss: unknown kind of reference");
+        }
+        for (float v : {c.clip_low, c.clip_high}) {
+            if (!(v >= 0.0f) || v > std::numeric_limits<float>::max()) raise(T8B_EINVAL, "policy loss: the clipped range must be finite and not negative");
+        }
+        for (float v : {c.kl, c.entropy}) {
+            if (!(std::abs(v) <= std::numeric_limits<float>::max())) raise(T8B_EINVAL, "policy loss: the coefficients must be finite");
+        }
+        if (c.rows < 0 || c.rows > std::numeric_limits<int32_t>::max()) raise(T8B_EINVAL, "policy loss: 0 to 2^31 - 1 rows");
+        if (c.n < 1 || c.n > (1 << 24)) raise(T8B_EINVAL, "policy loss: 1 to 2^24 logits a row");
+        const size_t size = type_size(c.type);
+        const int64_t words = c.mask_kind == T8B_MASK_BITS ? (c.n + 31) / 32 : c.n;
+        const size_t word = c.mask_kind == T8B_MASK_BITS ? 4 : 1;
+        check_matrix("policy loss logits", c.logits, c.rows, c.n, c.logits_stride, size);
+        if (dlogits) check_matrix("policy loss dlogits", dlogits, c.rows, c.n, dlogits_stride, size);
+        if (c.mask_kind) check_matrix("policy loss mask", c.mask, c.rows, words, c.mask_stride, word);
+        if (c.reference_kind == T8B_REFERENCE_LOGITS) check_matrix("policy loss reference", c.reference, c.rows, c.n, c.reference_stride, size);
+        if (c.reference_kind == T8B_REFERENCE_SAMPLED) check_matrix("policy loss reference", c.reference, 1, c.rows, c.rows, sizeof(float));
+        check_elements("policy loss actions", c.actions, sizeof(int64_t));
+        for (const float* p : {c.old_log_probabilities, c.advantages, c.weights, static_cast<const float*>(loss),
+                               static_cast<const float*>(log_probabilities), static_cast<const float*>(entropies), static_cast<const float*>(divergences)}) {
+            check_elements("policy loss", p, sizeof(float));
+        }
+        if (c.rows == 0) return;
+        if (c.actions == nullptr || c.old_log_probabilities == nullptr || c.advantages == nullptr) {
+            raise(T8B_EINVAL, "policy loss: actions, old log-probabilities or advantages are null");
+        }
+        Overlaps o{"policy loss"};
+        o.input(Span(c.logits, c.rows, c.n, c.logits_stride, size));
+        if (c.mask_kind) o.input(Span(c.mask, c.rows, words, c.mask_stride, word));
+        if (c.reference_kind == T8B_REFERENCE_LOGITS) o.input(Span(c.reference, c.rows, c.n, c.reference_stride, size));
+        if (c.reference_kind == T8B_REFERENCE_SAMPLED) o.input(span_of(c.reference, c.rows, sizeof(float)));
+        o.input(span_of(c.actions, c.rows, sizeof(int64_t)));
+        for (const float* p : {c.old_log_probabilities, c.advantages, c.weights}) o.input(span_of(p, c.rows, sizeof(float)));
+        for (float* p : {loss, log_probabilities, entropies, divergences}) o.output(span_of(p, c.rows, sizeof(float)));
+        if (dlogits) o.output(Span(dlogits, c.rows, c.n, dlogits_stride, size));
+        Loss a{};
+        a.logits = c.logits;
+        a.reference = c.reference;
+        a.mask = c.mask;
+        a.actions = c.actions;
+        a.old = c.old_log_probabilities;
+        a.advantages = c.advantages;
+        a.weights = c.weights;
+        a.loss = loss;
+        a.log_probabilities = log_probabilities;
+        a.entropies = entropies;
+        a.divergences = divergences;
+        a.gradient = dlogits;
+        a.logits_stride = c.logits_stride;
+        a.reference_stride = c.reference_stride;
+        a.mask_stride = c.mask_stride;
+        a.gradient_stride = dlogits_stride;
+        a.rows = c.rows;
+        a.n = static_cast<int>(c.n);
+        a.mask_kind = c.mask_kind;
+        a.reference_kind = c.reference_kind;
+        a.low = 1.0f - c.clip_low;
+        a.high = 1.0f + c.clip_high;
+        a.kl = c.kl;
+        a.entropy = c.entropy;
+        a.even = 1.0f / static_cast<float>(c.rows);
+        const bool reference = c.reference_kind == T8B_REFERENCE_LOGITS;
+        auto rows_on_packs = [&](const void* data, int64_t stride) { return aligned(data, 16) && (c.rows == 1 || stride * size % 16 == 0); };
+        // 16 bytes a lane where every row starts on 16 bytes, single logits otherwise
+        const bool wide = rows_on_packs(c.logits, c.logits_stride) && (!reference || rows_on_packs(c.reference, c.reference_stride)) &&
+            (!dlogits || rows_on_packs(dlogits, dlogits_stride));
+        with_type(c.type, [&](auto element) {
+            using T = decltype(element);
+            constexpr int V = 16 / sizeof(T);
+            cudaStream_t st = static_cast<cudaStream_t>(stream);
+            if (wide) {
+                reference ? launch_loss<T, V, true>(a, st) : launch_loss<T, V, false>(a, st);
+            } else {
+                reference ? launch_loss<T, 1, true>(a, st) : launch_loss<T, 1, false>(a, st);
+            }
+        });
+        check(cudaGetLastError(), "policy loss launch");
+    });
+}

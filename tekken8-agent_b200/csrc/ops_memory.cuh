@@ -1,0 +1,152 @@
+// What the sequence operators (causal convolution, selective scan) share: tracks, resets and lengths on
+// the device, and their checks on the host.
+#pragma once
+
+#include <algorithm>
+
+#include "ops.cuh"
+
+namespace t8b {
+namespace op {
+
+// Row t of sequence s of a track.
+template <typename T>
+struct Track {
+    T* data;
+    int64_t sequence, step;
+    Track() = default;
+    explicit Track(const t8b_track_t& t) : data(static_cast<T*>(t.data)), sequence(t.sequence), step(t.step) {}
+    __device__ __forceinline__ T* at(int64_t s) const { return data + s * sequence; }
+};
+
+struct Sequences {
+    int64_t sequences;
+    int steps, channels;
+    const uint8_t* reset;
+    int64_t reset_sequence, reset_step;
+    const int32_t* lengths;
+    Sequences() = default;
+    explicit Sequences(const t8b_sequences_t& q)
+        : sequences(q.sequences), steps(static_cast<int>(q.steps)), channels(static_cast<int>(q.channels)), reset(q.reset),
+          reset_sequence(q.reset_sequence), reset_step(q.reset_step), lengths(q.lengths) {}
+    // steps of sequence s that count
+    __device__ __forceinline__ int live(int64_t s) const {
+        return lengths == nullptr ? steps : min(max(lengths[s], 0), steps);
+    }
+    __device__ __forceinline__ bool resets(int64_t s, int t) const {
+        return reset != nullptr && reset[s * reset_sequence + t * reset_step] != 0;
+    }
+};
+
+// V consecutive elements as they lie in memory, and in fp32.
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> load_pack(const T* p) {
+    return *reinterpret_cast<const Pack<T, V>*>(p);
+}
+template <typename T, int V>
+__device__ __forceinline__ void unpack(const Pack<T, V>& p, float (&v)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = Element<T>::load(p.v[i]);
+}
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> pack(const float (&v)[V]) {
+    Pack<T, V> p;
+    if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+        uint32_t w[V / 2];
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) w[i] = Element<T>::pack(v[2 * i], v[2 * i + 1]);
+        p = *reinterpret_cast<Pack<T, V>*>(w);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) p.v[i] = Element<T>::store(v[i]);
+    }
+    return p;
+}
+
+constexpr float kLn2 = 0.69314718055994531f;
+// exp(v), the argument's product with log2 e to twice the precision: good to 2^x's own 2^-22.
+__device__ __forceinline__ float exponential(float v) {
+    const float high = v * kLog2E;
+    const float low = fmaf(v, 1.925963033e-8f, fmaf(v, kLog2E, -high));  // log2 e - fp32(log2 e)
+    const float r = power_of_two(high);
+    return fabsf(high) < 200.0f ? fmaf(r, low * kLn2, r) : r;
+}
+
+// ------------------------------------------------------------------ host checks
+constexpr int64_t kMostElements = int64_t{1} << 61;
+
+inline void check_sequences(const char* what, const t8b_sequences_t* q, bool step) {
+    const std::string name(what);
+    if (q == nullptr) raise(T8B_EINVAL, name + ": the sequences are null");
+    if (q->sequences < 0 || q->sequences > (int64_t{1} << 30)) raise(T8B_EINVAL, name + ": 0 to 2^30 sequences");
+    if (!step && (q->steps < 0 || q->steps > (int64_t{1} << 30))) raise(T8B_EINVAL, name + ": 0 to 2^30 steps");
+    if (q->channels < 1 || q->channels > (1 << 20)) raise(T8B_EINVAL, name + ": 1 to 2^20 channels");
+    const int64_t steps = step ? 1 : std::max<int64_t>(q->steps, 1);
+    if (q->reset != nullptr &&
+        (q->reset_sequence < 0 || q->reset_step < 0 || q->reset_sequence > kMostElements / std::max<int64_t>(q->sequences, 1) ||
+         q->reset_step > kMostElements / steps)) {
+        raise(T8B_EINVAL, name + ": the strides of reset are out of range");
+    }
+    check_elements(what, q->lengths, sizeof(int32_t));
+}
+inline void check_track(const char* what, const t8b_sequences_t& q, bool step, const t8b_track_t& t, int64_t width, size_t size,
+                        bool output) {
+    const std::string name(what);
+    const int64_t steps = step ? 1 : q.steps;
+    if (q.sequences == 0 || steps == 0) return;
+    if (t.data == nullptr) raise(T8B_EINVAL, name + " is null");
+    check_elements(what, t.data, size);
+    const int64_t s = q.sequences > 1 ? t.sequence : 0, r = steps > 1 ? t.step : 0;
+    if (s < 0 || r < 0 || s > kMostElements / q.sequences || r > kMostElements / steps) {
+        raise(T8B_EINVAL, name + ": a stride is out of range");
+    }
+    if (!output) return;
+    // no two of its rows may share an element: one axis lies within the other's stride
+    const int64_t of_steps = (steps - 1) * r + width, of_sequences = (q.sequences - 1) * s + width;
+    const bool inner_steps = (steps == 1 || r >= width) && (q.sequences == 1 || s >= of_steps);
+    const bool inner_sequences = (q.sequences == 1 || s >= width) && (steps == 1 || r >= of_sequences);
+    if (!inner_steps && !inner_sequences) raise(T8B_EINVAL, name + ": its rows overlap");
+}
+// The bytes that a track spans.
+inline Span span_of(const t8b_sequences_t& q, bool step, const t8b_track_t& t, int64_t width, size_t size) {
+    const int64_t steps = step ? 1 : q.steps;
+    Span span(t.data, 0, 0, 0, 0);
+    if (t.data != nullptr && q.sequences > 0 && steps > 0) {
+        const int64_t s = q.sequences > 1 ? t.sequence : 0, r = steps > 1 ? t.step : 0;
+        span.last = span.first + ((q.sequences - 1) * s + (steps - 1) * r + width) * size;
+    }
+    return span;
+}
+inline Span span_of(const void* data, int64_t count, size_t size) { return Span(data, 1, count, count, size); }
+// No output may overlap an input or another output.
+struct Overlaps {
+    const char* what;
+    std::vector<Span> inputs, outputs;
+    void input(const Span& s) { inputs.push_back(s); }
+    void output(const Span& s) {
+        for (const auto* others : {&inputs, &outputs}) {
+            for (const Span& o : *others) {
+                if (s.overlaps(o)) raise(T8B_EINVAL, std::string(what) + ": an output overlaps an input or another output");
+            }
+        }
+        outputs.push_back(s);
+    }
+};
+// Whether every row of a track starts on `bytes`.
+inline bool rows_aligned(const t8b_sequences_t& q, bool step, const t8b_track_t& t, size_t size, size_t bytes) {
+    const bool s = q.sequences <= 1 || t.sequence * size % bytes == 0;
+    const bool r = step || q.steps <= 1 || t.step * size % bytes == 0;
+    return aligned(t.data, bytes) && s && r;
+}
+
+template <typename Body>
+void with_type(int type, Body&& body) {
+    switch (type) {
+        case T8B_F32: body(float{}); break;
+        case T8B_BF16: body(bf16{}); break;
+        default: body(f16{}); break;
+    }
+}
+
+}  // namespace op
+}  // namespace t8b

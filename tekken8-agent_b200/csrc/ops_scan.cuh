@@ -1,0 +1,941 @@
+// Selective state space scan, forward and backward, over sequences with resets and lengths.
+//
+//   h_t = exp(D_t a) h_(t-1) + D_t u_t B_t,   s_t = sum_n C_t[n] h_t[n] + d u_t,   y_t = s_t silu(z_t)
+//   D_t = softplus(delta_t + bias), or without it
+// and with gs = dy silu(z), e_t = exp(D_t a), g_t = C_t gs_t + e_(t+1) g_(t+1) (the gradient of h_t):
+//   dC = sum_c gs h,   dB = sum_c D u g,   du = d gs + D sum_n B g,   dz = dy s silu'(z),
+//   dD = u sum_n B g + sum_n a e h_(t-1) g,   da = sum_t D e h_(t-1) g
+// At a reset e_t is 0, whatever h_(t-1) is.
+//
+// Forward: LN lanes share a channel and hold NS of its states each in registers, a block the channels
+// that one group of B and C serves; B and C of 8 steps at a time lie in shared memory as fp32.
+// Per (step, channel, state) one 2^x and four multiplications or additions, two of a kind to an
+// instruction: the 2^x unit's 16 results a clock and SM bound it, not memory.
+// Backward: each thread holds a tile of 2 channels x 4 states and goes through 8 steps forward
+// from what the forward pass kept (the state before every eighth step), h in registers, then back.
+// Sums over states and over channels leave the threads as partial sums in shared memory: a thread
+// that adds 16 bytes of them costs a third of what a tree of shuffles takes.
+// Sequences are cut into chunks where there are too few of them: a first pass takes each
+// chunk from a zero state, a second joins the chunks' ends, the last starts each where it belongs.
+#pragma once
+
+#include "ops_memory.cuh"
+
+namespace t8b {
+namespace op {
+namespace scan {
+
+constexpr int kThreads = 128;
+constexpr int kTile = 8;  // steps between two kept states, and of a tile
+constexpr int kSms = 148;
+constexpr int kMostStates = 64;
+
+struct Call {
+    Sequences q;
+    Track<void> u, delta, z, b, c, y, dy;
+    Track<void> du, ddelta, dz, db, dc;
+    int64_t b_group, c_group, db_group, dc_group;
+    const float *a, *d, *delta_bias, *state, *final_gradient;
+    float* final_state;
+    float* saved;    // [sequences][tiles][states][channels]: h before each tile
+    float* dstate;
+    // workspace
+    float* carry;    // [sequences][chunks][states][channels]: a chunk's end from zero, then what it starts from
+    float* sizes;    // [sequences][chunks][channels]: the sum of D over a chunk
+    float* keep;     // [sequences][chunks]: 0 where a chunk has a reset
+    float* shared;   // [blocks of a group][groups][sequences][steps][2][states]: sums of dB and dC
+    float* partial;  // [workers][states + 2][channels]: sums of da, dd and ddelta_bias
+    int groups, per, states, softplus;  // per: channels of a group
+    int chunks, chunk;                  // a chunk's steps, a multiple of kTile
+    int group_blocks, workers;
+};
+
+// ------------------------------------------------------------------ arithmetic
+// log(1 + x) for 0 <= x <= 1: 2 atanh(w), w = x / (2 + x) <= 1/3, by its series (next term 2^-26)
+__device__ __forceinline__ float log_one_plus(float x) {
+    const float w = x * reciprocal(2.0f + x), q = w * w;
+    float p = fmaf(q, 1.0f / 15.0f, 1.0f / 13.0f);
+    p = fmaf(q, p, 1.0f / 11.0f);
+    p = fmaf(q, p, 1.0f / 9.0f);
+    p = fmaf(q, p, 1.0f / 7.0f);
+    p = fmaf(q, p, 1.0f / 5.0f);
+    p = fmaf(q, p, 1.0f / 3.0f);
+    return 2.0f * fmaf(w * q, p, w);
+}
+// softplus(v) = max(v, 0) + log(1 + exp(-|v|)), and its slope sigmoid(v)
+__device__ __forceinline__ float softplus(float v) {
+    const float x = exponential(-fabsf(v));
+    return (v > 0.0f ? v : 0.0f) + log_one_plus(x);
+}
+__device__ __forceinline__ float softplus(float v, float& slope) {
+    const float x = exponential(-fabsf(v));
+    const float r = reciprocal(1.0f + x);
+    slope = v > 0.0f ? r : x * r;
+    return (v > 0.0f ? v : 0.0f) + log_one_plus(x);
+}
+__device__ __forceinline__ Two both(float v) { return Two(v, v); }
+__device__ __forceinline__ Two powers_of_two(const Two& v) {
+    const float2 f = v.get();
+    return Two(power_of_two(f.x), power_of_two(f.y));
+}
+__device__ __forceinline__ Two two(float2 v) { return Two(v.x, v.y); }
+
+// Which of a tile's steps are resets, one bit each: the same in every lane of a warp.
+__device__ __forceinline__ unsigned reset_bits(const Sequences& q, int64_t s, int t0, int end) {
+    if (q.reset == nullptr) return 0;
+    const int t = t0 + static_cast<int>(threadIdx.x & 7);
+    return __ballot_sync(0xffffffffu, t < end && q.resets(s, t)) & 0xffu;
+}
+
+// ------------------------------------------------------------------ forward
+// Where a block stands: block = (s * chunks + chunk) * (blocks of all groups) + group * group_blocks + part.
+struct Place {
+    int64_t s;
+    int chunk, group, part;
+    __device__ __forceinline__ Place(const Call& a, int64_t block) {
+        const int per_chunk = a.groups * a.group_blocks;
+        const int64_t at = block / per_chunk;
+        const int rest = static_cast<int>(block - at * per_chunk);
+        group = rest / a.group_blocks;
+        part = rest - group * a.group_blocks;
+        s = at / a.chunks;
+        chunk = static_cast<int>(at - s * a.chunks);
+    }
+};
+
+// ENDS: a chunk's end from a zero state, the sum of its D, and whether a reset cuts it, in place of y.
+template <typename T, int NS, int LN, bool ENDS>
+__global__ void __launch_bounds__(kThreads) k_scan_forward(Call a) {
+    constexpr int NP = NS * LN, CB = kThreads / LN;
+    wait_previous();
+    release_next();
+    __shared__ __align__(16) float bc[2][kTile][2][NP];
+    const Sequences& q = a.q;
+    const Place place(a, blockIdx.x);
+    const int64_t s = place.s;
+    const int lane = threadIdx.x % LN, local = place.part * CB + threadIdx.x / LN;
+    const bool mine = local < a.per;
+    const int c = place.group * a.per + (mine ? local : 0);
+    const int t0 = place.chunk * a.chunk, t1 = min(q.steps, t0 + a.chunk), last = q.live(s), end = min(t1, last);
+    const int n0 = lane * NS, channels = q.channels;
+    const T* u = static_cast<const T*>(a.u.data) + s * a.u.sequence + c;
+    const T* delta = static_cast<const T*>(a.delta.data) + s * a.delta.sequence + c;
+    const T* z = a.z.data && !ENDS ? static_cast<const T*>(a.z.data) + s * a.z.sequence + c : nullptr;
+    const T* b = static_cast<const T*>(a.b.data) + s * a.b.sequence + place.group * a.b_group;
+    const T* cc = static_cast<const T*>(a.c.data) + s * a.c.sequence + place.group * a.c_group;
+    T* y = static_cast<T*>(a.y.data) + s * a.y.sequence + c;
+    const int64_t at_chunk = s * a.chunks + place.chunk;
+
+    Two rate[NS / 2], h[NS / 2];  // a log2 e, and the states
+#pragma unroll
+    for (int i = 0; i < NS / 2; ++i) {
+        float2 r = make_float2(0.0f, 0.0f), v = r;
+        if (n0 + 2 * i < a.states) r.x = a.a[static_cast<int64_t>(c) * a.states + n0 + 2 * i] * kLog2E;
+        if (n0 + 2 * i + 1 < a.states) r.y = a.a[static_cast<int64_t>(c) * a.states + n0 + 2 * i + 1] * kLog2E;
+        if (!ENDS) {
+            if (a.chunks > 1) {
+                const float* from = a.carry + (at_chunk * a.states + n0 + 2 * i) * channels + c;
+                if (n0 + 2 * i < a.states) v.x = from[0];
+                if (n0 + 2 * i + 1 < a.states) v.y = from[channels];
+            } else if (a.state) {
+                const float* from = a.state + (s * channels + c) * a.states + n0 + 2 * i;
+                if (n0 + 2 * i < a.states) v.x = from[0];
+                if (n0 + 2 * i + 1 < a.states) v.y = from[1];
+            }
+        }
+        rate[i] = two(r);
+        h[i] = two(v);
+    }
+    const float skip = a.d ? a.d[c] : 0.0f, bias = a.delta_bias ? a.delta_bias[c] : 0.0f;
+
+    constexpr int PER = (2 * kTile * NP + kThreads - 1) / kThreads;
+    T raw_u[kTile], raw_delta[kTile], raw_z[kTile], raw_bc[PER];
+    auto fetch = [&](int t) {
+#pragma unroll
+        for (int i = 0; i < kTile; ++i) {
+            const bool live = mine && t + i < end;
+            raw_u[i] = live ? u[(t + i) * a.u.step] : Element<T>::store(0.0f);
+            raw_delta[i] = live ? delta[(t + i) * a.delta.step] : Element<T>::store(0.0f);
+            if (z) raw_z[i] = live ? z[(t + i) * a.z.step] : Element<T>::store(0.0f);
+        }
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int e = i * kThreads + threadIdx.x, step = e / (2 * NP), which = e / NP % 2, n = e % NP;
+            raw_bc[i] = Element<T>::store(0.0f);
+            if (step < kTile && t + step < end && n < a.states) {
+                raw_bc[i] = which ? cc[(t + step) * a.c.step + n] : b[(t + step) * a.b.step + n];
+            }
+        }
+    };
+    auto stage = [&](int buffer) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int e = i * kThreads + threadIdx.x;
+            if (e < 2 * kTile * NP) (&bc[buffer][0][0][0])[e] = Element<T>::load(raw_bc[i]);
+        }
+    };
+    int buffer = 0;
+    float total = 0.0f;
+    bool cut = false;
+    if (t0 < end) {
+        fetch(t0);
+        stage(0);
+        __syncthreads();
+    }
+    for (int t = t0; t < end; t += kTile, buffer ^= 1) {
+        float su[kTile], size[kTile], gate[kTile];
+#pragma unroll
+        for (int i = 0; i < kTile; ++i) {
+            su[i] = Element<T>::load(raw_u[i]);
+            const float v = Element<T>::load(raw_delta[i]) + bias;
+            size[i] = t + i < end ? (a.softplus ? softplus(v) : v) : 0.0f;  // past the end h stays
+            if (z) {
+                const float g = Element<T>::load(raw_z[i]);
+                gate[i] = g * sigmoid(g);
+            }
+        }
+        const unsigned resets = reset_bits(q, s, t, end);
+        if (t + kTile < end) fetch(t + kTile);
+        if (!ENDS && a.saved && mine) {
+            float* to = a.saved + ((s * ((q.steps + kTile - 1) / kTile) + t / kTile) * a.states + n0) * channels + c;
+#pragma unroll
+            for (int i = 0; i < NS; ++i) {
+                const float2 v = h[i / 2].get();
+                if (n0 + i < a.states) to[static_cast<int64_t>(i) * channels] = i % 2 ? v.y : v.x;
+            }
+        }
+        auto step = [&](int i) {
+            const Two by = both(size[i]), in = both(size[i] * su[i]);
+            Two out;
+#pragma unroll
+            for (int k = 0; k < NS / 4; ++k) {
+                const float4 vb = *reinterpret_cast<const float4*>(&bc[buffer][i][0][n0 + 4 * k]);
+                const Two e0 = powers_of_two(by * rate[2 * k]), e1 = powers_of_two(by * rate[2 * k + 1]);
+                h[2 * k] = multiply_add(e0, h[2 * k], in * Two(vb.x, vb.y));
+                h[2 * k + 1] = multiply_add(e1, h[2 * k + 1], in * Two(vb.z, vb.w));
+                if (!ENDS) {
+                    const float4 vc = *reinterpret_cast<const float4*>(&bc[buffer][i][1][n0 + 4 * k]);
+                    out = multiply_add(h[2 * k], Two(vc.x, vc.y), out);
+                    out = multiply_add(h[2 * k + 1], Two(vc.z, vc.w), out);
+                }
+            }
+            if (ENDS) {
+                total += size[i];
+                return;
+            }
+            float sum = out.sum();
+#pragma unroll
+            for (int o = LN / 2; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            sum = fmaf(skip, su[i], sum);
+            if (z) sum *= gate[i];
+            if (mine && lane == 0 && t + i < end) y[(t + i) * a.y.step] = Element<T>::store(sum);
+        };
+        if (resets == 0) {
+#pragma unroll
+            for (int i = 0; i < kTile; ++i) step(i);
+        } else {
+            cut = true;
+#pragma unroll
+            for (int i = 0; i < kTile; ++i) {
+                if (resets >> i & 1) {
+                    if (ENDS) total = 0.0f;
+#pragma unroll
+                    for (int k = 0; k < NS / 2; ++k) h[k] = Two();
+                }
+                step(i);
+            }
+        }
+        if (t + kTile < end) stage(buffer ^ 1);
+        __syncthreads();
+    }
+    if (ENDS) {
+        if (!mine) return;
+        float* to = a.carry + (at_chunk * a.states + n0) * channels + c;
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            const float2 v = h[i / 2].get();
+            if (n0 + i < a.states) to[static_cast<int64_t>(i) * channels] = i % 2 ? v.y : v.x;
+        }
+        if (lane == 0) a.sizes[at_chunk * channels + c] = total;
+        if (lane == 0 && local == 0 && place.group == 0) a.keep[at_chunk] = cut ? 0.0f : 1.0f;
+        return;
+    }
+    if (!mine) return;
+    if (lane == 0) {
+        for (int t = max(t0, end); t < t1; ++t) y[t * a.y.step] = Element<T>::store(0.0f);
+    }
+    if (a.final_state && (last > t0 ? last <= t1 : last == 0 && t0 == 0)) {
+        float* to = a.final_state + (s * channels + c) * a.states + n0;
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            const float2 v = h[i / 2].get();
+            if (n0 + i < a.states) to[i] = i % 2 ? v.y : v.x;
+        }
+    }
+}
+
+// The chunks of a sequence in order (backward: in reverse): what each starts from takes the place of its
+// own end. A thread has one state of one channel.
+static __global__ void __launch_bounds__(256) k_scan_join(Call a, bool backward) {
+    wait_previous();
+    release_next();
+    const int channels = a.q.channels;
+    const int64_t index = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+    const int64_t s = index / (static_cast<int64_t>(a.states) * channels);
+    if (s >= a.q.sequences) return;
+    const int rest = static_cast<int>(index - s * a.states * channels), n = rest / channels, c = rest - n * channels;
+    const float rate = a.a[static_cast<int64_t>(c) * a.states + n] * kLog2E;
+    const float* first = backward ? a.final_gradient : a.state;
+    float h = first ? first[(s * channels + c) * a.states + n] : 0.0f;
+    const int64_t apart = static_cast<int64_t>(a.states) * channels;
+    float* carry = a.carry + s * a.chunks * apart + rest;
+    const float* sizes = a.sizes + s * a.chunks * channels + c;
+    const float* keep = a.keep + s * a.chunks;
+    constexpr int AHEAD = 8;
+    for (int k = 0; k < a.chunks; k += AHEAD) {
+        float ends[AHEAD], size[AHEAD], kept[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            if (k + i >= a.chunks) break;
+            const int at = backward ? a.chunks - 1 - k - i : k + i;
+            ends[i] = carry[at * apart];
+            size[i] = sizes[static_cast<int64_t>(at) * channels];
+            kept[i] = keep[at];
+        }
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            if (k + i >= a.chunks) break;
+            const int at = backward ? a.chunks - 1 - k - i : k + i;
+            carry[at * apart] = h;
+            h = kept[i] != 0.0f ? fmaf(power_of_two(rate * size[i]), h, ends[i]) : ends[i];
+        }
+    }
+}
+
+// ------------------------------------------------------------------ backward
+// What a chunk adds to the gradient of the state before it, the sum of its D, and whether a reset cuts it.
+template <typename T, int NS, int LN>
+__global__ void __launch_bounds__(kThreads) k_scan_back_ends(Call a) {
+    constexpr int NP = NS * LN, CB = kThreads / LN;
+    wait_previous();
+    release_next();
+    __shared__ __align__(16) float vc[kTile][NP];
+    const Sequences& q = a.q;
+    const Place place(a, blockIdx.x);
+    const int64_t s = place.s;
+    const int lane = threadIdx.x % LN, local = place.part * CB + threadIdx.x / LN;
+    const bool mine = local < a.per;
+    const int c = place.group * a.per + (mine ? local : 0);
+    const int t0 = place.chunk * a.chunk, t1 = min(q.steps, t0 + a.chunk), end = min(t1, q.live(s));
+    const int n0 = lane * NS, channels = q.channels;
+    const T* delta = static_cast<const T*>(a.delta.data) + s * a.delta.sequence + c;
+    const T* z = a.z.data ? static_cast<const T*>(a.z.data) + s * a.z.sequence + c : nullptr;
+    const T* dy = static_cast<const T*>(a.dy.data) + s * a.dy.sequence + c;
+    const T* cc = static_cast<const T*>(a.c.data) + s * a.c.sequence + place.group * a.c_group;
+    Two rate[NS / 2], g[NS / 2];
+#pragma unroll
+    for (int i = 0; i < NS / 2; ++i) {
+        float2 r = make_float2(0.0f, 0.0f);
+        if (n0 + 2 * i < a.states) r.x = a.a[static_cast<int64_t>(c) * a.states + n0 + 2 * i] * kLog2E;
+        if (n0 + 2 * i + 1 < a.states) r.y = a.a[static_cast<int64_t>(c) * a.states + n0 + 2 * i + 1] * kLog2E;
+        rate[i] = two(r);
+    }
+    const float bias = a.delta_bias ? a.delta_bias[c] : 0.0f;
+    float total = 0.0f;
+    bool cut = false;
+    for (int t = t0 + (end - 1 - t0) / kTile * kTile; end > t0 && t >= t0; t -= kTile) {
+        float size[kTile], given[kTile];
+#pragma unroll
+        for (int i = 0; i < kTile; ++i) {
+            const bool live = mine && t + i < end;
+            const float v = live ? Element<T>::load(delta[(t + i) * a.delta.step]) + bias : 0.0f;
+            given[i] = live ? Element<T>::load(dy[(t + i) * a.dy.step]) : 0.0f;
+            if (z && live) {
+                const float w = Element<T>::load(z[(t + i) * a.z.step]);
+                given[i] *= w * sigmoid(w);
+            }
+            size[i] = live ? (a.softplus ? softplus(v) : v) : 0.0f;
+        }
+        __syncthreads();
+        for (int e = threadIdx.x; e < kTile * NP; e += kThreads) {
+            const int step = e / NP, n = e % NP;
+            vc[step][n] = t + step < end && n < a.states ? Element<T>::load(cc[(t + step) * a.c.step + n]) : 0.0f;
+        }
+        const unsigned resets = reset_bits(q, s, t, end);
+        cut = cut || resets != 0;
+        __syncthreads();
+#pragma unroll
+        for (int i = kTile - 1; i >= 0; --i) {
+            const Two by = both(size[i]), in = both(given[i]);
+            total += size[i];
+#pragma unroll
+            for (int k = 0; k < NS / 2; ++k) {
+                const float2 w = *reinterpret_cast<const float2*>(&vc[i][n0 + 2 * k]);
+                g[k] = multiply_add(in, two(w), g[k]) * powers_of_two(by * rate[k]);
+            }
+            if (resets >> i & 1) {
+#pragma unroll
+                for (int k = 0; k < NS / 2; ++k) g[k] = Two();
+            }
+        }
+    }
+    if (!mine) return;
+    const int64_t at_chunk = s * a.chunks + place.chunk;
+    float* to = a.carry + (at_chunk * a.states + n0) * channels + c;
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+        const float2 v = g[i / 2].get();
+        if (n0 + i < a.states) to[static_cast<int64_t>(i) * channels] = i % 2 ? v.y : v.x;
+    }
+    if (lane == 0) a.sizes[at_chunk * channels + c] = total;
+    if (lane == 0 && local == 0 && place.group == 0) a.keep[at_chunk] = cut ? 0.0f : 1.0f;
+}
+
+// Shared memory of a block of the backward pass, for LN lanes along the states (4 each).
+template <int LN>
+struct BackwardShape {
+    static constexpr int NP = 4 * LN, LC = 32 / LN;          // states; lanes along the channels
+    static constexpr int CB = (kThreads / 32) * LC * 2;      // channels of a block
+    static constexpr int PT = kTile * CB / kThreads;         // steps whose elementwise part a thread has
+    static constexpr int PARTS = LC * (kThreads / 32);       // pairs of channels, and partial sums of a state
+    static constexpr int SPLIT = PARTS > 16 ? 2 : 1;         // threads that add up four states' partial sums
+    // Where pair p's sums of lane `along` lie: rows are rotated, so that neither the threads that write
+    // them nor those that add them up meet in a bank.
+    __device__ __forceinline__ static int channel_at(int p, int along) { return (p + LC * along) % (CB / 2); }
+    __device__ __forceinline__ static int state_at(int p, int along) { return (p + SPLIT * along) % PARTS; }
+    struct Shared {
+        float size[kTile][CB], in[kTile][CB], given[kTile][CB];  // D, D u, gs
+        float u[kTile][CB], slope[kTile][CB], zslope[kTile][CB];
+        float b[kTile][NP], c[kTile][NP];
+        float2 channel_sums[kTile][3][LN][CB / 2];       // sum_n: C h, B g, a e h g, of each lane along the states
+        float4 state_sums[kTile][2][LN][PARTS];          // sum_c: D u g, gs h, of each pair of channels
+    };
+};
+
+template <typename T, int LN>
+__global__ void __launch_bounds__(kThreads, LN == 4 ? 3 : 2) k_scan_backward(Call a) {
+    using Shape = BackwardShape<LN>;
+    constexpr int NP = Shape::NP, LC = Shape::LC, CB = Shape::CB, PT = Shape::PT, PARTS = Shape::PARTS;
+    wait_previous();
+    release_next();
+    extern __shared__ __align__(16) unsigned char memory[];
+    auto& m = *reinterpret_cast<typename Shape::Shared*>(memory);
+    const Sequences& q = a.q;
+    const int group = blockIdx.x / a.group_blocks, part = blockIdx.x - group * a.group_blocks;
+    const int channels = q.channels, tiles = (q.steps + kTile - 1) / kTile;
+    // this thread's tile: channels c0 and c0 + 1, states n0 to n0 + 3
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, across = lane % LC, along = lane / LC;
+    const int pair = warp * LC + across, n0 = 4 * along;
+    const int c0 = group * a.per + part * CB + 2 * pair;
+    const bool has0 = part * CB + 2 * pair < a.per, has1 = part * CB + 2 * pair + 1 < a.per;
+    // and its elementwise part: channel ec, steps e0 to e0 + PT - 1 of a tile
+    const int el = threadIdx.x % CB, e0 = threadIdx.x / CB * PT;
+    const bool emine = part * CB + el < a.per;
+    const int ec = group * a.per + (emine ? part * CB + el : 0);
+    const float skip = a.d ? a.d[ec] : 0.0f, bias = a.delta_bias ? a.delta_bias[ec] : 0.0f;
+
+    Two rate[4], da[4];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+        float2 r = make_float2(0.0f, 0.0f);
+        if (n0 + n < a.states) {
+            if (has0) r.x = a.a[static_cast<int64_t>(c0) * a.states + n0 + n] * kLog2E;
+            if (has1) r.y = a.a[static_cast<int64_t>(c0 + 1) * a.states + n0 + n] * kLog2E;
+        }
+        rate[n] = two(r);
+    }
+    float dd = 0.0f, dbias = 0.0f;
+
+    constexpr int PER = (2 * kTile * NP + kThreads - 1) / kThreads;
+    T raw_u[PT], raw_delta[PT], raw_z[PT], raw_dy[PT], raw_bc[PER];
+    const bool gate = a.z.data != nullptr;
+    const int64_t items = q.sequences * a.chunks;
+    for (int64_t item = blockIdx.y; item < items; item += a.workers) {
+        const int64_t s = item / a.chunks;
+        const int chunk = static_cast<int>(item - s * a.chunks);
+        const int t0 = chunk * a.chunk, t1 = min(q.steps, t0 + a.chunk), last = q.live(s), end = min(t1, last);
+        const T* u = static_cast<const T*>(a.u.data) + s * a.u.sequence + ec;
+        const T* delta = static_cast<const T*>(a.delta.data) + s * a.delta.sequence + ec;
+        const T* z = static_cast<const T*>(a.z.data) + s * a.z.sequence + ec;
+        const T* dy = static_cast<const T*>(a.dy.data) + s * a.dy.sequence + ec;
+        T* du = static_cast<T*>(a.du.data) + s * a.du.sequence + ec;
+        T* ddelta = static_cast<T*>(a.ddelta.data) + s * a.ddelta.sequence + ec;
+        T* dz = static_cast<T*>(a.dz.data) + s * a.dz.sequence + ec;
+        const T* b = static_cast<const T*>(a.b.data) + s * a.b.sequence + group * a.b_group;
+        const T* cc = static_cast<const T*>(a.c.data) + s * a.c.sequence + group * a.c_group;
+        auto fetch = [&](int t) {
+#pragma unroll
+            for (int i = 0; i < PT; ++i) {
+                const int at = t + e0 + i;
+                raw_u[i] = raw_delta[i] = raw_z[i] = raw_dy[i] = Element<T>::store(0.0f);
+                if (emine && at < end) {
+                    raw_u[i] = u[at * a.u.step];
+                    raw_delta[i] = delta[at * a.delta.step];
+                    raw_dy[i] = dy[at * a.dy.step];
+                    if (gate) raw_z[i] = z[at * a.z.step];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const int e = i * kThreads + threadIdx.x, step = e / (2 * NP), which = e / NP % 2, n = e % NP;
+                raw_bc[i] = Element<T>::store(0.0f);
+                if (step < kTile && t + step < end && n < a.states) {
+                    raw_bc[i] = which ? cc[(t + step) * a.c.step + n] : b[(t + step) * a.b.step + n];
+                }
+            }
+        };
+        // the gradient of the state after the chunk
+        Two g[4];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            float2 v = make_float2(0.0f, 0.0f);
+            if (n0 + n < a.states) {
+                if (a.chunks > 1) {
+                    const float* from = a.carry + (item * a.states + n0 + n) * channels + c0;
+                    if (has0) v.x = from[0];
+                    if (has1) v.y = from[1];
+                } else if (a.final_gradient) {
+                    const float* from = a.final_gradient + (s * channels + c0) * a.states + n0 + n;
+                    if (has0) v.x = from[0];
+                    if (has1) v.y = from[a.states];
+                }
+            }
+            g[n] = two(v);
+        }
+        int t = t0 + (end - 1 - t0) / kTile * kTile;
+        if (end > t0) fetch(t);
+        for (; end > t0 && t >= t0; t -= kTile) {
+            // ---- elementwise: D, D u and gs of the tile into shared memory
+#pragma unroll
+            for (int i = 0; i < PT; ++i) {
+                const bool live = emine && t + e0 + i < end;
+                const float vu = Element<T>::load(raw_u[i]), v = Element<T>::load(raw_delta[i]) + bias, vdy = Element<T>::load(raw_dy[i]);
+                float slope = 1.0f, size = v, given = vdy, zslope = 0.0f;
+                if (a.softplus) size = softplus(v, slope);
+                if (gate) {
+                    const float w = Element<T>::load(raw_z[i]);
+                    float value;
+                    activate_slope<T8B_SILU>(w, value, zslope);
+                    given = vdy * value;
+                    zslope *= vdy;
+                }
+                m.size[e0 + i][el] = live ? size : 0.0f;
+                m.in[e0 + i][el] = live ? size * vu : 0.0f;
+                m.given[e0 + i][el] = live ? given : 0.0f;
+                m.u[e0 + i][el] = vu;
+                m.slope[e0 + i][el] = slope;
+                m.zslope[e0 + i][el] = zslope;
+            }
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const int e = i * kThreads + threadIdx.x, step = e / (2 * NP), which = e / NP % 2, n = e % NP;
+                if (step < kTile) (which ? m.c : m.b)[step][n] = Element<T>::load(raw_bc[i]);
+            }
+            const unsigned resets = reset_bits(q, s, t, end);
+            Two before[4];
+            {
+                const float* from = a.saved + ((s * tiles + t / kTile) * a.states + n0) * channels + c0;
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                    float2 v = make_float2(0.0f, 0.0f);
+                    if (n0 + n < a.states) {
+                        if (has0) v.x = from[static_cast<int64_t>(n) * channels];
+                        if (has1) v.y = from[static_cast<int64_t>(n) * channels + 1];
+                    }
+                    before[n] = two(v);
+                }
+            }
+            __syncthreads();
+            if (t > t0) fetch(t - kTile);
+            // ---- h through the tile, then g back
+            auto pass = [&](auto cuts) {
+                constexpr bool CUTS = decltype(cuts)::value != 0;
+                Two h[kTile][4];
+#pragma unroll
+                for (int i = 0; i < kTile; ++i) {
+                    const Two by = two(*reinterpret_cast<const float2*>(&m.size[i][2 * pair]));
+                    const Two in = two(*reinterpret_cast<const float2*>(&m.in[i][2 * pair]));
+                    const float4 vb = *reinterpret_cast<const float4*>(&m.b[i][n0]);
+                    const float bn[4] = {vb.x, vb.y, vb.z, vb.w};
+                    const bool reset = CUTS && (resets >> i & 1);
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) {
+                        const Two from = reset ? Two() : i ? h[i ? i - 1 : 0][n] : before[n];
+                        h[i][n] = multiply_add(powers_of_two(by * rate[n]), from, in * both(bn[n]));
+                    }
+                }
+#pragma unroll
+                for (int i = kTile - 1; i >= 0; --i) {
+                    const Two by = two(*reinterpret_cast<const float2*>(&m.size[i][2 * pair]));
+                    const Two in = two(*reinterpret_cast<const float2*>(&m.in[i][2 * pair]));
+                    const Two given = two(*reinterpret_cast<const float2*>(&m.given[i][2 * pair]));
+                    const float4 vb = *reinterpret_cast<const float4*>(&m.b[i][n0]), vc = *reinterpret_cast<const float4*>(&m.c[i][n0]);
+                    const float bn[4] = {vb.x, vb.y, vb.z, vb.w}, cn[4] = {vc.x, vc.y, vc.z, vc.w};
+                    const bool reset = CUTS && (resets >> i & 1);
+                    Two of_h, of_b, of_a;
+                    float4 db, dc;
+                    float* to_b = &db.x;
+                    float* to_c = &dc.x;
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) {
+                        g[n] = multiply_add(given, both(cn[n]), g[n]);
+                        of_h = multiply_add(h[i][n], both(cn[n]), of_h);
+                        of_b = multiply_add(g[n], both(bn[n]), of_b);
+                        to_b[n] = (in * g[n]).sum();
+                        to_c[n] = (given * h[i][n]).sum();
+                        g[n] = reset ? Two() : g[n] * powers_of_two(by * rate[n]);
+                        const Two from = reset ? Two() : i ? h[i ? i - 1 : 0][n] : before[n];
+                        const Two through = g[n] * from;
+                        of_a = multiply_add(through, rate[n], of_a);
+                        da[n] = multiply_add(through, by, da[n]);
+                    }
+                    m.channel_sums[i][0][along][Shape::channel_at(pair, along)] = of_h.get();
+                    m.channel_sums[i][1][along][Shape::channel_at(pair, along)] = of_b.get();
+                    m.channel_sums[i][2][along][Shape::channel_at(pair, along)] = of_a.get();
+                    m.state_sums[i][0][along][Shape::state_at(pair, along)] = db;
+                    m.state_sums[i][1][along][Shape::state_at(pair, along)] = dc;
+                }
+            };
+            if (resets == 0) {
+                pass(Constant<0>{});
+            } else {
+                pass(Constant<1>{});
+            }
+            __syncthreads();
+            // ---- the sums over states, and the gradients of u, delta and z
+#pragma unroll
+            for (int i = 0; i < PT; ++i) {
+                const int at = t + e0 + i;
+                float sum[3];
+#pragma unroll
+                for (int k = 0; k < 3; ++k) {
+                    sum[k] = 0.0f;
+#pragma unroll
+                    for (int l = 0; l < LN; ++l) {
+                        sum[k] += reinterpret_cast<const float*>(m.channel_sums[e0 + i][k][l])[2 * Shape::channel_at(el / 2, l) + el % 2];
+                    }
+                }
+                const float size = m.size[e0 + i][el], given = m.given[e0 + i][el], vu = m.u[e0 + i][el];
+                if (emine && at < t1) {
+                    const bool live = at < end;
+                    const float to_size = live ? (vu * sum[1] + kLn2 * sum[2]) * m.slope[e0 + i][el] : 0.0f;
+                    du[at * a.du.step] = Element<T>::store(live ? fmaf(skip, given, size * sum[1]) : 0.0f);
+                    ddelta[at * a.ddelta.step] = Element<T>::store(to_size);
+                    if (a.dz.data) dz[at * a.dz.step] = Element<T>::store(live ? m.zslope[e0 + i][el] * fmaf(skip, vu, sum[0]) : 0.0f);
+                    dbias += to_size;
+                    if (live) dd = fmaf(given, vu, dd);
+                }
+            }
+            // ---- the sums over channels
+            constexpr int SPLIT = Shape::SPLIT;
+            for (int e = threadIdx.x; e < kTile * 2 * LN * SPLIT; e += kThreads) {
+                const int quad = e / SPLIT, half = e % SPLIT, step = quad / (2 * LN), which = quad / LN % 2, l = quad % LN;
+                Two x, y;
+#pragma unroll
+                for (int p = 0; p < PARTS; p += SPLIT) {
+                    const float4 v = m.state_sums[step][which][l][Shape::state_at(p + half, l)];
+                    x = x + Two(v.x, v.y);
+                    y = y + Two(v.z, v.w);
+                }
+                float2 vx = x.get(), vy = y.get();
+                if (SPLIT == 2) {  // every lane is here: kTile 2 LN SPLIT is a multiple of kThreads
+                    vx.x += __shfl_xor_sync(0xffffffffu, vx.x, 1);
+                    vx.y += __shfl_xor_sync(0xffffffffu, vx.y, 1);
+                    vy.x += __shfl_xor_sync(0xffffffffu, vy.x, 1);
+                    vy.y += __shfl_xor_sync(0xffffffffu, vy.y, 1);
+                }
+                if (half != 0 || t + step >= end) continue;
+                const float sum[4] = {vx.x, vx.y, vy.x, vy.y};
+                float* to = a.shared +
+                    ((((static_cast<int64_t>(part) * a.groups + group) * q.sequences + s) * q.steps + t + step) * 2 + which) * a.states + 4 * l;
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                    if (4 * l + n < a.states) to[n] = sum[n];
+                }
+            }
+        }
+        // past the sequence's end
+        if (emine) {
+            for (int at = max(t0, t0 + (end > t0 ? (end - t0 + kTile - 1) / kTile * kTile : 0)) + threadIdx.x / CB; at < t1; at += kThreads / CB) {
+                du[at * a.du.step] = Element<T>::store(0.0f);
+                ddelta[at * a.ddelta.step] = Element<T>::store(0.0f);
+                if (a.dz.data) dz[at * a.dz.step] = Element<T>::store(0.0f);
+            }
+        }
+        if (chunk == 0 && a.dstate) {
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                const float2 v = g[n].get();
+                float* to = a.dstate + (s * channels + c0) * a.states + n0 + n;
+                if (n0 + n < a.states && has0) to[0] = v.x;
+                if (n0 + n < a.states && has1) to[a.states] = v.y;
+            }
+        }
+        __syncthreads();  // the next item's tile writes what this one's last still reads
+    }
+    // this worker's sums of the parameters' gradients
+    float* out = a.partial + static_cast<int64_t>(blockIdx.y) * (a.states + 2) * channels;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+        const float2 v = da[n].get();
+        if (n0 + n < a.states && has0) out[static_cast<int64_t>(n0 + n) * channels + c0] = v.x;
+        if (n0 + n < a.states && has1) out[static_cast<int64_t>(n0 + n) * channels + c0 + 1] = v.y;
+    }
+    m.size[e0 / PT][el] = dd;  // one row of threads, PT steps each, a row of the tile
+    m.in[e0 / PT][el] = dbias;
+    __syncthreads();
+    if (threadIdx.x < CB && emine) {
+        dd = dbias = 0.0f;
+        for (int r = 0; r < kTile / PT; ++r) {
+            dd += m.size[r][el];
+            dbias += m.in[r][el];
+        }
+        out[static_cast<int64_t>(a.states) * channels + ec] = dd;
+        out[static_cast<int64_t>(a.states + 1) * channels + ec] = dbias;
+    }
+}
+
+// da, dd and ddelta_bias from the workers' sums. Block (32, 16): 32 of the (states + 2) channels columns.
+static __global__ void k_scan_parameters(Call a, float* da, float* dd, float* dbias) {
+    wait_previous();
+    release_next();
+    __shared__ float sums[16][33];
+    const int channels = a.q.channels;
+    const int64_t columns = static_cast<int64_t>(a.states + 2) * channels, column = static_cast<int64_t>(blockIdx.x) * 32 + threadIdx.x;
+    float v = 0.0f;
+    if (column < columns) {
+#pragma unroll 4
+        for (int r = threadIdx.y; r < a.workers; r += 16) v += a.partial[r * columns + column];
+    }
+    sums[threadIdx.y][threadIdx.x] = v;
+    __syncthreads();
+    if (threadIdx.y != 0 || column >= columns) return;
+#pragma unroll
+    for (int r = 1; r < 16; ++r) v += sums[r][threadIdx.x];
+    const int n = static_cast<int>(column / channels), c = static_cast<int>(column - static_cast<int64_t>(n) * channels);
+    if (n < a.states) {
+        da[static_cast<int64_t>(c) * a.states + n] = v;
+    } else if (n == a.states) {
+        if (dd) dd[c] = v;
+    } else if (dbias) {
+        dbias[c] = v;
+    }
+}
+
+// dB and dC from the blocks' sums: one thread a (sequence, step, group, b or c, state).
+template <typename T>
+__global__ void __launch_bounds__(256) k_scan_shared(Call a) {
+    wait_previous();
+    release_next();
+    const Sequences& q = a.q;
+    const int64_t index = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    const int width = 2 * a.states;
+    const int64_t row = index / width;  // (group, sequence, step)
+    const int e = static_cast<int>(index - row * width);
+    const int64_t rows = q.sequences * q.steps;
+    if (row >= rows * a.groups) return;
+    const int group = static_cast<int>(row / rows);
+    const int64_t at = row - group * rows, s = at / q.steps;
+    const int t = static_cast<int>(at - s * q.steps), which = e / a.states, n = e - which * a.states;
+    float v = 0.0f;
+    if (t < q.live(s)) {
+        const int64_t apart = a.groups * rows * width;
+        for (int p = 0; p < a.group_blocks; ++p) v += a.shared[p * apart + index];
+    }
+    T* to = which ? static_cast<T*>(a.dc.data) + s * a.dc.sequence + t * a.dc.step + group * a.dc_group
+                  : static_cast<T*>(a.db.data) + s * a.db.sequence + t * a.db.step + group * a.db_group;
+    to[n] = Element<T>::store(v);
+}
+
+// ------------------------------------------------------------------ a single step
+// LP lanes (a power of two) share a channel of a sequence and hold V consecutive states each; bound by
+// the states' bytes, read once and written once. A thread takes several sequences, their states all in flight.
+constexpr int kStepAhead = 4;
+template <typename T, int V>
+__global__ void __launch_bounds__(256) k_scan_step(Call a, float* state, int lanes) {
+    wait_previous();
+    release_next();
+    const Sequences& q = a.q;
+    const int channels = q.channels;
+    const int64_t index = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    const int64_t unit = index / lanes;
+    const int lane = static_cast<int>(index - unit * lanes);
+    const int64_t turn = unit / channels;
+    const int c = static_cast<int>(unit - turn * channels), group = c / a.per;
+    const int64_t s0 = turn * kStepAhead;
+    const int count = static_cast<int>(max(int64_t{0}, min(int64_t{kStepAhead}, q.sequences - s0)));
+    const float skip = a.d ? a.d[c] : 0.0f, bias = a.delta_bias ? a.delta_bias[c] : 0.0f;
+    float sum[kStepAhead], size[kStepAhead], in[kStepAhead], vu[kStepAhead];
+    bool cut[kStepAhead];
+#pragma unroll
+    for (int i = 0; i < kStepAhead; ++i) {
+        sum[i] = 0.0f;
+        if (i >= count) continue;
+        const int64_t s = s0 + i;
+        vu[i] = Element<T>::load(static_cast<const T*>(a.u.data)[s * a.u.sequence + c]);
+        const float v = Element<T>::load(static_cast<const T*>(a.delta.data)[s * a.delta.sequence + c]) + bias;
+        size[i] = a.softplus ? softplus(v) : v;
+        in[i] = size[i] * vu[i];
+        cut[i] = q.reset != nullptr && q.reset[s * q.reset_sequence] != 0;
+    }
+    for (int n0 = lane * V; n0 < a.states; n0 += lanes * V) {
+        Pack<float, V> h[kStepAhead];
+        float rate[V];
+#pragma unroll
+        for (int i = 0; i < kStepAhead; ++i) {
+            if (i < count) h[i] = load_pack<float, V>(state + ((s0 + i) * channels + c) * a.states + n0);
+        }
+        const Pack<float, V> r = load_pack<float, V>(a.a + static_cast<int64_t>(c) * a.states + n0);
+#pragma unroll
+        for (int v = 0; v < V; ++v) rate[v] = r.v[v] * kLog2E;
+#pragma unroll
+        for (int i = 0; i < kStepAhead; ++i) {
+            if (i >= count) continue;
+            const int64_t s = s0 + i;
+            const T* b = static_cast<const T*>(a.b.data) + s * a.b.sequence + group * a.b_group + n0;
+            const T* cc = static_cast<const T*>(a.c.data) + s * a.c.sequence + group * a.c_group + n0;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const float from = cut[i] ? 0.0f : h[i].v[v];
+                h[i].v[v] = fmaf(power_of_two(size[i] * rate[v]), from, in[i] * Element<T>::load(b[v]));
+                sum[i] = fmaf(h[i].v[v], Element<T>::load(cc[v]), sum[i]);
+            }
+            *reinterpret_cast<Pack<float, V>*>(state + (s * channels + c) * a.states + n0) = h[i];
+        }
+    }
+    for (int o = lanes / 2; o >= 1; o >>= 1) {
+#pragma unroll
+        for (int i = 0; i < kStepAhead; ++i) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], o);
+    }
+    if (lane != 0) return;
+#pragma unroll
+    for (int i = 0; i < kStepAhead; ++i) {
+        if (i >= count) continue;
+        const int64_t s = s0 + i;
+        float y = fmaf(skip, vu[i], sum[i]);
+        if (a.z.data) {
+            const float w = Element<T>::load(static_cast<const T*>(a.z.data)[s * a.z.sequence + c]);
+            y *= w * sigmoid(w);
+        }
+        static_cast<T*>(a.y.data)[s * a.y.sequence + c] = Element<T>::store(y);
+    }
+}
+
+// ------------------------------------------------------------------ host
+// Lanes of a channel and states of a lane, for `states` states.
+inline int padded(int64_t states) { return states <= 16 ? 16 : states <= 32 ? 32 : 64; }
+inline int64_t tiles_of(int64_t steps) { return (steps + kTile - 1) / kTile; }
+
+// The forward pass's chunks.
+struct ForwardPlan {
+    int channels, group_blocks, chunks, chunk;
+    int64_t blocks;
+    ForwardPlan(const t8b_sequences_t& q, int64_t groups, int64_t states) {
+        channels = kThreads * 16 / padded(states);
+        group_blocks = static_cast<int>((q.channels / groups + channels - 1) / channels);
+        const int64_t per_chunk = q.sequences * groups * group_blocks, steps = std::max<int64_t>(q.steps, 1);
+        // cut where fewer than two blocks an SM would run; cutting takes every exponential twice
+        int64_t want = 1;
+        if (per_chunk < 2 * kSms) want = std::max<int64_t>(1, std::min<int64_t>(5 * kSms / std::max<int64_t>(per_chunk, 1), steps / 32));
+        if (want < 3) want = 1;
+        chunk = static_cast<int>(round_up((steps + want - 1) / want, kTile));
+        chunks = static_cast<int>((steps + chunk - 1) / chunk);
+        blocks = per_chunk * chunks;
+    }
+};
+struct BackwardPlan {
+    int channels, group_blocks, chunks, chunk, workers;
+    int end_blocks;  // blocks of a group in k_scan_back_ends
+    BackwardPlan(const t8b_sequences_t& q, int64_t groups, int64_t states) {
+        channels = kThreads / 32 * 2 * (32 / (padded(states) / 4));
+        group_blocks = static_cast<int>((q.channels / groups + channels - 1) / channels);
+        end_blocks = static_cast<int>((q.channels / groups + kThreads * 16 / padded(states) - 1) / (kThreads * 16 / padded(states)));
+        const int64_t across = groups * group_blocks, steps = std::max<int64_t>(q.steps, 1);
+        const int64_t resident = std::max<int64_t>(1, 3 * kSms / across);
+        // the least time by rounds of resident blocks; a cut takes a third more work
+        int64_t best = 0, want = 1;
+        for (int64_t parts = 1; parts <= std::max<int64_t>(1, steps / 64); parts = parts < 8 ? parts + 1 : parts + parts / 4) {
+            const int64_t length = round_up((steps + parts - 1) / parts, kTile), count = (steps + length - 1) / length;
+            const int64_t rounds = (q.sequences * count + resident - 1) / resident;
+            const int64_t cost = rounds * length * (count > 1 ? 4 : 3);
+            if (best == 0 || cost < best) {
+                best = cost;
+                want = parts;
+            }
+            if (q.sequences * count > 4 * resident) break;
+        }
+        chunk = static_cast<int>(round_up((steps + want - 1) / want, kTile));
+        chunks = static_cast<int>((steps + chunk - 1) / chunk);
+        workers = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(resident, q.sequences * chunks)));
+    }
+};
+
+template <typename T>
+void launch_forward(const Call& given, const ForwardPlan& plan, int64_t states, cudaStream_t stream) {
+    Call a = given;
+    a.chunks = plan.chunks;
+    a.chunk = plan.chunk;
+    a.group_blocks = plan.group_blocks;
+    auto go = [&](auto main, auto ends) {
+        const unsigned grid = static_cast<unsigned>(plan.blocks);
+        if (a.chunks > 1) {
+            launch_chain("k_scan_ends", ends, grid, kThreads, 0, stream, true, a);
+            launch_chain("k_scan_join", k_scan_join, blocks(a.q.sequences * states * a.q.channels, 256), 256, 0, stream, true, a, false);
+        }
+        launch_chain("k_scan_forward", main, grid, kThreads, 0, stream, true, a);
+    };
+    switch (padded(states)) {
+        case 16: go(k_scan_forward<T, 16, 1, false>, k_scan_forward<T, 16, 1, true>); break;
+        case 32: go(k_scan_forward<T, 16, 2, false>, k_scan_forward<T, 16, 2, true>); break;
+        default: go(k_scan_forward<T, 16, 4, false>, k_scan_forward<T, 16, 4, true>); break;
+    }
+}
+
+template <typename T, int LN>
+void launch_backward_tiles(const Call& a, cudaStream_t stream) {
+    constexpr size_t bytes = sizeof(typename BackwardShape<LN>::Shared);
+    static uint64_t configured = 0;
+    allow_smem(k_scan_backward<T, LN>, bytes, configured);
+    launch_chain("k_scan_backward", k_scan_backward<T, LN>, dim3(a.groups * a.group_blocks, a.workers), kThreads, bytes, stream, true, a);
+}
+
+template <typename T>
+void launch_backward(const Call& given, const BackwardPlan& plan, float* da, float* dd, float* dbias, cudaStream_t stream) {
+    Call a = given;
+    a.chunks = plan.chunks;
+    a.chunk = plan.chunk;
+    a.workers = plan.workers;
+    const int width = padded(a.states);
+    if (a.chunks > 1) {
+        a.group_blocks = plan.end_blocks;
+        const int64_t grid = a.q.sequences * a.chunks * a.groups * a.group_blocks;
+        auto ends = width == 16 ? k_scan_back_ends<T, 16, 1> : width == 32 ? k_scan_back_ends<T, 16, 2> : k_scan_back_ends<T, 16, 4>;
+        launch_chain("k_scan_back_ends", ends, static_cast<unsigned>(grid), kThreads, 0, stream, true, a);
+        launch_chain("k_scan_join", k_scan_join, blocks(a.q.sequences * a.states * a.q.channels, 256), 256, 0, stream, true, a, true);
+    }
+    a.group_blocks = plan.group_blocks;
+    switch (width) {
+        case 16: launch_backward_tiles<T, 4>(a, stream); break;
+        case 32: launch_backward_tiles<T, 8>(a, stream); break;
+        default: launch_backward_tiles<T, 16>(a, stream); break;
+    }
+    launch_chain("k_scan_parameters", k_scan_parameters, blocks(static_cast<int64_t>(a.states + 2) * a.q.channels, 32), dim3(32, 16), 0, stream,
+                 true, a, da, dd, dbias);
+    const int64_t outputs = a.groups * a.q.sequences * a.q.steps * 2 * a.states;
+    launch_chain("k_scan_shared", k_scan_shared<T>, static_cast<unsigned>((outputs + 255) / 256), 256, 0, stream, true, a);
+}
+
+template <typename T>
+void launch_step(const Call& a, float* state, bool wide, cudaStream_t stream) {
+    const int packs = wide ? a.states / 4 : a.states;
+    int lanes = 1;
+    while (lanes < packs && lanes < 32) lanes *= 2;
+    const int64_t turns = (a.q.sequences + kStepAhead - 1) / kStepAhead;
+    const int64_t grid = (turns * a.q.channels * lanes + 255) / 256;
+    if (grid > std::numeric_limits<int32_t>::max()) raise(T8B_EINVAL, "selective scan step: too many elements for one call");
+    launch_chain("k_scan_step", wide ? k_scan_step<T, 4> : k_scan_step<T, 1>, static_cast<unsigned>(grid), 256, 0, stream, true, a, state, lanes);
+}
+
+}  // namespace scan
+}  // namespace op
+}  // namespace t8b

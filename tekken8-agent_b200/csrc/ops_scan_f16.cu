@@ -1,0 +1,12 @@
+// The selective scan in f16.
+#include "ops_scan.cuh"
+
+namespace t8b {
+namespace op {
+namespace scan {
+template void launch_forward<f16>(const Call&, const ForwardPlan&, int64_t, cudaStream_t);
+template void launch_backward<f16>(const Call&, const BackwardPlan&, float*, float*, float*, cudaStream_t);
+template void launch_step<f16>(const Call&, float*, bool, cudaStream_t);
+}  // namespace scan
+}  // namespace op
+}  // namespace t8b

@@ -382,3 +382,50 @@ PROTOTYPES.update({
     "t8b_operators_status": (C.c_int, [vp]),
     "t8b_debug_operators_stall": (C.c_int, [C.c_uint32, vp]),
 })
+
+
+# ------------------------------------------------------------------ memory operators
+class Track(C.Structure):
+    _fields_ = [("data", vp), ("sequence", i64), ("step", i64)]
+
+
+class Sequences(C.Structure):
+    _fields_ = [("sequences", i64), ("steps", i64), ("channels", i64), ("reset", vp), ("reset_sequence", i64),
+                ("reset_step", i64), ("lengths", vp)]
+
+
+class Scan(C.Structure):
+    _fields_ = [("type", C.c_int), ("softplus", C.c_int), ("groups", i64), ("states", i64), ("u", Track),
+                ("delta", Track), ("z", Track), ("b", Track), ("c", Track), ("b_group", i64), ("c_group", i64), ("a", vp),
+                ("d", vp), ("delta_bias", vp), ("state", vp)]
+
+
+class ScanGradients(C.Structure):
+    _fields_ = [(n, Track) for n in ("du", "ddelta", "dz", "db", "dc")] + [("db_group", i64), ("dc_group", i64)] + \
+               [(n, vp) for n in ("da", "dd", "ddelta_bias", "dstate")]
+
+
+class PolicyLoss(C.Structure):
+    _fields_ = [("type", C.c_int), ("mask_kind", C.c_int), ("reference_kind", C.c_int)] + \
+               [(n, C.c_float) for n in ("clip_low", "clip_high", "kl", "entropy")] + \
+               [("rows", i64), ("n", i64), ("logits", vp), ("logits_stride", i64), ("actions", vp),
+                ("old_log_probabilities", vp), ("advantages", vp), ("mask", vp), ("mask_stride", i64), ("reference", vp),
+                ("reference_stride", i64), ("weights", vp)]
+
+
+_SEQUENCES = C.POINTER(Sequences)
+PROTOTYPES.update({
+    "t8b_causal_conv_forward": (C.c_int, [_SEQUENCES, C.c_int, Track, vp, vp, C.c_int, C.c_int, C.c_int, vp, Track, vp,
+                                          vp]),
+    "t8b_causal_conv_workspace": (C.c_size_t, [_SEQUENCES, C.c_int]),
+    "t8b_causal_conv_backward": (C.c_int, [_SEQUENCES, C.c_int, Track, Track, vp, vp, C.c_int, C.c_int, C.c_int, vp, vp,
+                                           Track, vp, vp, vp, vp, C.c_size_t, vp]),
+    "t8b_causal_conv_step": (C.c_int, [_SEQUENCES, C.c_int, Track, vp, vp, C.c_int, C.c_int, C.c_int, vp, Track, vp]),
+    "t8b_selective_scan_saved": (C.c_size_t, [_SEQUENCES, i64, i64]),
+    "t8b_selective_scan_workspace": (C.c_size_t, [_SEQUENCES, i64, i64, C.c_int]),
+    "t8b_selective_scan_forward": (C.c_int, [_SEQUENCES, C.POINTER(Scan), Track, vp, vp, vp, C.c_size_t, vp]),
+    "t8b_selective_scan_backward": (C.c_int, [_SEQUENCES, C.POINTER(Scan), Track, vp, vp, C.POINTER(ScanGradients), vp,
+                                              C.c_size_t, vp]),
+    "t8b_selective_scan_step": (C.c_int, [_SEQUENCES, C.POINTER(Scan), vp, Track, vp]),
+    "t8b_policy_loss": (C.c_int, [C.POINTER(PolicyLoss), vp, vp, vp, vp, vp, i64, vp]),
+})

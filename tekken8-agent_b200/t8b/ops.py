@@ -1,6 +1,7 @@
 """Operators of a residual policy torso over the t8b_layer_norm_* / t8b_linear_* / t8b_gated_* entry
-points: layer norm, the linear map with bias, activation and residual, and the gated projection,
-each with its gradients.
+points (layer norm, the linear map with bias, activation and residual, and the gated projection) and
+of a policy with memory over t8b_causal_conv_* / t8b_selective_scan_* / t8b_policy_loss (the short causal
+convolution, the selective scan, the clipped policy loss), each with its gradients.
 
 Arguments are CUDA tensors whose last axis is contiguous; leading axes count as rows and need one
 stride between them (a column range of a wider buffer is fine). Matrix operands are bf16 or f16,
@@ -26,7 +27,10 @@ ACTIVATIONS = ("none", "relu", "gelu", "silu", "tanh")
 
 _operators.bind(T8bError, torch.OutOfMemoryError, *(C.cast(getattr(_lib.lib(), "t8b_" + name), C.c_void_p).value for name in (
     "last_error", "layer_norm_forward", "layer_norm_workspace", "layer_norm_backward", "linear_workspace",
-    "linear_forward", "linear_backward", "gated_workspace", "gated_forward", "gated_backward")))
+    "linear_forward", "linear_backward", "gated_workspace", "gated_forward", "gated_backward", "causal_conv_forward",
+    "causal_conv_workspace", "causal_conv_backward", "causal_conv_step", "selective_scan_saved",
+    "selective_scan_workspace", "selective_scan_forward", "selective_scan_backward", "selective_scan_step",
+    "policy_loss")))
 
 
 def _on(stream, x):
@@ -92,6 +96,108 @@ def gated_backward(dh, x, weight, bias=None, pre=None, activation: str = "silu",
         with _on(stream, x):
             return _operators.gated_backward(dh, x, weight, bias, pre, activation, input_gradient)
     return _operators.gated_backward(dh, x, weight, bias, pre, activation, input_gradient)
+
+
+# ---------------------------------------------------------------- a policy with memory
+# Sequences are tensors [sequences][steps][channels] in any order of the first two axes (a rollout's
+# [step][fight] data as data.transpose(0, 1)); outputs lie in x's order. `reset` [sequences][steps] (bool or
+# uint8) marks the steps at which a new round begins: nothing before such a step, the initial state included,
+# reaches it. `lengths` [sequences] (int32) ends sequences early: what lies past a sequence's length is not
+# read, outputs and gradients there are 0, and its final state is the one after its last step.
+
+
+def causal_conv(x, weight, bias=None, activation: str = "none", state=None, reset=None, lengths=None,
+                final: bool = False, stream=None):
+    """activation(bias + sum over j of weight[:, width - 1 - j] x[t - j]), one filter of 2 to 4 taps a channel
+    (weight [channels][width]; weight and bias fp32 or of x's type). `state` [sequences][width - 1][channels]
+    of x's type holds the inputs before the first step, oldest first (zeros by default); with `final` also
+    the last inputs, which are the next call's state."""
+    if stream is not None:
+        with _on(stream, x):
+            return _operators.causal_conv(x, weight, bias, activation, state, reset, lengths, final)
+    return _operators.causal_conv(x, weight, bias, activation, state, reset, lengths, final)
+
+
+def causal_conv_backward(dy, x, weight, bias=None, activation: str = "none", state=None, reset=None, lengths=None,
+                         dfinal=None, stream=None):
+    """(dx, dweight, dbias, dstate) of causal_conv from its output's gradient and, where it is given, the
+    final state's. dbias and dstate are None where bias and state are."""
+    if stream is not None:
+        with _on(stream, x):
+            return _operators.causal_conv_backward(dy, x, weight, bias, activation, state, reset, lengths, dfinal)
+    return _operators.causal_conv_backward(dy, x, weight, bias, activation, state, reset, lengths, dfinal)
+
+
+def causal_conv_step(x, weight, bias, state, activation: str = "none", reset=None, stream=None):
+    """One step of causal_conv for every sequence: x [sequences][channels], reset [sequences]. `state` is moved
+    on in place."""
+    if stream is not None:
+        with _on(stream, x):
+            return _operators.causal_conv_step(x, weight, bias, state, activation, reset)
+    return _operators.causal_conv_step(x, weight, bias, state, activation, reset)
+
+
+def selective_scan(u, delta, a, b, c, d=None, z=None, delta_bias=None, softplus: bool = True, state=None, reset=None,
+                   lengths=None, final: bool = False, save: bool = False, stream=None):
+    """The selective state space scan: with size = softplus(delta + delta_bias) (or without the softplus),
+    h = exp(size a) h + size u b and y = (sum over states of c h + d u) silu(z).
+
+    u, delta and z [sequences][steps][channels], b and c [sequences][steps][states] or [sequences][steps]
+    [groups][states] (a group serves channels / groups channels in a row), all of one type; a [channels]
+    [states] (up to 64), d and delta_bias [channels], and `state` [sequences][channels][states] (zeros by
+    default) fp32. Returns y, then with `final` the state after the last step, then with `save` what the
+    backward pass needs."""
+    if stream is not None:
+        with _on(stream, u):
+            return _operators.selective_scan(u, delta, a, b, c, d, z, delta_bias, softplus, state, reset, lengths, final,
+                                             save)
+    return _operators.selective_scan(u, delta, a, b, c, d, z, delta_bias, softplus, state, reset, lengths, final, save)
+
+
+def selective_scan_backward(dy, u, delta, a, b, c, saved, d=None, z=None, delta_bias=None, softplus: bool = True,
+                            state=None, reset=None, lengths=None, dfinal=None, stream=None):
+    """(du, ddelta, da, db, dc, dd, dz, ddelta_bias, dstate) of selective_scan from its output's gradient, what
+    its `save` gave and, where it is given, the final state's gradient; the other arguments as they were. dd,
+    dz, ddelta_bias and dstate are None where d, z, delta_bias and state are."""
+    if stream is not None:
+        with _on(stream, u):
+            return _operators.selective_scan_backward(dy, u, delta, a, b, c, saved, d, z, delta_bias, softplus, state,
+                                                      reset, lengths, dfinal)
+    return _operators.selective_scan_backward(dy, u, delta, a, b, c, saved, d, z, delta_bias, softplus, state, reset,
+                                              lengths, dfinal)
+
+
+def selective_scan_step(u, delta, a, b, c, state, d=None, z=None, delta_bias=None, softplus: bool = True, reset=None,
+                        stream=None):
+    """One step of selective_scan for every sequence: u, delta and z [sequences][channels], b and c
+    [sequences][states] or [sequences][groups][states], reset [sequences]. `state` is moved on in place."""
+    if stream is not None:
+        with _on(stream, u):
+            return _operators.selective_scan_step(u, delta, a, b, c, state, d, z, delta_bias, softplus, reset)
+    return _operators.selective_scan_step(u, delta, a, b, c, state, d, z, delta_bias, softplus, reset)
+
+
+def policy_loss(logits, actions, old_log_probabilities, advantages, mask=None, reference=None, weights=None,
+                clip: float = 0.2, clip_high=None, kl: float = 0.0, entropy: float = 0.0, gradient: bool = True,
+                stream=None):
+    """(loss, log_probabilities, entropies, divergences), fp32 values of each row, of the clipped policy loss
+    -min(r advantage, min(max(r, 1 - clip), 1 + clip_high) advantage) + kl divergence - entropy H with r =
+    exp(log_probability - old), and with `gradient` also dlogits, the gradient of the sum over rows of
+    weight loss (weights fp32; by default 1 / rows each, the mean).
+
+    logits [...][n] of any type; actions (int64), old_log_probabilities and advantages (fp32) one a row. mask:
+    which logits are legal, bool or uint8 [...][n], or int32 [...][ceil(n / 32)] with one bit each as the
+    simulator packs them. reference: a frozen policy's logits (of the logits' type and shape: the
+    divergence is the exact one over the legal actions) or its log-probabilities of the actions (fp32, one
+    a row: exp(e) - e - 1 with e = reference - log_probability). A row whose action is not a legal one (-1, say:
+    padding) gives 0 everywhere. clip_high is `clip` by default. The rows of dlogits start on 16 bytes: it is a
+    column range of a wider buffer where n does not do that by itself."""
+    if stream is not None:
+        with _on(stream, logits):
+            return _operators.policy_loss(logits, actions, old_log_probabilities, advantages, mask, reference, weights,
+                                          clip, clip_high, kl, entropy, gradient)
+    return _operators.policy_loss(logits, actions, old_log_probabilities, advantages, mask, reference, weights, clip,
+                                  clip_high, kl, entropy, gradient)
 
 
 def status(stream=None, device=None):
