@@ -14,8 +14,8 @@ namespace op {
 namespace {
 
 constexpr int kThreads = 128;
-constexpr int kRun = 32;       // steps of a thread's run
-constexpr int kAhead = 4;      // rows in flight
+constexpr int kRun = 32;   // steps of a thread's run
+constexpr int kAhead = 4;  // rows that are taken together, and that are in flight meanwhile
 constexpr int kSms = 148;
 constexpr int kPartialRows = 16;
 
@@ -32,63 +32,104 @@ struct Conv {
     int parameter_type, activation, runs, packs;
 };
 
+// V channels as (V + 1) / 2 pairs.
 template <int V, int K>
-__device__ __forceinline__ void load_filter(const Conv& a, int c, float (&w)[K][V], float (&b)[V]) {
+__device__ __forceinline__ void load_filter(const Conv& a, int c, Two (&w)[K][(V + 1) / 2], Two (&b)[(V + 1) / 2]) {
+    float f[K + 1][V + 1] = {};
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        b[v] = a.bias ? load_any(a.bias, a.parameter_type, c + v) : 0.0f;
+        f[K][v] = a.bias ? load_any(a.bias, a.parameter_type, c + v) : 0.0f;
 #pragma unroll
-        for (int k = 0; k < K; ++k) w[k][v] = load_any(a.weight, a.parameter_type, static_cast<size_t>(c + v) * K + k);
+        for (int k = 0; k < K; ++k) f[k][v] = load_any(a.weight, a.parameter_type, static_cast<size_t>(c + v) * K + k);
+    }
+#pragma unroll
+    for (int i = 0; i < (V + 1) / 2; ++i) {
+        b[i] = Two(f[K][2 * i], f[K][2 * i + 1]);
+#pragma unroll
+        for (int k = 0; k < K; ++k) w[k][i] = Two(f[k][2 * i], f[k][2 * i + 1]);
     }
 }
-template <int V, int N>
-__device__ __forceinline__ void clear(float (&v)[N][V]) {
+template <int H, int N>
+__device__ __forceinline__ void clear(Two (&v)[N][H]) {
 #pragma unroll
     for (int k = 0; k < N; ++k) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[k][i] = 0.0f;
+        for (int i = 0; i < H; ++i) v[k][i] = Two();
     }
 }
-template <int V, int N>
-__device__ __forceinline__ void shift(float (&window)[N][V], const float (&x)[V]) {
+template <int H, int N>
+__device__ __forceinline__ void shift(Two (&window)[N][H], const Two (&x)[H]) {
 #pragma unroll
     for (int k = 0; k + 1 < N; ++k) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) window[k][i] = window[k + 1][i];
+        for (int i = 0; i < H; ++i) window[k][i] = window[k + 1][i];
     }
 #pragma unroll
-    for (int i = 0; i < V; ++i) window[N - 1][i] = x[i];
+    for (int i = 0; i < H; ++i) window[N - 1][i] = x[i];
+}
+template <int ACT>
+__device__ __forceinline__ Two activate_two(const Two& v) {
+    const float2 f = v.get();
+    return Two(activate<ACT>(f.x), activate<ACT>(f.y));
+}
+template <int ACT>
+__device__ __forceinline__ Two slope_of(const Two& v) {
+    const float2 f = v.get();
+    float value, x, y;
+    activate_slope<ACT>(f.x, value, x);
+    activate_slope<ACT>(f.y, value, y);
+    return Two(x, y);
+}
+// A row of a track after the other: one pointer, where an index would make one of every unrolled row.
+template <typename T>
+struct Walk {
+    T* at;
+    int64_t step;
+    __device__ __forceinline__ Walk(T* base, int64_t step_, int t) : at(base + t * step_), step(step_) {}
+    __device__ __forceinline__ void next() { at += step; }
+};
+template <int H, int K>
+__device__ __forceinline__ void filter(const Two (&w)[K][H], const Two (&b)[H], const Two (&window)[K - 1][H], const Two (&row)[H], Two (&p)[H]) {
+#pragma unroll
+    for (int i = 0; i < H; ++i) {
+        p[i] = multiply_add(w[K - 1][i], row[i], b[i]);
+#pragma unroll
+        for (int k = 0; k < K - 1; ++k) p[i] = multiply_add(w[k][i], window[k][i], p[i]);
+    }
 }
 // The K - 1 rows before step t0, as step t0 may see them (a reset at t0 itself is the caller's), and
 // how many steps of its round they reach back, at most K.
 template <typename T, int V, int K>
-__device__ __forceinline__ int load_window(const Conv& a, const T* x, int64_t s, int c, int t0, float (&window)[K - 1][V]) {
+__device__ __forceinline__ int load_window(const Conv& a, const T* x, int64_t s, int c, int t0, Two (&window)[K - 1][(V + 1) / 2]) {
+    constexpr int H = (V + 1) / 2;
     const Sequences& q = a.q;
     int since = K;
-    clear<V, K - 1>(window);
+    clear<H, K - 1>(window);
+    Pack<T, V> raw[K - 1];
+#pragma unroll
+    for (int k = 0; k < K - 1; ++k) {
+        const int t = t0 - (K - 1) + k;
+#pragma unroll
+        for (int v = 0; v < V; ++v) raw[k].v[v] = Element<T>::store(0.0f);
+        if (t >= 0) {
+            raw[k] = load_pack<T, V>(x + t * a.x.step);
+        } else if (a.state) {
+            raw[k] = load_pack<T, V>(static_cast<const T*>(a.state) + (s * (K - 1) + (K - 1 + t)) * q.channels + c);
+        }
+    }
 #pragma unroll
     for (int k = 0; k < K - 1; ++k) {
         const int t = t0 - (K - 1) + k;
         if (t >= 0) {
+            ++since;
             if (q.resets(s, t)) {
-                clear<V, K - 1>(window);
+                clear<H, K - 1>(window);
                 since = 0;
-            } else {
-                ++since;
             }
-            float row[V];
-            unpack<T, V>(load_pack<T, V>(x + t * a.x.step), row);
-            shift<V, K - 1>(window, row);
-        } else {
-            float row[V];
-#pragma unroll
-            for (int i = 0; i < V; ++i) row[i] = 0.0f;
-            if (a.state) {
-                const T* at = static_cast<const T*>(a.state) + (s * (K - 1) + (K - 1 + t)) * q.channels + c;
-                unpack<T, V>(load_pack<T, V>(at), row);
-            }
-            shift<V, K - 1>(window, row);
         }
+        Two row[H];
+        unpack<T, V>(raw[k], row);
+        shift<H, K - 1>(window, row);
     }
     return since;
 }
@@ -96,6 +137,7 @@ __device__ __forceinline__ int load_window(const Conv& a, const T* x, int64_t s,
 // One thread: a pack of channels, a run of steps of a sequence.
 template <typename T, int V, int K>
 __global__ void __launch_bounds__(kThreads) k_conv_forward(Conv a) {
+    constexpr int H = (V + 1) / 2;
     wait_previous();
     release_next();
     const Sequences& q = a.q;
@@ -103,62 +145,64 @@ __global__ void __launch_bounds__(kThreads) k_conv_forward(Conv a) {
     const int64_t item = index / a.packs;
     const int c = static_cast<int>(index - item * a.packs) * V;
     if (item >= q.sequences * a.runs) return;
-    const int64_t s = item % q.sequences;
-    const int t0 = static_cast<int>(item / q.sequences) * kRun, t1 = min(q.steps, t0 + kRun), last = q.live(s), end = min(t1, last);
+    const int64_t run = item / q.sequences, s = item - run * q.sequences;
+    const int t0 = static_cast<int>(run) * kRun, t1 = min(q.steps, t0 + kRun), last = q.live(s), end = min(t1, last);
     const T* x = static_cast<const T*>(a.x.data) + s * a.x.sequence + c;
     T* y = static_cast<T*>(a.y.data) + s * a.y.sequence + c;
     T* final_state = a.final_state ? static_cast<T*>(a.final_state) + s * (K - 1) * q.channels + c : nullptr;
-    float window[K - 1][V];
-    auto keep = [&]() {
+    const bool none = t0 == 0 && last == 0;  // no step: the final state is the initial one
+    Two window[K - 1][H];
+    if (end > t0 || (none && final_state)) load_window<T, V, K>(a, x, s, c, t0, window);
+    if (end > t0) {
+        Two w[K][H], b[H];
+        load_filter<V, K>(a, c, w, b);
+        with_activation(a.activation, [&](auto act) {
+            Pack<T, V> next[kAhead];
+            bool flag[kAhead];
+            Walk<const T> from(x, a.x.step, t0);
+            Walk<const uint8_t> begins(q.reset ? q.reset + s * q.reset_sequence : nullptr, q.reset_step, t0);
+            Walk<T> to(y, a.y.step, t0);
+            auto fetch = [&](int t) {
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i) {
+                    flag[i] = false;
+                    if (t + i < end) {
+                        next[i] = load_pack<T, V>(from.at);
+                        if (q.reset) flag[i] = *begins.at != 0;
+                    }
+                    from.next();
+                    begins.next();
+                }
+            };
+            fetch(t0);
+            for (int t = t0; t < end; t += kAhead) {
+                Pack<T, V> now[kAhead];
+                bool cut[kAhead];
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i) {
+                    now[i] = next[i];
+                    cut[i] = flag[i];
+                }
+                fetch(t + kAhead);
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i) {
+                    if (t + i >= end) continue;
+                    Two row[H], p[H];
+                    unpack<T, V>(now[i], row);
+                    if (cut[i]) clear<H, K - 1>(window);
+                    filter<H, K>(w, b, window, row, p);
+#pragma unroll
+                    for (int h = 0; h < H; ++h) p[h] = activate_two<decltype(act)::value>(p[h]);
+                    *reinterpret_cast<Pack<T, V>*>(to.at) = pack<T, V>(p);
+                    to.next();
+                    shift<H, K - 1>(window, row);
+                }
+            }
+        });
+    }
+    if (final_state && (none || (end > t0 && end == last))) {
 #pragma unroll
         for (int k = 0; k < K - 1; ++k) *reinterpret_cast<Pack<T, V>*>(final_state + k * q.channels) = pack<T, V>(window[k]);
-    };
-    if (end > t0 || (t0 == 0 && last == 0 && final_state)) load_window<T, V, K>(a, x, s, c, t0, window);
-    if (t0 == 0 && last == 0 && final_state) keep();
-    if (end > t0) {
-        float w[K][V], b[V];
-        load_filter<V, K>(a, c, w, b);
-        Pack<T, V> next[kAhead];
-        bool flag[kAhead];
-        auto fetch = [&](int t) {
-#pragma unroll
-            for (int i = 0; i < kAhead; ++i) {
-                if (t + i < end) {
-                    next[i] = load_pack<T, V>(x + (t + i) * a.x.step);
-                    flag[i] = q.resets(s, t + i);
-                }
-            }
-        };
-        fetch(t0);
-        for (int t = t0; t < end; t += kAhead) {
-            float row[kAhead][V];
-            bool cut[kAhead];
-#pragma unroll
-            for (int i = 0; i < kAhead; ++i) {
-                unpack<T, V>(next[i], row[i]);
-                cut[i] = flag[i];
-            }
-            fetch(t + kAhead);
-#pragma unroll
-            for (int i = 0; i < kAhead; ++i) {
-                if (t + i >= end) break;
-                if (cut[i]) clear<V, K - 1>(window);
-                float p[V];
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    p[v] = fmaf(w[K - 1][v], row[i][v], b[v]);
-#pragma unroll
-                    for (int k = 0; k < K - 1; ++k) p[v] = fmaf(w[k][v], window[k][v], p[v]);
-                }
-                with_activation(a.activation, [&](auto act) {
-#pragma unroll
-                    for (int v = 0; v < V; ++v) p[v] = activate<decltype(act)::value>(p[v]);
-                });
-                *reinterpret_cast<Pack<T, V>*>(y + (t + i) * a.y.step) = pack<T, V>(p);
-                shift<V, K - 1>(window, row[i]);
-            }
-        }
-        if (end == last && final_state) keep();
     }
     Pack<T, V> zero;
 #pragma unroll
@@ -170,24 +214,25 @@ __global__ void __launch_bounds__(kThreads) k_conv_forward(Conv a) {
 // multiple of the launch's workers apart and keeps its channels' sums of dw and db. A run's dx takes
 // dp of the K - 1 steps behind it too, which are computed again.
 template <typename T, int V, int K>
-__global__ void __launch_bounds__(kThreads) k_conv_backward(Conv a) {
+__global__ void __launch_bounds__(kThreads, 3) k_conv_backward(Conv a) {
+    constexpr int H = (V + 1) / 2;
     wait_previous();
     release_next();
     const Sequences& q = a.q;
     const int column = blockIdx.x * blockDim.x + threadIdx.x;
     const int c = column * V;
     const bool mine = column < a.packs;
-    float dw[K][V], db[1][V];
-    clear<V, K>(dw);
-    clear<V, 1>(db);
+    Two dw[K][H], db[1][H];
+    clear<H, K>(dw);
+    clear<H, 1>(db);
     if (mine) {
-        float w[K][V], b[V];
+        Two w[K][H], b[H];
         load_filter<V, K>(a, c, w, b);
         const int64_t items = q.sequences * a.runs;
         for (int64_t item = static_cast<int64_t>(blockIdx.y) * blockDim.y + threadIdx.y; item < items;
              item += static_cast<int64_t>(gridDim.y) * blockDim.y) {
-            const int64_t s = item % q.sequences;
-            const int t0 = static_cast<int>(item / q.sequences) * kRun, t1 = min(q.steps, t0 + kRun), last = q.live(s);
+            const int64_t run = item / q.sequences, s = item - run * q.sequences;
+            const int t0 = static_cast<int>(run) * kRun, t1 = min(q.steps, t0 + kRun), last = q.live(s);
             const T* x = static_cast<const T*>(a.x.data) + s * a.x.sequence + c;
             const T* dy = static_cast<const T*>(a.dy.data) + s * a.dy.sequence + c;
             T* dx = static_cast<T*>(a.y.data) + s * a.y.sequence + c;
@@ -195,134 +240,138 @@ __global__ void __launch_bounds__(kThreads) k_conv_backward(Conv a) {
             const T* given = a.final_gradient ? static_cast<const T*>(a.final_gradient) + s * (K - 1) * q.channels + c : nullptr;
             // pending[j]: the gradient so far of the row j before the current one; the oldest is complete
             // once the current step has added to it
-            float pending[K][V], window[K - 1][V];
-            clear<V, K>(pending);
-            const int end = min(t1, last), far = min(t1 + K - 1, last);
-            auto write = [&](int row, const float(&v)[V]) {
-                if (row >= t0 && row < t1) {
-                    if (dx) *reinterpret_cast<Pack<T, V>*>(dx + row * a.y.step) = pack<T, V>(v);
-                } else if (row < 0 && t0 == 0 && dstate) {
-                    *reinterpret_cast<Pack<T, V>*>(dstate + (K - 1 + row) * q.channels) = pack<T, V>(v);
-                }
-            };
-            auto add_final = [&](int since) {  // after step last - 1: row last - 1 - j is entry K - 2 - j
-                if (!given) return;
-#pragma unroll
-                for (int j = 0; j < K - 1; ++j) {
-                    float v[V];
-                    unpack<T, V>(load_pack<T, V>(given + (K - 2 - j) * q.channels), v);
-#pragma unroll
-                    for (int i = 0; i < V; ++i) pending[j][i] += since >= j ? v[i] : 0.0f;
-                }
-            };
-            if (end > t0) {
+            Two pending[K][H], window[K - 1][H];
+            clear<H, K>(pending);
+            const int far = min(t1 + K - 1, last);
+            if (last > t0) {
                 int since = load_window<T, V, K>(a, x, s, c, t0, window);
-                Pack<T, V> next_x[kAhead], next_dy[kAhead];
-                bool flag[kAhead];
-                auto fetch = [&](int t) {
+                with_activation(a.activation, [&](auto act) {
+                    Pack<T, V> next_x[kAhead], next_dy[kAhead], none;
 #pragma unroll
-                    for (int i = 0; i < kAhead; ++i) {
-                        if (t + i < far) {
-                            next_x[i] = load_pack<T, V>(x + (t + i) * a.x.step);
-                            next_dy[i] = load_pack<T, V>(dy + (t + i) * a.dy.step);
-                            flag[i] = q.resets(s, t + i);
+                    for (int v = 0; v < V; ++v) none.v[v] = Element<T>::store(0.0f);
+                    bool flag[kAhead];
+                    Walk<const T> from_x(x, a.x.step, t0), from_dy(dy, a.dy.step, t0);
+                    Walk<const uint8_t> begins(q.reset ? q.reset + s * q.reset_sequence : nullptr, q.reset_step, t0);
+                    Walk<T> to(dx, a.y.step, t0 - (K - 1));
+                    auto fetch = [&](int t) {
+#pragma unroll
+                        for (int i = 0; i < kAhead; ++i) {
+                            flag[i] = false;
+                            next_x[i] = next_dy[i] = none;
+                            if (t + i < far) {
+                                next_x[i] = load_pack<T, V>(from_x.at);
+                                next_dy[i] = load_pack<T, V>(from_dy.at);
+                                if (q.reset) flag[i] = *begins.at != 0;
+                            }
+                            from_x.next();
+                            from_dy.next();
+                            begins.next();
                         }
-                    }
-                };
-                fetch(t0);
-                for (int t = t0; t < far; t += kAhead) {
-                    float row[kAhead][V], g[kAhead][V];
-                    bool cut[kAhead];
+                    };
+                    fetch(t0);
+                    for (int t = t0; t < t1 + K - 1; t += kAhead) {
+                        Pack<T, V> now_x[kAhead], now_dy[kAhead];
+                        bool cut[kAhead];
 #pragma unroll
-                    for (int i = 0; i < kAhead; ++i) {
-                        unpack<T, V>(next_x[i], row[i]);
-                        unpack<T, V>(next_dy[i], g[i]);
-                        cut[i] = flag[i];
-                    }
-                    fetch(t + kAhead);
+                        for (int i = 0; i < kAhead; ++i) {
+                            now_x[i] = next_x[i];
+                            now_dy[i] = next_dy[i];
+                            cut[i] = flag[i];
+                        }
+                        fetch(t + kAhead);
 #pragma unroll
-                    for (int i = 0; i < kAhead; ++i) {
-                        const int at = t + i;
-                        if (at >= far) break;
-                        if (cut[i]) {
-                            clear<V, K - 1>(window);
-                            since = 0;
-                        } else {
+                        for (int i = 0; i < kAhead; ++i) {
+                            const int at = t + i;
+                            Two row[H], p[H], pre[H];
+                            unpack<T, V>(now_x[i], row);
+                            unpack<T, V>(now_dy[i], p);
                             since = min(since + 1, K);
-                        }
-                        float p[V];
-#pragma unroll
-                        for (int v = 0; v < V; ++v) {
-                            p[v] = fmaf(w[K - 1][v], row[i][v], b[v]);
-#pragma unroll
-                            for (int k = 0; k < K - 1; ++k) p[v] = fmaf(w[k][v], window[k][v], p[v]);
-                        }
-                        with_activation(a.activation, [&](auto act) {
-#pragma unroll
-                            for (int v = 0; v < V; ++v) {
-                                float value, slope;
-                                activate_slope<decltype(act)::value>(p[v], value, slope);
-                                p[v] = g[i][v] * slope;
+                            if (cut[i]) {
+                                clear<H, K - 1>(window);
+                                since = 0;
                             }
-                        });
+                            filter<H, K>(w, b, window, row, pre);
 #pragma unroll
-                        for (int j = K - 1; j >= 1; --j) {
-#pragma unroll
-                            for (int v = 0; v < V; ++v) pending[j][v] = pending[j - 1][v] + (since >= j ? w[K - 1 - j][v] * p[v] : 0.0f);
-                        }
-#pragma unroll
-                        for (int v = 0; v < V; ++v) pending[0][v] = w[K - 1][v] * p[v];
-                        if (at < t1) {
-#pragma unroll
-                            for (int v = 0; v < V; ++v) {
-                                db[0][v] += p[v];
-                                dw[K - 1][v] = fmaf(p[v], row[i][v], dw[K - 1][v]);
-#pragma unroll
-                                for (int k = 0; k < K - 1; ++k) dw[k][v] = fmaf(p[v], window[k][v], dw[k][v]);
+                            for (int h = 0; h < H; ++h) {
+                                p[h] = p[h] * slope_of<decltype(act)::value>(pre[h]);
+                                if (at >= last) p[h] = Two();  // behind the sequence nothing is added any more
                             }
+#pragma unroll
+                            for (int j = K - 1; j >= 1; --j) {
+#pragma unroll
+                                for (int h = 0; h < H; ++h) {
+                                    pending[j][h] = multiply_add(w[K - 1 - j][h], since >= j ? p[h] : Two(), pending[j - 1][h]);
+                                }
+                            }
+#pragma unroll
+                            for (int h = 0; h < H; ++h) {
+                                pending[0][h] = w[K - 1][h] * p[h];
+                                const Two own = at < t1 ? p[h] : Two();
+                                db[0][h] = db[0][h] + own;
+                                dw[K - 1][h] = multiply_add(own, row[h], dw[K - 1][h]);
+#pragma unroll
+                                for (int k = 0; k < K - 1; ++k) dw[k][h] = multiply_add(own, window[k][h], dw[k][h]);
+                            }
+                            if (at == last - 1 && given) {  // the final state's entry K - 2 - j is row last - 1 - j
+#pragma unroll
+                                for (int j = 0; j < K - 1; ++j) {
+                                    if (since < j) continue;
+                                    Two v[H];
+                                    unpack<T, V>(load_pack<T, V>(given + (K - 2 - j) * q.channels), v);
+#pragma unroll
+                                    for (int h = 0; h < H; ++h) pending[j][h] = pending[j][h] + v[h];
+                                }
+                            }
+                            const int done = at - (K - 1);
+                            if (done >= t0 && done < t1) {
+                                if (a.y.data) *reinterpret_cast<Pack<T, V>*>(to.at) = pack<T, V>(pending[K - 1]);
+                            } else if (done < 0 && t0 == 0 && dstate) {
+                                *reinterpret_cast<Pack<T, V>*>(dstate + (K - 1 + done) * q.channels) = pack<T, V>(pending[K - 1]);
+                            }
+                            to.next();
+                            shift<H, K - 1>(window, row);
                         }
-                        if (at == last - 1) add_final(since);
-                        write(at - (K - 1), pending[K - 1]);
-                        shift<V, K - 1>(window, row[i]);
                     }
-                }
-                // what ends with the sequence (a later run writes its rows itself)
-                if (far == last) {
+                });
+                continue;
+            }
+            if (t0 == 0 && dstate) {  // no step: the final state is the initial one
 #pragma unroll
-                    for (int j = K - 2; j >= 0; --j) write(far - 1 - j, pending[j]);
-                }
-            } else if (t0 == 0 && dstate) {  // no step: the final state is the initial one
-                if (given) {
-#pragma unroll
-                    for (int k = 0; k < K - 1; ++k) *reinterpret_cast<Pack<T, V>*>(dstate + k * q.channels) = load_pack<T, V>(given + k * q.channels);
-                } else {
-#pragma unroll
-                    for (int k = 0; k < K - 1; ++k) *reinterpret_cast<Pack<T, V>*>(dstate + k * q.channels) = pack<T, V>(pending[k]);
+                for (int k = 0; k < K - 1; ++k) {
+                    *reinterpret_cast<Pack<T, V>*>(dstate + k * q.channels) = given ? load_pack<T, V>(given + k * q.channels) : pack<T, V>(pending[k]);
                 }
             }
-            float zero[1][V];
-            clear<V, 1>(zero);
-            for (int t = max(t0, end); t < t1; ++t) write(t, zero[0]);
+            if (a.y.data) {
+                const Two zero[H];
+                for (int t = t0; t < t1; ++t) *reinterpret_cast<Pack<T, V>*>(dx + t * a.y.step) = pack<T, V>(zero);
+            }
         }
     }
     if (a.partial == nullptr) return;
     // the block's rows of threads meet in shared memory, in their order
-    __shared__ float joined[kThreads][(K + 1) * V + 1];
-    float* slot = joined[threadIdx.y * blockDim.x + threadIdx.x];
+    constexpr int WIDTH = (K + 1) * 2 * H + 1;
+    __shared__ float joined[kThreads * WIDTH];
+    float* slot = joined + (threadIdx.y * blockDim.x + threadIdx.x) * WIDTH;
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
+    for (int h = 0; h < H; ++h) {
 #pragma unroll
-        for (int k = 0; k < K; ++k) slot[k * V + v] = dw[k][v];
-        slot[K * V + v] = db[0][v];
+        for (int k = 0; k <= K; ++k) {
+            const float2 f = k < K ? dw[k < K ? k : 0][h].get() : db[0][h].get();
+            slot[(k * H + h) * 2] = f.x;
+            slot[(k * H + h) * 2 + 1] = f.y;
+        }
     }
     __syncthreads();
     if (threadIdx.y != 0 || !mine) return;
     float* out = a.partial + static_cast<size_t>(blockIdx.y) * (K + 1) * q.channels + c;
 #pragma unroll
-    for (int i = 0; i < (K + 1) * V; ++i) {
-        float sum = slot[i];
-        for (int r = 1; r < blockDim.y; ++r) sum += slot[r * blockDim.x * ((K + 1) * V + 1) + i];
-        out[static_cast<size_t>(i / V) * q.channels + i % V] = sum;
+    for (int k = 0; k <= K; ++k) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            float sum = 0.0f;
+            for (int r = 0; r < blockDim.y; ++r) sum += slot[r * blockDim.x * WIDTH + k * 2 * H + v];
+            out[static_cast<size_t>(k) * q.channels + v] = sum;
+        }
     }
 }
 
@@ -367,7 +416,8 @@ __global__ void __launch_bounds__(kThreads) k_conv_step(Conv a) {
 #pragma unroll
     for (int k = 0; k < K - 1; ++k) held[k] = load_pack<T, V>(state + k * q.channels);
     const bool cut = q.reset != nullptr && q.reset[s * q.reset_sequence] != 0;
-    float w[K][V], p[V], row[V];
+    constexpr int H = (V + 1) / 2;
+    Two w[K][H], p[H], row[H];
     load_filter<V, K>(a, c, w, p);
     if (cut) {
 #pragma unroll
@@ -378,16 +428,16 @@ __global__ void __launch_bounds__(kThreads) k_conv_step(Conv a) {
     }
     unpack<T, V>(raw, row);
 #pragma unroll
-    for (int v = 0; v < V; ++v) p[v] = fmaf(w[K - 1][v], row[v], p[v]);
+    for (int h = 0; h < H; ++h) p[h] = multiply_add(w[K - 1][h], row[h], p[h]);
 #pragma unroll
     for (int k = 0; k < K - 1; ++k) {
         unpack<T, V>(held[k], row);
 #pragma unroll
-        for (int v = 0; v < V; ++v) p[v] = fmaf(w[k][v], row[v], p[v]);
+        for (int h = 0; h < H; ++h) p[h] = multiply_add(w[k][h], row[h], p[h]);
     }
     with_activation(a.activation, [&](auto act) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) p[v] = activate<decltype(act)::value>(p[v]);
+        for (int h = 0; h < H; ++h) p[h] = activate_two<decltype(act)::value>(p[h]);
     });
     *reinterpret_cast<Pack<T, V>*>(static_cast<T*>(a.y.data) + s * a.y.sequence + c) = pack<T, V>(p);
 #pragma unroll
@@ -418,10 +468,8 @@ struct Layout {
 };
 int64_t runs_of(int64_t steps) { return std::max<int64_t>(1, (steps + kRun - 1) / kRun); }
 
-// V consecutive channels a thread where every row and state starts on a pack's boundary.
-template <typename T>
-constexpr int forward_pack() { return sizeof(T) == 2 ? 8 : 4; }
-constexpr int kBackwardPack = 4;
+// Consecutive channels of a thread where every row and state starts on a pack's boundary.
+constexpr int kPack = 4;
 
 void check_call(const char* what, const t8b_sequences_t* q, bool step, int type, const void* weight, const void* bias, int parameter_type,
                 int width, int activation) {
@@ -471,7 +519,7 @@ extern "C" int t8b_causal_conv_forward(const t8b_sequences_t* q, int type, t8b_t
         a.runs = static_cast<int>(runs_of(q->steps));
         with_type(type, [&](auto element) {
             using T = decltype(element);
-            constexpr int V = forward_pack<T>();
+            constexpr int V = kPack;
             const bool wide = q->channels % V == 0 && rows_aligned(*q, false, x, size, V * size) && rows_aligned(*q, false, y, size, V * size) &&
                 aligned(state, V * size) && aligned(final_state, V * size);
             a.packs = static_cast<int>(wide ? q->channels / V : q->channels);
@@ -490,7 +538,7 @@ extern "C" int t8b_causal_conv_forward(const t8b_sequences_t* q, int type, t8b_t
 extern "C" size_t t8b_causal_conv_workspace(const t8b_sequences_t* q, int width) {
     if (q == nullptr || q->sequences < 1 || q->channels < 1 || q->steps < 0 || width < 2 || width > 4) return 0;
     const int64_t items = q->sequences * runs_of(q->steps);
-    const Layout wide(items, static_cast<int>((q->channels + kBackwardPack - 1) / kBackwardPack)), single(items, static_cast<int>(q->channels));
+    const Layout wide(items, static_cast<int>((q->channels + kPack - 1) / kPack)), single(items, static_cast<int>(q->channels));
     return sizeof(float) * static_cast<size_t>(std::max(wide.workers, single.workers)) * (width + 1) * q->channels;
 }
 
@@ -540,7 +588,7 @@ extern "C" int t8b_causal_conv_backward(const t8b_sequences_t* q, int type, t8b_
         a.runs = static_cast<int>(runs_of(q->steps));
         with_type(type, [&](auto element) {
             using T = decltype(element);
-            constexpr int V = kBackwardPack;
+            constexpr int V = kPack;
             bool wide = q->channels % V == 0;
             for (const t8b_track_t* t : {&dy, &x, &dx}) wide = wide && rows_aligned(*q, false, *t, size, V * size);
             for (const void* p : {state, final_gradient, static_cast<const void*>(dstate)}) wide = wide && aligned(p, V * size);
@@ -585,7 +633,7 @@ extern "C" int t8b_causal_conv_step(const t8b_sequences_t* q, int type, t8b_trac
         a.activation = activation;
         with_type(type, [&](auto element) {
             using T = decltype(element);
-            constexpr int V = forward_pack<T>();
+            constexpr int V = kPack;
             const bool wide = q->channels % V == 0 && rows_aligned(*q, true, x, size, V * size) && rows_aligned(*q, true, y, size, V * size) &&
                 aligned(state, V * size);
             a.packs = static_cast<int>(wide ? q->channels / V : q->channels);

@@ -2,14 +2,17 @@
 // policy, and its gradient in the same pass.
 //
 //   lp = z[a] - lse(z),  r = exp(lp - old),  loss = -min(r A, clip(r) A) + kl K - entropy H
-//   dloss/dz_i = p_i (c + kl (z_i - q_i) + entropy (z_i - m)) + [i = a] slope,
+//   dloss/dz_i = p_i (c + kl log(p_i / q_i) + entropy log p_i) + [i = a] slope,
 //   slope = dloss/dlp = -r A where the unclipped term is the smaller (0 where not) + the sampled K's 1 - exp(e)
 //
 // where c gathers what is the same for a whole row. Bound by memory: logits (and a reference's) once in,
 // the gradient once out. A row of up to 1,024 logits lies in the registers of one warp. A longer one belongs to a
 // block that reads it twice, for its sums and for its gradient; the second read comes from L2, where
-// the rows that are worked on at once fit many times over. Sums of exponentials are joined in 64 bits and the logarithm
-// is taken there: the ratio and the divergence are differences of it.
+// the rows that are worked on at once fit many times over.
+// With v = log2(e) z, M the fp32 rounding of its largest and t_i = v_i - M (one multiply-add): e_i = 2^t_i,
+// and every logarithm of a probability is ln 2 (t_i - log2(sum e)), with the same M in all of them, so that
+// its rounding cancels; lse itself is ln 2 (M + log2(sum e)), taken in 64 bits, since the ratio and
+// the divergence are differences of it.
 #include "ops_memory.cuh"
 
 namespace t8b {
@@ -51,37 +54,71 @@ __device__ __forceinline__ bool legal(const Loss& a, int64_t row, int64_t action
     return action >= 0 && action < a.n && (legal_bits<1>(a, row, static_cast<int>(action)) & 1) != 0;
 }
 
-// A row's sums: m the largest legal logit, total = sum e, spread = sum e (z - m), apart = sum e (z - q)
-// with e = exp(z - m); the same of the reference as far as it is needed.
+constexpr float kLn2 = 0.69314718055994531f;
+constexpr double kExactLn2 = 0.693147180559945309;
+constexpr float kNever = -1000.0f;  // 2^kNever is 0, and a factor of 0 beside it gives 0, not NaN
+
+// max that keeps a NaN
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+// ln(v), v from about 2^-100 to 2^100, to 2^-34: v = 2^k w with w in [3/4, 3/2), ln w = 2 atanh(q), q = (w - 1) /
+// (w + 1) in [-1/7, 1/5], by its series (the next term is 2 q^15 / 15). Others (0, NaN, inf) by log().
+__device__ __forceinline__ double natural_log(double v) {
+    const int high = __double2hiint(v);
+    if (static_cast<unsigned>(high - ((1023 - 100) << 20)) > 200u << 20) return log(v);
+    const int k = ((high + (1 << 19)) >> 20) - 1023;
+    const double w = __hiloint2double(high - (k << 20), __double2loint(v));
+    const double below = w + 1.0;
+    double r = static_cast<double>(reciprocal(static_cast<float>(below)));  // two steps of Newton's method: 2^-22, 2^-44
+    r = fma(r, fma(-below, r, 1.0), r);
+    const double q = (w - 1.0) * r, square = q * q;
+    double p = fma(square, 1.0 / 13.0, 1.0 / 11.0);
+    p = fma(square, p, 1.0 / 9.0);
+    p = fma(square, p, 1.0 / 7.0);
+    p = fma(square, p, 1.0 / 5.0);
+    p = fma(square, p, 1.0 / 3.0);
+    return fma(static_cast<double>(k), kExactLn2, 2.0 * fma(q * square, p, q));
+}
+
+// A row's sums: M as above, total = sum e, spread = sum e t, apart = sum e (t - t of the reference); the first
+// two of the reference as far as it is needed.
 struct Sums {
     float m = -INFINITY, q_m = -INFINITY;
     float spread = 0.0f, apart = 0.0f;
     double total = 0.0, q_total = 0.0;
 };
-// What a row's gradient needs beside its logits.
+// A row's gradient: e scale (base + of_t t + of_apart (t - t of the reference)) + [i = action] slope
 struct Slopes {
-    float scale, slope, base;  // weight / total; weight slope; c
+    float scale, slope, base, of_t, of_apart;
 };
 
 // The row's outputs from its sums; every thread that calls it gets the slopes, `writes` stores.
-__device__ __forceinline__ Slopes finish(const Loss& a, int64_t row, int64_t action, float chosen, const Sums& s, bool writes) {
-    const double log_total = log(s.total);
-    const double lp = static_cast<double>(chosen) - static_cast<double>(s.m) - log_total;
-    const float share = static_cast<float>(1.0 / s.total);
-    const float entropy = static_cast<float>(log_total - static_cast<double>(s.spread * share));
+__device__ __forceinline__ Slopes finish(const Loss& a, int64_t row, float chosen, const Sums& s, bool writes) {
+    const double log_total = natural_log(s.total);
+    const double lse = fma(static_cast<double>(s.m), kExactLn2, log_total);
+    const double lp = static_cast<double>(chosen) - lse;
+    const float share = 1.0f / static_cast<float>(s.total), log_sum = static_cast<float>(log_total);
+    const float entropy = static_cast<float>(log_total - static_cast<double>(kLn2 * (s.spread * share)));
     const float advantage = a.advantages[row];
     const float ratio = expf(static_cast<float>(lp - static_cast<double>(a.old[row])));
     const float free = ratio * advantage, held = fminf(fmaxf(ratio, a.low), a.high) * advantage;
-    float loss = -(free <= held || free != free ? free : held), slope = free <= held || free != free ? -free : 0.0f;
-    float divergence = 0.0f, shift = 0.0f;
+    const bool unclipped = free <= held || free != free;
+    float loss = -(unclipped ? free : held), slope = unclipped ? -free : 0.0f, divergence = 0.0f;
+    Slopes out;
+    out.base = a.entropy * (entropy - log_sum);
+    out.of_t = a.entropy * kLn2;
+    out.of_apart = 0.0f;
     if (a.reference_kind == T8B_REFERENCE_LOGITS) {
-        // log p_i - log q_i = (z_i - q_i) - shift
-        const double gap = (static_cast<double>(s.m) + log_total) - (static_cast<double>(s.q_m) + log(s.q_total));
-        shift = static_cast<float>(gap);
-        divergence = static_cast<float>(static_cast<double>(s.apart) * (1.0 / s.total) - gap);
+        // log p_i - log q_i = ln 2 (t_i - t of q_i) - gap
+        const double gap = log_total - natural_log(s.q_total);
+        divergence = static_cast<float>(static_cast<double>(kLn2 * (s.apart * share)) - gap);
+        out.base -= a.kl * (static_cast<float>(gap) + divergence);
+        out.of_apart = a.kl * kLn2;
     } else if (a.reference_kind == T8B_REFERENCE_SAMPLED) {
-        const double gap = static_cast<double>(static_cast<const float*>(a.reference)[row]) - lp;
-        const float e = static_cast<float>(gap);
+        const float e = static_cast<float>(static_cast<double>(static_cast<const float*>(a.reference)[row]) - lp);
         // exp(e) - 1 - e, by its series where the difference would cancel
         const float grown = expm1f(e);
         divergence = fabsf(e) < 0.1f
@@ -89,6 +126,7 @@ __device__ __forceinline__ Slopes finish(const Loss& a, int64_t row, int64_t act
             : grown - e;
         slope -= a.kl * grown;
     }
+    out.base -= slope;
     loss += a.kl * divergence - a.entropy * entropy;
     if (writes) {
         if (a.loss) a.loss[row] = loss;
@@ -97,11 +135,8 @@ __device__ __forceinline__ Slopes finish(const Loss& a, int64_t row, int64_t act
         if (a.divergences) a.divergences[row] = divergence;
     }
     const float weight = a.weights ? a.weights[row] : a.even;
-    Slopes out;
     out.scale = weight * share;
     out.slope = weight * slope;
-    out.base = -slope + a.entropy * (entropy - static_cast<float>(log_total));
-    if (a.reference_kind == T8B_REFERENCE_LOGITS) out.base -= a.kl * (shift + divergence);
     return out;
 }
 __device__ __forceinline__ void finish_nothing(const Loss& a, int64_t row) {
@@ -109,11 +144,23 @@ __device__ __forceinline__ void finish_nothing(const Loss& a, int64_t row) {
         if (p) p[row] = 0.0f;
     }
 }
+template <typename T, int V>
+__device__ __forceinline__ void store_pack(T* to, const float (&v)[V]) {
+    *reinterpret_cast<Pack<T, V>*>(to) = pack<T, V>(v);
+}
+template <int V>
+__device__ __forceinline__ void add_chosen(float (&v)[V], int64_t e, int64_t action, float slope) {
+    if (action < e || action >= e + V) return;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        if (e + j == action) v[j] += slope;
+    }
+}
 
-// One warp a row; lane l holds the packs l, l + 32, ... of V logits, up to HELD logits.
-template <typename T, int V, int HELD, bool REFERENCE>
+// One warp a row; lane l holds the packs l, l + 32, ... of V logits, PACKS of them.
+template <typename T, int V, int PACKS, bool REFERENCE>
 __global__ void __launch_bounds__(32 * kWarps) k_policy_loss(Loss a) {
-    constexpr int PACKS = HELD / V;
+    constexpr int HELD = V * PACKS;
     wait_previous();
     release_next();
     const int64_t row = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
@@ -139,13 +186,11 @@ __global__ void __launch_bounds__(32 * kWarps) k_policy_loss(Loss a) {
     if (!legal(a, row, action)) {
         if (lane == 0) finish_nothing(a, row);
         if (g == nullptr) return;
-        float zero[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) zero[i] = 0.0f;
+        const float zero[V] = {};
 #pragma unroll
         for (int i = 0; i < PACKS; ++i) {
             const int e = (i * 32 + lane) * V;
-            if (e < a.n) *reinterpret_cast<Pack<T, V>*>(g + e) = pack<T, V>(zero);
+            if (e < a.n) store_pack<T, V>(g + e, zero);
         }
         return;
     }
@@ -169,23 +214,22 @@ __global__ void __launch_bounds__(32 * kWarps) k_policy_loss(Loss a) {
         s.m = fmaxf(s.m, __shfl_xor_sync(0xffffffffu, s.m, o));
         if (REFERENCE) s.q_m = fmaxf(s.q_m, __shfl_xor_sync(0xffffffffu, s.q_m, o));
     }
-    // e into v, and what multiplies p beside the row's constant into w
-    float total = 0.0f, q_total = 0.0f, extra[HELD];
+    s.m *= kLog2E;
+    s.q_m *= kLog2E;
+    // t stays in v, t - t of the reference in w, e in p
+    float total = 0.0f, q_total = 0.0f, p[HELD];
 #pragma unroll
     for (int i = 0; i < HELD; ++i) {
-        const bool in = bits[i / V] >> (i % V) & 1;
-        const float off = v[i] - s.m, e = in ? exponential(off) : 0.0f;
-        const bool counts = e != 0.0f;  // a logit of -inf adds nothing
-        total += e;
-        s.spread += counts ? e * off : 0.0f;
-        extra[i] = a.entropy * off;
+        v[i] = max_nan(fmaf(v[i], kLog2E, -s.m), kNever);
+        p[i] = power_of_two(v[i]);
+        total += p[i];
+        s.spread = fmaf(p[i], v[i], s.spread);
         if (REFERENCE) {
-            const float away = v[i] - w[REFERENCE ? i : 0];
-            s.apart += counts ? e * away : 0.0f;
-            extra[i] = fmaf(a.kl, away, extra[i]);
-            q_total += in ? exponential(w[REFERENCE ? i : 0] - s.q_m) : 0.0f;
+            const float t = fmaf(w[REFERENCE ? i : 0], kLog2E, -s.q_m);
+            q_total += power_of_two(t);
+            w[REFERENCE ? i : 0] = p[i] != 0.0f ? v[i] - t : 0.0f;
+            s.apart = fmaf(p[i], w[REFERENCE ? i : 0], s.apart);
         }
-        v[i] = e;
     }
     s.total = total;
     s.q_total = q_total;
@@ -198,7 +242,7 @@ __global__ void __launch_bounds__(32 * kWarps) k_policy_loss(Loss a) {
             s.apart += __shfl_xor_sync(0xffffffffu, s.apart, o);
         }
     }
-    const Slopes k = finish(a, row, action, chosen, s, lane == 0);
+    const Slopes k = finish(a, row, chosen, s, lane == 0);
     if (g == nullptr) return;
 #pragma unroll
     for (int i = 0; i < PACKS; ++i) {
@@ -207,10 +251,13 @@ __global__ void __launch_bounds__(32 * kWarps) k_policy_loss(Loss a) {
         float out[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const float p = v[i * V + j] * k.scale;
-            out[j] = (v[i * V + j] != 0.0f ? p * (k.base + extra[i * V + j]) : 0.0f) + (e + j == action ? k.slope : 0.0f);
+            const int at = i * V + j;
+            float inner = fmaf(k.of_t, v[at], k.base);
+            if (REFERENCE) inner = fmaf(k.of_apart, w[REFERENCE ? at : 0], inner);
+            out[j] = p[at] * k.scale * inner;
         }
-        *reinterpret_cast<Pack<T, V>*>(g + e) = pack<T, V>(out);
+        add_chosen<V>(out, e, action, k.slope);
+        store_pack<T, V>(g + e, out);
     }
 }
 
@@ -231,46 +278,54 @@ __global__ void __launch_bounds__(kMostThreads) k_policy_loss_long(Loss a) {
     if (!legal(a, row, action)) {
         if (threadIdx.x == 0) finish_nothing(a, row);
         if (g == nullptr) return;
-        float zero[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) zero[i] = 0.0f;
-        for (int e = threadIdx.x * V; e < whole; e += step) *reinterpret_cast<Pack<T, V>*>(g + e) = pack<T, V>(zero);
+        const float zero[V] = {};
+        for (int e = threadIdx.x * V; e < whole; e += step) store_pack<T, V>(g + e, zero);
         for (int e = whole + threadIdx.x; e < a.n; e += blockDim.x) g[e] = Element<T>::store(0.0f);
         return;
     }
     const float chosen = Element<T>::load(z[action]);
     Sums s;
     float total = 0.0f, q_total = 0.0f;
-    // the sums so far, moved to a new largest logit
-    auto take = [&](const float (&v)[V], const float (&w)[V], uint32_t bits) {
-        float m = s.m, q_m = s.q_m;
+    // COUNT logits into the sums, which move to a new largest one first. While a thread has seen nothing but
+    // -inf its M is 0 here: every e is 0.
+    auto take = [&](auto count, const float (&v)[V], const float (&w)[V], uint32_t bits) {
+        constexpr int COUNT = decltype(count)::value;
+        float x[COUNT], y[COUNT], m = -INFINITY, q_m = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
+        for (int j = 0; j < COUNT; ++j) {
             const bool in = bits >> j & 1;
-            m = fmaxf(m, in ? v[j] : -INFINITY);
-            if (REFERENCE) q_m = fmaxf(q_m, in ? w[j] : -INFINITY);
+            x[j] = in ? v[j] : -INFINITY;
+            m = fmaxf(m, x[j]);
+            if (REFERENCE) {
+                y[j] = in ? w[j] : -INFINITY;
+                q_m = fmaxf(q_m, y[j]);
+            }
         }
+        m *= kLog2E;
+        q_m *= kLog2E;
         if (m > s.m) {
-            const float f = exponential(s.m - m);
-            s.spread = total != 0.0f ? f * fmaf(s.m - m, total, s.spread) : 0.0f;
+            const float gap = s.m - m, f = power_of_two(gap);
+            s.spread = total != 0.0f ? f * fmaf(gap, total, s.spread) : 0.0f;
+            s.apart = total != 0.0f ? f * fmaf(gap, total, s.apart) : 0.0f;
             total *= f;
-            s.apart *= f;
             s.m = m;
         }
         if (REFERENCE && q_m > s.q_m) {
-            q_total *= exponential(s.q_m - q_m);
+            const float gap = s.q_m - q_m;
+            s.apart = total != 0.0f ? fmaf(-gap, total, s.apart) : 0.0f;
+            q_total *= power_of_two(gap);
             s.q_m = q_m;
         }
+        const float from = s.m == -INFINITY ? 0.0f : s.m, q_from = s.q_m == -INFINITY ? 0.0f : s.q_m;
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const bool in = bits >> j & 1;  // -inf adds nothing, also while it is all that the thread has seen
-            const float off = v[j] - s.m, e = in && v[j] != -INFINITY ? exponential(off) : 0.0f;
-            const bool counts = e != 0.0f;
+        for (int j = 0; j < COUNT; ++j) {
+            const float t = max_nan(fmaf(x[j], kLog2E, -from), kNever), e = power_of_two(t);
             total += e;
-            s.spread += counts ? e * off : 0.0f;
+            s.spread = fmaf(e, t, s.spread);
             if (REFERENCE) {
-                s.apart += counts ? e * (v[j] - w[j]) : 0.0f;
-                q_total += in && w[j] != -INFINITY ? exponential(w[j] - s.q_m) : 0.0f;
+                const float u = fmaf(y[j], kLog2E, -q_from);
+                q_total += power_of_two(u);
+                s.apart = fmaf(e, e != 0.0f ? t - u : 0.0f, s.apart);
             }
         }
     };
@@ -279,13 +334,13 @@ __global__ void __launch_bounds__(kMostThreads) k_policy_loss_long(Loss a) {
         float v[V], w[V];
         unpack<T, V>(load_pack<T, V>(z + e), v);
         if (REFERENCE) unpack<T, V>(load_pack<T, V>(q + e), w);
-        take(v, w, legal_bits<V>(a, row, e));
+        take(Constant<V>{}, v, w, legal_bits<V>(a, row, e));
     }
     for (int e = whole + threadIdx.x; e < a.n; e += blockDim.x) {
         float v[V], w[V];
         v[0] = Element<T>::load(z[e]);
         w[0] = REFERENCE ? Element<T>::load(q[e]) : 0.0f;
-        take(v, w, legal_bits<1>(a, row, e));
+        take(Constant<1>{}, v, w, legal_bits<1>(a, row, e));
     }
     // the threads' sums, each moved to the row's largest logit
     float m = s.m, q_m = s.q_m;
@@ -304,12 +359,12 @@ __global__ void __launch_bounds__(kMostThreads) k_policy_loss_long(Loss a) {
         if (REFERENCE) q_m = fmaxf(q_m, most[1][i]);
     }
     if (total != 0.0f) {
-        const float f = exponential(s.m - m);
-        s.spread = f * fmaf(s.m - m, total, s.spread);
-        s.apart *= f;
+        const float gap = s.m - m, f = power_of_two(gap);
+        s.spread = f * fmaf(gap, total, s.spread);
+        if (REFERENCE) s.apart = f * fmaf(gap - (s.q_m == -INFINITY ? -q_m : s.q_m - q_m), total, s.apart);
         total *= f;
     }
-    if (q_total != 0.0f) q_total *= exponential(s.q_m - q_m);
+    if (REFERENCE && q_total != 0.0f) q_total *= power_of_two(s.q_m - q_m);
     s.m = m;
     s.q_m = q_m;
     s.total = total;
@@ -338,13 +393,13 @@ __global__ void __launch_bounds__(kMostThreads) k_policy_loss_long(Loss a) {
         s.spread += sums[0][i];
         s.apart += sums[1][i];
     }
-    const Slopes k = finish(a, row, action, chosen, s, threadIdx.x == 0);
+    const Slopes k = finish(a, row, chosen, s, threadIdx.x == 0);
     if (g == nullptr) return;
-    auto slope_of = [&](float v, float w, bool in, int e) {
-        const float off = v - s.m, p = in ? exponential(off) * k.scale : 0.0f;
-        float extra = a.entropy * off;
-        if (REFERENCE) extra = fmaf(a.kl, v - w, extra);
-        return (p != 0.0f ? p * (k.base + extra) : 0.0f) + (e == action ? k.slope : 0.0f);
+    auto slope_of = [&](float v, float w, bool in) {
+        const float t = max_nan(fmaf(in ? v : -INFINITY, kLog2E, -s.m), kNever), e = power_of_two(t);
+        float inner = fmaf(k.of_t, t, k.base);
+        if (REFERENCE) inner = fmaf(k.of_apart, e != 0.0f ? t - fmaf(w, kLog2E, -s.q_m) : 0.0f, inner);
+        return e * k.scale * inner;
     };
 #pragma unroll 2
     for (int e = threadIdx.x * V; e < whole; e += step) {
@@ -353,11 +408,13 @@ __global__ void __launch_bounds__(kMostThreads) k_policy_loss_long(Loss a) {
         if (REFERENCE) unpack<T, V>(load_pack<T, V>(q + e), w);
         const uint32_t bits = legal_bits<V>(a, row, e);
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = slope_of(v[j], REFERENCE ? w[j] : 0.0f, bits >> j & 1, e + j);
-        *reinterpret_cast<Pack<T, V>*>(g + e) = pack<T, V>(v);
+        for (int j = 0; j < V; ++j) v[j] = slope_of(v[j], REFERENCE ? w[j] : 0.0f, bits >> j & 1);
+        add_chosen<V>(v, e, action, k.slope);
+        store_pack<T, V>(g + e, v);
     }
     for (int e = whole + threadIdx.x; e < a.n; e += blockDim.x) {
-        g[e] = Element<T>::store(slope_of(Element<T>::load(z[e]), REFERENCE ? Element<T>::load(q[e]) : 0.0f, legal_bits<1>(a, row, e) & 1, e));
+        const float v = slope_of(Element<T>::load(z[e]), REFERENCE ? Element<T>::load(q[e]) : 0.0f, legal_bits<1>(a, row, e) & 1);
+        g[e] = Element<T>::store(v + (e == action ? k.slope : 0.0f));
     }
 }
 
@@ -365,8 +422,15 @@ __global__ void __launch_bounds__(kMostThreads) k_policy_loss_long(Loss a) {
 template <typename T, int V, bool REFERENCE>
 void launch_loss(const Loss& a, cudaStream_t stream) {
     if (a.n <= 32 * kMostHeld && a.n % V == 0) {
-        const int held = static_cast<int>((a.n + 32 * V - 1) / (32 * V)) * V;
-        auto kernel = held <= 8 ? k_policy_loss<T, V, 8, REFERENCE> : held <= 16 ? k_policy_loss<T, V, 16, REFERENCE> : k_policy_loss<T, V, 32, REFERENCE>;
+        // as many packs a lane as hold the row, rounded up to what is built
+        const int packs = static_cast<int>((a.n + 32 * V - 1) / (32 * V));
+        constexpr int MOST = kMostHeld / V;  // 32, 8 or 4
+        auto kernel = k_policy_loss<T, V, MOST, REFERENCE>;
+        if (packs <= 1) kernel = k_policy_loss<T, V, 1, REFERENCE>;
+        else if (packs <= 2) kernel = k_policy_loss<T, V, 2, REFERENCE>;
+        else if (packs <= 3) kernel = k_policy_loss<T, V, 3, REFERENCE>;
+        else if (packs <= 4) kernel = k_policy_loss<T, V, 4, REFERENCE>;
+        else if (V == 1 && packs <= 12) kernel = k_policy_loss<T, V, V == 1 ? 12 : MOST, REFERENCE>;
         launch_chain("k_policy_loss", kernel, blocks(a.rows, kWarps), 32 * kWarps, 0, stream, true, a);
         return;
     }

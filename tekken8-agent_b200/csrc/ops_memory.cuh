@@ -63,6 +63,34 @@ __device__ __forceinline__ Pack<T, V> pack(const float (&v)[V]) {
     return p;
 }
 
+// The same as register pairs; a single element has 0 beside it.
+template <typename T, int V>
+__device__ __forceinline__ void unpack(const Pack<T, V>& p, Two (&v)[(V + 1) / 2]) {
+    if constexpr (V == 1) {
+        v[0] = Two(Element<T>::load(p.v[0]), 0.0f);
+    } else if constexpr (sizeof(T) == 2) {
+        const Pack<uint32_t, V / 2> w = *reinterpret_cast<const Pack<uint32_t, V / 2>*>(&p);
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) {
+            const float2 f = Element<T>::unpack(w.v[i]);
+            v[i] = Two(f.x, f.y);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) v[i] = Two(p.v[2 * i], p.v[2 * i + 1]);
+    }
+}
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> pack(const Two (&v)[(V + 1) / 2]) {
+    float f[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const float2 w = v[i / 2].get();
+        f[i] = i % 2 ? w.y : w.x;
+    }
+    return pack<T, V>(f);
+}
+
 constexpr float kLn2 = 0.69314718055994531f;
 // exp(v), the argument's product with log2 e to twice the precision: good to 2^x's own 2^-22.
 __device__ __forceinline__ float exponential(float v) {
