@@ -29,6 +29,10 @@ constexpr int kThreads = 128;
 constexpr int kTile = 8;  // steps between two kept states, and of a tile
 constexpr int kSms = 148;
 constexpr int kMostStates = 64;
+constexpr int kForwardThreads = 64;  // of a block of the forward pass: few, since all wait for one another every tile
+constexpr int kHeld = 16;            // states of a channel that one of its threads holds
+// Of every kSeriesOf quads of states the last one's second pair takes 2^x by its series.
+constexpr int kSeriesOf = 2;
 
 struct Call {
     Sequences q;
@@ -46,39 +50,65 @@ struct Call {
     float* shared;   // [blocks of a group][groups][sequences][steps][2][states]: sums of dB and dC
     float* partial;  // [workers][states + 2][channels]: sums of da, dd and ddelta_bias
     int groups, per, states, softplus;  // per: channels of a group
+    int paired, saved_paired;           // whether two neighbouring channels may be accessed at once
     int chunks, chunk;                  // a chunk's steps, a multiple of kTile
     int group_blocks, workers;
 };
 
 // ------------------------------------------------------------------ arithmetic
-// log(1 + x) for 0 <= x <= 1: 2 atanh(w), w = x / (2 + x) <= 1/3, by its series (next term 2^-26)
-__device__ __forceinline__ float log_one_plus(float x) {
-    const float w = x * reciprocal(2.0f + x), q = w * w;
-    float p = fmaf(q, 1.0f / 15.0f, 1.0f / 13.0f);
-    p = fmaf(q, p, 1.0f / 11.0f);
-    p = fmaf(q, p, 1.0f / 9.0f);
-    p = fmaf(q, p, 1.0f / 7.0f);
-    p = fmaf(q, p, 1.0f / 5.0f);
-    p = fmaf(q, p, 1.0f / 3.0f);
-    return 2.0f * fmaf(w * q, p, w);
-}
-// softplus(v) = max(v, 0) + log(1 + exp(-|v|)), and its slope sigmoid(v)
-__device__ __forceinline__ float softplus(float v) {
-    const float x = exponential(-fabsf(v));
-    return (v > 0.0f ? v : 0.0f) + log_one_plus(x);
-}
-__device__ __forceinline__ float softplus(float v, float& slope) {
-    const float x = exponential(-fabsf(v));
-    const float r = reciprocal(1.0f + x);
-    slope = v > 0.0f ? r : x * r;
-    return (v > 0.0f ? v : 0.0f) + log_one_plus(x);
-}
 __device__ __forceinline__ Two both(float v) { return Two(v, v); }
+__device__ __forceinline__ Two two(float2 v) { return Two(v.x, v.y); }
 __device__ __forceinline__ Two powers_of_two(const Two& v) {
     const float2 f = v.get();
     return Two(power_of_two(f.x), power_of_two(f.y));
 }
-__device__ __forceinline__ Two two(float2 v) { return Two(v.x, v.y); }
+// The same without the 2^x unit, from the units of multiplications: 2^i p(d) with i the nearest integer to v (an
+// addition that rounds the fraction away, and leaves i in the low bits) and d = v - i in [-1/2, 1/2]. p is a
+// polynomial with p(0) = 1, fitted for the least relative error: 2^-23, with fp32's roundings 2^-22, as much as
+// the unit's. Arguments are taken into -126 ... 128: what is below counts as 2^-126, above as infinite; a NaN
+// is lost (a NaN size is in what is added to h, too; a NaN rate is the caller's to see to).
+__device__ __forceinline__ Two powers_by_series(const Two& v) {
+    const float2 f = v.get();
+    const Two x(fminf(fmaxf(f.x, -126.0f), 128.0f), fminf(fmaxf(f.y, -126.0f), 128.0f));
+    const Two shifted = x + both(12582912.0f);  // 1.5 2^23
+    const Two d = multiply_add(shifted + both(-12582912.0f), both(-1.0f), x);
+    Two p = multiply_add(both(1.3264727e-3f), d, both(9.6715126e-3f));
+    p = multiply_add(p, d, both(5.5507337e-2f));
+    p = multiply_add(p, d, both(0.24022242f));
+    p = multiply_add(p, d, both(0.69314698f));
+    p = multiply_add(p, d, both(1.0f));
+    const float2 i = shifted.get(), m = p.get();
+    return Two(__int_as_float(__float_as_int(m.x) + (__float_as_int(i.x) << 23)), __int_as_float(__float_as_int(m.y) + (__float_as_int(i.y) << 23)));
+}
+// log(1 + x), 0 <= x <= 1: x times a polynomial fitted for the least relative error, 2^-25
+__device__ __forceinline__ Two log_one_plus(const Two& x) {
+    Two p = multiply_add(both(5.2326915e-3f), x, both(-2.9505228e-2f));
+    p = multiply_add(p, x, both(7.8225934e-2f));
+    p = multiply_add(p, x, both(-0.13663244f));
+    p = multiply_add(p, x, both(0.19106006f));
+    p = multiply_add(p, x, both(-0.24842982f));
+    p = multiply_add(p, x, both(0.33319097f));
+    p = multiply_add(p, x, both(-0.49999493f));
+    p = multiply_add(p, x, both(0.99999997f));
+    return p * x;
+}
+// softplus(v) = max(v, 0) + log(1 + exp(-|v|)), and its slope sigmoid(v). The argument's product with log2 e
+// is taken to twice fp32's precision.
+__device__ __forceinline__ Two softplus(const Two& v, Two* slope = nullptr) {
+    const float2 f = v.get();
+    const Two away(-fabsf(f.x), -fabsf(f.y));
+    const Two high = away * both(kLog2E);
+    const Two low = multiply_add(away, both(-kLog2E), high) * both(-kLn2);
+    Two x = powers_of_two(high);
+    x = multiply_add(x, fabsf(f.x) < 100.0f && fabsf(f.y) < 100.0f ? low : Two(), x);
+    if (slope) {
+        const float2 e = x.get();
+        const float rx = reciprocal(1.0f + e.x), ry = reciprocal(1.0f + e.y);
+        *slope = Two(f.x > 0.0f ? rx : e.x * rx, f.y > 0.0f ? ry : e.y * ry);
+    }
+    return log_one_plus(x) + Two(f.x > 0.0f ? f.x : 0.0f, f.y > 0.0f ? f.y : 0.0f);
+}
+__device__ __forceinline__ float softplus(float v) { return softplus(both(v)).get().x; }
 
 // Which of a tile's steps are resets, one bit each: the same in every lane of a warp.
 __device__ __forceinline__ unsigned reset_bits(const Sequences& q, int64_t s, int t0, int end) {
@@ -102,174 +132,238 @@ struct Place {
         chunk = static_cast<int>(at - s * a.chunks);
     }
 };
+// Rows of a track one after the other, two channels of each: one pointer for all of an unrolled tile's rows.
+template <typename T>
+struct Pairs {
+    T* at;
+    int64_t step;
+    __device__ __forceinline__ Pairs(const Track<void>& track, int64_t s, int t, int c)
+        : at(static_cast<T*>(track.data) + s * track.sequence + t * track.step + c), step(track.step) {}
+    // into shared memory; both at once (and asynchronously) where every row's pair starts on a pair
+    __device__ __forceinline__ void load(Pack<T, 2>* to, bool paired, bool second) const {
+        if (paired) {
+            asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))), "l"(at),
+                         "n"(2 * sizeof(T)) : "memory");
+            return;
+        }
+        Pack<T, 2> p;
+        p.v[0] = at[0];
+        p.v[1] = second ? at[1] : Element<T>::store(0.0f);
+        *to = p;
+    }
+    __device__ __forceinline__ void store(const Two& v, bool paired, bool second) const {
+        const Pack<T, 2> p = pack<T, 2>({v});
+        if (paired) {
+            *reinterpret_cast<Pack<T, 2>*>(at) = p;
+        } else {
+            at[0] = p.v[0];
+            if (second) at[1] = p.v[1];
+        }
+    }
+    __device__ __forceinline__ void next() { at += step; }
+};
+template <typename T>
+__device__ __forceinline__ Two value(const Pack<T, 2>& p) {
+    Two v[1];
+    unpack<T, 2>(p, v);
+    return v[0];
+}
+__device__ __forceinline__ Two silu(const Two& v) {
+    const float2 f = v.get();
+    return Two(f.x * sigmoid(f.x), f.y * sigmoid(f.y));
+}
 
+// Two channels of a thread, kHeld states of each; LN lanes share a pair of channels.
 // ENDS: a chunk's end from a zero state, the sum of its D, and whether a reset cuts it, in place of y.
-template <typename T, int NS, int LN, bool ENDS>
-__global__ void __launch_bounds__(kThreads) k_scan_forward(Call a) {
-    constexpr int NP = NS * LN, CB = kThreads / LN;
+template <typename T, int LN, bool ENDS>
+__global__ void __launch_bounds__(kForwardThreads, 8) k_scan_forward(Call a) {
+    constexpr int NP = kHeld * LN, CB = kForwardThreads / LN * 2, H = kHeld / 2;
     wait_previous();
     release_next();
     __shared__ __align__(16) float bc[2][kTile][2][NP];
+    __shared__ Pack<T, 2> rows[2][3][kTile][kForwardThreads];  // u, delta and z of a tile: each thread writes and reads its own
     const Sequences& q = a.q;
     const Place place(a, blockIdx.x);
     const int64_t s = place.s;
-    const int lane = threadIdx.x % LN, local = place.part * CB + threadIdx.x / LN;
-    const bool mine = local < a.per;
+    const int lane = threadIdx.x % LN, local = place.part * CB + threadIdx.x / LN * 2;
+    const bool mine = local < a.per, second = local + 1 < a.per, paired = a.paired != 0;
     const int c = place.group * a.per + (mine ? local : 0);
     const int t0 = place.chunk * a.chunk, t1 = min(q.steps, t0 + a.chunk), last = q.live(s), end = min(t1, last);
-    const int n0 = lane * NS, channels = q.channels;
-    const T* u = static_cast<const T*>(a.u.data) + s * a.u.sequence + c;
-    const T* delta = static_cast<const T*>(a.delta.data) + s * a.delta.sequence + c;
-    const T* z = a.z.data && !ENDS ? static_cast<const T*>(a.z.data) + s * a.z.sequence + c : nullptr;
+    const int n0 = lane * kHeld, channels = q.channels;
+    const bool gate = !ENDS && a.z.data != nullptr;
+    Pairs<T> u(a.u, s, t0, c), delta(a.delta, s, t0, c), z(gate ? a.z : a.u, s, t0, c);
+    Pairs<T> y(a.y, s, t0, c);
     const T* b = static_cast<const T*>(a.b.data) + s * a.b.sequence + place.group * a.b_group;
     const T* cc = static_cast<const T*>(a.c.data) + s * a.c.sequence + place.group * a.c_group;
-    T* y = static_cast<T*>(a.y.data) + s * a.y.sequence + c;
     const int64_t at_chunk = s * a.chunks + place.chunk;
 
-    Two rate[NS / 2], h[NS / 2];  // a log2 e, and the states
+    Two rate[2][H], h[2][H];  // a log2 e, and the states, in pairs of states
 #pragma unroll
-    for (int i = 0; i < NS / 2; ++i) {
-        float2 r = make_float2(0.0f, 0.0f), v = r;
-        if (n0 + 2 * i < a.states) r.x = a.a[static_cast<int64_t>(c) * a.states + n0 + 2 * i] * kLog2E;
-        if (n0 + 2 * i + 1 < a.states) r.y = a.a[static_cast<int64_t>(c) * a.states + n0 + 2 * i + 1] * kLog2E;
-        if (!ENDS) {
-            if (a.chunks > 1) {
-                const float* from = a.carry + (at_chunk * a.states + n0 + 2 * i) * channels + c;
-                if (n0 + 2 * i < a.states) v.x = from[0];
-                if (n0 + 2 * i + 1 < a.states) v.y = from[channels];
-            } else if (a.state) {
-                const float* from = a.state + (s * channels + c) * a.states + n0 + 2 * i;
-                if (n0 + 2 * i < a.states) v.x = from[0];
-                if (n0 + 2 * i + 1 < a.states) v.y = from[1];
+    for (int k = 0; k < 2; ++k) {
+        const int ck = c + (k && second ? 1 : 0);
+#pragma unroll
+        for (int i = 0; i < H; ++i) {
+            float r[2] = {0.0f, 0.0f}, v[2] = {0.0f, 0.0f};
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int n = n0 + 2 * i + j;
+                if (n >= a.states) continue;
+                r[j] = a.a[static_cast<int64_t>(ck) * a.states + n] * kLog2E;
+                if (!ENDS && a.chunks > 1) {
+                    v[j] = a.carry[(at_chunk * a.states + n) * channels + ck];
+                } else if (!ENDS && a.state) {
+                    v[j] = a.state[(s * channels + ck) * a.states + n];
+                }
+                if (r[j] != r[j]) r[j] = INFINITY;  // powers_by_series loses a NaN: 2^inf times h = 0 is one
             }
+            rate[k][i] = Two(r[0], r[1]);
+            h[k][i] = Two(v[0], v[1]);
         }
-        rate[i] = two(r);
-        h[i] = two(v);
     }
-    const float skip = a.d ? a.d[c] : 0.0f, bias = a.delta_bias ? a.delta_bias[c] : 0.0f;
+    const int c1 = c + (second ? 1 : 0);
+    const Two skip = a.d ? Two(a.d[c], a.d[c1]) : Two(), bias = a.delta_bias ? Two(a.delta_bias[c], a.delta_bias[c1]) : Two();
 
-    constexpr int PER = (2 * kTile * NP + kThreads - 1) / kThreads;
-    T raw_u[kTile], raw_delta[kTile], raw_z[kTile], raw_bc[PER];
-    auto fetch = [&](int t) {
+    constexpr int PER = 2 * kTile * NP / kForwardThreads;
+    T raw_bc[PER];
+    auto fetch = [&](int t, int buffer) {
 #pragma unroll
         for (int i = 0; i < kTile; ++i) {
-            const bool live = mine && t + i < end;
-            raw_u[i] = live ? u[(t + i) * a.u.step] : Element<T>::store(0.0f);
-            raw_delta[i] = live ? delta[(t + i) * a.delta.step] : Element<T>::store(0.0f);
-            if (z) raw_z[i] = live ? z[(t + i) * a.z.step] : Element<T>::store(0.0f);
+            if (mine && t + i < end) {
+                u.load(&rows[buffer][0][i][threadIdx.x], paired, second);
+                delta.load(&rows[buffer][1][i][threadIdx.x], paired, second);
+                if (gate) z.load(&rows[buffer][2][i][threadIdx.x], paired, second);
+            }
+            u.next();
+            delta.next();
+            z.next();
         }
+        asm volatile("cp.async.commit_group;" ::: "memory");
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            const int e = i * kThreads + threadIdx.x, step = e / (2 * NP), which = e / NP % 2, n = e % NP;
+            const int e = i * kForwardThreads + threadIdx.x, step = e / (2 * NP), which = e / NP % 2, n = e % NP;
             raw_bc[i] = Element<T>::store(0.0f);
-            if (step < kTile && t + step < end && n < a.states) {
-                raw_bc[i] = which ? cc[(t + step) * a.c.step + n] : b[(t + step) * a.b.step + n];
-            }
+            if (t + step < end && n < a.states) raw_bc[i] = which ? cc[(t + step) * a.c.step + n] : b[(t + step) * a.b.step + n];
         }
     };
     auto stage = [&](int buffer) {
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const int e = i * kThreads + threadIdx.x;
-            if (e < 2 * kTile * NP) (&bc[buffer][0][0][0])[e] = Element<T>::load(raw_bc[i]);
-        }
+        for (int i = 0; i < PER; ++i) (&bc[buffer][0][0][0])[i * kForwardThreads + threadIdx.x] = Element<T>::load(raw_bc[i]);
     };
     int buffer = 0;
-    float total = 0.0f;
+    Two total;
     bool cut = false;
     if (t0 < end) {
-        fetch(t0);
+        fetch(t0, 0);
         stage(0);
         __syncthreads();
     }
     for (int t = t0; t < end; t += kTile, buffer ^= 1) {
-        float su[kTile], size[kTile], gate[kTile];
-#pragma unroll
-        for (int i = 0; i < kTile; ++i) {
-            su[i] = Element<T>::load(raw_u[i]);
-            const float v = Element<T>::load(raw_delta[i]) + bias;
-            size[i] = t + i < end ? (a.softplus ? softplus(v) : v) : 0.0f;  // past the end h stays
-            if (z) {
-                const float g = Element<T>::load(raw_z[i]);
-                gate[i] = g * sigmoid(g);
-            }
-        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
         const unsigned resets = reset_bits(q, s, t, end);
-        if (t + kTile < end) fetch(t + kTile);
+        if (t + kTile < end) fetch(t + kTile, buffer ^ 1);
         if (!ENDS && a.saved && mine) {
             float* to = a.saved + ((s * ((q.steps + kTile - 1) / kTile) + t / kTile) * a.states + n0) * channels + c;
 #pragma unroll
-            for (int i = 0; i < NS; ++i) {
-                const float2 v = h[i / 2].get();
-                if (n0 + i < a.states) to[static_cast<int64_t>(i) * channels] = i % 2 ? v.y : v.x;
+            for (int i = 0; i < kHeld; ++i) {
+                const float2 v0 = h[0][i / 2].get(), v1 = h[1][i / 2].get();
+                const float w0 = i % 2 ? v0.y : v0.x, w1 = i % 2 ? v1.y : v1.x;
+                if (n0 + i < a.states) {
+                    if (a.saved_paired) {
+                        *reinterpret_cast<float2*>(to) = make_float2(w0, w1);
+                    } else {
+                        to[0] = w0;
+                        if (second) to[1] = w1;
+                    }
+                }
+                to += channels;
             }
         }
-        auto step = [&](int i) {
-            const Two by = both(size[i]), in = both(size[i] * su[i]);
-            Two out;
+        const int count = min(kTile, end - t);
+#pragma unroll 2
+        for (int i = 0; i < count; ++i) {
+            if (resets >> i & 1) {
+                cut = true;
+                total = Two();
 #pragma unroll
-            for (int k = 0; k < NS / 4; ++k) {
-                const float4 vb = *reinterpret_cast<const float4*>(&bc[buffer][i][0][n0 + 4 * k]);
-                const Two e0 = powers_of_two(by * rate[2 * k]), e1 = powers_of_two(by * rate[2 * k + 1]);
-                h[2 * k] = multiply_add(e0, h[2 * k], in * Two(vb.x, vb.y));
-                h[2 * k + 1] = multiply_add(e1, h[2 * k + 1], in * Two(vb.z, vb.w));
-                if (!ENDS) {
-                    const float4 vc = *reinterpret_cast<const float4*>(&bc[buffer][i][1][n0 + 4 * k]);
-                    out = multiply_add(h[2 * k], Two(vc.x, vc.y), out);
-                    out = multiply_add(h[2 * k + 1], Two(vc.z, vc.w), out);
+                for (int k = 0; k < 2; ++k) {
+#pragma unroll
+                    for (int n = 0; n < H; ++n) h[k][n] = Two();
+                }
+            }
+            const Two in_u = value<T>(rows[buffer][0][i][threadIdx.x]);
+            Two size = value<T>(rows[buffer][1][i][threadIdx.x]) + bias;
+            if (a.softplus) size = softplus(size);
+            const float2 by = size.get(), in = (size * in_u).get();
+            Two out[2];
+#pragma unroll
+            for (int n = 0; n < kHeld / 4; ++n) {
+                const float4 vb = *reinterpret_cast<const float4*>(&bc[buffer][i][0][n0 + 4 * n]);
+                const float4 vc = ENDS ? vb : *reinterpret_cast<const float4*>(&bc[buffer][i][1][n0 + 4 * n]);
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const Two at = both(k ? by.y : by.x), add = both(k ? in.y : in.x);
+                    const Two x = at * rate[k][2 * n], w = at * rate[k][2 * n + 1];
+                    const Two e0 = powers_of_two(x), e1 = n % kSeriesOf == kSeriesOf - 1 ? powers_by_series(w) : powers_of_two(w);
+                    h[k][2 * n] = multiply_add(e0, h[k][2 * n], add * Two(vb.x, vb.y));
+                    h[k][2 * n + 1] = multiply_add(e1, h[k][2 * n + 1], add * Two(vb.z, vb.w));
+                    if (!ENDS) {
+                        out[k] = multiply_add(h[k][2 * n], Two(vc.x, vc.y), out[k]);
+                        out[k] = multiply_add(h[k][2 * n + 1], Two(vc.z, vc.w), out[k]);
+                    }
                 }
             }
             if (ENDS) {
-                total += size[i];
-                return;
+                total = total + size;
+                continue;
             }
-            float sum = out.sum();
+            float s0 = out[0].sum(), s1 = out[1].sum();
 #pragma unroll
-            for (int o = LN / 2; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            sum = fmaf(skip, su[i], sum);
-            if (z) sum *= gate[i];
-            if (mine && lane == 0 && t + i < end) y[(t + i) * a.y.step] = Element<T>::store(sum);
-        };
-        if (resets == 0) {
-#pragma unroll
-            for (int i = 0; i < kTile; ++i) step(i);
-        } else {
-            cut = true;
-#pragma unroll
-            for (int i = 0; i < kTile; ++i) {
-                if (resets >> i & 1) {
-                    if (ENDS) total = 0.0f;
-#pragma unroll
-                    for (int k = 0; k < NS / 2; ++k) h[k] = Two();
-                }
-                step(i);
+            for (int o = LN / 2; o >= 1; o >>= 1) {
+                s0 += __shfl_xor_sync(0xffffffffu, s0, o);
+                s1 += __shfl_xor_sync(0xffffffffu, s1, o);
             }
+            Two sum = multiply_add(skip, in_u, Two(s0, s1));
+            if (gate) sum = sum * silu(value<T>(rows[buffer][2][i][threadIdx.x]));
+            if (mine && lane == 0) y.store(sum, paired, second);
+            y.next();
         }
         if (t + kTile < end) stage(buffer ^ 1);
         __syncthreads();
     }
+    if (!mine) return;
     if (ENDS) {
-        if (!mine) return;
         float* to = a.carry + (at_chunk * a.states + n0) * channels + c;
 #pragma unroll
-        for (int i = 0; i < NS; ++i) {
-            const float2 v = h[i / 2].get();
-            if (n0 + i < a.states) to[static_cast<int64_t>(i) * channels] = i % 2 ? v.y : v.x;
+        for (int i = 0; i < kHeld; ++i) {
+            const float2 v0 = h[0][i / 2].get(), v1 = h[1][i / 2].get();
+            if (n0 + i < a.states) {
+                to[0] = i % 2 ? v0.y : v0.x;
+                if (second) to[1] = i % 2 ? v1.y : v1.x;
+            }
+            to += channels;
         }
-        if (lane == 0) a.sizes[at_chunk * channels + c] = total;
-        if (lane == 0 && local == 0 && place.group == 0) a.keep[at_chunk] = cut ? 0.0f : 1.0f;
+        if (lane == 0) {
+            const float2 v = total.get();
+            a.sizes[at_chunk * channels + c] = v.x;
+            if (second) a.sizes[at_chunk * channels + c + 1] = v.y;
+            if (local == 0 && place.group == 0) a.keep[at_chunk] = cut ? 0.0f : 1.0f;
+        }
         return;
     }
-    if (!mine) return;
     if (lane == 0) {
-        for (int t = max(t0, end); t < t1; ++t) y[t * a.y.step] = Element<T>::store(0.0f);
+        Pairs<T> rest(a.y, s, max(t0, end), c);
+        for (int t = max(t0, end); t < t1; ++t, rest.next()) rest.store(Two(), paired, second);
     }
     if (a.final_state && (last > t0 ? last <= t1 : last == 0 && t0 == 0)) {
-        float* to = a.final_state + (s * channels + c) * a.states + n0;
 #pragma unroll
-        for (int i = 0; i < NS; ++i) {
-            const float2 v = h[i / 2].get();
-            if (n0 + i < a.states) to[i] = i % 2 ? v.y : v.x;
+        for (int k = 0; k < 2; ++k) {
+            if (k && !second) continue;
+            float* to = a.final_state + (s * channels + c + k) * a.states + n0;
+#pragma unroll
+            for (int i = 0; i < kHeld; ++i) {
+                const float2 v = h[k][i / 2].get();
+                if (n0 + i < a.states) to[i] = i % 2 ? v.y : v.x;
+            }
         }
     }
 }
@@ -392,11 +486,11 @@ __global__ void __launch_bounds__(kThreads) k_scan_back_ends(Call a) {
 }
 
 // Shared memory of a block of the backward pass, for LN lanes along the states (4 each).
-template <int LN>
-struct BackwardShape {
+template <typename T, int LN>
+struct Backward {
     static constexpr int NP = 4 * LN, LC = 32 / LN;          // states; lanes along the channels
     static constexpr int CB = (kThreads / 32) * LC * 2;      // channels of a block
-    static constexpr int PT = kTile * CB / kThreads;         // steps whose elementwise part a thread has
+    static constexpr int EV = kTile * CB / kThreads;         // channels of a thread's elementwise part: 4, 2 or 1
     static constexpr int PARTS = LC * (kThreads / 32);       // pairs of channels, and partial sums of a state
     static constexpr int SPLIT = PARTS > 16 ? 2 : 1;         // threads that add up four states' partial sums
     // Where pair p's sums of lane `along` lie: rows are rotated, so that neither the threads that write
@@ -404,18 +498,27 @@ struct BackwardShape {
     __device__ __forceinline__ static int channel_at(int p, int along) { return (p + LC * along) % (CB / 2); }
     __device__ __forceinline__ static int state_at(int p, int along) { return (p + SPLIT * along) % PARTS; }
     struct Shared {
+        Pack<T, EV> rows[4][kThreads];                           // u, delta, dy and z of a tile: each thread writes and reads its own
+        float2 before[4][kThreads];                              // the states before it: the same
         float size[kTile][CB], in[kTile][CB], given[kTile][CB];  // D, D u, gs
-        float u[kTile][CB], slope[kTile][CB], zslope[kTile][CB];
+        float slope[kTile][CB], zslope[kTile][CB];
         float b[kTile][NP], c[kTile][NP];
-        float2 channel_sums[kTile][3][LN][CB / 2];       // sum_n: C h, B g, a e h g, of each lane along the states
-        float4 state_sums[kTile][2][LN][PARTS];          // sum_c: D u g, gs h, of each pair of channels
+        float2 channel_sums[kTile][3][LN][CB / 2];               // sum_n: C h, B g, a e h g, of each lane along the states
+        float4 state_sums[kTile][2][LN][PARTS];                  // sum_c: D u g, gs h, of each pair of channels
     };
 };
 
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* to, const void* from) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))), "l"(from), "n"(BYTES)
+                 : "memory");
+}
+
 template <typename T, int LN>
-__global__ void __launch_bounds__(kThreads, LN == 4 ? 3 : 2) k_scan_backward(Call a) {
-    using Shape = BackwardShape<LN>;
-    constexpr int NP = Shape::NP, LC = Shape::LC, CB = Shape::CB, PT = Shape::PT, PARTS = Shape::PARTS;
+__global__ void __launch_bounds__(kThreads, 3) k_scan_backward(Call a) {
+    using Shape = Backward<T, LN>;
+    constexpr int NP = Shape::NP, LC = Shape::LC, CB = Shape::CB, EV = Shape::EV, PARTS = Shape::PARTS;
+    constexpr int ROW = CB / EV;  // threads of a row of the elementwise part: kThreads / ROW = kTile
     wait_previous();
     release_next();
     extern __shared__ __align__(16) unsigned char memory[];
@@ -428,11 +531,10 @@ __global__ void __launch_bounds__(kThreads, LN == 4 ? 3 : 2) k_scan_backward(Cal
     const int pair = warp * LC + across, n0 = 4 * along;
     const int c0 = group * a.per + part * CB + 2 * pair;
     const bool has0 = part * CB + 2 * pair < a.per, has1 = part * CB + 2 * pair + 1 < a.per;
-    // and its elementwise part: channel ec, steps e0 to e0 + PT - 1 of a tile
-    const int el = threadIdx.x % CB, e0 = threadIdx.x / CB * PT;
-    const bool emine = part * CB + el < a.per;
-    const int ec = group * a.per + (emine ? part * CB + el : 0);
-    const float skip = a.d ? a.d[ec] : 0.0f, bias = a.delta_bias ? a.delta_bias[ec] : 0.0f;
+    // and its elementwise part: EV channels from ec on, step es of a tile
+    const int el = threadIdx.x % ROW * EV, es = threadIdx.x / ROW;
+    const int ecount = max(0, min(EV, a.per - part * CB - el));
+    const int ec = group * a.per + (ecount > 0 ? part * CB + el : 0);
 
     Two rate[4], da[4];
 #pragma unroll
@@ -444,37 +546,52 @@ __global__ void __launch_bounds__(kThreads, LN == 4 ? 3 : 2) k_scan_backward(Cal
         }
         rate[n] = two(r);
     }
-    float dd = 0.0f, dbias = 0.0f;
+    float dd[EV] = {}, dbias[EV] = {};
+    float* partial = a.partial + static_cast<int64_t>(blockIdx.y) * (a.states + 2) * channels;
+    // this worker's sums of da so far: kept apart from a few tiles' sums, which are added to them
+    auto flush = [&](bool first) {
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            const float2 v = da[n].get();
+            da[n] = Two();
+            float* to = partial + static_cast<int64_t>(n0 + n) * channels + c0;
+            if (n0 + n < a.states && has0) to[0] = first ? v.x : to[0] + v.x;
+            if (n0 + n < a.states && has1) to[1] = first ? v.y : to[1] + v.y;
+        }
+    };
+    bool first = true;
 
     constexpr int PER = (2 * kTile * NP + kThreads - 1) / kThreads;
-    T raw_u[PT], raw_delta[PT], raw_z[PT], raw_dy[PT], raw_bc[PER];
+    T raw_bc[PER];
     const bool gate = a.z.data != nullptr;
     const int64_t items = q.sequences * a.chunks;
     for (int64_t item = blockIdx.y; item < items; item += a.workers) {
         const int64_t s = item / a.chunks;
         const int chunk = static_cast<int>(item - s * a.chunks);
         const int t0 = chunk * a.chunk, t1 = min(q.steps, t0 + a.chunk), last = q.live(s), end = min(t1, last);
-        const T* u = static_cast<const T*>(a.u.data) + s * a.u.sequence + ec;
-        const T* delta = static_cast<const T*>(a.delta.data) + s * a.delta.sequence + ec;
-        const T* z = static_cast<const T*>(a.z.data) + s * a.z.sequence + ec;
-        const T* dy = static_cast<const T*>(a.dy.data) + s * a.dy.sequence + ec;
-        T* du = static_cast<T*>(a.du.data) + s * a.du.sequence + ec;
-        T* ddelta = static_cast<T*>(a.ddelta.data) + s * a.ddelta.sequence + ec;
-        T* dz = static_cast<T*>(a.dz.data) + s * a.dz.sequence + ec;
-        const T* b = static_cast<const T*>(a.b.data) + s * a.b.sequence + group * a.b_group;
-        const T* cc = static_cast<const T*>(a.c.data) + s * a.c.sequence + group * a.c_group;
+        auto row_of = [&](const Track<void>& track, int t) { return static_cast<const T*>(track.data) + s * track.sequence + t * track.step + ec; };
         auto fetch = [&](int t) {
+            const int at = t + es;
 #pragma unroll
-            for (int i = 0; i < PT; ++i) {
-                const int at = t + e0 + i;
-                raw_u[i] = raw_delta[i] = raw_z[i] = raw_dy[i] = Element<T>::store(0.0f);
-                if (emine && at < end) {
-                    raw_u[i] = u[at * a.u.step];
-                    raw_delta[i] = delta[at * a.delta.step];
-                    raw_dy[i] = dy[at * a.dy.step];
-                    if (gate) raw_z[i] = z[at * a.z.step];
+            for (int k = 0; k < 4; ++k) {
+                if (k == 3 && !gate) continue;
+                const Track<void>& track = k == 0 ? a.u : k == 1 ? a.delta : k == 2 ? a.dy : a.z;
+                Pack<T, EV>* to = &m.rows[k][threadIdx.x];
+                if (at < end && ecount == EV && a.paired) {
+                    const T* from = row_of(track, at);
+                    if constexpr (EV * sizeof(T) >= 4) {
+                        copy_async<EV * sizeof(T)>(to, from);
+                    } else {
+                        *to = load_pack<T, EV>(from);
+                    }
+                } else {
+                    const T* from = row_of(track, at < end ? at : 0);
+#pragma unroll
+                    for (int i = 0; i < EV; ++i) to->v[i] = at < end && i < ecount ? from[i] : Element<T>::store(0.0f);
                 }
             }
+            const T* b = static_cast<const T*>(a.b.data) + s * a.b.sequence + group * a.b_group;
+            const T* cc = static_cast<const T*>(a.c.data) + s * a.c.sequence + group * a.c_group;
 #pragma unroll
             for (int i = 0; i < PER; ++i) {
                 const int e = i * kThreads + threadIdx.x, step = e / (2 * NP), which = e / NP % 2, n = e % NP;
@@ -483,6 +600,23 @@ __global__ void __launch_bounds__(kThreads, LN == 4 ? 3 : 2) k_scan_backward(Cal
                     raw_bc[i] = which ? cc[(t + step) * a.c.step + n] : b[(t + step) * a.b.step + n];
                 }
             }
+        };
+        auto fetch_before = [&](int t) {
+            const float* from = a.saved + ((s * tiles + t / kTile) * a.states + n0) * channels + c0;
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                float2* to = &m.before[n][threadIdx.x];
+                if (n0 + n < a.states && has1 && a.saved_paired) {
+                    copy_async<8>(to, from);
+                } else {
+                    float2 v = make_float2(0.0f, 0.0f);
+                    if (n0 + n < a.states && has0) v.x = from[0];
+                    if (n0 + n < a.states && has1) v.y = from[1];
+                    *to = v;
+                }
+                from += channels;
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
         };
         // the gradient of the state after the chunk
         Two g[4];
@@ -502,29 +636,56 @@ __global__ void __launch_bounds__(kThreads, LN == 4 ? 3 : 2) k_scan_backward(Cal
             }
             g[n] = two(v);
         }
-        int t = t0 + (end - 1 - t0) / kTile * kTile;
-        if (end > t0) fetch(t);
+        int t = t0 + (end - 1 - t0) / kTile * kTile, since = 0;
+        if (end > t0) {
+            fetch(t);
+            fetch_before(t);
+        }
         for (; end > t0 && t >= t0; t -= kTile) {
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
             // ---- elementwise: D, D u and gs of the tile into shared memory
+            const Pack<T, EV> raw_u = m.rows[0][threadIdx.x];
+            {
+                const bool live = t + es < end;
+                const Pack<T, EV> raw_delta = m.rows[1][threadIdx.x], raw_dy = m.rows[2][threadIdx.x];
+                const Pack<T, EV> raw_z = gate ? m.rows[3][threadIdx.x] : raw_u;
+                float size[EV], in[EV], given[EV], slope[EV], zslope[EV];
 #pragma unroll
-            for (int i = 0; i < PT; ++i) {
-                const bool live = emine && t + e0 + i < end;
-                const float vu = Element<T>::load(raw_u[i]), v = Element<T>::load(raw_delta[i]) + bias, vdy = Element<T>::load(raw_dy[i]);
-                float slope = 1.0f, size = v, given = vdy, zslope = 0.0f;
-                if (a.softplus) size = softplus(v, slope);
-                if (gate) {
-                    const float w = Element<T>::load(raw_z[i]);
-                    float value;
-                    activate_slope<T8B_SILU>(w, value, zslope);
-                    given = vdy * value;
-                    zslope *= vdy;
+                for (int i = 0; i < EV; i += 2) {
+                    constexpr int D = EV > 1 ? 1 : 0;
+                    const int j = i + D;
+                    const Two v = Two(Element<T>::load(raw_delta.v[i]), Element<T>::load(raw_delta.v[j])) +
+                        (a.delta_bias ? Two(a.delta_bias[ec + min(i, max(ecount - 1, 0))], a.delta_bias[ec + min(j, max(ecount - 1, 0))]) : Two());
+                    Two of_v = both(1.0f), of_size = v;
+                    if (a.softplus) of_size = softplus(v, &of_v);
+                    const Two of_in = of_size * Two(Element<T>::load(raw_u.v[i]), Element<T>::load(raw_u.v[j]));
+                    const float2 f = of_size.get(), k = of_v.get(), w = of_in.get();
+                    size[i] = f.x;
+                    slope[i] = k.x;
+                    in[i] = w.x;
+                    if (D) {
+                        size[j] = f.y;
+                        slope[j] = k.y;
+                        in[j] = w.y;
+                    }
                 }
-                m.size[e0 + i][el] = live ? size : 0.0f;
-                m.in[e0 + i][el] = live ? size * vu : 0.0f;
-                m.given[e0 + i][el] = live ? given : 0.0f;
-                m.u[e0 + i][el] = vu;
-                m.slope[e0 + i][el] = slope;
-                m.zslope[e0 + i][el] = zslope;
+#pragma unroll
+                for (int i = 0; i < EV; ++i) {
+                    given[i] = Element<T>::load(raw_dy.v[i]);
+                    zslope[i] = 0.0f;
+                    if (gate) {
+                        float value;
+                        activate_slope<T8B_SILU>(Element<T>::load(raw_z.v[i]), value, zslope[i]);
+                        zslope[i] *= given[i];
+                        given[i] *= value;
+                    }
+                    if (!live || i >= ecount) size[i] = in[i] = given[i] = 0.0f;
+                }
+                *reinterpret_cast<Pack<float, EV>*>(&m.size[es][el]) = pack<float, EV>(size);
+                *reinterpret_cast<Pack<float, EV>*>(&m.in[es][el]) = pack<float, EV>(in);
+                *reinterpret_cast<Pack<float, EV>*>(&m.given[es][el]) = pack<float, EV>(given);
+                *reinterpret_cast<Pack<float, EV>*>(&m.slope[es][el]) = pack<float, EV>(slope);
+                *reinterpret_cast<Pack<float, EV>*>(&m.zslope[es][el]) = pack<float, EV>(zslope);
             }
 #pragma unroll
             for (int i = 0; i < PER; ++i) {
@@ -532,24 +693,10 @@ __global__ void __launch_bounds__(kThreads, LN == 4 ? 3 : 2) k_scan_backward(Cal
                 if (step < kTile) (which ? m.c : m.b)[step][n] = Element<T>::load(raw_bc[i]);
             }
             const unsigned resets = reset_bits(q, s, t, end);
-            Two before[4];
-            {
-                const float* from = a.saved + ((s * tiles + t / kTile) * a.states + n0) * channels + c0;
-#pragma unroll
-                for (int n = 0; n < 4; ++n) {
-                    float2 v = make_float2(0.0f, 0.0f);
-                    if (n0 + n < a.states) {
-                        if (has0) v.x = from[static_cast<int64_t>(n) * channels];
-                        if (has1) v.y = from[static_cast<int64_t>(n) * channels + 1];
-                    }
-                    before[n] = two(v);
-                }
-            }
             __syncthreads();
             if (t > t0) fetch(t - kTile);
             // ---- h through the tile, then g back
-            auto pass = [&](auto cuts) {
-                constexpr bool CUTS = decltype(cuts)::value != 0;
+            {
                 Two h[kTile][4];
 #pragma unroll
                 for (int i = 0; i < kTile; ++i) {
@@ -557,11 +704,13 @@ __global__ void __launch_bounds__(kThreads, LN == 4 ? 3 : 2) k_scan_backward(Cal
                     const Two in = two(*reinterpret_cast<const float2*>(&m.in[i][2 * pair]));
                     const float4 vb = *reinterpret_cast<const float4*>(&m.b[i][n0]);
                     const float bn[4] = {vb.x, vb.y, vb.z, vb.w};
-                    const bool reset = CUTS && (resets >> i & 1);
+                    const bool on = (resets >> i & 1) == 0;
 #pragma unroll
                     for (int n = 0; n < 4; ++n) {
-                        const Two from = reset ? Two() : i ? h[i ? i - 1 : 0][n] : before[n];
-                        h[i][n] = multiply_add(powers_of_two(by * rate[n]), from, in * both(bn[n]));
+                        h[i][n] = in * both(bn[n]);
+                        const Two from = i ? h[i ? i - 1 : 0][n] : two(m.before[n][threadIdx.x]);
+                        const Two e = powers_of_two(by * rate[n]);
+                        if (on) h[i][n] = multiply_add(e, from, h[i][n]);
                     }
                 }
 #pragma unroll
@@ -571,59 +720,80 @@ __global__ void __launch_bounds__(kThreads, LN == 4 ? 3 : 2) k_scan_backward(Cal
                     const Two given = two(*reinterpret_cast<const float2*>(&m.given[i][2 * pair]));
                     const float4 vb = *reinterpret_cast<const float4*>(&m.b[i][n0]), vc = *reinterpret_cast<const float4*>(&m.c[i][n0]);
                     const float bn[4] = {vb.x, vb.y, vb.z, vb.w}, cn[4] = {vc.x, vc.y, vc.z, vc.w};
-                    const bool reset = CUTS && (resets >> i & 1);
+                    const bool on = (resets >> i & 1) == 0;
                     Two of_h, of_b, of_a;
-                    float4 db, dc;
-                    float* to_b = &db.x;
-                    float* to_c = &dc.x;
+                    float db[4], dc[4];
 #pragma unroll
                     for (int n = 0; n < 4; ++n) {
                         g[n] = multiply_add(given, both(cn[n]), g[n]);
                         of_h = multiply_add(h[i][n], both(cn[n]), of_h);
                         of_b = multiply_add(g[n], both(bn[n]), of_b);
-                        to_b[n] = (in * g[n]).sum();
-                        to_c[n] = (given * h[i][n]).sum();
-                        g[n] = reset ? Two() : g[n] * powers_of_two(by * rate[n]);
-                        const Two from = reset ? Two() : i ? h[i ? i - 1 : 0][n] : before[n];
+                        db[n] = (in * g[n]).sum();
+                        dc[n] = (given * h[i][n]).sum();
+                        g[n] = g[n] * powers_of_two(by * rate[n]);
+                        if (!on) g[n] = Two();
+                        const Two from = i ? h[i ? i - 1 : 0][n] : two(m.before[n][threadIdx.x]);
                         const Two through = g[n] * from;
-                        of_a = multiply_add(through, rate[n], of_a);
-                        da[n] = multiply_add(through, by, da[n]);
+                        if (on) of_a = multiply_add(through, rate[n], of_a);
+                        if (on) da[n] = multiply_add(through, by, da[n]);
                     }
                     m.channel_sums[i][0][along][Shape::channel_at(pair, along)] = of_h.get();
                     m.channel_sums[i][1][along][Shape::channel_at(pair, along)] = of_b.get();
                     m.channel_sums[i][2][along][Shape::channel_at(pair, along)] = of_a.get();
-                    m.state_sums[i][0][along][Shape::state_at(pair, along)] = db;
-                    m.state_sums[i][1][along][Shape::state_at(pair, along)] = dc;
+                    m.state_sums[i][0][along][Shape::state_at(pair, along)] = make_float4(db[0], db[1], db[2], db[3]);
+                    m.state_sums[i][1][along][Shape::state_at(pair, along)] = make_float4(dc[0], dc[1], dc[2], dc[3]);
                 }
-            };
-            if (resets == 0) {
-                pass(Constant<0>{});
-            } else {
-                pass(Constant<1>{});
+            }
+            if (t > t0) fetch_before(t - kTile);
+            if (++since == 16 || t == t0) {
+                flush(first);
+                first = false;
+                since = 0;
             }
             __syncthreads();
             // ---- the sums over states, and the gradients of u, delta and z
-#pragma unroll
-            for (int i = 0; i < PT; ++i) {
-                const int at = t + e0 + i;
-                float sum[3];
+            {
+                const int at = t + es;
+                float sum[3][EV] = {};
 #pragma unroll
                 for (int k = 0; k < 3; ++k) {
-                    sum[k] = 0.0f;
 #pragma unroll
                     for (int l = 0; l < LN; ++l) {
-                        sum[k] += reinterpret_cast<const float*>(m.channel_sums[e0 + i][k][l])[2 * Shape::channel_at(el / 2, l) + el % 2];
+                        const float* from = reinterpret_cast<const float*>(m.channel_sums[es][k][l]) + 2 * Shape::channel_at(el / 2, l) + (EV == 1 ? el % 2 : 0);
+                        const Pack<float, EV> v = load_pack<float, EV>(from);
+#pragma unroll
+                        for (int i = 0; i < EV; ++i) sum[k][i] += v.v[i];
                     }
                 }
-                const float size = m.size[e0 + i][el], given = m.given[e0 + i][el], vu = m.u[e0 + i][el];
-                if (emine && at < t1) {
+                if (ecount > 0 && at < t1) {
                     const bool live = at < end;
-                    const float to_size = live ? (vu * sum[1] + kLn2 * sum[2]) * m.slope[e0 + i][el] : 0.0f;
-                    du[at * a.du.step] = Element<T>::store(live ? fmaf(skip, given, size * sum[1]) : 0.0f);
-                    ddelta[at * a.ddelta.step] = Element<T>::store(to_size);
-                    if (a.dz.data) dz[at * a.dz.step] = Element<T>::store(live ? m.zslope[e0 + i][el] * fmaf(skip, vu, sum[0]) : 0.0f);
-                    dbias += to_size;
-                    if (live) dd = fmaf(given, vu, dd);
+                    const Pack<float, EV> size = load_pack<float, EV>(&m.size[es][el]), given = load_pack<float, EV>(&m.given[es][el]);
+                    const Pack<float, EV> slope = load_pack<float, EV>(&m.slope[es][el]), zslope = load_pack<float, EV>(&m.zslope[es][el]);
+                    float du[EV], ddelta[EV], dz[EV];
+#pragma unroll
+                    for (int i = 0; i < EV; ++i) {
+                        const float vu = Element<T>::load(raw_u.v[i]), skip = a.d && i < ecount ? a.d[ec + i] : 0.0f;
+                        du[i] = live ? fmaf(skip, given.v[i], size.v[i] * sum[1][i]) : 0.0f;
+                        ddelta[i] = live ? fmaf(kLn2, sum[2][i], vu * sum[1][i]) * slope.v[i] : 0.0f;
+                        dz[i] = live ? zslope.v[i] * fmaf(skip, vu, sum[0][i]) : 0.0f;
+                        dbias[i] += ddelta[i];
+                        if (live) dd[i] = fmaf(given.v[i], vu, dd[i]);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 3; ++k) {
+                        if (k == 2 && !a.dz.data) continue;
+                        const Track<void>& track = k == 0 ? a.du : k == 1 ? a.ddelta : a.dz;
+                        T* to = const_cast<T*>(row_of(track, at));
+                        const Pack<T, EV> v = pack<T, EV>(k == 0 ? du : k == 1 ? ddelta : dz);
+                        if (ecount == EV && a.paired) {
+                            *reinterpret_cast<Pack<T, EV>*>(to) = v;
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < EV; ++i) {
+                                if (i < ecount) to[i] = v.v[i];
+                            }
+                        }
+                    }
                 }
             }
             // ---- the sums over channels
@@ -644,22 +814,26 @@ __global__ void __launch_bounds__(kThreads, LN == 4 ? 3 : 2) k_scan_backward(Cal
                     vy.x += __shfl_xor_sync(0xffffffffu, vy.x, 1);
                     vy.y += __shfl_xor_sync(0xffffffffu, vy.y, 1);
                 }
-                if (half != 0 || t + step >= end) continue;
+                if (half != 0 || t + step >= end || 4 * l >= a.states) continue;
                 const float sum[4] = {vx.x, vx.y, vy.x, vy.y};
                 float* to = a.shared +
                     ((((static_cast<int64_t>(part) * a.groups + group) * q.sequences + s) * q.steps + t + step) * 2 + which) * a.states + 4 * l;
+                if (a.states % 4 == 0) {  // the workspace starts on 256 bytes
+                    *reinterpret_cast<float4*>(to) = make_float4(sum[0], sum[1], sum[2], sum[3]);
+                } else {
 #pragma unroll
-                for (int n = 0; n < 4; ++n) {
-                    if (4 * l + n < a.states) to[n] = sum[n];
+                    for (int n = 0; n < 4; ++n) {
+                        if (4 * l + n < a.states) to[n] = sum[n];
+                    }
                 }
             }
         }
         // past the sequence's end
-        if (emine) {
-            for (int at = max(t0, t0 + (end > t0 ? (end - t0 + kTile - 1) / kTile * kTile : 0)) + threadIdx.x / CB; at < t1; at += kThreads / CB) {
-                du[at * a.du.step] = Element<T>::store(0.0f);
-                ddelta[at * a.ddelta.step] = Element<T>::store(0.0f);
-                if (a.dz.data) dz[at * a.dz.step] = Element<T>::store(0.0f);
+        for (int at = t0 + (end > t0 ? (end - t0 + kTile - 1) / kTile * kTile : 0) + es; at < t1; at += kTile) {
+            for (int k = 0; k < 3; ++k) {
+                if (k == 2 && !a.dz.data) continue;
+                T* to = const_cast<T*>(row_of(k == 0 ? a.du : k == 1 ? a.ddelta : a.dz, at));
+                for (int i = 0; i < ecount; ++i) to[i] = Element<T>::store(0.0f);
             }
         }
         if (chunk == 0 && a.dstate) {
@@ -673,25 +847,25 @@ __global__ void __launch_bounds__(kThreads, LN == 4 ? 3 : 2) k_scan_backward(Cal
         }
         __syncthreads();  // the next item's tile writes what this one's last still reads
     }
-    // this worker's sums of the parameters' gradients
-    float* out = a.partial + static_cast<int64_t>(blockIdx.y) * (a.states + 2) * channels;
+    if (first) flush(true);  // no step at all: zeros
+    // the rows of threads, one step of a tile each, in their order
 #pragma unroll
-    for (int n = 0; n < 4; ++n) {
-        const float2 v = da[n].get();
-        if (n0 + n < a.states && has0) out[static_cast<int64_t>(n0 + n) * channels + c0] = v.x;
-        if (n0 + n < a.states && has1) out[static_cast<int64_t>(n0 + n) * channels + c0 + 1] = v.y;
+    for (int i = 0; i < EV; ++i) {
+        m.size[es][el + i] = dd[i];
+        m.in[es][el + i] = dbias[i];
     }
-    m.size[e0 / PT][el] = dd;  // one row of threads, PT steps each, a row of the tile
-    m.in[e0 / PT][el] = dbias;
     __syncthreads();
-    if (threadIdx.x < CB && emine) {
-        dd = dbias = 0.0f;
-        for (int r = 0; r < kTile / PT; ++r) {
-            dd += m.size[r][el];
-            dbias += m.in[r][el];
+    for (int i = threadIdx.x; i < CB; i += kThreads) {
+        if (part * CB + i >= a.per) continue;
+        float of_d = 0.0f, of_bias = 0.0f;
+#pragma unroll
+        for (int r = 0; r < kTile; ++r) {
+            of_d += m.size[r][i];
+            of_bias += m.in[r][i];
         }
-        out[static_cast<int64_t>(a.states) * channels + ec] = dd;
-        out[static_cast<int64_t>(a.states + 1) * channels + ec] = dbias;
+        const int c = group * a.per + part * CB + i;
+        partial[static_cast<int64_t>(a.states) * channels + c] = of_d;
+        partial[static_cast<int64_t>(a.states + 1) * channels + c] = of_bias;
     }
 }
 
@@ -831,12 +1005,12 @@ struct ForwardPlan {
     int channels, group_blocks, chunks, chunk;
     int64_t blocks;
     ForwardPlan(const t8b_sequences_t& q, int64_t groups, int64_t states) {
-        channels = kThreads * 16 / padded(states);
+        channels = kForwardThreads * 2 * kHeld / padded(states);
         group_blocks = static_cast<int>((q.channels / groups + channels - 1) / channels);
         const int64_t per_chunk = q.sequences * groups * group_blocks, steps = std::max<int64_t>(q.steps, 1);
         // cut where fewer than two blocks an SM would run; cutting takes every exponential twice
         int64_t want = 1;
-        if (per_chunk < 2 * kSms) want = std::max<int64_t>(1, std::min<int64_t>(5 * kSms / std::max<int64_t>(per_chunk, 1), steps / 32));
+        if (per_chunk < 4 * kSms) want = std::max<int64_t>(1, std::min<int64_t>(8 * kSms / std::max<int64_t>(per_chunk, 1), steps / 32));
         if (want < 3) want = 1;
         chunk = static_cast<int>(round_up((steps + want - 1) / want, kTile));
         chunks = static_cast<int>((steps + chunk - 1) / chunk);
@@ -879,21 +1053,21 @@ void launch_forward(const Call& given, const ForwardPlan& plan, int64_t states, 
     auto go = [&](auto main, auto ends) {
         const unsigned grid = static_cast<unsigned>(plan.blocks);
         if (a.chunks > 1) {
-            launch_chain("k_scan_ends", ends, grid, kThreads, 0, stream, true, a);
+            launch_chain("k_scan_ends", ends, grid, kForwardThreads, 0, stream, true, a);
             launch_chain("k_scan_join", k_scan_join, blocks(a.q.sequences * states * a.q.channels, 256), 256, 0, stream, true, a, false);
         }
-        launch_chain("k_scan_forward", main, grid, kThreads, 0, stream, true, a);
+        launch_chain("k_scan_forward", main, grid, kForwardThreads, 0, stream, true, a);
     };
     switch (padded(states)) {
-        case 16: go(k_scan_forward<T, 16, 1, false>, k_scan_forward<T, 16, 1, true>); break;
-        case 32: go(k_scan_forward<T, 16, 2, false>, k_scan_forward<T, 16, 2, true>); break;
-        default: go(k_scan_forward<T, 16, 4, false>, k_scan_forward<T, 16, 4, true>); break;
+        case 16: go(k_scan_forward<T, 1, false>, k_scan_forward<T, 1, true>); break;
+        case 32: go(k_scan_forward<T, 2, false>, k_scan_forward<T, 2, true>); break;
+        default: go(k_scan_forward<T, 4, false>, k_scan_forward<T, 4, true>); break;
     }
 }
 
 template <typename T, int LN>
 void launch_backward_tiles(const Call& a, cudaStream_t stream) {
-    constexpr size_t bytes = sizeof(typename BackwardShape<LN>::Shared);
+    constexpr size_t bytes = sizeof(typename Backward<T, LN>::Shared);
     static uint64_t configured = 0;
     allow_smem(k_scan_backward<T, LN>, bytes, configured);
     launch_chain("k_scan_backward", k_scan_backward<T, LN>, dim3(a.groups * a.group_blocks, a.workers), kThreads, bytes, stream, true, a);
