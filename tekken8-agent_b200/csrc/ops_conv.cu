@@ -6,7 +6,9 @@
 // where a term whose two steps lie on different sides of a reset is left out. Bound by memory: x (and
 // dy) once in, y (or dx) once out. A thread takes V consecutive channels of a run of steps and keeps
 // the last K - 1 rows in registers, so a row is read once but for the K - 1 rows around a run, which
-// neighbouring threads hold in L1 or L2; the rows of the next turn are in flight while one is worked on.
+// neighbouring threads hold in L1 or L2. Rows come through a ring in shared memory that a thread fills
+// (cp.async) and reads alone: two groups of rows are in flight while one is worked on, and no thread waits for
+// another.
 #include "ops_memory.cuh"
 
 namespace t8b {
@@ -15,7 +17,7 @@ namespace {
 
 constexpr int kThreads = 128;
 constexpr int kRun = 32;   // steps of a thread's run
-constexpr int kAhead = 4;  // rows that are taken together, and that are in flight meanwhile
+constexpr int kGroup = 4;  // rows that are taken together
 constexpr int kSms = 148;
 constexpr int kPartialRows = 16;
 
@@ -30,6 +32,7 @@ struct Conv {
     void* dstate;
     float* partial;  // [workers][width + 1][channels]: sums of dw and db
     int parameter_type, activation, runs, packs;
+    int lanes;  // neighbouring threads of one run: a power of two, at most a warp
 };
 
 // V channels as (V + 1) / 2 pairs.
@@ -80,14 +83,45 @@ __device__ __forceinline__ Two slope_of(const Two& v) {
     activate_slope<ACT>(f.y, value, y);
     return Two(x, y);
 }
-// A row of a track after the other: one pointer, where an index would make one of every unrolled row.
-template <typename T>
-struct Walk {
-    T* at;
+// The rows of a run one after the other, V elements of each, through this thread's slots of the ring: two
+// groups of kGroup rows, `kThreads` packs apart. Rows at and past `end` are zeros.
+template <typename T, int V>
+struct Ring {
+    Pack<T, V>* slots;
+    const T* from;  // the next row to fetch
     int64_t step;
-    __device__ __forceinline__ Walk(T* base, int64_t step_, int t) : at(base + t * step_), step(step_) {}
-    __device__ __forceinline__ void next() { at += step; }
+    int next, end;
+    __device__ __forceinline__ Ring(Pack<T, V>* slots_, const T* base, int64_t step_, int t0, int end_)
+        : slots(slots_), from(base + t0 * step_), step(step_), next(t0), end(end_) {}
+    __device__ __forceinline__ void fetch(int half) {
+#pragma unroll
+        for (int i = 0; i < kGroup; ++i, ++next, from += step) {
+            Pack<T, V>* to = slots + (half * kGroup + i) * kThreads;
+            if (next >= end) {
+#pragma unroll
+                for (int v = 0; v < V; ++v) to->v[v] = Element<T>::store(0.0f);
+            } else if constexpr (V * sizeof(T) >= 4) {
+                copy_async<V * sizeof(T)>(to, from);
+            } else {
+                *to = load_pack<T, V>(from);
+            }
+        }
+    }
+    __device__ __forceinline__ void take(int half, Pack<T, V> (&rows)[kGroup]) const {
+#pragma unroll
+        for (int i = 0; i < kGroup; ++i) rows[i] = slots[(half * kGroup + i) * kThreads];
+    }
 };
+// Which of the 32 steps from t0 on (those before `end`) are resets, a bit each: `lanes` threads find them together.
+__device__ __forceinline__ uint32_t resets_of(const Sequences& q, int64_t s, int t0, int end, int lanes) {
+    if (q.reset == nullptr) return 0;
+    uint32_t bits = 0;
+    for (int i = threadIdx.x & (lanes - 1); i < 32; i += lanes) {
+        if (t0 + i < end && q.resets(s, t0 + i)) bits |= 1u << i;
+    }
+    for (int o = lanes / 2; o >= 1; o >>= 1) bits |= __shfl_xor_sync(0xffffffffu, bits, o);
+    return bits;
+}
 template <int H, int K>
 __device__ __forceinline__ void filter(const Two (&w)[K][H], const Two (&b)[H], const Two (&window)[K - 1][H], const Two (&row)[H], Two (&p)[H]) {
 #pragma unroll
@@ -138,67 +172,68 @@ __device__ __forceinline__ int load_window(const Conv& a, const T* x, int64_t s,
 template <typename T, int V, int K>
 __global__ void __launch_bounds__(kThreads) k_conv_forward(Conv a) {
     constexpr int H = (V + 1) / 2;
+    __shared__ Pack<T, V> ring[2 * kGroup][kThreads];
     wait_previous();
     release_next();
     const Sequences& q = a.q;
     const int64_t index = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-    const int64_t item = index / a.packs;
-    const int c = static_cast<int>(index - item * a.packs) * V;
-    if (item >= q.sequences * a.runs) return;
-    const int64_t run = item / q.sequences, s = item - run * q.sequences;
+    const int across = (a.packs + a.lanes - 1) / a.lanes * a.lanes;
+    const int64_t item = index / across;
+    const int column = static_cast<int>(index - item * across), c = column * V;
+    const bool inside = item < q.sequences * a.runs;
+    const int64_t run = inside ? item / q.sequences : 0, s = inside ? item - run * q.sequences : 0;
     const int t0 = static_cast<int>(run) * kRun, t1 = min(q.steps, t0 + kRun), last = q.live(s), end = min(t1, last);
+    const uint32_t resets = resets_of(q, s, t0, end, a.lanes);
+    if (!inside || column >= a.packs) return;
     const T* x = static_cast<const T*>(a.x.data) + s * a.x.sequence + c;
-    T* y = static_cast<T*>(a.y.data) + s * a.y.sequence + c;
+    T* y = static_cast<T*>(a.y.data) + s * a.y.sequence + c + t0 * a.y.step;
     T* final_state = a.final_state ? static_cast<T*>(a.final_state) + s * (K - 1) * q.channels + c : nullptr;
     const bool none = t0 == 0 && last == 0;  // no step: the final state is the initial one
     Two window[K - 1][H];
-    if (end > t0 || (none && final_state)) load_window<T, V, K>(a, x, s, c, t0, window);
+    int t = t0;
     if (end > t0) {
+        Ring<T, V> rows(&ring[0][threadIdx.x], x, a.x.step, t0, end);
+        rows.fetch(0);
+        copies_commit();
+        rows.fetch(1);
+        copies_commit();
+        load_window<T, V, K>(a, x, s, c, t0, window);
         Two w[K][H], b[H];
         load_filter<V, K>(a, c, w, b);
         with_activation(a.activation, [&](auto act) {
-            Pack<T, V> next[kAhead];
-            bool flag[kAhead];
-            Walk<const T> from(x, a.x.step, t0);
-            Walk<const uint8_t> begins(q.reset ? q.reset + s * q.reset_sequence : nullptr, q.reset_step, t0);
-            Walk<T> to(y, a.y.step, t0);
-            auto fetch = [&](int t) {
-#pragma unroll
-                for (int i = 0; i < kAhead; ++i) {
-                    flag[i] = false;
-                    if (t + i < end) {
-                        next[i] = load_pack<T, V>(from.at);
-                        if (q.reset) flag[i] = *begins.at != 0;
-                    }
-                    from.next();
-                    begins.next();
-                }
-            };
-            fetch(t0);
-            for (int t = t0; t < end; t += kAhead) {
-                Pack<T, V> now[kAhead];
-                bool cut[kAhead];
-#pragma unroll
-                for (int i = 0; i < kAhead; ++i) {
-                    now[i] = next[i];
-                    cut[i] = flag[i];
-                }
-                fetch(t + kAhead);
-#pragma unroll
-                for (int i = 0; i < kAhead; ++i) {
-                    if (t + i >= end) continue;
+            for (int half = 0; t < end; half ^= 1) {
+                Pack<T, V> now[kGroup];
+                copies_wait<1>();
+                rows.take(half, now);
+                rows.fetch(half);
+                copies_commit();
+                auto step = [&](int i) {
                     Two row[H], p[H];
                     unpack<T, V>(now[i], row);
-                    if (cut[i]) clear<H, K - 1>(window);
                     filter<H, K>(w, b, window, row, p);
 #pragma unroll
                     for (int h = 0; h < H; ++h) p[h] = activate_two<decltype(act)::value>(p[h]);
-                    *reinterpret_cast<Pack<T, V>*>(to.at) = pack<T, V>(p);
-                    to.next();
+                    *reinterpret_cast<Pack<T, V>*>(y) = pack<T, V>(p);
+                    y += a.y.step;
                     shift<H, K - 1>(window, row);
+                };
+                if (t + kGroup <= end && (resets >> (t - t0) & ((1u << kGroup) - 1)) == 0) {
+#pragma unroll
+                    for (int i = 0; i < kGroup; ++i) step(i);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < kGroup; ++i) {
+                        if (t + i >= end) continue;
+                        if (resets >> (t - t0 + i) & 1) clear<H, K - 1>(window);
+                        step(i);
+                    }
                 }
+                t += kGroup;
             }
         });
+        copies_wait<0>();
+    } else if (none && final_state) {
+        load_window<T, V, K>(a, x, s, c, t0, window);
     }
     if (final_state && (none || (end > t0 && end == last))) {
 #pragma unroll
@@ -207,151 +242,159 @@ __global__ void __launch_bounds__(kThreads) k_conv_forward(Conv a) {
     Pack<T, V> zero;
 #pragma unroll
     for (int v = 0; v < V; ++v) zero.v[v] = Element<T>::store(0.0f);
-    for (int t = max(t0, end); t < t1; ++t) *reinterpret_cast<Pack<T, V>*>(y + t * a.y.step) = zero;
+    for (t = max(t0, end); t < t1; ++t, y += a.y.step) *reinterpret_cast<Pack<T, V>*>(y) = zero;
 }
 
 // Block (x, y): x packs of channels, y runs at a time; every thread goes through the runs that are a
 // multiple of the launch's workers apart and keeps its channels' sums of dw and db. A run's dx takes
 // dp of the K - 1 steps behind it too, which are computed again.
 template <typename T, int V, int K>
-__global__ void __launch_bounds__(kThreads, 3) k_conv_backward(Conv a) {
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 3) k_conv_backward(Conv a) {
     constexpr int H = (V + 1) / 2;
+    constexpr int WIDTH = (K + 1) * 2 * H + 1;
+    // the ring of x and dy, and at the end the sums of the block's threads
+    constexpr int RING = 4 * kGroup * kThreads * sizeof(Pack<T, V>), SUMS = kThreads * WIDTH * sizeof(float);
+    __shared__ __align__(16) unsigned char memory[RING > SUMS ? RING : SUMS];
+    auto* ring = reinterpret_cast<Pack<T, V>*>(memory) + threadIdx.y * blockDim.x + threadIdx.x;
     wait_previous();
     release_next();
     const Sequences& q = a.q;
     const int column = blockIdx.x * blockDim.x + threadIdx.x;
     const int c = column * V;
     const bool mine = column < a.packs;
-    Two dw[K][H], db[1][H];
+    const int cc = mine ? c : 0;
+    Two dw[K][H], db[1][H], w[K][H], b[H];
     clear<H, K>(dw);
     clear<H, 1>(db);
-    if (mine) {
-        Two w[K][H], b[H];
-        load_filter<V, K>(a, c, w, b);
-        const int64_t items = q.sequences * a.runs;
-        for (int64_t item = static_cast<int64_t>(blockIdx.y) * blockDim.y + threadIdx.y; item < items;
-             item += static_cast<int64_t>(gridDim.y) * blockDim.y) {
-            const int64_t run = item / q.sequences, s = item - run * q.sequences;
-            const int t0 = static_cast<int>(run) * kRun, t1 = min(q.steps, t0 + kRun), last = q.live(s);
-            const T* x = static_cast<const T*>(a.x.data) + s * a.x.sequence + c;
-            const T* dy = static_cast<const T*>(a.dy.data) + s * a.dy.sequence + c;
-            T* dx = static_cast<T*>(a.y.data) + s * a.y.sequence + c;
-            T* dstate = a.dstate ? static_cast<T*>(a.dstate) + s * (K - 1) * q.channels + c : nullptr;
-            const T* given = a.final_gradient ? static_cast<const T*>(a.final_gradient) + s * (K - 1) * q.channels + c : nullptr;
-            // pending[j]: the gradient so far of the row j before the current one; the oldest is complete
-            // once the current step has added to it
-            Two pending[K][H], window[K - 1][H];
-            clear<H, K>(pending);
-            const int far = min(t1 + K - 1, last);
-            if (last > t0) {
-                int since = load_window<T, V, K>(a, x, s, c, t0, window);
-                with_activation(a.activation, [&](auto act) {
-                    Pack<T, V> next_x[kAhead], next_dy[kAhead], none;
-#pragma unroll
-                    for (int v = 0; v < V; ++v) none.v[v] = Element<T>::store(0.0f);
-                    bool flag[kAhead];
-                    Walk<const T> from_x(x, a.x.step, t0), from_dy(dy, a.dy.step, t0);
-                    Walk<const uint8_t> begins(q.reset ? q.reset + s * q.reset_sequence : nullptr, q.reset_step, t0);
-                    Walk<T> to(dx, a.y.step, t0 - (K - 1));
-                    auto fetch = [&](int t) {
-#pragma unroll
-                        for (int i = 0; i < kAhead; ++i) {
-                            flag[i] = false;
-                            next_x[i] = next_dy[i] = none;
-                            if (t + i < far) {
-                                next_x[i] = load_pack<T, V>(from_x.at);
-                                next_dy[i] = load_pack<T, V>(from_dy.at);
-                                if (q.reset) flag[i] = *begins.at != 0;
-                            }
-                            from_x.next();
-                            from_dy.next();
-                            begins.next();
-                        }
-                    };
-                    fetch(t0);
-                    for (int t = t0; t < t1 + K - 1; t += kAhead) {
-                        Pack<T, V> now_x[kAhead], now_dy[kAhead];
-                        bool cut[kAhead];
-#pragma unroll
-                        for (int i = 0; i < kAhead; ++i) {
-                            now_x[i] = next_x[i];
-                            now_dy[i] = next_dy[i];
-                            cut[i] = flag[i];
-                        }
-                        fetch(t + kAhead);
-#pragma unroll
-                        for (int i = 0; i < kAhead; ++i) {
-                            const int at = t + i;
-                            Two row[H], p[H], pre[H];
-                            unpack<T, V>(now_x[i], row);
-                            unpack<T, V>(now_dy[i], p);
+    load_filter<V, K>(a, cc, w, b);
+    const int64_t items = q.sequences * a.runs;
+    // every thread of a warp makes as many turns: the resets are found together
+    for (int64_t turn = static_cast<int64_t>(blockIdx.y) * blockDim.y; turn < items; turn += static_cast<int64_t>(gridDim.y) * blockDim.y) {
+        const int64_t item = min(turn + threadIdx.y, items - 1);
+        const bool working = mine && turn + threadIdx.y < items;
+        const int64_t run = item / q.sequences, s = item - run * q.sequences;
+        const int t0 = static_cast<int>(run) * kRun, t1 = min(q.steps, t0 + kRun), last = q.live(s), far = min(t1 + K - 1, last);
+        const uint32_t resets = resets_of(q, s, t0, far, a.lanes);
+        const uint32_t behind = resets_of(q, s, t0 + kRun, far, a.lanes);
+        if (!working) continue;
+        const T* x = static_cast<const T*>(a.x.data) + s * a.x.sequence + c;
+        const T* dy = static_cast<const T*>(a.dy.data) + s * a.dy.sequence + c;
+        T* dx = a.y.data ? static_cast<T*>(a.y.data) + s * a.y.sequence + c : nullptr;
+        T* dstate = a.dstate ? static_cast<T*>(a.dstate) + s * (K - 1) * q.channels + c : nullptr;
+        const T* given = a.final_gradient ? static_cast<const T*>(a.final_gradient) + s * (K - 1) * q.channels + c : nullptr;
+        // pending[j]: the gradient so far of the row j before the current one; the oldest is complete
+        // once the current step has added to it
+        Two pending[K][H], window[K - 1][H];
+        clear<H, K>(pending);
+        if (last > t0) {
+            Ring<T, V> rows_x(ring, x, a.x.step, t0, far), rows_dy(ring + 2 * kGroup * kThreads, dy, a.dy.step, t0, far);
+            rows_x.fetch(0);
+            rows_dy.fetch(0);
+            copies_commit();
+            rows_x.fetch(1);
+            rows_dy.fetch(1);
+            copies_commit();
+            int since = load_window<T, V, K>(a, x, s, c, t0, window);
+            T* to = dx ? dx + (t0 - (K - 1)) * a.y.step : nullptr;
+            with_activation(a.activation, [&](auto act) {
+                int half = 0;
+                for (int t = t0; t < t1 + K - 1; t += kGroup, half ^= 1) {
+                    Pack<T, V> now_x[kGroup], now_dy[kGroup];
+                    copies_wait<1>();
+                    rows_x.take(half, now_x);
+                    rows_dy.take(half, now_dy);
+                    rows_x.fetch(half);
+                    rows_dy.fetch(half);
+                    copies_commit();
+                    const uint32_t begins = t - t0 < 32 ? resets >> (t - t0) : behind >> (t - t0 - 32);
+                    auto step = [&](auto whole, int i) {
+                        constexpr bool WHOLE = decltype(whole)::value != 0;  // within the run, and no reset near
+                        const int at = t + i;
+                        Two row[H], p[H], pre[H];
+                        unpack<T, V>(now_x[i], row);
+                        unpack<T, V>(now_dy[i], p);
+                        if (!WHOLE) {
                             since = min(since + 1, K);
-                            if (cut[i]) {
+                            if (begins >> i & 1) {
                                 clear<H, K - 1>(window);
                                 since = 0;
                             }
-                            filter<H, K>(w, b, window, row, pre);
+                        }
+                        filter<H, K>(w, b, window, row, pre);
+#pragma unroll
+                        for (int h = 0; h < H; ++h) {
+                            p[h] = p[h] * slope_of<decltype(act)::value>(pre[h]);
+                            if (!WHOLE && at >= last) p[h] = Two();  // behind the sequence nothing is added any more
+                        }
+#pragma unroll
+                        for (int j = K - 1; j >= 1; --j) {
 #pragma unroll
                             for (int h = 0; h < H; ++h) {
-                                p[h] = p[h] * slope_of<decltype(act)::value>(pre[h]);
-                                if (at >= last) p[h] = Two();  // behind the sequence nothing is added any more
+                                pending[j][h] = multiply_add(w[K - 1 - j][h], WHOLE || since >= j ? p[h] : Two(), pending[j - 1][h]);
                             }
+                        }
 #pragma unroll
-                            for (int j = K - 1; j >= 1; --j) {
+                        for (int h = 0; h < H; ++h) {
+                            pending[0][h] = w[K - 1][h] * p[h];
+                            const Two own = WHOLE || at < t1 ? p[h] : Two();
+                            db[0][h] = db[0][h] + own;
+                            dw[K - 1][h] = multiply_add(own, row[h], dw[K - 1][h]);
 #pragma unroll
-                                for (int h = 0; h < H; ++h) {
-                                    pending[j][h] = multiply_add(w[K - 1 - j][h], since >= j ? p[h] : Two(), pending[j - 1][h]);
-                                }
+                            for (int k = 0; k < K - 1; ++k) dw[k][h] = multiply_add(own, window[k][h], dw[k][h]);
+                        }
+                        if (!WHOLE && at == last - 1 && given) {  // the final state's entry K - 2 - j is row last - 1 - j
+#pragma unroll
+                            for (int j = 0; j < K - 1; ++j) {
+                                if (since < j) continue;
+                                Two v[H];
+                                unpack<T, V>(load_pack<T, V>(given + (K - 2 - j) * q.channels), v);
+#pragma unroll
+                                for (int h = 0; h < H; ++h) pending[j][h] = pending[j][h] + v[h];
                             }
+                        }
+                        const int done = at - (K - 1);
+                        if (WHOLE || (done >= t0 && done < t1)) {
+                            if (dx) *reinterpret_cast<Pack<T, V>*>(to) = pack<T, V>(pending[K - 1]);
+                        } else if (done < 0 && t0 == 0 && dstate) {
+                            *reinterpret_cast<Pack<T, V>*>(dstate + (K - 1 + done) * q.channels) = pack<T, V>(pending[K - 1]);
+                        }
+                        if (dx) to += a.y.step;
+                        shift<H, K - 1>(window, row);
+                    };
+                    const bool whole = since >= K - 1 && t >= t0 + K - 1 && t + kGroup <= t1 && t + kGroup < last && (begins & ((1u << kGroup) - 1)) == 0;
+                    if (whole) {
 #pragma unroll
-                            for (int h = 0; h < H; ++h) {
-                                pending[0][h] = w[K - 1][h] * p[h];
-                                const Two own = at < t1 ? p[h] : Two();
-                                db[0][h] = db[0][h] + own;
-                                dw[K - 1][h] = multiply_add(own, row[h], dw[K - 1][h]);
+                        for (int i = 0; i < kGroup; ++i) {
+                            in_order();
+                            step(Constant<1>{}, i);
+                        }
+                    } else {
 #pragma unroll
-                                for (int k = 0; k < K - 1; ++k) dw[k][h] = multiply_add(own, window[k][h], dw[k][h]);
-                            }
-                            if (at == last - 1 && given) {  // the final state's entry K - 2 - j is row last - 1 - j
-#pragma unroll
-                                for (int j = 0; j < K - 1; ++j) {
-                                    if (since < j) continue;
-                                    Two v[H];
-                                    unpack<T, V>(load_pack<T, V>(given + (K - 2 - j) * q.channels), v);
-#pragma unroll
-                                    for (int h = 0; h < H; ++h) pending[j][h] = pending[j][h] + v[h];
-                                }
-                            }
-                            const int done = at - (K - 1);
-                            if (done >= t0 && done < t1) {
-                                if (a.y.data) *reinterpret_cast<Pack<T, V>*>(to.at) = pack<T, V>(pending[K - 1]);
-                            } else if (done < 0 && t0 == 0 && dstate) {
-                                *reinterpret_cast<Pack<T, V>*>(dstate + (K - 1 + done) * q.channels) = pack<T, V>(pending[K - 1]);
-                            }
-                            to.next();
-                            shift<H, K - 1>(window, row);
+                        for (int i = 0; i < kGroup; ++i) {
+                            in_order();
+                            step(Constant<0>{}, i);
                         }
                     }
-                });
-                continue;
-            }
-            if (t0 == 0 && dstate) {  // no step: the final state is the initial one
-#pragma unroll
-                for (int k = 0; k < K - 1; ++k) {
-                    *reinterpret_cast<Pack<T, V>*>(dstate + k * q.channels) = given ? load_pack<T, V>(given + k * q.channels) : pack<T, V>(pending[k]);
                 }
+            });
+            copies_wait<0>();
+            continue;
+        }
+        if (t0 == 0 && dstate) {  // no step: the final state is the initial one
+#pragma unroll
+            for (int k = 0; k < K - 1; ++k) {
+                *reinterpret_cast<Pack<T, V>*>(dstate + k * q.channels) = given ? load_pack<T, V>(given + k * q.channels) : pack<T, V>(pending[k]);
             }
-            if (a.y.data) {
-                const Two zero[H];
-                for (int t = t0; t < t1; ++t) *reinterpret_cast<Pack<T, V>*>(dx + t * a.y.step) = pack<T, V>(zero);
-            }
+        }
+        if (dx) {
+            const Two zero[H];
+            for (int t = t0; t < t1; ++t) *reinterpret_cast<Pack<T, V>*>(dx + t * a.y.step) = pack<T, V>(zero);
         }
     }
     if (a.partial == nullptr) return;
     // the block's rows of threads meet in shared memory, in their order
-    constexpr int WIDTH = (K + 1) * 2 * H + 1;
-    __shared__ float joined[kThreads * WIDTH];
-    float* slot = joined + (threadIdx.y * blockDim.x + threadIdx.x) * WIDTH;
+    __syncthreads();
+    float* slot = reinterpret_cast<float*>(memory) + (threadIdx.y * blockDim.x + threadIdx.x) * WIDTH;
 #pragma unroll
     for (int h = 0; h < H; ++h) {
 #pragma unroll
@@ -466,6 +509,12 @@ struct Layout {
         workers = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((items + rows - 1) / rows, 4 * kSms / std::min(columns, 4 * kSms))));
     }
 };
+// Neighbouring threads of one run in the forward pass.
+int lanes_of(int packs) {
+    int lanes = 32;
+    while (lanes > 1 && lanes / 2 >= packs) lanes /= 2;
+    return lanes;
+}
 int64_t runs_of(int64_t steps) { return std::max<int64_t>(1, (steps + kRun - 1) / kRun); }
 
 // Consecutive channels of a thread where every row and state starts on a pack's boundary.
@@ -523,7 +572,8 @@ extern "C" int t8b_causal_conv_forward(const t8b_sequences_t* q, int type, t8b_t
             const bool wide = q->channels % V == 0 && rows_aligned(*q, false, x, size, V * size) && rows_aligned(*q, false, y, size, V * size) &&
                 aligned(state, V * size) && aligned(final_state, V * size);
             a.packs = static_cast<int>(wide ? q->channels / V : q->channels);
-            const int64_t grid = (q->sequences * a.runs * a.packs + kThreads - 1) / kThreads;
+            a.lanes = lanes_of(a.packs);
+            const int64_t grid = (q->sequences * a.runs * ((a.packs + a.lanes - 1) / a.lanes * a.lanes) + kThreads - 1) / kThreads;
             if (grid > std::numeric_limits<int32_t>::max()) raise(T8B_EINVAL, "causal conv: too many elements for one call");
             with_width(width, [&](auto k) {
                 constexpr int K = decltype(k)::value;
@@ -594,6 +644,7 @@ extern "C" int t8b_causal_conv_backward(const t8b_sequences_t* q, int type, t8b_
             for (const void* p : {state, final_gradient, static_cast<const void*>(dstate)}) wide = wide && aligned(p, V * size);
             a.packs = static_cast<int>(wide ? q->channels / V : q->channels);
             const Layout l(q->sequences * a.runs, a.packs);
+            a.lanes = std::min(l.across, 32);
             with_width(width, [&](auto k) {
                 constexpr int K = decltype(k)::value;
                 launch_chain("k_conv_backward", wide ? k_conv_backward<T, V, K> : k_conv_backward<T, 1, K>, dim3(l.columns, l.workers),

@@ -38,6 +38,22 @@ struct Sequences {
     }
 };
 
+// Keeps the compiler from moving an unrolled step's loads in front of the steps before it, where they
+// would wait in registers.
+__device__ __forceinline__ void in_order() { asm volatile("" ::: "memory"); }
+
+// 4, 8 or 16 bytes into shared memory without waiting for them.
+template <int BYTES>
+__device__ __forceinline__ void copy_async(void* to, const void* from) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))), "l"(from), "n"(BYTES)
+                 : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int PENDING>
+__device__ __forceinline__ void copies_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory");
+}
+
 // V consecutive elements as they lie in memory, and in fp32.
 template <typename T, int V>
 __device__ __forceinline__ Pack<T, V> load_pack(const T* p) {

@@ -97,10 +97,10 @@ Call call_of(const t8b_sequences_t& q, const t8b_scan_t& scan) {
     a.softplus = scan.softplus;
     return a;
 }
-// Whether two neighbouring channels of every row of a track may be accessed at once.
-bool paired(const t8b_sequences_t& q, const t8b_scan_t& scan, const t8b_track_t& t) {
+// Whether `count` neighbouring channels of every row of a track may be accessed at once.
+bool together(const t8b_sequences_t& q, const t8b_scan_t& scan, const t8b_track_t& t, int64_t count) {
     const size_t size = type_size(scan.type);
-    return t.data == nullptr || (q.channels / scan.groups % 2 == 0 && rows_aligned(q, false, t, size, 2 * size));
+    return t.data == nullptr || (q.channels / scan.groups % count == 0 && rows_aligned(q, false, t, size, count * size));
 }
 void check_room(const char* what, const void* workspace, size_t given, size_t needed) {
     if (needed && (workspace == nullptr || given < needed || !aligned(workspace, 256))) {
@@ -152,8 +152,8 @@ extern "C" int t8b_selective_scan_forward(const t8b_sequences_t* q, const t8b_sc
         a.y = Track<void>(y);
         a.final_state = final_state;
         a.saved = saved;
-        a.paired = paired(*q, *scan, scan->u) && paired(*q, *scan, scan->delta) && paired(*q, *scan, scan->z) && paired(*q, *scan, y);
-        a.saved_paired = q->channels / scan->groups % 2 == 0 && aligned(saved, 8);
+        a.wide = 1;
+        for (const t8b_track_t* t : {&scan->u, &scan->delta, &scan->z, static_cast<const t8b_track_t*>(&y)}) a.wide &= together(*q, *scan, *t, 16 / size);
         float* w = static_cast<float*>(workspace);
         a.carry = w + room.carry;
         a.sizes = w + room.sizes;
@@ -227,10 +227,10 @@ extern "C" int t8b_selective_scan_backward(const t8b_sequences_t* q, const t8b_s
         a.saved = const_cast<float*>(saved);
         // four channels of a row (or two, or one) at once in the backward pass's elementwise part
         const int width = scan->states <= 16 ? 4 : scan->states <= 32 ? 2 : 1;
-        auto together = [&](const t8b_track_t& t) {
-            return t.data == nullptr || (q->channels / scan->groups % width == 0 && rows_aligned(*q, false, t, size, width * size));
-        };
-        a.paired = together(scan->u) && together(scan->delta) && together(scan->z) && together(dy) && together(g.du) && together(g.ddelta) && together(g.dz);
+        a.paired = 1;
+        for (const t8b_track_t* t : {&scan->u, &scan->delta, &scan->z, static_cast<const t8b_track_t*>(&dy), &g.du, &g.ddelta, &g.dz}) {
+            a.paired &= together(*q, *scan, *t, width);
+        }
         a.saved_paired = q->channels / scan->groups % 2 == 0 && aligned(saved, 8);
         a.final_gradient = final_gradient;
         a.du = Track<void>(g.du);

@@ -29,10 +29,7 @@ constexpr int kThreads = 128;
 constexpr int kTile = 8;  // steps between two kept states, and of a tile
 constexpr int kSms = 148;
 constexpr int kMostStates = 64;
-constexpr int kForwardThreads = 64;  // of a block of the forward pass: few, since all wait for one another every tile
 constexpr int kHeld = 16;            // states of a channel that one of its threads holds
-// Of every kSeriesOf quads of states the last one's second pair takes 2^x by its series.
-constexpr int kSeriesOf = 2;
 
 struct Call {
     Sequences q;
@@ -50,9 +47,10 @@ struct Call {
     float* shared;   // [blocks of a group][groups][sequences][steps][2][states]: sums of dB and dC
     float* partial;  // [workers][states + 2][channels]: sums of da, dd and ddelta_bias
     int groups, per, states, softplus;  // per: channels of a group
-    int paired, saved_paired;           // whether two neighbouring channels may be accessed at once
+    int wide, paired, saved_paired;     // whether a row may be accessed by 16 bytes; by neighbouring channels
     int chunks, chunk;                  // a chunk's steps, a multiple of kTile
     int group_blocks, workers;
+    int splits;                         // blocks of a group in a single step
 };
 
 // ------------------------------------------------------------------ arithmetic
@@ -62,53 +60,27 @@ __device__ __forceinline__ Two powers_of_two(const Two& v) {
     const float2 f = v.get();
     return Two(power_of_two(f.x), power_of_two(f.y));
 }
-// The same without the 2^x unit, from the units of multiplications: 2^i p(d) with i the nearest integer to v (an
-// addition that rounds the fraction away, and leaves i in the low bits) and d = v - i in [-1/2, 1/2]. p is a
-// polynomial with p(0) = 1, fitted for the least relative error: 2^-23, with fp32's roundings 2^-22, as much as
-// the unit's. Arguments are taken into -126 ... 128: what is below counts as 2^-126, above as infinite; a NaN
-// is lost (a NaN size is in what is added to h, too; a NaN rate is the caller's to see to).
-__device__ __forceinline__ Two powers_by_series(const Two& v) {
-    const float2 f = v.get();
-    const Two x(fminf(fmaxf(f.x, -126.0f), 128.0f), fminf(fmaxf(f.y, -126.0f), 128.0f));
-    const Two shifted = x + both(12582912.0f);  // 1.5 2^23
-    const Two d = multiply_add(shifted + both(-12582912.0f), both(-1.0f), x);
-    Two p = multiply_add(both(1.3264727e-3f), d, both(9.6715126e-3f));
-    p = multiply_add(p, d, both(5.5507337e-2f));
-    p = multiply_add(p, d, both(0.24022242f));
-    p = multiply_add(p, d, both(0.69314698f));
-    p = multiply_add(p, d, both(1.0f));
-    const float2 i = shifted.get(), m = p.get();
-    return Two(__int_as_float(__float_as_int(m.x) + (__float_as_int(i.x) << 23)), __int_as_float(__float_as_int(m.y) + (__float_as_int(i.y) << 23)));
-}
 // log(1 + x), 0 <= x <= 1: x times a polynomial fitted for the least relative error, 2^-25
-__device__ __forceinline__ Two log_one_plus(const Two& x) {
-    Two p = multiply_add(both(5.2326915e-3f), x, both(-2.9505228e-2f));
-    p = multiply_add(p, x, both(7.8225934e-2f));
-    p = multiply_add(p, x, both(-0.13663244f));
-    p = multiply_add(p, x, both(0.19106006f));
-    p = multiply_add(p, x, both(-0.24842982f));
-    p = multiply_add(p, x, both(0.33319097f));
-    p = multiply_add(p, x, both(-0.49999493f));
-    p = multiply_add(p, x, both(0.99999997f));
+__device__ __forceinline__ float log_one_plus(float x) {
+    float p = fmaf(5.2326915e-3f, x, -2.9505228e-2f);
+    p = fmaf(p, x, 7.8225934e-2f);
+    p = fmaf(p, x, -0.13663244f);
+    p = fmaf(p, x, 0.19106006f);
+    p = fmaf(p, x, -0.24842982f);
+    p = fmaf(p, x, 0.33319097f);
+    p = fmaf(p, x, -0.49999493f);
+    p = fmaf(p, x, 0.99999997f);
     return p * x;
 }
-// softplus(v) = max(v, 0) + log(1 + exp(-|v|)), and its slope sigmoid(v). The argument's product with log2 e
-// is taken to twice fp32's precision.
-__device__ __forceinline__ Two softplus(const Two& v, Two* slope = nullptr) {
-    const float2 f = v.get();
-    const Two away(-fabsf(f.x), -fabsf(f.y));
-    const Two high = away * both(kLog2E);
-    const Two low = multiply_add(away, both(-kLog2E), high) * both(-kLn2);
-    Two x = powers_of_two(high);
-    x = multiply_add(x, fabsf(f.x) < 100.0f && fabsf(f.y) < 100.0f ? low : Two(), x);
-    if (slope) {
-        const float2 e = x.get();
-        const float rx = reciprocal(1.0f + e.x), ry = reciprocal(1.0f + e.y);
-        *slope = Two(f.x > 0.0f ? rx : e.x * rx, f.y > 0.0f ? ry : e.y * ry);
-    }
-    return log_one_plus(x) + Two(f.x > 0.0f ? f.x : 0.0f, f.y > 0.0f ? f.y : 0.0f);
+// softplus(v) = max(v, 0) + log(1 + exp(-|v|)), and its slope sigmoid(v)
+__device__ __forceinline__ float softplus(float v) {
+    return log_one_plus(exponential(-fabsf(v))) + (v > 0.0f ? v : 0.0f);
 }
-__device__ __forceinline__ float softplus(float v) { return softplus(both(v)).get().x; }
+__device__ __forceinline__ float softplus(float v, float& slope) {
+    const float x = exponential(-fabsf(v)), r = reciprocal(1.0f + x);
+    slope = v > 0.0f ? r : x * r;
+    return log_one_plus(x) + (v > 0.0f ? v : 0.0f);
+}
 
 // Which of a tile's steps are resets, one bit each: the same in every lane of a warp.
 __device__ __forceinline__ unsigned reset_bits(const Sequences& q, int64_t s, int t0, int end) {
@@ -132,238 +104,210 @@ struct Place {
         chunk = static_cast<int>(at - s * a.chunks);
     }
 };
-// Rows of a track one after the other, two channels of each: one pointer for all of an unrolled tile's rows.
-template <typename T>
-struct Pairs {
-    T* at;
-    int64_t step;
-    __device__ __forceinline__ Pairs(const Track<void>& track, int64_t s, int t, int c)
-        : at(static_cast<T*>(track.data) + s * track.sequence + t * track.step + c), step(track.step) {}
-    // into shared memory; both at once (and asynchronously) where every row's pair starts on a pair
-    __device__ __forceinline__ void load(Pack<T, 2>* to, bool paired, bool second) const {
-        if (paired) {
-            asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))), "l"(at),
-                         "n"(2 * sizeof(T)) : "memory");
-            return;
-        }
-        Pack<T, 2> p;
-        p.v[0] = at[0];
-        p.v[1] = second ? at[1] : Element<T>::store(0.0f);
-        *to = p;
-    }
-    __device__ __forceinline__ void store(const Two& v, bool paired, bool second) const {
-        const Pack<T, 2> p = pack<T, 2>({v});
-        if (paired) {
-            *reinterpret_cast<Pack<T, 2>*>(at) = p;
-        } else {
-            at[0] = p.v[0];
-            if (second) at[1] = p.v[1];
-        }
-    }
-    __device__ __forceinline__ void next() { at += step; }
-};
-template <typename T>
-__device__ __forceinline__ Two value(const Pack<T, 2>& p) {
-    Two v[1];
-    unpack<T, 2>(p, v);
-    return v[0];
-}
-__device__ __forceinline__ Two silu(const Two& v) {
-    const float2 f = v.get();
-    return Two(f.x * sigmoid(f.x), f.y * sigmoid(f.y));
-}
+__device__ __forceinline__ float silu(float v) { return v * sigmoid(v); }
 
-// Two channels of a thread, kHeld states of each; LN lanes share a pair of channels.
+// A thread has kHeld states of a channel; LN lanes share a channel, a block the channels that one group of
+// B and C serves. A tile's rows come into shared memory 16 bytes at a time while the one before is worked on,
+// and y leaves the same way; where rows do not start on 16 bytes (a.wide 0), element by element.
 // ENDS: a chunk's end from a zero state, the sum of its D, and whether a reset cuts it, in place of y.
 template <typename T, int LN, bool ENDS>
-__global__ void __launch_bounds__(kForwardThreads, 8) k_scan_forward(Call a) {
-    constexpr int NP = kHeld * LN, CB = kForwardThreads / LN * 2, H = kHeld / 2;
+__global__ void __launch_bounds__(kThreads, 5) k_scan_forward(Call a) {
+    constexpr int NP = kHeld * LN, CB = kThreads / LN;
+    constexpr int V = 16 / sizeof(T), PACKS = CB / V;  // of a row
     wait_previous();
     release_next();
     __shared__ __align__(16) float bc[2][kTile][2][NP];
-    __shared__ Pack<T, 2> rows[2][3][kTile][kForwardThreads];  // u, delta and z of a tile: each thread writes and reads its own
+    __shared__ __align__(16) T rows[2][3][kTile][CB];  // u, delta, z
+    __shared__ __align__(16) T ys[2][kTile][CB];
     const Sequences& q = a.q;
     const Place place(a, blockIdx.x);
     const int64_t s = place.s;
-    const int lane = threadIdx.x % LN, local = place.part * CB + threadIdx.x / LN * 2;
-    const bool mine = local < a.per, second = local + 1 < a.per, paired = a.paired != 0;
-    const int c = place.group * a.per + (mine ? local : 0);
+    const int lane = threadIdx.x % LN, column = threadIdx.x / LN, base = place.part * CB;
+    const int width = min(CB, a.per - base);  // channels of this block
+    const bool mine = column < width;
+    const int c = place.group * a.per + base + (mine ? column : 0);
     const int t0 = place.chunk * a.chunk, t1 = min(q.steps, t0 + a.chunk), last = q.live(s), end = min(t1, last);
     const int n0 = lane * kHeld, channels = q.channels;
     const bool gate = !ENDS && a.z.data != nullptr;
-    Pairs<T> u(a.u, s, t0, c), delta(a.delta, s, t0, c), z(gate ? a.z : a.u, s, t0, c);
-    Pairs<T> y(a.y, s, t0, c);
-    const T* b = static_cast<const T*>(a.b.data) + s * a.b.sequence + place.group * a.b_group;
-    const T* cc = static_cast<const T*>(a.c.data) + s * a.c.sequence + place.group * a.c_group;
     const int64_t at_chunk = s * a.chunks + place.chunk;
+    auto row_of = [&](const Track<void>& track, int t) {
+        return static_cast<T*>(track.data) + s * track.sequence + t * track.step + (place.group * a.per + base);
+    };
 
-    Two rate[2][H], h[2][H];  // a log2 e, and the states, in pairs of states
+    Two rate[kHeld / 2], h[kHeld / 2];  // a log2 e, and the states
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        const int ck = c + (k && second ? 1 : 0);
+    for (int i = 0; i < kHeld; i += 2) {
+        float r[2] = {0.0f, 0.0f}, from[2] = {0.0f, 0.0f};
 #pragma unroll
-        for (int i = 0; i < H; ++i) {
-            float r[2] = {0.0f, 0.0f}, v[2] = {0.0f, 0.0f};
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int n = n0 + 2 * i + j;
-                if (n >= a.states) continue;
-                r[j] = a.a[static_cast<int64_t>(ck) * a.states + n] * kLog2E;
-                if (!ENDS && a.chunks > 1) {
-                    v[j] = a.carry[(at_chunk * a.states + n) * channels + ck];
-                } else if (!ENDS && a.state) {
-                    v[j] = a.state[(s * channels + ck) * a.states + n];
-                }
-                if (r[j] != r[j]) r[j] = INFINITY;  // powers_by_series loses a NaN: 2^inf times h = 0 is one
+        for (int j = 0; j < 2; ++j) {
+            const int n = n0 + i + j;
+            if (n >= a.states) continue;
+            r[j] = a.a[static_cast<int64_t>(c) * a.states + n] * kLog2E;
+            if (!ENDS && a.chunks > 1) {
+                from[j] = a.carry[(at_chunk * a.states + n) * channels + c];
+            } else if (!ENDS && a.state) {
+                from[j] = a.state[(s * channels + c) * a.states + n];
             }
-            rate[k][i] = Two(r[0], r[1]);
-            h[k][i] = Two(v[0], v[1]);
         }
+        rate[i / 2] = Two(r[0], r[1]);
+        h[i / 2] = Two(from[0], from[1]);
     }
-    const int c1 = c + (second ? 1 : 0);
-    const Two skip = a.d ? Two(a.d[c], a.d[c1]) : Two(), bias = a.delta_bias ? Two(a.delta_bias[c], a.delta_bias[c1]) : Two();
+    const float skip = a.d ? a.d[c] : 0.0f, bias = a.delta_bias ? a.delta_bias[c] : 0.0f;
 
-    constexpr int PER = 2 * kTile * NP / kForwardThreads;
+    constexpr int PER = 2 * kTile * NP / kThreads;
     T raw_bc[PER];
+    bool flag = false;  // whether the next tile's step threadIdx % 8 is a reset
     auto fetch = [&](int t, int buffer) {
+        if (a.wide) {
 #pragma unroll
-        for (int i = 0; i < kTile; ++i) {
-            if (mine && t + i < end) {
-                u.load(&rows[buffer][0][i][threadIdx.x], paired, second);
-                delta.load(&rows[buffer][1][i][threadIdx.x], paired, second);
-                if (gate) z.load(&rows[buffer][2][i][threadIdx.x], paired, second);
+            for (int k = 0; k < 3; ++k) {
+                if (k == 2 && !gate) continue;
+#pragma unroll
+                for (int e = threadIdx.x; e < kTile * PACKS; e += kThreads) {
+                    const int i = e / PACKS, at = e % PACKS * V;
+                    if (t + i < end && at < width) copy_async<16>(&rows[buffer][k][i][at], row_of(k == 0 ? a.u : k == 1 ? a.delta : a.z, t + i) + at);
+                }
             }
-            u.next();
-            delta.next();
-            z.next();
+        } else if (mine) {
+            for (int i = lane; i < kTile; i += LN) {
+                if (t + i >= end) break;
+                rows[buffer][0][i][column] = row_of(a.u, t + i)[column];
+                rows[buffer][1][i][column] = row_of(a.delta, t + i)[column];
+                if (gate) rows[buffer][2][i][column] = row_of(a.z, t + i)[column];
+            }
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
+        copies_commit();
+        const T* b = static_cast<const T*>(a.b.data) + s * a.b.sequence + place.group * a.b_group;
+        const T* cc = static_cast<const T*>(a.c.data) + s * a.c.sequence + place.group * a.c_group;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            const int e = i * kForwardThreads + threadIdx.x, step = e / (2 * NP), which = e / NP % 2, n = e % NP;
+            const int e = i * kThreads + threadIdx.x, step = e / (2 * NP), which = e / NP % 2, n = e % NP;
             raw_bc[i] = Element<T>::store(0.0f);
             if (t + step < end && n < a.states) raw_bc[i] = which ? cc[(t + step) * a.c.step + n] : b[(t + step) * a.b.step + n];
         }
+        const int at = t + static_cast<int>(threadIdx.x & 7);
+        flag = at < end && q.resets(s, at);
     };
-    auto stage = [&](int buffer) {
-#pragma unroll
-        for (int i = 0; i < PER; ++i) (&bc[buffer][0][0][0])[i * kForwardThreads + threadIdx.x] = Element<T>::load(raw_bc[i]);
+    auto leave = [&](int t, int buffer) {  // a finished tile's y
+        if (ENDS || !a.wide) return;
+        for (int e = threadIdx.x; e < kTile * PACKS; e += kThreads) {
+            const int i = e / PACKS, at = e % PACKS * V;
+            if (t + i < end && at < width) {
+                *reinterpret_cast<Pack<T, V>*>(row_of(a.y, t + i) + at) = *reinterpret_cast<const Pack<T, V>*>(&ys[buffer][i][at]);
+            }
+        }
     };
     int buffer = 0;
-    Two total;
+    float total = 0.0f;
     bool cut = false;
-    if (t0 < end) {
-        fetch(t0, 0);
-        stage(0);
-        __syncthreads();
-    }
+    if (t0 < end) fetch(t0, 0);
     for (int t = t0; t < end; t += kTile, buffer ^= 1) {
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
-        const unsigned resets = reset_bits(q, s, t, end);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) (&bc[buffer][0][0][0])[i * kThreads + threadIdx.x] = Element<T>::load(raw_bc[i]);
+        copies_wait<0>();
+        const unsigned resets = q.reset ? __ballot_sync(0xffffffffu, flag) & 0xffu : 0u;
+        __syncthreads();  // this tile is there, and every thread is done with the one before
         if (t + kTile < end) fetch(t + kTile, buffer ^ 1);
+        if (t > t0) leave(t - kTile, buffer ^ 1);
         if (!ENDS && a.saved && mine) {
             float* to = a.saved + ((s * ((q.steps + kTile - 1) / kTile) + t / kTile) * a.states + n0) * channels + c;
 #pragma unroll
             for (int i = 0; i < kHeld; ++i) {
-                const float2 v0 = h[0][i / 2].get(), v1 = h[1][i / 2].get();
-                const float w0 = i % 2 ? v0.y : v0.x, w1 = i % 2 ? v1.y : v1.x;
-                if (n0 + i < a.states) {
-                    if (a.saved_paired) {
-                        *reinterpret_cast<float2*>(to) = make_float2(w0, w1);
-                    } else {
-                        to[0] = w0;
-                        if (second) to[1] = w1;
-                    }
-                }
+                if (n0 + i < a.states) *to = i % 2 ? h[i / 2].get().y : h[i / 2].get().x;
                 to += channels;
             }
         }
-        const int count = min(kTile, end - t);
-#pragma unroll 2
-        for (int i = 0; i < count; ++i) {
-            if (resets >> i & 1) {
-                cut = true;
-                total = Two();
+        // a step's D, D u, u and gate; and the states' part of it
+        struct Step {
+            float size, in, u, gate;
+        };
+        auto elementwise = [&](int i) {
+            Step v;
+            v.u = Element<T>::load(rows[buffer][0][i][column]);
+            v.size = Element<T>::load(rows[buffer][1][i][column]) + bias;
+            if (a.softplus) v.size = softplus(v.size);
+            v.in = v.size * v.u;
+            v.gate = gate ? silu(Element<T>::load(rows[buffer][2][i][column])) : 1.0f;
+            return v;
+        };
+        auto advance = [&](int i, const Step& v) {
+            Two out;
+            const Two by = both(v.size), in = both(v.in);
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
+            for (int n = 0; n < kHeld; n += 4) {
+                const Pack<float, 4> b = *reinterpret_cast<const Pack<float, 4>*>(&bc[buffer][i][0][n0 + n]);
+                const Pack<float, 4> c = ENDS ? b : *reinterpret_cast<const Pack<float, 4>*>(&bc[buffer][i][1][n0 + n]);
 #pragma unroll
-                    for (int n = 0; n < H; ++n) h[k][n] = Two();
-                }
-            }
-            const Two in_u = value<T>(rows[buffer][0][i][threadIdx.x]);
-            Two size = value<T>(rows[buffer][1][i][threadIdx.x]) + bias;
-            if (a.softplus) size = softplus(size);
-            const float2 by = size.get(), in = (size * in_u).get();
-            Two out[2];
-#pragma unroll
-            for (int n = 0; n < kHeld / 4; ++n) {
-                const float4 vb = *reinterpret_cast<const float4*>(&bc[buffer][i][0][n0 + 4 * n]);
-                const float4 vc = ENDS ? vb : *reinterpret_cast<const float4*>(&bc[buffer][i][1][n0 + 4 * n]);
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const Two at = both(k ? by.y : by.x), add = both(k ? in.y : in.x);
-                    const Two x = at * rate[k][2 * n], w = at * rate[k][2 * n + 1];
-                    const Two e0 = powers_of_two(x), e1 = n % kSeriesOf == kSeriesOf - 1 ? powers_by_series(w) : powers_of_two(w);
-                    h[k][2 * n] = multiply_add(e0, h[k][2 * n], add * Two(vb.x, vb.y));
-                    h[k][2 * n + 1] = multiply_add(e1, h[k][2 * n + 1], add * Two(vb.z, vb.w));
-                    if (!ENDS) {
-                        out[k] = multiply_add(h[k][2 * n], Two(vc.x, vc.y), out[k]);
-                        out[k] = multiply_add(h[k][2 * n + 1], Two(vc.z, vc.w), out[k]);
-                    }
+                for (int j = 0; j < 4; j += 2) {
+                    h[(n + j) / 2] = multiply_add(powers_of_two(by * rate[(n + j) / 2]), h[(n + j) / 2], in * Two(b.v[j], b.v[j + 1]));
+                    out = multiply_add(h[(n + j) / 2], Two(c.v[j], c.v[j + 1]), out);
                 }
             }
             if (ENDS) {
-                total = total + size;
-                continue;
+                total += v.size;
+                return;
             }
-            float s0 = out[0].sum(), s1 = out[1].sum();
+            float sum = out.sum();
 #pragma unroll
-            for (int o = LN / 2; o >= 1; o >>= 1) {
-                s0 += __shfl_xor_sync(0xffffffffu, s0, o);
-                s1 += __shfl_xor_sync(0xffffffffu, s1, o);
+            for (int o = LN / 2; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            sum = fmaf(skip, v.u, sum) * v.gate;
+            if (lane != 0) return;
+            if (a.wide) {
+                ys[buffer][i][column] = Element<T>::store(sum);
+            } else if (mine) {
+                row_of(a.y, t + i)[column] = Element<T>::store(sum);
             }
-            Two sum = multiply_add(skip, in_u, Two(s0, s1));
-            if (gate) sum = sum * silu(value<T>(rows[buffer][2][i][threadIdx.x]));
-            if (mine && lane == 0) y.store(sum, paired, second);
-            y.next();
+        };
+        auto begin = [&](int i) {
+            if ((resets >> i & 1) == 0) return;
+            cut = true;
+            total = 0.0f;
+#pragma unroll
+            for (int n = 0; n < kHeld / 2; ++n) h[n] = Two();
+        };
+        if (t + kTile <= end) {
+            // the next step's elementwise part, a chain of latencies, beside this one's states
+            Step v = elementwise(0);
+#pragma unroll
+            for (int i = 0; i < kTile; ++i) {
+                in_order();
+                begin(i);
+                const Step next = i + 1 < kTile ? elementwise(i + 1) : v;
+                advance(i, v);
+                v = next;
+            }
+        } else {
+#pragma unroll 1
+            for (int i = 0; i < end - t; ++i) {
+                begin(i);
+                advance(i, elementwise(i));
+            }
         }
-        if (t + kTile < end) stage(buffer ^ 1);
+    }
+    if (!ENDS && t0 < end) {
         __syncthreads();
+        leave(t0 + (end - 1 - t0) / kTile * kTile, buffer ^ 1);
     }
     if (!mine) return;
     if (ENDS) {
         float* to = a.carry + (at_chunk * a.states + n0) * channels + c;
 #pragma unroll
         for (int i = 0; i < kHeld; ++i) {
-            const float2 v0 = h[0][i / 2].get(), v1 = h[1][i / 2].get();
-            if (n0 + i < a.states) {
-                to[0] = i % 2 ? v0.y : v0.x;
-                if (second) to[1] = i % 2 ? v1.y : v1.x;
-            }
+            if (n0 + i < a.states) *to = i % 2 ? h[i / 2].get().y : h[i / 2].get().x;
             to += channels;
         }
-        if (lane == 0) {
-            const float2 v = total.get();
-            a.sizes[at_chunk * channels + c] = v.x;
-            if (second) a.sizes[at_chunk * channels + c + 1] = v.y;
-            if (local == 0 && place.group == 0) a.keep[at_chunk] = cut ? 0.0f : 1.0f;
-        }
+        if (lane == 0) a.sizes[at_chunk * channels + c] = total;
+        if (lane == 0 && base + column == 0 && place.group == 0) a.keep[at_chunk] = cut ? 0.0f : 1.0f;
         return;
     }
     if (lane == 0) {
-        Pairs<T> rest(a.y, s, max(t0, end), c);
-        for (int t = max(t0, end); t < t1; ++t, rest.next()) rest.store(Two(), paired, second);
+        for (int t = max(t0, end); t < t1; ++t) row_of(a.y, t)[column] = Element<T>::store(0.0f);
     }
     if (a.final_state && (last > t0 ? last <= t1 : last == 0 && t0 == 0)) {
+        float* to = a.final_state + (s * channels + c) * a.states + n0;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            if (k && !second) continue;
-            float* to = a.final_state + (s * channels + c + k) * a.states + n0;
-#pragma unroll
-            for (int i = 0; i < kHeld; ++i) {
-                const float2 v = h[k][i / 2].get();
-                if (n0 + i < a.states) to[i] = i % 2 ? v.y : v.x;
-            }
+        for (int i = 0; i < kHeld; ++i) {
+            if (n0 + i < a.states) to[i] = i % 2 ? h[i / 2].get().y : h[i / 2].get().x;
         }
     }
 }
@@ -501,17 +445,19 @@ struct Backward {
         Pack<T, EV> rows[4][kThreads];                           // u, delta, dy and z of a tile: each thread writes and reads its own
         float2 before[4][kThreads];                              // the states before it: the same
         float size[kTile][CB], in[kTile][CB], given[kTile][CB];  // D, D u, gs
-        float slope[kTile][CB], zslope[kTile][CB];
-        float b[kTile][NP], c[kTile][NP];
+        float2 b[kTile][NP], c[kTile][NP];                       // each value twice: an operand of packed arithmetic
         float2 channel_sums[kTile][3][LN][CB / 2];               // sum_n: C h, B g, a e h g, of each lane along the states
         float4 state_sums[kTile][2][LN][PARTS];                  // sum_c: D u g, gs h, of each pair of channels
     };
 };
 
-template <int BYTES>
-__device__ __forceinline__ void copy_async(void* to, const void* from) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))), "l"(from), "n"(BYTES)
-                 : "memory");
+// Four values that lie twice each.
+__device__ __forceinline__ void twice(const float2* from, Two (&v)[4]) {
+    const float4 x = reinterpret_cast<const float4*>(from)[0], y = reinterpret_cast<const float4*>(from)[1];
+    v[0] = Two(x.x, x.y);
+    v[1] = Two(x.z, x.w);
+    v[2] = Two(y.x, y.y);
+    v[3] = Two(y.z, y.w);
 }
 
 template <typename T, int LN>
@@ -563,6 +509,7 @@ __global__ void __launch_bounds__(kThreads, 3) k_scan_backward(Call a) {
 
     constexpr int PER = (2 * kTile * NP + kThreads - 1) / kThreads;
     T raw_bc[PER];
+    bool flag = false;  // whether the fetched tile's step threadIdx % 8 is a reset
     const bool gate = a.z.data != nullptr;
     const int64_t items = q.sequences * a.chunks;
     for (int64_t item = blockIdx.y; item < items; item += a.workers) {
@@ -601,6 +548,10 @@ __global__ void __launch_bounds__(kThreads, 3) k_scan_backward(Call a) {
                 }
             }
         };
+        auto fetch_flag = [&](int t) {
+            const int at = t + static_cast<int>(threadIdx.x & 7);
+            flag = at < end && q.resets(s, at);
+        };
         auto fetch_before = [&](int t) {
             const float* from = a.saved + ((s * tiles + t / kTile) * a.states + n0) * channels + c0;
 #pragma unroll
@@ -616,7 +567,7 @@ __global__ void __launch_bounds__(kThreads, 3) k_scan_backward(Call a) {
                 }
                 from += channels;
             }
-            asm volatile("cp.async.commit_group;" ::: "memory");
+            copies_commit();
         };
         // the gradient of the state after the chunk
         Two g[4];
@@ -639,35 +590,25 @@ __global__ void __launch_bounds__(kThreads, 3) k_scan_backward(Call a) {
         int t = t0 + (end - 1 - t0) / kTile * kTile, since = 0;
         if (end > t0) {
             fetch(t);
+            fetch_flag(t);
             fetch_before(t);
         }
         for (; end > t0 && t >= t0; t -= kTile) {
-            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            copies_wait<0>();
             // ---- elementwise: D, D u and gs of the tile into shared memory
             const Pack<T, EV> raw_u = m.rows[0][threadIdx.x];
+            float slope[EV], zslope[EV];
             {
                 const bool live = t + es < end;
                 const Pack<T, EV> raw_delta = m.rows[1][threadIdx.x], raw_dy = m.rows[2][threadIdx.x];
                 const Pack<T, EV> raw_z = gate ? m.rows[3][threadIdx.x] : raw_u;
-                float size[EV], in[EV], given[EV], slope[EV], zslope[EV];
+                float size[EV], in[EV], given[EV];
 #pragma unroll
-                for (int i = 0; i < EV; i += 2) {
-                    constexpr int D = EV > 1 ? 1 : 0;
-                    const int j = i + D;
-                    const Two v = Two(Element<T>::load(raw_delta.v[i]), Element<T>::load(raw_delta.v[j])) +
-                        (a.delta_bias ? Two(a.delta_bias[ec + min(i, max(ecount - 1, 0))], a.delta_bias[ec + min(j, max(ecount - 1, 0))]) : Two());
-                    Two of_v = both(1.0f), of_size = v;
-                    if (a.softplus) of_size = softplus(v, &of_v);
-                    const Two of_in = of_size * Two(Element<T>::load(raw_u.v[i]), Element<T>::load(raw_u.v[j]));
-                    const float2 f = of_size.get(), k = of_v.get(), w = of_in.get();
-                    size[i] = f.x;
-                    slope[i] = k.x;
-                    in[i] = w.x;
-                    if (D) {
-                        size[j] = f.y;
-                        slope[j] = k.y;
-                        in[j] = w.y;
-                    }
+                for (int i = 0; i < EV; ++i) {
+                    size[i] = Element<T>::load(raw_delta.v[i]) + (a.delta_bias ? a.delta_bias[ec + (i < ecount ? i : 0)] : 0.0f);
+                    slope[i] = 1.0f;
+                    if (a.softplus) size[i] = softplus(size[i], slope[i]);
+                    in[i] = size[i] * Element<T>::load(raw_u.v[i]);
                 }
 #pragma unroll
                 for (int i = 0; i < EV; ++i) {
@@ -684,30 +625,34 @@ __global__ void __launch_bounds__(kThreads, 3) k_scan_backward(Call a) {
                 *reinterpret_cast<Pack<float, EV>*>(&m.size[es][el]) = pack<float, EV>(size);
                 *reinterpret_cast<Pack<float, EV>*>(&m.in[es][el]) = pack<float, EV>(in);
                 *reinterpret_cast<Pack<float, EV>*>(&m.given[es][el]) = pack<float, EV>(given);
-                *reinterpret_cast<Pack<float, EV>*>(&m.slope[es][el]) = pack<float, EV>(slope);
-                *reinterpret_cast<Pack<float, EV>*>(&m.zslope[es][el]) = pack<float, EV>(zslope);
             }
 #pragma unroll
             for (int i = 0; i < PER; ++i) {
                 const int e = i * kThreads + threadIdx.x, step = e / (2 * NP), which = e / NP % 2, n = e % NP;
-                if (step < kTile) (which ? m.c : m.b)[step][n] = Element<T>::load(raw_bc[i]);
+                const float v = Element<T>::load(raw_bc[i]);
+                if (step < kTile) (which ? m.c : m.b)[step][n] = make_float2(v, v);
             }
-            const unsigned resets = reset_bits(q, s, t, end);
+            const unsigned resets = q.reset ? __ballot_sync(0xffffffffu, flag) & 0xffu : 0u;
             __syncthreads();
-            if (t > t0) fetch(t - kTile);
+            if (t > t0) {
+                fetch(t - kTile);
+                fetch_flag(t - kTile);
+            }
             // ---- h through the tile, then g back
-            {
+            auto pass = [&](auto cuts) {
+                constexpr bool CUTS = decltype(cuts)::value != 0;  // most tiles have no reset
                 Two h[kTile][4];
 #pragma unroll
                 for (int i = 0; i < kTile; ++i) {
+                    in_order();
                     const Two by = two(*reinterpret_cast<const float2*>(&m.size[i][2 * pair]));
                     const Two in = two(*reinterpret_cast<const float2*>(&m.in[i][2 * pair]));
-                    const float4 vb = *reinterpret_cast<const float4*>(&m.b[i][n0]);
-                    const float bn[4] = {vb.x, vb.y, vb.z, vb.w};
-                    const bool on = (resets >> i & 1) == 0;
+                    Two bn[4];
+                    twice(&m.b[i][n0], bn);
+                    const bool on = !CUTS || (resets >> i & 1) == 0;
 #pragma unroll
                     for (int n = 0; n < 4; ++n) {
-                        h[i][n] = in * both(bn[n]);
+                        h[i][n] = in * bn[n];
                         const Two from = i ? h[i ? i - 1 : 0][n] : two(m.before[n][threadIdx.x]);
                         const Two e = powers_of_two(by * rate[n]);
                         if (on) h[i][n] = multiply_add(e, from, h[i][n]);
@@ -715,19 +660,21 @@ __global__ void __launch_bounds__(kThreads, 3) k_scan_backward(Call a) {
                 }
 #pragma unroll
                 for (int i = kTile - 1; i >= 0; --i) {
+                    in_order();
                     const Two by = two(*reinterpret_cast<const float2*>(&m.size[i][2 * pair]));
                     const Two in = two(*reinterpret_cast<const float2*>(&m.in[i][2 * pair]));
                     const Two given = two(*reinterpret_cast<const float2*>(&m.given[i][2 * pair]));
-                    const float4 vb = *reinterpret_cast<const float4*>(&m.b[i][n0]), vc = *reinterpret_cast<const float4*>(&m.c[i][n0]);
-                    const float bn[4] = {vb.x, vb.y, vb.z, vb.w}, cn[4] = {vc.x, vc.y, vc.z, vc.w};
-                    const bool on = (resets >> i & 1) == 0;
+                    Two bn[4], cn[4];
+                    twice(&m.b[i][n0], bn);
+                    twice(&m.c[i][n0], cn);
+                    const bool on = !CUTS || (resets >> i & 1) == 0;
                     Two of_h, of_b, of_a;
                     float db[4], dc[4];
 #pragma unroll
                     for (int n = 0; n < 4; ++n) {
-                        g[n] = multiply_add(given, both(cn[n]), g[n]);
-                        of_h = multiply_add(h[i][n], both(cn[n]), of_h);
-                        of_b = multiply_add(g[n], both(bn[n]), of_b);
+                        g[n] = multiply_add(given, cn[n], g[n]);
+                        of_h = multiply_add(h[i][n], cn[n], of_h);
+                        of_b = multiply_add(g[n], bn[n], of_b);
                         db[n] = (in * g[n]).sum();
                         dc[n] = (given * h[i][n]).sum();
                         g[n] = g[n] * powers_of_two(by * rate[n]);
@@ -743,6 +690,11 @@ __global__ void __launch_bounds__(kThreads, 3) k_scan_backward(Call a) {
                     m.state_sums[i][0][along][Shape::state_at(pair, along)] = make_float4(db[0], db[1], db[2], db[3]);
                     m.state_sums[i][1][along][Shape::state_at(pair, along)] = make_float4(dc[0], dc[1], dc[2], dc[3]);
                 }
+            };
+            if (resets == 0) {
+                pass(Constant<0>{});
+            } else {
+                pass(Constant<1>{});
             }
             if (t > t0) fetch_before(t - kTile);
             if (++since == 16 || t == t0) {
@@ -768,14 +720,13 @@ __global__ void __launch_bounds__(kThreads, 3) k_scan_backward(Call a) {
                 if (ecount > 0 && at < t1) {
                     const bool live = at < end;
                     const Pack<float, EV> size = load_pack<float, EV>(&m.size[es][el]), given = load_pack<float, EV>(&m.given[es][el]);
-                    const Pack<float, EV> slope = load_pack<float, EV>(&m.slope[es][el]), zslope = load_pack<float, EV>(&m.zslope[es][el]);
                     float du[EV], ddelta[EV], dz[EV];
 #pragma unroll
                     for (int i = 0; i < EV; ++i) {
                         const float vu = Element<T>::load(raw_u.v[i]), skip = a.d && i < ecount ? a.d[ec + i] : 0.0f;
                         du[i] = live ? fmaf(skip, given.v[i], size.v[i] * sum[1][i]) : 0.0f;
-                        ddelta[i] = live ? fmaf(kLn2, sum[2][i], vu * sum[1][i]) * slope.v[i] : 0.0f;
-                        dz[i] = live ? zslope.v[i] * fmaf(skip, vu, sum[0][i]) : 0.0f;
+                        ddelta[i] = live ? fmaf(kLn2, sum[2][i], vu * sum[1][i]) * slope[i] : 0.0f;
+                        dz[i] = live ? zslope[i] * fmaf(skip, vu, sum[0][i]) : 0.0f;
                         dbias[i] += ddelta[i];
                         if (live) dd[i] = fmaf(given.v[i], vu, dd[i]);
                     }
@@ -922,76 +873,117 @@ __global__ void __launch_bounds__(256) k_scan_shared(Call a) {
 }
 
 // ------------------------------------------------------------------ a single step
-// LP lanes (a power of two) share a channel of a sequence and hold V consecutive states each; bound by
-// the states' bytes, read once and written once. A thread takes several sequences, their states all in flight.
+// LP lanes (a power of two) share a channel and hold V consecutive states of it each; a block takes kStepAhead
+// sequences and goes through the channels of one group, a tile of kStepThreads / LP of them at a time, with the
+// sequences' B and C in shared memory. Bound by the states' bytes, read once and written once: a thread has its
+// channel's states of every sequence in flight together. Lane l of a channel does the elementwise part of the
+// sequences l, l + LP, ... and gives D and D u to the others; the sums over its lanes end where they are used.
 constexpr int kStepAhead = 4;
-template <typename T, int V>
-__global__ void __launch_bounds__(256) k_scan_step(Call a, float* state, int lanes) {
+constexpr int kStepThreads = 256;
+template <typename T, int V, int LP>
+__global__ void __launch_bounds__(kStepThreads) k_scan_step(Call a, float* state) {
+    constexpr int HELD = V == 4 ? 4 : 2;                  // states of a lane at most: up to 64 over 16 or 32 lanes
+    constexpr int TIMES = HELD / V;
+    constexpr int OWN = LP >= kStepAhead ? 1 : kStepAhead / LP;  // sequences whose elementwise part a lane does
     wait_previous();
     release_next();
+    __shared__ __align__(16) float bc[kStepAhead][2][kMostStates];
     const Sequences& q = a.q;
     const int channels = q.channels;
-    const int64_t index = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-    const int64_t unit = index / lanes;
-    const int lane = static_cast<int>(index - unit * lanes);
-    const int64_t turn = unit / channels;
-    const int c = static_cast<int>(unit - turn * channels), group = c / a.per;
+    // block = (turn * groups + group) * splits + split
+    const int64_t at = static_cast<int64_t>(blockIdx.x) / a.splits;
+    const int split = static_cast<int>(blockIdx.x - at * a.splits);
+    const int64_t turn = at / a.groups;
+    const int group = static_cast<int>(at - turn * a.groups);
     const int64_t s0 = turn * kStepAhead;
-    const int count = static_cast<int>(max(int64_t{0}, min(int64_t{kStepAhead}, q.sequences - s0)));
-    const float skip = a.d ? a.d[c] : 0.0f, bias = a.delta_bias ? a.delta_bias[c] : 0.0f;
-    float sum[kStepAhead], size[kStepAhead], in[kStepAhead], vu[kStepAhead];
-    bool cut[kStepAhead];
-#pragma unroll
-    for (int i = 0; i < kStepAhead; ++i) {
-        sum[i] = 0.0f;
-        if (i >= count) continue;
-        const int64_t s = s0 + i;
-        vu[i] = Element<T>::load(static_cast<const T*>(a.u.data)[s * a.u.sequence + c]);
-        const float v = Element<T>::load(static_cast<const T*>(a.delta.data)[s * a.delta.sequence + c]) + bias;
-        size[i] = a.softplus ? softplus(v) : v;
-        in[i] = size[i] * vu[i];
-        cut[i] = q.reset != nullptr && q.reset[s * q.reset_sequence] != 0;
+    const int count = static_cast<int>(min(int64_t{kStepAhead}, q.sequences - s0));
+    for (int e = threadIdx.x; e < count * 2 * a.states; e += kStepThreads) {
+        const int i = e / (2 * a.states), rest = e - i * 2 * a.states, which = rest / a.states, n = rest - which * a.states;
+        const Track<void>& track = which ? a.c : a.b;
+        const int64_t apart = which ? a.c_group : a.b_group;
+        bc[i][which][n] = Element<T>::load(static_cast<const T*>(track.data)[(s0 + i) * track.sequence + group * apart + n]);
     }
-    for (int n0 = lane * V; n0 < a.states; n0 += lanes * V) {
-        Pack<float, V> h[kStepAhead];
-        float rate[V];
+    __syncthreads();
+    const int lane = threadIdx.x % LP, n0 = lane * V;
+    constexpr int TILE = kStepThreads / LP;
+    for (int local = split * TILE + threadIdx.x / LP; local - static_cast<int>(threadIdx.x) / LP < a.per; local += a.splits * TILE) {
+        const bool mine = local < a.per;
+        const int c = group * a.per + (mine ? local : 0);
+        Pack<float, V> h[kStepAhead][TIMES], rate[TIMES];
 #pragma unroll
         for (int i = 0; i < kStepAhead; ++i) {
-            if (i < count) h[i] = load_pack<float, V>(state + ((s0 + i) * channels + c) * a.states + n0);
-        }
-        const Pack<float, V> r = load_pack<float, V>(a.a + static_cast<int64_t>(c) * a.states + n0);
 #pragma unroll
-        for (int v = 0; v < V; ++v) rate[v] = r.v[v] * kLog2E;
-#pragma unroll
-        for (int i = 0; i < kStepAhead; ++i) {
-            if (i >= count) continue;
-            const int64_t s = s0 + i;
-            const T* b = static_cast<const T*>(a.b.data) + s * a.b.sequence + group * a.b_group + n0;
-            const T* cc = static_cast<const T*>(a.c.data) + s * a.c.sequence + group * a.c_group + n0;
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                const float from = cut[i] ? 0.0f : h[i].v[v];
-                h[i].v[v] = fmaf(power_of_two(size[i] * rate[v]), from, in[i] * Element<T>::load(b[v]));
-                sum[i] = fmaf(h[i].v[v], Element<T>::load(cc[v]), sum[i]);
+            for (int k = 0; k < TIMES; ++k) {
+                const int n = n0 + k * LP * V;
+                if (mine && i < count && n < a.states) h[i][k] = load_pack<float, V>(state + ((s0 + i) * channels + c) * a.states + n);
             }
-            *reinterpret_cast<Pack<float, V>*>(state + (s * channels + c) * a.states + n0) = h[i];
         }
-    }
-    for (int o = lanes / 2; o >= 1; o >>= 1) {
 #pragma unroll
-        for (int i = 0; i < kStepAhead; ++i) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], o);
-    }
-    if (lane != 0) return;
-#pragma unroll
-    for (int i = 0; i < kStepAhead; ++i) {
-        if (i >= count) continue;
-        const int64_t s = s0 + i;
-        float y = fmaf(skip, vu[i], sum[i]);
-        if (a.z.data) {
-            const float w = Element<T>::load(static_cast<const T*>(a.z.data)[s * a.z.sequence + c]);
-            y *= w * sigmoid(w);
+        for (int k = 0; k < TIMES; ++k) {
+            const int n = n0 + k * LP * V;
+            if (n < a.states) rate[k] = load_pack<float, V>(a.a + static_cast<int64_t>(c) * a.states + n);
         }
-        static_cast<T*>(a.y.data)[s * a.y.sequence + c] = Element<T>::store(y);
+        // the elementwise part of this lane's own sequences
+        float vu[OWN], size[OWN], gate[OWN];
+        const float skip = a.d ? a.d[c] : 0.0f, bias = a.delta_bias ? a.delta_bias[c] : 0.0f;
+#pragma unroll
+        for (int o = 0; o < OWN; ++o) {
+            const int i = lane + o * LP;
+            vu[o] = size[o] = 0.0f;
+            gate[o] = 1.0f;
+            if (i >= count || i >= kStepAhead) continue;
+            const int64_t s = s0 + i;
+            vu[o] = Element<T>::load(static_cast<const T*>(a.u.data)[s * a.u.sequence + c]);
+            size[o] = Element<T>::load(static_cast<const T*>(a.delta.data)[s * a.delta.sequence + c]) + bias;
+            if (a.softplus) size[o] = softplus(size[o]);
+            if (a.z.data) {
+                const float w = Element<T>::load(static_cast<const T*>(a.z.data)[s * a.z.sequence + c]);
+                gate[o] = w * sigmoid(w);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < TIMES; ++k) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) rate[k].v[v] *= kLog2E;
+        }
+        float sum[kStepAhead];
+#pragma unroll
+        for (int i = 0; i < kStepAhead; ++i) {
+            sum[i] = 0.0f;
+            // (the lanes of a channel are neighbours in a warp: width LP)
+            const float by = __shfl_sync(0xffffffffu, size[i / LP < OWN ? i / LP : 0], i % LP, LP);
+            const float in = by * __shfl_sync(0xffffffffu, vu[i / LP < OWN ? i / LP : 0], i % LP, LP);
+            if (i >= count) continue;
+            const bool cut = q.reset != nullptr && q.reset[(s0 + i) * q.reset_sequence] != 0;
+#pragma unroll
+            for (int k = 0; k < TIMES; ++k) {
+                const int n = n0 + k * LP * V;
+                if (n >= a.states) continue;
+                const Pack<float, V> b = load_pack<float, V>(&bc[i][0][n]), cc = load_pack<float, V>(&bc[i][1][n]);
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    const float from = cut ? 0.0f : h[i][k].v[v];
+                    h[i][k].v[v] = fmaf(power_of_two(by * rate[k].v[v]), from, in * b.v[v]);
+                    sum[i] = fmaf(h[i][k].v[v], cc.v[v], sum[i]);
+                }
+                if (mine) *reinterpret_cast<Pack<float, V>*>(state + ((s0 + i) * channels + c) * a.states + n) = h[i][k];
+            }
+        }
+#pragma unroll
+        for (int o = LP / 2; o >= 1; o >>= 1) {
+#pragma unroll
+            for (int i = 0; i < kStepAhead; ++i) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], o);
+        }
+#pragma unroll
+        for (int o = 0; o < OWN; ++o) {
+            const int i = lane + o * LP;
+            float y = sum[0];
+#pragma unroll
+            for (int k = 1; k < kStepAhead; ++k) y = i == k ? sum[k] : y;
+            if (mine && i < count && i < kStepAhead) {
+                static_cast<T*>(a.y.data)[(s0 + i) * a.y.sequence + c] = Element<T>::store(fmaf(skip, vu[o], y) * gate[o]);
+            }
+        }
     }
 }
 
@@ -1005,12 +997,12 @@ struct ForwardPlan {
     int channels, group_blocks, chunks, chunk;
     int64_t blocks;
     ForwardPlan(const t8b_sequences_t& q, int64_t groups, int64_t states) {
-        channels = kForwardThreads * 2 * kHeld / padded(states);
+        channels = kThreads * kHeld / padded(states);
         group_blocks = static_cast<int>((q.channels / groups + channels - 1) / channels);
         const int64_t per_chunk = q.sequences * groups * group_blocks, steps = std::max<int64_t>(q.steps, 1);
         // cut where fewer than two blocks an SM would run; cutting takes every exponential twice
         int64_t want = 1;
-        if (per_chunk < 4 * kSms) want = std::max<int64_t>(1, std::min<int64_t>(8 * kSms / std::max<int64_t>(per_chunk, 1), steps / 32));
+        if (per_chunk < 3 * kSms) want = std::max<int64_t>(1, std::min<int64_t>(6 * kSms / std::max<int64_t>(per_chunk, 1), steps / 32));
         if (want < 3) want = 1;
         chunk = static_cast<int>(round_up((steps + want - 1) / want, kTile));
         chunks = static_cast<int>((steps + chunk - 1) / chunk);
@@ -1053,10 +1045,10 @@ void launch_forward(const Call& given, const ForwardPlan& plan, int64_t states, 
     auto go = [&](auto main, auto ends) {
         const unsigned grid = static_cast<unsigned>(plan.blocks);
         if (a.chunks > 1) {
-            launch_chain("k_scan_ends", ends, grid, kForwardThreads, 0, stream, true, a);
+            launch_chain("k_scan_ends", ends, grid, kThreads, 0, stream, true, a);
             launch_chain("k_scan_join", k_scan_join, blocks(a.q.sequences * states * a.q.channels, 256), 256, 0, stream, true, a, false);
         }
-        launch_chain("k_scan_forward", main, grid, kForwardThreads, 0, stream, true, a);
+        launch_chain("k_scan_forward", main, grid, kThreads, 0, stream, true, a);
     };
     switch (padded(states)) {
         case 16: go(k_scan_forward<T, 1, false>, k_scan_forward<T, 1, true>); break;
@@ -1100,14 +1092,35 @@ void launch_backward(const Call& given, const BackwardPlan& plan, float* da, flo
 }
 
 template <typename T>
-void launch_step(const Call& a, float* state, bool wide, cudaStream_t stream) {
+void launch_step(const Call& given, float* state, bool wide, cudaStream_t stream) {
+    Call a = given;
     const int packs = wide ? a.states / 4 : a.states;
     int lanes = 1;
     while (lanes < packs && lanes < 32) lanes *= 2;
-    const int64_t turns = (a.q.sequences + kStepAhead - 1) / kStepAhead;
-    const int64_t grid = (turns * a.q.channels * lanes + 255) / 256;
+    const int64_t turns = (a.q.sequences + kStepAhead - 1) / kStepAhead, tiles = (a.per + kStepThreads / lanes - 1) / (kStepThreads / lanes);
+    // as many blocks as are resident at once, four an SM, where the sequences alone do not make them
+    a.splits = static_cast<int>(std::max<int64_t>(1, std::min(tiles, 4 * kSms / std::max<int64_t>(1, turns * a.groups))));
+    const int64_t grid = turns * a.groups * a.splits;
     if (grid > std::numeric_limits<int32_t>::max()) raise(T8B_EINVAL, "selective scan step: too many elements for one call");
-    launch_chain("k_scan_step", wide ? k_scan_step<T, 4> : k_scan_step<T, 1>, static_cast<unsigned>(grid), 256, 0, stream, true, a, state, lanes);
+    auto go = [&](auto kernel) { launch_chain("k_scan_step", kernel, static_cast<unsigned>(grid), kStepThreads, 0, stream, true, a, state); };
+    if (wide) {
+        switch (lanes) {
+            case 1: go(k_scan_step<T, 4, 1>); break;
+            case 2: go(k_scan_step<T, 4, 2>); break;
+            case 4: go(k_scan_step<T, 4, 4>); break;
+            case 8: go(k_scan_step<T, 4, 8>); break;
+            default: go(k_scan_step<T, 4, 16>); break;
+        }
+    } else {
+        switch (lanes) {
+            case 1: go(k_scan_step<T, 1, 1>); break;
+            case 2: go(k_scan_step<T, 1, 2>); break;
+            case 4: go(k_scan_step<T, 1, 4>); break;
+            case 8: go(k_scan_step<T, 1, 8>); break;
+            case 16: go(k_scan_step<T, 1, 16>); break;
+            default: go(k_scan_step<T, 1, 32>); break;
+        }
+    }
 }
 
 }  // namespace scan
