@@ -170,7 +170,7 @@ __device__ __forceinline__ int load_window(const Conv& a, const T* x, int64_t s,
 
 // One thread: a pack of channels, a run of steps of a sequence.
 template <typename T, int V, int K>
-__global__ void __launch_bounds__(kThreads) k_conv_forward(Conv a) {
+__global__ void __launch_bounds__(kThreads, 6) k_conv_forward(Conv a) {
     constexpr int H = (V + 1) / 2;
     __shared__ Pack<T, V> ring[2 * kGroup][kThreads];
     wait_previous();

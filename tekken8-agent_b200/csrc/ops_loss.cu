@@ -6,13 +6,13 @@
 //   slope = dloss/dlp = -r A where the unclipped term is the smaller (0 where not) + the sampled K's 1 - exp(e)
 //
 // where c gathers what is the same for a whole row. Bound by memory: logits (and a reference's) once in,
-// the gradient once out. A row of up to 1,024 logits lies in the registers of one warp. A longer one belongs to a
+// the gradient once out. A row of up to 1,024 logits lies in the registers of 8, 16 or 32 lanes, as few as hold it with 32
+// each: what a row costs beside its logits is shared by the rows of a warp (65,536 x 368, fp32, 32 lanes a row: 80 us). A longer one belongs to a
 // block that reads it twice, for its sums and for its gradient; the second read comes from L2, where
 // the rows that are worked on at once fit many times over.
-// With v = log2(e) z, M the fp32 rounding of its largest and t_i = v_i - M (one multiply-add): e_i = 2^t_i,
-// and every logarithm of a probability is ln 2 (t_i - log2(sum e)), with the same M in all of them, so that
-// its rounding cancels; lse itself is ln 2 (M + log2(sum e)), taken in 64 bits, since the ratio and
-// the divergence are differences of it.
+// With m the largest legal logit and t_i = log2(e) (z_i - m): e_i = 2^t_i, and every logarithm of a
+// probability is ln 2 t_i - ln(sum e); lse itself is m + ln(sum e), taken in 64 bits, since the ratio and the
+// divergence are differences of it.
 #include "ops_memory.cuh"
 
 namespace t8b {
@@ -21,6 +21,7 @@ namespace {
 
 constexpr int kWarps = 4;          // warps of a block that gives a row to each
 constexpr int kMostHeld = 32;      // logits of a lane there
+constexpr int kMostShort = 32 * kMostHeld;
 constexpr int kMostThreads = 512;  // threads of a block that shares a row
 
 struct Loss {
@@ -83,7 +84,7 @@ __device__ __forceinline__ double natural_log(double v) {
     return fma(static_cast<double>(k), kExactLn2, 2.0 * fma(q * square, p, q));
 }
 
-// A row's sums: M as above, total = sum e, spread = sum e t, apart = sum e (t - t of the reference); the first
+// A row's sums: m as above, total = sum e, spread = sum e t, apart = sum e (t - t of the reference); the first
 // two of the reference as far as it is needed.
 struct Sums {
     float m = -INFINITY, q_m = -INFINITY;
@@ -98,7 +99,7 @@ struct Slopes {
 // The row's outputs from its sums; every thread that calls it gets the slopes, `writes` stores.
 __device__ __forceinline__ Slopes finish(const Loss& a, int64_t row, float chosen, const Sums& s, bool writes) {
     const double log_total = natural_log(s.total);
-    const double lse = fma(static_cast<double>(s.m), kExactLn2, log_total);
+    const double lse = static_cast<double>(s.m) + log_total;
     const double lp = static_cast<double>(chosen) - lse;
     const float share = 1.0f / static_cast<float>(s.total), log_sum = static_cast<float>(log_total);
     const float entropy = static_cast<float>(log_total - static_cast<double>(kLn2 * (s.spread * share)));
@@ -113,7 +114,7 @@ __device__ __forceinline__ Slopes finish(const Loss& a, int64_t row, float chose
     out.of_apart = 0.0f;
     if (a.reference_kind == T8B_REFERENCE_LOGITS) {
         // log p_i - log q_i = ln 2 (t_i - t of q_i) - gap
-        const double gap = log_total - natural_log(s.q_total);
+        const double gap = log_total - natural_log(s.q_total);  // t has the rows' own largest logits in it
         divergence = static_cast<float>(static_cast<double>(kLn2 * (s.apart * share)) - gap);
         out.base -= a.kl * (static_cast<float>(gap) + divergence);
         out.of_apart = a.kl * kLn2;
@@ -144,6 +145,10 @@ __device__ __forceinline__ void finish_nothing(const Loss& a, int64_t row) {
         if (p) p[row] = 0.0f;
     }
 }
+__device__ __forceinline__ Two powers_of_two(const Two& v) {
+    const float2 f = v.get();
+    return Two(power_of_two(f.x), power_of_two(f.y));
+}
 template <typename T, int V>
 __device__ __forceinline__ void store_pack(T* to, const float (&v)[V]) {
     *reinterpret_cast<Pack<T, V>*>(to) = pack<T, V>(v);
@@ -157,24 +162,24 @@ __device__ __forceinline__ void add_chosen(float (&v)[V], int64_t e, int64_t act
     }
 }
 
-// One warp a row; lane l holds the packs l, l + 32, ... of V logits, PACKS of them.
-template <typename T, int V, int PACKS, bool REFERENCE>
+// LANES lanes a row; lane l holds the packs l, l + LANES, ... of V logits.
+template <typename T, int V, int LANES, int HELD, bool REFERENCE>
 __global__ void __launch_bounds__(32 * kWarps) k_policy_loss(Loss a) {
-    constexpr int HELD = V * PACKS;
+    constexpr int PACKS = HELD / V, H = HELD / 2;
     wait_previous();
     release_next();
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (row >= a.rows) return;
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * (32 * kWarps / LANES) + threadIdx.x / LANES;
+    const int lane = threadIdx.x % LANES;
+    const bool mine = at < a.rows;  // the last warp's lanes go along without a row of their own
+    const int64_t row = mine ? at : a.rows - 1;
     const T* z = static_cast<const T*>(a.logits) + row * a.logits_stride;
     const T* q = REFERENCE ? static_cast<const T*>(a.reference) + row * a.reference_stride : nullptr;
     T* g = a.gradient ? static_cast<T*>(a.gradient) + row * a.gradient_stride : nullptr;
-    float v[HELD], w[REFERENCE ? HELD : 1];
-    uint32_t bits[PACKS];
     Pack<T, V> raw[PACKS], raw_q[REFERENCE ? PACKS : 1];
+    uint32_t bits[PACKS];
 #pragma unroll
     for (int i = 0; i < PACKS; ++i) {
-        const int e = (i * 32 + lane) * V;
+        const int e = (i * LANES + lane) * V;
         bits[i] = 0;
         if (e < a.n) {  // n is a multiple of V
             raw[i] = load_pack<T, V>(z + e);
@@ -183,58 +188,49 @@ __global__ void __launch_bounds__(32 * kWarps) k_policy_loss(Loss a) {
         }
     }
     const int64_t action = a.actions[row];
-    if (!legal(a, row, action)) {
-        if (lane == 0) finish_nothing(a, row);
-        if (g == nullptr) return;
-        const float zero[V] = {};
-#pragma unroll
-        for (int i = 0; i < PACKS; ++i) {
-            const int e = (i * 32 + lane) * V;
-            if (e < a.n) store_pack<T, V>(g + e, zero);
-        }
-        return;
-    }
-    const float chosen = Element<T>::load(z[action]);
+    const bool counts = legal(a, row, action);
+    const float chosen = counts ? Element<T>::load(z[action]) : 0.0f;
     Sums s;
+    float v[HELD], w[REFERENCE ? HELD : 1];
 #pragma unroll
-    for (int i = 0; i < PACKS; ++i) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const bool in = bits[i] >> j & 1;
-            v[i * V + j] = in ? Element<T>::load(raw[i].v[j]) : -INFINITY;
-            s.m = fmaxf(s.m, v[i * V + j]);
-            if (REFERENCE) {
-                w[REFERENCE ? i * V + j : 0] = in ? Element<T>::load(raw_q[REFERENCE ? i : 0].v[j]) : -INFINITY;
-                s.q_m = fmaxf(s.q_m, w[REFERENCE ? i * V + j : 0]);
-            }
+    for (int i = 0; i < HELD; ++i) {
+        const bool in = bits[i / V] >> (i % V) & 1;
+        v[i] = in ? Element<T>::load(raw[i / V].v[i % V]) : -INFINITY;
+        s.m = fmaxf(s.m, v[i]);
+        if (REFERENCE) {
+            w[REFERENCE ? i : 0] = in ? Element<T>::load(raw_q[REFERENCE ? i / V : 0].v[i % V]) : -INFINITY;
+            s.q_m = fmaxf(s.q_m, w[REFERENCE ? i : 0]);
         }
     }
 #pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) {
+    for (int o = LANES / 2; o >= 1; o >>= 1) {
         s.m = fmaxf(s.m, __shfl_xor_sync(0xffffffffu, s.m, o));
         if (REFERENCE) s.q_m = fmaxf(s.q_m, __shfl_xor_sync(0xffffffffu, s.q_m, o));
     }
-    s.m *= kLog2E;
-    s.q_m *= kLog2E;
-    // t stays in v, t - t of the reference in w, e in p
-    float total = 0.0f, q_total = 0.0f, p[HELD];
+    // t, and t less the reference's
+    Two t[H], away[REFERENCE ? H : 1], total, q_total, spread, apart;
+    const Two scale(kLog2E, kLog2E), from(-s.m, -s.m), q_from(-s.q_m, -s.q_m);
 #pragma unroll
-    for (int i = 0; i < HELD; ++i) {
-        v[i] = max_nan(fmaf(v[i], kLog2E, -s.m), kNever);
-        p[i] = power_of_two(v[i]);
-        total += p[i];
-        s.spread = fmaf(p[i], v[i], s.spread);
+    for (int i = 0; i < H; ++i) {
+        const float2 x = ((Two(v[2 * i], v[2 * i + 1]) + from) * scale).get();
+        t[i] = Two(max_nan(x.x, kNever), max_nan(x.y, kNever));
+        const Two e = powers_of_two(t[i]);
+        total = total + e;
+        spread = multiply_add(e, t[i], spread);
         if (REFERENCE) {
-            const float t = fmaf(w[REFERENCE ? i : 0], kLog2E, -s.q_m);
-            q_total += power_of_two(t);
-            w[REFERENCE ? i : 0] = p[i] != 0.0f ? v[i] - t : 0.0f;
-            s.apart = fmaf(p[i], w[REFERENCE ? i : 0], s.apart);
+            const Two u = (Two(w[REFERENCE ? 2 * i : 0], w[REFERENCE ? 2 * i + 1 : 0]) + q_from) * scale;
+            q_total = q_total + powers_of_two(u);
+            const float2 f = e.get(), d = multiply_add(u, Two(-1.0f, -1.0f), t[i]).get();
+            away[REFERENCE ? i : 0] = Two(f.x != 0.0f ? d.x : 0.0f, f.y != 0.0f ? d.y : 0.0f);
+            apart = multiply_add(e, away[REFERENCE ? i : 0], apart);
         }
     }
-    s.total = total;
-    s.q_total = q_total;
+    s.total = total.sum();
+    s.q_total = q_total.sum();
+    s.spread = spread.sum();
+    s.apart = apart.sum();
 #pragma unroll
-    for (int o = 16; o >= 1; o >>= 1) {
+    for (int o = LANES / 2; o >= 1; o >>= 1) {
         s.total += __shfl_xor_sync(0xffffffffu, s.total, o);
         s.spread += __shfl_xor_sync(0xffffffffu, s.spread, o);
         if (REFERENCE) {
@@ -242,27 +238,43 @@ __global__ void __launch_bounds__(32 * kWarps) k_policy_loss(Loss a) {
             s.apart += __shfl_xor_sync(0xffffffffu, s.apart, o);
         }
     }
+    if (!mine) return;
+    if (!counts) {
+        if (lane == 0) finish_nothing(a, row);
+        if (g == nullptr) return;
+        const float zero[V] = {};
+#pragma unroll
+        for (int i = 0; i < PACKS; ++i) {
+            const int e = (i * LANES + lane) * V;
+            if (e < a.n) store_pack<T, V>(g + e, zero);
+        }
+        return;
+    }
     const Slopes k = finish(a, row, chosen, s, lane == 0);
     if (g == nullptr) return;
+    const Two of_t(k.of_t, k.of_t), base(k.base, k.base), of_apart(k.of_apart, k.of_apart), part(k.scale, k.scale);
+#pragma unroll
+    for (int i = 0; i < H; ++i) {
+        Two inner = multiply_add(of_t, t[i], base);
+        if (REFERENCE) inner = multiply_add(of_apart, away[REFERENCE ? i : 0], inner);
+        const float2 out = (powers_of_two(t[i]) * part * inner).get();
+        v[2 * i] = out.x;
+        v[2 * i + 1] = out.y;
+    }
 #pragma unroll
     for (int i = 0; i < PACKS; ++i) {
-        const int e = (i * 32 + lane) * V;
+        const int e = (i * LANES + lane) * V;
         if (e >= a.n) continue;
         float out[V];
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const int at = i * V + j;
-            float inner = fmaf(k.of_t, v[at], k.base);
-            if (REFERENCE) inner = fmaf(k.of_apart, w[REFERENCE ? at : 0], inner);
-            out[j] = p[at] * k.scale * inner;
-        }
+        for (int j = 0; j < V; ++j) out[j] = v[i * V + j];
         add_chosen<V>(out, e, action, k.slope);
         store_pack<T, V>(g + e, out);
     }
 }
 
-// One block a row, V consecutive logits a thread and a turn.
-template <typename T, int V, bool REFERENCE>
+// One block a row, V consecutive logits a thread and a turn. MASKED: some may not be legal.
+template <typename T, int V, bool REFERENCE, bool MASKED>
 __global__ void __launch_bounds__(kMostThreads) k_policy_loss_long(Loss a) {
     wait_previous();
     release_next();
@@ -284,64 +296,71 @@ __global__ void __launch_bounds__(kMostThreads) k_policy_loss_long(Loss a) {
         return;
     }
     const float chosen = Element<T>::load(z[action]);
+    const Two scale(kLog2E, kLog2E);
     Sums s;
-    float total = 0.0f, q_total = 0.0f;
-    // COUNT logits into the sums, which move to a new largest one first. While a thread has seen nothing but
-    // -inf its M is 0 here: every e is 0.
-    auto take = [&](auto count, const float (&v)[V], const float (&w)[V], uint32_t bits) {
+    Two total, q_total, spread, apart;  // two parts of each sum, alike in m
+    auto masked = [&](auto count, const T* from, int e, uint32_t bits, auto& x) {  // logits, -inf where they are not legal
         constexpr int COUNT = decltype(count)::value;
-        float x[COUNT], y[COUNT], m = -INFINITY, q_m = -INFINITY;
+        unpack<T, COUNT>(load_pack<T, COUNT>(from + e), x);
+        if (COUNT == 1) x[0] = Two(x[0].get().x, -INFINITY);
+        if (!MASKED) return;
 #pragma unroll
-        for (int j = 0; j < COUNT; ++j) {
-            const bool in = bits >> j & 1;
-            x[j] = in ? v[j] : -INFINITY;
-            m = fmaxf(m, x[j]);
+        for (int i = 0; i < (COUNT + 1) / 2; ++i) {
+            const float2 f = x[i].get();
+            x[i] = Two(bits >> (2 * i) & 1 ? f.x : -INFINITY, bits >> (2 * i + 1) & 1 ? f.y : -INFINITY);
+        }
+    };
+    // COUNT logits into the sums, which move to a new largest one first. While a thread has seen nothing but
+    // -inf its m is 0 here: every e is 0.
+    auto take = [&](auto count, int e) {
+        constexpr int COUNT = decltype(count)::value, H = (COUNT + 1) / 2;
+        const uint32_t bits = MASKED ? legal_bits<COUNT>(a, row, e) : 0;
+        Two x[H], y[H];
+        float m = -INFINITY, q_m = -INFINITY;
+        masked(count, z, e, bits, x);
+        if (REFERENCE) masked(count, q, e, bits, y);
+#pragma unroll
+        for (int i = 0; i < H; ++i) {
+            const float2 f = x[i].get();
+            m = fmaxf(m, fmaxf(f.x, f.y));
             if (REFERENCE) {
-                y[j] = in ? w[j] : -INFINITY;
-                q_m = fmaxf(q_m, y[j]);
+                const float2 k = y[i].get();
+                q_m = fmaxf(q_m, fmaxf(k.x, k.y));
             }
         }
-        m *= kLog2E;
-        q_m *= kLog2E;
-        if (m > s.m) {
-            const float gap = s.m - m, f = power_of_two(gap);
-            s.spread = total != 0.0f ? f * fmaf(gap, total, s.spread) : 0.0f;
-            s.apart = total != 0.0f ? f * fmaf(gap, total, s.apart) : 0.0f;
-            total *= f;
+        if (m > s.m) {  // nothing to move where nothing was summed (0 times the gap, which is -inf at first)
+            const float gap = fmaxf((s.m - m) * kLog2E, -10000.0f), f = power_of_two(gap);
+            const Two by(f, f), away(gap, gap);
+            spread = by * multiply_add(away, total, spread);
+            apart = by * multiply_add(away, total, apart);
+            total = by * total;
             s.m = m;
         }
         if (REFERENCE && q_m > s.q_m) {
-            const float gap = s.q_m - q_m;
-            s.apart = total != 0.0f ? fmaf(-gap, total, s.apart) : 0.0f;
-            q_total *= power_of_two(gap);
+            const float gap = (s.q_m - q_m) * kLog2E, f = power_of_two(gap), back = -fmaxf(gap, -10000.0f);
+            apart = multiply_add(Two(back, back), total, apart);
+            q_total = Two(f, f) * q_total;
             s.q_m = q_m;
         }
-        const float from = s.m == -INFINITY ? 0.0f : s.m, q_from = s.q_m == -INFINITY ? 0.0f : s.q_m;
+        const float from = s.m == -INFINITY ? 0.0f : -s.m, q_from = s.q_m == -INFINITY ? 0.0f : -s.q_m;
+        const Two off(from, from), q_off(q_from, q_from);
 #pragma unroll
-        for (int j = 0; j < COUNT; ++j) {
-            const float t = max_nan(fmaf(x[j], kLog2E, -from), kNever), e = power_of_two(t);
-            total += e;
-            s.spread = fmaf(e, t, s.spread);
+        for (int i = 0; i < H; ++i) {
+            const float2 f = ((x[i] + off) * scale).get();
+            const Two t(max_nan(f.x, kNever), max_nan(f.y, kNever)), p = powers_of_two(t);
+            total = total + p;
+            spread = multiply_add(p, t, spread);
             if (REFERENCE) {
-                const float u = fmaf(y[j], kLog2E, -q_from);
-                q_total += power_of_two(u);
-                s.apart = fmaf(e, e != 0.0f ? t - u : 0.0f, s.apart);
+                const Two u = (y[i] + q_off) * scale;
+                q_total = q_total + powers_of_two(u);
+                const float2 d = multiply_add(u, Two(-1.0f, -1.0f), t).get(), k = p.get();
+                apart = multiply_add(p, Two(k.x != 0.0f ? d.x : 0.0f, k.y != 0.0f ? d.y : 0.0f), apart);
             }
         }
     };
 #pragma unroll 2
-    for (int e = threadIdx.x * V; e < whole; e += step) {
-        float v[V], w[V];
-        unpack<T, V>(load_pack<T, V>(z + e), v);
-        if (REFERENCE) unpack<T, V>(load_pack<T, V>(q + e), w);
-        take(Constant<V>{}, v, w, legal_bits<V>(a, row, e));
-    }
-    for (int e = whole + threadIdx.x; e < a.n; e += blockDim.x) {
-        float v[V], w[V];
-        v[0] = Element<T>::load(z[e]);
-        w[0] = REFERENCE ? Element<T>::load(q[e]) : 0.0f;
-        take(Constant<1>{}, v, w, legal_bits<1>(a, row, e));
-    }
+    for (int e = threadIdx.x * V; e < whole; e += step) take(Constant<V>{}, e);
+    for (int e = whole + threadIdx.x; e < a.n; e += blockDim.x) take(Constant<1>{}, e);
     // the threads' sums, each moved to the row's largest logit
     float m = s.m, q_m = s.q_m;
 #pragma unroll
@@ -358,17 +377,20 @@ __global__ void __launch_bounds__(kMostThreads) k_policy_loss_long(Loss a) {
         m = fmaxf(m, most[0][i]);
         if (REFERENCE) q_m = fmaxf(q_m, most[1][i]);
     }
-    if (total != 0.0f) {
-        const float gap = s.m - m, f = power_of_two(gap);
-        s.spread = f * fmaf(gap, total, s.spread);
-        if (REFERENCE) s.apart = f * fmaf(gap - (s.q_m == -INFINITY ? -q_m : s.q_m - q_m), total, s.apart);
-        total *= f;
+    float sum = total.sum();
+    s.spread = spread.sum();
+    s.apart = apart.sum();
+    s.q_total = q_total.sum();
+    if (sum != 0.0f) {
+        const float gap = (s.m - m) * kLog2E, f = power_of_two(gap);
+        s.spread = f * fmaf(gap, sum, s.spread);
+        if (REFERENCE) s.apart = f * fmaf(gap - (s.q_m == -INFINITY ? -q_m : s.q_m - q_m) * kLog2E, sum, s.apart);
+        sum *= f;
     }
-    if (REFERENCE && q_total != 0.0f) q_total *= power_of_two(s.q_m - q_m);
+    if (REFERENCE && s.q_total != 0.0) s.q_total *= power_of_two((s.q_m - q_m) * kLog2E);
     s.m = m;
     s.q_m = q_m;
-    s.total = total;
-    s.q_total = q_total;
+    s.total = sum;
 #pragma unroll
     for (int o = 16; o >= 1; o >>= 1) {
         s.total += __shfl_xor_sync(0xffffffffu, s.total, o);
@@ -395,47 +417,62 @@ __global__ void __launch_bounds__(kMostThreads) k_policy_loss_long(Loss a) {
     }
     const Slopes k = finish(a, row, chosen, s, threadIdx.x == 0);
     if (g == nullptr) return;
-    auto slope_of = [&](float v, float w, bool in) {
-        const float t = max_nan(fmaf(in ? v : -INFINITY, kLog2E, -s.m), kNever), e = power_of_two(t);
-        float inner = fmaf(k.of_t, t, k.base);
-        if (REFERENCE) inner = fmaf(k.of_apart, e != 0.0f ? t - fmaf(w, kLog2E, -s.q_m) : 0.0f, inner);
-        return e * k.scale * inner;
+    const Two off(-s.m, -s.m), q_off(-s.q_m, -s.q_m);
+    const Two of_t(k.of_t, k.of_t), base(k.base, k.base), of_apart(k.of_apart, k.of_apart), part(k.scale, k.scale);
+    auto leave = [&](auto count, int e) {
+        constexpr int COUNT = decltype(count)::value, H = (COUNT + 1) / 2;
+        const uint32_t bits = MASKED ? legal_bits<COUNT>(a, row, e) : 0;
+        Two x[H], y[H];
+        masked(count, z, e, bits, x);
+        if (REFERENCE) masked(count, q, e, bits, y);
+        float out[2 * H];
+#pragma unroll
+        for (int i = 0; i < H; ++i) {
+            const float2 f = ((x[i] + off) * scale).get();
+            const Two t(max_nan(f.x, kNever), max_nan(f.y, kNever)), p = powers_of_two(t);
+            Two inner = multiply_add(of_t, t, base);
+            if (REFERENCE) {
+                const float2 d = multiply_add((y[i] + q_off) * scale, Two(-1.0f, -1.0f), t).get(), w = p.get();
+                inner = multiply_add(of_apart, Two(w.x != 0.0f ? d.x : 0.0f, w.y != 0.0f ? d.y : 0.0f), inner);
+            }
+            const float2 d = (p * part * inner).get();
+            out[2 * i] = d.x;
+            out[2 * i + 1] = d.y;
+        }
+        float kept[COUNT];
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) kept[i] = out[i];
+        add_chosen<COUNT>(kept, e, action, k.slope);
+        store_pack<T, COUNT>(g + e, kept);
     };
 #pragma unroll 2
-    for (int e = threadIdx.x * V; e < whole; e += step) {
-        float v[V], w[V];
-        unpack<T, V>(load_pack<T, V>(z + e), v);
-        if (REFERENCE) unpack<T, V>(load_pack<T, V>(q + e), w);
-        const uint32_t bits = legal_bits<V>(a, row, e);
-#pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = slope_of(v[j], REFERENCE ? w[j] : 0.0f, bits >> j & 1);
-        add_chosen<V>(v, e, action, k.slope);
-        store_pack<T, V>(g + e, v);
-    }
-    for (int e = whole + threadIdx.x; e < a.n; e += blockDim.x) {
-        const float v = slope_of(Element<T>::load(z[e]), REFERENCE ? Element<T>::load(q[e]) : 0.0f, legal_bits<1>(a, row, e) & 1);
-        g[e] = Element<T>::store(v + (e == action ? k.slope : 0.0f));
-    }
+    for (int e = threadIdx.x * V; e < whole; e += step) leave(Constant<V>{}, e);
+    for (int e = whole + threadIdx.x; e < a.n; e += blockDim.x) leave(Constant<1>{}, e);
 }
 
 // ------------------------------------------------------------------ dispatch
+template <typename T, int V, bool REFERENCE, int LANES, int HELD>
+void launch_short(const Loss& a, cudaStream_t stream) {
+    launch_chain("k_policy_loss", k_policy_loss<T, V, LANES, HELD, REFERENCE>, blocks(a.rows, 32 * kWarps / LANES), 32 * kWarps, 0, stream, true, a);
+}
 template <typename T, int V, bool REFERENCE>
 void launch_loss(const Loss& a, cudaStream_t stream) {
-    if (a.n <= 32 * kMostHeld && a.n % V == 0) {
-        // as many packs a lane as hold the row, rounded up to what is built
-        const int packs = static_cast<int>((a.n + 32 * V - 1) / (32 * V));
-        constexpr int MOST = kMostHeld / V;  // 32, 8 or 4
-        auto kernel = k_policy_loss<T, V, MOST, REFERENCE>;
-        if (packs <= 1) kernel = k_policy_loss<T, V, 1, REFERENCE>;
-        else if (packs <= 2) kernel = k_policy_loss<T, V, 2, REFERENCE>;
-        else if (packs <= 3) kernel = k_policy_loss<T, V, 3, REFERENCE>;
-        else if (packs <= 4) kernel = k_policy_loss<T, V, 4, REFERENCE>;
-        else if (V == 1 && packs <= 12) kernel = k_policy_loss<T, V, V == 1 ? 12 : MOST, REFERENCE>;
-        launch_chain("k_policy_loss", kernel, blocks(a.rows, kWarps), 32 * kWarps, 0, stream, true, a);
-        return;
+    if (a.n <= kMostShort && a.n % V == 0) {
+        // as few lanes as hold the row, and as few logits a lane, in steps of 8
+        const int lanes = a.n <= 8 * kMostHeld ? 8 : a.n <= 16 * kMostHeld ? 16 : 32;
+        const int held = static_cast<int>(round_up((a.n + lanes - 1) / lanes, 8));
+        if (lanes == 8 && held <= 8) return launch_short<T, V, REFERENCE, 8, 8>(a, stream);
+        if (lanes == 8 && held <= 16) return launch_short<T, V, REFERENCE, 8, 16>(a, stream);
+        if (lanes == 8 && held <= 24) return launch_short<T, V, REFERENCE, 8, 24>(a, stream);
+        if (lanes == 8) return launch_short<T, V, REFERENCE, 8, 32>(a, stream);
+        if (lanes == 16 && held <= 24) return launch_short<T, V, REFERENCE, 16, 24>(a, stream);
+        if (lanes == 16) return launch_short<T, V, REFERENCE, 16, 32>(a, stream);
+        if (held <= 24) return launch_short<T, V, REFERENCE, 32, 24>(a, stream);
+        return launch_short<T, V, REFERENCE, 32, 32>(a, stream);
     }
     const int threads = a.n <= 4096 ? 128 : a.n <= 16384 ? 256 : kMostThreads;
-    launch_chain("k_policy_loss_long", k_policy_loss_long<T, V, REFERENCE>, static_cast<unsigned>(a.rows), threads, 0, stream, true, a);
+    auto kernel = a.mask_kind ? k_policy_loss_long<T, V, REFERENCE, true> : k_policy_loss_long<T, V, REFERENCE, false>;
+    launch_chain("k_policy_loss_long", kernel, static_cast<unsigned>(a.rows), threads, 0, stream, true, a);
 }
 
 }  // namespace

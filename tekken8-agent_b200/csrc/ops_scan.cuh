@@ -27,6 +27,7 @@ namespace scan {
 
 constexpr int kThreads = 128;
 constexpr int kTile = 8;  // steps between two kept states, and of a tile
+constexpr int kHalf = 4;  // steps whose states a thread of the backward pass holds at once
 constexpr int kSms = 148;
 constexpr int kMostStates = 64;
 constexpr int kHeld = 16;            // states of a channel that one of its threads holds
@@ -436,7 +437,7 @@ struct Backward {
     static constexpr int CB = (kThreads / 32) * LC * 2;      // channels of a block
     static constexpr int EV = kTile * CB / kThreads;         // channels of a thread's elementwise part: 4, 2 or 1
     static constexpr int PARTS = LC * (kThreads / 32);       // pairs of channels, and partial sums of a state
-    static constexpr int SPLIT = PARTS > 16 ? 2 : 1;         // threads that add up four states' partial sums
+    static constexpr int SPLIT = kThreads / (kHalf * 2 * LN);  // threads that add up four states' partial sums
     // Where pair p's sums of lane `along` lie: rows are rotated, so that neither the threads that write
     // them nor those that add them up meet in a bank.
     __device__ __forceinline__ static int channel_at(int p, int along) { return (p + LC * along) % (CB / 2); }
@@ -445,9 +446,12 @@ struct Backward {
         Pack<T, EV> rows[4][kThreads];                           // u, delta, dy and z of a tile: each thread writes and reads its own
         float2 before[4][kThreads];                              // the states before it: the same
         float size[kTile][CB], in[kTile][CB], given[kTile][CB];  // D, D u, gs
+        float slope[kTile][CB], zslope[kTile][CB];               // softplus'(v), dy silu'(z)
+        float bias[CB], skip[CB];
         float2 b[kTile][NP], c[kTile][NP];                       // each value twice: an operand of packed arithmetic
-        float2 channel_sums[kTile][3][LN][CB / 2];               // sum_n: C h, B g, a e h g, of each lane along the states
-        float4 state_sums[kTile][2][LN][PARTS];                  // sum_c: D u g, gs h, of each pair of channels
+        // of half a tile
+        float2 channel_sums[kHalf][3][LN][CB / 2];               // sum_n: C h, B g, a e h g, of each lane along the states
+        float4 state_sums[kHalf][2][LN][PARTS];                  // sum_c: D u g, gs h, of each pair of channels
     };
 };
 
@@ -461,7 +465,7 @@ __device__ __forceinline__ void twice(const float2* from, Two (&v)[4]) {
 }
 
 template <typename T, int LN>
-__global__ void __launch_bounds__(kThreads, 3) k_scan_backward(Call a) {
+__global__ void __launch_bounds__(kThreads, 4) k_scan_backward(Call a) {
     using Shape = Backward<T, LN>;
     constexpr int NP = Shape::NP, LC = Shape::LC, CB = Shape::CB, EV = Shape::EV, PARTS = Shape::PARTS;
     constexpr int ROW = CB / EV;  // threads of a row of the elementwise part: kThreads / ROW = kTile
@@ -492,6 +496,12 @@ __global__ void __launch_bounds__(kThreads, 3) k_scan_backward(Call a) {
         }
         rate[n] = two(r);
     }
+    for (int i = threadIdx.x; i < CB; i += kThreads) {
+        const bool in = part * CB + i < a.per;
+        m.bias[i] = in && a.delta_bias ? a.delta_bias[group * a.per + part * CB + i] : 0.0f;
+        m.skip[i] = in && a.d ? a.d[group * a.per + part * CB + i] : 0.0f;
+    }
+    __syncthreads();
     float dd[EV] = {}, dbias[EV] = {};
     float* partial = a.partial + static_cast<int64_t>(blockIdx.y) * (a.states + 2) * channels;
     // this worker's sums of da so far: kept apart from a few tiles' sums, which are added to them
@@ -597,15 +607,15 @@ __global__ void __launch_bounds__(kThreads, 3) k_scan_backward(Call a) {
             copies_wait<0>();
             // ---- elementwise: D, D u and gs of the tile into shared memory
             const Pack<T, EV> raw_u = m.rows[0][threadIdx.x];
-            float slope[EV], zslope[EV];
             {
+                float slope[EV], zslope[EV];
                 const bool live = t + es < end;
                 const Pack<T, EV> raw_delta = m.rows[1][threadIdx.x], raw_dy = m.rows[2][threadIdx.x];
                 const Pack<T, EV> raw_z = gate ? m.rows[3][threadIdx.x] : raw_u;
                 float size[EV], in[EV], given[EV];
 #pragma unroll
                 for (int i = 0; i < EV; ++i) {
-                    size[i] = Element<T>::load(raw_delta.v[i]) + (a.delta_bias ? a.delta_bias[ec + (i < ecount ? i : 0)] : 0.0f);
+                    size[i] = Element<T>::load(raw_delta.v[i]) + m.bias[el + i];
                     slope[i] = 1.0f;
                     if (a.softplus) size[i] = softplus(size[i], slope[i]);
                     in[i] = size[i] * Element<T>::load(raw_u.v[i]);
@@ -625,6 +635,8 @@ __global__ void __launch_bounds__(kThreads, 3) k_scan_backward(Call a) {
                 *reinterpret_cast<Pack<float, EV>*>(&m.size[es][el]) = pack<float, EV>(size);
                 *reinterpret_cast<Pack<float, EV>*>(&m.in[es][el]) = pack<float, EV>(in);
                 *reinterpret_cast<Pack<float, EV>*>(&m.given[es][el]) = pack<float, EV>(given);
+                *reinterpret_cast<Pack<float, EV>*>(&m.slope[es][el]) = pack<float, EV>(slope);
+                *reinterpret_cast<Pack<float, EV>*>(&m.zslope[es][el]) = pack<float, EV>(zslope);
             }
 #pragma unroll
             for (int i = 0; i < PER; ++i) {
@@ -638,80 +650,97 @@ __global__ void __launch_bounds__(kThreads, 3) k_scan_backward(Call a) {
                 fetch(t - kTile);
                 fetch_flag(t - kTile);
             }
-            // ---- h through the tile, then g back
-            auto pass = [&](auto cuts) {
-                constexpr bool CUTS = decltype(cuts)::value != 0;  // most tiles have no reset
-                Two h[kTile][4];
+            // ---- h through half a tile, then g back through it: the later half first. The state between the halves
+            // is computed on the way, its way there again for the earlier half.
+            Two between[4];
+            auto state_of = [&](int i, const Two (&from)[4], Two (&to)[4]) {
+                in_order();
+                const Two by = two(*reinterpret_cast<const float2*>(&m.size[i][2 * pair]));
+                const Two in = two(*reinterpret_cast<const float2*>(&m.in[i][2 * pair]));
+                Two bn[4], e[4];
+                twice(&m.b[i][n0], bn);
 #pragma unroll
-                for (int i = 0; i < kTile; ++i) {
-                    in_order();
-                    const Two by = two(*reinterpret_cast<const float2*>(&m.size[i][2 * pair]));
-                    const Two in = two(*reinterpret_cast<const float2*>(&m.in[i][2 * pair]));
-                    Two bn[4];
-                    twice(&m.b[i][n0], bn);
-                    const bool on = !CUTS || (resets >> i & 1) == 0;
-#pragma unroll
-                    for (int n = 0; n < 4; ++n) {
-                        h[i][n] = in * bn[n];
-                        const Two from = i ? h[i ? i - 1 : 0][n] : two(m.before[n][threadIdx.x]);
-                        const Two e = powers_of_two(by * rate[n]);
-                        if (on) h[i][n] = multiply_add(e, from, h[i][n]);
-                    }
+                for (int n = 0; n < 4; ++n) {
+                    bn[n] = in * bn[n];
+                    e[n] = powers_of_two(by * rate[n]);
                 }
 #pragma unroll
-                for (int i = kTile - 1; i >= 0; --i) {
+                for (int n = 0; n < 4; ++n) to[n] = multiply_add(e[n], from[n], bn[n]);
+                if (resets >> i & 1) {  // (a branch that all take alike: selects would cost as much as the products)
                     in_order();
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) to[n] = bn[n];
+                }
+            };
+            auto before_tile = [&](Two (&h)[4]) {
+#pragma unroll
+                for (int n = 0; n < 4; ++n) h[n] = two(m.before[n][threadIdx.x]);
+            };
+            auto half = [&](auto which, auto&& between_passes) {
+                constexpr int FIRST = decltype(which)::value * kHalf;
+                Two h[kHalf][4];
+                if (FIRST) {
+                    state_of(FIRST, between, h[0]);
+                } else {
+                    before_tile(between);
+                    state_of(0, between, h[0]);
+                }
+#pragma unroll
+                for (int i = 1; i < kHalf; ++i) state_of(FIRST + i, h[i - 1], h[i]);
+                between_passes();
+#pragma unroll
+                for (int k = kHalf - 1; k >= 0; --k) {
+                    const int i = FIRST + k;
+                    if (k % 2) in_order();
                     const Two by = two(*reinterpret_cast<const float2*>(&m.size[i][2 * pair]));
                     const Two in = two(*reinterpret_cast<const float2*>(&m.in[i][2 * pair]));
                     const Two given = two(*reinterpret_cast<const float2*>(&m.given[i][2 * pair]));
                     Two bn[4], cn[4];
                     twice(&m.b[i][n0], bn);
                     twice(&m.c[i][n0], cn);
-                    const bool on = !CUTS || (resets >> i & 1) == 0;
-                    Two of_h, of_b, of_a;
-                    float db[4], dc[4];
+                    Two of_h, of_b, of_a, e[4];
+                        float db[4], dc[4];
 #pragma unroll
                     for (int n = 0; n < 4; ++n) {
+                        e[n] = powers_of_two(by * rate[n]);
                         g[n] = multiply_add(given, cn[n], g[n]);
-                        of_h = multiply_add(h[i][n], cn[n], of_h);
+                        of_h = multiply_add(h[k][n], cn[n], of_h);
                         of_b = multiply_add(g[n], bn[n], of_b);
                         db[n] = (in * g[n]).sum();
-                        dc[n] = (given * h[i][n]).sum();
-                        g[n] = g[n] * powers_of_two(by * rate[n]);
-                        if (!on) g[n] = Two();
-                        const Two from = i ? h[i ? i - 1 : 0][n] : two(m.before[n][threadIdx.x]);
-                        const Two through = g[n] * from;
-                        if (on) of_a = multiply_add(through, rate[n], of_a);
-                        if (on) da[n] = multiply_add(through, by, da[n]);
+                        dc[n] = (given * h[k][n]).sum();
                     }
-                    m.channel_sums[i][0][along][Shape::channel_at(pair, along)] = of_h.get();
-                    m.channel_sums[i][1][along][Shape::channel_at(pair, along)] = of_b.get();
-                    m.channel_sums[i][2][along][Shape::channel_at(pair, along)] = of_a.get();
-                    m.state_sums[i][0][along][Shape::state_at(pair, along)] = make_float4(db[0], db[1], db[2], db[3]);
-                    m.state_sums[i][1][along][Shape::state_at(pair, along)] = make_float4(dc[0], dc[1], dc[2], dc[3]);
+                    if (resets >> i & 1) {
+                        in_order();
+#pragma unroll
+                        for (int n = 0; n < 4; ++n) g[n] = Two();
+                    } else {
+#pragma unroll
+                        for (int n = 0; n < 4; ++n) {
+                            const Two from = k ? h[k ? k - 1 : 0][n] : between[n];
+                            g[n] = g[n] * e[n];
+                            const Two through = g[n] * from;
+                            of_a = multiply_add(through, rate[n], of_a);
+                            da[n] = multiply_add(through, by, da[n]);
+                        }
+                    }
+                    m.channel_sums[k][0][along][Shape::channel_at(pair, along)] = of_h.get();
+                    m.channel_sums[k][1][along][Shape::channel_at(pair, along)] = of_b.get();
+                    m.channel_sums[k][2][along][Shape::channel_at(pair, along)] = of_a.get();
+                    m.state_sums[k][0][along][Shape::state_at(pair, along)] = make_float4(db[0], db[1], db[2], db[3]);
+                    m.state_sums[k][1][along][Shape::state_at(pair, along)] = make_float4(dc[0], dc[1], dc[2], dc[3]);
                 }
             };
-            if (resets == 0) {
-                pass(Constant<0>{});
-            } else {
-                pass(Constant<1>{});
-            }
-            if (t > t0) fetch_before(t - kTile);
-            if (++since == 16 || t == t0) {
-                flush(first);
-                first = false;
-                since = 0;
-            }
-            __syncthreads();
+            auto leave = [&](auto which) {
+                constexpr int FIRST = decltype(which)::value * kHalf;
             // ---- the sums over states, and the gradients of u, delta and z
-            {
+            if (es / kHalf == FIRST / kHalf) {
                 const int at = t + es;
                 float sum[3][EV] = {};
 #pragma unroll
                 for (int k = 0; k < 3; ++k) {
 #pragma unroll
                     for (int l = 0; l < LN; ++l) {
-                        const float* from = reinterpret_cast<const float*>(m.channel_sums[es][k][l]) + 2 * Shape::channel_at(el / 2, l) + (EV == 1 ? el % 2 : 0);
+                        const float* from = reinterpret_cast<const float*>(m.channel_sums[es % kHalf][k][l]) + 2 * Shape::channel_at(el / 2, l) + (EV == 1 ? el % 2 : 0);
                         const Pack<float, EV> v = load_pack<float, EV>(from);
 #pragma unroll
                         for (int i = 0; i < EV; ++i) sum[k][i] += v.v[i];
@@ -720,13 +749,14 @@ __global__ void __launch_bounds__(kThreads, 3) k_scan_backward(Call a) {
                 if (ecount > 0 && at < t1) {
                     const bool live = at < end;
                     const Pack<float, EV> size = load_pack<float, EV>(&m.size[es][el]), given = load_pack<float, EV>(&m.given[es][el]);
+                    const Pack<float, EV> slope = load_pack<float, EV>(&m.slope[es][el]), zslope = load_pack<float, EV>(&m.zslope[es][el]);
                     float du[EV], ddelta[EV], dz[EV];
 #pragma unroll
                     for (int i = 0; i < EV; ++i) {
-                        const float vu = Element<T>::load(raw_u.v[i]), skip = a.d && i < ecount ? a.d[ec + i] : 0.0f;
+                        const float vu = Element<T>::load(raw_u.v[i]), skip = m.skip[el + i];
                         du[i] = live ? fmaf(skip, given.v[i], size.v[i] * sum[1][i]) : 0.0f;
-                        ddelta[i] = live ? fmaf(kLn2, sum[2][i], vu * sum[1][i]) * slope[i] : 0.0f;
-                        dz[i] = live ? zslope[i] * fmaf(skip, vu, sum[0][i]) : 0.0f;
+                        ddelta[i] = live ? fmaf(kLn2, sum[2][i], vu * sum[1][i]) * slope.v[i] : 0.0f;
+                        dz[i] = live ? zslope.v[i] * fmaf(skip, vu, sum[0][i]) : 0.0f;
                         dbias[i] += ddelta[i];
                         if (live) dd[i] = fmaf(given.v[i], vu, dd[i]);
                     }
@@ -747,28 +777,28 @@ __global__ void __launch_bounds__(kThreads, 3) k_scan_backward(Call a) {
                     }
                 }
             }
-            // ---- the sums over channels
+            // ---- the sums over channels: every thread has a part of four states'
             constexpr int SPLIT = Shape::SPLIT;
-            for (int e = threadIdx.x; e < kTile * 2 * LN * SPLIT; e += kThreads) {
-                const int quad = e / SPLIT, half = e % SPLIT, step = quad / (2 * LN), which = quad / LN % 2, l = quad % LN;
-                Two x, y;
+            const int quad = threadIdx.x / SPLIT, share = threadIdx.x % SPLIT, step = quad / (2 * LN), which_sum = quad / LN % 2, l = quad % LN;
+            Two x, y;
 #pragma unroll
-                for (int p = 0; p < PARTS; p += SPLIT) {
-                    const float4 v = m.state_sums[step][which][l][Shape::state_at(p + half, l)];
-                    x = x + Two(v.x, v.y);
-                    y = y + Two(v.z, v.w);
-                }
-                float2 vx = x.get(), vy = y.get();
-                if (SPLIT == 2) {  // every lane is here: kTile 2 LN SPLIT is a multiple of kThreads
-                    vx.x += __shfl_xor_sync(0xffffffffu, vx.x, 1);
-                    vx.y += __shfl_xor_sync(0xffffffffu, vx.y, 1);
-                    vy.x += __shfl_xor_sync(0xffffffffu, vy.x, 1);
-                    vy.y += __shfl_xor_sync(0xffffffffu, vy.y, 1);
-                }
-                if (half != 0 || t + step >= end || 4 * l >= a.states) continue;
+            for (int p = 0; p < PARTS; p += SPLIT) {
+                const float4 v = m.state_sums[step][which_sum][l][Shape::state_at(p + share, l)];
+                x = x + Two(v.x, v.y);
+                y = y + Two(v.z, v.w);
+            }
+            float2 vx = x.get(), vy = y.get();
+#pragma unroll
+            for (int o = SPLIT / 2; o >= 1; o >>= 1) {
+                vx.x += __shfl_xor_sync(0xffffffffu, vx.x, o);
+                vx.y += __shfl_xor_sync(0xffffffffu, vx.y, o);
+                vy.x += __shfl_xor_sync(0xffffffffu, vy.x, o);
+                vy.y += __shfl_xor_sync(0xffffffffu, vy.y, o);
+            }
+            if (share == 0 && t + FIRST + step < end && 4 * l < a.states) {
                 const float sum[4] = {vx.x, vx.y, vy.x, vy.y};
                 float* to = a.shared +
-                    ((((static_cast<int64_t>(part) * a.groups + group) * q.sequences + s) * q.steps + t + step) * 2 + which) * a.states + 4 * l;
+                    ((((static_cast<int64_t>(part) * a.groups + group) * q.sequences + s) * q.steps + t + FIRST + step) * 2 + which_sum) * a.states + 4 * l;
                 if (a.states % 4 == 0) {  // the workspace starts on 256 bytes
                     *reinterpret_cast<float4*>(to) = make_float4(sum[0], sum[1], sum[2], sum[3]);
                 } else {
@@ -778,6 +808,22 @@ __global__ void __launch_bounds__(kThreads, 3) k_scan_backward(Call a) {
                     }
                 }
             }
+            };
+            before_tile(between);
+#pragma unroll
+            for (int i = 0; i < kHalf; ++i) state_of(i, between, between);
+            half(Constant<1>{}, [] {});
+            __syncthreads();
+            leave(Constant<1>{});
+            half(Constant<0>{}, [] { __syncthreads(); });  // (what the later half left is read)
+            if (t > t0) fetch_before(t - kTile);
+            if (++since == 16 || t == t0) {
+                flush(first);
+                first = false;
+                since = 0;
+            }
+            __syncthreads();
+            leave(Constant<0>{});
         }
         // past the sequence's end
         for (int at = t0 + (end > t0 ? (end - t0 + kTile - 1) / kTile * kTile : 0) + es; at < t1; at += kTile) {
@@ -1017,7 +1063,7 @@ struct BackwardPlan {
         group_blocks = static_cast<int>((q.channels / groups + channels - 1) / channels);
         end_blocks = static_cast<int>((q.channels / groups + kThreads * 16 / padded(states) - 1) / (kThreads * 16 / padded(states)));
         const int64_t across = groups * group_blocks, steps = std::max<int64_t>(q.steps, 1);
-        const int64_t resident = std::max<int64_t>(1, 3 * kSms / across);
+        const int64_t resident = std::max<int64_t>(1, 4 * kSms / across);
         // the least time by rounds of resident blocks; a cut takes a third more work
         int64_t best = 0, want = 1;
         for (int64_t parts = 1; parts <= std::max<int64_t>(1, steps / 64); parts = parts < 8 ? parts + 1 : parts + parts / 4) {
