@@ -7,12 +7,12 @@
 //
 // where c gathers what is the same for a whole row. Bound by memory: logits (and a reference's) once in,
 // the gradient once out. A row of up to 1,024 logits lies in the registers of 8, 16 or 32 lanes, as few as hold it with 32
-// each: what a row costs beside its logits is shared by the rows of a warp (65,536 x 368, fp32, 32 lanes a row: 80 us). A longer one belongs to a
+// each: what a row costs beside its logits is shared by the rows of a warp. A longer one belongs to a
 // block that reads it twice, for its sums and for its gradient; the second read comes from L2, where
 // the rows that are worked on at once fit many times over.
 // With m the largest legal logit and t_i = log2(e) (z_i - m): e_i = 2^t_i, and every logarithm of a
-// probability is ln 2 t_i - ln(sum e); lse itself is m + ln(sum e), taken in 64 bits, since the ratio and the
-// divergence are differences of it.
+// probability is ln 2 t_i - ln(sum e), with the last taken in 64 bits, since the ratio and the divergence are
+// differences of it.
 #include "ops_memory.cuh"
 
 namespace t8b {
@@ -22,7 +22,11 @@ namespace {
 constexpr int kWarps = 4;          // warps of a block that gives a row to each
 constexpr int kMostHeld = 32;      // logits of a lane there
 constexpr int kMostShort = 32 * kMostHeld;
-constexpr int kMostThreads = 512;  // threads of a block that shares a row
+constexpr int kMostThreads = 256;  // threads of a block that shares a row
+
+// Blocks of that form that an SM is to hold: their loads wait together, and more of them hide more
+// (65,536 x 368 in fp32 with a reference, 24 logits a lane: 87 us with 4 blocks, 80 with 5, 77 with 6).
+__host__ __device__ constexpr int resident_blocks(int held) { return held <= 16 ? 8 : held <= 24 ? 6 : 4; }
 
 struct Loss {
     const void* logits;
@@ -96,15 +100,27 @@ struct Slopes {
     float scale, slope, base, of_t, of_apart;
 };
 
+// What a row has beside its logits.
+struct Scalars {
+    int64_t action = -1;
+    float old = 0.0f, advantage = 0.0f, weight = 0.0f, sampled = 0.0f;
+    __device__ __forceinline__ void load(const Loss& a, int64_t row) {
+        action = a.actions[row];
+        old = a.old[row];
+        advantage = a.advantages[row];
+        weight = a.weights ? a.weights[row] : a.even;
+        if (a.reference_kind == T8B_REFERENCE_SAMPLED) sampled = static_cast<const float*>(a.reference)[row];
+    }
+};
+
 // The row's outputs from its sums; every thread that calls it gets the slopes, `writes` stores.
-__device__ __forceinline__ Slopes finish(const Loss& a, int64_t row, float chosen, const Sums& s, bool writes) {
+__device__ __forceinline__ Slopes finish(const Loss& a, int64_t row, const Scalars& given, float chosen, const Sums& s, bool writes) {
     const double log_total = natural_log(s.total);
-    const double lse = static_cast<double>(s.m) + log_total;
-    const double lp = static_cast<double>(chosen) - lse;
+    const double lp = (static_cast<double>(chosen) - static_cast<double>(s.m)) - log_total;
     const float share = 1.0f / static_cast<float>(s.total), log_sum = static_cast<float>(log_total);
     const float entropy = static_cast<float>(log_total - static_cast<double>(kLn2 * (s.spread * share)));
-    const float advantage = a.advantages[row];
-    const float ratio = expf(static_cast<float>(lp - static_cast<double>(a.old[row])));
+    const float advantage = given.advantage;
+    const float ratio = expf(static_cast<float>(lp - static_cast<double>(given.old)));
     const float free = ratio * advantage, held = fminf(fmaxf(ratio, a.low), a.high) * advantage;
     const bool unclipped = free <= held || free != free;
     float loss = -(unclipped ? free : held), slope = unclipped ? -free : 0.0f, divergence = 0.0f;
@@ -119,7 +135,7 @@ __device__ __forceinline__ Slopes finish(const Loss& a, int64_t row, float chose
         out.base -= a.kl * (static_cast<float>(gap) + divergence);
         out.of_apart = a.kl * kLn2;
     } else if (a.reference_kind == T8B_REFERENCE_SAMPLED) {
-        const float e = static_cast<float>(static_cast<double>(static_cast<const float*>(a.reference)[row]) - lp);
+        const float e = static_cast<float>(static_cast<double>(given.sampled) - lp);
         // exp(e) - 1 - e, by its series where the difference would cancel
         const float grown = expm1f(e);
         divergence = fabsf(e) < 0.1f
@@ -135,9 +151,8 @@ __device__ __forceinline__ Slopes finish(const Loss& a, int64_t row, float chose
         if (a.entropies) a.entropies[row] = entropy;
         if (a.divergences) a.divergences[row] = divergence;
     }
-    const float weight = a.weights ? a.weights[row] : a.even;
-    out.scale = weight * share;
-    out.slope = weight * slope;
+    out.scale = given.weight * share;
+    out.slope = given.weight * slope;
     return out;
 }
 __device__ __forceinline__ void finish_nothing(const Loss& a, int64_t row) {
@@ -164,7 +179,7 @@ __device__ __forceinline__ void add_chosen(float (&v)[V], int64_t e, int64_t act
 
 // LANES lanes a row; lane l holds the packs l, l + LANES, ... of V logits.
 template <typename T, int V, int LANES, int HELD, bool REFERENCE>
-__global__ void __launch_bounds__(32 * kWarps) k_policy_loss(Loss a) {
+__global__ void __launch_bounds__(32 * kWarps, resident_blocks(HELD)) k_policy_loss(Loss a) {
     constexpr int PACKS = HELD / V, H = HELD / 2;
     wait_previous();
     release_next();
@@ -187,7 +202,9 @@ __global__ void __launch_bounds__(32 * kWarps) k_policy_loss(Loss a) {
             bits[i] = legal_bits<V>(a, row, e);
         }
     }
-    const int64_t action = a.actions[row];
+    Scalars scalars;
+    scalars.load(a, row);
+    const int64_t action = scalars.action;
     const bool counts = legal(a, row, action);
     const float chosen = counts ? Element<T>::load(z[action]) : 0.0f;
     Sums s;
@@ -250,7 +267,7 @@ __global__ void __launch_bounds__(32 * kWarps) k_policy_loss(Loss a) {
         }
         return;
     }
-    const Slopes k = finish(a, row, chosen, s, lane == 0);
+    const Slopes k = finish(a, row, scalars, chosen, s, lane == 0);
     if (g == nullptr) return;
     const Two of_t(k.of_t, k.of_t), base(k.base, k.base), of_apart(k.of_apart, k.of_apart), part(k.scale, k.scale);
 #pragma unroll
@@ -273,9 +290,16 @@ __global__ void __launch_bounds__(32 * kWarps) k_policy_loss(Loss a) {
     }
 }
 
+// What a new largest logit adds to every t, far enough down for 2^gap to be 0 where the old one was -inf or the lowest
+// value; and what the reference's adds to t less its t, where it had one before.
+__device__ __forceinline__ float gap_of(float m, float next) { return fmaxf((m - next) * kLog2E, -10000.0f); }
+__device__ __forceinline__ float back_of(float m, float next) {
+    return m == -INFINITY ? 0.0f : fminf((next - m) * kLog2E, 3.402823466e38f);
+}
+
 // One block a row, V consecutive logits a thread and a turn. MASKED: some may not be legal.
 template <typename T, int V, bool REFERENCE, bool MASKED>
-__global__ void __launch_bounds__(kMostThreads) k_policy_loss_long(Loss a) {
+__global__ void __launch_bounds__(kMostThreads, REFERENCE ? 4 : 5) k_policy_loss_long(Loss a) {
     wait_previous();
     release_next();
     __shared__ float most[2][kMostThreads / 32], sums[2][kMostThreads / 32];
@@ -285,7 +309,9 @@ __global__ void __launch_bounds__(kMostThreads) k_policy_loss_long(Loss a) {
     const T* z = static_cast<const T*>(a.logits) + row * a.logits_stride;
     const T* q = REFERENCE ? static_cast<const T*>(a.reference) + row * a.reference_stride : nullptr;
     T* g = a.gradient ? static_cast<T*>(a.gradient) + row * a.gradient_stride : nullptr;
-    const int64_t action = a.actions[row];
+    Scalars scalars;
+    scalars.load(a, row);
+    const int64_t action = scalars.action;
     const int whole = a.n / V * V, step = blockDim.x * V;
     if (!legal(a, row, action)) {
         if (threadIdx.x == 0) finish_nothing(a, row);
@@ -303,11 +329,12 @@ __global__ void __launch_bounds__(kMostThreads) k_policy_loss_long(Loss a) {
         constexpr int COUNT = decltype(count)::value;
         unpack<T, COUNT>(load_pack<T, COUNT>(from + e), x);
         if (COUNT == 1) x[0] = Two(x[0].get().x, -INFINITY);
-        if (!MASKED) return;
+        if constexpr (MASKED) {
 #pragma unroll
-        for (int i = 0; i < (COUNT + 1) / 2; ++i) {
-            const float2 f = x[i].get();
-            x[i] = Two(bits >> (2 * i) & 1 ? f.x : -INFINITY, bits >> (2 * i + 1) & 1 ? f.y : -INFINITY);
+            for (int i = 0; i < (COUNT + 1) / 2; ++i) {
+                const float2 f = x[i].get();
+                x[i] = Two(bits >> (2 * i) & 1 ? f.x : -INFINITY, bits >> (2 * i + 1) & 1 ? f.y : -INFINITY);
+            }
         }
     };
     // COUNT logits into the sums, which move to a new largest one first. While a thread has seen nothing but
@@ -328,16 +355,16 @@ __global__ void __launch_bounds__(kMostThreads) k_policy_loss_long(Loss a) {
                 q_m = fmaxf(q_m, fmaxf(k.x, k.y));
             }
         }
-        if (m > s.m) {  // nothing to move where nothing was summed (0 times the gap, which is -inf at first)
-            const float gap = fmaxf((s.m - m) * kLog2E, -10000.0f), f = power_of_two(gap);
+        if (m > s.m) {
+            const float gap = gap_of(s.m, m), f = power_of_two(gap);
             const Two by(f, f), away(gap, gap);
-            spread = by * multiply_add(away, total, spread);
-            apart = by * multiply_add(away, total, apart);
+            spread = f == 0.0f ? Two() : by * multiply_add(away, total, spread);
+            apart = f == 0.0f ? Two() : by * multiply_add(away, total, apart);
             total = by * total;
             s.m = m;
         }
         if (REFERENCE && q_m > s.q_m) {
-            const float gap = (s.q_m - q_m) * kLog2E, f = power_of_two(gap), back = -fmaxf(gap, -10000.0f);
+            const float back = back_of(s.q_m, q_m), f = power_of_two(gap_of(s.q_m, q_m));
             apart = multiply_add(Two(back, back), total, apart);
             q_total = Two(f, f) * q_total;
             s.q_m = q_m;
@@ -358,7 +385,7 @@ __global__ void __launch_bounds__(kMostThreads) k_policy_loss_long(Loss a) {
             }
         }
     };
-#pragma unroll 2
+#pragma unroll 4
     for (int e = threadIdx.x * V; e < whole; e += step) take(Constant<V>{}, e);
     for (int e = whole + threadIdx.x; e < a.n; e += blockDim.x) take(Constant<1>{}, e);
     // the threads' sums, each moved to the row's largest logit
@@ -382,12 +409,12 @@ __global__ void __launch_bounds__(kMostThreads) k_policy_loss_long(Loss a) {
     s.apart = apart.sum();
     s.q_total = q_total.sum();
     if (sum != 0.0f) {
-        const float gap = (s.m - m) * kLog2E, f = power_of_two(gap);
-        s.spread = f * fmaf(gap, sum, s.spread);
-        if (REFERENCE) s.apart = f * fmaf(gap - (s.q_m == -INFINITY ? -q_m : s.q_m - q_m) * kLog2E, sum, s.apart);
+        const float gap = gap_of(s.m, m), f = power_of_two(gap);
+        s.spread = f == 0.0f ? 0.0f : f * fmaf(gap, sum, s.spread);
+        if (REFERENCE) s.apart = f == 0.0f ? 0.0f : f * fmaf(gap + back_of(s.q_m, q_m), sum, s.apart);
         sum *= f;
     }
-    if (REFERENCE && s.q_total != 0.0) s.q_total *= power_of_two((s.q_m - q_m) * kLog2E);
+    if (REFERENCE && s.q_total != 0.0) s.q_total *= power_of_two(gap_of(s.q_m, q_m));
     s.m = m;
     s.q_m = q_m;
     s.total = sum;
@@ -415,7 +442,7 @@ __global__ void __launch_bounds__(kMostThreads) k_policy_loss_long(Loss a) {
         s.spread += sums[0][i];
         s.apart += sums[1][i];
     }
-    const Slopes k = finish(a, row, chosen, s, threadIdx.x == 0);
+    const Slopes k = finish(a, row, scalars, chosen, s, threadIdx.x == 0);
     if (g == nullptr) return;
     const Two off(-s.m, -s.m), q_off(-s.q_m, -s.q_m);
     const Two of_t(k.of_t, k.of_t), base(k.base, k.base), of_apart(k.of_apart, k.of_apart), part(k.scale, k.scale);
@@ -445,7 +472,7 @@ __global__ void __launch_bounds__(kMostThreads) k_policy_loss_long(Loss a) {
         add_chosen<COUNT>(kept, e, action, k.slope);
         store_pack<T, COUNT>(g + e, kept);
     };
-#pragma unroll 2
+#pragma unroll 4
     for (int e = threadIdx.x * V; e < whole; e += step) leave(Constant<V>{}, e);
     for (int e = whole + threadIdx.x; e < a.n; e += blockDim.x) leave(Constant<1>{}, e);
 }
@@ -470,7 +497,7 @@ void launch_loss(const Loss& a, cudaStream_t stream) {
         if (held <= 24) return launch_short<T, V, REFERENCE, 32, 24>(a, stream);
         return launch_short<T, V, REFERENCE, 32, 32>(a, stream);
     }
-    const int threads = a.n <= 4096 ? 128 : a.n <= 16384 ? 256 : kMostThreads;
+    const int threads = a.n <= 4096 ? 128 : kMostThreads;
     auto kernel = a.mask_kind ? k_policy_loss_long<T, V, REFERENCE, true> : k_policy_loss_long<T, V, REFERENCE, false>;
     launch_chain("k_policy_loss_long", kernel, static_cast<unsigned>(a.rows), threads, 0, stream, true, a);
 }

@@ -163,7 +163,6 @@ __global__ void __launch_bounds__(kThreads, 5) k_scan_forward(Call a) {
 #pragma unroll
             for (int k = 0; k < 3; ++k) {
                 if (k == 2 && !gate) continue;
-#pragma unroll
                 for (int e = threadIdx.x; e < kTile * PACKS; e += kThreads) {
                     const int i = e / PACKS, at = e % PACKS * V;
                     if (t + i < end && at < width) copy_async<16>(&rows[buffer][k][i][at], row_of(k == 0 ? a.u : k == 1 ? a.delta : a.z, t + i) + at);

@@ -166,7 +166,13 @@ def loss64(logits, actions, old, advantages, legal=None, reference=None, sampled
     counts = inside & legal.gather(1, at)[:, 0]
     zero, never = torch.zeros((), dtype=torch.float64, device=z.device), torch.tensor(-float("inf"), dtype=torch.float64, device=z.device)
     zm = torch.where(legal, z, never)
-    logp = zm - torch.logsumexp(zm, 1, keepdim=True)
+
+
+    def log_softmax(v):  # from the largest: beside one of 1e38 the logarithm of a sum is lost even in 64 bits
+        v = v - v.amax(1, keepdim=True)
+        return v - torch.log(torch.exp(v).sum(1, keepdim=True))
+
+    logp = log_softmax(zm)
     p = torch.where(legal, logp.exp(), zero)
     some = p > 0
     lp = logp.gather(1, at)[:, 0]
@@ -179,7 +185,7 @@ def loss64(logits, actions, old, advantages, legal=None, reference=None, sampled
     apart = torch.zeros_like(p)
     if reference is not None:
         q = torch.where(legal, reference.double(), never)
-        apart = torch.where(some, logp - (q - torch.logsumexp(q, 1, keepdim=True)), zero)
+        apart = torch.where(some, logp - log_softmax(q), zero)
         k = torch.where(some, p * apart, zero).sum(1)
     if sampled is not None:
         e = sampled.double() - lp
