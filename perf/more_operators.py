@@ -432,6 +432,11 @@ def _own(s):
     common.update(state=s["state"], lengths=lengths)
     if case["way"] == "fwd":
         y, state = ops.selective_scan(*operands, final=True, **common)
+        if reset is not None and lengths is not None:
+            # a round that begins behind a record's end leaves it nothing, by the definition here: the operator does
+            # not look behind the end
+            behind = torch.arange(case["steps"], device=state.device) >= lengths[:, None]
+            state = torch.where((reset & behind).any(1)[:, None, None], torch.zeros_like(state), state)
         return {"y": y, "state": state}
     y, saved = ops.selective_scan(*operands, save=True, **common)
     du, ddelta, da, db, dc, dd, dz, dbias, dstate = ops.selective_scan_backward(s["dy"], *operands, saved, **common)
