@@ -16,7 +16,8 @@ namespace op {
 namespace {
 
 constexpr int kThreads = 128;
-constexpr int kRun = 32;   // steps of a thread's run
+constexpr int kRun = 32;      // steps of a thread's run
+constexpr int kBackRun = 64;  // backward: the longer, the fewer steps are computed twice around its ends
 constexpr int kGroup = 4;  // rows that are taken together
 constexpr int kSms = 148;
 constexpr int kPartialRows = 16;
@@ -273,9 +274,10 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 3) k_conv_backw
         const int64_t item = min(turn + threadIdx.y, items - 1);
         const bool working = mine && turn + threadIdx.y < items;
         const int64_t run = item / q.sequences, s = item - run * q.sequences;
-        const int t0 = static_cast<int>(run) * kRun, t1 = min(q.steps, t0 + kRun), last = q.live(s), far = min(t1 + K - 1, last);
-        const uint32_t resets = resets_of(q, s, t0, far, a.lanes);
-        const uint32_t behind = resets_of(q, s, t0 + kRun, far, a.lanes);
+        const int t0 = static_cast<int>(run) * kBackRun, t1 = min(q.steps, t0 + kBackRun), last = q.live(s), far = min(t1 + K - 1, last);
+        static_assert(kBackRun == 64, "two words of resets, and one for the steps behind the run");
+        const uint64_t resets = resets_of(q, s, t0, far, a.lanes) | static_cast<uint64_t>(resets_of(q, s, t0 + 32, far, a.lanes)) << 32;
+        const uint32_t behind = resets_of(q, s, t0 + kBackRun, far, a.lanes);
         if (!working) continue;
         const T* x = static_cast<const T*>(a.x.data) + s * a.x.sequence + c;
         const T* dy = static_cast<const T*>(a.dy.data) + s * a.dy.sequence + c;
@@ -306,7 +308,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 3) k_conv_backw
                     rows_x.fetch(half);
                     rows_dy.fetch(half);
                     copies_commit();
-                    const uint32_t begins = t - t0 < 32 ? resets >> (t - t0) : behind >> (t - t0 - 32);
+                    const uint32_t begins = t - t0 < kBackRun ? static_cast<uint32_t>(resets >> (t - t0)) : behind >> (t - t0 - kBackRun);
                     auto step = [&](auto whole, int i) {
                         constexpr bool WHOLE = decltype(whole)::value != 0;  // within the run, and no reset near
                         const int at = t + i;
@@ -515,7 +517,7 @@ int lanes_of(int packs) {
     while (lanes > 1 && lanes / 2 >= packs) lanes /= 2;
     return lanes;
 }
-int64_t runs_of(int64_t steps) { return std::max<int64_t>(1, (steps + kRun - 1) / kRun); }
+int64_t runs_of(int64_t steps, int run) { return std::max<int64_t>(1, (steps + run - 1) / run); }
 
 // Consecutive channels of a thread where every row and state starts on a pack's boundary. (8 of 16 bits take fewer
 // instructions but twice the registers: 65,536 x 1,024 in bf16 forward 84 us against 72.)
@@ -566,7 +568,7 @@ extern "C" int t8b_causal_conv_forward(const t8b_sequences_t* q, int type, t8b_t
         a.final_state = final_state;
         a.parameter_type = parameter_type;
         a.activation = activation;
-        a.runs = static_cast<int>(runs_of(q->steps));
+        a.runs = static_cast<int>(runs_of(q->steps, kRun));
         with_type(type, [&](auto element) {
             using T = decltype(element);
             constexpr int V = kPack;
@@ -588,7 +590,7 @@ extern "C" int t8b_causal_conv_forward(const t8b_sequences_t* q, int type, t8b_t
 
 extern "C" size_t t8b_causal_conv_workspace(const t8b_sequences_t* q, int width) {
     if (q == nullptr || q->sequences < 1 || q->channels < 1 || q->steps < 0 || width < 2 || width > 4) return 0;
-    const int64_t items = q->sequences * runs_of(q->steps);
+    const int64_t items = q->sequences * runs_of(q->steps, kBackRun);
     const Layout wide(items, static_cast<int>((q->channels + kPack - 1) / kPack)), single(items, static_cast<int>(q->channels));
     return sizeof(float) * static_cast<size_t>(std::max(wide.workers, single.workers)) * (width + 1) * q->channels;
 }
@@ -636,7 +638,7 @@ extern "C" int t8b_causal_conv_backward(const t8b_sequences_t* q, int type, t8b_
         a.partial = parameters ? static_cast<float*>(workspace) : nullptr;
         a.parameter_type = parameter_type;
         a.activation = activation;
-        a.runs = static_cast<int>(runs_of(q->steps));
+        a.runs = static_cast<int>(runs_of(q->steps, kBackRun));
         with_type(type, [&](auto element) {
             using T = decltype(element);
             constexpr int V = kPack;
