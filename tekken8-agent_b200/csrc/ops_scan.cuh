@@ -167,14 +167,15 @@ __global__ void __launch_bounds__(kThreads, 5) k_scan_forward(Call a) {
     bool flag = false;  // whether the next tile's step threadIdx % 8 is a reset
     auto fetch = [&](int t, int buffer) {
         if (a.wide) {
-#pragma unroll
-            for (int k = 0; k < (ENDS ? 2 : 3); ++k) {
-                if (k == 2 && !gate) continue;
+            auto copy = [&](int k, const Track<void>& track) {
                 for (int e = threadIdx.x; e < kTile * PACKS; e += kThreads) {
                     const int i = e / PACKS, at = e % PACKS * V;
-                    if (t + i < end && at < width) copy_async<16>(&rows[buffer][k][i][at], row_of(k == 0 ? a.u : k == 1 ? a.delta : a.z, t + i) + at);
+                    if (t + i < end && at < width) copy_async<16>(&rows[buffer][k][i][at], row_of(track, t + i) + at);
                 }
-            }
+            };
+            copy(0, a.u);
+            copy(1, a.delta);
+            if (gate) copy(2, a.z);
         } else if (mine) {
             for (int i = lane; i < kTile; i += LN) {
                 if (t + i >= end) break;
@@ -196,11 +197,13 @@ __global__ void __launch_bounds__(kThreads, 5) k_scan_forward(Call a) {
         flag = at < end && q.resets(s, at);
     };
     auto leave = [&](int t, int buffer) {  // a finished tile's y
-        if (ENDS || !a.wide) return;
-        for (int e = threadIdx.x; e < kTile * PACKS; e += kThreads) {
-            const int i = e / PACKS, at = e % PACKS * V;
-            if (t + i < end && at < width) {
-                *reinterpret_cast<Pack<T, V>*>(row_of(a.y, t + i) + at) = *reinterpret_cast<const Pack<T, V>*>(&ys[buffer][i][at]);
+        if constexpr (!ENDS) {
+            if (!a.wide) return;
+            for (int e = threadIdx.x; e < kTile * PACKS; e += kThreads) {
+                const int i = e / PACKS, at = e % PACKS * V;
+                if (t + i < end && at < width) {
+                    *reinterpret_cast<Pack<T, V>*>(row_of(a.y, t + i) + at) = *reinterpret_cast<const Pack<T, V>*>(&ys[buffer][i][at]);
+                }
             }
         }
     };
