@@ -88,27 +88,26 @@ __device__ __forceinline__ Two slope_of(const Two& v) {
 // groups of kGroup rows, `kThreads` packs apart. Rows at and past `end` are zeros.
 template <typename T, int V>
 struct Ring {
-    Pack<T, V>* slots;
+    Held<T, V>* slots;
     const T* from;  // the next row to fetch
     int64_t step;
     int next, end;
-    __device__ __forceinline__ Ring(Pack<T, V>* slots_, const T* base, int64_t step_, int t0, int end_)
+    __device__ __forceinline__ Ring(Held<T, V>* slots_, const T* base, int64_t step_, int t0, int end_)
         : slots(slots_), from(base + t0 * step_), step(step_), next(t0), end(end_) {}
     __device__ __forceinline__ void fetch(int half) {
 #pragma unroll
         for (int i = 0; i < kGroup; ++i, ++next, from += step) {
-            Pack<T, V>* to = slots + (half * kGroup + i) * kThreads;
+            Held<T, V>* to = slots + (half * kGroup + i) * kThreads;
             if (next >= end) {
-#pragma unroll
-                for (int v = 0; v < V; ++v) to->v[v] = Element<T>::store(0.0f);
+                *to = Held<T, V>{};
             } else if constexpr (V * sizeof(T) >= 4) {
                 copy_async<V * sizeof(T)>(to, from);
             } else {
-                *to = load_pack<T, V>(from);
+                *to = load_held<T, V>(from);
             }
         }
     }
-    __device__ __forceinline__ void take(int half, Pack<T, V> (&rows)[kGroup]) const {
+    __device__ __forceinline__ void take(int half, Held<T, V> (&rows)[kGroup]) const {
 #pragma unroll
         for (int i = 0; i < kGroup; ++i) rows[i] = slots[(half * kGroup + i) * kThreads];
     }
@@ -140,16 +139,15 @@ __device__ __forceinline__ int load_window(const Conv& a, const T* x, int64_t s,
     const Sequences& q = a.q;
     int since = K;
     clear<H, K - 1>(window);
-    Pack<T, V> raw[K - 1];
+    Held<T, V> raw[K - 1];
 #pragma unroll
     for (int k = 0; k < K - 1; ++k) {
         const int t = t0 - (K - 1) + k;
-#pragma unroll
-        for (int v = 0; v < V; ++v) raw[k].v[v] = Element<T>::store(0.0f);
+        raw[k] = Held<T, V>{};
         if (t >= 0) {
-            raw[k] = load_pack<T, V>(x + t * a.x.step);
+            raw[k] = load_held<T, V>(x + t * a.x.step);
         } else if (a.state) {
-            raw[k] = load_pack<T, V>(static_cast<const T*>(a.state) + (s * (K - 1) + (K - 1 + t)) * q.channels + c);
+            raw[k] = load_held<T, V>(static_cast<const T*>(a.state) + (s * (K - 1) + (K - 1 + t)) * q.channels + c);
         }
     }
 #pragma unroll
@@ -173,7 +171,7 @@ __device__ __forceinline__ int load_window(const Conv& a, const T* x, int64_t s,
 template <typename T, int V, int K>
 __global__ void __launch_bounds__(kThreads, 6) k_conv_forward(Conv a) {
     constexpr int H = (V + 1) / 2;
-    __shared__ Pack<T, V> ring[2 * kGroup][kThreads];
+    __shared__ Held<T, V> ring[2 * kGroup][kThreads];
     wait_previous();
     release_next();
     const Sequences& q = a.q;
@@ -203,7 +201,7 @@ __global__ void __launch_bounds__(kThreads, 6) k_conv_forward(Conv a) {
         load_filter<V, K>(a, c, w, b);
         with_activation(a.activation, [&](auto act) {
             for (int half = 0; t < end; half ^= 1) {
-                Pack<T, V> now[kGroup];
+                Held<T, V> now[kGroup];
                 copies_wait<1>();
                 rows.take(half, now);
                 rows.fetch(half);
@@ -214,7 +212,7 @@ __global__ void __launch_bounds__(kThreads, 6) k_conv_forward(Conv a) {
                     filter<H, K>(w, b, window, row, p);
 #pragma unroll
                     for (int h = 0; h < H; ++h) p[h] = activate_two<decltype(act)::value>(p[h]);
-                    *reinterpret_cast<Pack<T, V>*>(y) = pack<T, V>(p);
+                    *reinterpret_cast<Held<T, V>*>(y) = pack<T, V>(p);
                     y += a.y.step;
                     shift<H, K - 1>(window, row);
                 };
@@ -238,12 +236,9 @@ __global__ void __launch_bounds__(kThreads, 6) k_conv_forward(Conv a) {
     }
     if (final_state && (none || (end > t0 && end == last))) {
 #pragma unroll
-        for (int k = 0; k < K - 1; ++k) *reinterpret_cast<Pack<T, V>*>(final_state + k * q.channels) = pack<T, V>(window[k]);
+        for (int k = 0; k < K - 1; ++k) *reinterpret_cast<Held<T, V>*>(final_state + k * q.channels) = pack<T, V>(window[k]);
     }
-    Pack<T, V> zero;
-#pragma unroll
-    for (int v = 0; v < V; ++v) zero.v[v] = Element<T>::store(0.0f);
-    for (t = max(t0, end); t < t1; ++t, y += a.y.step) *reinterpret_cast<Pack<T, V>*>(y) = zero;
+    for (t = max(t0, end); t < t1; ++t, y += a.y.step) *reinterpret_cast<Held<T, V>*>(y) = Held<T, V>{};
 }
 
 // Block (x, y): x packs of channels, y runs at a time; every thread goes through the runs that are a
@@ -254,9 +249,9 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 3) k_conv_backw
     constexpr int H = (V + 1) / 2;
     constexpr int WIDTH = (K + 1) * 2 * H + 1;
     // the ring of x and dy, and at the end the sums of the block's threads
-    constexpr int RING = 4 * kGroup * kThreads * sizeof(Pack<T, V>), SUMS = kThreads * WIDTH * sizeof(float);
+    constexpr int RING = 4 * kGroup * kThreads * sizeof(Held<T, V>), SUMS = kThreads * WIDTH * sizeof(float);
     __shared__ __align__(16) unsigned char memory[RING > SUMS ? RING : SUMS];
-    auto* ring = reinterpret_cast<Pack<T, V>*>(memory) + threadIdx.y * blockDim.x + threadIdx.x;
+    auto* ring = reinterpret_cast<Held<T, V>*>(memory) + threadIdx.y * blockDim.x + threadIdx.x;
     wait_previous();
     release_next();
     const Sequences& q = a.q;
@@ -301,7 +296,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 3) k_conv_backw
             with_activation(a.activation, [&](auto act) {
                 int half = 0;
                 for (int t = t0; t < t1 + K - 1; t += kGroup, half ^= 1) {
-                    Pack<T, V> now_x[kGroup], now_dy[kGroup];
+                    Held<T, V> now_x[kGroup], now_dy[kGroup];
                     copies_wait<1>();
                     rows_x.take(half, now_x);
                     rows_dy.take(half, now_dy);
@@ -349,16 +344,16 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 3) k_conv_backw
                             for (int j = 0; j < K - 1; ++j) {
                                 if (since < j) continue;
                                 Two v[H];
-                                unpack<T, V>(load_pack<T, V>(given + (K - 2 - j) * q.channels), v);
+                                unpack<T, V>(load_held<T, V>(given + (K - 2 - j) * q.channels), v);
 #pragma unroll
                                 for (int h = 0; h < H; ++h) pending[j][h] = pending[j][h] + v[h];
                             }
                         }
                         const int done = at - (K - 1);
                         if (WHOLE || (done >= t0 && done < t1)) {
-                            if (dx) *reinterpret_cast<Pack<T, V>*>(to) = pack<T, V>(pending[K - 1]);
+                            if (dx) *reinterpret_cast<Held<T, V>*>(to) = pack<T, V>(pending[K - 1]);
                         } else if (done < 0 && t0 == 0 && dstate) {
-                            *reinterpret_cast<Pack<T, V>*>(dstate + (K - 1 + done) * q.channels) = pack<T, V>(pending[K - 1]);
+                            *reinterpret_cast<Held<T, V>*>(dstate + (K - 1 + done) * q.channels) = pack<T, V>(pending[K - 1]);
                         }
                         if (dx) to += a.y.step;
                         shift<H, K - 1>(window, row);
@@ -385,12 +380,12 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 3) k_conv_backw
         if (t0 == 0 && dstate) {  // no step: the final state is the initial one
 #pragma unroll
             for (int k = 0; k < K - 1; ++k) {
-                *reinterpret_cast<Pack<T, V>*>(dstate + k * q.channels) = given ? load_pack<T, V>(given + k * q.channels) : pack<T, V>(pending[k]);
+                *reinterpret_cast<Held<T, V>*>(dstate + k * q.channels) = given ? load_held<T, V>(given + k * q.channels) : pack<T, V>(pending[k]);
             }
         }
         if (dx) {
             const Two zero[H];
-            for (int t = t0; t < t1; ++t) *reinterpret_cast<Pack<T, V>*>(dx + t * a.y.step) = pack<T, V>(zero);
+            for (int t = t0; t < t1; ++t) *reinterpret_cast<Held<T, V>*>(dx + t * a.y.step) = pack<T, V>(zero);
         }
     }
     if (a.partial == nullptr) return;
@@ -456,20 +451,17 @@ __global__ void __launch_bounds__(kThreads) k_conv_step(Conv a) {
     const int c = static_cast<int>(index - s * a.packs) * V;
     if (s >= q.sequences) return;
     T* state = static_cast<T*>(a.final_state) + s * (K - 1) * q.channels + c;
-    const Pack<T, V> raw = load_pack<T, V>(static_cast<const T*>(a.x.data) + s * a.x.sequence + c);
-    Pack<T, V> held[K - 1];
+    const Held<T, V> raw = load_held<T, V>(static_cast<const T*>(a.x.data) + s * a.x.sequence + c);
+    Held<T, V> held[K - 1];
 #pragma unroll
-    for (int k = 0; k < K - 1; ++k) held[k] = load_pack<T, V>(state + k * q.channels);
+    for (int k = 0; k < K - 1; ++k) held[k] = load_held<T, V>(state + k * q.channels);
     const bool cut = q.reset != nullptr && q.reset[s * q.reset_sequence] != 0;
     constexpr int H = (V + 1) / 2;
     Two w[K][H], p[H], row[H];
     load_filter<V, K>(a, c, w, p);
     if (cut) {
 #pragma unroll
-        for (int k = 0; k < K - 1; ++k) {
-#pragma unroll
-            for (int v = 0; v < V; ++v) held[k].v[v] = Element<T>::store(0.0f);
-        }
+        for (int k = 0; k < K - 1; ++k) held[k] = Held<T, V>{};
     }
     unpack<T, V>(raw, row);
 #pragma unroll
@@ -484,9 +476,9 @@ __global__ void __launch_bounds__(kThreads) k_conv_step(Conv a) {
 #pragma unroll
         for (int h = 0; h < H; ++h) p[h] = activate_two<decltype(act)::value>(p[h]);
     });
-    *reinterpret_cast<Pack<T, V>*>(static_cast<T*>(a.y.data) + s * a.y.sequence + c) = pack<T, V>(p);
+    *reinterpret_cast<Held<T, V>*>(static_cast<T*>(a.y.data) + s * a.y.sequence + c) = pack<T, V>(p);
 #pragma unroll
-    for (int k = 0; k < K - 1; ++k) *reinterpret_cast<Pack<T, V>*>(state + k * q.channels) = k + 1 < K - 1 ? held[k + 1 < K - 1 ? k + 1 : 0] : raw;
+    for (int k = 0; k < K - 1; ++k) *reinterpret_cast<Held<T, V>*>(state + k * q.channels) = k + 1 < K - 1 ? held[k + 1 < K - 1 ? k + 1 : 0] : raw;
 }
 
 // ------------------------------------------------------------------ dispatch

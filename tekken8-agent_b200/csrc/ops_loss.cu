@@ -166,7 +166,7 @@ __device__ __forceinline__ Two powers_of_two(const Two& v) {
 }
 template <typename T, int V>
 __device__ __forceinline__ void store_pack(T* to, const float (&v)[V]) {
-    *reinterpret_cast<Pack<T, V>*>(to) = pack<T, V>(v);
+    *reinterpret_cast<Held<T, V>*>(to) = pack<T, V>(v);
 }
 template <int V>
 __device__ __forceinline__ void add_chosen(float (&v)[V], int64_t e, int64_t action, float slope) {
@@ -190,15 +190,15 @@ __global__ void __launch_bounds__(32 * kWarps, resident_blocks(HELD)) k_policy_l
     const T* z = static_cast<const T*>(a.logits) + row * a.logits_stride;
     const T* q = REFERENCE ? static_cast<const T*>(a.reference) + row * a.reference_stride : nullptr;
     T* g = a.gradient ? static_cast<T*>(a.gradient) + row * a.gradient_stride : nullptr;
-    Pack<T, V> raw[PACKS], raw_q[REFERENCE ? PACKS : 1];
+    Held<T, V> raw[PACKS], raw_q[REFERENCE ? PACKS : 1];
     uint32_t bits[PACKS];
 #pragma unroll
     for (int i = 0; i < PACKS; ++i) {
         const int e = (i * LANES + lane) * V;
         bits[i] = 0;
         if (e < a.n) {  // n is a multiple of V
-            raw[i] = load_pack<T, V>(z + e);
-            if (REFERENCE) raw_q[REFERENCE ? i : 0] = load_pack<T, V>(q + e);
+            raw[i] = load_held<T, V>(z + e);
+            if (REFERENCE) raw_q[REFERENCE ? i : 0] = load_held<T, V>(q + e);
             bits[i] = legal_bits<V>(a, row, e);
         }
     }
@@ -210,13 +210,19 @@ __global__ void __launch_bounds__(32 * kWarps, resident_blocks(HELD)) k_policy_l
     Sums s;
     float v[HELD], w[REFERENCE ? HELD : 1];
 #pragma unroll
-    for (int i = 0; i < HELD; ++i) {
-        const bool in = bits[i / V] >> (i % V) & 1;
-        v[i] = in ? Element<T>::load(raw[i / V].v[i % V]) : -INFINITY;
-        s.m = fmaxf(s.m, v[i]);
-        if (REFERENCE) {
-            w[REFERENCE ? i : 0] = in ? Element<T>::load(raw_q[REFERENCE ? i / V : 0].v[i % V]) : -INFINITY;
-            s.q_m = fmaxf(s.q_m, w[REFERENCE ? i : 0]);
+    for (int i = 0; i < PACKS; ++i) {
+        float x[V], y[V];
+        unpack<T, V>(raw[i], x);
+        if (REFERENCE) unpack<T, V>(raw_q[REFERENCE ? i : 0], y);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const bool in = bits[i] >> j & 1;
+            v[i * V + j] = in ? x[j] : -INFINITY;
+            s.m = fmaxf(s.m, v[i * V + j]);
+            if (REFERENCE) {
+                w[REFERENCE ? i * V + j : 0] = in ? y[j] : -INFINITY;
+                s.q_m = fmaxf(s.q_m, w[REFERENCE ? i * V + j : 0]);
+            }
         }
     }
 #pragma unroll
@@ -327,7 +333,7 @@ __global__ void __launch_bounds__(kMostThreads, REFERENCE ? 4 : 5) k_policy_loss
     Two total, q_total, spread, apart;  // two parts of each sum, alike in m
     auto masked = [&](auto count, const T* from, int e, uint32_t bits, auto& x) {  // logits, -inf where they are not legal
         constexpr int COUNT = decltype(count)::value;
-        unpack<T, COUNT>(load_pack<T, COUNT>(from + e), x);
+        unpack<T, COUNT>(load_held<T, COUNT>(from + e), x);
         if (COUNT == 1) x[0] = Two(x[0].get().x, -INFINITY);
         if constexpr (MASKED) {
 #pragma unroll

@@ -3,6 +3,7 @@
 #pragma once
 
 #include <algorithm>
+#include <type_traits>
 
 #include "ops.cuh"
 
@@ -54,50 +55,63 @@ __device__ __forceinline__ void copies_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory");
 }
 
-// V consecutive elements as they lie in memory, and in fp32.
+// V consecutive elements as they lie in memory: whole words where they make one, so that no register holds half of
+// what it could (a struct of 16-bit elements is taken apart into them when it is copied).
 template <typename T, int V>
-__device__ __forceinline__ Pack<T, V> load_pack(const T* p) {
-    return *reinterpret_cast<const Pack<T, V>*>(p);
+struct alignas(sizeof(T) * V) Words {
+    uint32_t w[sizeof(T) * V / 4];
+};
+template <typename T, int V>
+using Held = std::conditional_t<(sizeof(T) * V >= 4), Words<T, V>, Pack<T, V>>;  // Held<T, V>{} are zeros
+template <typename T, int V>
+__device__ __forceinline__ Held<T, V> load_held(const T* p) {
+    return *reinterpret_cast<const Held<T, V>*>(p);
 }
 template <typename T, int V>
-__device__ __forceinline__ void unpack(const Pack<T, V>& p, float (&v)[V]) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = Element<T>::load(p.v[i]);
+__device__ __forceinline__ void store_held(T* p, const Held<T, V>& v) {
+    *reinterpret_cast<Held<T, V>*>(p) = v;
 }
+// In fp32,
 template <typename T, int V>
-__device__ __forceinline__ Pack<T, V> pack(const float (&v)[V]) {
-    Pack<T, V> p;
-    if constexpr (sizeof(T) == 2 && V % 2 == 0) {
-        uint32_t w[V / 2];
+__device__ __forceinline__ void unpack(const Held<T, V>& p, float (&v)[V]) {
+    if constexpr (sizeof(T) * V < 4) {
+        v[0] = Element<T>::load(p.v[0]);
+    } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int i = 0; i < V / 2; ++i) w[i] = Element<T>::pack(v[2 * i], v[2 * i + 1]);
-        p = *reinterpret_cast<Pack<T, V>*>(w);
+        for (int i = 0; i < V; ++i) v[i] = __uint_as_float(p.w[i]);
     } else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) p.v[i] = Element<T>::store(v[i]);
+        for (int i = 0; i < V / 2; ++i) {
+            const float2 f = Element<T>::unpack(p.w[i]);
+            v[2 * i] = f.x;
+            v[2 * i + 1] = f.y;
+        }
+    }
+}
+template <typename T, int V>
+__device__ __forceinline__ Held<T, V> pack(const float (&v)[V]) {
+    Held<T, V> p;
+    if constexpr (sizeof(T) * V < 4) {
+        p.v[0] = Element<T>::store(v[0]);
+    } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) p.w[i] = __float_as_uint(v[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) p.w[i] = Element<T>::pack(v[2 * i], v[2 * i + 1]);
     }
     return p;
 }
-
-// The same as register pairs; a single element has 0 beside it.
+// and as register pairs; a single element has 0 beside it.
 template <typename T, int V>
-__device__ __forceinline__ void unpack(const Pack<T, V>& p, Two (&v)[(V + 1) / 2]) {
-    if constexpr (V == 1) {
-        v[0] = Two(Element<T>::load(p.v[0]), 0.0f);
-    } else if constexpr (sizeof(T) == 2) {
-        const Pack<uint32_t, V / 2> w = *reinterpret_cast<const Pack<uint32_t, V / 2>*>(&p);
+__device__ __forceinline__ void unpack(const Held<T, V>& p, Two (&v)[(V + 1) / 2]) {
+    float f[V];
+    unpack<T, V>(p, f);
 #pragma unroll
-        for (int i = 0; i < V / 2; ++i) {
-            const float2 f = Element<T>::unpack(w.v[i]);
-            v[i] = Two(f.x, f.y);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < V / 2; ++i) v[i] = Two(p.v[2 * i], p.v[2 * i + 1]);
-    }
+    for (int i = 0; i < (V + 1) / 2; ++i) v[i] = Two(f[2 * i], 2 * i + 1 < V ? f[2 * i + 1 < V ? 2 * i + 1 : 0] : 0.0f);
 }
 template <typename T, int V>
-__device__ __forceinline__ Pack<T, V> pack(const Two (&v)[(V + 1) / 2]) {
+__device__ __forceinline__ Held<T, V> pack(const Two (&v)[(V + 1) / 2]) {
     float f[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {

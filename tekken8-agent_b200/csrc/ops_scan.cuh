@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(kThreads, 5) k_scan_forward(Call a) {
             for (int e = threadIdx.x; e < kTile * PACKS; e += kThreads) {
                 const int i = e / PACKS, at = e % PACKS * V;
                 if (t + i < end && at < width) {
-                    *reinterpret_cast<Pack<T, V>*>(row_of(a.y, t + i) + at) = *reinterpret_cast<const Pack<T, V>*>(&ys[buffer][i][at]);
+                    store_held<T, V>(row_of(a.y, t + i) + at, load_held<T, V>(&ys[buffer][i][at]));
                 }
             }
         }
@@ -452,7 +452,7 @@ struct Backward {
     __device__ __forceinline__ static int channel_at(int p, int along) { return (p + LC * along) % (CB / 2); }
     __device__ __forceinline__ static int state_at(int p, int along) { return (p + SPLIT * along) % PARTS; }
     struct Shared {
-        Pack<T, EV> rows[4][kThreads];                           // u, delta, dy and z of a tile: each thread writes and reads its own
+        Held<T, EV> rows[4][kThreads];                           // u, delta, dy and z of a tile: each thread writes and reads its own
         float2 before[4][kThreads];                              // the states before it: the same
         float size[kTile][CB], in[kTile][CB], given[kTile][CB];  // D, D u, gs
         float slope[kTile][CB], zslope[kTile][CB];               // softplus'(v), dy silu'(z)
@@ -542,18 +542,18 @@ __global__ void __launch_bounds__(kThreads, 4) k_scan_backward(Call a) {
             for (int k = 0; k < 4; ++k) {
                 if (k == 3 && !gate) continue;
                 const Track<void>& track = k == 0 ? a.u : k == 1 ? a.delta : k == 2 ? a.dy : a.z;
-                Pack<T, EV>* to = &m.rows[k][threadIdx.x];
+                Held<T, EV>* to = &m.rows[k][threadIdx.x];
                 if (at < end && ecount == EV && a.paired) {
                     const T* from = row_of(track, at);
                     if constexpr (EV * sizeof(T) >= 4) {
                         copy_async<EV * sizeof(T)>(to, from);
                     } else {
-                        *to = load_pack<T, EV>(from);
+                        *to = load_held<T, EV>(from);
                     }
                 } else {
                     const T* from = row_of(track, at < end ? at : 0);
 #pragma unroll
-                    for (int i = 0; i < EV; ++i) to->v[i] = at < end && i < ecount ? from[i] : Element<T>::store(0.0f);
+                    for (int i = 0; i < EV; ++i) reinterpret_cast<T*>(to)[i] = at < end && i < ecount ? from[i] : Element<T>::store(0.0f);
                 }
             }
             const T* b = static_cast<const T*>(a.b.data) + s * a.b.sequence + group * a.b_group;
@@ -615,37 +615,40 @@ __global__ void __launch_bounds__(kThreads, 4) k_scan_backward(Call a) {
         for (; end > t0 && t >= t0; t -= kTile) {
             copies_wait<0>();
             // ---- elementwise: D, D u and gs of the tile into shared memory
-            const Pack<T, EV> raw_u = m.rows[0][threadIdx.x];
+            const Held<T, EV> raw_u = m.rows[0][threadIdx.x];
             {
                 float slope[EV], zslope[EV];
                 const bool live = t + es < end;
-                const Pack<T, EV> raw_delta = m.rows[1][threadIdx.x], raw_dy = m.rows[2][threadIdx.x];
-                const Pack<T, EV> raw_z = gate ? m.rows[3][threadIdx.x] : raw_u;
+                float vu[EV], vdelta[EV], vdy[EV], vz[EV];
+                unpack<T, EV>(raw_u, vu);
+                unpack<T, EV>(m.rows[1][threadIdx.x], vdelta);
+                unpack<T, EV>(m.rows[2][threadIdx.x], vdy);
+                if (gate) unpack<T, EV>(m.rows[3][threadIdx.x], vz);
                 float size[EV], in[EV], given[EV];
 #pragma unroll
                 for (int i = 0; i < EV; ++i) {
-                    size[i] = Element<T>::load(raw_delta.v[i]) + m.bias[el + i];
+                    size[i] = vdelta[i] + m.bias[el + i];
                     slope[i] = 1.0f;
                     if (a.softplus) size[i] = softplus(size[i], slope[i]);
-                    in[i] = size[i] * Element<T>::load(raw_u.v[i]);
+                    in[i] = size[i] * vu[i];
                 }
 #pragma unroll
                 for (int i = 0; i < EV; ++i) {
-                    given[i] = Element<T>::load(raw_dy.v[i]);
+                    given[i] = vdy[i];
                     zslope[i] = 0.0f;
                     if (gate) {
                         float value;
-                        activate_slope<T8B_SILU>(Element<T>::load(raw_z.v[i]), value, zslope[i]);
+                        activate_slope<T8B_SILU>(vz[i], value, zslope[i]);
                         zslope[i] *= given[i];
                         given[i] *= value;
                     }
                     if (!live || i >= ecount) size[i] = in[i] = given[i] = 0.0f;
                 }
-                *reinterpret_cast<Pack<float, EV>*>(&m.size[es][el]) = pack<float, EV>(size);
-                *reinterpret_cast<Pack<float, EV>*>(&m.in[es][el]) = pack<float, EV>(in);
-                *reinterpret_cast<Pack<float, EV>*>(&m.given[es][el]) = pack<float, EV>(given);
-                *reinterpret_cast<Pack<float, EV>*>(&m.slope[es][el]) = pack<float, EV>(slope);
-                *reinterpret_cast<Pack<float, EV>*>(&m.zslope[es][el]) = pack<float, EV>(zslope);
+                *reinterpret_cast<Held<float, EV>*>(&m.size[es][el]) = pack<float, EV>(size);
+                *reinterpret_cast<Held<float, EV>*>(&m.in[es][el]) = pack<float, EV>(in);
+                *reinterpret_cast<Held<float, EV>*>(&m.given[es][el]) = pack<float, EV>(given);
+                *reinterpret_cast<Held<float, EV>*>(&m.slope[es][el]) = pack<float, EV>(slope);
+                *reinterpret_cast<Held<float, EV>*>(&m.zslope[es][el]) = pack<float, EV>(zslope);
             }
 #pragma unroll
             for (int i = 0; i < PER; ++i) {
@@ -750,37 +753,43 @@ __global__ void __launch_bounds__(kThreads, 4) k_scan_backward(Call a) {
 #pragma unroll
                     for (int l = 0; l < LN; ++l) {
                         const float* from = reinterpret_cast<const float*>(m.channel_sums[es % kHalf][k][l]) + 2 * Shape::channel_at(el / 2, l) + (EV == 1 ? el % 2 : 0);
-                        const Pack<float, EV> v = load_pack<float, EV>(from);
+                        float v[EV];
+                        unpack<float, EV>(load_held<float, EV>(from), v);
 #pragma unroll
-                        for (int i = 0; i < EV; ++i) sum[k][i] += v.v[i];
+                        for (int i = 0; i < EV; ++i) sum[k][i] += v[i];
                     }
                 }
                 if (ecount > 0 && at < t1) {
                     const bool live = at < end;
-                    const Pack<float, EV> size = load_pack<float, EV>(&m.size[es][el]), given = load_pack<float, EV>(&m.given[es][el]);
-                    const Pack<float, EV> slope = load_pack<float, EV>(&m.slope[es][el]), zslope = load_pack<float, EV>(&m.zslope[es][el]);
-                    float du[EV], ddelta[EV], dz[EV];
+                    float size[EV], given[EV];
+                    unpack<float, EV>(load_held<float, EV>(&m.size[es][el]), size);
+                    unpack<float, EV>(load_held<float, EV>(&m.given[es][el]), given);
+                    float slope[EV], zslope[EV];
+                    unpack<float, EV>(load_held<float, EV>(&m.slope[es][el]), slope);
+                    unpack<float, EV>(load_held<float, EV>(&m.zslope[es][el]), zslope);
+                    float du[EV], ddelta[EV], dz[EV], of_u[EV];
+                    unpack<T, EV>(raw_u, of_u);
 #pragma unroll
                     for (int i = 0; i < EV; ++i) {
-                        const float vu = Element<T>::load(raw_u.v[i]), skip = m.skip[el + i];
-                        du[i] = live ? fmaf(skip, given.v[i], size.v[i] * sum[1][i]) : 0.0f;
-                        ddelta[i] = live ? fmaf(kLn2, sum[2][i], vu * sum[1][i]) * slope.v[i] : 0.0f;
-                        dz[i] = live ? zslope.v[i] * fmaf(skip, vu, sum[0][i]) : 0.0f;
+                        const float vu = of_u[i], skip = m.skip[el + i];
+                        du[i] = live ? fmaf(skip, given[i], size[i] * sum[1][i]) : 0.0f;
+                        ddelta[i] = live ? fmaf(kLn2, sum[2][i], vu * sum[1][i]) * slope[i] : 0.0f;
+                        dz[i] = live ? zslope[i] * fmaf(skip, vu, sum[0][i]) : 0.0f;
                         dbias[i] += ddelta[i];
-                        if (live) dd[i] = fmaf(given.v[i], vu, dd[i]);
+                        if (live) dd[i] = fmaf(given[i], vu, dd[i]);
                     }
 #pragma unroll
                     for (int k = 0; k < 3; ++k) {
                         if (k == 2 && !a.dz.data) continue;
                         const Track<void>& track = k == 0 ? a.du : k == 1 ? a.ddelta : a.dz;
                         T* to = const_cast<T*>(row_of(track, at));
-                        const Pack<T, EV> v = pack<T, EV>(k == 0 ? du : k == 1 ? ddelta : dz);
+                        const Held<T, EV> v = pack<T, EV>(k == 0 ? du : k == 1 ? ddelta : dz);
                         if (ecount == EV && a.paired) {
-                            *reinterpret_cast<Pack<T, EV>*>(to) = v;
+                            store_held<T, EV>(to, v);
                         } else {
 #pragma unroll
                             for (int i = 0; i < EV; ++i) {
-                                if (i < ecount) to[i] = v.v[i];
+                                if (i < ecount) to[i] = reinterpret_cast<const T*>(&v)[i];
                             }
                         }
                     }
@@ -970,13 +979,13 @@ __global__ void __launch_bounds__(kStepThreads) k_scan_step(Call a, float* state
 #pragma unroll
             for (int k = 0; k < TIMES; ++k) {
                 const int n = n0 + k * LP * V;
-                if (mine && i < count && n < a.states) h[i][k] = load_pack<float, V>(state + ((s0 + i) * channels + c) * a.states + n);
+                if (mine && i < count && n < a.states) h[i][k] = *reinterpret_cast<const Pack<float, V>*>(state + ((s0 + i) * channels + c) * a.states + n);
             }
         }
 #pragma unroll
         for (int k = 0; k < TIMES; ++k) {
             const int n = n0 + k * LP * V;
-            if (n < a.states) rate[k] = load_pack<float, V>(a.a + static_cast<int64_t>(c) * a.states + n);
+            if (n < a.states) rate[k] = *reinterpret_cast<const Pack<float, V>*>(a.a + static_cast<int64_t>(c) * a.states + n);
         }
         // the elementwise part of this lane's own sequences
         float vu[OWN], size[OWN], gate[OWN];
@@ -1014,7 +1023,7 @@ __global__ void __launch_bounds__(kStepThreads) k_scan_step(Call a, float* state
             for (int k = 0; k < TIMES; ++k) {
                 const int n = n0 + k * LP * V;
                 if (n >= a.states) continue;
-                const Pack<float, V> b = load_pack<float, V>(&bc[i][0][n]), cc = load_pack<float, V>(&bc[i][1][n]);
+                const Pack<float, V> b = *reinterpret_cast<const Pack<float, V>*>(&bc[i][0][n]), cc = *reinterpret_cast<const Pack<float, V>*>(&bc[i][1][n]);
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
                     const float from = cut ? 0.0f : h[i][k].v[v];
