@@ -61,6 +61,9 @@ __device__ __forceinline__ bool legal(const Loss& a, int64_t row, int64_t action
 
 constexpr float kLn2 = 0.69314718055994531f;
 constexpr double kExactLn2 = 0.693147180559945309;
+// The machine's 2^x is off by -4.5e-8 to -5.1e-8 of the value in the mean for x below -0.25 (a million values of each range),
+// which all of a row's exponentials and their sum share: arguments are longer by what makes up for it.
+constexpr float kUnbiased = 6.9e-8f;
 constexpr float kNever = -1000.0f;  // 2^kNever is 0, and a factor of 0 beside it gives 0, not NaN
 
 // max that keeps a NaN
@@ -232,16 +235,16 @@ __global__ void __launch_bounds__(32 * kWarps, resident_blocks(HELD)) k_policy_l
     }
     // t, and t less the reference's
     Two t[H], away[REFERENCE ? H : 1], total, q_total, spread, apart;
-    const Two scale(kLog2E, kLog2E), from(-s.m, -s.m), q_from(-s.q_m, -s.q_m);
+    const Two scale(kLog2E, kLog2E), unbiased(kUnbiased, kUnbiased), from(-s.m, -s.m), q_from(-s.q_m, -s.q_m);
 #pragma unroll
     for (int i = 0; i < H; ++i) {
-        const float2 x = ((Two(v[2 * i], v[2 * i + 1]) + from) * scale).get();
+        const float2 x = multiply_add(Two(v[2 * i], v[2 * i + 1]) + from, scale, unbiased).get();
         t[i] = Two(max_nan(x.x, kNever), max_nan(x.y, kNever));
         const Two e = powers_of_two(t[i]);
         total = total + e;
         spread = multiply_add(e, t[i], spread);
         if (REFERENCE) {
-            const Two u = (Two(w[REFERENCE ? 2 * i : 0], w[REFERENCE ? 2 * i + 1 : 0]) + q_from) * scale;
+            const Two u = multiply_add(Two(w[REFERENCE ? 2 * i : 0], w[REFERENCE ? 2 * i + 1 : 0]) + q_from, scale, unbiased);
             q_total = q_total + powers_of_two(u);
             const float2 f = e.get(), d = multiply_add(u, Two(-1.0f, -1.0f), t[i]).get();
             away[REFERENCE ? i : 0] = Two(f.x != 0.0f ? d.x : 0.0f, f.y != 0.0f ? d.y : 0.0f);
@@ -328,7 +331,7 @@ __global__ void __launch_bounds__(kMostThreads, REFERENCE ? 4 : 5) k_policy_loss
         return;
     }
     const float chosen = Element<T>::load(z[action]);
-    const Two scale(kLog2E, kLog2E);
+    const Two scale(kLog2E, kLog2E), unbiased(kUnbiased, kUnbiased);
     Sums s;
     Two total, q_total, spread, apart;  // two parts of each sum, alike in m
     auto masked = [&](auto count, const T* from, int e, uint32_t bits, auto& x) {  // logits, -inf where they are not legal
@@ -379,12 +382,12 @@ __global__ void __launch_bounds__(kMostThreads, REFERENCE ? 4 : 5) k_policy_loss
         const Two off(from, from), q_off(q_from, q_from);
 #pragma unroll
         for (int i = 0; i < H; ++i) {
-            const float2 f = ((x[i] + off) * scale).get();
+            const float2 f = multiply_add(x[i] + off, scale, unbiased).get();
             const Two t(max_nan(f.x, kNever), max_nan(f.y, kNever)), p = powers_of_two(t);
             total = total + p;
             spread = multiply_add(p, t, spread);
             if (REFERENCE) {
-                const Two u = (y[i] + q_off) * scale;
+                const Two u = multiply_add(y[i] + q_off, scale, unbiased);
                 q_total = q_total + powers_of_two(u);
                 const float2 d = multiply_add(u, Two(-1.0f, -1.0f), t).get(), k = p.get();
                 apart = multiply_add(p, Two(k.x != 0.0f ? d.x : 0.0f, k.y != 0.0f ? d.y : 0.0f), apart);
@@ -461,11 +464,11 @@ __global__ void __launch_bounds__(kMostThreads, REFERENCE ? 4 : 5) k_policy_loss
         float out[2 * H];
 #pragma unroll
         for (int i = 0; i < H; ++i) {
-            const float2 f = ((x[i] + off) * scale).get();
+            const float2 f = multiply_add(x[i] + off, scale, unbiased).get();
             const Two t(max_nan(f.x, kNever), max_nan(f.y, kNever)), p = powers_of_two(t);
             Two inner = multiply_add(of_t, t, base);
             if (REFERENCE) {
-                const float2 d = multiply_add((y[i] + q_off) * scale, Two(-1.0f, -1.0f), t).get(), w = p.get();
+                const float2 d = multiply_add(multiply_add(y[i] + q_off, scale, unbiased), Two(-1.0f, -1.0f), t).get(), w = p.get();
                 inner = multiply_add(of_apart, Two(w.x != 0.0f ? d.x : 0.0f, w.y != 0.0f ? d.y : 0.0f), inner);
             }
             const float2 d = (p * part * inner).get();
