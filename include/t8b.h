@@ -645,7 +645,8 @@ typedef struct {
  * 0 (NULL: nowhere), a new round begins at step t: nothing before it, the initial state included,
  * reaches it. lengths [sequences] (NULL: all are `steps`; others are taken into 0 ... steps) ends
  * sequences early: what lies at and past a sequence's length is not read, its outputs and
- * gradients there are 0 and its final state is the one after its last step. */
+ * gradients there are 0 and its final state is the one after its last step. Up to 2^30 sequences
+ * and steps and 2^20 channels; the workspace queries answer 0 for more, which the calls refuse. */
 typedef struct {
     int64_t sequences, steps, channels;
     const uint8_t* reset;

@@ -583,7 +583,7 @@ extern "C" int t8b_causal_conv_forward(const t8b_sequences_t* q, int type, t8b_t
 }
 
 extern "C" size_t t8b_causal_conv_workspace(const t8b_sequences_t* q, int width) {
-    if (q == nullptr || q->sequences < 1 || q->channels < 1 || q->steps < 0 || width < 2 || width > 4) return 0;
+    if (q == nullptr || !countable(*q) || q->sequences < 1 || width < 2 || width > 4) return 0;
     const int64_t items = q->sequences * runs_of(q->steps, kBackRun);
     const Layout wide(items, static_cast<int>((q->channels + kPack - 1) / kPack)), single(items, static_cast<int>(q->channels));
     return sizeof(float) * static_cast<size_t>(std::max(wide.workers, single.workers)) * (width + 1) * q->channels;

@@ -132,13 +132,20 @@ __device__ __forceinline__ float exponential(float v) {
 
 // ------------------------------------------------------------------ host checks
 constexpr int64_t kMostElements = int64_t{1} << 61;
+constexpr int64_t kMostSequences = int64_t{1} << 30, kMostSteps = int64_t{1} << 30, kMostChannels = int64_t{1} << 20;
 
+// Whether the plans may count these sequences: the kernels' numbers of steps, channels and blocks have 32 bits. The
+// queries answer 0 for others, which the calls refuse.
+inline bool countable(const t8b_sequences_t& q) {
+    return q.sequences >= 0 && q.sequences <= kMostSequences && q.steps >= 0 && q.steps <= kMostSteps && q.channels >= 1 &&
+        q.channels <= kMostChannels;
+}
 inline void check_sequences(const char* what, const t8b_sequences_t* q, bool step) {
     const std::string name(what);
     if (q == nullptr) raise(T8B_EINVAL, name + ": the sequences are null");
-    if (q->sequences < 0 || q->sequences > (int64_t{1} << 30)) raise(T8B_EINVAL, name + ": 0 to 2^30 sequences");
-    if (!step && (q->steps < 0 || q->steps > (int64_t{1} << 30))) raise(T8B_EINVAL, name + ": 0 to 2^30 steps");
-    if (q->channels < 1 || q->channels > (1 << 20)) raise(T8B_EINVAL, name + ": 1 to 2^20 channels");
+    if (q->sequences < 0 || q->sequences > kMostSequences) raise(T8B_EINVAL, name + ": 0 to 2^30 sequences");
+    if (!step && (q->steps < 0 || q->steps > kMostSteps)) raise(T8B_EINVAL, name + ": 0 to 2^30 steps");
+    if (q->channels < 1 || q->channels > kMostChannels) raise(T8B_EINVAL, name + ": 1 to 2^20 channels");
     const int64_t steps = step ? 1 : std::max<int64_t>(q->steps, 1);
     if (q->reset != nullptr &&
         (q->reset_sequence < 0 || q->reset_step < 0 || q->reset_sequence > kMostElements / std::max<int64_t>(q->sequences, 1) ||

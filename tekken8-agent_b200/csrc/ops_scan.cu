@@ -41,7 +41,7 @@ struct Room {
 };
 
 bool sane(const t8b_sequences_t* q, int64_t groups, int64_t states) {
-    return q != nullptr && q->sequences >= 1 && q->steps >= 1 && q->channels >= 1 && groups >= 1 && q->channels % groups == 0 && states >= 1 &&
+    return q != nullptr && countable(*q) && q->sequences >= 1 && q->steps >= 1 && groups >= 1 && q->channels % groups == 0 && states >= 1 &&
         states <= kMostStates;
 }
 
