@@ -325,6 +325,13 @@ __global__ void __launch_bounds__(kThreads, 5) k_scan_forward(Call a) {
     }
 }
 
+// 2^x h wherever that has a place in fp32, though 2^x alone may have none: over a chunk whose sizes are negative x passes
+// 128 while its state is 0 (infinity times 0 is NaN) or small, and below -126 a large state still leaves something.
+__device__ __forceinline__ float grown(float x, float h) {
+    const float bounded = fabsf(x) > 1000.0f ? copysignf(1000.0f, x) : x;  // 2^1000 times the least h is infinite; NaN stays
+    const float whole = ceilf(bounded);
+    return ldexpf(power_of_two(bounded - whole + kUnbiased) * h, static_cast<int>(whole));
+}
 // The chunks of a sequence in order (backward: in reverse): what each starts from takes the place of its
 // own end. A thread has one state of one channel.
 static __global__ void __launch_bounds__(256) k_scan_join(Call a, bool backward) {
@@ -358,7 +365,7 @@ static __global__ void __launch_bounds__(256) k_scan_join(Call a, bool backward)
             if (k + i >= a.chunks) break;
             const int at = backward ? a.chunks - 1 - k - i : k + i;
             carry[at * apart] = h;
-            h = kept[i] != 0.0f ? fmaf(power_of_two(rate * size[i]), h, ends[i]) : ends[i];
+            h = kept[i] != 0.0f ? grown(rate * size[i], h) + ends[i] : ends[i];
         }
     }
 }
