@@ -154,6 +154,7 @@ __global__ void __launch_bounds__(kThreads, 5) k_scan_forward(Call a) {
             const int n = n0 + i + j;
             if (n >= a.states) continue;
             r[j] = a.a[static_cast<int64_t>(c) * a.states + n] * kLog2E;
+            if (r[j] == -INFINITY) r[j] = -3.402823466e38f;  // (a reset's size of 0 makes 1 of it, not NaN)
             if (!ENDS && a.chunks > 1) {
                 from[j] = a.carry[(at_chunk * a.states + n) * channels + c];
             } else if (!ENDS && a.state) {
@@ -240,6 +241,7 @@ __global__ void __launch_bounds__(kThreads, 5) k_scan_forward(Call a) {
             v.size = Element<T>::load(rows[buffer][1][i][column]) + bias;
             if (a.softplus) v.size = softplus(v.size);
             v.in = v.size * v.u;
+            if (resets >> i & 1) v.size = 0.0f;  // its decay of nothing is 1: its own may be infinite, and 0 of that NaN
             v.gate = gate ? silu(Element<T>::load(rows[buffer][2][i][column])) : 1.0f;
             return v;
         };
@@ -1054,8 +1056,8 @@ __global__ void __launch_bounds__(kStepThreads) k_scan_step(Call a, float* state
                 const Pack<float, V> b = *reinterpret_cast<const Pack<float, V>*>(&bc[i][0][n]), cc = *reinterpret_cast<const Pack<float, V>*>(&bc[i][1][n]);
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
-                    const float from = cut ? 0.0f : h[i][k].v[v];
-                    h[i][k].v[v] = fmaf(decay(by, rate[k].v[v]), from, in * b.v[v]);
+                    const float kept = cut ? 0.0f : decay(by, rate[k].v[v]), from = cut ? 0.0f : h[i][k].v[v];
+                    h[i][k].v[v] = fmaf(kept, from, in * b.v[v]);
                     sum[i] = fmaf(h[i][k].v[v], cc.v[v], sum[i]);
                 }
                 if (mine) *reinterpret_cast<Pack<float, V>*>(state + ((s0 + i) * channels + c) * a.states + n) = h[i][k];
