@@ -122,12 +122,13 @@ __device__ __forceinline__ Held<T, V> pack(const Two (&v)[(V + 1) / 2]) {
 }
 
 constexpr float kLn2 = 0.69314718055994531f;
-// exp(v), the argument's product with log2 e to twice the precision: good to 2^x's own 2^-22.
+// exp(v), v <= 0, the argument's product with log2 e to twice the precision: good to 2^x's own 2^-22, and without
+// the bias that it has for x below -0.25 (4.8e-8 of the value in the mean; above it next to none).
 __device__ __forceinline__ float exponential(float v) {
     const float high = v * kLog2E;
     const float low = fmaf(v, 1.925963033e-8f, fmaf(v, kLog2E, -high));  // log2 e - fp32(log2 e)
     const float r = power_of_two(high);
-    return fabsf(high) < 200.0f ? fmaf(r, low * kLn2, r) : r;
+    return fabsf(high) < 200.0f ? fmaf(r, fmaf(low, kLn2, high < -0.25f ? 4.8e-8f : 0.0f), r) : r;
 }
 
 // ------------------------------------------------------------------ host checks

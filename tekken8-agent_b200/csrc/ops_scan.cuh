@@ -71,17 +71,18 @@ __device__ __forceinline__ Two powers_of_two(const Two& v) {
     return Two(power_of_two(f.x), power_of_two(f.y));
 }
 __device__ __forceinline__ Two decay(const Two& size, const Two& rate) { return powers_of_two(multiply_add(size, rate, both(kUnbiased))); }
-// log(1 + x), 0 <= x <= 1: x times a polynomial fitted for the least relative error, 2^-25
+// log(1 + x), 0 <= x <= 1: x + x^2 p(x), p fitted for the least relative error (2^-27.5, one coefficient after the other
+// rounded to fp32 and the rest fitted again). In fp32 arithmetic at most 1.1e-7 off, within 6e-10 in the mean.
 __device__ __forceinline__ float log_one_plus(float x) {
-    float p = fmaf(5.2326915e-3f, x, -2.9505228e-2f);
-    p = fmaf(p, x, 7.8225934e-2f);
-    p = fmaf(p, x, -0.13663244f);
-    p = fmaf(p, x, 0.19106006f);
-    p = fmaf(p, x, -0.24842982f);
-    p = fmaf(p, x, 0.33319097f);
-    p = fmaf(p, x, -0.49999493f);
-    p = fmaf(p, x, 0.99999997f);
-    return p * x;
+    float p = fmaf(-3.2904686e-3f, x, 2.0086242e-2f);
+    p = fmaf(p, x, -5.7457231e-2f);
+    p = fmaf(p, x, 0.10661128f);
+    p = fmaf(p, x, -0.15344881f);
+    p = fmaf(p, x, 0.19692102f);
+    p = fmaf(p, x, -0.24958019f);
+    p = fmaf(p, x, 0.33330464f);
+    p = fmaf(p, x, -0.49999931f);
+    return fmaf(x * x, p, x);
 }
 // softplus(v) = max(v, 0) + log(1 + exp(-|v|)), and its slope sigmoid(v)
 __device__ __forceinline__ float softplus(float v) {
