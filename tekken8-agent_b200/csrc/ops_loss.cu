@@ -123,14 +123,15 @@ __device__ __forceinline__ Slopes finish(const Loss& a, int64_t row, const Scala
     const double log_total = natural_log(s.total);
     const double lp = (static_cast<double>(chosen) - static_cast<double>(s.m)) - log_total;
     const float share = 1.0f / static_cast<float>(s.total), log_sum = static_cast<float>(log_total);
-    const float entropy = static_cast<float>(log_total - static_cast<double>(kLn2 * (s.spread * share)));
+    // spread has t in it as it is lengthened, and so has the gradient
+    const float entropy = static_cast<float>(log_total - static_cast<double>(kLn2 * (s.spread * share - kUnbiased)));
     const float advantage = given.advantage;
     const float ratio = expf(static_cast<float>(lp - static_cast<double>(given.old)));
     const float free = ratio * advantage, held = fminf(fmaxf(ratio, a.low), a.high) * advantage;
     const bool unclipped = free <= held || free != free;
     float loss = -(unclipped ? free : held), slope = unclipped ? -free : 0.0f, divergence = 0.0f;
     Slopes out;
-    out.base = a.entropy * (entropy - log_sum);
+    out.base = a.entropy * ((entropy - log_sum) - kLn2 * kUnbiased);
     out.of_t = a.entropy * kLn2;
     out.of_apart = 0.0f;
     if (a.reference_kind == T8B_REFERENCE_LOGITS) {
