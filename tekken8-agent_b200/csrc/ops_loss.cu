@@ -103,6 +103,8 @@ struct Sums {
 // A row's gradient: e scale (base + of_t t + of_apart (t - t of the reference)) + [i = action] slope
 struct Slopes {
     float scale, slope, base, of_t, of_apart;
+    // Whether 0 times the rest is 0: an infinite divergence or advantage, say, makes NaN of a logit that is not legal.
+    __device__ __forceinline__ bool finite() const { return fabsf(scale) + fabsf(base) - kNever * fabsf(of_t) < INFINITY; }
 };
 
 // What a row has beside its logits.
@@ -180,6 +182,16 @@ __device__ __forceinline__ void add_chosen(float (&v)[V], int64_t e, int64_t act
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         if (e + j == action) v[j] += slope;
+    }
+}
+
+// 0 at the logits of a thread's pack that are not legal, behind its store.
+template <typename T, int V>
+__device__ __forceinline__ void clear_masked(const Loss& a, int64_t row, T* g, int e) {
+    const uint32_t bits = legal_bits<V>(a, row, e);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        if ((bits >> j & 1) == 0) g[e + j] = Element<T>::store(0.0f);
     }
 }
 
@@ -300,6 +312,8 @@ __global__ void __launch_bounds__(32 * kWarps, resident_blocks(HELD)) k_policy_l
         add_chosen<V>(out, e, action, k.slope);
         store_pack<T, V>(g + e, out);
     }
+    if (a.mask_kind == T8B_MASK_NONE || k.finite()) return;
+    for (int e = lane * V; e < a.n; e += LANES * V) clear_masked<T, V>(a, row, g, e);
 }
 
 // What a new largest logit adds to every t, far enough down for 2^gap to be 0 where the old one was -inf or the lowest
@@ -487,6 +501,11 @@ __global__ void __launch_bounds__(kMostThreads, REFERENCE ? 4 : 5) k_policy_loss
 #pragma unroll 4
     for (int e = threadIdx.x * V; e < whole; e += step) leave(Constant<V>{}, e);
     for (int e = whole + threadIdx.x; e < a.n; e += blockDim.x) leave(Constant<1>{}, e);
+    if constexpr (MASKED) {
+        if (k.finite()) return;
+        for (int e = threadIdx.x * V; e < whole; e += step) clear_masked<T, V>(a, row, g, e);
+        for (int e = whole + threadIdx.x; e < a.n; e += blockDim.x) clear_masked<T, 1>(a, row, g, e);
+    }
 }
 
 // ------------------------------------------------------------------ dispatch

@@ -37,3 +37,39 @@ def test_entropy_of_a_row_that_is_decided(cuda, n, type_name):
     assert float(h.min()) >= 0
     bound = (2 * max(16, n // 512) + 8 + 2 * want["logp"].abs().amax(1)) * 2 ** -24 * (1 + (want["p"] * want["logp"].abs()).sum(1))
     assert bool(((h.double() - want["entropies"]).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("n", [40, 368, 2000, 4099])
+@pytest.mark.parametrize("kind", ["bits", "bytes"])
+def test_masked_logits_of_a_row_that_is_not_finite(cuda, n, kind):
+    """An infinite divergence, an advantage, an old log-probability or a weight that is infinite or NaN, a legal NaN: the
+    gradient is 0 at masked logits all the same, and other rows are what they are alone."""
+    import torch
+    from test_memory_gpu import packed_bits
+    from t8b import ops
+    inf, nan = float("inf"), float("nan")
+    for T in (torch.float32, torch.bfloat16):
+        g = torch.Generator(device="cuda").manual_seed(n)
+        rows = 8
+        z, q = (torch.randn(rows, n, device="cuda", generator=g).to(T) for _ in range(2))
+        legal = torch.rand(rows, n, device="cuda", generator=g) < 0.5
+        actions, at = torch.randint(n, (rows,), device="cuda", generator=g), torch.arange(rows, device="cuda")
+        legal[at, actions] = True
+        legal[:, 5], actions[actions == 5] = True, 6
+        legal[at, actions] = True
+        old, advantages, weights = torch.full((rows,), -3.0, device="cuda"), torch.ones(rows, device="cuda"), torch.ones(rows, device="cuda")
+        clean = ops.policy_loss(z, actions, old, advantages, mask=legal, reference=q, weights=weights, kl=0.5, entropy=0.1)
+        q[0, 5], advantages[1], advantages[2], weights[4], z[5, 5] = -inf, nan, inf, inf, nan
+        old[3], advantages[3] = -inf, -1  # an infinite ratio, which nothing clips on this side
+        given = packed_bits(legal) if kind == "bits" else legal
+        grad = ops.policy_loss(z, actions, old, advantages, mask=given, reference=q, weights=weights, kl=0.5, entropy=0.1)[4]
+        assert not grad[~legal].any()
+        for row in range(6):
+            assert not bool(grad[row].isfinite().all()), row
+        assert torch.equal(grad[6:], clean[4][6:])
+        # without a reference, and its sampled form
+        grad = ops.policy_loss(z, actions, old, advantages, mask=given, weights=weights, entropy=0.1)[4]
+        assert not grad[~legal].any()
+        sampled = torch.full((rows,), -3.0, device="cuda")
+        sampled[6] = inf
+        assert not ops.policy_loss(z, actions, old, advantages, mask=given, reference=sampled, weights=weights, kl=0.5)[4][~legal].any()
