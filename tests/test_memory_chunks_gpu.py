@@ -122,3 +122,121 @@ def test_decays_of_a_chunk_beyond_the_range(cuda, size, start):
         assert ("k_scan_ends" in launched) == cut
         assert bool(want["y"].float().isfinite().all())
         check(got, want, bound)
+
+
+def near(got, want, limit, name):
+    off, size = float((got.double() - want.double()).norm()), float(want.double().norm())
+    assert off <= limit * size, (name, off, size, limit)  # (a state behind a reset may be 0)
+
+
+@pytest.mark.parametrize("s,t,n,groups,states", [(1, 1000, 40, 1, 16), (2, 777, 24, 2, 24), (1, 600, 12, 1, 64)])
+@pytest.mark.parametrize("cuts", [False, True])
+def test_slow_states_carry_over(cuda, s, t, n, groups, states, cuts):
+    """Sizes of some 0.02 under rates of 0.2 to 1: a state lasts for hundreds of steps, and what a chunk takes over is most of
+    what it gives. In the norm, against the definition and against the same sequence in three pieces that hand their
+    states on (the last two as gradients too): a decay is off by 2^-25 in the mean (all in one direction, at worst: t of
+    them) and by 2^-22 each way (t^0.5 of them); sums, products and one chunk's decay for all of its steps 2^-19.
+    A carry that is 0.1 % off is beyond that."""
+    import torch
+    from t8b import ops, profile
+    g = torch.Generator(device="cuda").manual_seed(t)
+
+    def normal(*shape):
+        return torch.randn(*shape, device="cuda", generator=g)
+
+    u, dy, z, b, c = normal(s, t, n), normal(s, t, n), normal(s, t, n), normal(s, t, groups, states), normal(s, t, groups, states)
+    delta, bias = 0.3 * normal(s, t, n), torch.full((n,), -4.0, device="cuda")
+    a = -(0.2 + 0.8 * torch.rand(n, states, device="cuda", generator=g))
+    state, dfinal, d = normal(s, n, states), normal(s, n, states), normal(n)
+    reset = lengths = None
+    if cuts:
+        reset = torch.rand(s, t, device="cuda", generator=g) < 1 / 300
+        lengths = torch.tensor([t - 77] + [t] * (s - 1), device="cuda", dtype=torch.int32)
+
+    def run(steps, state, dfinal):
+        rows = [v[:, steps] for v in (u, delta, b, c)]
+        more = dict(d=d, z=z[:, steps], delta_bias=bias, state=state, reset=None if reset is None else reset[:, steps],
+                    lengths=None if lengths is None else (lengths - steps.start).clamp(0, steps.stop - steps.start).int())
+        y, final, saved = ops.selective_scan(rows[0], rows[1], a, rows[2], rows[3], final=True, save=True, **more)
+        back = lambda dfinal: ops.selective_scan_backward(dy[:, steps], rows[0], rows[1], a, rows[2], rows[3], saved, dfinal=dfinal, **more)  # noqa: E731
+        return y, final, back
+
+    profile.enable()
+    try:
+        y, final, back = run(slice(0, t), state, None)
+        got = back(dfinal)
+        launched = profile.report()
+    finally:
+        profile.enable(False)
+    assert "k_scan_ends" in launched and "k_scan_back_ends" in launched
+
+    live = m.live_of(lengths, s, t, u.device)[:, :, None]
+    v = delta.double() + bias.double()
+    size = torch.nn.functional.softplus(v)
+    gate, slope = m.act64(z.double(), "silu")
+    out, states64, befores, end, decays = m.scan64(size, u, a, b, c, d, state, reset, lengths)
+    gs = torch.where(live, dy.double() * gate, torch.zeros_like(v))
+    du, dsize, da, db, dc, dd, dstate = m.scan_grad64(gs, size, u, a, b, c, d, states64, befores, decays, reset, lengths, dfinal)
+    dv = dsize * torch.sigmoid(v)
+    dz = torch.where(live, dy.double() * out * slope, torch.zeros_like(v))
+    limit = t * 2 ** -25 + t ** 0.5 * 2 ** -22 + 2 ** -19
+    names = ("du", "ddelta", "da", "db", "dc", "dd", "dz", "ddelta_bias", "dstate")
+    near(y, out * gate, limit, "y")
+    near(final, end, limit, "final")
+    for name, v, w in zip(names, got, (du, dv, da, db, dc, dd, dz, dv.sum((0, 1)), dstate)):
+        near(v, w, 2 * limit, name)
+
+    parts = [slice(0, t // 3), slice(t // 3, t // 2), slice(t // 2, t)]
+    held, runs = state, []
+    for part in parts:
+        piece, held, back = run(part, held, None)
+        runs.append((piece, back))
+    near(torch.cat([r[0] for r in runs], 1), y, limit, "y of pieces")
+    near(held, final, limit, "final of pieces")
+    carry, sums = dfinal, {k: 0 for k in ("da", "dd", "ddelta_bias")}
+    rows = {k: [] for k in ("du", "ddelta", "db", "dc", "dz")}
+    for _, back in reversed(runs):
+        grads = dict(zip(names, back(carry)))
+        carry = grads["dstate"]
+        for k in rows:
+            rows[k].insert(0, grads[k])
+        for k in sums:
+            sums[k] = sums[k] + grads[k]
+    for k, w in zip(names, got):
+        near(carry if k == "dstate" else sums[k] if k in sums else torch.cat(rows[k], 1), w, 2 * limit, k + " of pieces")
+
+
+def test_nothing_of_a_round_reaches_the_ones_before_it(cuda):
+    """In a sequence that is cut into chunks: NaN at a reset, bit for bit nothing of it in front."""
+    import torch
+    from t8b import ops, profile
+    g = torch.Generator(device="cuda").manual_seed(3)
+    s, t, n, states = 3, 600, 40, 16
+    u, delta, z, dy = (torch.randn(s, t, n, device="cuda", generator=g) for _ in range(4))
+    b, c = (torch.randn(s, t, states, device="cuda", generator=g) for _ in range(2))
+    a, d = -torch.exp(torch.randn(n, states, device="cuda", generator=g)), torch.ones(n, device="cuda")
+    state, at = torch.randn(s, n, states, device="cuda", generator=g), 303
+    reset = torch.zeros(s, t, dtype=torch.bool, device="cuda")
+    reset[:, at] = True
+
+    def run(u, delta, b, c, dy):
+        more = dict(d=d, z=z, delta_bias=d, state=state, reset=reset)
+        y, saved = ops.selective_scan(u, delta, a, b, c, save=True, **more)
+        return y, ops.selective_scan_backward(dy, u, delta, a, b, c, saved, **more)
+
+    profile.enable()
+    try:
+        y, want = run(u, delta, b, c, dy)
+        launched = profile.report()
+    finally:
+        profile.enable(False)
+    assert "k_scan_ends" in launched and "k_scan_back_ends" in launched
+    late = [v.clone() for v in (u, delta, b, c, dy)]
+    for v in late:
+        v[:, at:at + 2] = float("nan")
+        v[:, -1] = float("inf")
+    y2, got = run(*late)
+    assert torch.equal(y[:, :at], y2[:, :at]) and bool(y2[:, at].isnan().all())
+    for k in (0, 1, 3, 4, 6):
+        assert torch.equal(got[k][:, :at], want[k][:, :at]), k
+    assert torch.equal(got[8], want[8])
