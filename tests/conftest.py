@@ -14,6 +14,13 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a CUDA GPU (B200) and the built sm_100a library")
 
 
+def pytest_collection_modifyitems(items):
+    """What compares with the reference's own library or programs comes last: where those are not built, a run that
+    stops at its first failure has been through everything else."""
+    programs = {"test_oracle.py", "test_relinked_gpu.py"}
+    items.sort(key=lambda item: item.path.name in programs or not {"ref", "ref_roster"}.isdisjoint(getattr(item, "fixturenames", ())))
+
+
 @pytest.fixture(scope="session")
 def roster_raw() -> bytes:
     return lzma.decompress((GOLDEN / "roster41.bin.xz").read_bytes())
