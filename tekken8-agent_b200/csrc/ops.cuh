@@ -105,7 +105,8 @@ __device__ __forceinline__ Two multiply_add(const Two& a, const Two& b, const Tw
 }
 
 // ------------------------------------------------------------------ activations
-// In fp32, from the machine's 2^x and 1/x (each good to about 2^-22): exp(v) = 2^(v log2 e),
+// In fp32, from the machine's 2^x and 1/x (each good to about 2^-22): exp(v) = 2^(v log2 e), whose argument is
+// rounded once and adds |v| 2^-24,
 //   sigmoid(z) = 1 / (1 + exp(-z)),
 //   tanh(z) = 1 - 2 / (1 + exp(2z)), and below |z| = 0.2, where that difference cancels, the
 //     series z - z^3/3 + 2 z^5/15 - 17 z^7/315 (its next term is at most 2^-24 of z there),

@@ -11,7 +11,7 @@
 // that one group of B and C serves; rows and B and C of 8 steps at a time lie in shared memory, the next ones on
 // their way. Per (step, channel, state) one 2^x and four multiplications or additions, two of a kind to an
 // instruction; per (step, channel) three more results of the 2^x unit, whose 16 a clock and SM bound the pass
-// rather than memory: 65,536 x 1,024 x 16 in bf16 467 us, 284 by that unit, 93 by the bytes.
+// rather than memory: 65,536 x 1,024 x 16 in bf16 465 us, 284 by that unit, 93 by the bytes.
 // Backward: each thread holds a tile of 2 channels x 4 states and goes through half of 8 steps forward,
 // from what the forward pass kept (the state before every eighth step), its states in registers, then back; the later half
 // first. Sums over states and over channels leave the threads as partial sums in shared memory and are added up there by
@@ -19,7 +19,7 @@
 // state) pairs, at 60 % of the issue slots with 16 warps an SM; with a whole tile's states in registers and 12 warps 1,755.
 // Sequences are cut into chunks where there are too few of them: a first pass takes each
 // chunk from a zero state, a second joins the chunks' ends, the last starts each where it belongs (1 x 8,192 x 1,024 x
-// 16: 55, 17 and 72 us; 8 blocks would take it in one piece).
+// 16: 56, 18 and 74 us; 8 blocks would take it in one piece).
 #pragma once
 
 #include "ops_memory.cuh"
@@ -331,8 +331,7 @@ __global__ void __launch_bounds__(kThreads, 5) k_scan_forward(Call a) {
 // The cube root of 2^x, as which a chunk's decay is multiplied: 2^x alone may have no place in fp32 where its product with
 // the state has one. Over negative sizes x passes 128 while the state is 0 (infinity times 0 is NaN) or small, and below
 // -126 a large state still leaves something. 2^300 takes the least state to infinity, 2^-300 the largest to 0; NaN stays.
-// (Three products a chunk in a row: 1 x 8,192 x 1,024 x 16 17 us; with
-// ldexp() of the product 36.)
+// (Three products a chunk in a row: 18 us for 1 x 8,192 x 1,024 x 16, 103 chunks; with ldexp() of the product 36.)
 __device__ __forceinline__ float decay_root(float x) {
     const float third = x * (1.0f / 3.0f);
     return power_of_two((fabsf(third) > 100.0f ? copysignf(100.0f, third) : third) + kUnbiased);
@@ -972,7 +971,7 @@ __global__ void __launch_bounds__(256) k_scan_shared(Call a) {
 // sequences' B and C in shared memory. Bound by the states' bytes, read once and written once: a thread has its
 // channel's states of every sequence in flight together. Lane l of a channel does the elementwise part of the
 // sequences l, l + LP, ... and gives D and D u to the others; the sums over its lanes end where they are used.
-// 32,768 x 512 x 16 in bf16: 418 us, 83 % of the copy rate (every lane with its own elementwise part, B and C: 1,262).
+// 32,768 x 512 x 16 in bf16: 420 us, 83 % of the copy rate (every lane with its own elementwise part, B and C: 1,262).
 constexpr int kStepAhead = 4;
 constexpr int kStepThreads = 256;
 template <typename T, int V, int LP>
